@@ -378,7 +378,7 @@ def _run_sample(s, c):
     sorted_weight = torch.where(torch.arange(v, device="cuda") < k, weight.gather(1, order), 0)
     so_far = torch.cumsum(sorted_weight, 1)
     p24 = torch.round(torch.clamp(s["top_p"], max=1.0) * 2.0 ** 24).to(torch.int64)[:, None]
-    need = _part(p24, so_far[:, -1:])
+    need = torch.clamp(_part(p24, so_far[:, -1:]), min=1)
     inside = (so_far - sorted_weight < need) & (w.gather(1, order) >= s["min_p"][:, None])
     kept = torch.zeros_like(weight).scatter_(1, order, torch.where(inside, sorted_weight, 0))
     so_far = torch.cumsum(kept, 1)
