@@ -1,5 +1,5 @@
 """ctypes binding of libstyx_moe.so (include/styx_moe.h, include/styx_residency.h,
-include/styx_gguf.h, include/styx_attn.h).
+include/styx_gguf.h, include/styx_attn.h, include/styx_serve.h).
 
 There is no fallback: if the library is missing, importing the ops raises.
 """
@@ -14,11 +14,12 @@ LIB_PATH = os.path.join(HERE, "libstyx_moe.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 HEADER = os.path.join(INCLUDE, "styx_moe.h")
 HEADERS = [HEADER, os.path.join(INCLUDE, "styx_residency.h"), os.path.join(INCLUDE, "styx_gguf.h"),
-           os.path.join(INCLUDE, "styx_attn.h")]
+           os.path.join(INCLUDE, "styx_attn.h"), os.path.join(INCLUDE, "styx_serve.h")]
 
 STYX_OK, STYX_EINVAL, STYX_ECUDA, STYX_ENOMEM, STYX_ETIMEOUT, STYX_EUNSUPPORTED = 0, -1, -2, -3, -4, -5
 STYX_EIO, STYX_EEOF, STYX_EDATA = -6, -7, -8
 F32, Q8_0, Q4_K, Q5_K, Q6_K = 0, 8, 12, 13, 14
+F16, BF16 = 1, 30
 QTYPES = {"q8_0": Q8_0, "q4_K": Q4_K, "q5_K": Q5_K, "q6_K": Q6_K}
 BLOCK = {Q8_0: (32, 34), Q4_K: (256, 144), Q5_K: (256, 176), Q6_K: (256, 210)}
 SKIP = 0xFFFFFFFF
@@ -74,6 +75,13 @@ class AttnDims(C.Structure):
 class AttnLayer(C.Structure):
     _fields_ = [("attn_norm", C.c_void_p), ("wq", DenseTensor), ("wk", DenseTensor), ("wv", DenseTensor),
                 ("wo", DenseTensor), ("q_norm", C.c_void_p), ("k_norm", C.c_void_p)]
+
+
+class PagedKv(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("page_stride", C.c_int64), ("table", C.c_void_p),
+                ("lens", C.c_void_p), ("dtype", C.c_int32), ("n_pages", C.c_int32), ("page_size", C.c_int32),
+                ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("n_seqs", C.c_int32),
+                ("max_pages", C.c_int32), ("table_stride", C.c_int32)]
 
 
 _vp, _i, _f, _u64 = C.c_void_p, C.c_int, C.c_float, C.c_uint64
@@ -184,6 +192,17 @@ _SIGS = {
     "styx_attn_block_workspace_init": (_i, [_vp, _vp, _vp, _u64]),
     "styx_attn_block": (_i, [_vp, _vp, C.POINTER(AttnDims), C.POINTER(AttnLayer), _vp, _i, _vp, _vp, _vp, _i,
                              _vp, _u64]),
+    # include/styx_serve.h
+    "styx_paged_append": (_i, [_vp, _vp, C.POINTER(PagedKv), _i, _i, _vp, C.c_int64, _vp, C.c_int64, _vp, C.c_int64,
+                               _vp, _vp, _f, _f, _vp, _vp, _vp, _vp]),
+    "styx_paged_attend_workspace_bytes": (_i, [_vp, C.POINTER(PagedKv), _i, _i, C.POINTER(_u64)]),
+    "styx_paged_attend_workspace_init": (_i, [_vp, _vp, _vp, _u64]),
+    "styx_paged_attend": (_i, [_vp, _vp, C.POINTER(PagedKv), _i, _vp, _f, _i, _vp, _vp, _vp, _vp, C.c_int64, _vp,
+                               _u64]),
+    "styx_paged_evict_workspace_bytes": (_i, [C.POINTER(PagedKv), _i, C.POINTER(_u64)]),
+    "styx_paged_evict": (_i, [_vp, _vp, C.POINTER(PagedKv), _vp, _vp, _vp, C.c_int64, _i, _i, _i, _vp, _vp, _vp, _vp,
+                              _u64]),
+    "styx_sample": (_i, [_vp, _vp, _vp, C.c_int64, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
 }
 
 _lib = None

@@ -25,8 +25,10 @@ COMMON = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler",
           f"-I{os.path.join(ROOT, 'include')}", "--expt-relaxed-constexpr"]
 # per-source extra flags: the synthetic quantiser must round like the C oracle
 EXTRA = {"synth.cu": ["-fmad=false"]}
-SOURCES = ["moe_kernels.cu", "moe_fused.cu", "moe_cluster.cu", "batch.cu", "attn.cu", "attn_fused.cu", "attn_cluster.cu", "synth.cu", "api.cu", "residency.cpp", "gguf.cpp"]
-HEADERS = ["common.cuh", "qdot.cuh", "kernels.h", "moe_common.cuh", "cluster.cuh", "ep_sync.cuh"]
+SOURCES = ["moe_kernels.cu", "moe_fused.cu", "moe_cluster.cu", "batch.cu", "attn.cu", "attn_fused.cu", "attn_cluster.cu",
+           "paged.cu", "paged_attn.cu", "sample.cu", "serve_api.cu", "synth.cu", "api.cu", "residency.cpp", "gguf.cpp"]
+HEADERS = ["common.cuh", "qdot.cuh", "kernels.h", "moe_common.cuh", "cluster.cuh", "ep_sync.cuh",
+           "paged.cuh"]
 
 
 def nvcc() -> str:
@@ -47,7 +49,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(OUT_DIR, exist_ok=True)
     hdrs = [os.path.join(CSRC, h) for h in HEADERS] + [os.path.join(ROOT, "include", h)
                                                          for h in ("styx_moe.h", "styx_residency.h", "styx_gguf.h",
-                                                                   "styx_attn.h")]
+                                                                   "styx_attn.h", "styx_serve.h")]
     objs = []
     for src in SOURCES:
         sp = os.path.join(CSRC, src)

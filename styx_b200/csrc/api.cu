@@ -292,6 +292,13 @@ int styx::set_error(int code, const char *msg) {
     g_err = msg;
     return code;
 }
+int styx::ctx_enter(styx_ctx *ctx, int *sms, int **err) {
+    ENTER(ctx);
+    if (sms) *sms = ctx->sm_count;
+    if (err) *err = ctx->d_err;
+    return STYX_OK;
+}
+bool styx::range_ok(const void *p, uint64_t bytes) { return extent_ok(p, bytes); }
 
 // Scratch of styx_moe_block_noalloc: one statically sized array per device
 // (module global memory, zero at module load), shared by every call on that

@@ -363,6 +363,67 @@ cudaError_t launch_qk_norm_rope_kv(const QkRopeArgs &a, cudaStream_t st);
 cudaError_t launch_attn_decode(const AttnArgs &a, cudaStream_t st);
 cudaError_t launch_add_f32(const float *x, const float *y, float *d, int n, cudaStream_t st);
 
+// ------------------------------------------------ batched decoding over a paged KV cache
+// styx_paged_kv with the page size as a shift
+struct PagedKv {
+    void *k, *v;
+    long long page_stride;         // elements
+    const int32_t *table, *lens;   // device
+    int dtype, n_pages, page_shift, n_kv, hd, n_seqs, max_pages, table_stride;
+    int *err;                      // device error word
+};
+struct PagedAppendArgs {
+    PagedKv kv;
+    const float *q, *k, *v;
+    long long q_stride, k_stride, v_stride;   // floats between tokens
+    const float *q_norm, *k_norm;             // [hd] or null
+    float eps;
+    double theta_scale;                       // freq_base^(-2/hd)
+    const int32_t *pos, *seq, *row;           // seq, row may be null
+    float *q_out;
+    int n_tokens, n_heads;
+};
+struct PagedAttendArgs {
+    PagedKv kv;
+    const float *q;
+    float *out, *lse;              // lse may be null
+    const float *acc;
+    float *acc_out;                // null: no accumulation
+    long long acc_stride;
+    float scale;
+    int window, n_heads, gqa;
+    float *scores, *ml;            // workspace (with acc_out): [n_seqs][n_heads][max rows], [n_seqs][n_heads][2]
+};
+struct PagedEvictArgs {
+    PagedKv kv;
+    const float *acc;
+    const int32_t *pos, *next_pos;
+    long long stride;
+    int budget, n_recent, n_sink;
+    float *acc_out;
+    int32_t *pos_out, *lens_out;
+    int32_t *src, *places;         // workspace, [n_seqs][n_kv][budget] each: the row that row r is filled from; the places
+};
+struct SampleArgs {
+    const float *logits;
+    long long row_stride;
+    int n_rows, n_vocab;
+    const float *u, *temperature;
+    const int32_t *top_k;
+    const float *top_p, *min_p;    // each may be null
+    int32_t *token;
+    float *logprob;                // may be null
+};
+cudaError_t launch_paged_append(const PagedAppendArgs &a, cudaStream_t st);
+cudaError_t launch_paged_attend(const PagedAttendArgs &a, cudaStream_t st);
+cudaError_t launch_paged_evict(const PagedEvictArgs &a, cudaStream_t st);
+cudaError_t launch_sample(const SampleArgs &a, cudaStream_t st);
+
+// for the C entry points outside api.cu: makes the context's device current,
+// gives its SM count and error word; [p, p + bytes) inside its allocation
+int ctx_enter(styx_ctx *ctx, int *sms, int **err);
+bool range_ok(const void *p, uint64_t bytes);
+
 // A launch with programmatic stream serialisation: the kernel may be
 // scheduled while the previous one on the stream drains (its CTAs start once
 // every CTA of the previous kernel has started).  Every kernel launched this

@@ -664,3 +664,213 @@ def argmax_f32(x: torch.Tensor, out: Optional[torch.Tensor] = None, stream=None)
         out = torch.empty(1, dtype=torch.int32, device=x.device)
     check(lib().styx_argmax_f32(ctx(_dev(x)).handle, _stream(stream), _ptr(x), x.numel(), _ptr(out)))
     return out
+
+
+# ------------------------------------------------------------ batched decoding over a paged KV cache
+# include/styx_serve.h
+
+_KV_TYPES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+
+
+def _f32(t: torch.Tensor, shape: tuple, what: str, device: torch.device) -> int:
+    if t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device:
+        raise ValueError(f"{what}: contiguous float32 {shape} on {device} expected, got {t.dtype} {tuple(t.shape)} "
+                         f"strides {t.stride()} on {t.device}")
+    return t.data_ptr()
+
+
+def _i32(t: torch.Tensor, shape: tuple, what: str, device: torch.device) -> int:
+    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device:
+        raise ValueError(f"{what}: contiguous int32 {shape} on {device} expected, got {t.dtype} {tuple(t.shape)} "
+                         f"strides {t.stride()} on {t.device}")
+    return t.data_ptr()
+
+
+class _On:
+    """The stream a call runs on: the given one, else the current one of the
+    device.  What the call allocates belongs to that stream."""
+
+    def __init__(self, device: torch.device, stream):
+        self.device, self.stream = device, stream
+        self.handle = (torch.cuda.current_stream(device) if stream is None else stream).cuda_stream
+
+    def empty(self, shape, dtype) -> torch.Tensor:
+        if self.stream is None:
+            return torch.empty(shape, dtype=dtype, device=self.device)
+        with torch.cuda.stream(self.stream):
+            return torch.empty(shape, dtype=dtype, device=self.device)
+
+
+class PagedKV:
+    """A paged KV cache of many sequences (styx_paged_kv) and its operators.
+
+    k, v: pools [n_pages][n_kv_heads][page_size][head_dim], f32, f16 or bf16
+    (pages may be further apart than their size, as in one layer's slice of
+    a pool of all layers); table: int32 [n_seqs][max_pages] page ids; lens:
+    int32 [n_seqs] rows in use.  The tensors stay the caller's: page ids and
+    lengths are changed in place (or `lens` replaced through the attribute).
+    Calls on one object share its workspaces: not on two streams at once."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lens: torch.Tensor):
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.stride() != v.stride():
+            raise ValueError("k and v: two pools [n_pages][n_kv_heads][page_size][head_dim] of one type and layout")
+        if k.dtype not in _KV_TYPES:
+            raise ValueError(f"cache type {k.dtype}: float32, float16 or bfloat16")
+        n_pages, n_kv, page, hd = k.shape
+        if k.stride()[1:] != (page * hd, hd, 1):
+            raise ValueError(f"pages must be contiguous (strides {k.stride()})")
+        if not k.is_cuda or v.device != k.device:
+            raise ValueError("styx ops take CUDA tensors")
+        if table.dim() != 2 or table.dtype != torch.int32 or table.stride(1) != 1 or table.device != k.device:
+            raise ValueError("table: int32 [n_seqs][max_pages] with contiguous rows on the pools' device")
+        self.k, self.v, self.table = k, v, table
+        self.device = k.device
+        self.ctx = ctx(k.device.index)
+        self.n_seqs, self.n_kv_heads, self.head_dim = table.shape[0], n_kv, hd
+        self.max_rows = table.shape[1] * page
+        self._kv = _lib.PagedKv(k.data_ptr(), v.data_ptr(), k.stride(0) if n_pages > 1 else n_kv * page * hd,
+                                table.data_ptr(), None, _KV_TYPES[k.dtype], n_pages, page, n_kv, hd, self.n_seqs,
+                                table.shape[1], table.stride(0) if self.n_seqs > 1 else table.shape[1])
+        self._ref = C.byref(self._kv)
+        self.lens = lens
+        self._attend_ws: dict[tuple, torch.Tensor] = {}
+        self._evict_ws: list[torch.Tensor] = []   # the last is in use; smaller ones may still be on a stream
+
+    @property
+    def lens(self) -> torch.Tensor:
+        return self._lens
+
+    @lens.setter
+    def lens(self, t: torch.Tensor) -> None:
+        self._kv.lens = _i32(t, (self.n_seqs,), "lens", self.device)
+        self._lens = t
+
+    def append(self, q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor,
+               freq_base: float, q_norm: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None,
+               eps: float = 1e-6, seq: Optional[torch.Tensor] = None, row: Optional[torch.Tensor] = None,
+               out: Optional[torch.Tensor] = None, stream=None) -> Optional[torch.Tensor]:
+        """Per-head RMSNorm and RoPE of q [n][n_heads][head_dim] and k
+        [n][n_kv_heads][head_dim] at pos int32 [n], the K and V rows into the
+        pages; returns the rotated q.  Token t is of sequence seq[t] (None: t)
+        and goes to its row row[t] (None: lens - 1).  q, k and v may be slices
+        of one projection's output (any stride between tokens)."""
+        dev, hd = self.device, self.head_dim
+        n, n_heads = pos.shape[0], 0 if q is None else q.shape[1]
+        on = _On(dev, stream)
+        ptrs = []
+        for t, heads, what in ((q, n_heads, "q"), (k, self.n_kv_heads, "k"), (v, self.n_kv_heads, "v")):
+            if t is None:
+                ptrs += [None, 0]
+                continue
+            if t.dtype != torch.float32 or t.shape != (n, heads, hd) or t.stride(2) != 1 or \
+                    (heads > 1 and t.stride(1) != hd) or t.device != dev:
+                raise ValueError(f"{what}: float32 [{n}][{heads}][{hd}] with contiguous heads on {dev} expected, got "
+                                 f"{t.dtype} {tuple(t.shape)} strides {t.stride()} on {t.device}")
+            ptrs += [t.data_ptr(), t.stride(0) if n > 1 else heads * hd]
+        if q is not None and out is None:
+            out = on.empty((n, n_heads, hd), torch.float32)
+        check(lib().styx_paged_append(
+            self.ctx.handle, on.handle, self._ref, n, n_heads, *ptrs,
+            None if q_norm is None else _f32(q_norm, (hd,), "q_norm", dev),
+            None if k_norm is None else _f32(k_norm, (hd,), "k_norm", dev), eps, freq_base,
+            _i32(pos, (n,), "pos", dev), None if seq is None else _i32(seq, (n,), "seq", dev),
+            None if row is None else _i32(row, (n,), "row", dev),
+            None if q is None else _f32(out, (n, n_heads, hd), "out", dev)))
+        return out if q is not None else None
+
+    def _attend_workspace(self, n_heads: int, with_acc: bool, on: _On) -> torch.Tensor:
+        ws = self._attend_ws.get((n_heads, with_acc))
+        if ws is None:
+            nb = C.c_uint64()
+            check(lib().styx_paged_attend_workspace_bytes(self.ctx.handle, self._ref, n_heads, with_acc, C.byref(nb)))
+            ws = on.empty((nb.value,), torch.uint8)
+            check(lib().styx_paged_attend_workspace_init(self.ctx.handle, on.handle, ws.data_ptr(), nb.value))
+            self._attend_ws[(n_heads, with_acc)] = ws
+        return ws
+
+    def attend(self, q: torch.Tensor, scale: Optional[float] = None, window: int = 0,
+               out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
+               acc: Optional[torch.Tensor] = None, acc_out: Optional[torch.Tensor] = None,
+               stream=None) -> torch.Tensor:
+        """Attention of one token per sequence, q f32 [n_seqs][n_heads]
+        [head_dim], over its rows (the last `window` of them, 0: all); scale
+        None: head_dim ** -0.5.  lse f32 [n_seqs][n_heads] receives the log of
+        the softmax denominators; with acc f32 [n_seqs][n_kv_heads][>= rows],
+        acc_out (None: acc itself) receives it plus each row's weight summed
+        over the kv head's q heads."""
+        dev, b, hd = self.device, self.n_seqs, self.head_dim
+        n_heads = q.shape[1] if q.dim() == 3 else 0
+        qp = _f32(q, (b, n_heads, hd), "q", dev)
+        on = _On(dev, stream)
+        if out is None:
+            out = on.empty((b, n_heads, hd), torch.float32)
+        stride, accp, accop = 0, None, None
+        if acc is not None:
+            stride = acc.shape[-1]
+            shape = (b, self.n_kv_heads, stride)
+            accp = _f32(acc, shape, "acc", dev)
+            accop = accp if acc_out is None else _f32(acc_out, shape, "acc_out", dev)
+        elif acc_out is not None:
+            raise ValueError("acc_out without acc")
+        ws = self._attend_ws.get((n_heads, accp is not None))
+        if ws is None:
+            ws = self._attend_workspace(n_heads, accp is not None, on)
+        check(lib().styx_paged_attend(
+            self.ctx.handle, on.handle, self._ref, n_heads, qp, hd ** -0.5 if scale is None else scale, window,
+            _f32(out, (b, n_heads, hd), "out", dev), None if lse is None else _f32(lse, (b, n_heads), "lse", dev),
+            accp, accop, stride, ws.data_ptr(), ws.numel()))
+        return out
+
+    def evict(self, acc: torch.Tensor, pos: torch.Tensor, next_pos: torch.Tensor, budget: int, n_recent: int = 0,
+              n_sink: int = 0, acc_out: Optional[torch.Tensor] = None, pos_out: Optional[torch.Tensor] = None,
+              lens_out: Optional[torch.Tensor] = None, stream=None):
+        """At most `budget` rows of every sequence and kv head stay: the last
+        n_recent positions, the first n_sink, then those of most accumulated
+        weight; rows beyond the budget that stay move into the places of rows
+        that leave.  Returns (acc_out, pos_out, lens_out), new tensors of the
+        shapes of acc, pos and lens; `lens` itself changes only when the
+        caller assigns lens_out to it."""
+        dev, b = self.device, self.n_seqs
+        on = _On(dev, stream)
+        stride = acc.shape[-1]
+        shape = (b, self.n_kv_heads, stride)
+        acc_out = on.empty(shape, torch.float32) if acc_out is None else acc_out
+        pos_out = on.empty(shape, torch.int32) if pos_out is None else pos_out
+        lens_out = on.empty((b,), torch.int32) if lens_out is None else lens_out
+        nb = C.c_uint64()
+        check(lib().styx_paged_evict_workspace_bytes(self._ref, budget, C.byref(nb)))
+        if not self._evict_ws or self._evict_ws[-1].numel() < nb.value:
+            self._evict_ws.append(on.empty((nb.value,), torch.uint8))
+        ws = self._evict_ws[-1]
+        check(lib().styx_paged_evict(
+            self.ctx.handle, on.handle, self._ref, _f32(acc, shape, "acc", dev), _i32(pos, shape, "pos", dev),
+            _i32(next_pos, (b,), "next_pos", dev), stride, budget, n_recent, n_sink,
+            _f32(acc_out, shape, "acc_out", dev), _i32(pos_out, shape, "pos_out", dev),
+            _i32(lens_out, (b,), "lens_out", dev), ws.data_ptr(), ws.numel()))
+        return acc_out, pos_out, lens_out
+
+
+def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Optional[torch.Tensor] = None,
+           top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None,
+           min_p: Optional[torch.Tensor] = None, token: Optional[torch.Tensor] = None,
+           logprob: Optional[torch.Tensor] = None, stream=None):
+    """One token per row of logits f32 [n][vocab] from uniform numbers u f32
+    [n] (styx_sample): temperature, top_k (int32), top_p and min_p are [n]
+    tensors, None for 1, all, 1 and 0.  Returns (token int32 [n], logprob f32
+    [n] under the distribution drawn from); token -1 where nothing is left."""
+    if logits.dim() != 2 or logits.dtype != torch.float32 or not logits.is_cuda or logits.stride(1) != 1:
+        raise ValueError(f"logits: float32 [n][vocab] CUDA tensor with contiguous rows expected, got {logits.dtype} "
+                         f"{tuple(logits.shape)} strides {logits.stride()} on {logits.device}")
+    n, vocab = logits.shape
+    dev = logits.device
+    on = _On(dev, stream)
+    token = on.empty((n,), torch.int32) if token is None else token
+    logprob = on.empty((n,), torch.float32) if logprob is None else logprob
+    check(lib().styx_sample(
+        ctx(dev.index).handle, on.handle, logits.data_ptr(), logits.stride(0) if n > 1 else vocab, n, vocab,
+        _f32(u, (n,), "u", dev), None if temperature is None else _f32(temperature, (n,), "temperature", dev),
+        None if top_k is None else _i32(top_k, (n,), "top_k", dev),
+        None if top_p is None else _f32(top_p, (n,), "top_p", dev),
+        None if min_p is None else _f32(min_p, (n,), "min_p", dev), _i32(token, (n,), "token", dev),
+        _f32(logprob, (n,), "logprob", dev)))
+    return token, logprob

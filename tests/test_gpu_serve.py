@@ -1,0 +1,582 @@
+"""Batched decoding over a paged KV cache on the GPU (include/styx_serve.h)
+against the operators' definitions in 64 bits (tests/paged_case.py).
+
+Tolerances, from the arithmetic: attention 1e-5 of max|out| (the bound of
+the single-sequence attention: scores of size ~10 rounded to f32 move a
+weight by ~1e-6, sums of some thousand rows add as much again); accumulated
+weights the same, relative to a weight sum of 1 per head.  Rotated q 2e-6 of
+max|q| (an RMSNorm, a rounded sine and cosine, three roundings: 6 x 2^-24
+and a margin); K and V rows half an ulp of the cache's type more.  Eviction
+moves whole rows and sampling sums whole numbers: equal.  A drawn token's
+interval of the 64-bit cumulative distribution may miss u by 3e-6: a weight
+exp(y) carries |y| x 2^-23 + 2^-22 of relative error, averaged over the
+distribution at most 10 x 2^-23 + 2^-22, and 2^-40 for each of the tokens.
+"""
+import numpy as np
+import pytest
+import torch
+
+from styx_b200 import StyxError, _lib, ops
+from tests.paged_case import (DEV, TYPES, attend_ref, evict_ref, make_cache, read_rows, rope_norm_ref)
+
+pytestmark = pytest.mark.gpu
+
+
+def T(a):
+    return torch.from_numpy(np.ascontiguousarray(a)).to(DEV)
+
+
+def close(got, exp, tol, what=""):
+    got, exp = np.asarray(got, np.float64), np.asarray(exp, np.float64)
+    assert got.shape == exp.shape and np.all(np.isfinite(got)), what
+    err = np.max(np.abs(got - exp), initial=0.0) / max(np.max(np.abs(exp), initial=0.0), 1e-30)
+    assert err <= tol, f"{what} {err:.2e} > {tol}"
+
+
+def queries(rng, b, h, hd):
+    return (rng.normal(0, 1, (b, h, hd)) * rng.uniform(0.3, 3, (1, h, 1))).astype(np.float32)
+
+
+# ------------------------------------------------------------------ attention
+CASES = [
+    # lens, heads, kv heads, head_dim, page, type, window
+    ([1], 32, 4, 128, 16, "f16", 0),
+    ([37], 32, 4, 128, 16, "bf16", 0),
+    ([0, 1, 15, 16, 17, 31, 32, 33], 32, 4, 128, 16, "f16", 0),
+    ([0, 0], 8, 2, 64, 64, "bf16", 0),
+    ([700, 3, 0, 129, 64], 64, 4, 128, 64, "bf16", 0),
+    ([700, 3, 0, 129, 64], 64, 4, 128, 64, "f32", 0),
+    ([2049, 513], 32, 4, 128, 32, "f16", 300),
+    ([300, 20, 1], 16, 2, 128, 256, "f32", 17),
+    ([100, 7], 6, 6, 64, 16, "f16", 0),
+    ([257, 90], 28, 4, 80, 16, "bf16", 0),
+    ([130, 61], 5, 1, 96, 32, "f16", 1),
+    ([66, 400], 14, 2, 256, 16, "bf16", 0),
+    ([66, 400], 14, 2, 256, 16, "f32", 0),
+    ([70], 40, 1, 120, 64, "f16", 0),
+    ([70, 90], 33, 1, 8, 64, "bf16", 0),
+    ([50], 4, 4, 4, 1, "f32", 0),
+    ([45, 99], 8, 4, 128, 1, "f16", 50),
+    ([45, 99], 8, 4, 128, 2, "bf16", 0),
+    ([5000], 16, 8, 64, 4096, "f16", 0),
+    ([16384], 8, 1, 128, 128, "bf16", 0),
+]
+
+
+@pytest.mark.parametrize("lens,heads,n_kv,hd,page,dtype,window", CASES)
+def test_attend(lens, heads, n_kv, hd, page, dtype, window):
+    rng = np.random.default_rng(sum(lens) + heads + hd)
+    kv, ks, vs = make_cache(rng, lens, n_kv, hd, page, dtype)
+    q = queries(rng, len(lens), heads, hd)
+    out, lse, _ = attend_ref(q, ks, vs, hd ** -0.5, window)
+    l = torch.zeros(len(lens), heads, device=DEV)
+    got = kv.attend(T(q), window=window, lse=l).cpu().numpy()
+    close(got, out, 1e-5)
+    l = l.cpu().numpy()
+    assert np.array_equal(np.isinf(l), np.isinf(lse))
+    fine = np.isfinite(lse)
+    assert np.max(np.abs(l[fine] - lse[fine]), initial=0) < 1e-5 * max(1, np.max(np.abs(lse[fine]), initial=0))
+    kv.ctx.check_device_error()
+    again = kv.attend(T(q), window=window).cpu().numpy()
+    assert np.array_equal(got, again)          # the same bits, call after call
+
+
+@pytest.mark.parametrize("lens,heads,n_kv,hd,page,dtype,window", CASES)
+def test_attend_accumulates_the_weights(lens, heads, n_kv, hd, page, dtype, window):
+    rng = np.random.default_rng(sum(lens) + heads + hd + 1)
+    kv, ks, vs = make_cache(rng, lens, n_kv, hd, page, dtype)
+    q = queries(rng, len(lens), heads, hd)
+    out, _, ws = attend_ref(q, ks, vs, hd ** -0.5, window)
+    stride = kv.max_rows + 5
+    acc = rng.uniform(0, 2, (len(lens), n_kv, stride)).astype(np.float32)
+    exp = np.full((len(lens), n_kv, stride), 7.0)
+    for b, n in enumerate(lens):
+        exp[b, :, :n] = acc[b, :, :n] + ws[b]
+        if n:
+            exp[b, :, n - 1] = ws[b][:, n - 1]      # the newest row enters with its own weight
+            acc[b, :, n - 1] = np.nan
+        acc[b, :, n:] = np.nan
+    acc_out = torch.full((len(lens), n_kv, stride), 7.0, device=DEV)
+    got = kv.attend(T(q), window=window, acc=T(acc), acc_out=acc_out)
+    close(got.cpu().numpy(), out, 1e-5)
+    got_acc = acc_out.cpu().numpy()
+    assert np.all(np.isfinite(got_acc))
+    assert np.max(np.abs(got_acc - exp)) < 1e-5 * heads / n_kv
+    inplace = T(acc)
+    kv.attend(T(q), window=window, acc=inplace)
+    for b, n in enumerate(lens):
+        assert np.array_equal(inplace.cpu().numpy()[b, :, :n], got_acc[b, :, :n])
+    kv.ctx.check_device_error()
+
+
+def test_attend_sharp_and_flat_heads():
+    """One row with all the weight (scores of +-200: every other weight
+    underflows), equal rows (the mean of V), scores all far below zero."""
+    rng = np.random.default_rng(4)
+    for dtype in TYPES:
+        kv, ks, vs = make_cache(rng, [333, 333], 2, 128, 32, dtype)
+        q = np.zeros((2, 16, 128), np.float32)
+        for h in range(8):
+            q[0, h] = ks[0][40 * h, 0] * 20.0            # row 40 h by far
+            q[1, h] = -ks[1][40 * h, 0] * 20.0
+        out, lse, _ = attend_ref(q, ks, vs, 128 ** -0.5)
+        got = kv.attend(T(q)).cpu().numpy()
+        # scores up to 230 in f32: 2^-24 x 230 x 4 of a weight
+        close(got, out, 6e-5, dtype)
+        close(got[:, 8:], np.stack([np.broadcast_to(v[:, 1].mean(0), (8, 128)) for v in vs]), 1e-5, dtype)
+
+
+def test_attend_last_page_next_to_another_sequences_rows():
+    """A page past the sequence's end belongs to somebody else, or to nobody."""
+    rng = np.random.default_rng(5)
+    kv, ks, vs = make_cache(rng, [50, 64], 2, 64, 16, "f16", max_rows=200)
+    kv.table[0, 4:] = -7
+    kv.table[1, 4:] = 1 << 30
+    q = queries(rng, 2, 8, 64)
+    close(kv.attend(T(q)).cpu().numpy(), attend_ref(q, ks, vs, 0.125)[0], 1e-5)
+    kv.ctx.check_device_error()
+
+
+def test_attend_page_outside_the_pool_is_skipped_and_reported():
+    rng = np.random.default_rng(6)
+    for bad in (-1, 1 << 20):
+        kv, ks, vs = make_cache(rng, [50, 64], 2, 64, 16, "bf16")
+        kv.table[0, 1] = bad
+        q = queries(rng, 2, 8, 64)
+        got = kv.attend(T(q)).cpu().numpy()
+        with pytest.raises(StyxError):
+            kv.ctx.check_device_error()
+        ks[0], vs[0] = (np.delete(a, range(16, 32), 0) for a in (ks[0], vs[0]))
+        close(got, attend_ref(q, ks, vs, 0.125)[0], 1e-5)
+        kv.ctx.check_device_error()
+
+
+def test_attend_length_outside_the_table_is_clamped_and_reported():
+    rng = np.random.default_rng(7)
+    kv, ks, vs = make_cache(rng, [32, 32], 1, 64, 16, "f16")
+    q = queries(rng, 2, 4, 64)
+    exp = kv.attend(T(q)).cpu().numpy()
+    kv.lens.copy_(torch.tensor([33, 32]))
+    got = kv.attend(T(q)).cpu().numpy()
+    with pytest.raises(StyxError):
+        kv.ctx.check_device_error()
+    assert np.array_equal(got, exp)
+    kv.lens.copy_(torch.tensor([32, -1]))
+    got = kv.attend(T(q)).cpu().numpy()
+    with pytest.raises(StyxError):
+        kv.ctx.check_device_error()
+    assert np.array_equal(got[0], exp[0]) and not got[1].any()
+
+
+def test_attend_pools_of_more_than_2_31_elements():
+    """Pages of one layer far apart: element offsets past 32 bits."""
+    rng = np.random.default_rng(8)
+    far = (1 << 30) + 64
+    flat = [torch.empty(2 * far + 2 * 16 * 64, dtype=torch.float16, device=DEV) for _ in range(2)]
+    k, v = (f.as_strided((3, 2, 16, 64), (far, 16 * 64, 64, 1)) for f in flat)
+    for t in (k, v):
+        t.copy_(T(rng.normal(0, 1, (3, 2, 16, 64)).astype(np.float16)))
+    table = torch.tensor([[2, 0, 1]], dtype=torch.int32, device=DEV)
+    kv = ops.PagedKV(k, v, table, torch.tensor([41], dtype=torch.int32, device=DEV))
+    ks, vs = ([a] for a in read_rows(kv, 0, 41))
+    q = queries(rng, 1, 4, 64)
+    close(kv.attend(T(q)).cpu().numpy(), attend_ref(q, ks, vs, 0.125)[0], 1e-5)
+    pos = torch.tensor([[9000] + list(range(1, 48))] * 2, dtype=torch.int32, device=DEV)[None].contiguous()
+    acc = torch.arange(96, dtype=torch.float32, device=DEV).reshape(1, 2, 48).contiguous()
+    kv.evict(acc, pos, torch.tensor([48], dtype=torch.int32, device=DEV), 20)
+    new = read_rows(kv, 0, 20)
+    src = evict_ref(acc[0, 0].cpu().numpy(), pos[0, 0].cpu().numpy(), 41, 48, 20, 0, 0)
+    assert np.array_equal(new[0][:, 0], ks[0][src, 0]) and np.array_equal(new[1][:, 1], vs[0][src, 1])
+    kv.append(None, torch.ones(1, 2, 64, device=DEV), torch.ones(1, 2, 64, device=DEV),
+              torch.zeros(1, dtype=torch.int32, device=DEV), 1e4, row=torch.tensor([9], dtype=torch.int32, device=DEV))
+    assert read_rows(kv, 0, 20)[1][9].min() == 1.0
+    kv.ctx.check_device_error()
+
+
+def test_attend_on_another_stream_and_in_a_graph():
+    rng = np.random.default_rng(9)
+    kv, ks, vs = make_cache(rng, [200, 77], 4, 128, 16, "f16")
+    q = T(queries(rng, 2, 32, 128))
+    exp = kv.attend(q)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    got = kv.attend(q, stream=s)
+    s.synchronize()
+    assert torch.equal(got, exp)
+    out = torch.zeros_like(exp)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        kv.attend(q, out=out)
+    for lens in ([200, 77], [13, 0], [1, 200 - 56]):
+        kv.lens.copy_(torch.tensor(lens))
+        g.replay()
+        torch.cuda.synchronize()
+        ref = attend_ref(q.cpu().numpy(), [ks[0][:lens[0]], ks[1][:min(77, lens[1])]],
+                         [vs[0][:lens[0]], vs[1][:min(77, lens[1])]], 128 ** -0.5)[0]
+        close(out.cpu().numpy()[0], ref[0], 1e-5)
+        if lens[1] <= 77:
+            close(out.cpu().numpy()[1], ref[1], 1e-5)
+
+
+# --------------------------------------------------------------------- append
+HALF_ULP = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}
+
+
+@pytest.mark.parametrize("n_seqs,n_tokens,heads,n_kv,hd,page,dtype,norms",
+                         [(1, 1, 32, 4, 128, 16, "f16", True), (5, 5, 8, 2, 64, 64, "bf16", True),
+                          (3, 77, 5, 1, 96, 16, "f32", True), (2, 300, 4, 4, 256, 32, "f16", False),
+                          (64, 64, 32, 4, 128, 64, "bf16", True), (4, 9, 7, 7, 8, 1, "bf16", False),
+                          (2, 33, 0, 2, 80, 128, "f16", True), (1, 1000, 16, 2, 128, 256, "f32", True),
+                          (3, 3, 3, 1, 4, 2, "f32", True)])
+def test_append(n_seqs, n_tokens, heads, n_kv, hd, page, dtype, norms):
+    rng = np.random.default_rng(n_tokens + hd)
+    count = -(-n_tokens // n_seqs)
+    kv, ks, vs = make_cache(rng, [count + 40] * n_seqs, n_kv, hd, page, dtype)
+    seq = np.arange(n_tokens) % n_seqs
+    row = rng.permutation(count + 40)[: count].astype(np.int32)[np.arange(n_tokens) // n_seqs]
+    pos = rng.integers(0, 200000, n_tokens).astype(np.int32)
+    qkv = rng.normal(0, 2, (n_tokens, (heads + 2 * n_kv) * hd + 3)).astype(np.float32)
+    d = T(qkv)
+    cut = lambda a, lo, n: a[:, lo * hd:(lo + n) * hd].reshape(n_tokens, n, hd)   # noqa: E731
+    sl = lambda lo, n: d[:, lo * hd:(lo + n) * hd].unflatten(1, (n, hd))          # noqa: E731
+    qn, kn = ((rng.uniform(0.5, 1.5, hd).astype(np.float32) if norms else None) for _ in range(2))
+    q_out = kv.append(sl(0, heads) if heads else None, sl(heads, n_kv), sl(heads + n_kv, n_kv), T(pos), 1e6,
+                      q_norm=T(qn) if norms else None, k_norm=T(kn) if norms else None, eps=1e-6,
+                      seq=T(seq.astype(np.int32)), row=T(row))
+    kv.ctx.check_device_error()
+    if heads:
+        exp = rope_norm_ref(cut(qkv, 0, heads).astype(np.float64), qn, pos, 1e6, 1e-6)
+        close(q_out.cpu().numpy(), exp, 2e-6)
+    ek = rope_norm_ref(cut(qkv, heads, n_kv).astype(np.float64), kn, pos, 1e6, 1e-6)
+    ev = cut(qkv, heads + n_kv, n_kv).astype(np.float64)
+    for t in range(n_tokens):
+        ks[seq[t]][row[t]], vs[seq[t]][row[t]] = ek[t], ev[t]
+    for b in range(n_seqs):
+        gk, gv = read_rows(kv, b, count + 40)
+        top = np.max(np.abs(ks[b]))
+        assert np.all(np.abs(gk - ks[b]) <= HALF_ULP[dtype] * np.abs(ks[b]) + 2e-6 * top + 2.0 ** -25)
+        assert np.all(np.abs(gv - vs[b]) <= HALF_ULP[dtype] * np.abs(vs[b]) + 2.0 ** -25)
+
+
+def test_append_default_rows_and_empty_slots():
+    """row None: lens - 1; a slot of length 0 and a negative row write nothing and give a zero q."""
+    rng = np.random.default_rng(11)
+    kv, ks, vs = make_cache(rng, [5, 0, 17], 2, 64, 16, "f16", max_rows=32)
+    before = [read_rows(kv, b, 32) for b in range(3)]
+    x = rng.normal(0, 1, (3, 8, 64)).astype(np.float32)
+    pos = np.array([4, 99, 16], np.int32)
+    q = kv.append(T(x), T(x[:, :2]), T(x[:, 2:4]), T(pos), 1e4)
+    kv.ctx.check_device_error()
+    exp = rope_norm_ref(x.astype(np.float64), None, pos, 1e4, 0)
+    exp[1] = 0
+    close(q.cpu().numpy(), exp, 2e-6)
+    for b, r in ((0, 4), (1, None), (2, 16)):
+        now = read_rows(kv, b, 32)
+        for i, ref in ((0, exp[b, :2]), (1, x[b, 2:4])):
+            same = np.ones(32, bool)
+            if r is not None:
+                same[r] = False
+                assert np.max(np.abs(now[i][r] - ref)) <= 2.0 ** -11 * np.max(np.abs(ref)) + 1e-6
+            assert np.array_equal(now[i][same], before[b][i][same], equal_nan=True)
+    q = kv.append(T(x), T(x[:, :2]), T(x[:, 2:4]), T(pos), 1e4, row=torch.tensor([-1, -5, -1], dtype=torch.int32, device=DEV))
+    assert not q.any()
+    kv.ctx.check_device_error()
+
+
+def test_append_out_of_range_is_skipped_and_reported():
+    rng = np.random.default_rng(12)
+    for kind in ("row", "seq", "page"):
+        kv, ks, vs = make_cache(rng, [5, 9], 2, 64, 16, "f16")
+        seq, row = torch.tensor([0, 1], dtype=torch.int32), torch.tensor([2, 3], dtype=torch.int32)
+        if kind == "row":
+            row[0] = 16
+        elif kind == "seq":
+            seq[0] = 2
+        else:
+            kv.table[0, 0] = 99
+        pools = [kv.k.clone(), kv.v.clone()]
+        x = T(rng.normal(0, 1, (2, 2, 64)).astype(np.float32))
+        kv.append(x, x, x, torch.tensor([0, 0], dtype=torch.int32, device=DEV), 1e4, seq=seq.to(DEV), row=row.to(DEV))
+        with pytest.raises(StyxError):
+            kv.ctx.check_device_error()
+        changed = (kv.k != pools[0]) & ~torch.isnan(kv.k)
+        assert {int(i) for i in changed.nonzero()[:, 0]} == {int(kv.table[1, 0])}
+
+
+def test_append_attend_agree_with_the_single_sequence_path():
+    """The step of the flat f32 cache (styx_qk_norm_rope_kv, styx_attn_decode)
+    and the same step over pages: 2e-6 of max, 1e-5 after the attention."""
+    rng = np.random.default_rng(13)
+    nh, nkv, hd, n = 32, 4, 128, 300
+    kv, ks, vs = make_cache(rng, [n], nkv, hd, 16, "f32")
+    kc = T(np.concatenate(ks).reshape(n, -1).astype(np.float32))
+    vc = T(np.concatenate(vs).reshape(n, -1).astype(np.float32))
+    q, k, v = (T(rng.normal(0, 1, (1, h, hd)).astype(np.float32)) for h in (nh, nkv, nkv))
+    w = T(rng.uniform(0.5, 1.5, hd).astype(np.float32))
+    pos = torch.tensor([n - 1], dtype=torch.int32, device=DEV)
+    q2, k2 = q.clone(), k.clone()
+    ops.qk_norm_rope_kv(q2, k2, v, w, w, 1e-6, nh, nkv, hd, 1e6, pos, kc, vc, n)
+    flat = ops.attn_decode(q2.reshape(-1), kc, vc, n, hd, nkv * hd, nh // nkv, hd ** -0.5).reshape(1, nh, hd)
+    q3 = kv.append(q, k, v, pos, 1e6, q_norm=w, k_norm=w)
+    close(q3.cpu().numpy(), q2.cpu().numpy(), 2e-6)
+    close(kv.attend(q3).cpu().numpy(), flat.cpu().numpy(), 1e-5)
+
+
+# ------------------------------------------------------------------- eviction
+@pytest.mark.parametrize("lens,n_kv,hd,page,dtype,budget,recent,sink,kind",
+                         [([40], 2, 64, 16, "f16", 16, 4, 2, "plain"),
+                          ([40, 3, 0, 16, 17], 2, 64, 16, "bf16", 16, 4, 2, "ties"),
+                          ([1], 1, 8, 1, "f16", 1, 0, 0, "plain"), ([2], 1, 4, 1, "f32", 1, 1, 0, "plain"),
+                          ([1000, 999], 4, 128, 64, "f16", 999, 100, 4, "ties"),
+                          ([1000, 5], 1, 96, 32, "f32", 1, 0, 0, "plain"),
+                          ([5000, 1025, 1024], 2, 64, 256, "bf16", 1024, 512, 4, "special"),
+                          ([300], 3, 80, 16, "f16", 128, 128, 0, "same"),
+                          ([300, 300], 3, 80, 16, "f16", 128, 0, 0, "same"),
+                          ([20000], 1, 8, 64, "f16", 7001, 50, 1, "ties"),
+                          ([70000], 1, 8, 64, "f16", 64, 8, 4, "plain")])
+def test_evict(lens, n_kv, hd, page, dtype, budget, recent, sink, kind):
+    rng = np.random.default_rng(sum(lens) + budget)
+    kv, ks, vs = make_cache(rng, lens, n_kv, hd, page, dtype)
+    B, stride = len(lens), kv.max_rows + 3
+    acc = rng.exponential(1, (B, n_kv, stride)).astype(np.float32)
+    if kind == "ties":
+        acc = np.floor(acc * 3).astype(np.float32)
+    elif kind == "same":
+        acc[:] = 0.25
+    elif kind == "special":
+        which = rng.integers(0, 8, acc.shape)
+        for i, x in enumerate((np.nan, np.inf, -np.inf, 0.0, -0.0, -1.5)):
+            acc[which == i] = x
+    pos = np.stack([[rng.permutation(stride) for _ in range(n_kv)] for _ in range(B)]).astype(np.int32)
+    nxt = np.array([stride - 2] * B, np.int32)
+    acc_out = torch.full((B, n_kv, stride), 7.0, device=DEV)
+    pos_out = torch.full((B, n_kv, stride), 7, dtype=torch.int32, device=DEV)
+    lens_out = torch.zeros(B, dtype=torch.int32, device=DEV)
+    a, p = T(acc), T(pos)
+    for _ in range(2):      # the call repeats: the inputs are left as they are
+        kv.evict(a, p, T(nxt), budget, recent, sink, acc_out=acc_out, pos_out=pos_out, lens_out=lens_out)
+        kv.ctx.check_device_error()
+        assert np.array_equal(lens_out.cpu().numpy(), np.minimum(lens, budget))
+        ao, po = acc_out.cpu().numpy(), pos_out.cpu().numpy()
+        for b, n in enumerate(lens):
+            left = min(n, budget)
+            gk, gv = read_rows(kv, b, left)
+            for j in range(n_kv):
+                src = evict_ref(acc[b, j], pos[b, j], n, int(nxt[b]), budget, recent, sink)
+                assert np.array_equal(ao[b, j, :left], acc[b, j, src], equal_nan=True)
+                assert np.array_equal(po[b, j, :left], pos[b, j, src])
+                assert np.all(ao[b, j, left:] == 7) and np.all(po[b, j, left:] == 7)
+                if left:
+                    assert np.array_equal(gk[:, j], ks[b][src, j]) and np.array_equal(gv[:, j], vs[b][src, j])
+        assert np.array_equal(a.cpu().numpy(), acc, equal_nan=True) and np.array_equal(p.cpu().numpy(), pos)
+
+
+def test_evict_duplicate_positions_still_keep_the_budget():
+    """More protected rows than the budget (positions that repeat): the lowest rows of them."""
+    rng = np.random.default_rng(21)
+    kv, ks, vs = make_cache(rng, [50], 1, 64, 16, "f16")
+    acc = rng.uniform(0, 1, (1, 1, 64)).astype(np.float32)
+    pos = np.full((1, 1, 64), 9, np.int32)
+    _, _, n = kv.evict(T(acc), T(pos), T(np.array([10], np.int32)), 20, 5, 0)
+    assert n.tolist() == [20]
+    gk, _ = read_rows(kv, 0, 20)
+    assert np.array_equal(gk, ks[0][:20])
+
+
+def test_evict_then_decode_matches_attention_over_the_rows_that_stayed():
+    rng = np.random.default_rng(22)
+    kv, ks, vs = make_cache(rng, [400, 90], 2, 128, 16, "bf16")
+    acc = rng.exponential(1, (2, 2, kv.max_rows)).astype(np.float32)
+    pos = np.broadcast_to(np.arange(kv.max_rows, dtype=np.int32), acc.shape)
+    a, p, n = kv.evict(T(acc), T(pos), T(np.array([400, 90], np.int32)), 128, 32, 4)
+    kv.lens = n
+    q = queries(rng, 2, 8, 128)
+    got = kv.attend(T(q)).cpu().numpy()
+    for b, rows in ((0, 400), (1, 90)):
+        for j in range(2):
+            src = evict_ref(acc[b, j], pos[b, j], rows, rows, 128, 32, 4)
+            ref = attend_ref(q[b:b + 1, 4 * j:4 * j + 4], [ks[b][src][:, j:j + 1]], [vs[b][src][:, j:j + 1]], 128 ** -0.5)[0]
+            close(got[b, 4 * j:4 * j + 4], ref[0], 1e-5)
+
+
+# ------------------------------------------------------------------- sampling
+def sample_ok(x, u, t, k, p, m, token, logprob):
+    """The token's interval of the 64-bit distribution holds u, to 3e-6; its log-probability to 1e-5."""
+    x = np.where(np.isnan(x), -np.inf, x.astype(np.float64))
+    top = x.max()
+    if top == -np.inf:
+        assert token == -1 and logprob == -np.inf
+        return
+    if t <= 0:
+        assert token == int(np.argmax(x)) and logprob == 0
+        return
+    with np.errstate(invalid="ignore"):
+        y = np.where(x == top, 0.0, (x - top) / t)
+    w = np.exp(y)
+    order = np.argsort(-x, kind="stable")
+    if k > 0:
+        order = order[:k]
+    cum = np.cumsum(w[order])
+    tol = 3e-6
+    lo, hi, lps = [], [], []    # with the fewest and the most tokens that the rounded sums may keep
+    for kept in (order[(cum - w[order] < (min(p, 1.0) - tol) * cum[-1]) & (w[order] >= m * (1 + 1e-5))],
+                 order[(cum - w[order] <= (min(p, 1.0) + tol) * cum[-1]) & (w[order] >= m * (1 - 1e-5))]):
+        kept = np.sort(kept) if kept.size else order[:1]
+        c = np.cumsum(w[kept])
+        at = np.searchsorted(kept, token)
+        if at < kept.size and kept[at] == token:
+            lo.append((c[at] - w[token]) / c[-1])
+            hi.append(c[at] / c[-1])
+            lps.append(y[token] - np.log(c[-1]))
+    assert lo, f"token {token} is not among those kept"
+    near = 1e-5 * max(1, abs(lps[0])) + 2 * tol / max(min(p, 1.0), 1e-3)
+    assert min(lps) - near <= logprob <= max(lps) + near, (lps, logprob)
+    assert min(lo) - tol <= u <= max(hi) + tol, (u, lo, hi)
+
+
+SETTINGS = [(1.0, 0, 1.0, 0.0), (0.6, 20, 0.95, 0.0), (0.8, 40, 1.0, 0.05), (1.3, 0, 0.9, 0.0), (0.0, 0, 1.0, 0.0),
+            (0.7, 1000, 0.8, 0.0), (1.0, 0, 1.0, 0.1), (2.0, 1, 0.5, 0.5), (1.0, 10 ** 6, 0.999, 1e-6),
+            (0.05, 0, 0.01, 0.0), (1.0, 3, 1.0, 1.0), (5.0, 0, 0.5, 0.0), (-1.0, 5, 0.3, 0.2), (1.0, -4, 2.0, -1.0)]
+
+
+@pytest.mark.parametrize("vocab,rows,kind", [(1, 3, "plain"), (2, 5, "plain"), (31, 14, "plain"), (1000, 28, "plain"),
+                                             (1000, 28, "ties"), (4097, 28, "mask"), (151936, 14, "plain"),
+                                             (151936, 14, "ties"), (151936, 14, "flat"), (33333, 28, "low"),
+                                             (200003, 14, "mask"), (262145, 5, "flat"), (65537, 28, "nan")])
+def test_sample(vocab, rows, kind):
+    rng = np.random.default_rng(vocab + rows)
+    x = (rng.normal(0, 3, (rows, vocab))).astype(np.float32)
+    if kind == "ties":
+        x = np.round(x).astype(np.float32)
+    elif kind == "flat":
+        x[:] = 1.5
+    elif kind == "mask":
+        x[rng.uniform(size=x.shape) < 0.9] = -np.inf
+    elif kind == "low":       # a mask of the type's lowest value
+        x[rng.uniform(size=x.shape) < 0.9] = np.finfo(np.float32).min
+    elif kind == "nan":
+        x[rng.uniform(size=x.shape) < 0.3] = np.nan
+        x[rng.uniform(size=x.shape) < 0.1] = -0.0
+        x[rng.uniform(size=x.shape) < 0.1] = 0.0
+    par = [SETTINGS[i % len(SETTINGS)] for i in range(rows)]
+    u = rng.uniform(0, 1, rows).astype(np.float32)
+    u[0] = 0.0
+    u[-1] = np.float32(1 - 2.0 ** -24)
+    t, k, p, m = (np.array([q[i] for q in par], np.int32 if i == 1 else np.float32) for i in range(4))
+    token, logprob = ops.sample(T(x), T(u), T(t), T(k), T(p), T(m))
+    token, logprob = token.cpu().numpy(), logprob.cpu().numpy()
+    for b in range(rows):
+        assert 0 <= token[b] < vocab
+        sample_ok(x[b], float(u[b]), float(t[b]), int(k[b]), float(p[b]), min(float(m[b]), 1.0), int(token[b]),
+                  float(logprob[b]))
+
+
+def test_sample_rows_with_nothing_left_and_infinities():
+    v = 5000
+    x = np.full((6, v), -np.inf, np.float32)
+    x[1, 77] = -3e38                       # one finite value
+    x[2] = np.nan
+    x[3, [5, 900]] = np.inf                # infinite logits share all the weight
+    x[4] = np.finfo(np.float32).min        # all at the type's lowest value: uniform
+    x[5, :] = 0
+    x[5, 1000:] = -np.inf
+    u = np.array([0.3, 0.9, 0.5, 0.75, 0.5, 0.9995], np.float32)
+    token, lp = ops.sample(T(x), T(u))
+    assert token.tolist() == [-1, 77, -1, 900, 2500, 999]
+    exp = [-np.inf, 0.0, -np.inf, np.log(0.5), -np.log(v), -np.log(1000)]
+    assert np.allclose(lp.cpu().numpy(), exp, rtol=1e-6, atol=1e-7)
+    token, _ = ops.sample(T(x), T(u), temperature=torch.zeros(6, device=DEV))
+    assert token.tolist() == [-1, 77, -1, 5, 0, 0]
+
+
+def test_sample_ties_at_the_threshold_go_to_the_lowest_index():
+    x = np.zeros((64, 3000), np.float32)
+    x[:, 2000] = 1.0
+    u = (np.arange(64, dtype=np.float32) + 0.5) / 64
+    token, _ = ops.sample(T(x), T(u), top_k=torch.full((64,), 3, dtype=torch.int32, device=DEV))
+    assert set(token.tolist()) == {0, 1, 2000}
+    w = np.exp(-1.0)
+    token, _ = ops.sample(T(x), T(u), top_p=torch.full((64,), (1 + 1.5 * w) / (1 + 2999 * w), device=DEV))
+    assert set(token.tolist()) == {0, 1, 2000}
+
+
+def test_sample_strides_defaults_and_streams():
+    rng = np.random.default_rng(31)
+    big = T(rng.normal(0, 2, (9, 4000)).astype(np.float32))
+    u = T(rng.uniform(0, 1, 9).astype(np.float32))
+    for view in (big[:, 1:3998], big[:, 3:4], big[::2, 7:1000]):
+        n = view.shape[0]
+        exp = ops.sample(view.contiguous(), u[:n].contiguous())
+        got = ops.sample(view, u[:n].contiguous())
+        assert torch.equal(exp[0], got[0]) and torch.equal(exp[1], got[1])
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        got = ops.sample(view, u[:n].contiguous(), stream=s)
+        s.synchronize()
+        assert torch.equal(exp[0], got[0])
+
+
+def test_sample_frequencies_follow_the_distribution():
+    """20000 draws of 8 tokens: every frequency within five standard deviations."""
+    p = np.array([0.4, 0.2, 0.15, 0.1, 0.06, 0.05, 0.03, 0.01])
+    n = 20000
+    x = T(np.broadcast_to(np.log(p), (n, 8)).astype(np.float32))
+    u = T(np.random.default_rng(32).uniform(0, 1, n).astype(np.float32))
+    token, lp = ops.sample(x, u)
+    got = np.bincount(token.cpu().numpy(), minlength=8) / n
+    assert np.all(np.abs(got - p) < 5 * np.sqrt(p * (1 - p) / n))
+    assert np.allclose(lp.cpu().numpy(), np.log(p)[token.cpu().numpy()], atol=1e-6)
+
+
+# ------------------------------------------------------------------- refusals
+def test_refusals():
+    rng = np.random.default_rng(41)
+    kv, _, _ = make_cache(rng, [20, 30], 2, 64, 16, "f16")
+    q = T(queries(rng, 2, 8, 64))
+    i32 = lambda *a: torch.tensor(a, dtype=torch.int32, device=DEV)   # noqa: E731
+    f = lambda *s: torch.zeros(*s, device=DEV)                        # noqa: E731
+    for call in (lambda: kv.attend(q[:1]), lambda: kv.attend(q.half()), lambda: kv.attend(q.transpose(0, 1)),
+                 lambda: kv.attend(q.cpu()), lambda: kv.attend(q, acc_out=f(2, 2, 32)),
+                 lambda: kv.attend(q, out=f(2, 8, 63)), lambda: kv.append(q, q, q, i32(0, 0), 1e4),
+                 lambda: kv.append(q, q[:, :2].half(), q[:, :2], i32(0, 0), 1e4),
+                 lambda: kv.append(q, q[:, :2], q[:, :2], f(2), 1e4),
+                 lambda: ops.sample(f(3), f(3)), lambda: ops.sample(f(3, 4), f(2)),
+                 lambda: ops.sample(f(4, 3).t(), f(3)), lambda: ops.sample(f(3, 4), f(3), top_k=f(3)),
+                 lambda: ops.PagedKV(kv.k, kv.v, kv.table.long(), kv.lens),
+                 lambda: ops.PagedKV(kv.k, kv.v.float(), kv.table, kv.lens),
+                 lambda: ops.PagedKV(kv.k.transpose(1, 2), kv.v.transpose(1, 2), kv.table, kv.lens),
+                 lambda: ops.PagedKV(kv.k, kv.v, kv.table, kv.lens[:1])):
+        with pytest.raises(ValueError):
+            call()
+    acc, pos = f(2, 2, 32), torch.zeros(2, 2, 32, dtype=torch.int32, device=DEV)
+    odd = lambda n_kv, page, hd, t=torch.float16: ops.PagedKV(   # noqa: E731
+        torch.zeros(8, n_kv, page, hd, dtype=t, device=DEV), torch.zeros(8, n_kv, page, hd, dtype=t, device=DEV),
+        kv.table, kv.lens)
+    for call in (lambda: kv.attend(T(queries(rng, 2, 7, 64))),                      # not a multiple of n_kv_heads
+                 lambda: kv.attend(q, window=-1), lambda: kv.attend(q, scale=float("nan")),
+                 lambda: kv.attend(q, acc=f(2, 2, 31)),                             # shorter than the rows
+                 lambda: odd(2, 24, 64).attend(q),                                  # page not a power of two
+                 lambda: odd(2, 16, 12).attend(f(2, 8, 12)),                        # rows of 24 bytes
+                 lambda: odd(2, 16, 264).attend(f(2, 8, 264)),
+                 lambda: odd(2, 16, 2, torch.float32).attend(f(2, 8, 2)),
+                 lambda: kv.append(q, q[:, :2], q[:, :2], i32(0, 0), 0.0),
+                 lambda: kv.append(q, q[:, :2], q[:, :2], i32(0, 0), 1e4, out=q),   # in place
+                 lambda: kv.append(f(3, 8, 64), f(3, 2, 64), f(3, 2, 64), i32(0, 0, 0), 1e4),   # 3 tokens, 2 sequences
+                 lambda: kv.evict(acc, pos, i32(9, 9), 0), lambda: kv.evict(acc, pos, i32(9, 9), 8, 6, 3),
+                 lambda: kv.evict(acc, pos, i32(9, 9), 8, -1),
+                 lambda: kv.evict(acc, pos, i32(9, 9), 8, acc_out=acc),
+                 lambda: kv.evict(acc, pos, i32(9, 9), 8, lens_out=kv.lens),
+                 lambda: kv.evict(f(2, 2, 31), pos[..., :31].contiguous(), i32(9, 9), 8)):
+        with pytest.raises(StyxError) as e:
+            call()
+        assert e.value.code == _lib.STYX_EINVAL
+    L, cx = _lib.lib(), kv.ctx.handle
+    assert L.styx_sample(cx, None, None, 4, 1, 4, None, None, None, None, None, None, None) == _lib.STYX_EINVAL
+    assert L.styx_paged_attend(cx, None, None, 8, None, 1.0, 0, None, None, None, None, 0, None, 0) == _lib.STYX_EINVAL
+    kv.attend(q)
+    ws = kv._attend_workspace(8, False, None)
+    out = torch.empty_like(q)
+    assert L.styx_paged_attend(cx, None, kv._ref, 8, q.data_ptr(), 1.0, 0, out.data_ptr(), None, None, None, 0,
+                               ws.data_ptr(), 16) == _lib.STYX_EINVAL and b"workspace" in L.styx_last_error()
+    kv.ctx.check_device_error()
