@@ -392,8 +392,14 @@ struct PagedAttendArgs {
     long long acc_stride;
     float scale;
     int window, n_heads, gqa;
-    float *scores, *ml;            // workspace (with acc_out): [n_seqs][n_heads][max rows], [n_seqs][n_heads][2]
+    // workspace (with acc_out): scores in units of log2, [n_seqs][n_kv][max
+    // rows][gqa]; maximum and sum of every head, [n_seqs][n_heads][2]
+    float *scores, *ml;
+    float *part;                   // workspace: the portions' partial results, kAttendPart floats each
+    unsigned *cnt;                 // workspace: finished portions per (sequence, kv head, group), zero between calls
 };
+// a portion of up to 16 heads of up to 128 elements: O, maxima, sums
+constexpr int kAttendPart = 16 * 128 + 32;
 struct PagedEvictArgs {
     PagedKv kv;
     const float *acc;
@@ -416,6 +422,11 @@ struct SampleArgs {
 };
 cudaError_t launch_paged_append(const PagedAppendArgs &a, cudaStream_t st);
 cudaError_t launch_paged_attend(const PagedAttendArgs &a, cudaStream_t st);
+// the tensor-core form: mk, mv map the pools as {head_dim, n_kv * page rows,
+// pages}, box 64 x min(page, 128) rows, 128-byte swizzle
+cudaError_t launch_attend_tc(const PagedAttendArgs &a, const CUtensorMap &mk, const CUtensorMap &mv, int sms,
+                             cudaStream_t st);
+cudaError_t launch_paged_acc(const PagedAttendArgs &a, cudaStream_t st);
 cudaError_t launch_paged_evict(const PagedEvictArgs &a, cudaStream_t st);
 cudaError_t launch_sample(const SampleArgs &a, cudaStream_t st);
 
@@ -423,6 +434,8 @@ cudaError_t launch_sample(const SampleArgs &a, cudaStream_t st);
 // gives its SM count and error word; [p, p + bytes) inside its allocation
 int ctx_enter(styx_ctx *ctx, int *sms, int **err);
 bool range_ok(const void *p, uint64_t bytes);
+// cuTensorMapEncodeTiled of a 3-D map, 16-bit elements, 128-byte swizzle; strides in bytes
+int encode_map3(CUtensorMap *out, void *base, const uint64_t dims[3], const uint64_t strides[2], const uint32_t box[3]);
 
 // A launch with programmatic stream serialisation: the kernel may be
 // scheduled while the previous one on the stream drains (its CTAs start once

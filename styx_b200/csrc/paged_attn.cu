@@ -35,7 +35,7 @@ __global__ void __launch_bounds__(kThreads) k_paged_attend(PagedAttendArgs a) {
     const int n = paged_len(kv, b, threadIdx.x == 0 && j == 0 && g0 == 0);
     const int first = a.window > 0 && a.window < n ? n - a.window : 0;
     const long long h0 = static_cast<long long>(b) * a.n_heads + j * a.gqa + g0;   // global index of the first head
-    for (int i = threadIdx.x; i < ng * hd; i += kThreads) sq[i / hd][i % hd] = a.q[h0 * hd + i] * a.scale;
+    for (int i = threadIdx.x; i < ng * hd; i += kThreads) sq[i / hd][i % hd] = a.q[h0 * hd + i] * (a.scale * 1.4426950408889634f);
     __syncthreads();
     float m[kHeads], l[kHeads], o[kHeads][kPerLane];
 #pragma unroll
@@ -45,7 +45,8 @@ __global__ void __launch_bounds__(kThreads) k_paged_attend(PagedAttendArgs a) {
 #pragma unroll
         for (int i = 0; i < kPerLane; i++) o[g][i] = 0.f;
     }
-    const long long max_rows = static_cast<long long>(kv.max_pages) << kv.page_shift;
+    float *scores = a.scores + (static_cast<long long>(b) * kv.n_kv + j) *
+                                   (static_cast<long long>(kv.max_pages) << kv.page_shift) * a.gqa + g0;
     for (int r = first + warp; r < n; r += kWarps) {
         const long long off = paged_off(kv, b, j, r);
         if (off < 0 && lane == 0) atomicExch(kv.err, kErrBadPos);
@@ -64,9 +65,9 @@ __global__ void __launch_bounds__(kThreads) k_paged_attend(PagedAttendArgs a) {
                 for (int i = 0; i < kPerLane; i++)
                     if (lane + 32 * i < hd) s += kr[i] * sq[g][lane + 32 * i];
                 s = off >= 0 ? warp_sum(s) : -INFINITY;
-                if (a.acc_out && lane == 0) a.scores[(h0 + g) * max_rows + r] = s;
+                if (a.acc_out && lane == 0) scores[static_cast<long long>(r) * a.gqa + g] = s;
                 if (s > -INFINITY) {
-                    const float mn = fmaxf(m[g], s), f = expf(m[g] - mn), p = expf(s - mn);
+                    const float mn = fmaxf(m[g], s), f = exp2f(m[g] - mn), p = exp2f(s - mn);
                     m[g] = mn;
                     l[g] = l[g] * f + p;
 #pragma unroll
@@ -87,8 +88,8 @@ __global__ void __launch_bounds__(kThreads) k_paged_attend(PagedAttendArgs a) {
         if (g >= ng) break;
         float M = -INFINITY, L = 0.f;
         for (int w = 0; w < kWarps; w++) M = fmaxf(M, sm[w][g]);
-        for (int w = 0; w < kWarps; w++) L += sl[w][g] > 0.f ? expf(sm[w][g] - M) * sl[w][g] : 0.f;
-        const float f = l[g] > 0.f ? expf(m[g] - M) / L : 0.f;
+        for (int w = 0; w < kWarps; w++) L += sl[w][g] > 0.f ? exp2f(sm[w][g] - M) * sl[w][g] : 0.f;
+        const float f = l[g] > 0.f ? exp2f(m[g] - M) / L : 0.f;
 #pragma unroll
         for (int i = 0; i < kPerLane; i++)
             if (lane + 32 * i < hd) so[warp][lane + 32 * i] = f > 0.f ? o[g][i] * f : 0.f;
@@ -99,7 +100,7 @@ __global__ void __launch_bounds__(kThreads) k_paged_attend(PagedAttendArgs a) {
             a.out[(h0 + g) * hd + c] = s;
         }
         if (threadIdx.x == 0) {
-            if (a.lse) a.lse[h0 + g] = L > 0.f ? M + logf(L) : -INFINITY;
+            if (a.lse) a.lse[h0 + g] = L > 0.f ? M * 0.6931471805599453f + logf(L) : -INFINITY;
             if (a.acc_out) {
                 a.ml[2 * (h0 + g)] = M;
                 a.ml[2 * (h0 + g) + 1] = L;
@@ -121,12 +122,13 @@ __global__ void __launch_bounds__(256) k_paged_acc(PagedAttendArgs a) {
     const long long max_rows = static_cast<long long>(kv.max_pages) << kv.page_shift;
     const long long h0 = static_cast<long long>(b) * a.n_heads + j * a.gqa;
     const long long line = (static_cast<long long>(b) * kv.n_kv + j) * a.acc_stride;
+    const float *scores = a.scores + (static_cast<long long>(b) * kv.n_kv + j) * max_rows * a.gqa;
     for (int r = blockIdx.x * 256 + threadIdx.x; r < n; r += gridDim.x * 256) {
         float w = 0.f;
         if (r >= first)
             for (int g = 0; g < a.gqa; g++) {
                 const float L = a.ml[2 * (h0 + g) + 1];
-                if (L > 0.f) w += expf(a.scores[(h0 + g) * max_rows + r] - a.ml[2 * (h0 + g)]) / L;
+                if (L > 0.f) w += exp2f(scores[static_cast<long long>(r) * a.gqa + g] - a.ml[2 * (h0 + g)]) / L;
             }
         a.acc_out[line + r] = r == n - 1 ? w : a.acc[line + r] + w;
     }
@@ -140,7 +142,10 @@ cudaError_t launch_paged_attend(const PagedAttendArgs &a, cudaStream_t st) {
     if (a.kv.dtype == STYX_F16) e = launch_pdl(k_paged_attend<__half>, grid, block, 0, st, a);
     else if (a.kv.dtype == STYX_BF16) e = launch_pdl(k_paged_attend<__nv_bfloat16>, grid, block, 0, st, a);
     else e = launch_pdl(k_paged_attend<float>, grid, block, 0, st, a);
-    if (e != cudaSuccess || !a.acc_out) return e;
+    return e;
+}
+
+cudaError_t launch_paged_acc(const PagedAttendArgs &a, cudaStream_t st) {
     const long long max_rows = static_cast<long long>(a.kv.max_pages) << a.kv.page_shift;
     const dim3 ga(static_cast<unsigned>(max_rows < 64 * 256 ? (max_rows + 255) / 256 : 64),
                   static_cast<unsigned>(a.kv.n_seqs) * a.kv.n_kv);

@@ -85,15 +85,20 @@ int check_kv(const styx_paged_kv *kv, bool with_buffers, styx::PagedKv &o) {
 }
 uint64_t max_rows(const styx_paged_kv *kv) { return static_cast<uint64_t>(kv->max_pages) * kv->page_size; }
 
-// attend's workspace: with weights, every head's maximum and sum, and every
-// row's scores
+// attend's workspace: the finished portions of every (sequence, kv head,
+// group of 8 or more heads), two partial results per CTA; with weights,
+// every head's maximum and sum, and every row's scores
 struct AttendWs {
-    uint64_t ml, scores, total;
+    uint64_t cnt, part, ml, scores, total;
 };
-AttendWs attend_ws(const styx_paged_kv *kv, int n_heads, bool with_acc) {
+AttendWs attend_ws(const styx_paged_kv *kv, int n_heads, bool with_acc, int sms) {
     AttendWs w{};
-    uint64_t o = 256;
+    uint64_t o = 0;
     const uint64_t heads = static_cast<uint64_t>(kv->n_seqs) * n_heads;
+    w.cnt = o;
+    o += a256(heads * 4);
+    w.part = o;
+    o += a256(2ull * sms * styx::kAttendPart * 4);
     w.ml = o;
     if (with_acc) o += a256(heads * 8);
     w.scores = o;
@@ -161,11 +166,12 @@ int styx_paged_append(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv
 
 int styx_paged_attend_workspace_bytes(styx_ctx *ctx, const styx_paged_kv *kv, int n_heads, int with_acc, uint64_t *out) {
     styx::PagedKv o{};
-    CHECK(styx::ctx_enter(ctx, nullptr, nullptr));
+    int sms = 0;
+    CHECK(styx::ctx_enter(ctx, &sms, nullptr));
     CHECK(check_kv(kv, false, o));
     NEED(out && n_heads > 0 && n_heads % kv->n_kv_heads == 0, "n_heads %d must be a multiple of n_kv_heads %d", n_heads,
          kv->n_kv_heads);
-    *out = attend_ws(kv, n_heads, with_acc != 0).total;
+    *out = attend_ws(kv, n_heads, with_acc != 0, sms).total;
     return STYX_OK;
 }
 
@@ -180,7 +186,8 @@ int styx_paged_attend(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv
                       float scale, int window, float *out, float *lse, const float *acc, float *acc_out,
                       int64_t acc_stride, void *workspace, uint64_t workspace_bytes) {
     styx::PagedAttendArgs a{};
-    CHECK(styx::ctx_enter(ctx, nullptr, &a.kv.err));
+    int sms = 0;
+    CHECK(styx::ctx_enter(ctx, &sms, &a.kv.err));
     CHECK(check_kv(kv, true, a.kv));
     NEED(n_heads > 0 && n_heads <= 65535 && n_heads % kv->n_kv_heads == 0, "n_heads %d must be a multiple of n_kv_heads %d",
          n_heads, kv->n_kv_heads);
@@ -201,7 +208,7 @@ int styx_paged_attend(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv
         NEED(kv->n_seqs * static_cast<int64_t>(kv->n_kv_heads) <= 65535, "accumulation: n_seqs x n_kv_heads <= 65535");
         NEED(styx::range_ok(acc, lines) && styx::range_ok(acc_out, lines), "acc / acc_out smaller than n_seqs x n_kv_heads lines");
     }
-    const AttendWs w = attend_ws(kv, n_heads, acc_out != nullptr);
+    const AttendWs w = attend_ws(kv, n_heads, acc_out != nullptr, sms);
     NEED(workspace_bytes >= w.total && styx::range_ok(workspace, w.total), "workspace: %llu bytes needed",
          static_cast<unsigned long long>(w.total));
     char *ws = static_cast<char *>(workspace);
@@ -217,7 +224,24 @@ int styx_paged_attend(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv
     a.gqa = n_heads / kv->n_kv_heads;
     a.ml = reinterpret_cast<float *>(ws + w.ml);
     a.scores = reinterpret_cast<float *>(ws + w.scores);
-    CK(styx::launch_paged_attend(a, S(stream)));
+    a.part = reinterpret_cast<float *>(ws + w.part);
+    a.cnt = reinterpret_cast<unsigned *>(ws + w.cnt);
+    // the tensor cores take 16-bit rows of 64 to 128 elements in pages of 16
+    // rows or more (a TMA box of fewer rows would break the operands' 8-row
+    // groups); everything else runs on the FMA units
+    if (kv->dtype != STYX_F32 && kv->head_dim >= 64 && kv->head_dim <= 128 && kv->page_size >= 16) {
+        CUtensorMap mk, mv;
+        const uint64_t dims[3] = {static_cast<uint64_t>(kv->head_dim), static_cast<uint64_t>(kv->n_kv_heads) * kv->page_size,
+                                  static_cast<uint64_t>(kv->n_pages)};
+        const uint64_t strides[2] = {kv->head_dim * 2ull, static_cast<uint64_t>(kv->page_stride) * 2};
+        const uint32_t box[3] = {64, static_cast<uint32_t>(kv->page_size < 128 ? kv->page_size : 128), 1};
+        CHECK(styx::encode_map3(&mk, kv->k, dims, strides, box));
+        CHECK(styx::encode_map3(&mv, kv->v, dims, strides, box));
+        CK(styx::launch_attend_tc(a, mk, mv, sms, S(stream)));
+    } else {
+        CK(styx::launch_paged_attend(a, S(stream)));
+    }
+    if (acc_out) CK(styx::launch_paged_acc(a, S(stream)));
     return STYX_OK;
 }
 
