@@ -23,13 +23,16 @@
 // CTA that finishes a segment's last portion joins them in order.  Which CTA
 // that is does not change the result.
 //
-// Roles, linked by mbarriers with bounded waits: warps 0-3 softmax (thread =
-// row of the tile; in the end thread = element of head_dim), warp 4 copies K,
-// warp 5 copies V (a ring of 3 stages of 128 rows, 192 KB: more than the
-// bytes in flight that HBM's latency needs), warp 6 issues the MMAs.  The
-// maximum a row is measured against moves only when a score passes it by
-// 2^8, so the accumulator is rescaled rarely and no tile waits for an exact
-// running maximum; sums and exponentials are unaffected by which one is used.
+// Roles, linked by mbarriers with bounded waits: two softmax warpgroups take
+// alternate tiles (thread = row of the tile), each with its own score buffer,
+// maxima, sums, P and accumulator, so that one's chain scores -> exponentials
+// -> P -> product overlaps the other's; they are added up at the portion's
+// end (thread = element of head_dim).  One warp copies K, one copies V (rings
+// of 2 or 3 tiles, 160 to 192 KB: more than the bytes in flight that HBM's
+// latency needs), one thread issues the MMAs.  The maximum a row is measured
+// against moves only when a score passes it by 2^8, so the accumulator is
+// rescaled rarely and no tile waits for an exact running maximum; sums and
+// exponentials are unaffected by which one is used.
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -40,45 +43,49 @@ namespace styx {
 namespace {
 
 constexpr int kTile = 128;                 // rows of a tile = M of both products
-constexpr int kStages = 3;
 constexpr int kHalfBytes = kTile * 128;    // 64 columns of a tile: 128-byte rows
 constexpr int kSlotBytes = 2 * kHalfBytes; // K or V of a tile
-constexpr int kThreads = 224;
-constexpr int kWarpK = 4, kWarpV = 5, kWarpMma = 6;
-constexpr uint32_t kTmemCols = 256, kColS = 64, kColO = 128;
+constexpr int kThreads = 352;
+constexpr int kWarpK = 8, kWarpV = 9, kWarpMma = 10;
+constexpr uint32_t kTmemCols = 256, kColS = 0, kColO = 128, kColStep = 64;   // two score buffers, two accumulators
 constexpr float kSlack = 8.f;              // log2 units a score may pass the maximum by
+constexpr float kNone = -3e38f;            // maximum of no scores: finite, so that differences stay numbers
 
 template <bool BF, int NH>
 struct Cfg {
     static constexpr int terms = BF ? 3 : 2;
     static constexpr int nb = (terms * NH + 15) / 16 * 16;   // N of the products (M 128: multiples of 16)
     static constexpr int q_bytes = 2 * nb * 128, p_bytes = 2 * nb * 128;
-    static constexpr int smem = 2 * kStages * kSlotBytes + q_bytes + p_bytes + 1024;
+    // a P buffer also holds the join's weights: NH for each of up to 152 portions
+    static constexpr int p_alloc = (p_bytes > 152 * NH * 4 ? p_bytes : 152 * NH * 4) + 1023 & ~1023;
+    static constexpr int k_stages = 3, v_stages = nb <= 32 ? 3 : 2;   // what 227 KB hold
+    static constexpr int smem = (k_stages + v_stages) * kSlotBytes + q_bytes + 2 * p_alloc + 1024;
     // term of a small p keeps its bits; bf16 has f32's range
 };
 
 // ------------------------------------------------------------ tensor-core helpers
-// shared-memory operand, 128-byte swizzle, descriptor version 1.  K-major:
-// sbo = bytes between groups of 8 rows.  M-major: lbo = bytes between blocks
-// of 64 along M, sbo = bytes between groups of 8 along K.
-__device__ __forceinline__ uint64_t desc_sw128(uint32_t addr, uint32_t lbo, uint32_t sbo) {
-    uint64_t d = static_cast<uint64_t>((addr >> 4) & 0x3FFFu);
-    d |= static_cast<uint64_t>((lbo >> 4) & 0x3FFFu) << 16;
-    d |= static_cast<uint64_t>((sbo >> 4) & 0x3FFFu) << 32;
-    d |= static_cast<uint64_t>(1) << 46;
-    d |= static_cast<uint64_t>(2) << 61;
-    return d;
-}
+// Shared-memory operand descriptors (version 1, 128-byte swizzle).  The high
+// word is the same for all: 1024 bytes between groups of 8 rows (K-major) or
+// of 8 along K (M-major).  The low word is address / 16, and for M-major the
+// bytes / 16 between blocks of 64 along M: advancing is an addition.
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lbo) { return (addr >> 4) | ((lbo >> 4) << 16); }
 // f32 accumulator, A and B both f16 or both bf16, M 128; a_mn: A is M-major
 constexpr uint32_t idesc(bool bf, int n, bool a_mn) {
     return (1u << 4) | (bf ? (1u << 7) | (1u << 10) : 0u) | (a_mn ? 1u << 15 : 0u) |
            (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kTile >> 4) << 24);
 }
-__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t id, bool acc) {
+__device__ __forceinline__ void mma(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t id, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(id), "r"(static_cast<uint32_t>(acc)));
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}\n" ::"r"(d),
+        "r"(a_lo), "r"(b_lo), "r"(id), "r"(acc), "n"(kDescHi));
+}
+__device__ __forceinline__ bool elect() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
 }
 __device__ __forceinline__ void commit(uint64_t *bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
@@ -102,13 +109,9 @@ __device__ __forceinline__ void st8(uint32_t addr, const float *v) {
                  "r"(__float_as_uint(v[6])), "r"(__float_as_uint(v[7]))
                  : "memory");
 }
-// N columns of this thread's lane; the values are valid after the wait, which
-// the compiler must not move their uses across
+// the loads above are done; no use of their values moves up across this
 template <int N>
-__device__ __forceinline__ void ld_cols(uint32_t addr, float (&v)[N]) {
-    static_assert(N % 8 == 0, "columns by eights");
-#pragma unroll
-    for (int c = 0; c < N; c += 8) ld8(addr + c, v + c);
+__device__ __forceinline__ void ld_done(float (&v)[N]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
     for (int c = 0; c < N; c++) asm volatile("" : "+f"(v[c]));
@@ -120,14 +123,18 @@ __device__ __forceinline__ void tma3(void *dst, const CUtensorMap *map, int x, i
         "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar))
         : "memory");
 }
-__device__ __forceinline__ void wg_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
-__device__ __forceinline__ bool wg_any(bool v) {
+// barriers of one softmax warpgroup (0 or 1), and of both
+__device__ __forceinline__ void wg_sync(int wg) { asm volatile("bar.sync %0, 128;" ::"r"(1 + wg) : "memory"); }
+__device__ __forceinline__ void both_sync() { asm volatile("bar.sync 3, 256;" ::: "memory"); }
+__device__ __forceinline__ void read_arrive() { asm volatile("bar.arrive 4, 256;" ::: "memory"); }
+__device__ __forceinline__ void read_sync() { asm volatile("bar.sync 4, 256;" ::: "memory"); }
+__device__ __forceinline__ bool wg_any(int wg, bool v) {
     uint32_t r;
     asm volatile(
         "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\t"
-        "barrier.cta.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        "barrier.cta.red.or.pred q, %2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
         : "=r"(r)
-        : "r"(static_cast<uint32_t>(v))
+        : "r"(static_cast<uint32_t>(v)), "r"(1 + wg)
         : "memory");
     return r != 0;
 }
@@ -137,17 +144,18 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// v as a sum of terms of the cache's type, largest first
+// v as a sum of terms of the cache's type, largest first.  bf16: the f32's 24
+// significant bits cut into 8 + 8 + 8, exactly; f16: rounded to 11, the rest
+// rounded to 11.
 template <bool BF>
 __device__ __forceinline__ void split(float v, uint16_t (&t)[BF ? 3 : 2]) {
     if constexpr (BF) {
-        const __nv_bfloat16 a = __float2bfloat16_rn(v);
-        const float r = v - __bfloat162float(a);
-        const __nv_bfloat16 b = __float2bfloat16_rn(r);
-        const __nv_bfloat16 c = __float2bfloat16_rn(r - __bfloat162float(b));
-        t[0] = __bfloat16_as_ushort(a);
-        t[1] = __bfloat16_as_ushort(b);
-        t[2] = __bfloat16_as_ushort(c);
+        const uint32_t a = __float_as_uint(v);
+        const uint32_t b = __float_as_uint(v - __uint_as_float(a & 0xFFFF0000u));
+        const uint32_t c = __float_as_uint(__uint_as_float(b) - __uint_as_float(b & 0xFFFF0000u));
+        t[0] = static_cast<uint16_t>(a >> 16);
+        t[1] = static_cast<uint16_t>(b >> 16);
+        t[2] = static_cast<uint16_t>(c >> 16);
     } else {
         const __half a = __float2half_rn(v);
         t[0] = __half_as_ushort(a);
@@ -160,8 +168,8 @@ __device__ __forceinline__ uint32_t b_off(int nb, int n, int c) {
 }
 
 struct Bars {
-    uint64_t kfull[kStages], kempty[kStages], vfull[kStages], vempty[kStages];
-    uint64_t sfull[2], pfull, odone, qfull, drain;
+    uint64_t kfull[3], kempty[3], vfull[3], vempty[3];
+    uint64_t sfull[2], pfull[2], odone[2], qfull, drain;
 };
 
 // rows of a sequence that are seen, and its tiles (an empty one counts one
@@ -206,28 +214,31 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int NB = C::nb, TERMS = C::terms;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *sm = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
-    uint8_t *sK = sm, *sV = sm + kStages * kSlotBytes, *sQ = sV + kStages * kSlotBytes, *sP = sQ + C::q_bytes;
+    uint8_t *sK = sm, *sV = sm + C::k_stages * kSlotBytes, *sQ = sV + C::v_stages * kSlotBytes, *sP = sQ + C::q_bytes;
     __shared__ Bars bars;
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort, s_b0, s_last;
     __shared__ long long s_off, s_scan[kThreads];
-    __shared__ float s_red[4][16], s_f[16];
+    __shared__ float s_red[8][16], s_l[8][16], s_ml[2][16], s_f[16];
     const PagedKv &kv = a.kv;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int groups = (a.gqa + NH - 1) / NH, segs = kv.n_kv * groups;
 
     pdl_trigger();
+    if (tid == 32 * kWarpK) asm volatile("prefetch.tensormap [%0];" ::"l"(&mk));
+    if (tid == 32 * kWarpV) asm volatile("prefetch.tensormap [%0];" ::"l"(&mv));
     if (tid == 0) {
-        for (int i = 0; i < kStages; i++) {
+        for (int i = 0; i < 3; i++) {
             mbar_init(&bars.kfull[i], 1);
             mbar_init(&bars.kempty[i], 1);
             mbar_init(&bars.vfull[i], 1);
             mbar_init(&bars.vempty[i], 1);
         }
-        mbar_init(&bars.sfull[0], 1);
-        mbar_init(&bars.sfull[1], 1);
-        mbar_init(&bars.pfull, 128);
-        mbar_init(&bars.odone, 1);
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&bars.sfull[i], 1);
+            mbar_init(&bars.pfull[i], 128);
+            mbar_init(&bars.odone[i], 1);
+        }
         mbar_init(&bars.qfull, 128);
         mbar_init(&bars.drain, 1);
         fence_mbar_init();
@@ -248,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int b = lo; b < hi; b++) mine += static_cast<long long>(Seq(a, b, blockIdx.x == 0).nt) * segs;
         s_scan[tid] = mine;
         __syncthreads();
-        if (warp == 0) {   // inclusive scan of the kThreads chunks, seven per lane
+        if (warp == 0) {   // inclusive scan of the kThreads chunks
             long long v[kThreads / 32], run = 0;
 #pragma unroll
             for (int i = 0; i < kThreads / 32; i++) {
@@ -309,6 +320,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == kWarpK || warp == kWarpV) {
         // ---------------- copies: boxes of min(page, 128) rows x 64 columns
         const bool isv = warp == kWarpV;
+        const int stages = isv ? C::v_stages : C::k_stages;
         const CUtensorMap *map = isv ? &mv : &mk;
         uint8_t *ring = isv ? sV : sK;
         uint64_t *full = isv ? bars.vfull : bars.kfull, *empty = isv ? bars.vempty : bars.kempty;
@@ -322,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int j = wk.seg / groups;
             const int32_t *table = kv.table + static_cast<long long>(wk.b) * kv.table_stride;
             for (int t = wk.t0; t < wk.t1; t++, q++) {
-                const int st = q % kStages, use = q / kStages;
+                const int st = q % stages, use = q / stages;
                 const int r0 = (s.tile0 + t) * kTile + (pi << rb_shift);
                 bool on = lane < boxes && r0 < s.n && r0 + rows > s.first;
                 int page = 0;
@@ -346,50 +358,62 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
         // nothing of this warp's is still landing when the CTA ends
-        for (int i = max(0, q - kStages); i < q; i++) mbar_wait(&full[i % kStages], static_cast<uint32_t>((i / kStages) & 1), nullptr, 0);
+        for (int i = max(0, q - stages); i < q; i++)
+            mbar_wait(&full[i % stages], static_cast<uint32_t>((i / stages) & 1), nullptr, 0);
     } else if (warp == kWarpMma) {
-        // ---------------- one thread issues the products
-        if (lane == 0) {
-            constexpr uint32_t id_s = idesc(BF, NB, false), id_o = idesc(BF, NB, true);
-            const int ksteps = (kv.hd + 15) / 16;
-            const uint32_t aK = smem_addr(sK), aV = smem_addr(sV), aQ = smem_addr(sQ), aP = smem_addr(sP);
-            int q = 0, portion = 0;
-            bool live = true;
-            auto scores = [&](int i) {   // S of tile i (global number) into buffer i % 2
-                const int st = i % kStages;
-                if (!wait(&bars.kfull[st], static_cast<uint32_t>((i / kStages) & 1))) return false;
-                fence_after();
-                for (int k = 0; k < ksteps; k++) {
-                    const uint32_t in = static_cast<uint32_t>(k & 3) * 32;
-                    mma(tmem + (i & 1) * kColS,
-                        desc_sw128(aK + st * kSlotBytes + (k >> 2) * kHalfBytes + in, 16, 1024),
-                        desc_sw128(aQ + (k >> 2) * NB * 128 + in, 16, 1024), id_s, k > 0);
-                }
+        // ---------------- the products: the warp walks together (what an
+        // MMA is given stays in uniform registers), one lane issues
+        constexpr uint32_t id_s = idesc(BF, NB, false), id_o = idesc(BF, NB, true);
+        const bool leader = elect();
+        const int ksteps = (kv.hd + 15) / 16;
+        const uint32_t dK = desc_lo(smem_addr(sK), 16), dV = desc_lo(smem_addr(sV), kHalfBytes);
+        const uint32_t dQ = desc_lo(smem_addr(sQ), 16), dP = desc_lo(smem_addr(sP), 16);
+        int q = 0, portion = 0;
+        bool live = true;
+        auto scores = [&](int i) {   // S of tile i (global number) into buffer i % 2
+            const int st = i % C::k_stages;
+            if (!__all_sync(0xffffffffu, wait(&bars.kfull[st], static_cast<uint32_t>((i / C::k_stages) & 1)))) return false;
+            fence_after();
+            if (leader) {
+                const uint32_t dk = dK + static_cast<uint32_t>(st) * (kSlotBytes / 16), d = tmem + kColS + (i & 1) * kColStep;
+#pragma unroll
+                for (int k = 0; k < 8; k++)
+                    if (k < ksteps)
+                        mma(d, dk + (k >> 2) * (kHalfBytes / 16) + (k & 3) * 2, dQ + (k >> 2) * (NB * 128 / 16) + (k & 3) * 2,
+                            id_s, k > 0);
                 commit(&bars.kempty[st]);
                 commit(&bars.sfull[i & 1]);
-                return true;
-            };
-            while (live && wk.next(a, segs)) {
-                const int nt = wk.t1 - wk.t0;
-                if (!wait(&bars.qfull, static_cast<uint32_t>(portion & 1))) break;
+            }
+            __syncwarp();
+            return true;
+        };
+        while (live && wk.next(a, segs)) {
+            const int nt = wk.t1 - wk.t0;
+            if (!__all_sync(0xffffffffu, wait(&bars.qfull, static_cast<uint32_t>(portion & 1)))) break;
+            fence_after();
+            live = scores(q) && (nt < 2 || scores(q + 1));
+            for (int t = 0; t < nt && live; t++, q++) {
+                const int st = q % C::v_stages, wg = q & 1;
+                live = __all_sync(0xffffffffu, wait(&bars.vfull[st], static_cast<uint32_t>((q / C::v_stages) & 1)) &&
+                                                   wait(&bars.pfull[wg], static_cast<uint32_t>((q >> 1) & 1)));
+                if (!live) break;
                 fence_after();
-                live = scores(q);
-                for (int t = 0; t < nt && live; t++, q++) {
-                    if (t + 1 < nt && !(live = scores(q + 1))) break;
-                    const int st = q % kStages;
-                    if (!(live = wait(&bars.vfull[st], static_cast<uint32_t>((q / kStages) & 1)))) break;
-                    if (!(live = wait(&bars.pfull, static_cast<uint32_t>(q & 1)))) break;
-                    fence_after();
+                if (leader) {
+                    const uint32_t dv = dV + static_cast<uint32_t>(st) * (kSlotBytes / 16), d = tmem + kColO + wg * kColStep;
+                    const uint32_t dp = dP + static_cast<uint32_t>(wg) * (C::p_alloc / 16);
 #pragma unroll
                     for (int k = 0; k < kTile / 16; k++)
-                        mma(tmem + kColO, desc_sw128(aV + st * kSlotBytes + k * 2048, kHalfBytes, 1024),
-                            desc_sw128(aP + (k >> 2) * NB * 128 + (k & 3) * 32, 16, 1024), id_o, t > 0 || k > 0);
+                        mma(d, dv + k * (2048 / 16), dp + (k >> 2) * (NB * 128 / 16) + (k & 3) * 2, id_o, t > 1 || k > 0);
                     commit(&bars.vempty[st]);
-                    commit(&bars.odone);
+                    commit(&bars.odone[wg]);
                 }
-                portion++;
+                __syncwarp();
+                if (t + 2 < nt) live = scores(q + 2);   // the warpgroup has read its scores of tile q
             }
-            // every product issued here has completed before TMEM is freed
+            portion++;
+        }
+        // every product issued here has completed before TMEM is freed
+        if (leader) {
             commit(&bars.drain);
             mbar_wait(&bars.drain, 0u, nullptr, 0);
         }
@@ -397,81 +421,95 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else {
         // ---------------- softmax: thread = row of the tile.  A wait that gave
         // up is not looked at here: every thread goes on to the end, so the
-        // four warps stay together at their barriers (later waits return at
-        // once, the results are void and the error word says so).
-        const uint32_t lane_base = static_cast<uint32_t>(32 * warp) << 16;
+        // warps stay together at their barriers (later waits return at once,
+        // the results are void and the error word says so).
+        const int wg = warp >> 2, tg = tid & 127;
+        const uint32_t lane_base = static_cast<uint32_t>(32 * (warp & 3)) << 16;
+        const uint32_t colS = tmem + kColS + wg * kColStep + lane_base, colO = tmem + kColO + wg * kColStep + lane_base;
+        uint8_t *myP = sP + wg * C::p_alloc;
         const float l2 = a.scale * 1.4426950408889634f;   // scores in units of log2
         const long long max_rows = static_cast<long long>(kv.max_pages) << kv.page_shift;
-        int q = 0;
+        int q = 0, portion = 0;                            // the portion's first tile (global number), its number
         while (wk.next(a, segs)) {
             const Seq s(a, wk.b, false);
             const int j = wk.seg / groups, g0 = (wk.seg - j * groups) * NH, ng = min(NH, a.gqa - g0);
             const long long h0 = static_cast<long long>(wk.b) * a.n_heads + j * a.gqa + g0;
             const int32_t *table = kv.table + static_cast<long long>(wk.b) * kv.table_stride;
-            float fh[NH];          // what a column of S is in units of its terms
-            {                      // Q: thread = element, split into terms
+            if (wg == 1) {
+                // Q, by the second warpgroup, so that the next portion starts while the first still writes the last
+                // one's result.  Thread = element.  f16 has few exponents: every head's largest |q| is brought to
+                // [2^9, 2^10), and s_f says what a column of S is in units of its terms.
                 float qv[NH];
 #pragma unroll
-                for (int h = 0; h < NH; h++) qv[h] = h < ng && tid < kv.hd ? __ldg(a.q + (h0 + h) * kv.hd + tid) * l2 : 0.f;
+                for (int h = 0; h < NH; h++) qv[h] = h < ng && tg < kv.hd ? __ldg(a.q + (h0 + h) * kv.hd + tg) * l2 : 0.f;
                 if constexpr (!BF) {
-                    // f16 has few exponents: every head's largest |q| is brought to [2^9, 2^10)
 #pragma unroll
                     for (int h = 0; h < NH; h++) {
-                        const unsigned m = __reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(qv[h])));
-                        if (lane == 0) s_red[warp][h] = __uint_as_float(m);
+                        const unsigned mx = __reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(qv[h])));
+                        if (lane == 0) s_red[warp][h] = __uint_as_float(mx);
                     }
-                    wg_sync();
+                    wg_sync(1);
 #pragma unroll
                     for (int h = 0; h < NH; h++) {
-                        const float m = fmaxf(fmaxf(s_red[0][h], s_red[1][h]), fmaxf(s_red[2][h], s_red[3][h]));
-                        int e = static_cast<int>(__float_as_uint(m) >> 23) - 127 - 9;   // m in [2^(e+9), 2^(e+10))
+                        const float *r = &s_red[4][h];
+                        const float mx = fmaxf(fmaxf(r[0], r[16]), fmaxf(r[32], r[48]));
+                        int e = static_cast<int>(__float_as_uint(mx) >> 23) - 127 - 9;
                         e = max(-110, min(110, e));
-                        fh[h] = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+                        if (tg == 0) s_f[h] = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
                         qv[h] *= __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
                     }
-                    wg_sync();
-                } else {
-#pragma unroll
-                    for (int h = 0; h < NH; h++) fh[h] = 1.f;
                 }
 #pragma unroll
                 for (int h = 0; h < NH; h++) {
                     uint16_t t[TERMS];
                     split<BF>(qv[h], t);
 #pragma unroll
-                    for (int i = 0; i < TERMS; i++) *reinterpret_cast<uint16_t *>(sQ + b_off(NB, i * NH + h, tid)) = t[i];
+                    for (int i = 0; i < TERMS; i++) *reinterpret_cast<uint16_t *>(sQ + b_off(NB, i * NH + h, tg)) = t[i];
                 }
                 fence_async();
                 mbar_arrive(&bars.qfull);
+                if (portion > 0) read_sync();   // the first warpgroup has read what lies in this one's P
             }
-            float m[NH], l[NH];
+            if constexpr (!BF) {
+                wait(&bars.qfull, static_cast<uint32_t>(portion & 1));   // s_f
+                __syncwarp();
+            }
+            portion++;
+            float fh[NH], m[NH], l[NH];
 #pragma unroll
             for (int h = 0; h < NH; h++) {
-                m[h] = -INFINITY;
+                fh[h] = BF ? 1.f : s_f[h];
+                m[h] = kNone;
                 l[h] = 0.f;
             }
-            const int ntp = wk.t1 - wk.t0;
-            int row = (s.tile0 + wk.t0) * kTile + tid;
-            auto page_ok = [&](int r) {
+            const int ntp = wk.t1 - wk.t0, t_first = (q ^ wg) & 1;   // this warpgroup's tiles: t_first, t_first + 2, ...
+            int row = (s.tile0 + wk.t0 + t_first) * kTile + tg;
+            auto seen = [&](int r) {
                 return r >= s.first && r < s.n &&
                        static_cast<unsigned>(__ldg(table + (r >> kv.page_shift))) < static_cast<unsigned>(kv.n_pages);
             };
-            bool on = page_ok(row);
-            for (int t = 0; t < ntp; t++, q++, row += kTile) {
-                const bool on_next = t + 1 < ntp && page_ok(row + kTile);
-                wait(&bars.sfull[q & 1], static_cast<uint32_t>((q >> 1) & 1));
+            bool on = t_first < ntp && seen(row);
+            for (int t = t_first; t < ntp; t += 2, row += 2 * kTile) {
+                const int qt = q + t;
+                const uint32_t par = static_cast<uint32_t>((qt >> 1) & 1);
+                const bool on_next = t + 2 < ntp && seen(row + 2 * kTile);
+                wait(&bars.sfull[wg], par);
                 __syncwarp();
                 fence_after();
-                float sv[NB];
-                ld_cols<NB>(tmem + (q & 1) * kColS + lane_base, sv);
                 float x[NH];
                 bool up = false;
 #pragma unroll
-                for (int h = 0; h < NH; h++) {
-                    float y = sv[h] + sv[NH + h];
-                    if constexpr (TERMS == 3) y = sv[h] + (sv[NH + h] + sv[2 * NH + h]);
-                    x[h] = on ? y * fh[h] : -INFINITY;
-                    up |= x[h] > m[h] + kSlack;
+                for (int hb = 0; hb < NH; hb += 8) {   // by eight heads: fewer registers at once
+                    float sv[TERMS * 8];
+#pragma unroll
+                    for (int i = 0; i < TERMS; i++) ld8(colS + i * NH + hb, sv + 8 * i);
+                    ld_done(sv);
+#pragma unroll
+                    for (int h = 0; h < 8; h++) {
+                        const float y = TERMS == 3 ? sv[h] + (sv[8 + h] + sv[(TERMS - 1) * 8 + h]) : sv[h] + sv[8 + h];
+                        x[hb + h] = on ? (BF ? y : y * fh[hb + h]) : -INFINITY;
+                        up |= x[hb + h] > m[hb + h] + kSlack;
+                    }
                 }
                 if (a.acc_out && on) {
                     float *sc = a.scores + ((static_cast<long long>(wk.b) * kv.n_kv + j) * max_rows + row) * a.gqa + g0;
@@ -484,7 +522,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             if (h < ng) sc[h] = x[h];
                     }
                 }
-                if (wg_any(up)) {
+                if (wg_any(wg, up)) {
                     // new maxima over the tile's rows; what was summed against the old ones is rescaled
 #pragma unroll
                     for (int h = 0; h < NH; h++) {
@@ -493,48 +531,55 @@ __global__ void __launch_bounds__(kThreads, 1)
                         for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
                         if (lane == 0) s_red[warp][h] = v;
                     }
-                    wg_sync();
-                    float f[NH];
+                    wg_sync(wg);
+                    if (t > 1) wait(&bars.odone[wg], par ^ 1u);
+                    __syncwarp();
+                    fence_after();
 #pragma unroll
-                    for (int h = 0; h < NH; h++) {
-                        const float v = fmaxf(m[h], fmaxf(fmaxf(s_red[0][h], s_red[1][h]), fmaxf(s_red[2][h], s_red[3][h])));
-                        f[h] = m[h] > -INFINITY ? ex2(m[h] - v) : 0.f;
-                        l[h] *= f[h];
-                        m[h] = v;
+                    for (int hb = 0; hb < NH; hb += 8) {
+                        float f[8];
+#pragma unroll
+                        for (int h = 0; h < 8; h++) {
+                            const float *r = &s_red[4 * wg][hb + h];
+                            const float v = fmaxf(m[hb + h], fmaxf(fmaxf(r[0], r[16]), fmaxf(r[32], r[48])));
+                            f[h] = ex2(m[hb + h] - v);
+                            l[hb + h] *= f[h];
+                            m[hb + h] = v;
+                        }
+                        if (t > 1) {
+                            float ov[TERMS * 8];
+#pragma unroll
+                            for (int i = 0; i < TERMS; i++) ld8(colO + i * NH + hb, ov + 8 * i);
+                            ld_done(ov);
+#pragma unroll
+                            for (int h = 0; h < 8; h++)
+#pragma unroll
+                                for (int i = 0; i < TERMS; i++) ov[8 * i + h] *= f[h];
+#pragma unroll
+                            for (int i = 0; i < TERMS; i++) st8(colO + i * NH + hb, ov + 8 * i);
+                        }
                     }
-                    wg_sync();   // s_red is free again
-                    if (t > 0) {
-                        wait(&bars.odone, static_cast<uint32_t>((q - 1) & 1));
-                        __syncwarp();
-                        fence_after();
-                        float ov[NB];
-                        ld_cols<NB>(tmem + kColO + lane_base, ov);
-#pragma unroll
-                        for (int h = 0; h < NH; h++)
-#pragma unroll
-                            for (int i = 0; i < TERMS; i++) ov[i * NH + h] *= f[h];
-#pragma unroll
-                        for (int c = 0; c < NB; c += 8) st8(tmem + kColO + lane_base + c, ov + c);
-                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                    }
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    wg_sync(wg);   // s_red is free again
                 }
-                if (t > 0) wait(&bars.odone, static_cast<uint32_t>((q - 1) & 1));   // P is free
+                if (t > 1) wait(&bars.odone[wg], par ^ 1u);   // P is free
                 __syncwarp();
 #pragma unroll
                 for (int h = 0; h < NH; h++) {
-                    const float p = on ? ex2(x[h] - (m[h] > -INFINITY ? m[h] : 0.f)) : 0.f;
+                    const float p = on ? ex2(x[h] - m[h]) : 0.f;
                     l[h] += p;
                     uint16_t tt[TERMS];
+                    // f16: p up to 2^8 is carried as p * 2^7, so that the second term of a small p keeps its bits
                     split<BF>(BF ? p : p * 128.f, tt);
 #pragma unroll
-                    for (int i = 0; i < TERMS; i++) *reinterpret_cast<uint16_t *>(sP + b_off(NB, i * NH + h, tid)) = tt[i];
+                    for (int i = 0; i < TERMS; i++) *reinterpret_cast<uint16_t *>(myP + b_off(NB, i * NH + h, tg)) = tt[i];
                 }
                 if (!on) {
                     // 0 x (whatever lies in a row that is not seen) has to be 0
-                    const int st = q % kStages;
-                    wait(&bars.vfull[st], static_cast<uint32_t>((q / kStages) & 1));
+                    const int st = qt % C::v_stages;
+                    wait(&bars.vfull[st], static_cast<uint32_t>((qt / C::v_stages) & 1));
                     const uint4 z = make_uint4(0, 0, 0, 0);
-                    uint8_t *vr = sV + st * kSlotBytes + tid * 128;
+                    uint8_t *vr = sV + st * kSlotBytes + tg * 128;
 #pragma unroll
                     for (int c = 0; c < 8; c++) {
                         *reinterpret_cast<uint4 *>(vr + 16 * c) = z;
@@ -544,124 +589,147 @@ __global__ void __launch_bounds__(kThreads, 1)
                 __syncwarp();
                 fence_async();
                 fence_before();
-                mbar_arrive(&bars.pfull);
+                mbar_arrive(&bars.pfull[wg]);
                 on = on_next;
             }
-            wait(&bars.odone, static_cast<uint32_t>((q - 1) & 1));
+            // ---------------- the portion's end: thread = element of head_dim
+            const bool any = t_first < ntp;
+            if (any) wait(&bars.odone[wg], static_cast<uint32_t>(((q + ((ntp - 1 - t_first) & ~1) + t_first) >> 1) & 1));
             __syncwarp();
             fence_after();
-            // ---------------- the portion's end: thread = element of head_dim
-            float ov[NB], o[NH];
-            ld_cols<NB>(tmem + kColO + lane_base, ov);
+            q += ntp;
+            float o[NH];
+#pragma unroll
+            for (int hb = 0; hb < NH; hb += 8) {
+                float ov[TERMS * 8];
+                if (any) {
+#pragma unroll
+                    for (int i = 0; i < TERMS; i++) ld8(colO + i * NH + hb, ov + 8 * i);
+                    ld_done(ov);
+                }
+#pragma unroll
+                for (int h = 0; h < 8; h++) {
+                    const float y = TERMS == 3 ? ov[h] + (ov[8 + h] + ov[(TERMS - 1) * 8 + h]) : ov[h] + ov[8 + h];
+                    o[hb + h] = any ? (BF ? y : y * 0x1p-7f) : 0.f;
+                }
+            }
+            fence_before();
 #pragma unroll
             for (int h = 0; h < NH; h++) {
-                o[h] = TERMS == 3 ? ov[h] + (ov[NH + h] + ov[(TERMS - 1) * NH + h]) : ov[h] + ov[NH + h];
-                if constexpr (!BF) o[h] *= 0x1p-7f;
                 float v = l[h];
 #pragma unroll
                 for (int k = 16; k; k >>= 1) v += __shfl_xor_sync(0xffffffffu, v, k);
-                if (lane == 0) s_red[warp][h] = v;
+                if (lane == 0) s_l[warp][h] = v;
             }
-            fence_before();
-            wg_sync();
+            // the second warpgroup's share goes through its P
+            float *ex = reinterpret_cast<float *>(sP + C::p_alloc);
+            if (wg == 1) {
+#pragma unroll
+                for (int h = 0; h < NH; h++) {
+                    ex[h * 128 + tg] = o[h];
+                    if (tg == h) s_ml[1][h] = m[h];
+                }
+            }
+            both_sync();
+            if (wg == 1) continue;
             float L[NH];
 #pragma unroll
-            for (int h = 0; h < NH; h++) L[h] = (s_red[0][h] + s_red[1][h]) + (s_red[2][h] + s_red[3][h]);
-            // whole segment: out; else a part of it
-            const long long seg_at = wk.at - wk.t1;              // the segment's first tile in the list
-            const long long own0 = ((seg_at + 1) * G - 1) / T, own1 = ((seg_at + wk.nt) * G - 1) / T;
-            if (own0 == own1) {
+            for (int h = 0; h < NH; h++) {
+                const float *r = &s_l[0][h];
+                const float L0 = (r[0] + r[16]) + (r[32] + r[48]), L1 = (r[64] + r[80]) + (r[96] + r[112]);
+                const float m1 = s_ml[1][h], M = fmaxf(m[h], m1), f0 = ex2(m[h] - M), f1 = ex2(m1 - M);
+                o[h] = o[h] * f0 + ex[h * 128 + tg] * f1;
+                L[h] = L0 * f0 + L1 * f1;
+                m[h] = M;
+            }
+            read_arrive();
+            auto write_out = [&](const float (&ov)[NH], const float (&mv)[NH], const float (&lv)[NH]) {
 #pragma unroll
                 for (int h = 0; h < NH; h++)
                     if (h < ng) {
-                        if (tid < kv.hd) a.out[(h0 + h) * kv.hd + tid] = L[h] > 0.f ? o[h] / L[h] : 0.f;
-                        if (tid == h) {
-                            if (a.lse) a.lse[h0 + h] = L[h] > 0.f ? m[h] * 0.6931471805599453f + logf(L[h]) : -INFINITY;
+                        if (tg < kv.hd) a.out[(h0 + h) * kv.hd + tg] = lv[h] > 0.f ? ov[h] / lv[h] : 0.f;
+                        if (tg == h) {
+                            if (a.lse) a.lse[h0 + h] = lv[h] > 0.f ? mv[h] * 0.6931471805599453f + logf(lv[h]) : -INFINITY;
                             if (a.acc_out) {
-                                a.ml[2 * (h0 + h)] = m[h];
-                                a.ml[2 * (h0 + h) + 1] = L[h];
+                                a.ml[2 * (h0 + h)] = mv[h];
+                                a.ml[2 * (h0 + h) + 1] = lv[h];
                             }
                         }
                     }
-                wg_sync();   // s_red
+            };
+            if (wk.t0 == 0 && wk.t1 == wk.nt) {   // the whole segment
+                write_out(o, m, L);
                 continue;
             }
+            // a part of it: the CTAs that own its first and last tiles (CTA i's tiles begin at floor(i T / G))
+            const long long seg_at = wk.at - wk.t1;
+            auto owner = [&](long long x) {
+                const long long n = (x + 1) * G - 1;
+                return T * G < (1ll << 31) ? static_cast<int>(static_cast<unsigned>(n) / static_cast<unsigned>(T))
+                                       : static_cast<int>(n / T);
+            };
+            const int own0 = wk.t0 == 0 ? static_cast<int>(blockIdx.x) : owner(seg_at);
+            const int own1 = wk.t1 == wk.nt ? static_cast<int>(blockIdx.x) : owner(seg_at + wk.nt - 1);
             const int slot = 2 * static_cast<int>(blockIdx.x) + (wk.t0 == 0 ? 1 : 0);
             float *part = a.part + static_cast<long long>(slot) * kAttendPart;
 #pragma unroll
             for (int h = 0; h < NH; h++) {
-                part[h * 128 + tid] = o[h];
-                if (tid == h) {
+                part[h * 128 + tg] = o[h];
+                if (tg == h) {
                     part[NH * 128 + h] = m[h];
                     part[NH * 128 + NH + h] = L[h];
                 }
             }
-            wg_sync();
-            if (tid == 0) {
-                __threadfence();
-                unsigned *cnt = a.cnt + static_cast<long long>(wk.b) * segs + wk.seg;
-                s_last = atomicAdd(cnt, 1u) == static_cast<unsigned>(own1 - own0);
+            wg_sync(0);
+            if (tg == 0) {
+                unsigned *cnt = a.cnt + static_cast<long long>(wk.b) * segs + wk.seg, old;
+                // ordered after the warpgroup's stores (the barrier above) and before the loads below
+                asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(old) : "l"(cnt) : "memory");
+                s_last = old == static_cast<unsigned>(own1 - own0);
                 if (s_last) *cnt = 0;   // for the next call
-                __threadfence();
             }
-            wg_sync();
-            if (s_last) {
-                // part i is of CTA own0 + i: slot 2 own0 + 1, then 2 (own0 + i)
-                const int np = static_cast<int>(own1 - own0) + 1;
-                auto part_of = [&](int i) {
-                    return a.part + (2 * (own0 + i) + (i == 0 ? 1 : 0)) * kAttendPart;
-                };
-                float *wgt = reinterpret_cast<float *>(sQ);   // [np][NH]: Q and P are not in use
-                for (int i = tid; i < np * NH; i += 128) wgt[i] = __ldcg(part_of(i / NH) + NH * 128 + i % NH);
-                wg_sync();
-                float M[NH];
+            wg_sync(0);
+            if (!s_last) continue;
+            // part i is of CTA own0 + i: slot 2 own0 + 1, then 2 (own0 + i)
+            const int np = own1 - own0 + 1;
+            const float *parts = a.part + 2ll * own0 * kAttendPart;
+            auto part_of = [&](int i) { return parts + (i == 0 ? 1 : 2 * i) * kAttendPart; };
+            float *wgt = reinterpret_cast<float *>(sP);   // [np][NH]: this warpgroup's P is not in use
+            for (int i = tg; i < np * NH; i += 128) wgt[i] = __ldcg(part_of(i / NH) + NH * 128 + i % NH);
+            wg_sync(0);
 #pragma unroll
-                for (int h = 0; h < NH; h++) M[h] = -INFINITY;
-                for (int i = 0; i < np; i++)
+            for (int h = 0; h < NH; h++) m[h] = kNone;
+            for (int i = 0; i < np; i++)
 #pragma unroll
-                    for (int h = 0; h < NH; h++) M[h] = fmaxf(M[h], wgt[i * NH + h]);
-                wg_sync();
-                if (tid < NH) {
+                for (int h = 0; h < NH; h++) m[h] = fmaxf(m[h], wgt[i * NH + h]);
 #pragma unroll
-                    for (int h = 0; h < NH; h++)
-                        if (tid == h) s_f[h] = M[h];
-                }
-                wg_sync();
-                for (int i = tid; i < np * NH; i += 128) {
-                    const float mi = wgt[i], MM = s_f[i % NH];
-                    wgt[i] = mi > -INFINITY ? ex2(mi - MM) : 0.f;
-                }
-                wg_sync();
-                float acc[NH], Ls[NH];
+            for (int h = 0; h < NH; h++) {
+                o[h] = 0.f;
+                L[h] = 0.f;
+            }
+            constexpr int AT = 32 / NH;   // parts at once: 32 loads in flight
+            for (int i0 = 0; i0 < np; i0 += AT) {
+                float v[AT][NH], lv[AT][NH];
 #pragma unroll
-                for (int h = 0; h < NH; h++) {
-                    acc[h] = 0.f;
-                    Ls[h] = 0.f;
-                }
-#pragma unroll 4
-                for (int i = 0; i < np; i++) {
-                    const float *pp = part_of(i);
+                for (int i = 0; i < AT; i++) {
+                    const float *pp = part_of(min(i0 + i, np - 1));
 #pragma unroll
                     for (int h = 0; h < NH; h++) {
-                        const float f = wgt[i * NH + h];
-                        acc[h] += f * __ldcg(pp + h * 128 + tid);
-                        Ls[h] += f * __ldcg(pp + NH * 128 + NH + h);
+                        v[i][h] = __ldcg(pp + h * 128 + tg);
+                        lv[i][h] = __ldcg(pp + NH * 128 + NH + h);
                     }
                 }
 #pragma unroll
-                for (int h = 0; h < NH; h++)
-                    if (h < ng) {
-                        if (tid < kv.hd) a.out[(h0 + h) * kv.hd + tid] = Ls[h] > 0.f ? acc[h] / Ls[h] : 0.f;
-                        if (tid == h) {
-                            if (a.lse) a.lse[h0 + h] = Ls[h] > 0.f ? M[h] * 0.6931471805599453f + logf(Ls[h]) : -INFINITY;
-                            if (a.acc_out) {
-                                a.ml[2 * (h0 + h)] = M[h];
-                                a.ml[2 * (h0 + h) + 1] = Ls[h];
-                            }
+                for (int i = 0; i < AT; i++)
+                    if (i0 + i < np)
+#pragma unroll
+                        for (int h = 0; h < NH; h++) {
+                            const float f = ex2(wgt[(i0 + i) * NH + h] - m[h]);
+                            o[h] += f * v[i][h];
+                            L[h] += f * lv[i][h];
                         }
-                    }
-                wg_sync();   // the weights' place is Q's again
             }
+            write_out(o, m, L);
         }
     }
     __syncthreads();
@@ -672,7 +740,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <bool BF, int NH>
 cudaError_t launch(const PagedAttendArgs &a, const CUtensorMap &mk, const CUtensorMap &mv, int grid, cudaStream_t st) {
     constexpr int smem = Cfg<BF, NH>::smem;
-    static_assert(smem <= 227 * 1024 - 8 * 1024, "shared memory");
+    static_assert(smem <= 227 * 1024 - 6 * 1024, "shared memory");
     const cudaError_t e = cudaFuncSetAttribute(k_attend_tc<BF, NH>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     return launch_pdl(k_attend_tc<BF, NH>, dim3(grid), dim3(kThreads), smem, st, a, mk, mv);
