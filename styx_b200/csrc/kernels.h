@@ -396,7 +396,7 @@ struct PagedAttendArgs {
     // rows][gqa]; maximum and sum of every head, [n_seqs][n_heads][2]
     float *scores, *ml;
     float *part;                   // workspace: the portions' partial results, kAttendPart floats each
-    unsigned *cnt;                 // workspace: finished portions per (sequence, kv head, group), zero between calls
+    unsigned *cnt;                 // workspace, per (sequence, kv head, group): first CTA << 16 | portions (0: not cut)
 };
 // a portion of up to 16 heads of up to 128 elements: O, maxima, sums
 constexpr int kAttendPart = 16 * 128 + 32;

@@ -19,9 +19,10 @@
 // NH q heads).  All tiles of the call form one list; CTA i of G takes the
 // i-th G-th of it, so ragged lengths spread evenly over the SMs.  A portion
 // (a CTA's consecutive tiles of one segment) ends in (max, sum, O) per head:
-// written out where it is the whole segment, else to the workspace, and the
-// CTA that finishes a segment's last portion joins them in order.  Which CTA
-// that is does not change the result.
+// written out where it is the whole segment, else to the workspace, from
+// where k_attend_join, one CTA per segment, adds the portions up in order.
+// (Joining inside this kernel, by the CTA that finishes a segment last, kept
+// four of 148 SMs 12 us longer than the rest at one sequence of 131071 rows.)
 //
 // Roles, linked by mbarriers with bounded waits: two softmax warpgroups take
 // alternate tiles (thread = row of the tile), each with its own score buffer,
@@ -51,15 +52,16 @@ constexpr uint32_t kTmemCols = 256, kColS = 0, kColO = 128, kColStep = 64;   // 
 constexpr float kSlack = 8.f;              // log2 units a score may pass the maximum by
 constexpr float kNone = -3e38f;            // maximum of no scores: finite, so that differences stay numbers
 
+constexpr int kJoinParts = 152;            // CTAs, and so portions of a segment, at most (B200: 148 SMs)
+
 template <bool BF, int NH>
 struct Cfg {
     static constexpr int terms = BF ? 3 : 2;
     static constexpr int nb = (terms * NH + 15) / 16 * 16;   // N of the products (M 128: multiples of 16)
     static constexpr int q_bytes = 2 * nb * 128, p_bytes = 2 * nb * 128;
-    // a P buffer also holds the join's weights: NH for each of up to 152 portions
-    static constexpr int p_alloc = (p_bytes > 152 * NH * 4 ? p_bytes : 152 * NH * 4) + 1023 & ~1023;
-    static constexpr int k_stages = 3, v_stages = nb <= 32 ? 3 : 2;   // what 227 KB hold
-    static constexpr int smem = (k_stages + v_stages) * kSlotBytes + q_bytes + 2 * p_alloc + 1024;
+    static constexpr int k_stages = 3, v_stages = NH == 8 ? 3 : 2;   // what 227 KB hold
+    static constexpr int qn_bytes = NH * 128 * 4;                    // the next portion's q
+    static constexpr int smem = (k_stages + v_stages) * kSlotBytes + q_bytes + 2 * p_bytes + qn_bytes + 1024;
     // term of a small p keeps its bits; bf16 has f32's range
 };
 
@@ -138,6 +140,11 @@ __device__ __forceinline__ bool wg_any(int wg, bool v) {
         : "memory");
     return r != 0;
 }
+__device__ __forceinline__ float warp_max(float v) {   // NaN only where every lane has it
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -215,13 +222,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     extern __shared__ uint8_t smem_raw[];
     uint8_t *sm = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
     uint8_t *sK = sm, *sV = sm + C::k_stages * kSlotBytes, *sQ = sV + C::v_stages * kSlotBytes, *sP = sQ + C::q_bytes;
+    float *sQn = reinterpret_cast<float *>(sP + 2 * C::p_bytes);
     __shared__ Bars bars;
     __shared__ uint32_t s_tmem;
-    __shared__ int s_abort, s_b0, s_last;
+    __shared__ int s_abort, s_b0;
     __shared__ long long s_off, s_scan[kThreads];
     __shared__ float s_red[8][16], s_l[8][16], s_ml[2][16], s_f[16];
     const PagedKv &kv = a.kv;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const int groups = (a.gqa + NH - 1) / NH, segs = kv.n_kv * groups;
 
     pdl_trigger();
@@ -327,35 +335,43 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int rb_shift = min(kv.page_shift, 7), rows = 1 << rb_shift, halves = kv.hd > 64 ? 2 : 1;
         const int boxes = (kTile >> rb_shift) * halves;   // <= 16
         const int pi = lane / halves, half = lane - pi * halves;
-        int q = 0;
-        bool live = true;
-        while (live && wk.next(a, segs)) {
+        // a tile's box of this lane: its first row, where that lies in the page, the page's id (loaded one tile ahead)
+        struct Box {
+            bool on;
+            int page, y;
+        };
+        bool more = wk.next(a, segs);
+        int t = wk.t0;
+        auto fetch = [&]() {
+            Box x{false, 0, 0};
+            if (!more) return x;
             const Seq s(a, wk.b, false);
-            const int j = wk.seg / groups;
-            const int32_t *table = kv.table + static_cast<long long>(wk.b) * kv.table_stride;
-            for (int t = wk.t0; t < wk.t1; t++, q++) {
-                const int st = q % stages, use = q / stages;
-                const int r0 = (s.tile0 + t) * kTile + (pi << rb_shift);
-                bool on = lane < boxes && r0 < s.n && r0 + rows > s.first;
-                int page = 0;
-                if (on) {
-                    page = __ldg(table + (r0 >> kv.page_shift));
-                    if (static_cast<unsigned>(page) >= static_cast<unsigned>(kv.n_pages)) {
-                        if (!isv) atomicExch(kv.err, kErrBadPos);
-                        on = false;
-                    }
-                }
-                const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, on)) * static_cast<uint32_t>(rows) * 128u;
-                if (use > 0 && !__all_sync(0xffffffffu, wait(&empty[st], static_cast<uint32_t>((use - 1) & 1)))) {
-                    live = false;
-                    break;
-                }
-                if (lane == 0) mbar_arrive_expect_tx(&full[st], bytes);
-                __syncwarp();
-                if (on)
-                    tma3(ring + st * kSlotBytes + half * kHalfBytes + (pi << rb_shift) * 128, map, half * 64,
-                         (j << kv.page_shift) + (r0 & ((1 << kv.page_shift) - 1)), page, &full[st]);
+            const int r0 = (s.tile0 + t) * kTile + (pi << rb_shift);
+            x.on = lane < boxes && r0 < s.n && r0 + rows > s.first;
+            if (x.on) x.page = __ldg(kv.table + static_cast<long long>(wk.b) * kv.table_stride + (r0 >> kv.page_shift));
+            x.y = ((wk.seg / groups) << kv.page_shift) + (r0 & ((1 << kv.page_shift) - 1));
+            return x;
+        };
+        Box nxt = fetch();
+        int q = 0;
+        for (; more; q++) {
+            Box x = nxt;
+            if (++t == wk.t1) {
+                more = wk.next(a, segs);
+                t = wk.t0;
             }
+            nxt = fetch();
+            const int st = q % stages, use = q / stages;
+            if (use > 0 && !__all_sync(0xffffffffu, wait(&empty[st], static_cast<uint32_t>((use - 1) & 1)))) break;
+            if (x.on && static_cast<unsigned>(x.page) >= static_cast<unsigned>(kv.n_pages)) {
+                if (!isv) atomicExch(kv.err, kErrBadPos);
+                x.on = false;
+            }
+            const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, x.on)) * static_cast<uint32_t>(rows) * 128u;
+            if (lane == 0) mbar_arrive_expect_tx(&full[st], bytes);
+            __syncwarp();
+            if (x.on)
+                tma3(ring + st * kSlotBytes + half * kHalfBytes + (pi << rb_shift) * 128, map, half * 64, x.y, x.page, &full[st]);
         }
         // nothing of this warp's is still landing when the CTA ends
         for (int i = max(0, q - stages); i < q; i++)
@@ -400,7 +416,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 fence_after();
                 if (leader) {
                     const uint32_t dv = dV + static_cast<uint32_t>(st) * (kSlotBytes / 16), d = tmem + kColO + wg * kColStep;
-                    const uint32_t dp = dP + static_cast<uint32_t>(wg) * (C::p_alloc / 16);
+                    const uint32_t dp = dP + static_cast<uint32_t>(wg) * (C::p_bytes / 16);
 #pragma unroll
                     for (int k = 0; k < kTile / 16; k++)
                         mma(d, dv + k * (2048 / 16), dp + (k >> 2) * (NB * 128 / 16) + (k & 3) * 2, id_o, t > 1 || k > 0);
@@ -426,10 +442,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int wg = warp >> 2, tg = tid & 127;
         const uint32_t lane_base = static_cast<uint32_t>(32 * (warp & 3)) << 16;
         const uint32_t colS = tmem + kColS + wg * kColStep + lane_base, colO = tmem + kColO + wg * kColStep + lane_base;
-        uint8_t *myP = sP + wg * C::p_alloc;
+        uint8_t *myP = sP + wg * C::p_bytes;
         const float l2 = a.scale * 1.4426950408889634f;   // scores in units of log2
         const long long max_rows = static_cast<long long>(kv.max_pages) << kv.page_shift;
         int q = 0, portion = 0;                            // the portion's first tile (global number), its number
+        // q of a portion into shared memory: every thread the elements that it will read itself
+        auto stage_q = [&](const Walk &w) {
+            const int j = w.seg / groups, g0 = (w.seg - j * groups) * NH;
+            const float *qp = a.q + (static_cast<long long>(w.b) * a.n_heads + j * a.gqa + g0) * kv.hd + tg;
+#pragma unroll
+            for (int h = 0; h < NH; h++)
+                if (h < a.gqa - g0 && tg < kv.hd)
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_addr(sQn + h * 128 + tg)),
+                                 "l"(qp + h * kv.hd)
+                                 : "memory");
+        };
         while (wk.next(a, segs)) {
             const Seq s(a, wk.b, false);
             const int j = wk.seg / groups, g0 = (wk.seg - j * groups) * NH, ng = min(NH, a.gqa - g0);
@@ -440,8 +467,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // one's result.  Thread = element.  f16 has few exponents: every head's largest |q| is brought to
                 // [2^9, 2^10), and s_f says what a column of S is in units of its terms.
                 float qv[NH];
+                if (portion == 0) stage_q(wk);
+                asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll
-                for (int h = 0; h < NH; h++) qv[h] = h < ng && tg < kv.hd ? __ldg(a.q + (h0 + h) * kv.hd + tg) * l2 : 0.f;
+                for (int h = 0; h < NH; h++) qv[h] = h < ng && tg < kv.hd ? sQn[h * 128 + tg] * l2 : 0.f;
+                Walk ahead = wk;   // the next portion's q is on its way while this one runs
+                if (ahead.next(a, segs)) stage_q(ahead);
                 if constexpr (!BF) {
 #pragma unroll
                     for (int h = 0; h < NH; h++) {
@@ -484,15 +515,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             const int ntp = wk.t1 - wk.t0, t_first = (q ^ wg) & 1;   // this warpgroup's tiles: t_first, t_first + 2, ...
             int row = (s.tile0 + wk.t0 + t_first) * kTile + tg;
-            auto seen = [&](int r) {
-                return r >= s.first && r < s.n &&
-                       static_cast<unsigned>(__ldg(table + (r >> kv.page_shift))) < static_cast<unsigned>(kv.n_pages);
-            };
-            bool on = t_first < ntp && seen(row);
+            auto page_of = [&](int r) { return r >= s.first && r < s.n ? __ldg(table + (r >> kv.page_shift)) : -1; };
+            int page = t_first < ntp ? page_of(row) : -1;
             for (int t = t_first; t < ntp; t += 2, row += 2 * kTile) {
                 const int qt = q + t;
                 const uint32_t par = static_cast<uint32_t>((qt >> 1) & 1);
-                const bool on_next = t + 2 < ntp && seen(row + 2 * kTile);
+                const bool on = static_cast<unsigned>(page) < static_cast<unsigned>(kv.n_pages);
+                page = t + 2 < ntp ? page_of(row + 2 * kTile) : -1;   // loaded one tile ahead
                 wait(&bars.sfull[wg], par);
                 __syncwarp();
                 fence_after();
@@ -526,9 +555,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     // new maxima over the tile's rows; what was summed against the old ones is rescaled
 #pragma unroll
                     for (int h = 0; h < NH; h++) {
-                        float v = x[h];
-#pragma unroll
-                        for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+                        const float v = warp_max(x[h]);
                         if (lane == 0) s_red[warp][h] = v;
                     }
                     wg_sync(wg);
@@ -590,7 +617,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                 fence_async();
                 fence_before();
                 mbar_arrive(&bars.pfull[wg]);
-                on = on_next;
             }
             // ---------------- the portion's end: thread = element of head_dim
             const bool any = t_first < ntp;
@@ -622,7 +648,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (lane == 0) s_l[warp][h] = v;
             }
             // the second warpgroup's share goes through its P
-            float *ex = reinterpret_cast<float *>(sP + C::p_alloc);
+            float *ex = reinterpret_cast<float *>(sP + C::p_bytes);
             if (wg == 1) {
 #pragma unroll
                 for (int h = 0; h < NH; h++) {
@@ -659,19 +685,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             };
             if (wk.t0 == 0 && wk.t1 == wk.nt) {   // the whole segment
                 write_out(o, m, L);
+                if (tg == 0) a.cnt[static_cast<long long>(wk.b) * segs + wk.seg] = 0;
                 continue;
             }
-            // a part of it: the CTAs that own its first and last tiles (CTA i's tiles begin at floor(i T / G))
-            const long long seg_at = wk.at - wk.t1;
-            auto owner = [&](long long x) {
-                const long long n = (x + 1) * G - 1;
-                return T * G < (1ll << 31) ? static_cast<int>(static_cast<unsigned>(n) / static_cast<unsigned>(T))
-                                       : static_cast<int>(n / T);
-            };
-            const int own0 = wk.t0 == 0 ? static_cast<int>(blockIdx.x) : owner(seg_at);
-            const int own1 = wk.t1 == wk.nt ? static_cast<int>(blockIdx.x) : owner(seg_at + wk.nt - 1);
-            const int slot = 2 * static_cast<int>(blockIdx.x) + (wk.t0 == 0 ? 1 : 0);
-            float *part = a.part + static_cast<long long>(slot) * kAttendPart;
+            if (wk.t1 == wk.nt && tg == 0) {
+                // for the join: the segment's first owner (CTA i's tiles begin at floor(i T / G)) and its portions
+                const long long n = (wk.at - wk.nt + 1) * G - 1;
+                const int own0 = static_cast<int>(T * G < (1ll << 31) ? static_cast<unsigned>(n) / static_cast<unsigned>(T) : n / T);
+                a.cnt[static_cast<long long>(wk.b) * segs + wk.seg] = static_cast<unsigned>(own0) << 16 | (blockIdx.x - own0 + 1);
+            }
+            // a part of it: CTA i's portion that begins its segment goes to slot 2 i + 1, any other to slot 2 i
+            float *part = a.part + (2ll * blockIdx.x + (wk.t0 == 0 ? 1 : 0)) * kAttendPart;
 #pragma unroll
             for (int h = 0; h < NH; h++) {
                 part[h * 128 + tg] = o[h];
@@ -680,56 +704,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                     part[NH * 128 + NH + h] = L[h];
                 }
             }
-            wg_sync(0);
-            if (tg == 0) {
-                unsigned *cnt = a.cnt + static_cast<long long>(wk.b) * segs + wk.seg, old;
-                // ordered after the warpgroup's stores (the barrier above) and before the loads below
-                asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(old) : "l"(cnt) : "memory");
-                s_last = old == static_cast<unsigned>(own1 - own0);
-                if (s_last) *cnt = 0;   // for the next call
-            }
-            wg_sync(0);
-            if (!s_last) continue;
-            // part i is of CTA own0 + i: slot 2 own0 + 1, then 2 (own0 + i)
-            const int np = own1 - own0 + 1;
-            const float *parts = a.part + 2ll * own0 * kAttendPart;
-            auto part_of = [&](int i) { return parts + (i == 0 ? 1 : 2 * i) * kAttendPart; };
-            float *wgt = reinterpret_cast<float *>(sP);   // [np][NH]: this warpgroup's P is not in use
-            for (int i = tg; i < np * NH; i += 128) wgt[i] = __ldcg(part_of(i / NH) + NH * 128 + i % NH);
-            wg_sync(0);
-#pragma unroll
-            for (int h = 0; h < NH; h++) m[h] = kNone;
-            for (int i = 0; i < np; i++)
-#pragma unroll
-                for (int h = 0; h < NH; h++) m[h] = fmaxf(m[h], wgt[i * NH + h]);
-#pragma unroll
-            for (int h = 0; h < NH; h++) {
-                o[h] = 0.f;
-                L[h] = 0.f;
-            }
-            constexpr int AT = 32 / NH;   // parts at once: 32 loads in flight
-            for (int i0 = 0; i0 < np; i0 += AT) {
-                float v[AT][NH], lv[AT][NH];
-#pragma unroll
-                for (int i = 0; i < AT; i++) {
-                    const float *pp = part_of(min(i0 + i, np - 1));
-#pragma unroll
-                    for (int h = 0; h < NH; h++) {
-                        v[i][h] = __ldcg(pp + h * 128 + tg);
-                        lv[i][h] = __ldcg(pp + NH * 128 + NH + h);
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < AT; i++)
-                    if (i0 + i < np)
-#pragma unroll
-                        for (int h = 0; h < NH; h++) {
-                            const float f = ex2(wgt[(i0 + i) * NH + h] - m[h]);
-                            o[h] += f * v[i][h];
-                            L[h] += f * lv[i][h];
-                        }
-            }
-            write_out(o, m, L);
         }
     }
     __syncthreads();
@@ -737,13 +711,79 @@ __global__ void __launch_bounds__(kThreads, 1)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
 }
 
+// CTA = one segment that was cut: its portions, in order.  Warp w takes heads
+// w, w + 8, ..., lane l elements 4 l ..; eight portions' loads in flight.
+template <int NH>
+__global__ void __launch_bounds__(256) k_attend_join(PagedAttendArgs a) {
+    pdl_trigger();
+    __shared__ float sm_m[kJoinParts][NH], sm_l[kJoinParts][NH];
+    const PagedKv &kv = a.kv;
+    const int groups = (a.gqa + NH - 1) / NH, segs = kv.n_kv * groups;
+    const int b = blockIdx.x / segs, seg = blockIdx.x - b * segs, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int j = seg / groups, g0 = (seg - j * groups) * NH, ng = min(NH, a.gqa - g0);
+    pdl_wait();
+    const unsigned c = __ldcg(a.cnt + blockIdx.x);
+    const int np = static_cast<int>(c & 0xFFFFu);
+    if (np == 0) return;
+    const float *parts = a.part + 2ll * (c >> 16) * kAttendPart;
+    auto part_of = [&](int i) { return parts + (i == 0 ? 1 : 2 * i) * kAttendPart; };
+    for (int i = threadIdx.x; i < np * NH; i += 256) {
+        const float *pp = part_of(i / NH) + NH * 128 + i % NH;
+        sm_m[i / NH][i % NH] = __ldcg(pp);
+        sm_l[i / NH][i % NH] = __ldcg(pp + NH);
+    }
+    __syncthreads();
+    for (int h = warp; h < ng; h += 8) {
+        float4 v[8];
+        auto load = [&](int i0) {
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                v[i] = __ldcg(reinterpret_cast<const float4 *>(part_of(min(i0 + i, np - 1)) + h * 128) + lane);
+        };
+        load(0);
+        float M = kNone, L = 0.f;
+        for (int i = lane; i < np; i += 32) M = fmaxf(M, sm_m[i][h]);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i0 = 0; i0 < np; i0 += 8) {
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (i0 + i < np) {
+                    const float f = ex2(sm_m[i0 + i][h] - M);
+                    L += f * sm_l[i0 + i][h];
+                    o.x += f * v[i].x;
+                    o.y += f * v[i].y;
+                    o.z += f * v[i].z;
+                    o.w += f * v[i].w;
+                }
+            if (i0 + 8 < np) load(i0 + 8);
+        }
+        const long long at = static_cast<long long>(b) * a.n_heads + j * a.gqa + g0 + h;
+        const float r = L > 0.f ? 1.f / L : 0.f;
+        if (4 * lane < kv.hd)
+            *reinterpret_cast<float4 *>(a.out + at * kv.hd + 4 * lane) = make_float4(o.x * r, o.y * r, o.z * r, o.w * r);
+        if (lane == 0) {
+            if (a.lse) a.lse[at] = L > 0.f ? M * 0.6931471805599453f + logf(L) : -INFINITY;
+            if (a.acc_out) {
+                a.ml[2 * at] = M;
+                a.ml[2 * at + 1] = L;
+            }
+        }
+    }
+}
+
 template <bool BF, int NH>
 cudaError_t launch(const PagedAttendArgs &a, const CUtensorMap &mk, const CUtensorMap &mv, int grid, cudaStream_t st) {
     constexpr int smem = Cfg<BF, NH>::smem;
     static_assert(smem <= 227 * 1024 - 6 * 1024, "shared memory");
-    const cudaError_t e = cudaFuncSetAttribute(k_attend_tc<BF, NH>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaError_t e = cudaFuncSetAttribute(k_attend_tc<BF, NH>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
-    return launch_pdl(k_attend_tc<BF, NH>, dim3(grid), dim3(kThreads), smem, st, a, mk, mv);
+    e = launch_pdl(k_attend_tc<BF, NH>, dim3(grid), dim3(kThreads), smem, st, a, mk, mv);
+    // nothing is cut where no sequence can have a second tile
+    if (e != cudaSuccess || (static_cast<long long>(a.kv.max_pages) << a.kv.page_shift) <= kTile) return e;
+    const int groups = (a.gqa + NH - 1) / NH;
+    return launch_pdl(k_attend_join<NH>, dim3(a.kv.n_seqs * a.kv.n_kv * groups), dim3(256), 0, st, a);
 }
 
 }  // namespace
@@ -754,6 +794,7 @@ cudaError_t launch_attend_tc(const PagedAttendArgs &a, const CUtensorMap &mk, co
     const long long tiles = static_cast<long long>(a.kv.n_seqs) * a.kv.n_kv * groups *
                             (((static_cast<long long>(a.kv.max_pages) << a.kv.page_shift) + kTile - 1) / kTile);
     const int grid = static_cast<int>(tiles < sms ? tiles : sms);
+    if (grid > kJoinParts) return cudaErrorInvalidConfiguration;
     if (a.kv.dtype == STYX_BF16) return nh == 8 ? launch<true, 8>(a, mk, mv, grid, st) : launch<true, 16>(a, mk, mv, grid, st);
     return nh == 8 ? launch<false, 8>(a, mk, mv, grid, st) : launch<false, 16>(a, mk, mv, grid, st);
 }

@@ -237,7 +237,7 @@ int styx_paged_attend(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv
         const uint32_t box[3] = {64, static_cast<uint32_t>(kv->page_size < 128 ? kv->page_size : 128), 1};
         CHECK(styx::encode_map3(&mk, kv->k, dims, strides, box));
         CHECK(styx::encode_map3(&mv, kv->v, dims, strides, box));
-        CK(styx::launch_attend_tc(a, mk, mv, sms, S(stream)));
+        CK(styx::launch_attend_tc(a, mk, mv, sms < 152 ? sms : 152, S(stream)));
     } else {
         CK(styx::launch_paged_attend(a, S(stream)));
     }
