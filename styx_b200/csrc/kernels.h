@@ -423,7 +423,7 @@ struct SampleArgs {
 cudaError_t launch_paged_append(const PagedAppendArgs &a, cudaStream_t st);
 cudaError_t launch_paged_attend(const PagedAttendArgs &a, cudaStream_t st);
 // the tensor-core form: mk, mv map the pools as {head_dim, n_kv * page rows,
-// pages}, box 64 x min(page, 128) rows, 128-byte swizzle
+// pages}, box 64 x min(page, 128) rows (V: 64), 128-byte swizzle
 cudaError_t launch_attend_tc(const PagedAttendArgs &a, const CUtensorMap &mk, const CUtensorMap &mv, int sms,
                              cudaStream_t st);
 cudaError_t launch_paged_acc(const PagedAttendArgs &a, cudaStream_t st);

@@ -28,9 +28,11 @@
 // alternate tiles (thread = row of the tile), each with its own score buffer,
 // maxima, sums, P and accumulator, so that one's chain scores -> exponentials
 // -> P -> product overlaps the other's; they are added up at the portion's
-// end (thread = element of head_dim).  One warp copies K, one copies V (rings
-// of 2 or 3 tiles, 160 to 192 KB: more than the bytes in flight that HBM's
-// latency needs), one thread issues the MMAs.  The maximum a row is measured
+// end (thread = element of head_dim).  One warp copies K, one copies V, one
+// issues S, one O.  K and V share one ring of 16 KB slots (half the columns
+// of a K tile, half the rows of a V tile), 11 or 12 of them, filled in the
+// order K0 K1 V0 K2 V1 K3 ... in which they are used, so the whole 176 to 192
+// KB are in flight for whichever is needed next.  The maximum a row is measured
 // against moves only when a score passes it by 2^8, so the accumulator is
 // rescaled rarely and no tile waits for an exact running maximum; sums and
 // exponentials are unaffected by which one is used.
@@ -45,9 +47,13 @@ namespace {
 
 constexpr int kTile = 128;                 // rows of a tile = M of both products
 constexpr int kHalfBytes = kTile * 128;    // 64 columns of a tile: 128-byte rows
-constexpr int kSlotBytes = 2 * kHalfBytes; // K or V of a tile
-constexpr int kThreads = 352;
-constexpr int kWarpK = 8, kWarpV = 9, kWarpMma = 10;
+constexpr int kSlotBytes = kHalfBytes;     // K: 128 rows x 64 columns; V: 2 x (64 rows x 64 columns)
+constexpr int kThreads = 384;
+constexpr int kWarpK = 8, kWarpV = 9, kWarpS = 10, kWarpO = 11;
+// what a segment's start costs a CTA (Q, the first maxima, the result), in
+// tiles: the partition counts it, so that CTAs with many short segments get
+// fewer tiles
+constexpr int kSegCost = 3;
 constexpr uint32_t kTmemCols = 256, kColS = 0, kColO = 128, kColStep = 64;   // two score buffers, two accumulators
 constexpr float kSlack = 8.f;              // log2 units a score may pass the maximum by
 constexpr float kNone = -3e38f;            // maximum of no scores: finite, so that differences stay numbers
@@ -59,9 +65,9 @@ struct Cfg {
     static constexpr int terms = BF ? 3 : 2;
     static constexpr int nb = (terms * NH + 15) / 16 * 16;   // N of the products (M 128: multiples of 16)
     static constexpr int q_bytes = 2 * nb * 128, p_bytes = 2 * nb * 128;
-    static constexpr int k_stages = 3, v_stages = NH == 8 ? 3 : 2;   // what 227 KB hold
+    static constexpr int slots = NH == 8 ? 12 : 11;                  // what 227 KB hold
     static constexpr int qn_bytes = NH * 128 * 4;                    // the next portion's q
-    static constexpr int smem = (k_stages + v_stages) * kSlotBytes + q_bytes + 2 * p_bytes + qn_bytes + 1024;
+    static constexpr int smem = slots * kSlotBytes + q_bytes + 2 * p_bytes + qn_bytes + 1024;
     // term of a small p keeps its bits; bf16 has f32's range
 };
 
@@ -175,9 +181,14 @@ __device__ __forceinline__ uint32_t b_off(int nb, int n, int c) {
 }
 
 struct Bars {
-    uint64_t kfull[3], kempty[3], vfull[3], vempty[3];
-    uint64_t sfull[2], pfull[2], odone[2], qfull, drain;
+    uint64_t full[12], empty[12];
+    uint64_t sfull[2], pfull[2], odone[2], qfull, drain[2];
 };
+
+// Position of a portion's copies in its list (K0 K1 V0 K2 V1 ... of nt tiles,
+// kh slots for a K tile, 2 for a V tile)
+__device__ __forceinline__ int pos_k(int t, int kh) { return kh * t + 2 * max(0, t - 1); }
+__device__ __forceinline__ int pos_v(int t, int nt, int kh) { return kh * min(t + 2, nt) + 2 * t; }
 
 // rows of a sequence that are seen, and its tiles (an empty one counts one
 // tile, so that somebody writes its zeros)
@@ -191,26 +202,30 @@ struct Seq {
     }
 };
 
-// the CTA's share of the tile list, portion by portion
+// the CTA's share of the list, portion by portion.  A segment is kSegCost
+// empty units, then its tiles.
 struct Walk {
-    int b, seg, t, nt;             // sequence, (kv head, group) in it, next tile of nt
-    long long at, end;             // global tile numbers
+    int b, seg, u, nt;             // sequence, (kv head, group) in it, next unit of kSegCost + nt
+    long long at, end;             // global unit numbers
     int t0, t1;                    // the portion: tiles [t0, t1) of the segment
     __device__ __forceinline__ bool next(const PagedAttendArgs &a, int segs) {
-        if (at >= end) return false;
-        if (t == nt) {
-            t = 0;
-            if (++seg == segs) {
-                seg = 0;
-                b++;
-                nt = Seq(a, b, false).nt;
+        while (at < end) {
+            if (u == kSegCost + nt) {
+                u = 0;
+                if (++seg == segs) {
+                    seg = 0;
+                    b++;
+                    nt = Seq(a, b, false).nt;
+                }
             }
+            const int u1 = static_cast<int>(min(static_cast<long long>(kSegCost + nt), u + (end - at)));
+            t0 = max(0, u - kSegCost);
+            t1 = max(0, u1 - kSegCost);
+            at += u1 - u;
+            u = u1;
+            if (t1 > t0) return true;
         }
-        t0 = t;
-        t1 = static_cast<int>(min(static_cast<long long>(nt), t + (end - at)));
-        at += t1 - t0;
-        t = t1;
-        return true;
+        return false;
     }
 };
 
@@ -221,7 +236,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int NB = C::nb, TERMS = C::terms;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *sm = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
-    uint8_t *sK = sm, *sV = sm + C::k_stages * kSlotBytes, *sQ = sV + C::v_stages * kSlotBytes, *sP = sQ + C::q_bytes;
+    uint8_t *ring = sm, *sQ = ring + C::slots * kSlotBytes, *sP = sQ + C::q_bytes;
     float *sQn = reinterpret_cast<float *>(sP + 2 * C::p_bytes);
     __shared__ Bars bars;
     __shared__ uint32_t s_tmem;
@@ -236,11 +251,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (tid == 32 * kWarpK) asm volatile("prefetch.tensormap [%0];" ::"l"(&mk));
     if (tid == 32 * kWarpV) asm volatile("prefetch.tensormap [%0];" ::"l"(&mv));
     if (tid == 0) {
-        for (int i = 0; i < 3; i++) {
-            mbar_init(&bars.kfull[i], 1);
-            mbar_init(&bars.kempty[i], 1);
-            mbar_init(&bars.vfull[i], 1);
-            mbar_init(&bars.vempty[i], 1);
+        for (int i = 0; i < C::slots; i++) {
+            mbar_init(&bars.full[i], 1);
+            mbar_init(&bars.empty[i], 1);
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(&bars.sfull[i], 1);
@@ -248,11 +261,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&bars.odone[i], 1);
         }
         mbar_init(&bars.qfull, 128);
-        mbar_init(&bars.drain, 1);
+        mbar_init(&bars.drain[0], 1);
+        mbar_init(&bars.drain[1], 1);
         fence_mbar_init();
         s_abort = 0;
     }
-    if (warp == kWarpMma) {
+    if (warp == kWarpO) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)),
                      "r"(kTmemCols));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -264,7 +278,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     {
         const int per = (kv.n_seqs + kThreads - 1) / kThreads, lo = min(kv.n_seqs, tid * per), hi = min(kv.n_seqs, lo + per);
         long long mine = 0;
-        for (int b = lo; b < hi; b++) mine += static_cast<long long>(Seq(a, b, blockIdx.x == 0).nt) * segs;
+        for (int b = lo; b < hi; b++) mine += static_cast<long long>(Seq(a, b, blockIdx.x == 0).nt + kSegCost) * segs;
         s_scan[tid] = mine;
         __syncthreads();
         if (warp == 0) {   // inclusive scan of the kThreads chunks
@@ -292,7 +306,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             long long off = at - before;
             int b = lo;
             for (; b < hi; b++) {
-                const long long nb = static_cast<long long>(Seq(a, b, false).nt) * segs;
+                const long long nb = static_cast<long long>(Seq(a, b, false).nt + kSegCost) * segs;
                 if (off < nb) break;
                 off -= nb;
             }
@@ -302,14 +316,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncthreads();
         w0.b = s_b0;
         w0.nt = Seq(a, w0.b, false).nt;
-        w0.seg = static_cast<int>(s_off / w0.nt);
-        w0.t = static_cast<int>(s_off - static_cast<long long>(w0.seg) * w0.nt);
+        w0.seg = static_cast<int>(s_off / (w0.nt + kSegCost));
+        w0.u = static_cast<int>(s_off - static_cast<long long>(w0.seg) * (w0.nt + kSegCost));
         w0.at = at;
         w0.end = end;
     }
     const long long T = s_scan[kThreads - 1], G = min(static_cast<long long>(gridDim.x), T);
     const uint32_t tmem = s_tmem;
     Walk wk = w0;
+    const int kh = kv.hd > 64 ? 2 : 1;   // K slots of a tile
 
     auto wait = [&](uint64_t *bar, uint32_t parity) {
         if (mbar_try_wait(bar, parity)) return true;
@@ -327,111 +342,163 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (warp == kWarpK || warp == kWarpV) {
         // ---------------- copies: boxes of min(page, 128) rows x 64 columns
+        // (V: min(page, 64) rows).  Lane = box; a slot's boxes are of eight
+        // or fewer neighbouring lanes.
         const bool isv = warp == kWarpV;
-        const int stages = isv ? C::v_stages : C::k_stages;
         const CUtensorMap *map = isv ? &mv : &mk;
-        uint8_t *ring = isv ? sV : sK;
-        uint64_t *full = isv ? bars.vfull : bars.kfull, *empty = isv ? bars.vempty : bars.kempty;
-        const int rb_shift = min(kv.page_shift, 7), rows = 1 << rb_shift, halves = kv.hd > 64 ? 2 : 1;
-        const int boxes = (kTile >> rb_shift) * halves;   // <= 16
-        const int pi = lane / halves, half = lane - pi * halves;
-        // a tile's box of this lane: its first row, where that lies in the page, the page's id (loaded one tile ahead)
+        const int rb_shift = min(kv.page_shift, isv ? 6 : 7), rows = 1 << rb_shift;
+        const int halves = kh, nbox = kTile >> rb_shift;      // boxes along the rows (<= 8) and the columns
+        // K: slot = column half, boxes along the rows; V: slot = row half, boxes (rows of it) x column halves
+        const int n_slots = isv ? 2 : kh, per = isv ? nbox / 2 * halves : nbox;
+        const int sl = lane / per, in = lane - sl * per;      // this lane's slot and box in it
+        const int pi = isv ? sl * (nbox / 2) + in / halves : in, half = isv ? in % halves : sl;
+        const bool mine = lane < n_slots * per;
+        const int dst = isv ? half * (64 * 128) + (((in / halves) << rb_shift) * 128) : (pi << rb_shift) * 128;
+        const unsigned slot_lanes = mine ? ((1u << per) - 1u) << (sl * per) : 0u;
+        // a tile's box of this lane: the page's id (loaded one tile ahead) and the row in the page
         struct Box {
             bool on;
             int page, y;
         };
         bool more = wk.next(a, segs);
-        int t = wk.t0;
+        int t = wk.t0, base = 0, nt = wk.t1 - wk.t0, i = 0;   // the portion's first position, its tiles, the tile in it
         auto fetch = [&]() {
             Box x{false, 0, 0};
             if (!more) return x;
             const Seq s(a, wk.b, false);
             const int r0 = (s.tile0 + t) * kTile + (pi << rb_shift);
-            x.on = lane < boxes && r0 < s.n && r0 + rows > s.first;
+            x.on = mine && r0 < s.n && r0 + rows > s.first;
             if (x.on) x.page = __ldg(kv.table + static_cast<long long>(wk.b) * kv.table_stride + (r0 >> kv.page_shift));
             x.y = ((wk.seg / groups) << kv.page_shift) + (r0 & ((1 << kv.page_shift) - 1));
             return x;
         };
         Box nxt = fetch();
-        int q = 0;
-        for (; more; q++) {
+        while (more) {
             Box x = nxt;
+            const int first = base + (isv ? pos_v(i, nt, kh) : pos_k(i, kh));
+            i++;
             if (++t == wk.t1) {
+                base += nt * (kh + 2);
                 more = wk.next(a, segs);
                 t = wk.t0;
+                nt = wk.t1 - wk.t0;
+                i = 0;
             }
             nxt = fetch();
-            const int st = q % stages, use = q / stages;
-            if (use > 0 && !__all_sync(0xffffffffu, wait(&empty[st], static_cast<uint32_t>((use - 1) & 1)))) break;
             if (x.on && static_cast<unsigned>(x.page) >= static_cast<unsigned>(kv.n_pages)) {
                 if (!isv) atomicExch(kv.err, kErrBadPos);
                 x.on = false;
             }
-            const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, x.on)) * static_cast<uint32_t>(rows) * 128u;
-            if (lane == 0) mbar_arrive_expect_tx(&full[st], bytes);
-            __syncwarp();
-            if (x.on)
-                tma3(ring + st * kSlotBytes + half * kHalfBytes + (pi << rb_shift) * 128, map, half * 64, x.y, x.page, &full[st]);
+            const unsigned on = __ballot_sync(0xffffffffu, x.on);
+            // the slots in order: a slot is armed, then its lanes copy
+            bool live = true;
+            for (int k = 0; k < n_slots; k++) {
+                const int p = first + k, st = p % C::slots, use = p / C::slots;
+                if (use > 0 && !__all_sync(0xffffffffu, wait(&bars.empty[st], static_cast<uint32_t>((use - 1) & 1)))) {
+                    live = false;
+                    break;
+                }
+                const unsigned lanes = __shfl_sync(0xffffffffu, slot_lanes, k * per);
+                if (lane == 0)
+                    mbar_arrive_expect_tx(&bars.full[st], __popc(on & lanes) * static_cast<uint32_t>(rows) * 128u);
+                __syncwarp();
+                if (x.on && sl == k) tma3(ring + st * kSlotBytes + dst, map, half * 64, x.y, x.page, &bars.full[st]);
+            }
+            if (!live) break;
         }
-        // nothing of this warp's is still landing when the CTA ends
-        for (int i = max(0, q - stages); i < q; i++)
-            mbar_wait(&full[i % stages], static_cast<uint32_t>((i / stages) & 1), nullptr, 0);
-    } else if (warp == kWarpMma) {
-        // ---------------- the products: the warp walks together (what an
-        // MMA is given stays in uniform registers), one lane issues
-        constexpr uint32_t id_s = idesc(BF, NB, false), id_o = idesc(BF, NB, true);
+        // Every copy is waited for by the products that read it.  Where a wait gave up, nothing of this warp's may still
+        // be landing when the CTA ends: copies take microseconds, a millisecond is given to them.
+        if (*reinterpret_cast<volatile int *>(&s_abort))
+            for (const long long c0 = clock64(); clock64() - c0 < 2000000;) {
+            }
+    } else if (warp == kWarpS) {
+        // ---------------- S = K Q^T.  The warp walks together (what an MMA is
+        // given stays in uniform registers), one lane issues.
+        constexpr uint32_t id = idesc(BF, NB, false);
         const bool leader = elect();
         const int ksteps = (kv.hd + 15) / 16;
-        const uint32_t dK = desc_lo(smem_addr(sK), 16), dV = desc_lo(smem_addr(sV), kHalfBytes);
-        const uint32_t dQ = desc_lo(smem_addr(sQ), 16), dP = desc_lo(smem_addr(sP), 16);
-        int q = 0, portion = 0;
+        const uint32_t dK = desc_lo(smem_addr(ring), 16), dQ = desc_lo(smem_addr(sQ), 16);
+        int q = 0, portion = 0, base = 0;   // tile number, portion, its first slot position
         bool live = true;
-        auto scores = [&](int i) {   // S of tile i (global number) into buffer i % 2
-            const int st = i % C::k_stages;
-            if (!__all_sync(0xffffffffu, wait(&bars.kfull[st], static_cast<uint32_t>((i / C::k_stages) & 1)))) return false;
-            fence_after();
-            if (leader) {
-                const uint32_t dk = dK + static_cast<uint32_t>(st) * (kSlotBytes / 16), d = tmem + kColS + (i & 1) * kColStep;
-#pragma unroll
-                for (int k = 0; k < 8; k++)
-                    if (k < ksteps)
-                        mma(d, dk + (k >> 2) * (kHalfBytes / 16) + (k & 3) * 2, dQ + (k >> 2) * (NB * 128 / 16) + (k & 3) * 2,
-                            id_s, k > 0);
-                commit(&bars.kempty[st]);
-                commit(&bars.sfull[i & 1]);
-            }
-            __syncwarp();
-            return true;
-        };
         while (live && wk.next(a, segs)) {
             const int nt = wk.t1 - wk.t0;
-            if (!__all_sync(0xffffffffu, wait(&bars.qfull, static_cast<uint32_t>(portion & 1)))) break;
-            fence_after();
-            live = scores(q) && (nt < 2 || scores(q + 1));
-            for (int t = 0; t < nt && live; t++, q++) {
-                const int st = q % C::v_stages, wg = q & 1;
-                live = __all_sync(0xffffffffu, wait(&bars.vfull[st], static_cast<uint32_t>((q / C::v_stages) & 1)) &&
-                                                   wait(&bars.pfull[wg], static_cast<uint32_t>((q >> 1) & 1)));
-                if (!live) break;
+            int st = base % C::slots;
+            uint32_t ph = static_cast<uint32_t>(base / C::slots) & 1;
+            live = wait(&bars.qfull, static_cast<uint32_t>(portion & 1));
+            for (int t = 0; t < nt; t++, q++) {
+                // the buffer's earlier scores (tile q - 2) have been read
+                if (q > 1) live &= wait(&bars.pfull[q & 1], static_cast<uint32_t>((q >> 1) + 1) & 1);
+                const int s1 = st + 1 == C::slots ? 0 : st + 1;
+                live &= wait(&bars.full[st], ph);
+                if (kh == 2) live &= wait(&bars.full[s1], st + 1 == C::slots ? ph ^ 1 : ph);
                 fence_after();
                 if (leader) {
-                    const uint32_t dv = dV + static_cast<uint32_t>(st) * (kSlotBytes / 16), d = tmem + kColO + wg * kColStep;
-                    const uint32_t dp = dP + static_cast<uint32_t>(wg) * (C::p_bytes / 16);
+                    const uint32_t d = tmem + kColS + (q & 1) * kColStep;
 #pragma unroll
-                    for (int k = 0; k < kTile / 16; k++)
-                        mma(d, dv + k * (2048 / 16), dp + (k >> 2) * (NB * 128 / 16) + (k & 3) * 2, id_o, t > 1 || k > 0);
-                    commit(&bars.vempty[st]);
-                    commit(&bars.odone[wg]);
+                    for (int k = 0; k < 8; k++)
+                        if (k < ksteps)
+                            mma(d, dK + static_cast<uint32_t>(k < 4 ? st : s1) * (kSlotBytes / 16) + (k & 3) * 2,
+                                dQ + (k >> 2) * (NB * 128 / 16) + (k & 3) * 2, id, k > 0);
+                    commit(&bars.sfull[q & 1]);
+                    commit(&bars.empty[st]);
+                    if (kh == 2) commit(&bars.empty[s1]);
                 }
-                __syncwarp();
-                if (t + 2 < nt) live = scores(q + 2);   // the warpgroup has read its scores of tile q
+                live = __all_sync(0xffffffffu, live);
+                if (!live) break;
+                st += t == 0 ? kh : kh + 2;   // K0 K1 V0 K2 V1 ...
+                if (st >= C::slots) {
+                    st -= C::slots;
+                    ph ^= 1;
+                }
             }
+            base += nt * (kh + 2);
             portion++;
         }
-        // every product issued here has completed before TMEM is freed
+        if (leader) {   // every product issued here has completed before TMEM is freed
+            commit(&bars.drain[0]);
+            mbar_wait(&bars.drain[0], 0u, nullptr, 0);
+        }
+        __syncwarp();
+    } else if (warp == kWarpO) {
+        // ---------------- O^T += V^T P^T
+        constexpr uint32_t id = idesc(BF, NB, true);
+        const bool leader = elect();
+        const uint32_t dV = desc_lo(smem_addr(ring), 64 * 128), dP = desc_lo(smem_addr(sP), 16);
+        int q = 0, base = 0;
+        bool live = true;
+        while (live && wk.next(a, segs)) {
+            const int nt = wk.t1 - wk.t0, p0 = base + pos_v(0, nt, kh);
+            int st = p0 % C::slots;
+            uint32_t ph = static_cast<uint32_t>(p0 / C::slots) & 1;
+            for (int t = 0; t < nt; t++, q++) {
+                const int wg = q & 1, s1 = st + 1 == C::slots ? 0 : st + 1;
+                live &= wait(&bars.full[st], ph);
+                live &= wait(&bars.full[s1], st + 1 == C::slots ? ph ^ 1 : ph);
+                live &= wait(&bars.pfull[wg], static_cast<uint32_t>((q >> 1) & 1));
+                fence_after();
+                if (leader) {
+                    const uint32_t d = tmem + kColO + wg * kColStep, dp = dP + static_cast<uint32_t>(wg) * (C::p_bytes / 16);
+#pragma unroll
+                    for (int k = 0; k < 8; k++)
+                        mma(d, dV + static_cast<uint32_t>(k < 4 ? st : s1) * (kSlotBytes / 16) + (k & 3) * (2048 / 16),
+                            dp + (k >> 2) * (NB * 128 / 16) + (k & 3) * 2, id, t > 1 || k > 0);
+                    commit(&bars.odone[wg]);
+                    commit(&bars.empty[st]);
+                    commit(&bars.empty[s1]);
+                }
+                live = __all_sync(0xffffffffu, live);
+                if (!live) break;
+                st += t + 2 < nt ? kh + 2 : 2;
+                if (st >= C::slots) {
+                    st -= C::slots;
+                    ph ^= 1;
+                }
+            }
+            base += nt * (kh + 2);
+        }
         if (leader) {
-            commit(&bars.drain);
-            mbar_wait(&bars.drain, 0u, nullptr, 0);
+            commit(&bars.drain[1]);
+            mbar_wait(&bars.drain[1], 0u, nullptr, 0);
         }
         __syncwarp();
     } else {
@@ -445,7 +512,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint8_t *myP = sP + wg * C::p_bytes;
         const float l2 = a.scale * 1.4426950408889634f;   // scores in units of log2
         const long long max_rows = static_cast<long long>(kv.max_pages) << kv.page_shift;
-        int q = 0, portion = 0;                            // the portion's first tile (global number), its number
+        int q = 0, portion = 0, base = 0;                  // the portion's first tile, its number, its first slot position
         // q of a portion into shared memory: every thread the elements that it will read itself
         auto stage_q = [&](const Walk &w) {
             const int j = w.seg / groups, g0 = (w.seg - j * groups) * NH;
@@ -471,8 +538,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                 asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll
                 for (int h = 0; h < NH; h++) qv[h] = h < ng && tg < kv.hd ? sQn[h * 128 + tg] * l2 : 0.f;
-                Walk ahead = wk;   // the next portion's q is on its way while this one runs
-                if (ahead.next(a, segs)) stage_q(ahead);
                 if constexpr (!BF) {
 #pragma unroll
                     for (int h = 0; h < NH; h++) {
@@ -499,6 +564,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 fence_async();
                 mbar_arrive(&bars.qfull);
+                Walk ahead = wk;   // the next portion's q is on its way while this one runs
+                if (ahead.next(a, segs)) stage_q(ahead);
                 if (portion > 0) read_sync();   // the first warpgroup has read what lies in this one's P
             }
             if constexpr (!BF) {
@@ -603,14 +670,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 if (!on) {
                     // 0 x (whatever lies in a row that is not seen) has to be 0
-                    const int st = qt % C::v_stages;
-                    wait(&bars.vfull[st], static_cast<uint32_t>((qt / C::v_stages) & 1));
+                    const int p = base + pos_v(t, ntp, kh) + (tg >> 6), st = p % C::slots;
+                    wait(&bars.full[st], static_cast<uint32_t>((p / C::slots) & 1));
                     const uint4 z = make_uint4(0, 0, 0, 0);
-                    uint8_t *vr = sV + st * kSlotBytes + tg * 128;
+                    uint8_t *vr = ring + st * kSlotBytes + (tg & 63) * 128;
 #pragma unroll
                     for (int c = 0; c < 8; c++) {
                         *reinterpret_cast<uint4 *>(vr + 16 * c) = z;
-                        *reinterpret_cast<uint4 *>(vr + kHalfBytes + 16 * c) = z;
+                        *reinterpret_cast<uint4 *>(vr + 64 * 128 + 16 * c) = z;
                     }
                 }
                 __syncwarp();
@@ -624,6 +691,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             fence_after();
             q += ntp;
+            base += ntp * (kh + 2);
             float o[NH];
 #pragma unroll
             for (int hb = 0; hb < NH; hb += 8) {
@@ -689,7 +757,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 continue;
             }
             if (wk.t1 == wk.nt && tg == 0) {
-                // for the join: the segment's first owner (CTA i's tiles begin at floor(i T / G)) and its portions
+                // for the join: the first tile's owner (CTA i's units begin at floor(i T / G)) and the portions
                 const long long n = (wk.at - wk.nt + 1) * G - 1;
                 const int own0 = static_cast<int>(T * G < (1ll << 31) ? static_cast<unsigned>(n) / static_cast<unsigned>(T) : n / T);
                 a.cnt[static_cast<long long>(wk.b) * segs + wk.seg] = static_cast<unsigned>(own0) << 16 | (blockIdx.x - own0 + 1);
@@ -707,7 +775,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     }
     __syncthreads();
-    if (warp == kWarpMma)
+    if (warp == kWarpO)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
 }
 

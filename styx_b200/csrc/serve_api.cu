@@ -234,9 +234,10 @@ int styx_paged_attend(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv
         const uint64_t dims[3] = {static_cast<uint64_t>(kv->head_dim), static_cast<uint64_t>(kv->n_kv_heads) * kv->page_size,
                                   static_cast<uint64_t>(kv->n_pages)};
         const uint64_t strides[2] = {kv->head_dim * 2ull, static_cast<uint64_t>(kv->page_stride) * 2};
-        const uint32_t box[3] = {64, static_cast<uint32_t>(kv->page_size < 128 ? kv->page_size : 128), 1};
-        CHECK(styx::encode_map3(&mk, kv->k, dims, strides, box));
-        CHECK(styx::encode_map3(&mv, kv->v, dims, strides, box));
+        const uint32_t box_k[3] = {64, static_cast<uint32_t>(kv->page_size < 128 ? kv->page_size : 128), 1};
+        const uint32_t box_v[3] = {64, static_cast<uint32_t>(kv->page_size < 64 ? kv->page_size : 64), 1};
+        CHECK(styx::encode_map3(&mk, kv->k, dims, strides, box_k));
+        CHECK(styx::encode_map3(&mv, kv->v, dims, strides, box_v));
         CK(styx::launch_attend_tc(a, mk, mv, sms < 152 ? sms : 152, S(stream)));
     } else {
         CK(styx::launch_paged_attend(a, S(stream)));
