@@ -398,7 +398,7 @@ struct PagedAttendArgs {
     float *part;                   // workspace: the portions' partial results, kAttendPart floats each
     unsigned *cnt;                 // workspace, per (sequence, kv head, group): first CTA << 16 | portions (0: not cut)
 };
-// a portion of up to 16 heads of up to 128 elements: O, maxima, sums
+// a portion of up to 16 heads of up to 128 elements, or 8 of 256: O, 16 maxima, 16 sums
 constexpr int kAttendPart = 16 * 128 + 32;
 struct PagedEvictArgs {
     PagedKv kv;
@@ -421,12 +421,15 @@ struct SampleArgs {
     float *logprob;                // may be null
 };
 cudaError_t launch_paged_append(const PagedAppendArgs &a, cudaStream_t st);
-cudaError_t launch_paged_attend(const PagedAttendArgs &a, cudaStream_t st);
-// the tensor-core form: mk, mv map the pools as {head_dim, n_kv * page rows,
-// pages}, box 64 x min(page, 128) rows (V: 64), 128-byte swizzle
+// attention on the FMA units; on the tensor cores (mk, mv map the pools as
+// {head_dim, n_kv * page rows, pages}, box 64 x min(page, 128) rows (V: 64),
+// 128-byte swizzle); and what ends both: portions of nh heads, pitch floats
+// each, joined, and the weights accumulated
+cudaError_t launch_attend_fma(const PagedAttendArgs &a, int sms, cudaStream_t st);
 cudaError_t launch_attend_tc(const PagedAttendArgs &a, const CUtensorMap &mk, const CUtensorMap &mv, int sms,
                              cudaStream_t st);
-cudaError_t launch_paged_acc(const PagedAttendArgs &a, cudaStream_t st);
+cudaError_t launch_attend_finish(const PagedAttendArgs &a, int nh, int pitch, cudaStream_t st);
+int attend_grid(const PagedAttendArgs &a, int nh, int sms);
 cudaError_t launch_paged_evict(const PagedEvictArgs &a, cudaStream_t st);
 cudaError_t launch_sample(const SampleArgs &a, cudaStream_t st);
 

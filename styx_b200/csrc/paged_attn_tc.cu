@@ -20,7 +20,7 @@
 // i-th G-th of it, so ragged lengths spread evenly over the SMs.  A portion
 // (a CTA's consecutive tiles of one segment) ends in (max, sum, O) per head:
 // written out where it is the whole segment, else to the workspace, from
-// where k_attend_join, one CTA per segment, adds the portions up in order.
+// where k_attend_finish adds the portions up in order.
 // (Joining inside this kernel, by the CTA that finishes a segment last, kept
 // four of 148 SMs 12 us longer than the rest at one sequence of 131071 rows.)
 //
@@ -40,25 +40,17 @@
 
 #include <cstdint>
 
-#include "paged.cuh"
+#include "paged_split.cuh"
 
 namespace styx {
 namespace {
 
-constexpr int kTile = 128;                 // rows of a tile = M of both products
 constexpr int kHalfBytes = kTile * 128;    // 64 columns of a tile: 128-byte rows
 constexpr int kSlotBytes = kHalfBytes;     // K: 128 rows x 64 columns; V: 2 x (64 rows x 64 columns)
 constexpr int kThreads = 384;
 constexpr int kWarpK = 8, kWarpV = 9, kWarpS = 10, kWarpO = 11;
-// what a segment's start costs a CTA (Q, the first maxima, the result), in
-// tiles: the partition counts it, so that CTAs with many short segments get
-// fewer tiles
-constexpr int kSegCost = 3;
 constexpr uint32_t kTmemCols = 256, kColS = 0, kColO = 128, kColStep = 64;   // two score buffers, two accumulators
 constexpr float kSlack = 8.f;              // log2 units a score may pass the maximum by
-constexpr float kNone = -3e38f;            // maximum of no scores: finite, so that differences stay numbers
-
-constexpr int kJoinParts = 152;            // CTAs, and so portions of a segment, at most (B200: 148 SMs)
 
 template <bool BF, int NH>
 struct Cfg {
@@ -151,12 +143,6 @@ __device__ __forceinline__ float warp_max(float v) {   // NaN only where every l
     asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
     return r;
 }
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // v as a sum of terms of the cache's type, largest first.  bf16: the f32's 24
 // significant bits cut into 8 + 8 + 8, exactly; f16: rounded to 11, the rest
 // rounded to 11.
@@ -190,45 +176,6 @@ struct Bars {
 __device__ __forceinline__ int pos_k(int t, int kh) { return kh * t + 2 * max(0, t - 1); }
 __device__ __forceinline__ int pos_v(int t, int nt, int kh) { return kh * min(t + 2, nt) + 2 * t; }
 
-// rows of a sequence that are seen, and its tiles (an empty one counts one
-// tile, so that somebody writes its zeros)
-struct Seq {
-    int n, first, tile0, nt;
-    __device__ __forceinline__ Seq(const PagedAttendArgs &a, int b, bool report) {
-        n = paged_len(a.kv, b, report);
-        first = a.window > 0 && a.window < n ? n - a.window : 0;
-        tile0 = first / kTile;
-        nt = max(1, (n + kTile - 1) / kTile - tile0);
-    }
-};
-
-// the CTA's share of the list, portion by portion.  A segment is kSegCost
-// empty units, then its tiles.
-struct Walk {
-    int b, seg, u, nt;             // sequence, (kv head, group) in it, next unit of kSegCost + nt
-    long long at, end;             // global unit numbers
-    int t0, t1;                    // the portion: tiles [t0, t1) of the segment
-    __device__ __forceinline__ bool next(const PagedAttendArgs &a, int segs) {
-        while (at < end) {
-            if (u == kSegCost + nt) {
-                u = 0;
-                if (++seg == segs) {
-                    seg = 0;
-                    b++;
-                    nt = Seq(a, b, false).nt;
-                }
-            }
-            const int u1 = static_cast<int>(min(static_cast<long long>(kSegCost + nt), u + (end - at)));
-            t0 = max(0, u - kSegCost);
-            t1 = max(0, u1 - kSegCost);
-            at += u1 - u;
-            u = u1;
-            if (t1 > t0) return true;
-        }
-        return false;
-    }
-};
-
 template <bool BF, int NH>
 __global__ void __launch_bounds__(kThreads, 1)
     k_attend_tc(PagedAttendArgs a, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv) {
@@ -240,8 +187,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     float *sQn = reinterpret_cast<float *>(sP + 2 * C::p_bytes);
     __shared__ Bars bars;
     __shared__ uint32_t s_tmem;
-    __shared__ int s_abort, s_b0;
-    __shared__ long long s_off, s_scan[kThreads];
+    __shared__ Share<kThreads> share;
+    __shared__ int s_abort;
     __shared__ float s_red[8][16], s_l[8][16], s_ml[2][16], s_f[16];
     const PagedKv &kv = a.kv;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
@@ -273,57 +220,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     pdl_wait();
 
-    // ---------------- the CTA's share: tiles before each chunk of sequences, total
-    Walk w0;
-    {
-        const int per = (kv.n_seqs + kThreads - 1) / kThreads, lo = min(kv.n_seqs, tid * per), hi = min(kv.n_seqs, lo + per);
-        long long mine = 0;
-        for (int b = lo; b < hi; b++) mine += static_cast<long long>(Seq(a, b, blockIdx.x == 0).nt + kSegCost) * segs;
-        s_scan[tid] = mine;
-        __syncthreads();
-        if (warp == 0) {   // inclusive scan of the kThreads chunks
-            long long v[kThreads / 32], run = 0;
-#pragma unroll
-            for (int i = 0; i < kThreads / 32; i++) {
-                run += s_scan[lane * (kThreads / 32) + i];
-                v[i] = run;
-            }
-            long long x = run;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const long long u = __shfl_up_sync(0xffffffffu, x, o);
-                if (lane >= o) x += u;
-            }
-#pragma unroll
-            for (int i = 0; i < kThreads / 32; i++) s_scan[lane * (kThreads / 32) + i] = v[i] + x - run;
-        }
-        __syncthreads();
-        const long long T = s_scan[kThreads - 1];
-        const long long G = min(static_cast<long long>(gridDim.x), T);
-        const long long at = blockIdx.x < G ? blockIdx.x * T / G : 0, end = blockIdx.x < G ? (blockIdx.x + 1) * T / G : 0;
-        const long long before = s_scan[tid] - mine;
-        if (mine > 0 && at >= before && at < before + mine) {
-            long long off = at - before;
-            int b = lo;
-            for (; b < hi; b++) {
-                const long long nb = static_cast<long long>(Seq(a, b, false).nt + kSegCost) * segs;
-                if (off < nb) break;
-                off -= nb;
-            }
-            s_b0 = b;
-            s_off = off;
-        }
-        __syncthreads();
-        w0.b = s_b0;
-        w0.nt = Seq(a, w0.b, false).nt;
-        w0.seg = static_cast<int>(s_off / (w0.nt + kSegCost));
-        w0.u = static_cast<int>(s_off - static_cast<long long>(w0.seg) * (w0.nt + kSegCost));
-        w0.at = at;
-        w0.end = end;
-    }
-    const long long T = s_scan[kThreads - 1], G = min(static_cast<long long>(gridDim.x), T);
+    long long T, G;
+    Walk wk;
+    share_of<kThreads>(a, segs, share, wk, T, G);
     const uint32_t tmem = s_tmem;
-    Walk wk = w0;
     const int kh = kv.hd > 64 ? 2 : 1;   // K slots of a tile
 
     auto wait = [&](uint64_t *bar, uint32_t parity) {
@@ -751,25 +651,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     }
             };
+            if (wk.t1 == wk.nt && tg == 0) a.cnt[static_cast<long long>(wk.b) * segs + wk.seg] = cut_of(wk, T, G);
             if (wk.t0 == 0 && wk.t1 == wk.nt) {   // the whole segment
                 write_out(o, m, L);
-                if (tg == 0) a.cnt[static_cast<long long>(wk.b) * segs + wk.seg] = 0;
                 continue;
             }
-            if (wk.t1 == wk.nt && tg == 0) {
-                // for the join: the first tile's owner (CTA i's units begin at floor(i T / G)) and the portions
-                const long long n = (wk.at - wk.nt + 1) * G - 1;
-                const int own0 = static_cast<int>(T * G < (1ll << 31) ? static_cast<unsigned>(n) / static_cast<unsigned>(T) : n / T);
-                a.cnt[static_cast<long long>(wk.b) * segs + wk.seg] = static_cast<unsigned>(own0) << 16 | (blockIdx.x - own0 + 1);
-            }
-            // a part of it: CTA i's portion that begins its segment goes to slot 2 i + 1, any other to slot 2 i
-            float *part = a.part + (2ll * blockIdx.x + (wk.t0 == 0 ? 1 : 0)) * kAttendPart;
+            float *part = part_at(a, blockIdx.x, wk.t0 == 0);
 #pragma unroll
             for (int h = 0; h < NH; h++) {
                 part[h * 128 + tg] = o[h];
                 if (tg == h) {
-                    part[NH * 128 + h] = m[h];
-                    part[NH * 128 + NH + h] = L[h];
+                    part[kAttendPart - 32 + h] = m[h];
+                    part[kAttendPart - 16 + h] = L[h];
                 }
             }
         }
@@ -779,68 +672,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
 }
 
-// CTA = one segment that was cut: its portions, in order.  Warp w takes heads
-// w, w + 8, ..., lane l elements 4 l ..; eight portions' loads in flight.
-template <int NH>
-__global__ void __launch_bounds__(256) k_attend_join(PagedAttendArgs a) {
-    pdl_trigger();
-    __shared__ float sm_m[kJoinParts][NH], sm_l[kJoinParts][NH];
-    const PagedKv &kv = a.kv;
-    const int groups = (a.gqa + NH - 1) / NH, segs = kv.n_kv * groups;
-    const int b = blockIdx.x / segs, seg = blockIdx.x - b * segs, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int j = seg / groups, g0 = (seg - j * groups) * NH, ng = min(NH, a.gqa - g0);
-    pdl_wait();
-    const unsigned c = __ldcg(a.cnt + blockIdx.x);
-    const int np = static_cast<int>(c & 0xFFFFu);
-    if (np == 0) return;
-    const float *parts = a.part + 2ll * (c >> 16) * kAttendPart;
-    auto part_of = [&](int i) { return parts + (i == 0 ? 1 : 2 * i) * kAttendPart; };
-    for (int i = threadIdx.x; i < np * NH; i += 256) {
-        const float *pp = part_of(i / NH) + NH * 128 + i % NH;
-        sm_m[i / NH][i % NH] = __ldcg(pp);
-        sm_l[i / NH][i % NH] = __ldcg(pp + NH);
-    }
-    __syncthreads();
-    for (int h = warp; h < ng; h += 8) {
-        float4 v[8];
-        auto load = [&](int i0) {
-#pragma unroll
-            for (int i = 0; i < 8; i++)
-                v[i] = __ldcg(reinterpret_cast<const float4 *>(part_of(min(i0 + i, np - 1)) + h * 128) + lane);
-        };
-        load(0);
-        float M = kNone, L = 0.f;
-        for (int i = lane; i < np; i += 32) M = fmaxf(M, sm_m[i][h]);
-#pragma unroll
-        for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int i0 = 0; i0 < np; i0 += 8) {
-#pragma unroll
-            for (int i = 0; i < 8; i++)
-                if (i0 + i < np) {
-                    const float f = ex2(sm_m[i0 + i][h] - M);
-                    L += f * sm_l[i0 + i][h];
-                    o.x += f * v[i].x;
-                    o.y += f * v[i].y;
-                    o.z += f * v[i].z;
-                    o.w += f * v[i].w;
-                }
-            if (i0 + 8 < np) load(i0 + 8);
-        }
-        const long long at = static_cast<long long>(b) * a.n_heads + j * a.gqa + g0 + h;
-        const float r = L > 0.f ? 1.f / L : 0.f;
-        if (4 * lane < kv.hd)
-            *reinterpret_cast<float4 *>(a.out + at * kv.hd + 4 * lane) = make_float4(o.x * r, o.y * r, o.z * r, o.w * r);
-        if (lane == 0) {
-            if (a.lse) a.lse[at] = L > 0.f ? M * 0.6931471805599453f + logf(L) : -INFINITY;
-            if (a.acc_out) {
-                a.ml[2 * at] = M;
-                a.ml[2 * at + 1] = L;
-            }
-        }
-    }
-}
-
 template <bool BF, int NH>
 cudaError_t launch(const PagedAttendArgs &a, const CUtensorMap &mk, const CUtensorMap &mv, int grid, cudaStream_t st) {
     constexpr int smem = Cfg<BF, NH>::smem;
@@ -848,21 +679,13 @@ cudaError_t launch(const PagedAttendArgs &a, const CUtensorMap &mk, const CUtens
     cudaError_t e = cudaFuncSetAttribute(k_attend_tc<BF, NH>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     e = launch_pdl(k_attend_tc<BF, NH>, dim3(grid), dim3(kThreads), smem, st, a, mk, mv);
-    // nothing is cut where no sequence can have a second tile
-    if (e != cudaSuccess || (static_cast<long long>(a.kv.max_pages) << a.kv.page_shift) <= kTile) return e;
-    const int groups = (a.gqa + NH - 1) / NH;
-    return launch_pdl(k_attend_join<NH>, dim3(a.kv.n_seqs * a.kv.n_kv * groups), dim3(256), 0, st, a);
+    return e != cudaSuccess ? e : launch_attend_finish(a, NH, 128, st);
 }
 
 }  // namespace
 
 cudaError_t launch_attend_tc(const PagedAttendArgs &a, const CUtensorMap &mk, const CUtensorMap &mv, int sms, cudaStream_t st) {
-    const int nh = a.gqa <= 8 ? 8 : 16, groups = (a.gqa + nh - 1) / nh;
-    // no more CTAs than tiles there can be
-    const long long tiles = static_cast<long long>(a.kv.n_seqs) * a.kv.n_kv * groups *
-                            (((static_cast<long long>(a.kv.max_pages) << a.kv.page_shift) + kTile - 1) / kTile);
-    const int grid = static_cast<int>(tiles < sms ? tiles : sms);
-    if (grid > kJoinParts) return cudaErrorInvalidConfiguration;
+    const int nh = a.gqa <= 8 ? 8 : 16, grid = attend_grid(a, nh, sms);
     if (a.kv.dtype == STYX_BF16) return nh == 8 ? launch<true, 8>(a, mk, mv, grid, st) : launch<true, 16>(a, mk, mv, grid, st);
     return nh == 8 ? launch<false, 8>(a, mk, mv, grid, st) : launch<false, 16>(a, mk, mv, grid, st);
 }

@@ -205,7 +205,7 @@ int styx_paged_attend(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv
          "q / out / lse smaller than n_seqs x n_heads");
     if (acc_out) {
         const uint64_t lines = static_cast<uint64_t>(kv->n_seqs) * kv->n_kv_heads * acc_stride * 4;
-        NEED(kv->n_seqs * static_cast<int64_t>(kv->n_kv_heads) <= 65535, "accumulation: n_seqs x n_kv_heads <= 65535");
+        NEED(kv->n_seqs * static_cast<int64_t>(kv->n_kv_heads) <= 65535, "accumulation: n_seqs x n_kv_heads <= 65535");   // lines x row blocks: a grid's x
         NEED(styx::range_ok(acc, lines) && styx::range_ok(acc_out, lines), "acc / acc_out smaller than n_seqs x n_kv_heads lines");
     }
     const AttendWs w = attend_ws(kv, n_heads, acc_out != nullptr, sms);
@@ -238,11 +238,10 @@ int styx_paged_attend(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv
         const uint32_t box_v[3] = {64, static_cast<uint32_t>(kv->page_size < 64 ? kv->page_size : 64), 1};
         CHECK(styx::encode_map3(&mk, kv->k, dims, strides, box_k));
         CHECK(styx::encode_map3(&mv, kv->v, dims, strides, box_v));
-        CK(styx::launch_attend_tc(a, mk, mv, sms < 152 ? sms : 152, S(stream)));
+        CK(styx::launch_attend_tc(a, mk, mv, sms, S(stream)));
     } else {
-        CK(styx::launch_paged_attend(a, S(stream)));
+        CK(styx::launch_attend_fma(a, sms, S(stream)));
     }
-    if (acc_out) CK(styx::launch_paged_acc(a, S(stream)));
     return STYX_OK;
 }
 
