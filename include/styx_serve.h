@@ -65,7 +65,8 @@ typedef struct styx_paged_kv {
  * pairs (i, i + head_dim / 2), theta = pos * freq_base^(-2i/head_dim).  A
  * token whose row is negative (a slot of length 0 among them) writes no row
  * and a zero q_out; a row past max_pages * page_size or a page outside the
- * pool is skipped and reported.  n_heads may be 0 (no q), q_out may not
+ * pool is skipped and reported.  n_heads may be 0 (no q); q_out, 16-byte
+ * aligned, may not
  * overlap q.  Two tokens with one (sequence, row) leave either's row. */
 int styx_paged_append(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv, int n_tokens, int n_heads,
                       const float *q, int64_t q_stride, const float *k, int64_t k_stride, const float *v,

@@ -378,7 +378,7 @@ struct PagedAppendArgs {
     long long q_stride, k_stride, v_stride;   // floats between tokens
     const float *q_norm, *k_norm;             // [hd] or null
     float eps;
-    double theta_scale;                       // freq_base^(-2/hd)
+    double log2_base;                         // log2(freq_base^(-2/hd))
     const int32_t *pos, *seq, *row;           // seq, row may be null
     float *q_out;
     int n_tokens, n_heads;
@@ -408,7 +408,7 @@ struct PagedEvictArgs {
     int budget, n_recent, n_sink;
     float *acc_out;
     int32_t *pos_out, *lens_out;
-    int32_t *src, *places;         // workspace, [n_seqs][n_kv][budget] each: the row that row r is filled from; the places
+    int32_t *src, *places;         // workspace, [n_seqs][n_kv][budget] each: the rows that move, and the places they move to
 };
 struct SampleArgs {
     const float *logits;
@@ -420,7 +420,7 @@ struct SampleArgs {
     int32_t *token;
     float *logprob;                // may be null
 };
-cudaError_t launch_paged_append(const PagedAppendArgs &a, cudaStream_t st);
+cudaError_t launch_paged_append(const PagedAppendArgs &a, int sms, cudaStream_t st);
 // attention on the FMA units; on the tensor cores (mk, mv map the pools as
 // {head_dim, n_kv * page rows, pages}, box 64 x min(page, 128) rows (V: 64),
 // 128-byte swizzle); and what ends both: portions of nh heads, pitch floats

@@ -1,12 +1,13 @@
 // paged.cu -- rows into and out of a paged KV cache (include/styx_serve.h):
 //
 //   k_paged_append   per-head RMSNorm, RoPE and the rounded K / V rows
-//   k_evict_select   the rows that stay, and the row each place is filled from
-//   k_evict_move     K, V, weight and position of the rows that move
+//   k_paged_evict    the rows that stay, and the moves that close the gaps
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 
+#include "cluster.cuh"
 #include "paged.cuh"
 
 namespace styx {
@@ -18,77 +19,134 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
-// CTA (token t, head h): h < n_heads a q head, else kv head h - n_heads.
-// Thread i < hd/2 owns the pair (i, i + hd/2).
+// ------------------------------------------------------------ append
+// A CTA takes tokens in turn (blockIdx.y: a share of their rows when tokens
+// are few).  The token's cosines and sines are computed once, by the first
+// threads, into shared memory: the angle in turns, pos * base^(-2i/d) / 2 pi,
+// is held in 64 bits and reduced to a fraction of a turn before it is rounded
+// to f32, so its error does not grow with the position.  Then a warp takes
+// four of the token's rows (q heads, k heads, v heads) at a time, all loads
+// first; lane l holds the pairs (i, i + d/2) of i = 2 l, 2 l + 1 (+ 64).
+constexpr int kAppThreads = 256, kAppRows = 4;
+
 template <class T>
-__global__ void __launch_bounds__(128) k_paged_append(PagedAppendArgs a) {
+__device__ __forceinline__ void store2(T *p, float a, float b) {
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float2 *>(p) = make_float2(a, b);
+    } else {
+        T v[2] = {from_f<T>(a), from_f<T>(b)};
+        *reinterpret_cast<uint32_t *>(p) = *reinterpret_cast<uint32_t *>(v);
+    }
+}
+
+// K: rounds of 64 pairs, d <= 128 K (d/2 is even: rows are of 16 bytes'
+// multiples).  vec: every row of the inputs is 8-byte aligned, else loads are
+// by element.
+template <class T, int K>
+__global__ void __launch_bounds__(kAppThreads) k_paged_append(PagedAppendArgs a, bool vec) {
     pdl_trigger();
-    pdl_wait();
-    __shared__ float red[4];
+    __shared__ float s_cs[2][2][128];
     const PagedKv &kv = a.kv;
-    const int rows = a.n_heads + kv.n_kv, hd = kv.hd, half = hd >> 1, i = threadIdx.x;
-    const int t = blockIdx.x / rows, h = blockIdx.x - t * rows;
-    const bool is_q = h < a.n_heads;
-    const int head = is_q ? h : h - a.n_heads;
-    const int b = a.seq ? a.seq[t] : t;
-    if (static_cast<unsigned>(b) >= static_cast<unsigned>(kv.n_seqs)) {
-        if (i == 0) atomicExch(kv.err, kErrBadPos);
-        if (is_q)
-            for (int c = i; c < hd; c += 128) a.q_out[(static_cast<long long>(t) * a.n_heads + head) * hd + c] = 0.f;
-        return;
-    }
-    const int r = a.row ? a.row[t] : kv.lens[b] - 1;
-    if (r < 0) {   // padding, or an empty slot
-        if (is_q)
-            for (int c = i; c < hd; c += 128) a.q_out[(static_cast<long long>(t) * a.n_heads + head) * hd + c] = 0.f;
-        return;
-    }
-    const float *src = is_q ? a.q + t * a.q_stride + static_cast<long long>(head) * hd
-                            : a.k + t * a.k_stride + static_cast<long long>(head) * hd;
-    const float *w = is_q ? a.q_norm : a.k_norm;
-    const bool on = i < half;
-    float x0 = on ? src[i] : 0.f, x1 = on ? src[i + half] : 0.f;
-    if (w) {
-        float ss = warp_sum(x0 * x0 + x1 * x1);
-        if ((i & 31) == 0) red[i >> 5] = ss;
-        __syncthreads();
-        ss = red[0] + red[1] + red[2] + red[3];
-        const float scale = 1.0f / sqrtf(ss / static_cast<float>(hd) + a.eps);
-        if (on) {
-            x0 = x0 * scale * w[i];
-            x1 = x1 * scale * w[i + half];
+    const int hd = kv.hd, half = hd >> 1, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rows = a.n_heads + 2 * kv.n_kv;
+    const double turn = tid < half ? exp2(a.log2_base * tid) * 0.15915494309189535 : 0.0;   // 1 / 2 pi
+    pdl_wait();
+    int buf = 0;
+    for (int t = blockIdx.x; t < a.n_tokens; t += gridDim.x, buf ^= 1) {
+        const int b = a.seq ? __ldg(a.seq + t) : t, pos = __ldg(a.pos + t);
+        const bool seq_ok = static_cast<unsigned>(b) < static_cast<unsigned>(kv.n_seqs);
+        const int r = !seq_ok ? -1 : a.row ? __ldg(a.row + t) : __ldg(kv.lens + b) - 1;
+        bool row_ok = r >= 0 && r < (static_cast<long long>(kv.max_pages) << kv.page_shift);
+        const long long off = row_ok ? paged_off(kv, b, 0, r) : -1;   // of kv head 0
+        row_ok = off >= 0;
+        if (tid == 0 && blockIdx.y == 0 && (!seq_ok || (r >= 0 && !row_ok))) atomicExch(kv.err, kErrBadPos);
+        if (tid < half) {
+            const double x = pos * turn, f = x - rint(x);
+            float s, c;
+            sincospif(static_cast<float>(2.0 * f), &s, &c);
+            s_cs[buf][0][tid] = c;
+            s_cs[buf][1][tid] = s;
         }
-    }
-    long long off = 0;
-    if (!is_q) {
-        off = r < (static_cast<long long>(kv.max_pages) << kv.page_shift) ? paged_off(kv, b, head, r) : -1;
-        if (off < 0) {
-            if (i == 0) atomicExch(kv.err, kErrBadPos);
-            return;
-        }
-        const float *vh = a.v + t * a.v_stride + static_cast<long long>(head) * hd;
-        T *vrow = static_cast<T *>(kv.v) + off;
-        for (int c = i; c < hd; c += 128) vrow[c] = from_f<T>(vh[c]);
-    }
-    if (on) {
-        double sn, cs;
-        sincos(static_cast<double>(a.pos[t]) * pow(a.theta_scale, static_cast<double>(i)), &sn, &cs);
-        const float c = static_cast<float>(cs), s = static_cast<float>(sn);
-        const float y0 = x0 * c - x1 * s, y1 = x0 * s + x1 * c;
-        if (is_q) {
-            float *o = a.q_out + (static_cast<long long>(t) * a.n_heads + head) * hd;
-            o[i] = y0;
-            o[i + half] = y1;
-        } else {
-            T *krow = static_cast<T *>(kv.k) + off;
-            krow[i] = from_f<T>(y0);
-            krow[i + half] = from_f<T>(y1);
+        __syncthreads();   // (the other buffer is free again: every warp has passed here once more since it read it)
+        for (int h0 = (blockIdx.y * (kAppThreads / 32) + warp) * kAppRows; h0 < rows;
+             h0 += gridDim.y * (kAppThreads / 32) * kAppRows) {
+            float2 x[kAppRows][K], y[kAppRows][K];
+#pragma unroll
+            for (int j = 0; j < kAppRows; j++) {
+                const int h = h0 + j;
+                if (h >= rows) break;
+                const float *src = h < a.n_heads             ? a.q + t * a.q_stride + static_cast<long long>(h) * hd
+                                   : h < a.n_heads + kv.n_kv ? a.k + t * a.k_stride + static_cast<long long>(h - a.n_heads) * hd
+                                                             : a.v + t * a.v_stride + static_cast<long long>(h - a.n_heads - kv.n_kv) * hd;
+#pragma unroll
+                for (int k = 0; k < K; k++) {
+                    const int i = 2 * lane + 64 * k;
+                    x[j][k] = y[j][k] = make_float2(0.f, 0.f);
+                    if (i < half) {
+                        if (vec) {
+                            x[j][k] = __ldcs(reinterpret_cast<const float2 *>(src + i));
+                            y[j][k] = __ldcs(reinterpret_cast<const float2 *>(src + half + i));
+                        } else {
+                            x[j][k] = make_float2(src[i], src[i + 1]);
+                            y[j][k] = make_float2(src[half + i], src[half + i + 1]);
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < kAppRows; j++) {
+                const int h = h0 + j;
+                if (h >= rows) break;
+                const bool is_q = h < a.n_heads, is_v = h >= a.n_heads + kv.n_kv;
+                const float *w = is_q ? a.q_norm : a.k_norm;
+                if (w && !is_v) {
+                    float ss = 0.f;
+#pragma unroll
+                    for (int k = 0; k < K; k++)
+                        ss += x[j][k].x * x[j][k].x + x[j][k].y * x[j][k].y + y[j][k].x * y[j][k].x + y[j][k].y * y[j][k].y;
+                    const float scale = 1.0f / sqrtf(warp_sum(ss) / static_cast<float>(hd) + a.eps);
+#pragma unroll
+                    for (int k = 0; k < K; k++) {
+                        const int i = 2 * lane + 64 * k;
+                        if (i < half) {
+                            x[j][k].x *= scale * __ldg(w + i);
+                            x[j][k].y *= scale * __ldg(w + i + 1);
+                            y[j][k].x *= scale * __ldg(w + half + i);
+                            y[j][k].y *= scale * __ldg(w + half + i + 1);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < K; k++) {
+                    const int i = 2 * lane + 64 * k;
+                    if (i >= half) continue;
+                    float2 u = x[j][k], v = y[j][k];
+                    if (!is_v) {
+                        const float2 c = *reinterpret_cast<const float2 *>(&s_cs[buf][0][i]);
+                        const float2 s = *reinterpret_cast<const float2 *>(&s_cs[buf][1][i]);
+                        u = make_float2(x[j][k].x * c.x - y[j][k].x * s.x, x[j][k].y * c.y - y[j][k].y * s.y);
+                        v = make_float2(x[j][k].x * s.x + y[j][k].x * c.x, x[j][k].y * s.y + y[j][k].y * c.y);
+                    }
+                    if (is_q) {
+                        if (r < 0) u = v = make_float2(0.f, 0.f);   // padding, or an empty slot
+                        float *o = a.q_out + (static_cast<long long>(t) * a.n_heads + h) * hd;
+                        store2(o + i, u.x, u.y);
+                        store2(o + half + i, v.x, v.y);
+                    } else if (row_ok) {
+                        const int head = h - a.n_heads - (is_v ? kv.n_kv : 0);
+                        T *o = static_cast<T *>(is_v ? kv.v : kv.k) + off + (static_cast<long long>(head) << kv.page_shift) * hd;
+                        store2(o + i, u.x, u.y);
+                        store2(o + half + i, v.x, v.y);
+                    }
+                }
+            }
         }
     }
 }
 
 // ------------------------------------------------------------ eviction
-constexpr int kEvThreads = 1024;
+constexpr int kEvThreads = 512, kEvWarps = kEvThreads / 32;
+constexpr int kEvSlice = 40960;   // keys that a CTA holds in shared memory
 
 // order of the weights as unsigned integers, larger first: protected rows
 // above all, NaN as -inf, -0 as +0
@@ -99,159 +157,264 @@ __device__ __forceinline__ uint32_t evict_key(float acc, int pos, int next_pos, 
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);   // +inf: 0xFF800000, below the protected rows' key
 }
 
-__device__ __forceinline__ int block_scan(int v, int *warps, int &total) {
+// what a cluster's CTAs write into each other
+struct EvictShared {
+    unsigned cnt[2][16][8];                      // [buffer][CTA][threshold]
+    unsigned ties[16], holes[16], movers[16];
+    unsigned w[2][kEvWarps][8], scan[kEvWarps];
+};
+
+// exclusive prefix over the CTA, and the total
+__device__ __forceinline__ unsigned cta_scan(unsigned v, unsigned *sh, unsigned &tot) {
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    int s = v;
+    unsigned s = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, s, o);
+        const unsigned u = __shfl_up_sync(0xffffffffu, s, o);
         if (lane >= o) s += u;
     }
-    if (lane == 31) warps[w] = s;
     __syncthreads();
-    if (w == 0) {
-        int x = warps[lane];
+    if (lane == 31) sh[w] = s;
+    __syncthreads();
+    unsigned x = lane < kEvWarps ? sh[lane] : 0;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int u = __shfl_up_sync(0xffffffffu, x, o);
-            if (lane >= o) x += u;
-        }
-        warps[lane] = x;
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned u = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += u;
     }
-    __syncthreads();
-    const int before = w ? warps[w - 1] : 0;
-    total = warps[31];
-    __syncthreads();
-    return before + s - v;   // exclusive
+    tot = __shfl_sync(0xffffffffu, x, 31);
+    const unsigned before = __shfl_sync(0xffffffffu, x, w ? w - 1 : 0);
+    return (w ? before : 0) + s - v;
 }
 
-// CTA (sequence, kv head): the key of the budget-th row by radix selection
-// (four digits of 8 bits, from the top), then, tile by tile in row order,
-// who stays: keys above the threshold, and the first rows at it.  Places
-// (rows below the budget that leave) and movers (rows beyond that stay) are
-// numbered as they come; place and mover i meet through the source list.
-__global__ void __launch_bounds__(kEvThreads) k_evict_select(PagedEvictArgs a) {
+// A cluster of C CTAs per line (sequence, kv head), each with a slice of its
+// rows, whose keys stay in shared memory (STAGED; else they are made again
+// from L2 each time).  The key of the budget-th row is found eightfold: seven
+// thresholds are counted at once, 11 rounds for 32 bits, one barrier each; no
+// atomics, so equal weights cost nothing extra.  Then rows are numbered in
+// order: who stays (keys above the threshold, the first rows at it), the
+// places below the budget that become free, the rows beyond it that stay;
+// the i-th of these moves into the i-th place.  Sources lie at or beyond the
+// budget, places below it, so no row is both.
+template <bool STAGED>
+__global__ void __launch_bounds__(kEvThreads) k_paged_evict(PagedEvictArgs a, int C, int row_bytes) {
+    extern __shared__ uint32_t keys[];
+    __shared__ EvictShared sh;
     pdl_trigger();
-    pdl_wait();
-    __shared__ unsigned hist[256];
-    __shared__ int warps[32];
-    __shared__ unsigned s_prefix;
-    __shared__ int s_need;
     const PagedKv &kv = a.kv;
-    const int b = blockIdx.x / kv.n_kv, j = blockIdx.x - b * kv.n_kv, tid = threadIdx.x;
-    const int n = paged_len(kv, b, tid == 0 && j == 0);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rank = C > 1 ? static_cast<int>(cluster_ctarank()) : 0, line_no = blockIdx.x / C;
+    const int b = line_no / kv.n_kv, j = line_no - b * kv.n_kv;
+    auto all_sync = [&] {
+        if (C > 1) {
+            cl_arrive();
+            cl_wait();
+        } else {
+            __syncthreads();
+        }
+    };
+    auto tell = [&](unsigned *slot, unsigned v, int to) {   // into CTA `to`'s copy of slot
+        if (C > 1) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cl_map(smem_addr(slot), to)), "r"(v) : "memory");
+        else *slot = v;
+    };
+    if (C > 1) cl_arrive_relaxed();   // the others have started: waited for before the first store to them
+    pdl_wait();
+    const int n = paged_len(kv, b, tid == 0 && j == 0 && rank == 0);
     const int left = min(n, a.budget);
-    const long long line = (static_cast<long long>(b) * kv.n_kv + j) * a.stride;
+    const long long line = static_cast<long long>(line_no) * a.stride;
     const float *acc = a.acc + line;
     const int32_t *pos = a.pos + line;
-    int32_t *src = a.src + (static_cast<long long>(b) * kv.n_kv + j) * a.budget;
-    if (j == 0 && tid == 0) a.lens_out[b] = left;
-    if (n <= a.budget) {
-        for (int r = tid; r < n; r += kEvThreads) src[r] = r;
+    if (j == 0 && tid == 0 && rank == 0) a.lens_out[b] = left;
+    const int slice = (((n + C - 1) / C) + 3) & ~3, lo = min(n, rank * slice), hi = min(n, lo + slice), len = hi - lo;
+    if (C > 1) cl_wait();
+    if (n <= a.budget) {   // all stay (every CTA of the cluster comes here)
+        for (int r = lo + tid; r < hi; r += kEvThreads) {
+            a.acc_out[line + r] = acc[r];
+            a.pos_out[line + r] = pos[r];
+        }
         return;
     }
-    const int np = a.next_pos[b];
-    if (tid == 0) {
-        s_prefix = 0;
-        s_need = left;
+    const int np = __ldg(a.next_pos + b);
+    if (STAGED) {
+#pragma unroll 4
+        for (int i = tid; i < len; i += kEvThreads) keys[i] = evict_key(acc[lo + i], pos[lo + i], np, a.n_recent, a.n_sink);
+        __syncthreads();
     }
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256) hist[tid] = 0;
-        __syncthreads();
-        const unsigned prefix = s_prefix;
-        const int need = s_need;
-        for (int r = tid; r < n; r += kEvThreads) {
-            const uint32_t k = evict_key(acc[r], pos[r], np, a.n_recent, a.n_sink);
-            if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255], 1u);
+    auto key_at = [&](int i) { return STAGED ? keys[i] : evict_key(acc[lo + i], pos[lo + i], np, a.n_recent, a.n_sink); };
+    // ---------------- threshold: at least `left` keys are >= t0, fewer are >= t1
+    unsigned long long t0 = 0, t1 = 1ull << 32;
+    unsigned above = 0;                                    // keys >= t1
+    for (int buf = 0; t1 - t0 > 1; buf ^= 1) {
+        const unsigned long long w = t1 - t0;
+        unsigned th[7], c[7];
+#pragma unroll
+        for (int i = 0; i < 7; i++) {
+            th[i] = static_cast<unsigned>(t0 + (w * (i + 1)) / 8);
+            c[i] = 0;
         }
+        for (int i = tid; i < len; i += kEvThreads) {
+            const uint32_t k = key_at(i);
+#pragma unroll
+            for (int z = 0; z < 7; z++) c[z] += k >= th[z];
+        }
+        unsigned mine = 0;
+#pragma unroll
+        for (int z = 0; z < 7; z++) {
+            const unsigned s = __reduce_add_sync(0xffffffffu, c[z]);
+            if (lane == z) mine = s;
+        }
+        if (lane < 7) sh.w[buf][warp][lane] = mine;
         __syncthreads();
-        if (tid == 0) {
-            int above = 0, d = 255;
-            for (; d > 0; d--) {
-                if (above + static_cast<int>(hist[d]) >= need) break;
-                above += static_cast<int>(hist[d]);
+        // lane z of every warp: the CTA's count of threshold z
+        unsigned tot = 0;
+        if (lane < 7)
+#pragma unroll
+            for (int q = 0; q < kEvWarps; q++) tot += sh.w[buf][q][lane];
+        if (C > 1) {
+            if (warp < C && lane < 7) tell(&sh.cnt[buf][rank][lane], tot, warp);
+            all_sync();
+            tot = 0;
+            if (lane < 7)
+                for (int q = 0; q < C; q++) tot += sh.cnt[buf][q][lane];
+        }
+        // thresholds rise, counts fall: the last that still reaches `left`
+        const unsigned reach = __ballot_sync(0xffffffffu, lane < 7 && tot >= static_cast<unsigned>(left));
+        const int z = __popc(reach) - 1;
+        const unsigned long long n0 = t0 + (w * (z + 1)) / 8, n1 = t0 + (w * (z + 2)) / 8;
+        if (z < 6) above = __shfl_sync(0xffffffffu, tot, z + 1);
+        t1 = z < 6 ? n1 : t1;
+        t0 = z < 0 ? t0 : n0;
+    }
+    const uint32_t thr = static_cast<uint32_t>(t0);
+    const unsigned ties = static_cast<unsigned>(left) - above;   // of the rows at thr, the first `ties` stay
+    // ---------------- numbering, in row order: ties, then places and movers
+    unsigned n_ties = 0;
+    for (int i = tid; i < len; i += kEvThreads) n_ties += key_at(i) == thr;
+    unsigned tot;
+    cta_scan(n_ties, sh.scan, tot);
+    if (tid < C) tell(&sh.ties[rank], tot, tid);
+    all_sync();
+    unsigned tie0 = 0;
+    for (int q = 0; q < rank; q++) tie0 += sh.ties[q];
+    // pass 0 counts this slice's places and movers, pass 1 lists them
+    unsigned hole0 = 0, mover0 = 0;
+    for (int pass = 0; pass < 2; pass++) {
+        unsigned t_run = tie0, h_run = hole0, m_run = mover0;
+        for (int base = 0; base < len; base += kEvThreads) {
+            const int i = base + tid, r = lo + i;
+            const bool in = i < len;
+            const uint32_t k = in ? key_at(i) : 0u;
+            const unsigned tr = cta_scan(in && k == thr, sh.scan, tot);
+            const bool stay = in && (k > thr || (k == thr && t_run + tr < ties));
+            t_run += tot;
+            const bool hole = in && r < left && !stay, mover = in && r >= left && stay;
+            // (a tile's places and movers in one scan: counts below 2^16)
+            const unsigned hm = cta_scan((hole ? 1u : 0u) | (mover ? 1u << 16 : 0u), sh.scan, tot);
+            if (pass == 1) {
+                int32_t *lists = a.places + static_cast<long long>(line_no) * a.budget;
+                if (hole) lists[h_run + (hm & 0xFFFFu)] = r;
+                if (mover) (a.src + static_cast<long long>(line_no) * a.budget)[m_run + (hm >> 16)] = r;
+                if (in && r < left && stay) {
+                    a.acc_out[line + r] = acc[r];
+                    a.pos_out[line + r] = pos[r];
+                }
             }
-            s_prefix = prefix | (static_cast<unsigned>(d) << shift);
-            s_need = need - above;   // rows to take at the threshold digit
+            h_run += tot & 0xFFFFu;
+            m_run += tot >> 16;
         }
-        __syncthreads();
-    }
-    const unsigned thr = s_prefix;
-    const int ties = s_need;   // of the rows equal to thr, the first `ties` stay
-    int tie0 = 0, place0 = 0, mover0 = 0;
-    // pass 1: places, in order, into the source list's tail end (as row
-    // numbers); pass 2: movers.  Both lists are as long: the i-th mover goes
-    // to the i-th place.
-    for (int base = 0; base < n; base += kEvThreads) {
-        const int r = base + tid;
-        const bool in = r < n;
-        const uint32_t k = in ? evict_key(acc[r], pos[r], np, a.n_recent, a.n_sink) : 0u;
-        int tot;
-        const int tr = block_scan(in && k == thr, warps, tot);
-        const bool stay = in && (k > thr || (k == thr && tie0 + tr < ties));
-        tie0 += tot;
-        const bool place = in && r < left && !stay, mover = in && r >= left && stay;
-        const int pr = block_scan(place, warps, tot);
-        if (place) a.places[(static_cast<long long>(b) * kv.n_kv + j) * a.budget + place0 + pr] = r;
-        place0 += tot;
-        const int mr = block_scan(mover, warps, tot);
-        if (in && r < left && stay) src[r] = r;
-        __syncthreads();   // every place of a tile is listed before a later tile's mover reads it
-        if (mover) src[a.places[(static_cast<long long>(b) * kv.n_kv + j) * a.budget + mover0 + mr]] = r;
-        mover0 += tot;
-    }
-}
-
-// CTA (sequence, kv head, part of the budget): weights and positions of the
-// rows that stay, and K and V of those that move.  Sources lie at or beyond
-// the budget, places below it, so no row is both.
-template <class T>
-__global__ void __launch_bounds__(256) k_evict_move(PagedEvictArgs a) {
-    pdl_trigger();
-    pdl_wait();
-    const PagedKv &kv = a.kv;
-    const int b = blockIdx.x / kv.n_kv, j = blockIdx.x - b * kv.n_kv;
-    const int n = paged_len(kv, b, false);
-    const int left = min(n, a.budget);
-    const long long head = static_cast<long long>(b) * kv.n_kv + j;
-    const int32_t *src = a.src + head * a.budget;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int r = blockIdx.y * 8 + warp; r < left; r += gridDim.y * 8) {
-        const int s = src[r];
-        if (lane == 0) {
-            a.acc_out[head * a.stride + r] = a.acc[head * a.stride + s];
-            a.pos_out[head * a.stride + r] = a.pos[head * a.stride + s];
-        }
-        if (s == r) continue;
-        const long long from = paged_off(kv, b, j, s), to = paged_off(kv, b, j, r);
-        if (from < 0 || to < 0) {
-            if (lane == 0) atomicExch(kv.err, kErrBadPos);
-            continue;
-        }
-        const T *k = static_cast<const T *>(kv.k), *v = static_cast<const T *>(kv.v);
-        for (int c = lane; c < kv.hd; c += 32) {
-            static_cast<T *>(kv.k)[to + c] = k[from + c];
-            static_cast<T *>(kv.v)[to + c] = v[from + c];
+        if (pass == 0) {
+            if (tid < C) {
+                tell(&sh.holes[rank], h_run, tid);
+                tell(&sh.movers[rank], m_run, tid);
+            }
+            all_sync();
+            for (int q = 0; q < rank; q++) {
+                hole0 += sh.holes[q];
+                mover0 += sh.movers[q];
+            }
         }
     }
+    all_sync();   // the lists are complete (and visible: release and acquire at cluster scope)
+    unsigned moves = 0;
+    for (int q = 0; q < C; q++) moves += sh.movers[q];
+    // ---------------- moves: a row's K and V by 16-byte pieces, half a warp each where they are 256 bytes
+    const int32_t *from_l = a.src + static_cast<long long>(line_no) * a.budget;
+    const int32_t *to_l = a.places + static_cast<long long>(line_no) * a.budget;
+    const int pieces = row_bytes / 16, size = row_bytes / kv.hd;
+    for (unsigned i0 = (rank * kEvWarps + warp) * 4; i0 < moves; i0 += C * kEvWarps * 4) {
+        long long from[4], to[4];
+#pragma unroll
+        for (int z = 0; z < 4; z++) {
+            from[z] = to[z] = -1;
+            if (i0 + z < moves) {
+                const int s = __ldcg(from_l + i0 + z), d = __ldcg(to_l + i0 + z);
+                if (lane == 0) {
+                    a.acc_out[line + d] = acc[s];
+                    a.pos_out[line + d] = pos[s];
+                }
+                from[z] = paged_off(kv, b, j, s);
+                to[z] = paged_off(kv, b, j, d);
+                if ((from[z] < 0 || to[z] < 0) && lane == 0) atomicExch(kv.err, kErrBadPos);
+            }
+        }
+        for (int p = lane; p < 2 * pieces; p += 32) {
+            char *pool = static_cast<char *>(p < pieces ? kv.k : kv.v);
+            const int at = (p < pieces ? p : p - pieces) * 16;
+            uint4 v[4];
+#pragma unroll
+            for (int z = 0; z < 4; z++)
+                if (from[z] >= 0 && to[z] >= 0) v[z] = *reinterpret_cast<const uint4 *>(pool + from[z] * size + at);
+#pragma unroll
+            for (int z = 0; z < 4; z++)
+                if (from[z] >= 0 && to[z] >= 0) *reinterpret_cast<uint4 *>(pool + to[z] * size + at) = v[z];
+        }
+    }
+    if (C > 1) all_sync();   // no CTA leaves while another reads its counts
 }
 
 }  // namespace
 
-cudaError_t launch_paged_append(const PagedAppendArgs &a, cudaStream_t st) {
-    const dim3 grid(static_cast<unsigned>(a.n_tokens) * (a.n_heads + a.kv.n_kv)), block(128);
-    if (a.kv.dtype == STYX_F16) return launch_pdl(k_paged_append<__half>, grid, block, 0, st, a);
-    if (a.kv.dtype == STYX_BF16) return launch_pdl(k_paged_append<__nv_bfloat16>, grid, block, 0, st, a);
-    return launch_pdl(k_paged_append<float>, grid, block, 0, st, a);
+cudaError_t launch_paged_append(const PagedAppendArgs &a, int sms, cudaStream_t st) {
+    const int rows = a.n_heads + 2 * a.kv.n_kv, per = kAppThreads / 32 * kAppRows;
+    // few tokens: their rows over several CTAs; many: eight CTAs per SM take them in turn
+    const int parts = std::max(1, std::min((rows + per - 1) / per, 2 * sms / a.n_tokens));
+    const dim3 grid(static_cast<unsigned>(std::min(a.n_tokens, 8 * sms)), static_cast<unsigned>(parts));
+    auto al8 = [](const void *p, long long s) { return (reinterpret_cast<uintptr_t>(p) & 7) == 0 && s % 2 == 0; };
+    const bool vec = al8(a.q, a.q_stride) && al8(a.k, a.k_stride) && al8(a.v, a.v_stride);
+    const bool two = a.kv.hd > 128;
+    const dim3 block(kAppThreads);
+    if (a.kv.dtype == STYX_F16)
+        return two ? launch_pdl(k_paged_append<__half, 2>, grid, block, 0, st, a, vec) : launch_pdl(k_paged_append<__half, 1>, grid, block, 0, st, a, vec);
+    if (a.kv.dtype == STYX_BF16)
+        return two ? launch_pdl(k_paged_append<__nv_bfloat16, 2>, grid, block, 0, st, a, vec)
+                   : launch_pdl(k_paged_append<__nv_bfloat16, 1>, grid, block, 0, st, a, vec);
+    return two ? launch_pdl(k_paged_append<float, 2>, grid, block, 0, st, a, vec) : launch_pdl(k_paged_append<float, 1>, grid, block, 0, st, a, vec);
 }
 
 cudaError_t launch_paged_evict(const PagedEvictArgs &a, cudaStream_t st) {
-    const unsigned lines = static_cast<unsigned>(a.kv.n_seqs) * a.kv.n_kv;
-    cudaError_t e = launch_pdl(k_evict_select, dim3(lines), dim3(kEvThreads), 0, st, a);
+    const long long rows = static_cast<long long>(a.kv.max_pages) << a.kv.page_shift;
+    int C = 1;
+    while (C < 8 && rows > 4096ll * C) C <<= 1;
+    const long long slice = ((rows + C - 1) / C + 3) & ~3ll;
+    const bool staged = slice <= kEvSlice;
+    const int row_bytes = a.kv.hd * (a.kv.dtype == STYX_F32 ? 4 : 2);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(a.kv.n_seqs) * a.kv.n_kv * C);
+    cfg.blockDim = dim3(kEvThreads);
+    cfg.dynamicSmemBytes = staged ? static_cast<size_t>(slice) * 4 : 0;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = C;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = C > 1 ? 2 : 1;
+    if (!staged) return cudaLaunchKernelEx(&cfg, k_paged_evict<false>, a, C, row_bytes);
+    const cudaError_t e = cudaFuncSetAttribute(k_paged_evict<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kEvSlice * 4);
     if (e != cudaSuccess) return e;
-    const dim3 grid(lines, static_cast<unsigned>(min(64, (a.budget + 7) / 8)));
-    if (a.kv.dtype == STYX_F32) return launch_pdl(k_evict_move<uint32_t>, grid, dim3(256), 0, st, a);
-    return launch_pdl(k_evict_move<uint16_t>, grid, dim3(256), 0, st, a);
+    return cudaLaunchKernelEx(&cfg, k_paged_evict<true>, a, C, row_bytes);
 }
 
 }  // namespace styx

@@ -122,12 +122,13 @@ int styx_paged_append(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv
                       int64_t v_stride, const float *q_norm, const float *k_norm, float eps, float freq_base,
                       const int32_t *pos, const int32_t *seq, const int32_t *row, float *q_out) {
     styx::PagedAppendArgs a{};
-    CHECK(styx::ctx_enter(ctx, nullptr, &a.kv.err));
+    int sms = 0;
+    CHECK(styx::ctx_enter(ctx, &sms, &a.kv.err));
     CHECK(check_kv(kv, true, a.kv));
     NEED(n_tokens > 0 && n_heads >= 0 && static_cast<int64_t>(n_tokens) * (n_heads + kv->n_kv_heads) < (int64_t(1) << 31),
          "n_tokens %d, n_heads %d", n_tokens, n_heads);
     NEED(seq || n_tokens <= kv->n_seqs, "%d tokens without seq for %d sequences", n_tokens, kv->n_seqs);
-    NEED(kv->head_dim % 2 == 0, "head_dim %d: even needed", kv->head_dim);
+    NEED(aligned(q_out, 16), "q_out must be 16-byte aligned");
     const int64_t qd = static_cast<int64_t>(n_heads) * kv->head_dim, kd = static_cast<int64_t>(kv->n_kv_heads) * kv->head_dim;
     NEED(k && v && pos && (n_heads == 0 || (q && q_out)), "null pointer");
     NEED((n_heads == 0 || q_stride >= qd) && k_stride >= kd && v_stride >= kd, "a token stride smaller than its heads");
@@ -153,14 +154,14 @@ int styx_paged_append(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv
     a.q_norm = q_norm;
     a.k_norm = k_norm;
     a.eps = eps;
-    a.theta_scale = std::pow(static_cast<double>(freq_base), -2.0 / static_cast<double>(kv->head_dim));
+    a.log2_base = -2.0 / static_cast<double>(kv->head_dim) * std::log2(static_cast<double>(freq_base));
     a.pos = pos;
     a.seq = seq;
     a.row = row;
     a.q_out = q_out;
     a.n_tokens = n_tokens;
     a.n_heads = n_heads;
-    CK(styx::launch_paged_append(a, S(stream)));
+    CK(styx::launch_paged_append(a, sms, S(stream)));
     return STYX_OK;
 }
 
