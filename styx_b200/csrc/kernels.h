@@ -419,6 +419,7 @@ struct SampleArgs {
     const float *top_p, *min_p;    // each may be null
     int32_t *token;
     float *logprob;                // may be null
+    int *err;                      // device error word
 };
 cudaError_t launch_paged_append(const PagedAppendArgs &a, int sms, cudaStream_t st);
 // attention on the FMA units; on the tensor cores (mk, mv map the pools as

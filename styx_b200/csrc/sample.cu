@@ -7,14 +7,23 @@
 // largest one's), so every sum is exact whatever its order.
 //
 // k_sample_cluster (n_vocab <= 262144): a cluster of eight CTAs per row holds
-// the row in shared memory, so the logits are read once.  One histogram over
-// 2048 equal steps of log weight (tokens below e^-28 have weight 0 and take
-// no part in anything) shows the step in which the threshold lies.  Where the
-// tokens down to there are at most 512, they go to the cluster's first CTA,
-// which sorts them and does the rest; else only that step's tokens go there,
-// the threshold comes back, and every CTA sums its kept tokens for the draw.
-// Only more than 512 tokens in one step (a flat row) are resolved by
-// bisection of the key.  (The row in registers, 1024 threads of 64, spilled.)
+// the row in shared memory, so the logits are read once.
+//   top-k up to 120: the k-th largest of the cluster's 128 warps' maxima is a
+//     bound that the k-th largest logit reaches; the tokens at or above it
+//     (22 on average for k = 20, 355 for 120, where large ones are spread
+//     evenly) go to the cluster's first CTA, which sorts them and does the rest.
+//   else, with top-k or top-p: one histogram over 2048 equal steps of log
+//     weight (tokens below e^-28 have weight 0 and take no part in anything)
+//     shows the step in which the threshold lies.  Where the tokens down to
+//     there are at most 512 they go to the first CTA as above; else only that
+//     step's tokens go there and the threshold comes back.  Top-p after such
+//     a top-k is a second histogram, of the tokens kept.  Only more than 512
+//     tokens in one step (a flat row) are resolved by bisection of the key.
+//   the draw, where it is not the first CTA's: sums of the kept weights per
+//     warp, each over a stretch of indexes of its own, then inside one warp.
+// (The row in registers, 1024 threads of 64, spilled; a conversion of the
+// weights by F2I and sums per round of the CTA made the draw of an unfiltered
+// row 18000 of 34000 cycles.)
 //
 // k_sample (larger vocabularies): one CTA per row, radix selection from L2.
 #include <cuda_runtime.h>
@@ -40,6 +49,14 @@ __device__ __forceinline__ u64 part_of(u64 of, u64 total) {
     return (total >> 24) * of + (((total & 0xFFFFFFu) * of) >> 24);
 }
 
+// floor(w 2^40) for 0 <= w <= 1, by its bits (a conversion to 64 bits costs
+// several times the shift)
+__device__ __forceinline__ u64 whole_of(float w) {
+    const uint32_t b = __float_as_uint(w), e = b >> 23, f = (b & 0x7FFFFFu) | 0x800000u;
+    if (e >= 110) return static_cast<u64>(f) << (e - 110);
+    return e >= 87 ? f >> (110 - e) : 0u;
+}
+
 struct Row {
     const float *x;
     float m, inv_t;
@@ -49,7 +66,7 @@ struct Row {
         if (v == -INFINITY) return 0.f;   // an infinite temperature included
         return hot ? expf((v - m) * inv_t) : 0.f;
     }
-    __device__ __forceinline__ u64 whole(float v) const { return static_cast<u64>(weight(v) * 0x1p40f); }
+    __device__ __forceinline__ u64 whole(float v) const { return whole_of(weight(v)); }
 };
 
 template <class V>
@@ -242,12 +259,13 @@ constexpr int kNT = 512, kNW = kNT / 32;    // threads and warps of a CTA
 constexpr int kBins = 4 * kNT, kCap = kNT;
 constexpr float kBinScale = kBins / 28.f;
 constexpr int kSlice = 32768;               // logits of a CTA at most
-constexpr int kEnt = kSlice / (4 * kNT) * kNW;
+constexpr int kTopK = 120;                  // top-k by the warps' maxima (128 of them)
 
 struct Exchange {                           // what the cluster's CTAs write into each other
-    float top[kC];
+    float top[kC * kNW];
     u64 sum[2][kC];
     unsigned cnt[2][kC];
+    unsigned n_of[kC];                      // candidates of each CTA
     unsigned n_cand, thr;
     u64 ties;
     u64 cand[kCap];                         // (inverted key << 32) | index: ascending = the order of the tokens
@@ -255,8 +273,10 @@ struct Exchange {                           // what the cluster's CTAs write int
 struct CtaShared {
     Exchange xc;
     unsigned cnt[kBins], lo[kBins], hi[kBins];
-    u64 red[32], buf[kNT], ent[2][kEnt + 1];
-    float redf[32];
+    u64 red[32], buf[kNT], ent[2][kNW + 1];
+    uint64_t bar;
+    float bound;
+    unsigned n_mine;
     int step, upto;
     u64 before, in_step;
 };
@@ -344,65 +364,72 @@ __device__ __forceinline__ u64 cta_sort(u64 v, int n, u64 *buf) {
     return v;
 }
 
-__global__ void __launch_bounds__(kNT, 2) k_sample_cluster(SampleArgs a, int slice, bool vec) {
-    extern __shared__ __align__(16) float xs[];   // [slice], cleaned
+// slice: logits of a CTA, kNW * region of them, a warp's stretch each (region
+// a multiple of 128).  bulk: the slices start on 16 bytes, and one bulk copy
+// brings a CTA's.
+__global__ void __launch_bounds__(kNT, 2) k_sample_cluster(SampleArgs a, int region, bool bulk) {
+    extern __shared__ __align__(128) float xs[];
     __shared__ __align__(16) CtaShared sh;
     pdl_trigger();
     cl_arrive_relaxed();                          // the others have started: waited for before the first store to them
     Exchange &xc = sh.xc;
     const uint32_t rank = cluster_ctarank();
     const int b = blockIdx.x / kC, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n = a.n_vocab;
-    const int lo = static_cast<int>(rank) * slice, len = max(0, min(n - lo, slice));
+    const int slice = kNW * region, lo = static_cast<int>(rank) * slice, len = max(0, min(n - lo, slice));
+    const int first = warp * region;              // the warp's stretch of the slice
     auto peer = [&](const void *p, uint32_t r) { return cl_map(smem_addr(p), r); };
     const uint4 z4 = make_uint4(0, 0, 0, 0);
     reinterpret_cast<uint4 *>(sh.cnt)[tid] = z4;
     reinterpret_cast<uint4 *>(sh.lo)[tid] = z4;
     reinterpret_cast<uint4 *>(sh.hi)[tid] = z4;
-    if (tid == 0) xc.n_cand = 0;
-    pdl_wait();
-    // ---------------- the slice, once; its maximum
-    const float *src = a.logits + b * a.row_stride + lo;
-    float m = -INFINITY;
-#pragma unroll 5
-    for (int i = 4 * tid; i < slice; i += 4 * kNT) {
-        float4 v;
-        if (vec && i + 4 <= len) {
-            v = __ldcs(reinterpret_cast<const float4 *>(src + i));
-        } else {
-            v.x = i < len ? src[i] : -INFINITY;
-            v.y = i + 1 < len ? src[i + 1] : -INFINITY;
-            v.z = i + 2 < len ? src[i + 2] : -INFINITY;
-            v.w = i + 3 < len ? src[i + 3] : -INFINITY;
-        }
-        v = make_float4(clean(v.x), clean(v.y), clean(v.z), clean(v.w));
-        *reinterpret_cast<float4 *>(xs + i) = v;
-        m = fmaxf(m, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
+    if (tid == 0) {
+        xc.n_cand = 0;
+        sh.n_mine = 0;
+        mbar_init(&sh.bar, 1);
+        fence_mbar_init();
     }
+    pdl_wait();
+    // ---------------- the slice, once; the warps' maxima
+    const float *src = a.logits + b * a.row_stride + lo;
+    const int whole4 = bulk ? len & ~3 : 0;
+    if (tid == 0 && whole4) {
+        mbar_arrive_expect_tx(&sh.bar, static_cast<uint32_t>(whole4) * 4);
+        bulk_g2s(xs, src, static_cast<uint32_t>(whole4) * 4, &sh.bar);
+    }
+    const float t = a.temperature ? __ldg(a.temperature + b) : 1.f, top_p = a.top_p ? __ldg(a.top_p + b) : 1.f;
+    const float min_p = a.min_p ? __ldg(a.min_p + b) : 0.f, u = __ldg(a.u + b);
+    int k = a.top_k ? __ldg(a.top_k + b) : 0;
+    for (int i = whole4 + tid; i < slice; i += kNT) xs[i] = i < len ? src[i] : -INFINITY;
+    __syncthreads();
+    if (whole4) mbar_wait(&sh.bar, 0, a.err, kErrWaitFull);
     Row row;
     row.x = nullptr;
-    const float t = a.temperature ? a.temperature[b] : 1.f;
     row.hot = t > 0.f;
     row.inv_t = 1.0f / t;
-    int k = a.top_k ? a.top_k[b] : 0;
-    const float p = a.top_p ? fminf(a.top_p[b], 1.f) : 1.f;
+    const float p = fminf(top_p, 1.f), mp = fminf(min_p, 1.f);   // the maximum always stays
     const u64 p24 = p > 0.f ? static_cast<u64>(rintf(p * 0x1p24f)) : 0ull;
-    const float mp = a.min_p ? fminf(a.min_p[b], 1.f) : 0.f;   // the maximum always stays
-    const u64 u24 = static_cast<u64>(fminf(fmaxf(a.u[b], 0.f), 0x1.fffffep-1f) * 0x1p24f);
+    const u64 u24 = static_cast<u64>(fminf(fmaxf(u, 0.f), 0x1.fffffep-1f) * 0x1p24f);
+    float m = -INFINITY;
+#pragma unroll 4
+    for (int i = first + 4 * lane; i < first + region; i += 128) {
+        const float4 v = *reinterpret_cast<const float4 *>(xs + i);
+        const float4 c = make_float4(clean(v.x), clean(v.y), clean(v.z), clean(v.w));
+        const uint4 d = make_uint4(__float_as_uint(v.x) ^ __float_as_uint(c.x), __float_as_uint(v.y) ^ __float_as_uint(c.y),
+                                   __float_as_uint(v.z) ^ __float_as_uint(c.z), __float_as_uint(v.w) ^ __float_as_uint(c.w));
+        if (d.x | d.y | d.z | d.w) *reinterpret_cast<float4 *>(xs + i) = c;
+        m = fmaxf(m, fmaxf(fmaxf(c.x, c.y), fmaxf(c.z, c.w)));
+    }
 #pragma unroll
     for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (lane == 0) sh.redf[warp] = m;
-    __syncthreads();
     cl_wait();
-    if (warp == 0) {
-        m = lane < kNW ? sh.redf[lane] : -INFINITY;
+    if (lane < kC) cl_st(peer(&xc.top[rank * kNW + warp], lane), m);
+    cluster_sync();
+    {
+        const float4 v = reinterpret_cast<const float4 *>(xc.top)[lane];   // 128 maxima, four a lane
+        m = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
 #pragma unroll
         for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        if (lane < kC) cl_st(peer(&xc.top[rank], lane), m);
     }
-    cluster_sync();
-    m = xc.top[0];
-#pragma unroll
-    for (int i = 1; i < kC; i++) m = fmaxf(m, xc.top[i]);
     row.m = m;
     if (!(m > -INFINITY)) {   // nothing to draw from
         if (rank == 0 && tid == 0) {
@@ -416,7 +443,8 @@ __global__ void __launch_bounds__(kNT, 2) k_sample_cluster(SampleArgs a, int sli
     const bool by_k = k < n, by_p = p24 < (1ull << 24);
     // all of the slice's logits, (place in the slice, logit)
     auto each = [&](auto f) {
-        for (int i = 4 * tid; i < slice; i += 4 * kNT) {
+#pragma unroll 2
+        for (int i = first + 4 * lane; i < first + region; i += 128) {
             const float4 v = *reinterpret_cast<const float4 *>(xs + i);
             f(i, v.x);
             f(i + 1, v.y);
@@ -424,23 +452,140 @@ __global__ void __launch_bounds__(kNT, 2) k_sample_cluster(SampleArgs a, int sli
             f(i + 3, v.w);
         }
     };
-    // the step of a token: kBins or more where the weight is 0
-    const float bs = row.inv_t * kBinScale;
-    auto step_of = [&](float v) {
-        return v == m ? 0 : row.hot && v > -INFINITY ? static_cast<int>(fminf((m - v) * bs, kBins)) : kBins;
-    };
     auto finish = [&](int i, float v, u64 total) {   // by the thread that has the token
         a.token[b] = i;
         if (a.logprob)
             a.logprob[b] = (v == m ? 0.f : (v - m) * row.inv_t) - logf(static_cast<float>(total) * 0x1p-40f);
     };
+    auto as_cand = [&](int i, float v) {
+        return (static_cast<u64>(~key_of(v)) << 32) | static_cast<unsigned>(lo + i);
+    };
+    // the first CTA, with nc candidates (cand(i), any order) among which is all that is kept: sorted, top-k and top-p
+    // keep the first ones, min-p too; then the draw in index order.  need_p: top-p's sum, where it is known.
+    auto solve = [&](int nc, auto cand, bool p_known, u64 need_p) {
+        int n2 = 32;
+        while (n2 < nc) n2 <<= 1;
+        const u64 v = cta_sort(tid < nc ? cand(tid) : ~0ull, n2, sh.buf);
+        const uint32_t key = ~static_cast<uint32_t>(v >> 32);
+        const float xv = logit_of_key(key);
+        const bool in = tid < nc && tid < k;
+        const u64 w = in ? row.whole(xv) : 0ull;
+        bool kept = in && row.weight(xv) >= mp;
+        u64 tot;
+        if (by_p) {
+            const u64 before = cta_prefix(w, sh.red, tot);
+            kept = kept && before < (p_known ? need_p : max(part_of(p24, tot), 1ull));
+        }
+        const u64 z = cta_sort(kept ? ((v & 0xFFFFFFFFull) << 32) | key : ~0ull, n2, sh.buf);
+        const float zx = logit_of_key(static_cast<uint32_t>(z));
+        const u64 zw = z != ~0ull ? row.whole(zx) : 0ull, zb = cta_prefix(zw, sh.red, tot), target = part_of(u24, tot);
+        if (zb <= target && target < zb + zw) finish(static_cast<int>(z >> 32), zx, tot);
+    };
     uint32_t thr = 0;          // kept: keys above thr, and the first `ties` at it
     u64 ties = 0;
-    if (by_k || by_p) {
-        const bool weigh = !by_k;
+    if (by_k && k <= kTopK) {
+        // the k-th largest of the 128 maxima: thread t counts those before maximum t
+        if (tid < kC * kNW) {
+            const float mine = xc.top[tid];
+            int before = 0;
+#pragma unroll 8
+            for (int i = 0; i < kC * kNW; i += 4) {
+                const float4 v = *reinterpret_cast<const float4 *>(&xc.top[i]);
+                before += (v.x > mine || (v.x == mine && i < tid)) + (v.y > mine || (v.y == mine && i + 1 < tid)) +
+                          (v.z > mine || (v.z == mine && i + 2 < tid)) + (v.w > mine || (v.w == mine && i + 3 < tid));
+            }
+            if (before == k - 1) sh.bound = mine;
+        }
+        __syncthreads();
+        const float bound = sh.bound;
+        constexpr unsigned kSeg = kCap / kC;       // the first CTA's places for each CTA's candidates
+        if (bound > -INFINITY)
+            each([&](int i, float v) {
+                if (v >= bound) {
+                    const unsigned at = atomicAdd(&sh.n_mine, 1u);
+                    if (at < kSeg) st_u64(peer(&xc.cand[rank * kSeg + at], 0), as_cand(i, v));
+                }
+            });
+        __syncthreads();
+        if (tid < kC) st_u32(peer(&xc.n_of[rank], tid), bound > -INFINITY ? sh.n_mine : kSeg + 1);
+        cluster_sync();
+        int nc = 0;
+        bool fits = true;
+#pragma unroll
+        for (int r = 0; r < kC; r++) {
+            nc += xc.n_of[r];
+            fits = fits && xc.n_of[r] <= kSeg;
+        }
+        if (fits) {
+            if (rank == 0)
+                solve(nc, [&](int i) {
+                    int r = 0;
+                    while (i >= static_cast<int>(xc.n_of[r])) i -= xc.n_of[r++];
+                    return xc.cand[r * kSeg + i];
+                }, false, 0);
+            return;
+        }
+    }
+    // the step of a token: kBins or more where the weight is 0
+    const float bs = row.inv_t * kBinScale;
+    auto step_of = [&](float v) {
+        return v == m ? 0 : row.hot && v > -INFINITY ? static_cast<int>(fminf((m - v) * bs, kBins)) : kBins;
+    };
+    // Sum over the row's keys >= from of 1 or the weight; of the keys at floor_key only floor_ties count, none below it.
+    auto measure = [&](uint32_t from, uint32_t floor_key, u64 floor_ties, bool weights, int slot) {
+        u64 s = 0, eq = 0;
+        each([&](int, float v) {
+            const uint32_t key = key_of(v);
+            if (key < from || key < floor_key || step_of(v) >= kBins) return;
+            if (key == floor_key) eq++;
+            else s += weights ? row.whole(v) : 1ull;
+        });
+        s = cta_sum(s, sh.red);
+        eq = cta_sum(eq, sh.red);
+        if (tid < kC) {
+            st_u64(peer(&xc.sum[slot][rank], tid), s);
+            st_u32(peer(&xc.cnt[slot][rank], tid), static_cast<unsigned>(eq));
+        }
+        cluster_sync();
+        u64 all = 0, q = 0;
+#pragma unroll
+        for (int r = 0; r < kC; r++) {
+            all += xc.sum[slot][r];
+            q += xc.cnt[slot][r];
+        }
+        return all + min(q, floor_ties) * (weights ? row.whole(logit_of_key(floor_key)) : 1ull);
+    };
+    // the largest key whose sum reaches lim, and how many of the tokens at it that takes
+    auto bisect = [&](u64 lim, bool weights, uint32_t floor_key, u64 floor_ties) {
+        uint32_t l = max(floor_key, 1u), h = key_of(m);   // measure(l) >= lim
+        int slot = 0;
+        while (l < h) {
+            const uint32_t mid = l + (h - l) / 2 + 1;
+            if (measure(mid, floor_key, floor_ties, weights, slot) >= lim) l = mid;
+            else h = mid - 1;
+            slot ^= 1;
+        }
+        const u64 above = measure(l + 1, l + 1, ~0ull, weights, slot);
+        const u64 w = weights ? max(row.whole(logit_of_key(l)), 1ull) : 1ull;
+        thr = l;
+        ties = (lim - above + w - 1) / w;
+        if (l == floor_key) ties = min(ties, floor_ties);
+        cluster_sync();
+    };
+    // round 0: top-k by counts; round 1: top-p by weights, of what top-k has kept (keys above thr, `ties` at it)
+    for (int round = by_k ? 0 : 1; round < (by_p ? 2 : 1); round++) {
+        const bool weigh = round == 1;
+        const uint32_t fk = thr;
+        const u64 ft = ties, fw = fk ? row.whole(logit_of_key(fk)) : 0ull;
+        if (weigh && by_k) {   // once more from empty counts
+            cluster_sync();
+            reinterpret_cast<uint4 *>(sh.cnt)[tid] = z4;
+            if (tid == 0) xc.n_cand = 0;
+            cluster_sync();
+        }
         each([&](int, float v) {
             const int s = step_of(v);
-            if (s >= kBins) return;
+            if (s >= kBins || key_of(v) <= fk) return;       // (tokens at the floor are added below)
             atomicAdd(&sh.cnt[s], 1u);
             if (weigh) {   // a 64-bit sum as two words: the carry goes with the high one
                 const u64 w = row.whole(v);
@@ -453,32 +598,49 @@ __global__ void __launch_bounds__(kNT, 2) k_sample_cluster(SampleArgs a, int sli
         // every CTA adds the eight histograms up, four steps per thread, and scans them from the top
         unsigned c4[4] = {0, 0, 0, 0};
         u64 w4[4] = {0, 0, 0, 0};
+        {
+            uint4 v[kC];
 #pragma unroll
-        for (int r = 0; r < kC; r++) {
-            const uint4 v = ld_v4(peer(&sh.cnt[4 * tid], r));
-            c4[0] += v.x, c4[1] += v.y, c4[2] += v.z, c4[3] += v.w;
+            for (int r = 0; r < kC; r++) v[r] = ld_v4(peer(&sh.cnt[4 * tid], r));
+#pragma unroll
+            for (int r = 0; r < kC; r++) c4[0] += v[r].x, c4[1] += v[r].y, c4[2] += v[r].z, c4[3] += v[r].w;
         }
         if (weigh) {
+            uint4 l[kC], h[kC];
 #pragma unroll
             for (int r = 0; r < kC; r++) {
-                const uint4 l = ld_v4(peer(&sh.lo[4 * tid], r)), h = ld_v4(peer(&sh.hi[4 * tid], r));
-                w4[0] += l.x + (static_cast<u64>(h.x) << 32);
-                w4[1] += l.y + (static_cast<u64>(h.y) << 32);
-                w4[2] += l.z + (static_cast<u64>(h.z) << 32);
-                w4[3] += l.w + (static_cast<u64>(h.w) << 32);
+                l[r] = ld_v4(peer(&sh.lo[4 * tid], r));
+                h[r] = ld_v4(peer(&sh.hi[4 * tid], r));
+            }
+#pragma unroll
+            for (int r = 0; r < kC; r++) {
+                w4[0] += l[r].x + (static_cast<u64>(h[r].x) << 32);
+                w4[1] += l[r].y + (static_cast<u64>(h[r].y) << 32);
+                w4[2] += l[r].z + (static_cast<u64>(h[r].z) << 32);
+                w4[3] += l[r].w + (static_cast<u64>(h[r].w) << 32);
+            }
+            if (fk) {   // top-k's last key: its kept ties, in its step
+                const int s = step_of(logit_of_key(fk));
+                if (s < kBins && s >> 2 == tid)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if ((s & 3) == i) {
+                            c4[i] += static_cast<unsigned>(ft);
+                            w4[i] += ft * fw;
+                        }
             }
         }
         u64 all_c, all_w = 0;
         u64 c0 = cta_prefix(static_cast<u64>(c4[0]) + c4[1] + c4[2] + c4[3], sh.red, all_c), w0 = 0;
         if (weigh) w0 = cta_prefix(w4[0] + w4[1] + w4[2] + w4[3], sh.red, all_w);
         // the step with the k-th token, or the one where top-p's sum is reached
-        const u64 need = by_k ? min(static_cast<u64>(k), all_c) : max(part_of(p24, all_w), 1ull);
+        const u64 need = weigh ? max(part_of(p24, all_w), 1ull) : min(static_cast<u64>(k), all_c);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const u64 before = by_k ? c0 : w0, here = by_k ? c4[i] : w4[i];
+            const u64 before = weigh ? w0 : c0, here = weigh ? w4[i] : c4[i];
             if (before < need && need <= before + here) {
                 sh.step = 4 * tid + i;
-                sh.upto = static_cast<int>(c0 + c4[i]);   // tokens down to here
+                sh.upto = static_cast<int>(min(c0 + c4[i], static_cast<u64>(kCap + 1)));   // tokens down to here
                 sh.before = before;
                 sh.in_step = c4[i];
             }
@@ -487,155 +649,85 @@ __global__ void __launch_bounds__(kNT, 2) k_sample_cluster(SampleArgs a, int sli
         }
         __syncthreads();
         const int step = sh.step;
-        const bool small = sh.upto <= kCap, gather = small || sh.in_step <= kCap;
-        if (gather) {
-            each([&](int i, float v) {
-                const int s = step_of(v);
-                if (small ? s <= step : s == step) {
-                    const unsigned at = add_u32(peer(&xc.n_cand, 0), 1);
-                    st_u64(peer(&xc.cand[at], 0),
-                           (static_cast<u64>(~key_of(v)) << 32) | static_cast<unsigned>(lo + i));
-                }
-            });
-            cluster_sync();
-            if (small && rank != 0) return;          // the first CTA has all that is needed
-            if (rank == 0) {
-                const int nc = static_cast<int>(xc.n_cand);
-                int n2 = 32;
-                while (n2 < nc) n2 <<= 1;
-                const bool in = tid < nc;
-                const u64 v = cta_sort(in ? xc.cand[tid] : ~0ull, n2, sh.buf);
-                const uint32_t key = ~static_cast<uint32_t>(v >> 32);
-                const float xv = logit_of_key(key);
-                const u64 w = in ? row.whole(xv) : 0ull;
-                u64 tot;
-                if (small) {
-                    // sorted: top-k and top-p keep the first ones
-                    const u64 before = cta_prefix(tid < k ? w : 0ull, sh.red, tot);
-                    const u64 lim = !by_p ? ~0ull : by_k ? max(part_of(p24, tot), 1ull) : need;
-                    const bool kept = in && tid < k && before < lim && row.weight(xv) >= mp;
-                    const u64 total = cta_sum(kept ? w : 0ull, sh.red);
-                    const u64 target = part_of(u24, total);
-                    // the draw, in index order
-                    const u64 z = cta_sort(kept ? ((v & 0xFFFFFFFFull) << 32) | key : ~0ull, n2, sh.buf);
-                    const float zx = logit_of_key(static_cast<uint32_t>(z));
-                    const u64 zw = z != ~0ull ? row.whole(zx) : 0ull;
-                    const u64 zb = cta_prefix(zw, sh.red, tot);
-                    if (zb <= target && target < zb + zw) finish(static_cast<int>(z >> 32), zx, total);
-                    return;
-                }
-                // the threshold inside the step
-                const u64 mine = by_k ? 1ull : w;
-                const u64 before = sh.before + cta_prefix(in ? mine : 0ull, sh.red, tot);
-                if (in && before < need && need <= before + mine) xc.thr = key;
-                __syncthreads();
-                const uint32_t key_t = xc.thr;
-                const u64 eq = cta_sum(in && key == key_t && before < need ? 1ull : 0ull, sh.red);
-                if (tid < kC) {
-                    st_u32(peer(&xc.thr, tid), key_t);
-                    st_u64(peer(&xc.ties, tid), eq);
-                }
-            }
-            cluster_sync();
-            thr = xc.thr;
-            ties = xc.ties;
+        // (after a top-k the first CTA could not tell its ties apart by index: no shortcut there)
+        const bool small = sh.upto <= kCap && !(weigh && by_k), gather = small || sh.in_step <= kCap;
+        if (!gather) {
+            bisect(need, weigh, fk, ft);
+            continue;
         }
-        // Sum over the row's keys >= from of 1 or the weight; of the keys at floor_key only floor_ties count, none
-        // below it.  Used by bisection: steps of more than kCap tokens, and top-p after a top-k of more than kCap.
-        auto measure = [&](uint32_t from, uint32_t floor_key, u64 floor_ties, bool weights, int slot) {
-            u64 s = 0, eq = 0;
-            each([&](int, float v) {
-                const uint32_t key = key_of(v);
-                if (key < from || key < floor_key || step_of(v) >= kBins) return;
-                if (key == floor_key) eq++;
-                else s += weights ? row.whole(v) : 1ull;
-            });
-            s = cta_sum(s, sh.red);
-            eq = cta_sum(eq, sh.red);
+        each([&](int i, float v) {
+            const int s = step_of(v);
+            if (key_of(v) > fk && (small ? s <= step : s == step)) {
+                const unsigned at = add_u32(peer(&xc.n_cand, 0), 1);
+                st_u64(peer(&xc.cand[at], 0), as_cand(i, v));
+            }
+        });
+        cluster_sync();
+        if (small) {                                   // the first CTA has all that is needed
+            if (rank == 0) solve(static_cast<int>(xc.n_cand), [&](int i) { return xc.cand[i]; }, weigh, need);
+            return;
+        }
+        if (rank == 0) {
+            // the threshold inside the step; past its tokens lies the floor
+            const int nc = static_cast<int>(xc.n_cand);
+            int n2 = 32;
+            while (n2 < nc) n2 <<= 1;
+            const bool in = tid < nc;
+            const u64 v = cta_sort(in ? xc.cand[tid] : ~0ull, n2, sh.buf);
+            const uint32_t key = ~static_cast<uint32_t>(v >> 32);
+            const u64 mine = !in ? 0ull : weigh ? row.whole(logit_of_key(key)) : 1ull;
+            u64 tot;
+            const u64 before = sh.before + cta_prefix(mine, sh.red, tot);
+            if (tid == 0) xc.thr = 0;
+            __syncthreads();
+            if (in && before < need && need <= before + mine) xc.thr = key;
+            __syncthreads();
+            uint32_t key_t = xc.thr;
+            u64 eq = cta_sum(in && key == key_t && before < need ? 1ull : 0ull, sh.red);
+            if (key_t == 0) {                          // reached by ties at the floor only
+                key_t = fk;
+                eq = min((need - sh.before - tot + fw - 1) / max(fw, 1ull), ft);
+            }
+            __syncthreads();
             if (tid < kC) {
-                st_u64(peer(&xc.sum[slot][rank], tid), s);
-                st_u32(peer(&xc.cnt[slot][rank], tid), static_cast<unsigned>(eq));
+                st_u32(peer(&xc.thr, tid), key_t);
+                st_u64(peer(&xc.ties, tid), eq);
             }
-            cluster_sync();
-            u64 all = 0, q = 0;
-#pragma unroll
-            for (int r = 0; r < kC; r++) {
-                all += xc.sum[slot][r];
-                q += xc.cnt[slot][r];
-            }
-            return all + min(q, floor_ties) * (weights ? row.whole(logit_of_key(floor_key)) : 1ull);
-        };
-        // the largest key whose sum reaches lim, and how many of the tokens at it that takes
-        auto bisect = [&](u64 lim, bool weights, uint32_t floor_key, u64 floor_ties) {
-            uint32_t l = max(floor_key, 1u), h = key_of(m);   // measure(l) >= lim
-            int slot = 0;
-            while (l < h) {
-                const uint32_t mid = l + (h - l) / 2 + 1;
-                if (measure(mid, floor_key, floor_ties, weights, slot) >= lim) l = mid;
-                else h = mid - 1;
-                slot ^= 1;
-            }
-            const u64 above = measure(l + 1, l + 1, ~0ull, weights, slot);
-            const u64 w = weights ? max(row.whole(logit_of_key(l)), 1ull) : 1ull;
-            thr = l;
-            ties = (lim - above + w - 1) / w;
-            if (l == floor_key) ties = min(ties, floor_ties);
-            cluster_sync();
-        };
-        if (!gather) bisect(need, weigh, 0, 0);
-        if (by_k && by_p && !small) {
-            const uint32_t fk = thr;
-            const u64 ft = ties;
-            cluster_sync();
-            const u64 tot = measure(fk, fk, ft, true, 0);
-            cluster_sync();
-            bisect(max(part_of(p24, tot), 1ull), true, fk, ft);
         }
+        cluster_sync();
+        thr = xc.thr;
+        ties = xc.ties;
     }
-    // ---------------- the draw over all CTAs: per (round of 4 kNT logits, warp) the kept weight above the threshold
-    // and the tokens at it, in index order
+    // ---------------- the draw over all CTAs: per warp (its stretch of indexes) the kept weight above the threshold and
+    // the tokens at it
     const u64 w_thr = thr ? row.whole(logit_of_key(thr)) : 0ull;
     const bool thr_ok = thr && row.weight(logit_of_key(thr)) >= mp;
-    const int rounds = (slice + 4 * kNT - 1) / (4 * kNT), ents = rounds * kNW;
-    auto part = [&](float v, u64 &s, u64 &q) {
+    auto part = [&](float v, u64 &s, unsigned &q) {
         const uint32_t key = key_of(v);
-        if (key > thr) {
-            const float w = row.weight(v);
-            if (w >= mp) s += static_cast<u64>(w * 0x1p40f);
-        }
-        q += key == thr && thr_ok ? 1 : 0;
+        const float w = row.weight(v);
+        if (key > thr && w >= mp) s += whole_of(w);
+        q += key == thr && thr_ok ? 1u : 0u;
     };
-    for (int e = 0; e < rounds; e++) {
-        const int i = 4 * (e * kNT + tid);
-        u64 s = 0, q = 0;
-        if (i < slice) {
-            const float4 v = *reinterpret_cast<const float4 *>(xs + i);
-            part(v.x, s, q);
-            part(v.y, s, q);
-            part(v.z, s, q);
-            part(v.w, s, q);
-        }
+    {
+        u64 s = 0;
+        unsigned q = 0;
+        each([&](int, float v) { part(v, s, q); });
         s = warp_sum64(s);
-        const unsigned qs = __reduce_add_sync(0xffffffffu, static_cast<unsigned>(q));
+        q = __reduce_add_sync(0xffffffffu, q);
         if (lane == 0) {
-            sh.ent[0][e * kNW + warp] = s;
-            sh.ent[1][e * kNW + warp] = qs;
+            sh.ent[0][warp] = s;
+            sh.ent[1][warp] = q;
         }
     }
     __syncthreads();
-    if (warp < 2) {   // exclusive scans of the entries; the total after the last
-        u64 run = 0;
-        for (int i0 = 0; i0 < ents; i0 += 32) {
-            const u64 v = i0 + lane < ents ? sh.ent[warp][i0 + lane] : 0ull;
-            const u64 inc = warp_scan64(v);
-            __syncwarp();
-            if (i0 + lane < ents) sh.ent[warp][i0 + lane] = run + inc - v;
-            run += __shfl_sync(0xffffffffu, inc, 31);
-        }
-        if (lane == 0) sh.ent[warp][ents] = run;
+    if (warp < 2) {   // exclusive scans over the warps; the total after the last
+        const u64 v = lane < kNW ? sh.ent[warp][lane] : 0ull, inc = warp_scan64(v);
+        __syncwarp();
+        if (lane <= kNW) sh.ent[warp][lane] = inc - v;   // (lane kNW: the total)
+        const u64 all = __shfl_sync(0xffffffffu, inc, 31);
         if (lane < kC) {
-            if (warp == 0) st_u64(peer(&xc.sum[0][rank], lane), run);
-            else st_u32(peer(&xc.cnt[0][rank], lane), static_cast<unsigned>(run));
+            if (warp == 0) st_u64(peer(&xc.sum[0][rank], lane), all);
+            else st_u32(peer(&xc.cnt[0][rank], lane), static_cast<unsigned>(all));
         }
     }
     cluster_sync();
@@ -652,26 +744,28 @@ __global__ void __launch_bounds__(kNT, 2) k_sample_cluster(SampleArgs a, int sli
     // the kept weight before a place with s above the threshold and q tokens at it before it
     auto kept = [&](u64 s, u64 q) { return s + min(q, ties) * w_thr; };
     const u64 total = kept(s_all, q_all), target = part_of(u24, total);
-    for (int e = 0; e < rounds; e++) {
-        const int at = e * kNW + warp;
-        u64 s = s_me + sh.ent[0][at], q = q_me + sh.ent[1][at];
-        if (!(kept(s, q) <= target && target < kept(s_me + sh.ent[0][at + 1], q_me + sh.ent[1][at + 1]))) continue;
-        const int i = 4 * (e * kNT + tid);
-        float4 v = i < slice ? *reinterpret_cast<const float4 *>(xs + i) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-        u64 ls = 0, lq = 0;
-        part(v.x, ls, lq);
-        part(v.y, ls, lq);
-        part(v.z, ls, lq);
-        part(v.w, ls, lq);
-        s += warp_scan64(ls) - ls;
-        q += warp_scan64(lq) - lq;
+    u64 s0 = s_me + sh.ent[0][warp], q0 = q_me + sh.ent[1][warp];
+    if (!(kept(s0, q0) <= target && target < kept(s_me + sh.ent[0][warp + 1], q_me + sh.ent[1][warp + 1]))) return;
+    for (int i = first + 4 * lane; i < first + region; i += 128) {   // the warp that has the token: 128 at a time
+        const float4 v = *reinterpret_cast<const float4 *>(xs + i);
         const float vs[4] = {v.x, v.y, v.z, v.w};
+        u64 ls = 0;
+        unsigned lq = 0;
+#pragma unroll
+        for (int c = 0; c < 4; c++) part(vs[c], ls, lq);
+        const u64 is = warp_scan64(ls), iq = warp_scan64(lq);
+        u64 s = s0 + is - ls;
+        unsigned q = static_cast<unsigned>(q0 + iq) - lq;
+        s0 += __shfl_sync(0xffffffffu, is, 31);
+        q0 += __shfl_sync(0xffffffffu, iq, 31);
+        if (kept(s0, q0) <= target) continue;
 #pragma unroll
         for (int c = 0; c < 4; c++) {
             const u64 b0 = kept(s, q);
             part(vs[c], s, q);
             if (b0 <= target && target < kept(s, q)) finish(lo + i + c, vs[c], total);
         }
+        break;
     }
 }
 
@@ -680,14 +774,14 @@ __global__ void __launch_bounds__(kNT, 2) k_sample_cluster(SampleArgs a, int sli
 cudaError_t launch_sample(const SampleArgs &a, cudaStream_t st) {
     // (a row up to 262144 logits fits eight CTAs' shared memory; beyond that it is read once per digit)
     if (a.n_vocab > kC * kSlice) return launch_pdl(k_sample, dim3(a.n_rows), dim3(kThreads), 0, st, a);
-    const int slice = (((a.n_vocab + kC - 1) / kC) + 3) & ~3;
-    const bool vec = (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0 && a.row_stride % 4 == 0;
+    const int region = ((a.n_vocab + kC * kNW - 1) / (kC * kNW) + 127) & ~127;
+    const bool bulk = (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0 && a.row_stride % 4 == 0;
     const cudaError_t e = cudaFuncSetAttribute(k_sample_cluster, cudaFuncAttributeMaxDynamicSharedMemorySize, kSlice * 4);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(a.n_rows) * kC);
     cfg.blockDim = dim3(kNT);
-    cfg.dynamicSmemBytes = static_cast<size_t>(slice) * 4;
+    cfg.dynamicSmemBytes = static_cast<size_t>(region) * kNW * 4;
     cfg.stream = st;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -697,7 +791,7 @@ cudaError_t launch_sample(const SampleArgs &a, cudaStream_t st) {
     at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, k_sample_cluster, a, slice, vec);
+    return cudaLaunchKernelEx(&cfg, k_sample_cluster, a, region, bulk);
 }
 
 }  // namespace styx

@@ -301,7 +301,7 @@ int styx_sample(styx_ctx *ctx, styx_stream stream, const float *logits, int64_t 
                 const float *u, const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
                 int32_t *token, float *logprob) {
     styx::SampleArgs a{};
-    CHECK(styx::ctx_enter(ctx, nullptr, nullptr));
+    CHECK(styx::ctx_enter(ctx, nullptr, &a.err));
     NEED(logits && u && token, "null pointer");
     NEED(n_rows > 0 && n_vocab > 0 && n_vocab <= (1 << 22) && row_stride >= n_vocab, "n_rows %d, n_vocab %d, row_stride %lld",
          n_rows, n_vocab, static_cast<long long>(row_stride));
