@@ -13,11 +13,13 @@
 //     (22 on average for k = 20, 355 for 120, where large ones are spread
 //     evenly) go to the cluster's first CTA, which sorts them and does the rest.
 //   else, with top-k or top-p: one histogram over 2048 equal steps of log
-//     weight (tokens below e^-28 have weight 0 and take no part in anything)
-//     shows the step in which the threshold lies.  Where the tokens down to
-//     there are at most 512 they go to the first CTA as above; else only that
+//     weight (tokens below e^-28 have weight 0 and take no part in anything),
+//     of counts or of weights, shows the step in which the threshold lies;
+//     each CTA adds up an eighth of it (all of it in every CTA was 190 KB
+//     over distributed shared memory, 12000 cycles).  Where the tokens down to
+//     there are at most 2048 they go to the first CTA as above; else only that
 //     step's tokens go there and the threshold comes back.  Top-p after such
-//     a top-k is a second histogram, of the tokens kept.  Only more than 512
+//     a top-k is a second histogram, of the tokens kept.  Only more than 2048
 //     tokens in one step (a flat row) are resolved by bisection of the key.
 //   the draw, where it is not the first CTA's: sums of the kept weights per
 //     warp, each over a stretch of indexes of its own, then inside one warp.
@@ -28,6 +30,7 @@
 // k_sample (larger vocabularies): one CTA per row, radix selection from L2.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 
 #include "cluster.cuh"
@@ -61,11 +64,8 @@ struct Row {
     const float *x;
     float m, inv_t;
     bool hot;
-    __device__ __forceinline__ float weight(float v) const {
-        if (v == m) return 1.f;
-        if (v == -INFINITY) return 0.f;   // an infinite temperature included
-        return hot ? expf((v - m) * inv_t) : 0.f;
-    }
+    // inv_t: infinite for the greedy pick, else finite and above 0, so that (v - m) inv_t is no NaN
+    __device__ __forceinline__ float weight(float v) const { return v == m ? 1.f : expf((v - m) * inv_t); }
     __device__ __forceinline__ u64 whole(float v) const { return whole_of(weight(v)); }
 };
 
@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(kThreads) k_sample(SampleArgs a) {
     row.x = a.logits + b * a.row_stride;
     const float t = a.temperature ? a.temperature[b] : 1.f;
     row.hot = t > 0.f;
-    row.inv_t = 1.0f / t;
+    row.inv_t = row.hot ? fmaxf(1.0f / t, 0x1p-126f) : INFINITY;
     float m = -INFINITY;
     for (int i = tid; i < n; i += kThreads) m = fmaxf(m, clean(row.x[i]));
 #pragma unroll
@@ -256,29 +256,24 @@ __global__ void __launch_bounds__(kThreads) k_sample(SampleArgs a) {
 // ------------------------------------------------------------ one cluster per row
 constexpr int kC = 8;                       // CTAs of a row
 constexpr int kNT = 512, kNW = kNT / 32;    // threads and warps of a CTA
-constexpr int kBins = 4 * kNT, kCap = kNT;
+constexpr int kBins = 4 * kNT, kCap = 4 * kNT, kShare = kBins / kC;
 constexpr float kBinScale = kBins / 28.f;
 constexpr int kSlice = 32768;               // logits of a CTA at most
 constexpr int kTopK = 120;                  // top-k by the warps' maxima (128 of them)
 
-struct Exchange {                           // what the cluster's CTAs write into each other
-    float top[kC * kNW];
-    u64 sum[2][kC];
-    unsigned cnt[2][kC];
-    unsigned n_of[kC];                      // candidates of each CTA
-    unsigned n_cand, thr;
-    u64 ties;
-    u64 cand[kCap];                         // (inverted key << 32) | index: ascending = the order of the tokens
-};
 struct CtaShared {
-    Exchange xc;
-    unsigned cnt[kBins], lo[kBins], hi[kBins];
-    u64 red[32], buf[kNT], ent[2][kNW + 1];
+    union {
+        unsigned hist[3][kBins];            // counts, or the low and high words of the weights' sums (0, 1)
+        u64 cand[kCap];                     // (inverted key << 32) | index: ascending = the order of the tokens
+    };
+    u64 red[32], ent[2][kNW + 1];
     uint64_t bar;
     float bound;
     unsigned n_mine;
-    int step, upto;
-    u64 before, in_step;
+    // what the cluster's CTAs write into each other
+    __align__(16) float top[kC * kNW];
+    u64 sum[2][kC], before, ties;
+    unsigned cnt[2][kC], n_of[kC], step, thr;
 };
 
 __device__ __forceinline__ void cluster_sync() {
@@ -291,18 +286,10 @@ __device__ __forceinline__ void st_u32(uint32_t addr, unsigned v) {
 __device__ __forceinline__ void st_u64(uint32_t addr, u64 v) {
     asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
 }
-__device__ __forceinline__ uint4 ld_v4(uint32_t addr) {
-    uint4 v;
-    asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                 : "r"(addr)
-                 : "memory");
+__device__ __forceinline__ unsigned ld_u32(uint32_t addr) {
+    unsigned v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
     return v;
-}
-__device__ __forceinline__ unsigned add_u32(uint32_t addr, unsigned v) {
-    unsigned o;
-    asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(o) : "r"(addr), "r"(v) : "memory");
-    return o;
 }
 __device__ __forceinline__ u64 warp_sum64(u64 v) {
 #pragma unroll
@@ -342,18 +329,34 @@ __device__ __forceinline__ float logit_of_key(uint32_t key) {
     return __uint_as_float((key & 0x80000000u) ? (key & 0x7FFFFFFFu) : ~key);
 }
 
-// The CTA's values sorted ascending over its first n threads (a power of two,
-// 32 or more; what lies beyond must be ~0): bitonic, strides below a warp by
-// shuffles.
-__device__ __forceinline__ u64 cta_sort(u64 v, int n, u64 *buf) {
+// buf[0, n) sorted ascending (n a power of two, 32 or more): bitonic; up to one
+// value per thread, strides below a warp by shuffles
+__device__ __forceinline__ void cta_sort(u64 *buf, int n) {
     const int t = threadIdx.x;
+    __syncthreads();
+    if (n > kNT) {
+        for (int size = 2; size <= n; size <<= 1)
+            for (int stride = size >> 1; stride; stride >>= 1) {
+                for (int p = t; p < n / 2; p += kNT) {
+                    const int i = 2 * p - (p & (stride - 1)), j = i + stride;   // i has no `stride` bit
+                    const u64 v = buf[i], w = buf[j];
+                    if ((v > w) == ((i & size) == 0)) {
+                        buf[i] = w;
+                        buf[j] = v;
+                    }
+                }
+                __syncthreads();
+            }
+        return;
+    }
+    u64 v = t < n ? buf[t] : ~0ull;
     for (int size = 2; size <= n; size <<= 1) {
         const bool up = (t & size) == 0;
         for (int stride = size >> 1; stride >= 32; stride >>= 1) {
-            buf[t] = v;
             __syncthreads();
-            const u64 w = buf[t ^ stride];
+            if (t < n) buf[t] = v;
             __syncthreads();
+            const u64 w = t < n ? buf[t ^ stride] : ~0ull;
             v = ((t & stride) == 0) == up ? min(v, w) : max(v, w);
         }
         for (int stride = min(size >> 1, 16); stride; stride >>= 1) {
@@ -361,7 +364,9 @@ __device__ __forceinline__ u64 cta_sort(u64 v, int n, u64 *buf) {
             v = ((t & stride) == 0) == up ? min(v, w) : max(v, w);
         }
     }
-    return v;
+    __syncthreads();
+    if (t < n) buf[t] = v;
+    __syncthreads();
 }
 
 // slice: logits of a CTA, kNW * region of them, a warp's stretch each (region
@@ -372,18 +377,13 @@ __global__ void __launch_bounds__(kNT, 2) k_sample_cluster(SampleArgs a, int reg
     __shared__ __align__(16) CtaShared sh;
     pdl_trigger();
     cl_arrive_relaxed();                          // the others have started: waited for before the first store to them
-    Exchange &xc = sh.xc;
     const uint32_t rank = cluster_ctarank();
     const int b = blockIdx.x / kC, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n = a.n_vocab;
     const int slice = kNW * region, lo = static_cast<int>(rank) * slice, len = max(0, min(n - lo, slice));
     const int first = warp * region;              // the warp's stretch of the slice
     auto peer = [&](const void *p, uint32_t r) { return cl_map(smem_addr(p), r); };
     const uint4 z4 = make_uint4(0, 0, 0, 0);
-    reinterpret_cast<uint4 *>(sh.cnt)[tid] = z4;
-    reinterpret_cast<uint4 *>(sh.lo)[tid] = z4;
-    reinterpret_cast<uint4 *>(sh.hi)[tid] = z4;
     if (tid == 0) {
-        xc.n_cand = 0;
         sh.n_mine = 0;
         mbar_init(&sh.bar, 1);
         fence_mbar_init();
@@ -405,7 +405,8 @@ __global__ void __launch_bounds__(kNT, 2) k_sample_cluster(SampleArgs a, int reg
     Row row;
     row.x = nullptr;
     row.hot = t > 0.f;
-    row.inv_t = 1.0f / t;
+    // (an infinite temperature: no product with -inf may be NaN)
+    row.inv_t = row.hot ? fmaxf(1.0f / t, 0x1p-126f) : INFINITY;
     const float p = fminf(top_p, 1.f), mp = fminf(min_p, 1.f);   // the maximum always stays
     const u64 p24 = p > 0.f ? static_cast<u64>(rintf(p * 0x1p24f)) : 0ull;
     const u64 u24 = static_cast<u64>(fminf(fmaxf(u, 0.f), 0x1.fffffep-1f) * 0x1p24f);
@@ -422,10 +423,10 @@ __global__ void __launch_bounds__(kNT, 2) k_sample_cluster(SampleArgs a, int reg
 #pragma unroll
     for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     cl_wait();
-    if (lane < kC) cl_st(peer(&xc.top[rank * kNW + warp], lane), m);
+    if (lane < kC) cl_st(peer(&sh.top[rank * kNW + warp], lane), m);
     cluster_sync();
     {
-        const float4 v = reinterpret_cast<const float4 *>(xc.top)[lane];   // 128 maxima, four a lane
+        const float4 v = reinterpret_cast<const float4 *>(sh.top)[lane];   // 128 maxima, four a lane
         m = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
 #pragma unroll
         for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -462,35 +463,55 @@ __global__ void __launch_bounds__(kNT, 2) k_sample_cluster(SampleArgs a, int reg
     };
     // the first CTA, with nc candidates (cand(i), any order) among which is all that is kept: sorted, top-k and top-p
     // keep the first ones, min-p too; then the draw in index order.  need_p: top-p's sum, where it is known.
+    u64 *buf = reinterpret_cast<u64 *>(xs);       // (its own logits are no longer needed then)
     auto solve = [&](int nc, auto cand, bool p_known, u64 need_p) {
         int n2 = 32;
         while (n2 < nc) n2 <<= 1;
-        const u64 v = cta_sort(tid < nc ? cand(tid) : ~0ull, n2, sh.buf);
-        const uint32_t key = ~static_cast<uint32_t>(v >> 32);
-        const float xv = logit_of_key(key);
-        const bool in = tid < nc && tid < k;
-        const u64 w = in ? row.whole(xv) : 0ull;
-        bool kept = in && row.weight(xv) >= mp;
-        u64 tot;
+        const int per = max(1, n2 / kNT), i0 = tid * per;   // a thread's values, neighbours
+        __syncthreads();
+        for (int i = tid; i < n2; i += kNT) buf[i] = i < nc ? cand(i) : ~0ull;
+        cta_sort(buf, n2);
+        u64 before = 0, tot = 0;
         if (by_p) {
-            const u64 before = cta_prefix(w, sh.red, tot);
-            kept = kept && before < (p_known ? need_p : max(part_of(p24, tot), 1ull));
+            u64 w = 0;
+            for (int i = i0; i < i0 + per && i < min(nc, k); i++) w += row.whole(logit_of_key(~static_cast<uint32_t>(buf[i] >> 32)));
+            before = cta_prefix(w, sh.red, tot);
         }
-        const u64 z = cta_sort(kept ? ((v & 0xFFFFFFFFull) << 32) | key : ~0ull, n2, sh.buf);
-        const float zx = logit_of_key(static_cast<uint32_t>(z));
-        const u64 zw = z != ~0ull ? row.whole(zx) : 0ull, zb = cta_prefix(zw, sh.red, tot), target = part_of(u24, tot);
-        if (zb <= target && target < zb + zw) finish(static_cast<int>(z >> 32), zx, tot);
+        const u64 need = !by_p ? ~0ull : p_known ? need_p : max(part_of(p24, tot), 1ull);
+        for (int i = i0; i < i0 + per && i < n2; i++) {
+            const u64 v = buf[i];
+            const uint32_t key = ~static_cast<uint32_t>(v >> 32);
+            const float xv = logit_of_key(key);
+            const bool in = i < nc && i < k;
+            const bool kept = in && before < need && row.weight(xv) >= mp;
+            if (by_p && in) before += row.whole(xv);
+            buf[i] = kept ? ((v & 0xFFFFFFFFull) << 32) | key : ~0ull;
+        }
+        cta_sort(buf, n2);
+        u64 w = 0;
+        for (int i = i0; i < i0 + per && i < n2; i++)
+            if (buf[i] != ~0ull) w += row.whole(logit_of_key(static_cast<uint32_t>(buf[i])));
+        u64 at = cta_prefix(w, sh.red, tot);
+        const u64 target = part_of(u24, tot);
+        for (int i = i0; i < i0 + per && i < n2; i++) {
+            const u64 z = buf[i];
+            if (z == ~0ull) break;
+            const float zx = logit_of_key(static_cast<uint32_t>(z));
+            const u64 zw = row.whole(zx);
+            if (at <= target && target < at + zw) finish(static_cast<int>(z >> 32), zx, tot);
+            at += zw;
+        }
     };
     uint32_t thr = 0;          // kept: keys above thr, and the first `ties` at it
     u64 ties = 0;
     if (by_k && k <= kTopK) {
         // the k-th largest of the 128 maxima: thread t counts those before maximum t
         if (tid < kC * kNW) {
-            const float mine = xc.top[tid];
+            const float mine = sh.top[tid];
             int before = 0;
 #pragma unroll 8
             for (int i = 0; i < kC * kNW; i += 4) {
-                const float4 v = *reinterpret_cast<const float4 *>(&xc.top[i]);
+                const float4 v = *reinterpret_cast<const float4 *>(&sh.top[i]);
                 before += (v.x > mine || (v.x == mine && i < tid)) + (v.y > mine || (v.y == mine && i + 1 < tid)) +
                           (v.z > mine || (v.z == mine && i + 2 < tid)) + (v.w > mine || (v.w == mine && i + 3 < tid));
             }
@@ -503,34 +524,32 @@ __global__ void __launch_bounds__(kNT, 2) k_sample_cluster(SampleArgs a, int reg
             each([&](int i, float v) {
                 if (v >= bound) {
                     const unsigned at = atomicAdd(&sh.n_mine, 1u);
-                    if (at < kSeg) st_u64(peer(&xc.cand[rank * kSeg + at], 0), as_cand(i, v));
+                    if (at < kSeg) st_u64(peer(&sh.cand[rank * kSeg + at], 0), as_cand(i, v));
                 }
             });
         __syncthreads();
-        if (tid < kC) st_u32(peer(&xc.n_of[rank], tid), bound > -INFINITY ? sh.n_mine : kSeg + 1);
+        if (tid < kC) st_u32(peer(&sh.n_of[rank], tid), bound > -INFINITY ? sh.n_mine : kSeg + 1);
         cluster_sync();
         int nc = 0;
         bool fits = true;
 #pragma unroll
         for (int r = 0; r < kC; r++) {
-            nc += xc.n_of[r];
-            fits = fits && xc.n_of[r] <= kSeg;
+            nc += sh.n_of[r];
+            fits = fits && sh.n_of[r] <= kSeg;
         }
         if (fits) {
             if (rank == 0)
                 solve(nc, [&](int i) {
                     int r = 0;
-                    while (i >= static_cast<int>(xc.n_of[r])) i -= xc.n_of[r++];
-                    return xc.cand[r * kSeg + i];
+                    while (i >= static_cast<int>(sh.n_of[r])) i -= sh.n_of[r++];
+                    return sh.cand[r * kSeg + i];
                 }, false, 0);
             return;
         }
     }
     // the step of a token: kBins or more where the weight is 0
     const float bs = row.inv_t * kBinScale;
-    auto step_of = [&](float v) {
-        return v == m ? 0 : row.hot && v > -INFINITY ? static_cast<int>(fminf((m - v) * bs, kBins)) : kBins;
-    };
+    auto step_of = [&](float v) { return v == m ? 0 : static_cast<int>(fminf((m - v) * bs, kBins)); };
     // Sum over the row's keys >= from of 1 or the weight; of the keys at floor_key only floor_ties count, none below it.
     auto measure = [&](uint32_t from, uint32_t floor_key, u64 floor_ties, bool weights, int slot) {
         u64 s = 0, eq = 0;
@@ -543,15 +562,15 @@ __global__ void __launch_bounds__(kNT, 2) k_sample_cluster(SampleArgs a, int reg
         s = cta_sum(s, sh.red);
         eq = cta_sum(eq, sh.red);
         if (tid < kC) {
-            st_u64(peer(&xc.sum[slot][rank], tid), s);
-            st_u32(peer(&xc.cnt[slot][rank], tid), static_cast<unsigned>(eq));
+            st_u64(peer(&sh.sum[slot][rank], tid), s);
+            st_u32(peer(&sh.cnt[slot][rank], tid), static_cast<unsigned>(eq));
         }
         cluster_sync();
         u64 all = 0, q = 0;
 #pragma unroll
         for (int r = 0; r < kC; r++) {
-            all += xc.sum[slot][r];
-            q += xc.cnt[slot][r];
+            all += sh.sum[slot][r];
+            q += sh.cnt[slot][r];
         }
         return all + min(q, floor_ties) * (weights ? row.whole(logit_of_key(floor_key)) : 1ull);
     };
@@ -577,136 +596,151 @@ __global__ void __launch_bounds__(kNT, 2) k_sample_cluster(SampleArgs a, int reg
         const bool weigh = round == 1;
         const uint32_t fk = thr;
         const u64 ft = ties, fw = fk ? row.whole(logit_of_key(fk)) : 0ull;
-        if (weigh && by_k) {   // once more from empty counts
-            cluster_sync();
-            reinterpret_cast<uint4 *>(sh.cnt)[tid] = z4;
-            if (tid == 0) xc.n_cand = 0;
-            cluster_sync();
-        }
+        cluster_sync();                                      // nothing of an earlier use of the histogram is in flight
+#pragma unroll
+        for (int i = 0; i < 3; i++) reinterpret_cast<uint4 *>(sh.hist[i])[tid] = z4;
+        __syncthreads();
         each([&](int, float v) {
             const int s = step_of(v);
             if (s >= kBins || key_of(v) <= fk) return;       // (tokens at the floor are added below)
-            atomicAdd(&sh.cnt[s], 1u);
-            if (weigh) {   // a 64-bit sum as two words: the carry goes with the high one
+            if (!weigh) {
+                atomicAdd(&sh.hist[0][s], 1u);
+            } else {   // a 64-bit sum as two words: the carry goes with the high one
                 const u64 w = row.whole(v);
-                const unsigned l = static_cast<unsigned>(w), old = atomicAdd(&sh.lo[s], l);
+                const unsigned l = static_cast<unsigned>(w), old = atomicAdd(&sh.hist[0][s], l);
                 const unsigned h = static_cast<unsigned>(w >> 32) + (old + l < old ? 1u : 0u);
-                if (h) atomicAdd(&sh.hi[s], h);
+                if (h) atomicAdd(&sh.hist[1][s], h);
             }
         });
         cluster_sync();
-        // every CTA adds the eight histograms up, four steps per thread, and scans them from the top
-        unsigned c4[4] = {0, 0, 0, 0};
-        u64 w4[4] = {0, 0, 0, 0};
-        {
-            uint4 v[kC];
-#pragma unroll
-            for (int r = 0; r < kC; r++) v[r] = ld_v4(peer(&sh.cnt[4 * tid], r));
-#pragma unroll
-            for (int r = 0; r < kC; r++) c4[0] += v[r].x, c4[1] += v[r].y, c4[2] += v[r].z, c4[3] += v[r].w;
-        }
-        if (weigh) {
-            uint4 l[kC], h[kC];
+        // this CTA's share of the steps, a step per thread, added up over the cluster
+        u64 val = 0;
+        const int my_step = static_cast<int>(rank) * kShare + tid;
+        if (tid < kShare) {
+            unsigned l[kC], h[kC];
 #pragma unroll
             for (int r = 0; r < kC; r++) {
-                l[r] = ld_v4(peer(&sh.lo[4 * tid], r));
-                h[r] = ld_v4(peer(&sh.hi[4 * tid], r));
+                l[r] = ld_u32(peer(&sh.hist[0][my_step], r));
+                h[r] = weigh ? ld_u32(peer(&sh.hist[1][my_step], r)) : 0u;
             }
 #pragma unroll
-            for (int r = 0; r < kC; r++) {
-                w4[0] += l[r].x + (static_cast<u64>(h[r].x) << 32);
-                w4[1] += l[r].y + (static_cast<u64>(h[r].y) << 32);
-                w4[2] += l[r].z + (static_cast<u64>(h[r].z) << 32);
-                w4[3] += l[r].w + (static_cast<u64>(h[r].w) << 32);
-            }
-            if (fk) {   // top-k's last key: its kept ties, in its step
-                const int s = step_of(logit_of_key(fk));
-                if (s < kBins && s >> 2 == tid)
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if ((s & 3) == i) {
-                            c4[i] += static_cast<unsigned>(ft);
-                            w4[i] += ft * fw;
-                        }
-            }
+            for (int r = 0; r < kC; r++) val += l[r] + (static_cast<u64>(h[r]) << 32);
+            if (fk && step_of(logit_of_key(fk)) == my_step) val += ft * fw;   // top-k's last key: its kept ties
         }
-        u64 all_c, all_w = 0;
-        u64 c0 = cta_prefix(static_cast<u64>(c4[0]) + c4[1] + c4[2] + c4[3], sh.red, all_c), w0 = 0;
-        if (weigh) w0 = cta_prefix(w4[0] + w4[1] + w4[2] + w4[3], sh.red, all_w);
+        u64 mine, before = cta_prefix(val, sh.red, mine);
+        if (tid < kC) st_u64(peer(&sh.sum[0][rank], tid), mine);
+        cluster_sync();
+        u64 all = 0;
+#pragma unroll
+        for (int r = 0; r < kC; r++) {
+            if (r < static_cast<int>(rank)) before += sh.sum[0][r];
+            all += sh.sum[0][r];
+        }
         // the step with the k-th token, or the one where top-p's sum is reached
-        const u64 need = weigh ? max(part_of(p24, all_w), 1ull) : min(static_cast<u64>(k), all_c);
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const u64 before = weigh ? w0 : c0, here = weigh ? w4[i] : c4[i];
-            if (before < need && need <= before + here) {
-                sh.step = 4 * tid + i;
-                sh.upto = static_cast<int>(min(c0 + c4[i], static_cast<u64>(kCap + 1)));   // tokens down to here
-                sh.before = before;
-                sh.in_step = c4[i];
+        const u64 need = weigh ? max(part_of(p24, all), 1ull) : min(static_cast<u64>(k), all);
+        if (before < need && need <= before + val)
+            for (int r = 0; r < kC; r++) {
+                st_u32(peer(&sh.step, r), my_step);
+                st_u64(peer(&sh.before, r), before);
             }
-            c0 += c4[i];
-            w0 += w4[i];
+        cluster_sync();
+        const int step = static_cast<int>(sh.step);
+        // how many tokens lie down to the step, and in it
+        unsigned le = 0, eq = 0;
+        each([&](int, float v) {
+            const int s = step_of(v);
+            if (key_of(v) <= fk) return;
+            le += s <= step;
+            eq += s == step;
+        });
+        le = static_cast<unsigned>(cta_sum(le, sh.red));
+        eq = static_cast<unsigned>(cta_sum(eq, sh.red));
+        if (tid < kC) {
+            st_u32(peer(&sh.cnt[0][rank], tid), le);
+            st_u32(peer(&sh.cnt[1][rank], tid), eq);
         }
-        __syncthreads();
-        const int step = sh.step;
-        // (after a top-k the first CTA could not tell its ties apart by index: no shortcut there)
-        const bool small = sh.upto <= kCap && !(weigh && by_k), gather = small || sh.in_step <= kCap;
-        if (!gather) {
+        if (tid == 0) sh.n_mine = 0;
+        cluster_sync();
+        unsigned n_le = 0, n_eq = 0, o_le = 0, o_eq = 0;     // in all, and of the CTAs before this one
+#pragma unroll
+        for (int r = 0; r < kC; r++) {
+            if (r == static_cast<int>(rank)) {
+                o_le = n_le;
+                o_eq = n_eq;
+            }
+            n_le += sh.cnt[0][r];
+            n_eq += sh.cnt[1][r];
+        }
+        // (after a top-k the floor's ties are not among the candidates: no shortcut there)
+        const bool small = n_le <= kCap && !(weigh && by_k);
+        if (!small && n_eq > kCap) {
             bisect(need, weigh, fk, ft);
             continue;
         }
         each([&](int i, float v) {
             const int s = step_of(v);
             if (key_of(v) > fk && (small ? s <= step : s == step)) {
-                const unsigned at = add_u32(peer(&xc.n_cand, 0), 1);
-                st_u64(peer(&xc.cand[at], 0), as_cand(i, v));
+                const unsigned at = (small ? o_le : o_eq) + atomicAdd(&sh.n_mine, 1u);
+                st_u64(peer(&sh.cand[at], 0), as_cand(i, v));
             }
         });
         cluster_sync();
-        if (small) {                                   // the first CTA has all that is needed
-            if (rank == 0) solve(static_cast<int>(xc.n_cand), [&](int i) { return xc.cand[i]; }, weigh, need);
+        if (small) {                                         // the first CTA has all that is needed
+            if (rank == 0) solve(static_cast<int>(n_le), [&](int i) { return sh.cand[i]; }, weigh, need);
             return;
         }
         if (rank == 0) {
             // the threshold inside the step; past its tokens lies the floor
-            const int nc = static_cast<int>(xc.n_cand);
             int n2 = 32;
+            const int nc = static_cast<int>(n_eq);
             while (n2 < nc) n2 <<= 1;
-            const bool in = tid < nc;
-            const u64 v = cta_sort(in ? xc.cand[tid] : ~0ull, n2, sh.buf);
-            const uint32_t key = ~static_cast<uint32_t>(v >> 32);
-            const u64 mine = !in ? 0ull : weigh ? row.whole(logit_of_key(key)) : 1ull;
-            u64 tot;
-            const u64 before = sh.before + cta_prefix(mine, sh.red, tot);
-            if (tid == 0) xc.thr = 0;
+            for (int i = nc + tid; i < n2; i += kNT) sh.cand[i] = ~0ull;
+            cta_sort(sh.cand, n2);
+            const int per = max(1, n2 / kNT), i0 = tid * per;
+            auto measure_of = [&](u64 v) { return weigh ? row.whole(logit_of_key(~static_cast<uint32_t>(v >> 32))) : 1ull; };
+            u64 w = 0, tot;
+            for (int i = i0; i < min(i0 + per, nc); i++) w += measure_of(sh.cand[i]);
+            u64 at = sh.before + cta_prefix(w, sh.red, tot);
+            if (tid == 0) sh.thr = 0;
             __syncthreads();
-            if (in && before < need && need <= before + mine) xc.thr = key;
+            const u64 at0 = at;
+            for (int i = i0; i < min(i0 + per, nc); i++) {
+                const u64 x = measure_of(sh.cand[i]);
+                if (at < need && need <= at + x) sh.thr = ~static_cast<uint32_t>(sh.cand[i] >> 32);
+                at += x;
+            }
             __syncthreads();
-            uint32_t key_t = xc.thr;
-            u64 eq = cta_sum(in && key == key_t && before < need ? 1ull : 0ull, sh.red);
-            if (key_t == 0) {                          // reached by ties at the floor only
+            uint32_t key_t = sh.thr;
+            u64 n_t = 0;
+            at = at0;
+            for (int i = i0; i < min(i0 + per, nc); i++) {
+                if (~static_cast<uint32_t>(sh.cand[i] >> 32) == key_t && at < need) n_t++;
+                at += measure_of(sh.cand[i]);
+            }
+            n_t = cta_sum(n_t, sh.red);
+            if (key_t == 0) {                                // reached by ties at the floor only
                 key_t = fk;
-                eq = min((need - sh.before - tot + fw - 1) / max(fw, 1ull), ft);
+                n_t = min((need - sh.before - tot + fw - 1) / max(fw, 1ull), ft);
             }
             __syncthreads();
             if (tid < kC) {
-                st_u32(peer(&xc.thr, tid), key_t);
-                st_u64(peer(&xc.ties, tid), eq);
+                st_u32(peer(&sh.thr, tid), key_t);
+                st_u64(peer(&sh.ties, tid), n_t);
             }
         }
         cluster_sync();
-        thr = xc.thr;
-        ties = xc.ties;
+        thr = sh.thr;
+        ties = sh.ties;
     }
     // ---------------- the draw over all CTAs: per warp (its stretch of indexes) the kept weight above the threshold and
     // the tokens at it
     const u64 w_thr = thr ? row.whole(logit_of_key(thr)) : 0ull;
     const bool thr_ok = thr && row.weight(logit_of_key(thr)) >= mp;
+    const float x_thr = thr ? logit_of_key(thr) : -INFINITY;
     auto part = [&](float v, u64 &s, unsigned &q) {
-        const uint32_t key = key_of(v);
         const float w = row.weight(v);
-        if (key > thr && w >= mp) s += whole_of(w);
-        q += key == thr && thr_ok ? 1u : 0u;
+        if (v > x_thr && w >= mp) s += whole_of(w);
+        q += v == x_thr && thr_ok ? 1u : 0u;
     };
     {
         u64 s = 0;
@@ -726,8 +760,8 @@ __global__ void __launch_bounds__(kNT, 2) k_sample_cluster(SampleArgs a, int reg
         if (lane <= kNW) sh.ent[warp][lane] = inc - v;   // (lane kNW: the total)
         const u64 all = __shfl_sync(0xffffffffu, inc, 31);
         if (lane < kC) {
-            if (warp == 0) st_u64(peer(&xc.sum[0][rank], lane), all);
-            else st_u32(peer(&xc.cnt[0][rank], lane), static_cast<unsigned>(all));
+            if (warp == 0) st_u64(peer(&sh.sum[0][rank], lane), all);
+            else st_u32(peer(&sh.cnt[0][rank], lane), static_cast<unsigned>(all));
         }
     }
     cluster_sync();
@@ -738,8 +772,8 @@ __global__ void __launch_bounds__(kNT, 2) k_sample_cluster(SampleArgs a, int reg
             s_me = s_all;
             q_me = q_all;
         }
-        s_all += xc.sum[0][r];
-        q_all += xc.cnt[0][r];
+        s_all += sh.sum[0][r];
+        q_all += sh.cnt[0][r];
     }
     // the kept weight before a place with s above the threshold and q tokens at it before it
     auto kept = [&](u64 s, u64 q) { return s + min(q, ties) * w_thr; };
@@ -781,7 +815,7 @@ cudaError_t launch_sample(const SampleArgs &a, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(a.n_rows) * kC);
     cfg.blockDim = dim3(kNT);
-    cfg.dynamicSmemBytes = static_cast<size_t>(region) * kNW * 4;
+    cfg.dynamicSmemBytes = std::max(static_cast<size_t>(region) * kNW * 4, static_cast<size_t>(kCap) * 8);   // (solve sorts there)
     cfg.stream = st;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
