@@ -55,9 +55,8 @@ __device__ __forceinline__ u64 part_of(u64 of, u64 total) {
 // floor(w 2^40) for 0 <= w <= 1, by its bits (a conversion to 64 bits costs
 // several times the shift)
 __device__ __forceinline__ u64 whole_of(float w) {
-    const uint32_t b = __float_as_uint(w), e = b >> 23, f = (b & 0x7FFFFFu) | 0x800000u;
-    if (e >= 110) return static_cast<u64>(f) << (e - 110);
-    return e >= 87 ? f >> (110 - e) : 0u;
+    const uint32_t b = __float_as_uint(w), f = (b & 0x7FFFFFu) | 0x800000u;
+    return (static_cast<u64>(f) << 17) >> min(127u - (b >> 23), 63u);   // (below 2^-40, and 0: shifted out)
 }
 
 struct Row {
@@ -329,24 +328,60 @@ __device__ __forceinline__ float logit_of_key(uint32_t key) {
     return __uint_as_float((key & 0x80000000u) ? (key & 0x7FFFFFFFu) : ~key);
 }
 
+// E values per thread, neighbours: strides below E in registers, below 32 E by
+// shuffles, the rest through buf
+template <int E>
+__device__ __forceinline__ void cta_sort_regs(u64 *buf) {
+    const int t = threadIdx.x;
+    u64 v[E];
+#pragma unroll
+    for (int i = 0; i < E; i++) v[i] = buf[E * t + i];
+    for (int size = 2; size <= E * kNT; size <<= 1) {
+        for (int stride = size >> 1; stride >= 32 * E; stride >>= 1) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < E; i++) buf[E * t + i] = v[i];
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < E; i++) {
+                const int at = E * t + i;
+                const u64 w = buf[at ^ stride];
+                v[i] = ((at & stride) == 0) == ((at & size) == 0) ? min(v[i], w) : max(v[i], w);
+            }
+        }
+        for (int stride = min(size >> 1, 16 * E); stride >= E; stride >>= 1)
+#pragma unroll
+            for (int i = 0; i < E; i++) {
+                const int at = E * t + i;
+                const u64 w = __shfl_xor_sync(0xffffffffu, v[i], stride / E);
+                v[i] = ((at & stride) == 0) == ((at & size) == 0) ? min(v[i], w) : max(v[i], w);
+            }
+#pragma unroll
+        for (int stride = E / 2; stride; stride >>= 1)
+            if (stride < size)
+#pragma unroll
+                for (int i = 0; i < E; i++)
+                    if ((i & stride) == 0) {
+                        const u64 x = v[i], y = v[i + stride];
+                        const bool up = ((E * t + i) & size) == 0;
+                        v[i] = up ? min(x, y) : max(x, y);
+                        v[i + stride] = up ? max(x, y) : min(x, y);
+                    }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < E; i++) buf[E * t + i] = v[i];
+    __syncthreads();
+}
+
 // buf[0, n) sorted ascending (n a power of two, 32 or more): bitonic; up to one
 // value per thread, strides below a warp by shuffles
 __device__ __forceinline__ void cta_sort(u64 *buf, int n) {
     const int t = threadIdx.x;
     __syncthreads();
     if (n > kNT) {
-        for (int size = 2; size <= n; size <<= 1)
-            for (int stride = size >> 1; stride; stride >>= 1) {
-                for (int p = t; p < n / 2; p += kNT) {
-                    const int i = 2 * p - (p & (stride - 1)), j = i + stride;   // i has no `stride` bit
-                    const u64 v = buf[i], w = buf[j];
-                    if ((v > w) == ((i & size) == 0)) {
-                        buf[i] = w;
-                        buf[j] = v;
-                    }
-                }
-                __syncthreads();
-            }
+        if (n == 2 * kNT) cta_sort_regs<2>(buf);
+        else cta_sort_regs<4>(buf);
         return;
     }
     u64 v = t < n ? buf[t] : ~0ull;
@@ -465,9 +500,51 @@ __global__ void __launch_bounds__(kNT, 2) k_sample_cluster(SampleArgs a, int reg
     // keep the first ones, min-p too; then the draw in index order.  need_p: top-p's sum, where it is known.
     u64 *buf = reinterpret_cast<u64 *>(xs);       // (its own logits are no longer needed then)
     auto solve = [&](int nc, auto cand, bool p_known, u64 need_p) {
+        if (nc <= 96) {
+            // few: each candidate's thread counts and sums over the others
+            u64 *wk = buf + 128, *wd = buf + 256;
+            const u64 v = tid < nc ? cand(tid) : ~0ull;
+            const uint32_t key = ~static_cast<uint32_t>(v >> 32);
+            const float xv = logit_of_key(key);
+            const u64 w = tid < nc ? row.whole(xv) : 0ull;
+            __syncthreads();
+            if (tid < nc) buf[tid] = v;
+            __syncthreads();
+            int place = 0;
+            if (tid < nc) {
+                for (int i = 0; i < nc; i++) place += buf[i] < v;
+                wk[tid] = place < k ? w : 0ull;
+            }
+            __syncthreads();
+            if (tid < nc) {
+                bool kept = place < k && row.weight(xv) >= mp;
+                if (by_p) {
+                    u64 before = 0, tot = 0;
+                    for (int i = 0; i < nc; i++) {
+                        const u64 x = wk[i];
+                        before += buf[i] < v ? x : 0ull;
+                        tot += x;
+                    }
+                    kept = kept && before < (p_known ? need_p : max(part_of(p24, tot), 1ull));
+                }
+                wd[tid] = kept ? w : 0ull;
+            }
+            __syncthreads();
+            if (tid < nc && wd[tid]) {
+                u64 at = 0, tot = 0;
+                for (int i = 0; i < nc; i++) {
+                    const u64 x = wd[i];
+                    at += static_cast<uint32_t>(buf[i]) < static_cast<uint32_t>(v) ? x : 0ull;
+                    tot += x;
+                }
+                const u64 target = part_of(u24, tot);
+                if (at <= target && target < at + wd[tid]) finish(static_cast<int>(static_cast<uint32_t>(v)), xv, tot);
+            }
+            return;
+        }
         int n2 = 32;
         while (n2 < nc) n2 <<= 1;
-        const int per = max(1, n2 / kNT), i0 = tid * per;   // a thread's values, neighbours
+        int per = max(1, n2 / kNT), i0 = tid * per;   // a thread's values, neighbours
         __syncthreads();
         for (int i = tid; i < n2; i += kNT) buf[i] = i < nc ? cand(i) : ~0ull;
         cta_sort(buf, n2);
@@ -478,6 +555,7 @@ __global__ void __launch_bounds__(kNT, 2) k_sample_cluster(SampleArgs a, int reg
             before = cta_prefix(w, sh.red, tot);
         }
         const u64 need = !by_p ? ~0ull : p_known ? need_p : max(part_of(p24, tot), 1ull);
+        unsigned n_kept = 0;
         for (int i = i0; i < i0 + per && i < n2; i++) {
             const u64 v = buf[i];
             const uint32_t key = ~static_cast<uint32_t>(v >> 32);
@@ -486,7 +564,14 @@ __global__ void __launch_bounds__(kNT, 2) k_sample_cluster(SampleArgs a, int reg
             const bool kept = in && before < need && row.weight(xv) >= mp;
             if (by_p && in) before += row.whole(xv);
             buf[i] = kept ? ((v & 0xFFFFFFFFull) << 32) | key : ~0ull;
+            n_kept += kept;
         }
+        // (the kept ones are the first of the order)
+        n_kept = static_cast<unsigned>(cta_sum(n_kept, sh.red));
+        n2 = 32;
+        while (n2 < static_cast<int>(n_kept)) n2 <<= 1;
+        per = max(1, n2 / kNT);
+        i0 = tid * per;
         cta_sort(buf, n2);
         u64 w = 0;
         for (int i = i0; i < i0 + per && i < n2; i++)
@@ -505,17 +590,20 @@ __global__ void __launch_bounds__(kNT, 2) k_sample_cluster(SampleArgs a, int reg
     uint32_t thr = 0;          // kept: keys above thr, and the first `ties` at it
     u64 ties = 0;
     if (by_k && k <= kTopK) {
-        // the k-th largest of the 128 maxima: thread t counts those before maximum t
-        if (tid < kC * kNW) {
-            const float mine = sh.top[tid];
+        // the k-th largest of the 128 maxima: four threads each count a quarter of those before maximum t
+        {
+            const int t = tid >> 2, i0 = (tid & 3) * 4;
+            const float mine = sh.top[t];
             int before = 0;
-#pragma unroll 8
-            for (int i = 0; i < kC * kNW; i += 4) {
+#pragma unroll
+            for (int i = i0; i < kC * kNW; i += 16) {
                 const float4 v = *reinterpret_cast<const float4 *>(&sh.top[i]);
-                before += (v.x > mine || (v.x == mine && i < tid)) + (v.y > mine || (v.y == mine && i + 1 < tid)) +
-                          (v.z > mine || (v.z == mine && i + 2 < tid)) + (v.w > mine || (v.w == mine && i + 3 < tid));
+                before += (v.x > mine || (v.x == mine && i < t)) + (v.y > mine || (v.y == mine && i + 1 < t)) +
+                          (v.z > mine || (v.z == mine && i + 2 < t)) + (v.w > mine || (v.w == mine && i + 3 < t));
             }
-            if (before == k - 1) sh.bound = mine;
+            before += __shfl_xor_sync(0xffffffffu, before, 1);
+            before += __shfl_xor_sync(0xffffffffu, before, 2);
+            if (before == k - 1 && (tid & 3) == 0) sh.bound = mine;
         }
         __syncthreads();
         const float bound = sh.bound;
@@ -600,9 +688,10 @@ __global__ void __launch_bounds__(kNT, 2) k_sample_cluster(SampleArgs a, int reg
 #pragma unroll
         for (int i = 0; i < 3; i++) reinterpret_cast<uint4 *>(sh.hist[i])[tid] = z4;
         __syncthreads();
+        const float x_floor = fk ? logit_of_key(fk) : -INFINITY;
         each([&](int, float v) {
             const int s = step_of(v);
-            if (s >= kBins || key_of(v) <= fk) return;       // (tokens at the floor are added below)
+            if (s >= kBins || v <= x_floor) return;          // (tokens at the floor are added below)
             if (!weigh) {
                 atomicAdd(&sh.hist[0][s], 1u);
             } else {   // a 64-bit sum as two words: the carry goes with the high one
@@ -645,13 +734,30 @@ __global__ void __launch_bounds__(kNT, 2) k_sample_cluster(SampleArgs a, int reg
             }
         cluster_sync();
         const int step = static_cast<int>(sh.step);
+        // the smallest logits down to the step, and down to the one before: 32 candidates at a time (step_of falls with
+        // the logit), so that the passes below only compare
+        auto least = [&](int st) {
+            u64 l = 0, h = key_of(m);                        // step_of(h) <= st; of l - 1, if there is one, > st
+            while (l < h) {
+                const u64 d = h - l, mid = l + d * lane / 32;
+                const float xv = logit_of_key(static_cast<uint32_t>(mid));
+                const unsigned ok = __ballot_sync(0xffffffffu, xv == xv && step_of(xv) <= st);   // lanes from the first on
+                const int f = ok ? __ffs(ok) - 1 : 32;
+                const u64 nh = f < 32 ? l + d * f / 32 : h;
+                l = f > 0 ? l + d * (f - 1) / 32 + 1 : l;
+                h = nh;
+            }
+            return logit_of_key(static_cast<uint32_t>(h));
+        };
+        const float x_le = fmaxf(least(step), x_floor), x_lt = step > 0 ? least(step - 1) : INFINITY;
+        const bool top_step = step == 0;                     // (x_lt then bounds nothing)
+        auto in_le = [&](float v) { return v >= x_le && v > x_floor; };
+        auto in_eq = [&](float v) { return in_le(v) && (top_step || v < x_lt); };
         // how many tokens lie down to the step, and in it
         unsigned le = 0, eq = 0;
         each([&](int, float v) {
-            const int s = step_of(v);
-            if (key_of(v) <= fk) return;
-            le += s <= step;
-            eq += s == step;
+            le += in_le(v);
+            eq += in_eq(v);
         });
         le = static_cast<unsigned>(cta_sum(le, sh.red));
         eq = static_cast<unsigned>(cta_sum(eq, sh.red));
@@ -678,8 +784,7 @@ __global__ void __launch_bounds__(kNT, 2) k_sample_cluster(SampleArgs a, int reg
             continue;
         }
         each([&](int i, float v) {
-            const int s = step_of(v);
-            if (key_of(v) > fk && (small ? s <= step : s == step)) {
+            if (small ? in_le(v) : in_eq(v)) {
                 const unsigned at = (small ? o_le : o_eq) + atomicAdd(&sh.n_mine, 1u);
                 st_u64(peer(&sh.cand[at], 0), as_cand(i, v));
             }
