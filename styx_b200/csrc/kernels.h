@@ -408,7 +408,10 @@ struct PagedEvictArgs {
     int budget, n_recent, n_sink;
     float *acc_out;
     int32_t *pos_out, *lens_out;
-    int32_t *src, *places;         // workspace, [n_seqs][n_kv][budget] each: the rows that move, and the places they move to
+    // workspace: [n_seqs][n_kv][budget] each, the rows that move and the places they move to; their number,
+    // [n_seqs][n_kv]; the keys of lines too long for shared memory, [n_seqs][n_kv][max rows]
+    int32_t *src, *places, *moves;
+    uint32_t *keys;
 };
 struct SampleArgs {
     const float *logits;
@@ -431,7 +434,8 @@ cudaError_t launch_attend_tc(const PagedAttendArgs &a, const CUtensorMap &mk, co
                              cudaStream_t st);
 cudaError_t launch_attend_finish(const PagedAttendArgs &a, int nh, int pitch, cudaStream_t st);
 int attend_grid(const PagedAttendArgs &a, int nh, int sms);
-cudaError_t launch_paged_evict(const PagedEvictArgs &a, cudaStream_t st);
+cudaError_t launch_paged_evict(const PagedEvictArgs &a, int sms, cudaStream_t st);
+bool evict_staged(long long rows);   // the keys of lines of so many rows fit shared memory
 cudaError_t launch_sample(const SampleArgs &a, cudaStream_t st);
 
 // for the C entry points outside api.cu: makes the context's device current,

@@ -1,7 +1,8 @@
 // paged.cu -- rows into and out of a paged KV cache (include/styx_serve.h):
 //
 //   k_paged_append   per-head RMSNorm, RoPE and the rounded K / V rows
-//   k_paged_evict    the rows that stay, and the moves that close the gaps
+//   k_evict_select   the rows that stay, and the moves that close the gaps
+//   k_evict_move     K, V, weight and position of the rows that move
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -146,22 +147,24 @@ __global__ void __launch_bounds__(kAppThreads) k_paged_append(PagedAppendArgs a,
 
 // ------------------------------------------------------------ eviction
 constexpr int kEvThreads = 512, kEvWarps = kEvThreads / 32;
-constexpr int kEvSlice = 40960;   // keys that a CTA holds in shared memory
+constexpr int kEvSlice = 40960;               // keys that a CTA holds in shared memory
+constexpr int kEvBins = 2048, kEvShare = 4;   // steps of a round; of a thread
 
 // order of the weights as unsigned integers, larger first: protected rows
 // above all, NaN as -inf, -0 as +0
+constexpr uint32_t kProtected = 0xFFFFFFFFu;
 __device__ __forceinline__ uint32_t evict_key(float acc, int pos, int next_pos, int n_recent, int n_sink) {
-    if (static_cast<long long>(pos) >= static_cast<long long>(next_pos) - n_recent || pos < n_sink) return 0xFFFFFFFFu;
+    if (static_cast<long long>(pos) >= static_cast<long long>(next_pos) - n_recent || pos < n_sink) return kProtected;
     if (acc != acc) acc = -INFINITY;
     const uint32_t b = __float_as_uint(acc + 0.f);
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);   // +inf: 0xFF800000, below the protected rows' key
 }
 
-// what a cluster's CTAs write into each other
 struct EvictShared {
-    unsigned cnt[2][16][8];                      // [buffer][CTA][threshold]
-    unsigned ties[16], holes[16], movers[16];
-    unsigned w[2][kEvWarps][8], scan[kEvWarps];
+    __align__(16) unsigned hist[kEvBins];
+    unsigned scan[kEvWarps], red[3][kEvWarps];
+    // what a cluster's CTAs write into each other
+    unsigned lo[8], hi[8], prot[8], sum[8], bin, before, ties[8], holes[8], movers[8];
 };
 
 // exclusive prefix over the CTA, and the total
@@ -188,17 +191,19 @@ __device__ __forceinline__ unsigned cta_scan(unsigned v, unsigned *sh, unsigned 
 }
 
 // A cluster of C CTAs per line (sequence, kv head), each with a slice of its
-// rows, whose keys stay in shared memory (STAGED; else they are made again
-// from L2 each time).  The key of the budget-th row is found eightfold: seven
-// thresholds are counted at once, 11 rounds for 32 bits, one barrier each; no
-// atomics, so equal weights cost nothing extra.  Then rows are numbered in
-// order: who stays (keys above the threshold, the first rows at it), the
-// places below the budget that become free, the rows beyond it that stay;
-// the i-th of these moves into the i-th place.  Sources lie at or beyond the
-// budget, places below it, so no row is both.
+// rows, whose keys stay in shared memory (STAGED) or, above 40960 rows a CTA,
+// in the workspace.  The key of the last row that stays is found by rounds of
+// a histogram of 2048 equal steps over the range that is left of the keys
+// (first that of the line's own keys, so weights of one magnitude still
+// spread): three rounds at most.  Then rows are numbered in order, a
+// neighbourhood per thread: who stays (keys above the threshold, the first
+// rows at it), the places below the budget that become free, the rows beyond
+// it that stay; the i-th of these will move into the i-th place.
+// (Counting seven thresholds at once for eleven rounds took 17000 cycles of a
+// line of 2176 rows, scans tile by tile as many.)
 template <bool STAGED>
-__global__ void __launch_bounds__(kEvThreads) k_paged_evict(PagedEvictArgs a, int C, int row_bytes) {
-    extern __shared__ uint32_t keys[];
+__global__ void __launch_bounds__(kEvThreads) k_evict_select(PagedEvictArgs a, int C) {
+    extern __shared__ uint32_t staged[];
     __shared__ EvictShared sh;
     pdl_trigger();
     const PagedKv &kv = a.kv;
@@ -217,145 +222,211 @@ __global__ void __launch_bounds__(kEvThreads) k_paged_evict(PagedEvictArgs a, in
         if (C > 1) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cl_map(smem_addr(slot), to)), "r"(v) : "memory");
         else *slot = v;
     };
+    auto total = [&](const unsigned *v) {
+        unsigned t = 0;
+        for (int q = 0; q < C; q++) t += v[q];
+        return t;
+    };
     if (C > 1) cl_arrive_relaxed();   // the others have started: waited for before the first store to them
     pdl_wait();
-    const int n = paged_len(kv, b, tid == 0 && j == 0 && rank == 0);
+    const int n = paged_len(kv, b, tid == 0 && j == 0 && rank == 0), np = __ldg(a.next_pos + b);
     const int left = min(n, a.budget);
     const long long line = static_cast<long long>(line_no) * a.stride;
     const float *acc = a.acc + line;
     const int32_t *pos = a.pos + line;
     if (j == 0 && tid == 0 && rank == 0) a.lens_out[b] = left;
-    const int slice = (((n + C - 1) / C) + 3) & ~3, lo = min(n, rank * slice), hi = min(n, lo + slice), len = hi - lo;
+    const int slice = (n + C - 1) / C, first = min(n, rank * slice), len = min(n, first + slice) - first;
+    uint32_t *keys = STAGED ? staged : a.keys + (static_cast<long long>(line_no) * kv.max_pages << kv.page_shift) + first;
     if (C > 1) cl_wait();
     if (n <= a.budget) {   // all stay (every CTA of the cluster comes here)
-        for (int r = lo + tid; r < hi; r += kEvThreads) {
+        for (int r = first + tid; r < first + len; r += kEvThreads) {
             a.acc_out[line + r] = acc[r];
             a.pos_out[line + r] = pos[r];
         }
+        if (tid == 0 && rank == 0) a.moves[line_no] = 0;
         return;
     }
-    const int np = __ldg(a.next_pos + b);
-    if (STAGED) {
+    // ---------------- keys, their range, the protected rows
+    unsigned k_lo = 0xFFFFFFFFu, k_hi = 0, prot = 0;
 #pragma unroll 4
-        for (int i = tid; i < len; i += kEvThreads) keys[i] = evict_key(acc[lo + i], pos[lo + i], np, a.n_recent, a.n_sink);
-        __syncthreads();
+    for (int i = tid; i < len; i += kEvThreads) {
+        const uint32_t k = evict_key(acc[first + i], pos[first + i], np, a.n_recent, a.n_sink);
+        keys[i] = k;
+        if (k == kProtected) {
+            prot++;
+        } else {
+            k_lo = min(k_lo, k);
+            k_hi = max(k_hi, k);
+        }
     }
-    auto key_at = [&](int i) { return STAGED ? keys[i] : evict_key(acc[lo + i], pos[lo + i], np, a.n_recent, a.n_sink); };
-    // ---------------- threshold: at least `left` keys are >= t0, fewer are >= t1
-    unsigned long long t0 = 0, t1 = 1ull << 32;
-    unsigned above = 0;                                    // keys >= t1
-    for (int buf = 0; t1 - t0 > 1; buf ^= 1) {
-        const unsigned long long w = t1 - t0;
-        unsigned th[7], c[7];
-#pragma unroll
-        for (int i = 0; i < 7; i++) {
-            th[i] = static_cast<unsigned>(t0 + (w * (i + 1)) / 8);
-            c[i] = 0;
+    k_lo = __reduce_min_sync(0xffffffffu, k_lo);
+    k_hi = __reduce_max_sync(0xffffffffu, k_hi);
+    prot = __reduce_add_sync(0xffffffffu, prot);
+    if (lane == 0) {
+        sh.red[0][warp] = k_lo;
+        sh.red[1][warp] = k_hi;
+        sh.red[2][warp] = prot;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        k_lo = __reduce_min_sync(0xffffffffu, lane < kEvWarps ? sh.red[0][lane] : 0xFFFFFFFFu);
+        k_hi = __reduce_max_sync(0xffffffffu, lane < kEvWarps ? sh.red[1][lane] : 0u);
+        prot = __reduce_add_sync(0xffffffffu, lane < kEvWarps ? sh.red[2][lane] : 0u);
+        if (lane < C) {
+            tell(&sh.lo[rank], k_lo, lane);
+            tell(&sh.hi[rank], k_hi, lane);
+            tell(&sh.prot[rank], prot, lane);
         }
-        for (int i = tid; i < len; i += kEvThreads) {
-            const uint32_t k = key_at(i);
+    }
+    all_sync();
+    for (int q = 0; q < C; q++) {
+        k_lo = q ? min(k_lo, sh.lo[q]) : sh.lo[0];
+        k_hi = q ? max(k_hi, sh.hi[q]) : sh.hi[0];
+    }
+    prot = total(sh.prot);
+    // ---------------- threshold: `ties` of the rows at thr stay, and all above it
+    uint32_t thr = kProtected;
+    unsigned ties = static_cast<unsigned>(left);
+    if (prot < static_cast<unsigned>(left)) {
+        unsigned need = static_cast<unsigned>(left) - prot;       // of the keys in [k_lo, k_hi], the largest
+        while (k_hi > k_lo) {
+            const int shift = max(0, 21 - __clz(k_hi - k_lo));    // (range >> shift) < 2048
 #pragma unroll
-            for (int z = 0; z < 7; z++) c[z] += k >= th[z];
-        }
-        unsigned mine = 0;
-#pragma unroll
-        for (int z = 0; z < 7; z++) {
-            const unsigned s = __reduce_add_sync(0xffffffffu, c[z]);
-            if (lane == z) mine = s;
-        }
-        if (lane < 7) sh.w[buf][warp][lane] = mine;
-        __syncthreads();
-        // lane z of every warp: the CTA's count of threshold z
-        unsigned tot = 0;
-        if (lane < 7)
-#pragma unroll
-            for (int q = 0; q < kEvWarps; q++) tot += sh.w[buf][q][lane];
-        if (C > 1) {
-            if (warp < C && lane < 7) tell(&sh.cnt[buf][rank][lane], tot, warp);
+            for (int i = 0; i < kEvBins / 4 / kEvThreads; i++)
+                reinterpret_cast<uint4 *>(sh.hist)[tid + i * kEvThreads] = make_uint4(0, 0, 0, 0);
+            __syncthreads();
+#pragma unroll 4
+            for (int i = tid; i < len; i += kEvThreads) {
+                const uint32_t k = keys[i];
+                if (k >= k_lo && k <= k_hi) atomicAdd(&sh.hist[(k_hi - k) >> shift], 1u);   // step 0: the largest
+            }
             all_sync();
-            tot = 0;
-            if (lane < 7)
-                for (int q = 0; q < C; q++) tot += sh.cnt[buf][q][lane];
+            // the CTA's share of the steps, added up over the cluster, scanned from the largest down
+            const int share = kEvBins / C, per = (share + kEvThreads - 1) / kEvThreads, s0 = rank * share + tid * per;
+            unsigned c[kEvShare], mine = 0;
+#pragma unroll
+            for (int i = 0; i < kEvShare; i++) {
+                c[i] = 0;
+                if (i < per && tid * per + i < share) {
+                    if (C == 1) {
+                        c[i] = sh.hist[s0 + i];
+                    } else {
+                        unsigned v[8];
+#pragma unroll
+                        for (int q = 0; q < 8; q++) {
+                            v[q] = 0;
+                            if (q < C)
+                                asm volatile("ld.shared::cluster.u32 %0, [%1];"
+                                             : "=r"(v[q])
+                                             : "r"(cl_map(smem_addr(&sh.hist[s0 + i]), q))
+                                             : "memory");
+                        }
+#pragma unroll
+                        for (int q = 0; q < 8; q++) c[i] += v[q];
+                    }
+                }
+                mine += c[i];
+            }
+            unsigned tot, before = cta_scan(mine, sh.scan, tot);
+            if (C > 1) {
+                if (tid < C) tell(&sh.sum[rank], tot, tid);
+                all_sync();
+                for (int q = 0; q < rank; q++) before += sh.sum[q];
+            }
+#pragma unroll
+            for (int i = 0; i < kEvShare; i++) {
+                if (before < need && need <= before + c[i])
+                    for (int q = 0; q < C; q++) {
+                        tell(&sh.bin, s0 + i, q);
+                        tell(&sh.before, before, q);
+                    }
+                before += c[i];
+            }
+            all_sync();
+            need -= sh.before;
+            const uint32_t top = k_hi - (sh.bin << shift), width = (1u << shift) - 1;
+            k_lo = top - k_lo > width ? top - width : k_lo;
+            k_hi = top;
+            __syncthreads();   // (bin and before are read before the next round writes them)
         }
-        // thresholds rise, counts fall: the last that still reaches `left`
-        const unsigned reach = __ballot_sync(0xffffffffu, lane < 7 && tot >= static_cast<unsigned>(left));
-        const int z = __popc(reach) - 1;
-        const unsigned long long n0 = t0 + (w * (z + 1)) / 8, n1 = t0 + (w * (z + 2)) / 8;
-        if (z < 6) above = __shfl_sync(0xffffffffu, tot, z + 1);
-        t1 = z < 6 ? n1 : t1;
-        t0 = z < 0 ? t0 : n0;
+        thr = k_lo;
+        ties = need;
     }
-    const uint32_t thr = static_cast<uint32_t>(t0);
-    const unsigned ties = static_cast<unsigned>(left) - above;   // of the rows at thr, the first `ties` stay
-    // ---------------- numbering, in row order: ties, then places and movers
-    unsigned n_ties = 0;
-    for (int i = tid; i < len; i += kEvThreads) n_ties += key_at(i) == thr;
-    unsigned tot;
-    cta_scan(n_ties, sh.scan, tot);
+    // ---------------- numbering, in row order: a thread's neighbouring rows (an odd number: no bank is met twice)
+    const int per = ((len + kEvThreads - 1) / kEvThreads) | 1, i0 = min(len, tid * per), i1 = min(len, i0 + per);
+    unsigned n_ties = 0, tot;
+    for (int i = i0; i < i1; i++) n_ties += keys[i] == thr;
+    unsigned tie = cta_scan(n_ties, sh.scan, tot);
     if (tid < C) tell(&sh.ties[rank], tot, tid);
     all_sync();
-    unsigned tie0 = 0;
-    for (int q = 0; q < rank; q++) tie0 += sh.ties[q];
-    // pass 0 counts this slice's places and movers, pass 1 lists them
-    unsigned hole0 = 0, mover0 = 0;
-    for (int pass = 0; pass < 2; pass++) {
-        unsigned t_run = tie0, h_run = hole0, m_run = mover0;
-        for (int base = 0; base < len; base += kEvThreads) {
-            const int i = base + tid, r = lo + i;
-            const bool in = i < len;
-            const uint32_t k = in ? key_at(i) : 0u;
-            const unsigned tr = cta_scan(in && k == thr, sh.scan, tot);
-            const bool stay = in && (k > thr || (k == thr && t_run + tr < ties));
-            t_run += tot;
-            const bool hole = in && r < left && !stay, mover = in && r >= left && stay;
-            // (a tile's places and movers in one scan: counts below 2^16)
-            const unsigned hm = cta_scan((hole ? 1u : 0u) | (mover ? 1u << 16 : 0u), sh.scan, tot);
-            if (pass == 1) {
-                int32_t *lists = a.places + static_cast<long long>(line_no) * a.budget;
-                if (hole) lists[h_run + (hm & 0xFFFFu)] = r;
-                if (mover) (a.src + static_cast<long long>(line_no) * a.budget)[m_run + (hm >> 16)] = r;
-                if (in && r < left && stay) {
-                    a.acc_out[line + r] = acc[r];
-                    a.pos_out[line + r] = pos[r];
-                }
-            }
-            h_run += tot & 0xFFFFu;
-            m_run += tot >> 16;
-        }
-        if (pass == 0) {
-            if (tid < C) {
-                tell(&sh.holes[rank], h_run, tid);
-                tell(&sh.movers[rank], m_run, tid);
-            }
-            all_sync();
-            for (int q = 0; q < rank; q++) {
-                hole0 += sh.holes[q];
-                mover0 += sh.movers[q];
-            }
-        }
+    for (int q = 0; q < rank; q++) tie += sh.ties[q];
+    unsigned n_holes = 0, n_movers = 0;
+    for (int i = i0; i < i1; i++) {
+        const uint32_t k = keys[i];
+        const bool stay = k > thr || (k == thr && tie < ties);
+        tie += k == thr;
+        keys[i] = stay;
+        n_holes += !stay && first + i < left;
+        n_movers += stay && first + i >= left;
     }
-    all_sync();   // the lists are complete (and visible: release and acquire at cluster scope)
-    unsigned moves = 0;
-    for (int q = 0; q < C; q++) moves += sh.movers[q];
-    // ---------------- moves: a row's K and V by 16-byte pieces, half a warp each where they are 256 bytes
+    unsigned hole = cta_scan(n_holes, sh.scan, tot);
+    if (tid < C) tell(&sh.holes[rank], tot, tid);
+    unsigned mover = cta_scan(n_movers, sh.scan, tot);
+    if (tid < C) tell(&sh.movers[rank], tot, tid);
+    all_sync();
+    for (int q = 0; q < rank; q++) {
+        hole += sh.holes[q];
+        mover += sh.movers[q];
+    }
+    int32_t *from = a.src + static_cast<long long>(line_no) * a.budget, *to = a.places + static_cast<long long>(line_no) * a.budget;
+    for (int i = i0; i < i1; i++) {
+        if (!keys[i] && first + i < left) to[hole++] = first + i;
+        if (keys[i] && first + i >= left) from[mover++] = first + i;
+    }
+    if (tid == 0 && rank == 0) a.moves[line_no] = static_cast<int32_t>(total(sh.movers));
+    // rows that stay where they are
+#pragma unroll 4
+    for (int i = tid; i < min(len, left - first); i += kEvThreads)
+        if (keys[i]) {
+            a.acc_out[line + first + i] = acc[first + i];
+            a.pos_out[line + first + i] = pos[first + i];
+        }
+    if (C > 1) all_sync();   // no CTA leaves while another reads its counts
+}
+
+// Warp = four moves of a line: weight, position, and K and V by 16-byte
+// pieces, all four rows' loads in flight.  Sources lie at or beyond the
+// budget, places below it, so no row is both.
+__global__ void __launch_bounds__(256) k_evict_move(PagedEvictArgs a, int blocks, int row_bytes) {
+    pdl_trigger();
+    const PagedKv &kv = a.kv;
+    const int line_no = blockIdx.x / blocks, b = line_no / kv.n_kv, j = line_no - b * kv.n_kv;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const long long line = static_cast<long long>(line_no) * a.stride;
     const int32_t *from_l = a.src + static_cast<long long>(line_no) * a.budget;
     const int32_t *to_l = a.places + static_cast<long long>(line_no) * a.budget;
     const int pieces = row_bytes / 16, size = row_bytes / kv.hd;
-    for (unsigned i0 = (rank * kEvWarps + warp) * 4; i0 < moves; i0 += C * kEvWarps * 4) {
+    pdl_wait();
+    const int moves = __ldcg(a.moves + line_no);
+    for (int i0 = ((blockIdx.x - line_no * blocks) * 8 + warp) * 4; i0 < moves; i0 += blocks * 32) {
+        // lanes 0-3: the four sources, 4-7: their places; each looks its page up
+        int r = 0;
+        long long off = -1;
+        if (lane < 8 && i0 + (lane & 3) < moves) {
+            r = __ldcg((lane < 4 ? from_l : to_l) + i0 + (lane & 3));
+            off = paged_off(kv, b, j, r);
+            if (off < 0) atomicExch(kv.err, kErrBadPos);
+        }
+        const int place = __shfl_down_sync(0xffffffffu, r, 4);
+        if (lane < 4 && i0 + lane < moves) {
+            a.acc_out[line + place] = a.acc[line + r];
+            a.pos_out[line + place] = a.pos[line + r];
+        }
         long long from[4], to[4];
 #pragma unroll
         for (int z = 0; z < 4; z++) {
-            from[z] = to[z] = -1;
-            if (i0 + z < moves) {
-                const int s = __ldcg(from_l + i0 + z), d = __ldcg(to_l + i0 + z);
-                if (lane == 0) {
-                    a.acc_out[line + d] = acc[s];
-                    a.pos_out[line + d] = pos[s];
-                }
-                from[z] = paged_off(kv, b, j, s);
-                to[z] = paged_off(kv, b, j, d);
-                if ((from[z] < 0 || to[z] < 0) && lane == 0) atomicExch(kv.err, kErrBadPos);
-            }
+            from[z] = __shfl_sync(0xffffffffu, off, z);
+            to[z] = __shfl_sync(0xffffffffu, off, 4 + z);
         }
         for (int p = lane; p < 2 * pieces; p += 32) {
             char *pool = static_cast<char *>(p < pieces ? kv.k : kv.v);
@@ -369,7 +440,6 @@ __global__ void __launch_bounds__(kEvThreads) k_paged_evict(PagedEvictArgs a, in
                 if (from[z] >= 0 && to[z] >= 0) *reinterpret_cast<uint4 *>(pool + to[z] * size + at) = v[z];
         }
     }
-    if (C > 1) all_sync();   // no CTA leaves while another reads its counts
 }
 
 }  // namespace
@@ -391,17 +461,22 @@ cudaError_t launch_paged_append(const PagedAppendArgs &a, int sms, cudaStream_t 
     return two ? launch_pdl(k_paged_append<float, 2>, grid, block, 0, st, a, vec) : launch_pdl(k_paged_append<float, 1>, grid, block, 0, st, a, vec);
 }
 
-cudaError_t launch_paged_evict(const PagedEvictArgs &a, cudaStream_t st) {
-    const long long rows = static_cast<long long>(a.kv.max_pages) << a.kv.page_shift;
+// CTAs of a line: 4096 rows each, eight at most
+static int evict_ctas(long long rows) {
     int C = 1;
     while (C < 8 && rows > 4096ll * C) C <<= 1;
-    const long long slice = ((rows + C - 1) / C + 3) & ~3ll;
-    const bool staged = slice <= kEvSlice;
-    const int row_bytes = a.kv.hd * (a.kv.dtype == STYX_F32 ? 4 : 2);
+    return C;
+}
+bool evict_staged(long long rows) { return (rows + evict_ctas(rows) - 1) / evict_ctas(rows) <= kEvSlice; }
+
+cudaError_t launch_paged_evict(const PagedEvictArgs &a, int sms, cudaStream_t st) {
+    const long long rows = static_cast<long long>(a.kv.max_pages) << a.kv.page_shift;
+    const int C = evict_ctas(rows), lines = a.kv.n_seqs * a.kv.n_kv;
+    const bool staged = evict_staged(rows);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(a.kv.n_seqs) * a.kv.n_kv * C);
+    cfg.gridDim = dim3(static_cast<unsigned>(lines) * C);
     cfg.blockDim = dim3(kEvThreads);
-    cfg.dynamicSmemBytes = staged ? static_cast<size_t>(slice) * 4 : 0;
+    cfg.dynamicSmemBytes = staged ? static_cast<size_t>((rows + C - 1) / C) * 4 : 0;
     cfg.stream = st;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -411,10 +486,15 @@ cudaError_t launch_paged_evict(const PagedEvictArgs &a, cudaStream_t st) {
     at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = C > 1 ? 2 : 1;
-    if (!staged) return cudaLaunchKernelEx(&cfg, k_paged_evict<false>, a, C, row_bytes);
-    const cudaError_t e = cudaFuncSetAttribute(k_paged_evict<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kEvSlice * 4);
+    cudaError_t e = cudaSuccess;
+    if (staged) e = cudaFuncSetAttribute(k_evict_select<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kEvSlice * 4);
+    if (e == cudaSuccess)
+        e = staged ? cudaLaunchKernelEx(&cfg, k_evict_select<true>, a, C) : cudaLaunchKernelEx(&cfg, k_evict_select<false>, a, C);
     if (e != cudaSuccess) return e;
-    return cudaLaunchKernelEx(&cfg, k_paged_evict<true>, a, C, row_bytes);
+    // four moves a warp, at most eight CTAs per SM in all
+    const int blocks = std::max(1, std::min((a.budget + 31) / 32, 8 * sms / lines));
+    return launch_pdl(k_evict_move, dim3(static_cast<unsigned>(lines) * blocks), dim3(256), 0, st, a, blocks,
+                      a.kv.hd * (a.kv.dtype == STYX_F32 ? 4 : 2));
 }
 
 }  // namespace styx

@@ -107,6 +107,20 @@ AttendWs attend_ws(const styx_paged_kv *kv, int n_heads, bool with_acc, int sms)
     return w;
 }
 
+// evict's workspace: the moves' sources, places and number; the keys of long lines
+struct EvictWs {
+    uint64_t places, moves, keys, total;
+};
+EvictWs evict_ws(const styx_paged_kv *kv, int budget) {
+    EvictWs w{};
+    const uint64_t lines = static_cast<uint64_t>(kv->n_seqs) * kv->n_kv_heads;
+    w.places = a256(lines * budget * 4);
+    w.moves = w.places * 2;
+    w.keys = w.moves + a256(lines * 4);
+    w.total = w.keys + (styx::evict_staged(static_cast<long long>(max_rows(kv))) ? 0 : a256(lines * max_rows(kv) * 4));
+    return w;
+}
+
 #define CHECK(call)                                                                                \
     do {                                                                                           \
         int rc_ = (call);                                                                          \
@@ -250,7 +264,7 @@ int styx_paged_evict_workspace_bytes(const styx_paged_kv *kv, int budget, uint64
     styx::PagedKv o{};
     CHECK(check_kv(kv, false, o));
     NEED(out && budget > 0, "budget %d", budget);
-    *out = 2 * a256(static_cast<uint64_t>(kv->n_seqs) * kv->n_kv_heads * budget * 4);
+    *out = evict_ws(kv, budget).total;
     return STYX_OK;
 }
 
@@ -258,7 +272,8 @@ int styx_paged_evict(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv,
                      const int32_t *next_pos, int64_t stride, int budget, int n_recent, int n_sink, float *acc_out,
                      int32_t *pos_out, int32_t *lens_out, void *workspace, uint64_t workspace_bytes) {
     styx::PagedEvictArgs a{};
-    CHECK(styx::ctx_enter(ctx, nullptr, &a.kv.err));
+    int sms = 0;
+    CHECK(styx::ctx_enter(ctx, &sms, &a.kv.err));
     CHECK(check_kv(kv, true, a.kv));
     NEED(acc && pos && next_pos && acc_out && pos_out && lens_out && workspace, "null pointer");
     NEED(budget > 0 && n_recent >= 0 && n_sink >= 0 && static_cast<int64_t>(n_recent) + n_sink <= budget,
@@ -277,10 +292,10 @@ int styx_paged_evict(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv,
     };
     NEED(apart(acc, acc_out, lines) && apart(pos, pos_out, lines) && apart(kv->lens, lens_out, kv->n_seqs * 4ull),
          "acc_out, pos_out and lens_out must be other arrays than the inputs");
-    uint64_t need = 0;
-    CHECK(styx_paged_evict_workspace_bytes(kv, budget, &need));
-    NEED(workspace_bytes >= need && aligned(workspace, 256) && styx::range_ok(workspace, need),
-         "workspace: %llu bytes, 256-byte aligned, needed", static_cast<unsigned long long>(need));
+    const EvictWs w = evict_ws(kv, budget);
+    NEED(workspace_bytes >= w.total && aligned(workspace, 256) && styx::range_ok(workspace, w.total),
+         "workspace: %llu bytes, 256-byte aligned, needed", static_cast<unsigned long long>(w.total));
+    char *ws = static_cast<char *>(workspace);
     a.acc = acc;
     a.pos = pos;
     a.next_pos = next_pos;
@@ -291,9 +306,11 @@ int styx_paged_evict(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv,
     a.acc_out = acc_out;
     a.pos_out = pos_out;
     a.lens_out = lens_out;
-    a.src = static_cast<int32_t *>(workspace);
-    a.places = reinterpret_cast<int32_t *>(static_cast<char *>(workspace) + need / 2);
-    CK(styx::launch_paged_evict(a, S(stream)));
+    a.src = reinterpret_cast<int32_t *>(ws);
+    a.places = reinterpret_cast<int32_t *>(ws + w.places);
+    a.moves = reinterpret_cast<int32_t *>(ws + w.moves);
+    a.keys = reinterpret_cast<uint32_t *>(ws + w.keys);
+    CK(styx::launch_paged_evict(a, sms, S(stream)));
     return STYX_OK;
 }
 

@@ -334,7 +334,9 @@ def test_append_attend_agree_with_the_single_sequence_path():
                           ([300], 3, 80, 16, "f16", 128, 128, 0, "same"),
                           ([300, 300], 3, 80, 16, "f16", 128, 0, 0, "same"),
                           ([20000], 1, 8, 64, "f16", 7001, 50, 1, "ties"),
-                          ([70000], 1, 8, 64, "f16", 64, 8, 4, "plain")])
+                          ([70000], 1, 8, 64, "f16", 64, 8, 4, "plain"), ([9000], 2, 8, 64, "f16", 4096, 0, 0, "magnitudes"),
+                          ([3000, 4097], 2, 8, 32, "f16", 2500, 2400, 4, "plain"),
+                          ([400000, 5], 1, 8, 64, "f16", 300000, 1000, 4, "ties")])
 def test_evict(lens, n_kv, hd, page, dtype, budget, recent, sink, kind):
     rng = np.random.default_rng(sum(lens) + budget)
     kv, ks, vs = make_cache(rng, lens, n_kv, hd, page, dtype)
@@ -344,6 +346,9 @@ def test_evict(lens, n_kv, hd, page, dtype, budget, recent, sink, kind):
         acc = np.floor(acc * 3).astype(np.float32)
     elif kind == "same":
         acc[:] = 0.25
+    elif kind == "magnitudes":      # every exponent there is, subnormal weights among them
+        acc = np.exp2(rng.uniform(-149, 127, acc.shape)).astype(np.float32) * np.where(rng.uniform(size=acc.shape) < 0.1, -1, 1)
+        acc = acc.astype(np.float32)
     elif kind == "special":
         which = rng.integers(0, 8, acc.shape)
         for i, x in enumerate((np.nan, np.inf, -np.inf, 0.0, -0.0, -1.5)):
