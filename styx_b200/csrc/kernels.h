@@ -2,6 +2,7 @@
 // (internal to libstyx_moe.so; the public surface is include/styx_moe.h).
 #pragma once
 
+#include <atomic>
 #include <cstdint>
 #include <cuda.h>
 #include <cuda_fp16.h>
@@ -463,6 +464,19 @@ inline cudaError_t launch_pdl(Kern kern, dim3 grid, dim3 block, size_t smem, cud
     cfg.attrs = at;
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
+// Allows `kern` `bytes` of dynamic shared memory (always the same number for
+// one kernel), once per device: an eager caller does not pay for it each time.
+template <auto kern>
+inline cudaError_t allow_smem(int bytes) {
+    static std::atomic<unsigned long long> done{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1))) return e;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+    return e;
 }
 
 // Whether `grid` CTAs of `kern` (threads, smem bytes each) can all be

@@ -487,7 +487,7 @@ cudaError_t launch_paged_evict(const PagedEvictArgs &a, int sms, cudaStream_t st
     cfg.attrs = at;
     cfg.numAttrs = C > 1 ? 2 : 1;
     cudaError_t e = cudaSuccess;
-    if (staged) e = cudaFuncSetAttribute(k_evict_select<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kEvSlice * 4);
+    if (staged) e = allow_smem<k_evict_select<true>>(kEvSlice * 4);
     if (e == cudaSuccess)
         e = staged ? cudaLaunchKernelEx(&cfg, k_evict_select<true>, a, C) : cudaLaunchKernelEx(&cfg, k_evict_select<false>, a, C);
     if (e != cudaSuccess) return e;

@@ -469,7 +469,7 @@ template <class T, int LPR>
 cudaError_t launch(const PagedAttendArgs &a, int grid, cudaStream_t st) {
     constexpr int ring = Lay<T, LPR>::stage * Lay<T, LPR>::stages, join = kWarps * NH * 8 * LPR * 4;
     constexpr int smem = ring > join ? ring : join;
-    const cudaError_t e = cudaFuncSetAttribute(k_attend_fma<T, LPR>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    const cudaError_t e = allow_smem<k_attend_fma<T, LPR>>(smem);
     if (e != cudaSuccess) return e;
     return launch_pdl(k_attend_fma<T, LPR>, dim3(grid), dim3(kThreads), smem, st, a);
 }

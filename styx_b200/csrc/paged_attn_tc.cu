@@ -676,7 +676,7 @@ template <bool BF, int NH>
 cudaError_t launch(const PagedAttendArgs &a, const CUtensorMap &mk, const CUtensorMap &mv, int grid, cudaStream_t st) {
     constexpr int smem = Cfg<BF, NH>::smem;
     static_assert(smem <= 227 * 1024 - 6 * 1024, "shared memory");
-    cudaError_t e = cudaFuncSetAttribute(k_attend_tc<BF, NH>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaError_t e = allow_smem<k_attend_tc<BF, NH>>(smem);
     if (e != cudaSuccess) return e;
     e = launch_pdl(k_attend_tc<BF, NH>, dim3(grid), dim3(kThreads), smem, st, a, mk, mv);
     return e != cudaSuccess ? e : launch_attend_finish(a, NH, 128, st);

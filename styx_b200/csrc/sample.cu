@@ -915,7 +915,7 @@ cudaError_t launch_sample(const SampleArgs &a, cudaStream_t st) {
     if (a.n_vocab > kC * kSlice) return launch_pdl(k_sample, dim3(a.n_rows), dim3(kThreads), 0, st, a);
     const int region = ((a.n_vocab + kC * kNW - 1) / (kC * kNW) + 127) & ~127;
     const bool bulk = (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0 && a.row_stride % 4 == 0;
-    const cudaError_t e = cudaFuncSetAttribute(k_sample_cluster, cudaFuncAttributeMaxDynamicSharedMemorySize, kSlice * 4);
+    const cudaError_t e = allow_smem<k_sample_cluster>(kSlice * 4);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(a.n_rows) * kC);

@@ -672,33 +672,36 @@ def argmax_f32(x: torch.Tensor, out: Optional[torch.Tensor] = None, stream=None)
 _KV_TYPES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 
 
-def _f32(t: torch.Tensor, shape: tuple, what: str, device: torch.device) -> int:
-    if t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device:
-        raise ValueError(f"{what}: contiguous float32 {shape} on {device} expected, got {t.dtype} {tuple(t.shape)} "
-                         f"strides {t.stride()} on {t.device}")
-    return t.data_ptr()
+def _checked(t: torch.Tensor, dtype: torch.dtype, shape: tuple, what: str, index: int) -> int:
+    """The address of a contiguous tensor of that type and shape on that device; ValueError for any other."""
+    if t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.get_device() == index:
+        return t.data_ptr()
+    raise ValueError(f"{what}: contiguous {dtype} {tuple(shape)} on cuda:{index} expected, got {t.dtype} "
+                     f"{tuple(t.shape)} strides {t.stride()} on {t.device}")
 
 
-def _i32(t: torch.Tensor, shape: tuple, what: str, device: torch.device) -> int:
-    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device:
-        raise ValueError(f"{what}: contiguous int32 {shape} on {device} expected, got {t.dtype} {tuple(t.shape)} "
-                         f"strides {t.stride()} on {t.device}")
-    return t.data_ptr()
+def _f32(t: torch.Tensor, shape: tuple, what: str, index: int) -> int:
+    return _checked(t, torch.float32, shape, what, index)
 
 
-class _On:
-    """The stream a call runs on: the given one, else the current one of the
-    device.  What the call allocates belongs to that stream."""
+def _i32(t: torch.Tensor, shape: tuple, what: str, index: int) -> int:
+    return _checked(t, torch.int32, shape, what, index)
 
-    def __init__(self, device: torch.device, stream):
-        self.device, self.stream = device, stream
-        self.handle = (torch.cuda.current_stream(device) if stream is None else stream).cuda_stream
 
-    def empty(self, shape, dtype) -> torch.Tensor:
-        if self.stream is None:
-            return torch.empty(shape, dtype=dtype, device=self.device)
-        with torch.cuda.stream(self.stream):
-            return torch.empty(shape, dtype=dtype, device=self.device)
+def _current(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# (the same handle without building a Stream object, 0.1 us instead of 2.2, where torch has it)
+_current = getattr(torch._C, "_cuda_getCurrentRawStream", _current)
+
+
+def _empty(shape, dtype, device: torch.device, stream) -> torch.Tensor:
+    """A new tensor that belongs to the stream of the call."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
 
 
 class PagedKV:
@@ -724,8 +727,8 @@ class PagedKV:
         if table.dim() != 2 or table.dtype != torch.int32 or table.stride(1) != 1 or table.device != k.device:
             raise ValueError("table: int32 [n_seqs][max_pages] with contiguous rows on the pools' device")
         self.k, self.v, self.table = k, v, table
-        self.device = k.device
-        self.ctx = ctx(k.device.index)
+        self.device, self.index = k.device, k.device.index
+        self.ctx = ctx(self.index)
         self.n_seqs, self.n_kv_heads, self.head_dim = table.shape[0], n_kv, hd
         self.max_rows = table.shape[1] * page
         self._kv = _lib.PagedKv(k.data_ptr(), v.data_ptr(), k.stride(0) if n_pages > 1 else n_kv * page * hd,
@@ -733,8 +736,10 @@ class PagedKV:
                                 table.shape[1], table.stride(0) if self.n_seqs > 1 else table.shape[1])
         self._ref = C.byref(self._kv)
         self.lens = lens
-        self._attend_ws: dict[tuple, torch.Tensor] = {}
-        self._evict_ws: list[torch.Tensor] = []   # the last is in use; smaller ones may still be on a stream
+        self._lib = lib()
+        self._attend_ws: dict[tuple, tuple] = {}     # (heads, with weights) -> (tensor, address, bytes)
+        self._evict_ws: list[torch.Tensor] = []      # the last is in use; smaller ones may still be on a stream
+        self._evict_bytes: dict[int, int] = {}
 
     @property
     def lens(self) -> torch.Tensor:
@@ -742,7 +747,7 @@ class PagedKV:
 
     @lens.setter
     def lens(self, t: torch.Tensor) -> None:
-        self._kv.lens = _i32(t, (self.n_seqs,), "lens", self.device)
+        self._kv.lens = _i32(t, (self.n_seqs,), "lens", self.index)
         self._lens = t
 
     def append(self, q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor,
@@ -754,38 +759,43 @@ class PagedKV:
         pages; returns the rotated q.  Token t is of sequence seq[t] (None: t)
         and goes to its row row[t] (None: lens - 1).  q, k and v may be slices
         of one projection's output (any stride between tokens)."""
-        dev, hd = self.device, self.head_dim
+        dev, hd, n_kv = self.index, self.head_dim, self.n_kv_heads
         n, n_heads = pos.shape[0], 0 if q is None else q.shape[1]
-        on = _On(dev, stream)
-        ptrs = []
-        for t, heads, what in ((q, n_heads, "q"), (k, self.n_kv_heads, "k"), (v, self.n_kv_heads, "v")):
-            if t is None:
-                ptrs += [None, 0]
-                continue
-            if t.dtype != torch.float32 or t.shape != (n, heads, hd) or t.stride(2) != 1 or \
-                    (heads > 1 and t.stride(1) != hd) or t.device != dev:
-                raise ValueError(f"{what}: float32 [{n}][{heads}][{hd}] with contiguous heads on {dev} expected, got "
-                                 f"{t.dtype} {tuple(t.shape)} strides {t.stride()} on {t.device}")
-            ptrs += [t.data_ptr(), t.stride(0) if n > 1 else heads * hd]
-        if q is not None and out is None:
-            out = on.empty((n, n_heads, hd), torch.float32)
-        check(lib().styx_paged_append(
-            self.ctx.handle, on.handle, self._ref, n, n_heads, *ptrs,
-            None if q_norm is None else _f32(q_norm, (hd,), "q_norm", dev),
+        f32 = torch.float32
+
+        def rows(t, heads, what):
+            sn, sh, se = t.stride()
+            if t.dtype is f32 and t.shape == (n, heads, hd) and se == 1 and (sh == hd or heads == 1) and \
+                    t.get_device() == dev:
+                return t.data_ptr(), sn if n > 1 else heads * hd
+            raise ValueError(f"{what}: float32 [{n}][{heads}][{hd}] with contiguous heads on cuda:{dev} expected, got "
+                             f"{t.dtype} {tuple(t.shape)} strides {t.stride()} on {t.device}")
+
+        qp, qs, op = None, 0, None
+        if q is not None:
+            qp, qs = rows(q, n_heads, "q")
+            if out is None:
+                out = _empty((n, n_heads, hd), f32, self.device, stream)
+            op = _checked(out, f32, (n, n_heads, hd), "out", dev)
+        kp, ks = rows(k, n_kv, "k")
+        vp, vs = rows(v, n_kv, "v")
+        rc = self._lib.styx_paged_append(
+            self.ctx.handle, _current(dev) if stream is None else stream.cuda_stream, self._ref, n, n_heads, qp, qs,
+            kp, ks, vp, vs, None if q_norm is None else _f32(q_norm, (hd,), "q_norm", dev),
             None if k_norm is None else _f32(k_norm, (hd,), "k_norm", dev), eps, freq_base,
             _i32(pos, (n,), "pos", dev), None if seq is None else _i32(seq, (n,), "seq", dev),
-            None if row is None else _i32(row, (n,), "row", dev),
-            None if q is None else _f32(out, (n, n_heads, hd), "out", dev)))
+            None if row is None else _i32(row, (n,), "row", dev), op)
+        if rc:
+            check(rc)
         return out if q is not None else None
 
-    def _attend_workspace(self, n_heads: int, with_acc: bool, on: _On) -> torch.Tensor:
-        ws = self._attend_ws.get((n_heads, with_acc))
-        if ws is None:
-            nb = C.c_uint64()
-            check(lib().styx_paged_attend_workspace_bytes(self.ctx.handle, self._ref, n_heads, with_acc, C.byref(nb)))
-            ws = on.empty((nb.value,), torch.uint8)
-            check(lib().styx_paged_attend_workspace_init(self.ctx.handle, on.handle, ws.data_ptr(), nb.value))
-            self._attend_ws[(n_heads, with_acc)] = ws
+    def _attend_workspace(self, n_heads: int, with_acc: bool, stream=None) -> tuple:
+        nb = C.c_uint64()
+        check(self._lib.styx_paged_attend_workspace_bytes(self.ctx.handle, self._ref, n_heads, with_acc, C.byref(nb)))
+        t = _empty((nb.value,), torch.uint8, self.device, stream)
+        check(self._lib.styx_paged_attend_workspace_init(
+            self.ctx.handle, _current(self.index) if stream is None else stream.cuda_stream, t.data_ptr(), nb.value))
+        self._attend_ws[(n_heads, with_acc)] = ws = (t, t.data_ptr(), nb.value)
         return ws
 
     def attend(self, q: torch.Tensor, scale: Optional[float] = None, window: int = 0,
@@ -798,27 +808,27 @@ class PagedKV:
         the softmax denominators; with acc f32 [n_seqs][n_kv_heads][>= rows],
         acc_out (None: acc itself) receives it plus each row's weight summed
         over the kv head's q heads."""
-        dev, b, hd = self.device, self.n_seqs, self.head_dim
+        dev, b, hd = self.index, self.n_seqs, self.head_dim
         n_heads = q.shape[1] if q.dim() == 3 else 0
-        qp = _f32(q, (b, n_heads, hd), "q", dev)
-        on = _On(dev, stream)
+        shape = (b, n_heads, hd)
+        qp = _f32(q, shape, "q", dev)
         if out is None:
-            out = on.empty((b, n_heads, hd), torch.float32)
+            out = _empty(shape, torch.float32, self.device, stream)
         stride, accp, accop = 0, None, None
         if acc is not None:
             stride = acc.shape[-1]
-            shape = (b, self.n_kv_heads, stride)
-            accp = _f32(acc, shape, "acc", dev)
-            accop = accp if acc_out is None else _f32(acc_out, shape, "acc_out", dev)
+            lines = (b, self.n_kv_heads, stride)
+            accp = _f32(acc, lines, "acc", dev)
+            accop = accp if acc_out is None else _f32(acc_out, lines, "acc_out", dev)
         elif acc_out is not None:
             raise ValueError("acc_out without acc")
-        ws = self._attend_ws.get((n_heads, accp is not None))
-        if ws is None:
-            ws = self._attend_workspace(n_heads, accp is not None, on)
-        check(lib().styx_paged_attend(
-            self.ctx.handle, on.handle, self._ref, n_heads, qp, hd ** -0.5 if scale is None else scale, window,
-            _f32(out, (b, n_heads, hd), "out", dev), None if lse is None else _f32(lse, (b, n_heads), "lse", dev),
-            accp, accop, stride, ws.data_ptr(), ws.numel()))
+        ws = self._attend_ws.get((n_heads, accp is not None)) or self._attend_workspace(n_heads, accp is not None, stream)
+        rc = self._lib.styx_paged_attend(
+            self.ctx.handle, _current(dev) if stream is None else stream.cuda_stream, self._ref, n_heads, qp,
+            hd ** -0.5 if scale is None else scale, window, _f32(out, shape, "out", dev),
+            None if lse is None else _f32(lse, (b, n_heads), "lse", dev), accp, accop, stride, ws[1], ws[2])
+        if rc:
+            check(rc)
         return out
 
     def evict(self, acc: torch.Tensor, pos: torch.Tensor, next_pos: torch.Tensor, budget: int, n_recent: int = 0,
@@ -830,23 +840,27 @@ class PagedKV:
         that leave.  Returns (acc_out, pos_out, lens_out), new tensors of the
         shapes of acc, pos and lens; `lens` itself changes only when the
         caller assigns lens_out to it."""
-        dev, b = self.device, self.n_seqs
-        on = _On(dev, stream)
+        dev, b = self.index, self.n_seqs
         stride = acc.shape[-1]
         shape = (b, self.n_kv_heads, stride)
-        acc_out = on.empty(shape, torch.float32) if acc_out is None else acc_out
-        pos_out = on.empty(shape, torch.int32) if pos_out is None else pos_out
-        lens_out = on.empty((b,), torch.int32) if lens_out is None else lens_out
-        nb = C.c_uint64()
-        check(lib().styx_paged_evict_workspace_bytes(self._ref, budget, C.byref(nb)))
-        if not self._evict_ws or self._evict_ws[-1].numel() < nb.value:
-            self._evict_ws.append(on.empty((nb.value,), torch.uint8))
+        acc_out = _empty(shape, torch.float32, self.device, stream) if acc_out is None else acc_out
+        pos_out = _empty(shape, torch.int32, self.device, stream) if pos_out is None else pos_out
+        lens_out = _empty((b,), torch.int32, self.device, stream) if lens_out is None else lens_out
+        need = self._evict_bytes.get(budget)
+        if need is None:
+            nb = C.c_uint64()
+            check(self._lib.styx_paged_evict_workspace_bytes(self._ref, budget, C.byref(nb)))
+            need = self._evict_bytes[budget] = nb.value
+        if not self._evict_ws or self._evict_ws[-1].numel() < need:
+            self._evict_ws.append(_empty((need,), torch.uint8, self.device, stream))
         ws = self._evict_ws[-1]
-        check(lib().styx_paged_evict(
-            self.ctx.handle, on.handle, self._ref, _f32(acc, shape, "acc", dev), _i32(pos, shape, "pos", dev),
-            _i32(next_pos, (b,), "next_pos", dev), stride, budget, n_recent, n_sink,
-            _f32(acc_out, shape, "acc_out", dev), _i32(pos_out, shape, "pos_out", dev),
-            _i32(lens_out, (b,), "lens_out", dev), ws.data_ptr(), ws.numel()))
+        rc = self._lib.styx_paged_evict(
+            self.ctx.handle, _current(dev) if stream is None else stream.cuda_stream, self._ref,
+            _f32(acc, shape, "acc", dev), _i32(pos, shape, "pos", dev), _i32(next_pos, (b,), "next_pos", dev), stride,
+            budget, n_recent, n_sink, _f32(acc_out, shape, "acc_out", dev), _i32(pos_out, shape, "pos_out", dev),
+            _i32(lens_out, (b,), "lens_out", dev), ws.data_ptr(), ws.numel())
+        if rc:
+            check(rc)
         return acc_out, pos_out, lens_out
 
 
@@ -858,19 +872,21 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Optional[torch.Te
     [n] (styx_sample): temperature, top_k (int32), top_p and min_p are [n]
     tensors, None for 1, all, 1 and 0.  Returns (token int32 [n], logprob f32
     [n] under the distribution drawn from); token -1 where nothing is left."""
-    if logits.dim() != 2 or logits.dtype != torch.float32 or not logits.is_cuda or logits.stride(1) != 1:
+    if logits.dim() != 2 or logits.dtype is not torch.float32 or not logits.is_cuda or logits.stride(1) != 1:
         raise ValueError(f"logits: float32 [n][vocab] CUDA tensor with contiguous rows expected, got {logits.dtype} "
                          f"{tuple(logits.shape)} strides {logits.stride()} on {logits.device}")
     n, vocab = logits.shape
-    dev = logits.device
-    on = _On(dev, stream)
-    token = on.empty((n,), torch.int32) if token is None else token
-    logprob = on.empty((n,), torch.float32) if logprob is None else logprob
-    check(lib().styx_sample(
-        ctx(dev.index).handle, on.handle, logits.data_ptr(), logits.stride(0) if n > 1 else vocab, n, vocab,
-        _f32(u, (n,), "u", dev), None if temperature is None else _f32(temperature, (n,), "temperature", dev),
-        None if top_k is None else _i32(top_k, (n,), "top_k", dev),
-        None if top_p is None else _f32(top_p, (n,), "top_p", dev),
-        None if min_p is None else _f32(min_p, (n,), "min_p", dev), _i32(token, (n,), "token", dev),
-        _f32(logprob, (n,), "logprob", dev)))
+    dev, one = logits.get_device(), (n,)
+    token = _empty(one, torch.int32, logits.device, stream) if token is None else token
+    logprob = _empty(one, torch.float32, logits.device, stream) if logprob is None else logprob
+    rc = lib().styx_sample(
+        ctx(dev).handle, _current(dev) if stream is None else stream.cuda_stream, logits.data_ptr(),
+        logits.stride(0) if n > 1 else vocab, n, vocab, _f32(u, one, "u", dev),
+        None if temperature is None else _f32(temperature, one, "temperature", dev),
+        None if top_k is None else _i32(top_k, one, "top_k", dev),
+        None if top_p is None else _f32(top_p, one, "top_p", dev),
+        None if min_p is None else _f32(min_p, one, "min_p", dev), _i32(token, one, "token", dev),
+        _f32(logprob, one, "logprob", dev))
+    if rc:
+        check(rc)
     return token, logprob

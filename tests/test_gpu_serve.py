@@ -580,7 +580,7 @@ def test_refusals():
     assert L.styx_sample(cx, None, None, 4, 1, 4, None, None, None, None, None, None, None) == _lib.STYX_EINVAL
     assert L.styx_paged_attend(cx, None, None, 8, None, 1.0, 0, None, None, None, None, 0, None, 0) == _lib.STYX_EINVAL
     kv.attend(q)
-    ws = kv._attend_workspace(8, False, None)
+    ws = torch.zeros(1 << 22, dtype=torch.uint8, device=DEV)
     out = torch.empty_like(q)
     assert L.styx_paged_attend(cx, None, kv._ref, 8, q.data_ptr(), 1.0, 0, out.data_ptr(), None, None, None, 0,
                                ws.data_ptr(), 16) == _lib.STYX_EINVAL and b"workspace" in L.styx_last_error()
