@@ -1443,22 +1443,6 @@ EncodeTiledFn encode_tiled() {
     });
     return fn;
 }
-}  // namespace
-
-extern "C++" int styx::encode_map3(CUtensorMap *out, void *base, const uint64_t dims[3], const uint64_t strides[2],
-                      const uint32_t box[3]) {
-    EncodeTiledFn fn = encode_tiled();
-    NEED(fn, "cuTensorMapEncodeTiled is not available");
-    const cuuint64_t d[3] = {dims[0], dims[1], dims[2]}, st[2] = {strides[0], strides[1]};
-    const cuuint32_t bx[3] = {box[0], box[1], box[2]}, es[3] = {1, 1, 1};
-    const CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, base, d, st, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    NEED(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
-    return STYX_OK;
-}
-
-namespace {
 // The TMA descriptors of one expert matrix: for each source present (hot,
 // arena, full) a 3-D byte tensor {row bytes, rows, slabs} with strides {row
 // bytes, slab stride}, box {one 256-element chunk of a row, 128 rows, 1}.

@@ -393,6 +393,7 @@ struct PagedAttendArgs {
     long long acc_stride;
     float scale;
     int window, n_heads, gqa;
+    int ctas;                      // of the launch: portions are theirs
     // workspace (with acc_out): scores in units of log2, [n_seqs][n_kv][max
     // rows][gqa]; maximum and sum of every head, [n_seqs][n_heads][2]
     float *scores, *ml;
@@ -426,13 +427,9 @@ struct SampleArgs {
     int *err;                      // device error word
 };
 cudaError_t launch_paged_append(const PagedAppendArgs &a, int sms, cudaStream_t st);
-// attention on the FMA units; on the tensor cores (mk, mv map the pools as
-// {head_dim, n_kv * page rows, pages}, box 64 x min(page, 128) rows (V: 64),
-// 128-byte swizzle); and what ends both: portions of nh heads, pitch floats
-// each, joined, and the weights accumulated
-cudaError_t launch_attend_fma(const PagedAttendArgs &a, int sms, cudaStream_t st);
-cudaError_t launch_attend_tc(const PagedAttendArgs &a, const CUtensorMap &mk, const CUtensorMap &mv, int sms,
-                             cudaStream_t st);
+// attention on the FMA units; and what ends it: portions of nh heads, pitch
+// floats each, joined, and the weights accumulated (a.ctas set)
+cudaError_t launch_attend_fma(PagedAttendArgs a, int sms, cudaStream_t st);
 cudaError_t launch_attend_finish(const PagedAttendArgs &a, int nh, int pitch, cudaStream_t st);
 int attend_grid(const PagedAttendArgs &a, int nh, int sms);
 cudaError_t launch_paged_evict(const PagedEvictArgs &a, int sms, cudaStream_t st);
@@ -443,8 +440,6 @@ cudaError_t launch_sample(const SampleArgs &a, cudaStream_t st);
 // gives its SM count and error word; [p, p + bytes) inside its allocation
 int ctx_enter(styx_ctx *ctx, int *sms, int **err);
 bool range_ok(const void *p, uint64_t bytes);
-// cuTensorMapEncodeTiled of a 3-D map, 16-bit elements, 128-byte swizzle; strides in bytes
-int encode_map3(CUtensorMap *out, void *base, const uint64_t dims[3], const uint64_t strides[2], const uint32_t box[3]);
 
 // A launch with programmatic stream serialisation: the kernel may be
 // scheduled while the previous one on the stream drains (its CTAs start once

@@ -54,9 +54,9 @@ __global__ void __launch_bounds__(kAppThreads) k_paged_append(PagedAppendArgs a,
     pdl_wait();
     int buf = 0;
     for (int t = blockIdx.x; t < a.n_tokens; t += gridDim.x, buf ^= 1) {
-        const int b = a.seq ? __ldg(a.seq + t) : t, pos = __ldg(a.pos + t);
+        const int b = a.seq ? ld_now(a.seq + t) : t, pos = ld_now(a.pos + t);
         const bool seq_ok = static_cast<unsigned>(b) < static_cast<unsigned>(kv.n_seqs);
-        const int r = !seq_ok ? -1 : a.row ? __ldg(a.row + t) : __ldg(kv.lens + b) - 1;
+        const int r = !seq_ok ? -1 : a.row ? ld_now(a.row + t) : ld_now(kv.lens + b) - 1;
         bool row_ok = r >= 0 && r < (static_cast<long long>(kv.max_pages) << kv.page_shift);
         const long long off = row_ok ? paged_off(kv, b, 0, r) : -1;   // of kv head 0
         row_ok = off >= 0;
@@ -85,8 +85,8 @@ __global__ void __launch_bounds__(kAppThreads) k_paged_append(PagedAppendArgs a,
                     x[j][k] = y[j][k] = make_float2(0.f, 0.f);
                     if (i < half) {
                         if (vec) {
-                            x[j][k] = __ldcs(reinterpret_cast<const float2 *>(src + i));
-                            y[j][k] = __ldcs(reinterpret_cast<const float2 *>(src + half + i));
+                            x[j][k] = *reinterpret_cast<const float2 *>(src + i);
+                            y[j][k] = *reinterpret_cast<const float2 *>(src + half + i);
                         } else {
                             x[j][k] = make_float2(src[i], src[i + 1]);
                             y[j][k] = make_float2(src[half + i], src[half + i + 1]);
@@ -110,10 +110,10 @@ __global__ void __launch_bounds__(kAppThreads) k_paged_append(PagedAppendArgs a,
                     for (int k = 0; k < K; k++) {
                         const int i = 2 * lane + 64 * k;
                         if (i < half) {
-                            x[j][k].x *= scale * __ldg(w + i);
-                            x[j][k].y *= scale * __ldg(w + i + 1);
-                            y[j][k].x *= scale * __ldg(w + half + i);
-                            y[j][k].y *= scale * __ldg(w + half + i + 1);
+                            x[j][k].x *= scale * ld_now(w + i);
+                            x[j][k].y *= scale * ld_now(w + i + 1);
+                            y[j][k].x *= scale * ld_now(w + half + i);
+                            y[j][k].y *= scale * ld_now(w + half + i + 1);
                         }
                     }
                 }
@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(kEvThreads) k_evict_select(PagedEvictArgs a, i
     };
     if (C > 1) cl_arrive_relaxed();   // the others have started: waited for before the first store to them
     pdl_wait();
-    const int n = paged_len(kv, b, tid == 0 && j == 0 && rank == 0), np = __ldg(a.next_pos + b);
+    const int n = paged_len(kv, b, tid == 0 && j == 0 && rank == 0), np = ld_now(a.next_pos + b);
     const int left = min(n, a.budget);
     const long long line = static_cast<long long>(line_no) * a.stride;
     const float *acc = a.acc + line;
@@ -407,13 +407,13 @@ __global__ void __launch_bounds__(256) k_evict_move(PagedEvictArgs a, int blocks
     const int32_t *to_l = a.places + static_cast<long long>(line_no) * a.budget;
     const int pieces = row_bytes / 16, size = row_bytes / kv.hd;
     pdl_wait();
-    const int moves = __ldcg(a.moves + line_no);
+    const int moves = ld_cg(a.moves + line_no);
     for (int i0 = ((blockIdx.x - line_no * blocks) * 8 + warp) * 4; i0 < moves; i0 += blocks * 32) {
         // lanes 0-3: the four sources, 4-7: their places; each looks its page up
         int r = 0;
         long long off = -1;
         if (lane < 8 && i0 + (lane & 3) < moves) {
-            r = __ldcg((lane < 4 ? from_l : to_l) + i0 + (lane & 3));
+            r = ld_cg((lane < 4 ? from_l : to_l) + i0 + (lane & 3));
             off = paged_off(kv, b, j, r);
             if (off < 0) atomicExch(kv.err, kErrBadPos);
         }

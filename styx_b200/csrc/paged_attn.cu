@@ -1,7 +1,5 @@
 // paged_attn.cu -- attention of one new token per sequence over a paged KV
-// cache (styx_paged_attend, include/styx_serve.h): the form on the FMA units,
-// for f32 caches and for shapes that the tensor-core form (paged_attn_tc.cu)
-// does not take, and the finish of both.
+// cache (styx_paged_attend, include/styx_serve.h).
 //
 // k_attend_fma.  CTA (an equal share of the tile list, paged_split.cuh): eight
 // warps take rows in turn, LPR lanes per row with eight elements each, so that
@@ -113,7 +111,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_fma(PagedAttendArgs a) {
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 const int c = Y::elem(rl, e);
-                (&q[h][0].x)[e] = h < ng && c < hd ? __ldg(a.q + (h0 + h) * hd + c) * l2 : 0.f;
+                (&q[h][0].x)[e] = h < ng && c < hd ? ld_now(a.q + (h0 + h) * hd + c) * l2 : 0.f;
             }
         float2 o[NH][4];
 #pragma unroll
@@ -123,7 +121,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_fma(PagedAttendArgs a) {
         float m = kNone, l = 0.f;                    // of head myh, over this lane's rows
         auto page_of = [&](int it) {
             const int r = row0 + it * STEP;
-            return it < iters && r < hi ? __ldg(table + (r >> kv.page_shift)) : -1;
+            return it < iters && r < hi ? ld_now(table + (r >> kv.page_shift)) : -1;
         };
         // copies of iteration `it` into its stage; returns whether the row is seen
         auto copy = [&](int it, int page) {
@@ -301,9 +299,13 @@ __global__ void __launch_bounds__(256) k_attend_finish(PagedAttendArgs a, int jo
     pdl_wait();
     if (static_cast<int>(blockIdx.x) < joins) {
         const int at = blockIdx.x / (NHG / HPC), h = (blockIdx.x - at * (NHG / HPC)) * HPC + warp / WPH, w = warp % WPH;
-        const unsigned c = __ldcg(a.cnt + at);
+        const unsigned c = ld_cg(a.cnt + at);
         const int np = static_cast<int>(c & 0xFFFFu);
         if (np == 0) return;
+        if (static_cast<int>(c >> 16) + np > a.ctas) {   // (lengths that changed during the call)
+            if (threadIdx.x == 0) atomicExch(kv.err, kErrBadPos);
+            return;
+        }
         const int b = at / segs, seg = at - b * segs, j = seg / groups, g0 = (seg - j * groups) * NHG;
         const int own0 = static_cast<int>(c >> 16);
         const bool on = h < min(NHG, a.gqa - g0);
@@ -319,10 +321,10 @@ __global__ void __launch_bounds__(256) k_attend_finish(PagedAttendArgs a, int jo
                 for (int i = 0; i < 8; i++) {
                     const int k = i0 + i * WPH, p = min(k, np - 1);
                     const float *pp = part_at(a, own0 + p, p == 0);
-                    m[i] = __ldcg(pp + kAttendPart - 32 + h);
-                    l[i] = __ldcg(pp + kAttendPart - 16 + h);
+                    m[i] = ld_cg(pp + kAttendPart - 32 + h);
+                    l[i] = ld_cg(pp + kAttendPart - 16 + h);
 #pragma unroll
-                    for (int v = 0; v < NV; v++) x[i][v] = __ldcg(reinterpret_cast<const float4 *>(pp + h * 128 * NV) + v * 32 + lane);
+                    for (int v = 0; v < NV; v++) x[i][v] = ld_cg(reinterpret_cast<const float4 *>(pp + h * 128 * NV) + v * 32 + lane);
                 }
 #pragma unroll
                 for (int i = 0; i < 8; i++) top = fmaxf(top, m[i]);
@@ -398,17 +400,17 @@ __global__ void __launch_bounds__(256) k_attend_finish(PagedAttendArgs a, int jo
             __syncthreads();
             for (int g = warp; g < gn; g += 8) {
                 const int h = gc + g, seg = j * groups + h / NHG, hh = h % NHG;
-                const unsigned c = __ldcg(a.cnt + static_cast<long long>(b) * segs + seg);
-                const int np = static_cast<int>(c & 0xFFFFu), own0 = static_cast<int>(c >> 16);
+                const unsigned c = ld_cg(a.cnt + static_cast<long long>(b) * segs + seg);
+                const int own0 = static_cast<int>(c >> 16), np = min(static_cast<int>(c & 0xFFFFu), a.ctas - own0);
                 float M = kNone, L = 0.f;
                 if (np == 0) {
                     const float *ml = a.ml + 2 * (static_cast<long long>(b) * a.n_heads + j * a.gqa + h);
-                    M = __ldcg(ml);
-                    L = __ldcg(ml + 1);
+                    M = ld_cg(ml);
+                    L = ld_cg(ml + 1);
                 } else {
                     for (int i = lane; i < np; i += 32) {
                         const float *pp = part_at(a, own0 + i, i == 0);
-                        const float m = __ldcg(pp + kAttendPart - 32 + hh), l = __ldcg(pp + kAttendPart - 16 + hh);
+                        const float m = ld_cg(pp + kAttendPart - 32 + hh), l = ld_cg(pp + kAttendPart - 16 + hh);
                         const float top = fmaxf(M, m);
                         L = L * ex2(M - top) + l * ex2(m - top);
                         M = top;
@@ -432,11 +434,11 @@ __global__ void __launch_bounds__(256) k_attend_finish(PagedAttendArgs a, int jo
                 int g = 0;
                 if ((a.gqa & 3) == 0)
                     for (; g < gn; g += 4) {
-                        const float4 x = __ldcg(reinterpret_cast<const float4 *>(sc + g));
+                        const float4 x = ld_cg(reinterpret_cast<const float4 *>(sc + g));
                         w += ex2(x.x - s_M[g]) * s_L[g] + ex2(x.y - s_M[g + 1]) * s_L[g + 1] +
                              ex2(x.z - s_M[g + 2]) * s_L[g + 2] + ex2(x.w - s_M[g + 3]) * s_L[g + 3];
                     }
-                for (; g < gn; g++) w += ex2(__ldcg(sc + g) - s_M[g]) * s_L[g];
+                for (; g < gn; g++) w += ex2(ld_cg(sc + g) - s_M[g]) * s_L[g];
             }
         }
         if (r < n) a.acc_out[line + r] = old + w;
@@ -492,8 +494,8 @@ cudaError_t launch_attend_finish(const PagedAttendArgs &a, int nh, int pitch, cu
     return nh == 8 ? finish<8, 1>(a, st) : finish<16, 1>(a, st);
 }
 
-cudaError_t launch_attend_fma(const PagedAttendArgs &a, int sms, cudaStream_t st) {
-    const int grid = attend_grid(a, NH, sms);
+cudaError_t launch_attend_fma(PagedAttendArgs a, int sms, cudaStream_t st) {
+    const int grid = a.ctas = attend_grid(a, NH, sms);
     const cudaError_t e = a.kv.dtype == STYX_F16    ? launch_t<__half>(a, grid, st)
                           : a.kv.dtype == STYX_BF16 ? launch_t<__nv_bfloat16>(a, grid, st)
                                                     : launch_t<float>(a, grid, st);

@@ -45,7 +45,10 @@ struct Walk {
                 u = 0;
                 if (++seg == segs) {
                     seg = 0;
-                    b++;
+                    if (++b >= a.kv.n_seqs) {   // (lengths that changed during the call)
+                        end = at;
+                        return false;
+                    }
                     nt = Seq(a, b, false).nt;
                 }
             }

@@ -431,9 +431,9 @@ __global__ void __launch_bounds__(kNT, 2) k_sample_cluster(SampleArgs a, int reg
         mbar_arrive_expect_tx(&sh.bar, static_cast<uint32_t>(whole4) * 4);
         bulk_g2s(xs, src, static_cast<uint32_t>(whole4) * 4, &sh.bar);
     }
-    const float t = a.temperature ? __ldg(a.temperature + b) : 1.f, top_p = a.top_p ? __ldg(a.top_p + b) : 1.f;
-    const float min_p = a.min_p ? __ldg(a.min_p + b) : 0.f, u = __ldg(a.u + b);
-    int k = a.top_k ? __ldg(a.top_k + b) : 0;
+    const float t = a.temperature ? a.temperature[b] : 1.f, top_p = a.top_p ? a.top_p[b] : 1.f;
+    const float min_p = a.min_p ? a.min_p[b] : 0.f, u = a.u[b];
+    int k = a.top_k ? a.top_k[b] : 0;
     for (int i = whole4 + tid; i < slice; i += kNT) xs[i] = i < len ? src[i] : -INFINITY;
     __syncthreads();
     if (whole4) mbar_wait(&sh.bar, 0, a.err, kErrWaitFull);

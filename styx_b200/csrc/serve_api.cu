@@ -241,22 +241,7 @@ int styx_paged_attend(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv
     a.scores = reinterpret_cast<float *>(ws + w.scores);
     a.part = reinterpret_cast<float *>(ws + w.part);
     a.cnt = reinterpret_cast<unsigned *>(ws + w.cnt);
-    // the tensor cores take 16-bit rows of 64 to 128 elements in pages of 16
-    // rows or more (a TMA box of fewer rows would break the operands' 8-row
-    // groups); everything else runs on the FMA units
-    if (kv->dtype != STYX_F32 && kv->head_dim >= 64 && kv->head_dim <= 128 && kv->page_size >= 16) {
-        CUtensorMap mk, mv;
-        const uint64_t dims[3] = {static_cast<uint64_t>(kv->head_dim), static_cast<uint64_t>(kv->n_kv_heads) * kv->page_size,
-                                  static_cast<uint64_t>(kv->n_pages)};
-        const uint64_t strides[2] = {kv->head_dim * 2ull, static_cast<uint64_t>(kv->page_stride) * 2};
-        const uint32_t box_k[3] = {64, static_cast<uint32_t>(kv->page_size < 128 ? kv->page_size : 128), 1};
-        const uint32_t box_v[3] = {64, static_cast<uint32_t>(kv->page_size < 64 ? kv->page_size : 64), 1};
-        CHECK(styx::encode_map3(&mk, kv->k, dims, strides, box_k));
-        CHECK(styx::encode_map3(&mv, kv->v, dims, strides, box_v));
-        CK(styx::launch_attend_tc(a, mk, mv, sms, S(stream)));
-    } else {
-        CK(styx::launch_attend_fma(a, sms, S(stream)));
-    }
+    CK(styx::launch_attend_fma(a, sms, S(stream)));
     return STYX_OK;
 }
 
