@@ -26,7 +26,7 @@ COMMON = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler",
 # per-source extra flags: the synthetic quantiser must round like the C oracle
 EXTRA = {"synth.cu": ["-fmad=false"]}
 SOURCES = ["moe_kernels.cu", "moe_fused.cu", "moe_cluster.cu", "batch.cu", "attn.cu", "attn_fused.cu", "attn_cluster.cu",
-           "paged.cu", "paged_attn.cu", "sample.cu", "serve_api.cu", "synth.cu", "api.cu", "residency.cpp", "gguf.cpp"]
+           "paged.cu", "paged_attn.cu", "paged_attn_mma.cu", "sample.cu", "serve_api.cu", "synth.cu", "api.cu", "residency.cpp", "gguf.cpp"]
 HEADERS = ["common.cuh", "qdot.cuh", "kernels.h", "moe_common.cuh", "cluster.cuh", "ep_sync.cuh",
            "paged.cuh", "paged_split.cuh"]
 

@@ -427,9 +427,11 @@ struct SampleArgs {
     int *err;                      // device error word
 };
 cudaError_t launch_paged_append(const PagedAppendArgs &a, int sms, cudaStream_t st);
-// attention on the FMA units; and what ends it: portions of nh heads, pitch
-// floats each, joined, and the weights accumulated (a.ctas set)
+// attention on the FMA units, on the tensor cores; and what ends both:
+// portions of nh heads, pitch floats each, joined, and the weights
+// accumulated (a.ctas set)
 cudaError_t launch_attend_fma(PagedAttendArgs a, int sms, cudaStream_t st);
+cudaError_t launch_attend_mma(PagedAttendArgs a, int sms, cudaStream_t st);
 cudaError_t launch_attend_finish(const PagedAttendArgs &a, int nh, int pitch, cudaStream_t st);
 int attend_grid(const PagedAttendArgs &a, int nh, int sms);
 cudaError_t launch_paged_evict(const PagedEvictArgs &a, int sms, cudaStream_t st);

@@ -241,7 +241,13 @@ int styx_paged_attend(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv
     a.scores = reinterpret_cast<float *>(ws + w.scores);
     a.part = reinterpret_cast<float *>(ws + w.part);
     a.cnt = reinterpret_cast<unsigned *>(ws + w.cnt);
-    CK(styx::launch_attend_fma(a, sms, S(stream)));
+    // the tensor cores take 16-bit rows of up to 128 elements in pages of 16
+    // rows or more (a warp's 16 rows then lie together); everything else runs
+    // on the FMA units
+    if (kv->dtype != STYX_F32 && kv->head_dim <= 128 && kv->page_size >= 16)
+        CK(styx::launch_attend_mma(a, sms, S(stream)));
+    else
+        CK(styx::launch_attend_fma(a, sms, S(stream)));
     return STYX_OK;
 }
 
