@@ -14,12 +14,13 @@
 // significant bits, so q and p are split into 3 or 2 terms of the cache's
 // type that add up to 24 / 22 bits; products are exact, sums f32.
 //
-// A warp takes 16 rows at a time for itself: its copies (cp.async, 4 KB of K
-// and 4 KB of V, contiguous in the page) go round a ring of its own, three
-// deep, so that no warp waits for another between a portion's ends and 128 KB
-// or more per SM are in flight.  The maximum a row is measured against moves
-// only when a score passes it by 2^8.  The next portion's first copies are
-// issued before the last one's result is joined from the eight warps.
+// A warp takes 16 rows at a time for itself; with more than eight q heads per
+// kv head, two warps share them, eight heads each.  Copies (cp.async, 4 KB of
+// K or V, contiguous in the page) go round a ring of the team's own, so that
+// nobody else waits between a portion's ends and 160 KB per SM are in flight.
+// The maximum that a row is measured against moves only when a score passes
+// it by 2^8.  The next portion's first copies are issued before the last
+// one's result is joined from the eight warps.
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -30,12 +31,12 @@ namespace styx {
 namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kRows = 16;                      // rows of a warp at once
-constexpr int kBuf = kRows * 256;              // K or V of them, 256-byte rows (head_dim 128)
-constexpr int kStage = 2 * kBuf, kStages = 3;
-constexpr int kRing = kWarps * kStages * kStage;
+constexpr int kRows = 16;                      // rows of a tile
+constexpr int kUnit = kRows * 256;             // K or V of them, 256-byte rows (head_dim 128)
+constexpr int kUnits = 48;                     // of all rings
+constexpr int kRing = kUnits * kUnit;
 constexpr int kPad = 132;                      // floats of a head's O in the join: no two heads on one bank
-constexpr int kJoin = kWarps * 8 * kPad * 4;   // eight heads of every warp
+constexpr int kJoin = kWarps * 4 * kPad * 4;   // four heads of every warp
 constexpr float kSlack = 8.f;                  // log2 units a score may pass the maximum by
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool on) {   // off: zeros
@@ -94,9 +95,11 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t (&t)[BF ? 3 : 
     }
 }
 
-// a portion of the CTA's share: its rows [lo, hi) of one segment
+// a portion of the CTA's share: its rows [lo, hi) of one segment, tile i of
+// team t from row base + (i teams + t) 16 on (base: lo rounded down to 16)
+template <int TEAMS>
 struct Part {
-    int b, j, g0, ng, lo, hi, base, iters;   // base: lo rounded down to 16
+    int b, j, g0, ng, lo, hi, base, iters;
     long long h0;
     const int32_t *table;
     __device__ __forceinline__ void set(const PagedAttendArgs &a, const Walk &wk, int groups, int nh) {
@@ -110,92 +113,105 @@ struct Part {
         lo = max(s.first, (s.tile0 + wk.t0) * kTile);
         hi = min(s.n, (s.tile0 + wk.t1) * kTile);
         base = lo & ~(kRows - 1);
-        iters = hi > lo ? (hi - base + kRows * kWarps - 1) / (kRows * kWarps) : 0;
+        iters = hi > lo ? (hi - base + kRows * TEAMS - 1) / (kRows * TEAMS) : 0;
     }
 };
 
-// NT: eights of q heads of a group
-template <bool BF, int NT>
+// TEAM: warps that share a tile, eight q heads each; KS: 16-element steps of a
+// row (what head_dim leaves of them is zeros)
+template <bool BF, int TEAM, int KS>
 __global__ void __launch_bounds__(kThreads, 1) k_attend_mma(PagedAttendArgs a) {
-    constexpr int TERMS = BF ? 3 : 2, NH = 8 * NT;
-    extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ float s_m[kWarps][NH], s_l[kWarps][NH], s_M[NH], s_L[NH];
+    constexpr int TERMS = BF ? 3 : 2, NH = 8 * TEAM, TEAMS = kWarps / TEAM, S = kUnits / TEAMS;
+    extern __shared__ __align__(256) uint8_t smem[];   // (rows are swizzled by xor of address bits 4 to 7)
+    __shared__ float s_m[kWarps][8], s_l[kWarps][8], s_M[NH], s_L[NH];
     const PagedKv &kv = a.kv;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hd = kv.hd;
+    const int team = warp / TEAM, in = warp % TEAM;   // in: which eight heads
     const int lr = lane >> 2, lc = lane & 3;   // of the fragments: row (B: column), pair of columns
-    const int groups = (a.gqa + NH - 1) / NH, segs = kv.n_kv * groups, ksteps = (hd + 15) / 16, chunks = hd / 8;
+    const int groups = (a.gqa + NH - 1) / NH, segs = kv.n_kv * groups;
     long long T, G;
     Walk wk;
     pdl_trigger();
     pdl_wait();
     share_of<kThreads>(a, segs, *reinterpret_cast<Share<kThreads> *>(smem), wk, T, G);
     __syncthreads();                  // what it left in the ring is read
-    const uint32_t ring = smem_addr(smem) + warp * kStages * kStage;
+    const uint32_t ring = smem_addr(smem) + team * S * kUnit;
     float *so = reinterpret_cast<float *>(smem + kRing);
     const float l2 = a.scale * 1.4426950408889634f;   // scores in units of log2
-
-    // a tile's page: of its sixteen rows; -1: none
-    auto page_of = [&](const Part &p, int it) {
-        const int r = p.base + (it * kWarps + warp) * kRows;
-        return it < p.iters && r < p.hi ? ld_now(p.table + (r >> kv.page_shift)) : -1;
+    auto team_sync = [&] {
+        if constexpr (TEAM == 1) __syncwarp();
+        else asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(32 * TEAM) : "memory");
     };
-    // copies of tile `it` of p into slot; what lies outside [lo, hi) or in a page outside the pool is zeros
-    auto issue = [&](const Part &p, int it, int page, int slot) {
-        const int r0 = p.base + (it * kWarps + warp) * kRows;
-        const bool some = it < p.iters && r0 < p.hi, ok = static_cast<unsigned>(page) < static_cast<unsigned>(kv.n_pages);
-        if (some) {
-            if (!ok && lane == 0) atomicExch(kv.err, kErrBadPos);
-            const long long at = ok ? page * kv.page_stride + static_cast<long long>((p.j << kv.page_shift) +
-                                                                                     (r0 & ((1 << kv.page_shift) - 1))) * hd
-                                    : 0;
-            const uint8_t *k = static_cast<const uint8_t *>(kv.k) + at * 2, *v = static_cast<const uint8_t *>(kv.v) + at * 2;
-            const int c = lane & 15;
+
+    Part<TEAMS> P{};
+    // ---------------- the ring: units K(0), V(0), K(1), ... of the team's tiles
+    const bool col = (lane & 15) < hd / 8;
+    // the lane's copies of a unit: rows at_row + 2 TEAM i, swizzled chunk lane % 16
+    const int at_row = 2 * in + (lane >> 4), at_src = (at_row * hd + (col ? lane & 15 : 0) * 8) * 2;
+    const uint32_t at_dst = ring + at_row * 256 + (((lane & 15) ^ at_row) << 4);
+    int slot = 0;                     // of the next unit to be used
+    unsigned seen = 0;                // bit s: slot s holds a tile of which rows are seen
+    int kpage = -1, vpage = -1;       // the page of the next K, V to be copied; -1: none
+    auto page_of = [&](int it) {
+        const int r = P.base + (it * TEAMS + team) * kRows;
+        return it < P.iters && r < P.hi ? ld_now(P.table + (r >> kv.page_shift)) : -1;
+    };
+    // copies of K or V of tile `it` into slot s; rows outside [lo, hi) are zeros, a page outside the pool is reported
+    auto issue = [&](bool is_v, int it, int s) {
+        const int page = is_v ? vpage : kpage, r0 = P.base + (it * TEAMS + team) * kRows;
+        const bool some = it < P.iters && r0 < P.hi, ok = some && static_cast<unsigned>(page) < static_cast<unsigned>(kv.n_pages);
+        if (some && !ok && lane == 0) atomicExch(kv.err, kErrBadPos);
+        if (ok) {
+            const long long at = page * kv.page_stride + static_cast<long long>((P.j << kv.page_shift) +
+                                                                                (r0 & ((1 << kv.page_shift) - 1))) * hd;
+            const uint8_t *src = static_cast<const uint8_t *>(is_v ? kv.v : kv.k) + at * 2 + at_src;
+            const unsigned first = r0 + at_row - P.lo, rows = P.hi - P.lo;
 #pragma unroll
-            for (int i = 0; i < kRows / 2; i++) {
-                const int r = 2 * i + (lane >> 4);
-                const bool on = ok && c < chunks && r0 + r >= p.lo && r0 + r < p.hi;
-                const uint32_t dst = ring + slot * kStage + r * 256 + ((c ^ (r & 7)) << 4);
-                const int src = on ? r * hd * 2 + c * 16 : 0;
-                copy16(dst, k + src, on);
-                copy16(dst + kBuf, v + src, on);
-            }
+            for (int r = 0; r < kRows; r += 2 * TEAM)
+                copy16((at_dst ^ ((r & 7) << 4)) + s * kUnit + r * 256, src + 2 * r * hd, col && first + r < rows);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
-        return some && ok;
-    };
-
-    Part P;
-    bool have = wk.next(a, segs);
-    int slot = 0;                     // of the portion's next tile
-    unsigned seen = 0;                // bit s: slot s holds rows that are seen
-    int page = -1;
-    auto start = [&] {                // a portion's first copies
-        P.set(a, wk, groups, NH);
-        page = page_of(P, 0);
-        int s = slot;
-#pragma unroll
-        for (int i = 0; i < kStages - 1; i++) {
-            const int nx = page_of(P, i + 1);
-            const bool on = issue(P, i, page, s);
-            seen = on ? seen | (1u << s) : seen & ~(1u << s);
-            page = nx;
-            s = s + 1 == kStages ? 0 : s + 1;
+        seen = ok ? seen | (1u << s) : seen & ~(1u << s);
+        if (!is_v) {
+            vpage = kpage;
+            kpage = page_of(it + 1);
         }
     };
+    auto start = [&] {                // a portion's first copies
+        P.set(a, wk, groups, NH);
+        kpage = page_of(0);
+        int s = slot;
+#pragma unroll
+        for (int u = 0; u < S - 1; u++) {
+            issue(u & 1, u / 2, s);
+            s = s + 1 == S ? 0 : s + 1;
+        }
+    };
+    // unit (it, is_v) is there for the whole team, and the copies of the one S - 1 later are on their way, into the
+    // slot that the team has just read; returns the slot
+    auto advance = [&](bool is_v, int it) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
+        team_sync();
+        const int now = slot;
+        slot = slot + 1 == S ? 0 : slot + 1;
+        issue((is_v + S - 1) & 1, it + (is_v + S - 1) / 2, now == 0 ? S - 1 : now - 1);
+        return now;
+    };
+
+    bool have = wk.next(a, segs);
     if (have) start();
     while (have) {
         // ---------------- q as B fragments, in terms.  f16 has few exponents: a head's largest |q| is brought to
         // [2^9, 2^10), and fh says what its column of S is in units of its terms
-        uint32_t qf[NT][8][TERMS][2];
-        float fh[NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-            const int h = 8 * nt + lr;
+        uint32_t qf[KS][TERMS][2];
+        float fh[2];
+        {
+            const int h = 8 * in + lr;
             const float *q = a.q + (P.h0 + h) * hd + 2 * lc;
-            float2 v[8][2];
+            float2 v[KS][2];
             float mx = 0.f;
 #pragma unroll
-            for (int k = 0; k < 8; k++)
+            for (int k = 0; k < KS; k++)
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
                     const int d = 16 * k + 8 * i;
@@ -214,233 +230,205 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_mma(PagedAttendArgs a) {
                 up = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
                 down = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
             }
-            fh[nt][0] = __shfl_sync(0xffffffffu, down, 8 * lc);        // heads 2 lc, 2 lc + 1 of the eight
-            fh[nt][1] = __shfl_sync(0xffffffffu, down, 8 * lc + 4);
+            fh[0] = __shfl_sync(0xffffffffu, down, 8 * lc);        // heads 2 lc, 2 lc + 1 of the eight
+            fh[1] = __shfl_sync(0xffffffffu, down, 8 * lc + 4);
 #pragma unroll
-            for (int k = 0; k < 8; k++)
+            for (int k = 0; k < KS; k++)
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
                     uint32_t t[TERMS];
                     split2<BF>(v[k][i].x * up, v[k][i].y * up, t);
 #pragma unroll
-                    for (int z = 0; z < TERMS; z++) qf[nt][k][z][i] = t[z];
+                    for (int z = 0; z < TERMS; z++) qf[k][z][i] = t[z];
                 }
         }
-        float m[NT][2], l[NT][2], o[8][NT][4];
+        float m[2] = {kNone, kNone}, l[2] = {0.f, 0.f}, o[KS][4];
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-            m[nt][0] = m[nt][1] = kNone;
-            l[nt][0] = l[nt][1] = 0.f;
-#pragma unroll
-            for (int t = 0; t < 8; t++) o[t][nt][0] = o[t][nt][1] = o[t][nt][2] = o[t][nt][3] = 0.f;
-        }
+        for (int t = 0; t < KS; t++) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
+        const int hh = 8 * in + 2 * lc;        // the lane's heads of the group: hh, hh + 1
         float *scores = a.scores + (static_cast<long long>(P.b) * kv.n_kv + P.j) *
-                                       (static_cast<long long>(kv.max_pages) << kv.page_shift) * a.gqa + P.g0 + 2 * lc;
+                                       (static_cast<long long>(kv.max_pages) << kv.page_shift) * a.gqa + P.g0 + hh;
         for (int it = 0; it < P.iters; it++) {
-            {   // the tile kStages - 1 ahead, into the slot of the last one (which every lane has read)
-                __syncwarp();
-                const int nx = page_of(P, it + kStages), s = slot == 0 ? kStages - 1 : slot - 1;
-                const bool on = issue(P, it + kStages - 1, page, s);
-                seen = on ? seen | (1u << s) : seen & ~(1u << s);
-                page = nx;
-            }
-            asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
-            __syncwarp();
-            const uint32_t kt = ring + slot * kStage, vt = kt + kBuf;
-            const bool live = (seen >> slot) & 1;
-            slot = slot + 1 == kStages ? 0 : slot + 1;
-            const int r0 = P.base + (it * kWarps + warp) * kRows;
-            if (!live) {
-                // no row of it is seen: past the end, or in a page outside the pool
-                if (a.acc_out && r0 < P.hi)
+            const int r0 = P.base + (it * TEAMS + team) * kRows + lr;   // the lane's rows: r0, r0 + 8
+            const int kslot = advance(false, it);
+            const bool live = (seen >> kslot) & 1;
+            const bool in0 = r0 >= P.lo && r0 < P.hi, in1 = r0 + 8 >= P.lo && r0 + 8 < P.hi;
+            uint32_t pf[TERMS][2];
+            if (live) {
+                // ---------------- S^T: row lr (+ 8), heads 2 lc, + 1
+                float s[TERMS][4];
 #pragma unroll
-                    for (int i = 0; i < 2; i++)
-                        for (int h = 0; h < NH; h++)
-                            if ((h & 7) >> 1 == lc && h < P.ng && r0 + lr + 8 * i >= P.lo && r0 + lr + 8 * i < P.hi)
-                                scores[static_cast<long long>(r0 + lr + 8 * i) * a.gqa + h - 2 * lc] = -INFINITY;
-                continue;
-            }
-            // ---------------- S^T: row lr (+ 8), heads 2 lc, + 1
-            float s[NT][TERMS][4];
+                for (int z = 0; z < TERMS; z++) s[z][0] = s[z][1] = s[z][2] = s[z][3] = 0.f;
+                const uint32_t kt = ring + kslot * kUnit + (lane & 15) * 256 + (((lane >> 4) ^ (lane & 7)) << 4);
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++)
+                for (int k = 0; k < KS; k++) {
+                    uint32_t A[4];
+                    ldm4(kt ^ (k << 5), A);
 #pragma unroll
-                for (int z = 0; z < TERMS; z++) s[nt][z][0] = s[nt][z][1] = s[nt][z][2] = s[nt][z][3] = 0.f;
-            {
-                const int row = lane & 15;
-#pragma unroll
-                for (int k = 0; k < 8; k++)
-                    if (k < ksteps) {
-                        uint32_t A[4];
-                        ldm4(kt + row * 256 + (((2 * k + (lane >> 4)) ^ (row & 7)) << 4), A);
-#pragma unroll
-                        for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                            for (int z = 0; z < TERMS; z++) mma<BF>(s[nt][z], A, qf[nt][k][z][0], qf[nt][k][z][1]);
-                    }
-            }
-            const bool on[2] = {r0 + lr >= P.lo && r0 + lr < P.hi, r0 + lr + 8 >= P.lo && r0 + lr + 8 < P.hi};
-            float x[NT][4];                    // (row lr: heads 0, 1; row lr + 8: heads 0, 1)
-            bool up = false;
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++)
+                    for (int z = 0; z < TERMS; z++) mma<BF>(s[z], A, qf[k][z][0], qf[k][z][1]);
+                }
+                const bool on[2] = {in0, in1};
+                float x[4];                    // (row lr: heads 0, 1; row lr + 8: heads 0, 1)
+                bool up = false;
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    float y = s[nt][0][i] + s[nt][1][i];
-                    if constexpr (TERMS == 3) y = s[nt][0][i] + (s[nt][1][i] + s[nt][TERMS - 1][i]);
-                    x[nt][i] = on[i >> 1] ? (BF ? y : y * fh[nt][i & 1]) : -INFINITY;
-                    up |= x[nt][i] > m[nt][i & 1] + kSlack;
+                    float y = s[0][i] + s[1][i];
+                    if constexpr (TERMS == 3) y = s[0][i] + (s[1][i] + s[TERMS - 1][i]);
+                    x[i] = on[i >> 1] ? (BF ? y : y * fh[i & 1]) : -INFINITY;
+                    up |= x[i] > m[i & 1] + kSlack;
                 }
-            if (a.acc_out)
+                if (a.acc_out)
 #pragma unroll
-                for (int i = 0; i < 2; i++)
-                    if (on[i]) {
-                        float *sc = scores + static_cast<long long>(r0 + lr + 8 * i) * a.gqa;
-#pragma unroll
-                        for (int nt = 0; nt < NT; nt++) {
-                            if (8 * nt + 2 * lc < P.ng) sc[8 * nt] = x[nt][2 * i];
-                            if (8 * nt + 2 * lc + 1 < P.ng) sc[8 * nt + 1] = x[nt][2 * i + 1];
+                    for (int i = 0; i < 2; i++)
+                        if (on[i]) {
+                            float *sc = scores + static_cast<long long>(r0 + 8 * i) * a.gqa;
+                            if (hh < P.ng) sc[0] = x[2 * i];
+                            if (hh + 1 < P.ng) sc[1] = x[2 * i + 1];
                         }
-                    }
-            if (__any_sync(0xffffffffu, up)) {
-                // new maxima over the sixteen rows; what was summed against the old ones is rescaled
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++)
+                if (__any_sync(0xffffffffu, up)) {
+                    // new maxima over the sixteen rows; what was summed against the old ones is rescaled
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        float v = fmaxf(x[nt][e], x[nt][2 + e]);
+                        float v = fmaxf(x[e], x[2 + e]);
                         v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
                         v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
                         v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
-                        v = fmaxf(v, m[nt][e]);
-                        const float f = ex2(m[nt][e] - v);
-                        m[nt][e] = v;
-                        l[nt][e] *= f;
+                        v = fmaxf(v, m[e]);
+                        const float f = ex2(m[e] - v);
+                        m[e] = v;
+                        l[e] *= f;
 #pragma unroll
-                        for (int t = 0; t < 8; t++) {
-                            o[t][nt][e] *= f;
-                            o[t][nt][2 + e] *= f;
+                        for (int t = 0; t < KS; t++) {
+                            o[t][e] *= f;
+                            o[t][2 + e] *= f;
                         }
                     }
-            }
-            // ---------------- P^T as B fragments: eight rows by eight heads, transposed across the warp
-            uint32_t pf[NT][TERMS][2];
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++)
+                }
+                // ---------------- P^T as B fragments: eight rows by eight heads, transposed across the warp
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    const float p0 = on[i] ? ex2(x[nt][2 * i] - m[nt][0]) : 0.f, p1 = on[i] ? ex2(x[nt][2 * i + 1] - m[nt][1]) : 0.f;
-                    l[nt][0] += p0;
-                    l[nt][1] += p1;
+                    const float p0 = on[i] ? ex2(x[2 * i] - m[0]) : 0.f, p1 = on[i] ? ex2(x[2 * i + 1] - m[1]) : 0.f;
+                    l[0] += p0;
+                    l[1] += p1;
                     uint32_t t[TERMS];
                     // f16: p up to 2^8 is carried as p * 2^7, so that the second term of a small p keeps its bits
                     split2<BF>(BF ? p0 : p0 * 128.f, BF ? p1 : p1 * 128.f, t);
 #pragma unroll
-                    for (int z = 0; z < TERMS; z++) pf[nt][z][i] = transposed(t[z]);
+                    for (int z = 0; z < TERMS; z++) pf[z][i] = transposed(t[z]);
                 }
-            // ---------------- O^T += V^T P^T
-            {
-                const int row = (lane & 7) + ((lane >> 4) << 3), half = (lane >> 3) & 1;
+            } else if (a.acc_out) {            // rows of a page outside the pool
+                if (in0 && hh < P.ng) scores[static_cast<long long>(r0) * a.gqa] = -INFINITY;
+                if (in0 && hh + 1 < P.ng) scores[static_cast<long long>(r0) * a.gqa + 1] = -INFINITY;
+                if (in1 && hh < P.ng) scores[static_cast<long long>(r0 + 8) * a.gqa] = -INFINITY;
+                if (in1 && hh + 1 < P.ng) scores[static_cast<long long>(r0 + 8) * a.gqa + 1] = -INFINITY;
+            }
+            const int vslot = advance(true, it);
+            if (live) {
+                // ---------------- O^T += V^T P^T
+                const uint32_t vt = ring + vslot * kUnit + ((lane & 7) + ((lane >> 4) << 3)) * 256 +
+                                    ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
 #pragma unroll
-                for (int t = 0; t < 8; t++)
-                    if (t < ksteps) {
-                        uint32_t A[4];
-                        ldm4t(vt + row * 256 + (((2 * t + half) ^ (row & 7)) << 4), A);
+                for (int t = 0; t < KS; t++) {
+                    uint32_t A[4];
+                    ldm4t(vt ^ (t << 5), A);
 #pragma unroll
-                        for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                            for (int z = 0; z < TERMS; z++) mma<BF>(o[t][nt], A, pf[nt][z][0], pf[nt][z][1]);
-                    }
+                    for (int z = 0; z < TERMS; z++) mma<BF>(o[t], A, pf[z][0], pf[z][1]);
+                }
             }
         }
         // ---------------- the portion's end: the next one's first copies, then the warps' results joined
-        const Part D = P;
+        const int ng = P.ng;
+        const long long h0 = P.h0;
         const bool first = wk.t0 == 0, whole = first && wk.t1 == wk.nt;
         if (wk.t1 == wk.nt && tid == 0) a.cnt[static_cast<long long>(wk.b) * segs + wk.seg] = cut_of(wk, T, G);
         have = wk.next(a, segs);
-        __syncwarp();
+        team_sync();
         if (have) start();
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                float v = l[nt][e];
-                v += __shfl_xor_sync(0xffffffffu, v, 4);
-                v += __shfl_xor_sync(0xffffffffu, v, 8);
-                v += __shfl_xor_sync(0xffffffffu, v, 16);
-                if (lr == 0) {
-                    s_m[warp][8 * nt + 2 * lc + e] = m[nt][e];
-                    s_l[warp][8 * nt + 2 * lc + e] = v;
-                }
+        for (int e = 0; e < 2; e++) {
+            float v = l[e];
+            v += __shfl_xor_sync(0xffffffffu, v, 4);
+            v += __shfl_xor_sync(0xffffffffu, v, 8);
+            v += __shfl_xor_sync(0xffffffffu, v, 16);
+            if (lr == 0) {
+                s_m[warp][2 * lc + e] = m[e];
+                s_l[warp][2 * lc + e] = v;
             }
+        }
         float *part = part_at(a, blockIdx.x, first);
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) {   // eight heads at a time
+        for (int n = 0; n < 2; n++) {          // four heads of every warp at a time
+            if (lc >> 1 == n)
 #pragma unroll
-            for (int t = 0; t < 8; t++)
+                for (int t = 0; t < KS; t++)
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    so[(warp * 8 + 2 * lc + (i & 1)) * kPad + 16 * t + lr + 8 * (i >> 1)] = BF ? o[t][nt][i] : o[t][nt][i] * 0x1p-7f;
+                    for (int i = 0; i < 4; i++)
+                        so[(warp * 4 + 2 * (lc & 1) + (i & 1)) * kPad + 16 * t + lr + 8 * (i >> 1)] =
+                            BF ? o[t][i] : o[t][i] * 0x1p-7f;
             __syncthreads();
-            if (nt == 0) {
+            if (n == 0) {
                 if (tid < NH) {
                     float M = kNone, L = 0.f;
-                    for (int w = 0; w < kWarps; w++) M = fmaxf(M, s_m[w][tid]);
-                    for (int w = 0; w < kWarps; w++) {
-                        const float f = ex2(s_m[w][tid] - M);
-                        L += s_l[w][tid] * f;
-                        s_m[w][tid] = f;
+                    for (int w = 0; w < TEAMS; w++) M = fmaxf(M, s_m[w * TEAM + tid / 8][tid & 7]);
+                    for (int w = 0; w < TEAMS; w++) {
+                        float &mw = s_m[w * TEAM + tid / 8][tid & 7];
+                        mw = ex2(mw - M);
+                        L += s_l[w * TEAM + tid / 8][tid & 7] * mw;
                     }
                     s_M[tid] = M;
                     s_L[tid] = L;
                 }
                 __syncthreads();
             }
-            for (int i = tid; i < 8 * hd; i += kThreads) {
-                const int g = i / hd, c = i - g * hd, h = 8 * nt + g;
-                if (h >= D.ng) break;
+            for (int i = tid; i < 4 * TEAM * hd; i += kThreads) {
+                const int g = i / hd, c = i - g * hd, e = g / 4, h4 = g & 3, h = 8 * e + 4 * n + h4;
+                if (h >= ng) continue;
                 float v = 0.f;
 #pragma unroll
-                for (int w = 0; w < kWarps; w++) v += so[(w * 8 + g) * kPad + c] * s_m[w][h];
-                if (whole) a.out[(D.h0 + h) * hd + c] = s_L[h] > 0.f ? v / s_L[h] : 0.f;
+                for (int w = 0; w < TEAMS; w++) v += so[((w * TEAM + e) * 4 + h4) * kPad + c] * s_m[w * TEAM + e][4 * n + h4];
+                if (whole) a.out[(h0 + h) * hd + c] = s_L[h] > 0.f ? v / s_L[h] : 0.f;
                 else part[h * 128 + c] = v;
             }
-            if (nt + 1 < NT) __syncthreads();
+            if (n == 0) __syncthreads();
         }
-        if (tid < D.ng) {
+        if (tid < ng) {
             const float M = s_M[tid], L = s_L[tid];
             if (!whole) {
                 part[kAttendPart - 32 + tid] = M;
                 part[kAttendPart - 16 + tid] = L;
             } else {
-                if (a.lse) a.lse[D.h0 + tid] = L > 0.f ? M * 0.6931471805599453f + logf(L) : -INFINITY;
+                if (a.lse) a.lse[h0 + tid] = L > 0.f ? M * 0.6931471805599453f + logf(L) : -INFINITY;
                 if (a.acc_out) {
-                    a.ml[2 * (D.h0 + tid)] = M;
-                    a.ml[2 * (D.h0 + tid) + 1] = L;
+                    a.ml[2 * (h0 + tid)] = M;
+                    a.ml[2 * (h0 + tid) + 1] = L;
                 }
             }
         }
-        __syncthreads();                        // the join's buffers are free again
+        __syncthreads();                       // the join's buffers are free again
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-template <bool BF, int NT>
+template <bool BF, int TEAM, int KS>
 cudaError_t launch(const PagedAttendArgs &a, cudaStream_t st) {
     constexpr int smem = kRing + kJoin;
-    const cudaError_t e = allow_smem<k_attend_mma<BF, NT>>(smem);
+    const cudaError_t e = allow_smem<k_attend_mma<BF, TEAM, KS>>(smem);
     if (e != cudaSuccess) return e;
-    const cudaError_t e2 = launch_pdl(k_attend_mma<BF, NT>, dim3(a.ctas), dim3(kThreads), smem, st, a);
-    return e2 != cudaSuccess ? e2 : launch_attend_finish(a, 8 * NT, 128, st);
+    const cudaError_t e2 = launch_pdl(k_attend_mma<BF, TEAM, KS>, dim3(a.ctas), dim3(kThreads), smem, st, a);
+    return e2 != cudaSuccess ? e2 : launch_attend_finish(a, 8 * TEAM, 128, st);
+}
+template <bool BF>
+cudaError_t launch_t(const PagedAttendArgs &a, int team, cudaStream_t st) {
+    if (a.kv.hd <= 64) return team == 1 ? launch<BF, 1, 4>(a, st) : launch<BF, 2, 4>(a, st);
+    return team == 1 ? launch<BF, 1, 8>(a, st) : launch<BF, 2, 8>(a, st);
 }
 
 }  // namespace
 
 cudaError_t launch_attend_mma(PagedAttendArgs a, int sms, cudaStream_t st) {
-    const int nt = a.gqa <= 8 ? 1 : 2;
-    a.ctas = attend_grid(a, 8 * nt, sms);
-    if (a.kv.dtype == STYX_BF16) return nt == 1 ? launch<true, 1>(a, st) : launch<true, 2>(a, st);
-    return nt == 1 ? launch<false, 1>(a, st) : launch<false, 2>(a, st);
+    const int team = a.gqa <= 8 ? 1 : 2;
+    a.ctas = attend_grid(a, 8 * team, sms);
+    return a.kv.dtype == STYX_BF16 ? launch_t<true>(a, team, st) : launch_t<false>(a, team, st);
 }
 
 }  // namespace styx
