@@ -37,6 +37,7 @@ constexpr int kUnits = 48;                     // of all rings
 constexpr int kRing = kUnits * kUnit;
 constexpr int kPad = 132;                      // floats of a head's O in the join: no two heads on one bank
 constexpr int kJoin = kWarps * 4 * kPad * 4;   // four heads of every warp
+constexpr int kQ = 8 * kPad * 4;               // q of eight heads
 constexpr float kSlack = 8.f;                  // log2 units a score may pass the maximum by
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool on) {   // off: zeros
@@ -152,13 +153,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_mma(PagedAttendArgs a) {
     int slot = 0;                     // of the next unit to be used
     unsigned seen = 0;                // bit s: slot s holds a tile of which rows are seen
     int kpage = -1, vpage = -1;       // the page of the next K, V to be copied; -1: none
+    float *sq = reinterpret_cast<float *>(smem + kRing + kJoin);   // the portion's q; two buffers in turn
     auto page_of = [&](int it) {
         const int r = P.base + (it * TEAMS + team) * kRows;
         return it < P.iters && r < P.hi ? ld_now(P.table + (r >> kv.page_shift)) : -1;
     };
-    // copies of K or V of tile `it` into slot s; rows outside [lo, hi) are zeros, a page outside the pool is reported
-    auto issue = [&](bool is_v, int it, int s) {
-        const int page = is_v ? vpage : kpage, r0 = P.base + (it * TEAMS + team) * kRows;
+    // copies of K or V of tile `it` in a page into slot s; rows outside [lo, hi) are zeros, a page outside the pool is reported
+    auto issue = [&](bool is_v, int it, int s, int page) {
+        const int r0 = P.base + (it * TEAMS + team) * kRows;
         const bool some = it < P.iters && r0 < P.hi, ok = some && static_cast<unsigned>(page) < static_cast<unsigned>(kv.n_pages);
         if (some && !ok && lane == 0) atomicExch(kv.err, kErrBadPos);
         if (ok) {
@@ -172,18 +174,25 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_mma(PagedAttendArgs a) {
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
         seen = ok ? seen | (1u << s) : seen & ~(1u << s);
-        if (!is_v) {
-            vpage = kpage;
-            kpage = page_of(it + 1);
-        }
     };
-    auto start = [&] {                // a portion's first copies
+    auto start = [&] {                // a portion's first copies: q, then S - 1 units
         P.set(a, wk, groups, NH);
-        kpage = page_of(0);
+        sq = reinterpret_cast<float *>(smem + kRing + kJoin + (reinterpret_cast<uint8_t *>(sq) == smem + kRing + kJoin ? TEAM * kQ : 0));
+        int pages[S / 2];
+#pragma unroll
+        for (int i = 0; i < S / 2; i++) pages[i] = page_of(i);
+        kpage = page_of(S / 2);
+        vpage = pages[S / 2 - 1];
+        const int per = hd / 4;
+        for (int i = tid; i < P.ng * per; i += kThreads) {
+            const int h = i / per, c = i - h * per;
+            copy16(smem_addr(sq + h * kPad + 4 * c), a.q + (P.h0 + h) * hd + 4 * c, true);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
         int s = slot;
 #pragma unroll
         for (int u = 0; u < S - 1; u++) {
-            issue(u & 1, u / 2, s);
+            issue(u & 1, u / 2, s, pages[u / 2]);
             s = s + 1 == S ? 0 : s + 1;
         }
     };
@@ -194,20 +203,30 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_mma(PagedAttendArgs a) {
         team_sync();
         const int now = slot;
         slot = slot + 1 == S ? 0 : slot + 1;
-        issue((is_v + S - 1) & 1, it + (is_v + S - 1) / 2, now == 0 ? S - 1 : now - 1);
+        static_assert(S % 2 == 0, "V follows K");
+        const int s = now == 0 ? S - 1 : now - 1;
+        if (is_v) {
+            issue(false, it + S / 2, s, kpage);
+            vpage = kpage;
+            kpage = page_of(it + S / 2 + 1);
+        } else {
+            issue(true, it + S / 2 - 1, s, vpage);
+        }
         return now;
     };
 
     bool have = wk.next(a, segs);
     if (have) start();
     while (have) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(S - 1) : "memory");
+        __syncthreads();              // q is there; the last join's buffers are free again
         // ---------------- q as B fragments, in terms.  f16 has few exponents: a head's largest |q| is brought to
         // [2^9, 2^10), and fh says what its column of S is in units of its terms
         uint32_t qf[KS][TERMS][2];
         float fh[2];
         {
             const int h = 8 * in + lr;
-            const float *q = a.q + (P.h0 + h) * hd + 2 * lc;
+            const float *q = sq + h * kPad + 2 * lc;
             float2 v[KS][2];
             float mx = 0.f;
 #pragma unroll
@@ -404,14 +423,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_mma(PagedAttendArgs a) {
                 }
             }
         }
-        __syncthreads();                       // the join's buffers are free again
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 template <bool BF, int TEAM, int KS>
 cudaError_t launch(const PagedAttendArgs &a, cudaStream_t st) {
-    constexpr int smem = kRing + kJoin;
+    constexpr int smem = kRing + kJoin + TEAM * 2 * kQ;
     const cudaError_t e = allow_smem<k_attend_mma<BF, TEAM, KS>>(smem);
     if (e != cudaSuccess) return e;
     const cudaError_t e2 = launch_pdl(k_attend_mma<BF, TEAM, KS>, dim3(a.ctas), dim3(kThreads), smem, st, a);

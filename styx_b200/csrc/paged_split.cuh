@@ -64,6 +64,12 @@ struct Walk {
 };
 
 
+// x y / d, all below 2^31: a 32-bit division (a 64-bit one is some 300 clocks) where the product allows it
+__device__ __forceinline__ long long mul_div(long long x, long long y, long long d) {
+    const unsigned long long p = static_cast<unsigned long long>(x) * y;
+    return p >> 32 ? static_cast<long long>(p / d) : static_cast<long long>(static_cast<unsigned>(p) / static_cast<unsigned>(d));
+}
+
 // A CTA's share: units before each chunk of sequences, their total T, the
 // first of CTA i's units (floor(i T / G)) as (sequence, head, unit).
 template <int THREADS>
@@ -100,7 +106,7 @@ __device__ __forceinline__ void share_of(const PagedAttendArgs &a, int segs, Sha
     __syncthreads();
     T = sh.scan[THREADS - 1];
     G = min(static_cast<long long>(gridDim.x), T);
-    const long long i = blockIdx.x, at = i < G ? i * T / G : 0, end = i < G ? (i + 1) * T / G : 0;
+    const long long i = blockIdx.x, at = i < G ? mul_div(i, T, G) : 0, end = i < G ? mul_div(i + 1, T, G) : 0;
     const long long before = sh.scan[tid] - mine;
     if (mine > 0 && at >= before && at < before + mine) {
         long long off = at - before;
@@ -116,7 +122,7 @@ __device__ __forceinline__ void share_of(const PagedAttendArgs &a, int segs, Sha
     __syncthreads();
     w.b = sh.b0;
     w.nt = Seq(a, w.b, false).nt;
-    w.seg = static_cast<int>(sh.off / (w.nt + kSegCost));
+    w.seg = static_cast<int>(mul_div(1, sh.off, w.nt + kSegCost));
     w.u = static_cast<int>(sh.off - static_cast<long long>(w.seg) * (w.nt + kSegCost));
     w.at = at;
     w.end = end;
