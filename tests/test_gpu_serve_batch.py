@@ -1,0 +1,103 @@
+"""styx_b200.serve (append, attend, evict and sample as one batched decode
+step) against the oracle and the single-sequence decode step over the same
+weights."""
+import numpy as np
+import pytest
+import torch
+
+from styx_b200 import serve
+from tests.decode_case import make_model, oracle_greedy, write_gguf
+from tests.test_gpu_decode import gpu_model
+
+pytestmark = pytest.mark.gpu
+
+PROMPTS = [[5, 17, 99], [640], [3, 1, 4, 1, 5, 9, 2], [1000, 2, 77]]
+
+
+def decoder(m, **kw):
+    return serve.BatchDecoder.of(gpu_model(m, 8), len(PROMPTS), kw.pop("n_ctx", 64), **kw)
+
+
+@pytest.mark.parametrize("hd,page", [(64, 16), (128, 4)])
+def test_greedy_tokens_are_those_of_the_oracle(hd, page):
+    m = make_model(0, hd=hd)
+    expect = [oracle_greedy(m, p, 12) for p in PROMPTS]
+    # f32 rows and f32 experts: the same arithmetic up to the order of sums
+    d = decoder(m, page=page, cache=torch.float32, moe_batch=False)
+    assert d.generate(PROMPTS, 12) == expect
+    assert d.generate(PROMPTS, 12) == expect                     # from the start again
+    # a budget that nothing reaches changes nothing
+    d = decoder(m, page=page, cache=torch.float32, moe_batch=False, budget=32, n_recent=8, n_sink=2)
+    assert d.generate(PROMPTS, 12) == expect
+
+
+@pytest.mark.parametrize("cache", ["f16", "bf16"])
+def test_logits_of_16_bit_rows_and_batched_experts(cache):
+    """K and V rounded to 2^-11 (bf16: 2^-8) of themselves and the experts'
+    operands to f16 (1e-3 of a block's largest update): two layers, each update
+    no larger than the residual stream, stay within 4 (2^-11 + 1e-3) and
+    4 (2^-8 + 1e-3) of the largest logit."""
+    m = make_model(1)
+    one = gpu_model(m, 64)
+    d = decoder(m, cache=serve.CACHE_TYPES[cache])
+    assert d.moe_batch
+    tol = 4 * ((2.0 ** -11 if cache == "f16" else 2.0 ** -8) + 1e-3)
+    rng = np.random.default_rng(2)
+    toks = rng.integers(0, m.hp["n_vocab"], (9, len(PROMPTS)))
+    got = []
+    for t in toks:
+        d.tok.copy_(torch.from_numpy(t.astype(np.int32)))
+        got.append(d.step().cpu().numpy().copy())
+    for b in range(len(PROMPTS)):
+        one.reset()
+        for i, t in enumerate(toks):
+            ref = one.forward_token(int(t[b])).cpu().numpy()
+            assert np.abs(got[i][b] - ref).max() <= tol * np.abs(ref).max()
+
+
+def test_a_budget_bounds_rows_and_pages():
+    m = make_model(2)
+    budget, recent, sinks, page = 24, 8, 2, 8
+    d = decoder(m, page=page, cache=torch.float16, budget=budget, n_recent=recent, n_sink=sinks, n_pages=4 * 4)
+    out = d.generate(PROMPTS, 60, temperature=0.8, top_k=50, top_p=0.95, min_p=0.01, seed=3)
+    assert all(len(o) == 60 and all(0 <= t < m.hp["n_vocab"] for t in o) for o in out)
+    lens = d.lens.tolist()
+    assert lens == d.rows and all(budget <= n < budget + page for n in lens)
+    used = [p for ps in d.pages for p in ps]
+    assert sorted(used + d.free) == list(range(16)) and [len(ps) for ps in d.pages] == [-(-n // page) for n in lens]
+    assert [d.table[b, :len(ps)].tolist() for b, ps in enumerate(d.pages)] == d.pages
+    for b, p in enumerate(sorted(PROMPTS, key=lambda p: -len(p))):
+        nxt = len(p) + 59
+        assert d.pos[b].item() == nxt
+        for li in range(m.hp["n_layers"]):
+            rows = d.row_pos[li][b, :, :lens[b]].cpu().numpy()
+            for r in rows:      # no position twice; the first ones and the last ones are there
+                assert len(set(r.tolist())) == len(r)
+                assert set(range(sinks)) | set(range(nxt - recent, nxt)) <= set(r.tolist())
+    # the same settings and seed draw the same tokens; another seed others
+    assert d.generate(PROMPTS, 60, temperature=0.8, top_k=50, top_p=0.95, min_p=0.01, seed=3) == out
+    assert d.generate(PROMPTS, 60, temperature=0.8, top_k=50, top_p=0.95, min_p=0.01, seed=4) != out
+
+
+def test_full_caches_and_pools_are_refused():
+    m = make_model(0, n_layers=1)
+    d = decoder(m, n_ctx=8, page=4)
+    with pytest.raises(ValueError, match="cache full"):
+        d.generate(PROMPTS, 4)
+    d = decoder(m, page=4, n_pages=5)
+    with pytest.raises(ValueError, match="no page left"):
+        d.generate(PROMPTS, 20)
+    with pytest.raises(ValueError, match="prompts"):
+        d.generate(PROMPTS[:2], 4)
+
+
+def test_command_line(tmp_path, capsys):
+    m = make_model(0)
+    path = str(tmp_path / "m.gguf")
+    write_gguf(m, path)
+    argv = [path, "-n", "10", "--ctx", "64", "--cache", "f32"]
+    for p in PROMPTS[:2]:
+        argv += ["--prompt", ",".join(map(str, p))]
+    assert serve.main(argv) == 0
+    out = capsys.readouterr().out.split()
+    assert len(out) == 2 and all(len(o.split(",")) == 10 for o in out)

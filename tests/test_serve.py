@@ -80,3 +80,15 @@ def test_rope_definition():
     x = np.array([[[1.0, 0, 0, 0]]])
     y = rope_norm_ref(x, None, np.array([2]), 100.0, 0)
     assert np.allclose(y, [[[np.cos(2), 0, np.sin(2), 0]]])
+
+
+def test_batch_decoder_refuses_what_it_cannot_hold():
+    from styx_b200.decode import DecodeParams
+    from styx_b200.serve import BatchDecoder
+    hp = DecodeParams(1, 512, 8, 2, 64, 256, 16, 4, 1024)
+    with pytest.raises(ValueError, match="sequences"):
+        BatchDecoder(hp, None, [], None, None, 0, 64)
+    with pytest.raises(ValueError, match="sequences"):
+        BatchDecoder(hp, None, [], None, None, 65, 64)
+    with pytest.raises(ValueError, match="budget"):
+        BatchDecoder(hp, None, [], None, None, 4, 64, budget=16, n_recent=14, n_sink=4)
