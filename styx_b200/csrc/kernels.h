@@ -379,7 +379,7 @@ struct PagedAppendArgs {
     long long q_stride, k_stride, v_stride;   // floats between tokens
     const float *q_norm, *k_norm;             // [hd] or null
     float eps;
-    double log2_base;                         // log2(freq_base^(-2/hd))
+    double log2_base, step;                   // log2(freq_base^(-2/hd)); freq_base^(-2/hd)
     const int32_t *pos, *seq, *row;           // seq, row may be null
     float *q_out;
     int n_tokens, n_heads;

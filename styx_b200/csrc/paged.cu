@@ -7,6 +7,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "cluster.cuh"
 #include "paged.cuh"
@@ -14,135 +15,151 @@
 namespace styx {
 namespace {
 
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-}
-
 // ------------------------------------------------------------ append
-// A CTA takes tokens in turn (blockIdx.y: a share of their rows when tokens
-// are few).  The token's cosines and sines are computed once, by the first
-// threads, into shared memory: the angle in turns, pos * base^(-2i/d) / 2 pi,
-// is held in 64 bits and reduced to a fraction of a turn before it is rounded
-// to f32, so its error does not grow with the position.  Then a warp takes
-// four of the token's rows (q heads, k heads, v heads) at a time, all loads
-// first; lane l holds the pairs (i, i + d/2) of i = 2 l, 2 l + 1 (+ 64).
-constexpr int kAppThreads = 256, kAppRows = 4;
+// A warp takes a token's rows (q heads, k heads, v heads), or a share of them:
+// LPR lanes per row, lane l of them the pairs (i, i + d/2) of i = 4 l ... + 3,
+// kAppRows x 32 / LPR rows at a time, all loads first.  The token's place and
+// its cosines and sines, in the lane's registers for all its rows, are found
+// while the first loads are on their way; nothing is shared between warps.
+// The angle in turns, pos * base^(-2i/d) / 2 pi, is held in 64 bits and
+// reduced to a fraction of a turn before it is rounded to f32, so its error
+// does not grow with the position.
+constexpr int kAppThreads = 128, kAppRows = 4;
 
 template <class T>
-__device__ __forceinline__ void store2(T *p, float a, float b) {
-    if constexpr (sizeof(T) == 4) {
-        *reinterpret_cast<float2 *>(p) = make_float2(a, b);
-    } else {
-        T v[2] = {from_f<T>(a), from_f<T>(b)};
-        *reinterpret_cast<uint32_t *>(p) = *reinterpret_cast<uint32_t *>(v);
-    }
+__device__ __forceinline__ void store4(T *p, const float (&v)[4]) {
+    T u[4] = {from_f<T>(v[0]), from_f<T>(v[1]), from_f<T>(v[2]), from_f<T>(v[3])};
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<float4 *>(p) = *reinterpret_cast<const float4 *>(u);
+    else *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<const uint2 *>(u);
 }
 
-// K: rounds of 64 pairs, d <= 128 K (d/2 is even: rows are of 16 bytes'
-// multiples).  vec: every row of the inputs is 8-byte aligned, else loads are
-// by element.
-template <class T, int K>
-__global__ void __launch_bounds__(kAppThreads) k_paged_append(PagedAppendArgs a, bool vec) {
+// VEC: d is a multiple of 8 and every row of the inputs is 16-byte aligned;
+// else loads and stores are by element.  splits: warps per token, share rows
+// each.
+template <class T, int LPR, bool VEC>
+__global__ void __launch_bounds__(kAppThreads) k_paged_append(PagedAppendArgs a, int splits, int share) {
     pdl_trigger();
-    __shared__ float s_cs[2][2][128];
+    constexpr int RPW = 32 / LPR;
     const PagedKv &kv = a.kv;
-    const int hd = kv.hd, half = hd >> 1, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int rows = a.n_heads + 2 * kv.n_kv;
-    const double turn = tid < half ? exp2(a.log2_base * tid) * 0.15915494309189535 : 0.0;   // 1 / 2 pi
+    const int hd = kv.hd, half = hd >> 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int i0 = lane % LPR * 4, sub = lane / LPR, rows = a.n_heads + 2 * kv.n_kv;
+    double turn[4];
+    turn[0] = exp2(a.log2_base * i0) * 0.15915494309189535;   // 1 / 2 pi
+#pragma unroll
+    for (int e = 1; e < 4; e++) turn[e] = turn[e - 1] * a.step;
+    bool in[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) in[e] = VEC ? i0 < half : i0 + e < half;
     pdl_wait();
-    int buf = 0;
-    for (int t = blockIdx.x; t < a.n_tokens; t += gridDim.x, buf ^= 1) {
+    float wq[2][4], wk[2][4];
+#pragma unroll
+    for (int y = 0; y < 2; y++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            wq[y][e] = a.q_norm && in[e] ? ld_now(a.q_norm + y * half + i0 + e) : 1.f;
+            wk[y][e] = a.k_norm && in[e] ? ld_now(a.k_norm + y * half + i0 + e) : 1.f;
+        }
+    const unsigned units = static_cast<unsigned>(a.n_tokens) * splits;
+    for (unsigned u = blockIdx.x * (kAppThreads / 32) + warp; u < units; u += gridDim.x * (kAppThreads / 32)) {
+        const int t = u / splits, h_begin = (u - t * splits) * share, h_end = min(rows, h_begin + share);
+        float x[kAppRows][4], y[kAppRows][4];
+        auto load = [&](int h0) {
+#pragma unroll
+            for (int j = 0; j < kAppRows; j++) {
+                const int h = h0 + j * RPW + sub;
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[j][e] = y[j][e] = 0.f;
+                if (h < h_end && in[0]) {
+                    const int hk = h - a.n_heads;
+                    const float *src = hk < 0         ? a.q + t * a.q_stride + static_cast<long long>(h) * hd
+                                       : hk < kv.n_kv ? a.k + t * a.k_stride + static_cast<long long>(hk) * hd
+                                                      : a.v + t * a.v_stride + static_cast<long long>(hk - kv.n_kv) * hd;
+                    if constexpr (VEC) {
+                        *reinterpret_cast<float4 *>(x[j]) = *reinterpret_cast<const float4 *>(src + i0);
+                        *reinterpret_cast<float4 *>(y[j]) = *reinterpret_cast<const float4 *>(src + half + i0);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (in[e]) {
+                                x[j][e] = src[i0 + e];
+                                y[j][e] = src[half + i0 + e];
+                            }
+                    }
+                }
+            }
+        };
+        load(h_begin);
         const int b = a.seq ? ld_now(a.seq + t) : t, pos = ld_now(a.pos + t);
         const bool seq_ok = static_cast<unsigned>(b) < static_cast<unsigned>(kv.n_seqs);
         const int r = !seq_ok ? -1 : a.row ? ld_now(a.row + t) : ld_now(kv.lens + b) - 1;
         bool row_ok = r >= 0 && r < (static_cast<long long>(kv.max_pages) << kv.page_shift);
         const long long off = row_ok ? paged_off(kv, b, 0, r) : -1;   // of kv head 0
         row_ok = off >= 0;
-        if (tid == 0 && blockIdx.y == 0 && (!seq_ok || (r >= 0 && !row_ok))) atomicExch(kv.err, kErrBadPos);
-        if (tid < half) {
-            const double x = pos * turn, f = x - rint(x);
-            float s, c;
-            sincospif(static_cast<float>(2.0 * f), &s, &c);
-            s_cs[buf][0][tid] = c;
-            s_cs[buf][1][tid] = s;
+        if (lane == 0 && h_begin == 0 && (!seq_ok || (r >= 0 && !row_ok))) atomicExch(kv.err, kErrBadPos);
+        float c[4], s[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const double f = pos * turn[e];
+            sincospif(static_cast<float>(2.0 * (f - rint(f))), &s[e], &c[e]);
         }
-        __syncthreads();   // (the other buffer is free again: every warp has passed here once more since it read it)
-        for (int h0 = (blockIdx.y * (kAppThreads / 32) + warp) * kAppRows; h0 < rows;
-             h0 += gridDim.y * (kAppThreads / 32) * kAppRows) {
-            float2 x[kAppRows][K], y[kAppRows][K];
+        for (int h0 = h_begin;;) {
 #pragma unroll
             for (int j = 0; j < kAppRows; j++) {
-                const int h = h0 + j;
-                if (h >= rows) break;
-                const float *src = h < a.n_heads             ? a.q + t * a.q_stride + static_cast<long long>(h) * hd
-                                   : h < a.n_heads + kv.n_kv ? a.k + t * a.k_stride + static_cast<long long>(h - a.n_heads) * hd
-                                                             : a.v + t * a.v_stride + static_cast<long long>(h - a.n_heads - kv.n_kv) * hd;
-#pragma unroll
-                for (int k = 0; k < K; k++) {
-                    const int i = 2 * lane + 64 * k;
-                    x[j][k] = y[j][k] = make_float2(0.f, 0.f);
-                    if (i < half) {
-                        if (vec) {
-                            x[j][k] = *reinterpret_cast<const float2 *>(src + i);
-                            y[j][k] = *reinterpret_cast<const float2 *>(src + half + i);
-                        } else {
-                            x[j][k] = make_float2(src[i], src[i + 1]);
-                            y[j][k] = make_float2(src[half + i], src[half + i + 1]);
-                        }
-                    }
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < kAppRows; j++) {
-                const int h = h0 + j;
-                if (h >= rows) break;
-                const bool is_q = h < a.n_heads, is_v = h >= a.n_heads + kv.n_kv;
-                const float *w = is_q ? a.q_norm : a.k_norm;
-                if (w && !is_v) {
+                const int h = h0 + j * RPW + sub, hk = h - a.n_heads;
+                const bool is_q = hk < 0, is_v = hk >= kv.n_kv;
+                if (a.q_norm || a.k_norm) {            // (for all lanes: their rows may be of two kinds)
                     float ss = 0.f;
 #pragma unroll
-                    for (int k = 0; k < K; k++)
-                        ss += x[j][k].x * x[j][k].x + x[j][k].y * x[j][k].y + y[j][k].x * y[j][k].x + y[j][k].y * y[j][k].y;
-                    const float scale = 1.0f / sqrtf(warp_sum(ss) / static_cast<float>(hd) + a.eps);
+                    for (int e = 0; e < 4; e++) ss += x[j][e] * x[j][e] + y[j][e] * y[j][e];
 #pragma unroll
-                    for (int k = 0; k < K; k++) {
-                        const int i = 2 * lane + 64 * k;
-                        if (i < half) {
-                            x[j][k].x *= scale * ld_now(w + i);
-                            x[j][k].y *= scale * ld_now(w + i + 1);
-                            y[j][k].x *= scale * ld_now(w + half + i);
-                            y[j][k].y *= scale * ld_now(w + half + i + 1);
-                        }
+                    for (int o = LPR / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o, LPR);
+                    const bool normed = is_q ? a.q_norm != nullptr : !is_v && a.k_norm;
+                    const float scale = !normed ? 1.f : 1.0f / sqrtf(ss / static_cast<float>(hd) + a.eps);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        x[j][e] *= scale * (is_v ? 1.f : is_q ? wq[0][e] : wk[0][e]);
+                        y[j][e] *= scale * (is_v ? 1.f : is_q ? wq[1][e] : wk[1][e]);
                     }
                 }
+                float p[4], q[4];
 #pragma unroll
-                for (int k = 0; k < K; k++) {
-                    const int i = 2 * lane + 64 * k;
-                    if (i >= half) continue;
-                    float2 u = x[j][k], v = y[j][k];
-                    if (!is_v) {
-                        const float2 c = *reinterpret_cast<const float2 *>(&s_cs[buf][0][i]);
-                        const float2 s = *reinterpret_cast<const float2 *>(&s_cs[buf][1][i]);
-                        u = make_float2(x[j][k].x * c.x - y[j][k].x * s.x, x[j][k].y * c.y - y[j][k].y * s.y);
-                        v = make_float2(x[j][k].x * s.x + y[j][k].x * c.x, x[j][k].y * s.y + y[j][k].y * c.y);
-                    }
-                    if (is_q) {
-                        if (r < 0) u = v = make_float2(0.f, 0.f);   // padding, or an empty slot
-                        float *o = a.q_out + (static_cast<long long>(t) * a.n_heads + h) * hd;
-                        store2(o + i, u.x, u.y);
-                        store2(o + half + i, v.x, v.y);
-                    } else if (row_ok) {
-                        const int head = h - a.n_heads - (is_v ? kv.n_kv : 0);
-                        T *o = static_cast<T *>(is_v ? kv.v : kv.k) + off + (static_cast<long long>(head) << kv.page_shift) * hd;
-                        store2(o + i, u.x, u.y);
-                        store2(o + half + i, v.x, v.y);
-                    }
+                for (int e = 0; e < 4; e++) {
+                    p[e] = is_v ? x[j][e] : x[j][e] * c[e] - y[j][e] * s[e];
+                    q[e] = is_v ? y[j][e] : x[j][e] * s[e] + y[j][e] * c[e];
+                    if (r < 0) p[e] = q[e] = 0.f;          // padding, or an empty slot
                 }
+                if (h >= h_end || !in[0]) continue;
+                auto put = [&](auto *o) {
+                    if constexpr (VEC) {
+                        store4(o + i0, p);
+                        store4(o + half + i0, q);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (in[e]) {
+                                o[i0 + e] = from_f<std::remove_pointer_t<decltype(o)>>(p[e]);
+                                o[half + i0 + e] = from_f<std::remove_pointer_t<decltype(o)>>(q[e]);
+                            }
+                    }
+                };
+                if (is_q) put(a.q_out + (static_cast<long long>(t) * a.n_heads + h) * hd);
+                else if (row_ok)
+                    put(static_cast<T *>(is_v ? kv.v : kv.k) + off +
+                        (static_cast<long long>(is_v ? hk - kv.n_kv : hk) << kv.page_shift) * hd);
             }
+            h0 += kAppRows * RPW;
+            if (h0 >= h_end) break;
+            load(h0);
         }
     }
+}
+
+template <class T>
+cudaError_t append_t(const PagedAppendArgs &a, bool vec, int lpr, dim3 grid, int splits, int share, cudaStream_t st) {
+    auto go = [&](auto *kern) { return launch_pdl(kern, grid, dim3(kAppThreads), 0, st, a, splits, share); };
+    if (lpr == 8) return vec ? go(k_paged_append<T, 8, true>) : go(k_paged_append<T, 8, false>);
+    if (lpr == 16) return vec ? go(k_paged_append<T, 16, true>) : go(k_paged_append<T, 16, false>);
+    return vec ? go(k_paged_append<T, 32, true>) : go(k_paged_append<T, 32, false>);
 }
 
 // ------------------------------------------------------------ eviction
@@ -445,20 +462,20 @@ __global__ void __launch_bounds__(256) k_evict_move(PagedEvictArgs a, int blocks
 }  // namespace
 
 cudaError_t launch_paged_append(const PagedAppendArgs &a, int sms, cudaStream_t st) {
-    const int rows = a.n_heads + 2 * a.kv.n_kv, per = kAppThreads / 32 * kAppRows;
-    // few tokens: their rows over several CTAs; many: eight CTAs per SM take them in turn
-    const int parts = std::max(1, std::min((rows + per - 1) / per, 2 * sms / a.n_tokens));
-    const dim3 grid(static_cast<unsigned>(std::min(a.n_tokens, 8 * sms)), static_cast<unsigned>(parts));
-    auto al8 = [](const void *p, long long s) { return (reinterpret_cast<uintptr_t>(p) & 7) == 0 && s % 2 == 0; };
-    const bool vec = al8(a.q, a.q_stride) && al8(a.k, a.k_stride) && al8(a.v, a.v_stride);
-    const bool two = a.kv.hd > 128;
-    const dim3 block(kAppThreads);
-    if (a.kv.dtype == STYX_F16)
-        return two ? launch_pdl(k_paged_append<__half, 2>, grid, block, 0, st, a, vec) : launch_pdl(k_paged_append<__half, 1>, grid, block, 0, st, a, vec);
-    if (a.kv.dtype == STYX_BF16)
-        return two ? launch_pdl(k_paged_append<__nv_bfloat16, 2>, grid, block, 0, st, a, vec)
-                   : launch_pdl(k_paged_append<__nv_bfloat16, 1>, grid, block, 0, st, a, vec);
-    return two ? launch_pdl(k_paged_append<float, 2>, grid, block, 0, st, a, vec) : launch_pdl(k_paged_append<float, 1>, grid, block, 0, st, a, vec);
+    const int rows = a.n_heads + 2 * a.kv.n_kv, hd = a.kv.hd, lpr = hd <= 64 ? 8 : hd <= 128 ? 16 : 32;
+    const int batch = kAppRows * (32 / lpr), batches = (rows + batch - 1) / batch;
+    // warps per token: one for each batch of rows while that makes no more than eight waves of 24 warps per SM
+    const long long want = (8ll * 24 * sms + a.n_tokens - 1) / a.n_tokens;
+    const int share = (batches + static_cast<int>(std::min<long long>(batches, want)) - 1) /
+                      static_cast<int>(std::min<long long>(batches, want)) * batch;
+    const int splits = (rows + share - 1) / share;
+    const long long ctas = (static_cast<long long>(a.n_tokens) * splits + kAppThreads / 32 - 1) / (kAppThreads / 32);
+    const dim3 grid(static_cast<unsigned>(std::min<long long>(ctas, 32ll * sms)));
+    auto al16 = [](const void *p, long long s) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && s % 4 == 0; };
+    const bool vec = hd % 8 == 0 && al16(a.q, a.q_stride) && al16(a.k, a.k_stride) && al16(a.v, a.v_stride);
+    return a.kv.dtype == STYX_F16    ? append_t<__half>(a, vec, lpr, grid, splits, share, st)
+           : a.kv.dtype == STYX_BF16 ? append_t<__nv_bfloat16>(a, vec, lpr, grid, splits, share, st)
+                                     : append_t<float>(a, vec, lpr, grid, splits, share, st);
 }
 
 // CTAs of a line: 4096 rows each, eight at most

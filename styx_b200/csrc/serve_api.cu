@@ -169,6 +169,7 @@ int styx_paged_append(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv
     a.k_norm = k_norm;
     a.eps = eps;
     a.log2_base = -2.0 / static_cast<double>(kv->head_dim) * std::log2(static_cast<double>(freq_base));
+    a.step = std::exp2(a.log2_base);
     a.pos = pos;
     a.seq = seq;
     a.row = row;
