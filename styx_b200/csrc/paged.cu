@@ -24,7 +24,12 @@ namespace {
 // The angle in turns, pos * base^(-2i/d) / 2 pi, is held in 64 bits and
 // reduced to a fraction of a turn before it is rounded to f32, so its error
 // does not grow with the position.
-constexpr int kAppThreads = 128, kAppRows = 4;
+// Bound by HBM on prompts (8191 tokens of 32 q and 2 x 4 k / v heads of 128:
+// 319 MB in 57 us, 5.6 TB/s; two rows at a time and 32 warps per SM: 65 us
+// with four rows, whose registers spill at that many warps, 61 with four rows
+// and 20 warps), by the latency of position, page and rows on a step of 64
+// tokens (3.6 us).
+constexpr int kAppThreads = 128, kAppRows = 2;
 
 template <class T>
 __device__ __forceinline__ void store4(T *p, const float (&v)[4]) {
@@ -37,7 +42,7 @@ __device__ __forceinline__ void store4(T *p, const float (&v)[4]) {
 // else loads and stores are by element.  splits: warps per token, share rows
 // each.
 template <class T, int LPR, bool VEC>
-__global__ void __launch_bounds__(kAppThreads) k_paged_append(PagedAppendArgs a, int splits, int share) {
+__global__ void __launch_bounds__(kAppThreads, 8) k_paged_append(PagedAppendArgs a, int splits, int share) {
     pdl_trigger();
     constexpr int RPW = 32 / LPR;
     const PagedKv &kv = a.kv;
@@ -464,8 +469,10 @@ __global__ void __launch_bounds__(256) k_evict_move(PagedEvictArgs a, int blocks
 cudaError_t launch_paged_append(const PagedAppendArgs &a, int sms, cudaStream_t st) {
     const int rows = a.n_heads + 2 * a.kv.n_kv, hd = a.kv.hd, lpr = hd <= 64 ? 8 : hd <= 128 ? 16 : 32;
     const int batch = kAppRows * (32 / lpr), batches = (rows + batch - 1) / batch;
-    // warps per token: one for each batch of rows while that makes no more than eight waves of 24 warps per SM
-    const long long want = (8ll * 24 * sms + a.n_tokens - 1) / a.n_tokens;
+    // warps per token: one where that fills the SMs (24 warps each), else as many as there are batches of rows
+    // (8191 tokens of 32 + 2 x 4 rows: 61 us with one warp each, 69 with three, 72 with five, at four rows at a time;
+    // 64 tokens: 4.1 us with five)
+    const long long want = (24ll * sms + a.n_tokens - 1) / a.n_tokens;
     const int share = (batches + static_cast<int>(std::min<long long>(batches, want)) - 1) /
                       static_cast<int>(std::min<long long>(batches, want)) * batch;
     const int splits = (rows + share - 1) / share;
