@@ -105,14 +105,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_fma(PagedAttendArgs a) {
         const int row0 = lo + warp * Y::rpw + rw;
         float *scores = a.scores + (static_cast<long long>(wk.b) * kv.n_kv + j) *
                                        (static_cast<long long>(kv.max_pages) << kv.page_shift) * a.gqa + g0;
-        float2 q[NH][4];
-#pragma unroll
-        for (int h = 0; h < NH; h++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const int c = Y::elem(rl, e);
-                (&q[h][0].x)[e] = h < ng && c < hd ? ld_now(a.q + (h0 + h) * hd + c) * l2 : 0.f;
-            }
         float2 o[NH][4];
 #pragma unroll
         for (int h = 0; h < NH; h++)
@@ -142,13 +134,25 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_fma(PagedAttendArgs a) {
             asm volatile("cp.async.commit_group;" ::: "memory");
             return ok;
         };
+        // the first rows' pages and q, all loads at once, then the first copies
         unsigned seen = 0;                           // bit it % 32: that iteration's row is seen
-        int page = page_of(0);
-        for (int it = 0; it < Y::stages - 1; it++) {
-            const int nx = page_of(it + 1);
-            seen |= static_cast<unsigned>(copy(it, page)) << (it & 31);
-            page = nx;
-        }
+        int pages[Y::stages];
+#pragma unroll
+        for (int it = 0; it < Y::stages; it++) pages[it] = page_of(it);
+        float2 q[NH][4];
+#pragma unroll
+        for (int h = 0; h < NH; h++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int c = Y::elem(rl, 4 * i);    // (head_dim is a multiple of 4)
+                const float4 v = h < ng && c < hd ? *reinterpret_cast<const float4 *>(a.q + (h0 + h) * hd + c)
+                                                  : make_float4(0.f, 0.f, 0.f, 0.f);
+                q[h][2 * i] = make_float2(v.x * l2, v.y * l2);
+                q[h][2 * i + 1] = make_float2(v.z * l2, v.w * l2);
+            }
+#pragma unroll
+        for (int it = 0; it < Y::stages - 1; it++) seen |= static_cast<unsigned>(copy(it, pages[it])) << (it & 31);
+        int page = pages[Y::stages - 1];
         for (int it = 0; it < iters; it++) {
             const int nxt = it + Y::stages - 1, np = page_of(nxt + 1);
             const unsigned bit = 1u << (nxt & 31);
