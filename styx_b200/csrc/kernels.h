@@ -394,6 +394,7 @@ struct PagedAttendArgs {
     float scale;
     int window, n_heads, gqa;
     int ctas;                      // of the launch: portions are theirs
+    int tile_shift, seg_cost;      // see paged_split.cuh; the kernel's
     // workspace (with acc_out): scores in units of log2, [n_seqs][n_kv][max
     // rows][gqa]; maximum and sum of every head, [n_seqs][n_heads][2]
     float *scores, *ml;

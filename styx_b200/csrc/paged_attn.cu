@@ -21,6 +21,7 @@ namespace {
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int NH = 8;                 // q heads of a group
 constexpr int kPitch = 256;           // floats of a head's O in a portion's result
+constexpr int kSets = 2;              // rows of a lane at once: two chains of exchanges in flight
 constexpr float kSlack = 8.f;
 
 // LPR lanes per row, 8 elements each: head_dim <= 8 LPR.  f32: two 16-byte
@@ -28,9 +29,10 @@ constexpr float kSlack = 8.f;
 template <class T, int LPR>
 struct Lay {
     static constexpr int chunks = sizeof(T) == 4 ? 2 : 1;
-    static constexpr int rpw = 32 / LPR;                      // rows of a warp at once
-    static constexpr int stage = 2 * chunks * 16 * kThreads;  // bytes of a stage, K then V
-    static constexpr int stages = sizeof(T) == 4 ? 10 : 16;   // 160 KB, 128 KB
+    static constexpr int rpw = 32 / LPR;                      // rows of a warp side by side
+    static constexpr int set = 2 * chunks * 16 * kThreads;    // bytes of the CTA's rows side by side, K then V
+    static constexpr int stage = kSets * set;
+    static constexpr int stages = (sizeof(T) == 4 ? 10 : 16) / kSets;   // 160 KB, 128 KB
     __device__ static __forceinline__ int elem(int l, int e) {   // element e of lane l of the row
         return chunks == 2 ? (e < 4 ? 4 * l + e : 4 * (LPR + l) + e - 4) : 8 * l + e;
     }
@@ -93,14 +95,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_fma(PagedAttendArgs a) {
     const int myh = ((rl & (LPR / 2)) ? 4 : 0) | ((rl & (LPR / 4)) ? 2 : 0) | ((rl & (LPR / 8)) ? 1 : 0);
     const uint32_t mine = smem_addr(ring) + tid * 16;
     const float l2 = a.scale * 1.4426950408889634f;
-    constexpr int STEP = kWarps * Y::rpw;            // rows of the CTA at once
+    constexpr int SIDE = kWarps * Y::rpw, STEP = kSets * SIDE;   // rows of the CTA side by side; at once
 
     while (wk.next(a, segs)) {
         const Seq s(a, wk.b, false);
         const int j = wk.seg / groups, g0 = (wk.seg - j * groups) * NH, ng = min(NH, a.gqa - g0);
         const long long h0 = static_cast<long long>(wk.b) * a.n_heads + j * a.gqa + g0;
         const int32_t *table = kv.table + static_cast<long long>(wk.b) * kv.table_stride;
-        const int lo = max(s.first, (s.tile0 + wk.t0) * kTile), hi = min(s.n, (s.tile0 + wk.t1) * kTile);
+        const int lo = max(s.first, (s.tile0 + wk.t0) << a.tile_shift);
+        const int hi = static_cast<int>(min(static_cast<long long>(s.n), static_cast<long long>(s.tile0 + wk.t1) << a.tile_shift));
         const int iters = hi > lo ? (hi - lo + STEP - 1) / STEP : 0;
         const int row0 = lo + warp * Y::rpw + rw;
         float *scores = a.scores + (static_cast<long long>(wk.b) * kv.n_kv + j) *
@@ -111,19 +114,20 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_fma(PagedAttendArgs a) {
 #pragma unroll
             for (int e = 0; e < 4; e++) o[h][e] = make_float2(0.f, 0.f);
         float m = kNone, l = 0.f;                    // of head myh, over this lane's rows
-        auto page_of = [&](int it) {
-            const int r = row0 + it * STEP;
-            return it < iters && r < hi ? ld_now(table + (r >> kv.page_shift)) : -1;
+        // set n: the lane's row row0 + n SIDE
+        auto page_of = [&](int n) {
+            const int r = row0 + n * SIDE;
+            return r < hi ? ld_now(table + (r >> kv.page_shift)) : -1;
         };
-        // copies of iteration `it` into its stage; returns whether the row is seen
-        auto copy = [&](int it, int page) {
-            const int r = row0 + it * STEP;
-            const bool in = it < iters && r < hi, ok = in && static_cast<unsigned>(page) < static_cast<unsigned>(kv.n_pages);
+        // copies of set n; returns whether its row is seen
+        auto copy = [&](int n, int page) {
+            const int r = row0 + n * SIDE;
+            const bool in = r < hi, ok = in && static_cast<unsigned>(page) < static_cast<unsigned>(kv.n_pages);
             if (in && !ok && rl == 0) atomicExch(kv.err, kErrBadPos);
             const long long off = ok ? page * kv.page_stride + static_cast<long long>((j << kv.page_shift) +
                                                                                      (r & ((1 << kv.page_shift) - 1))) * hd
                                      : 0;
-            const uint32_t dst = mine + (it % Y::stages) * Y::stage;
+            const uint32_t dst = mine + (n % (kSets * Y::stages)) * Y::set;
 #pragma unroll
             for (int c = 0; c < Y::chunks; c++) {
                 const int e = Y::elem(rl, 4 * c);
@@ -131,14 +135,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_fma(PagedAttendArgs a) {
                 copy16(dst + c * 16 * kThreads, static_cast<const T *>(kv.k) + (on ? off + e : 0), on);
                 copy16(dst + (Y::chunks + c) * 16 * kThreads, static_cast<const T *>(kv.v) + (on ? off + e : 0), on);
             }
-            asm volatile("cp.async.commit_group;" ::: "memory");
             return ok;
         };
         // the first rows' pages and q, all loads at once, then the first copies
-        unsigned seen = 0;                           // bit it % 32: that iteration's row is seen
-        int pages[Y::stages];
+        unsigned seen = 0;                           // bit n % 32: set n's row is seen
+        int pages[kSets * Y::stages];
 #pragma unroll
-        for (int it = 0; it < Y::stages; it++) pages[it] = page_of(it);
+        for (int n = 0; n < kSets * Y::stages; n++) pages[n] = page_of(n);
         float2 q[NH][4];
 #pragma unroll
         for (int h = 0; h < NH; h++)
@@ -151,50 +154,67 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_fma(PagedAttendArgs a) {
                 q[h][2 * i + 1] = make_float2(v.z * l2, v.w * l2);
             }
 #pragma unroll
-        for (int it = 0; it < Y::stages - 1; it++) seen |= static_cast<unsigned>(copy(it, pages[it])) << (it & 31);
-        int page = pages[Y::stages - 1];
+        for (int n = 0; n < kSets * (Y::stages - 1); n++) {
+            seen |= static_cast<unsigned>(copy(n, pages[n])) << (n & 31);
+            if (n % kSets == kSets - 1) asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+        int page[kSets];
+#pragma unroll
+        for (int u = 0; u < kSets; u++) page[u] = pages[kSets * (Y::stages - 1) + u];
         for (int it = 0; it < iters; it++) {
-            const int nxt = it + Y::stages - 1, np = page_of(nxt + 1);
-            const unsigned bit = 1u << (nxt & 31);
-            seen = copy(nxt, page) ? seen | bit : seen & ~bit;
-            page = np;
+#pragma unroll
+            for (int u = 0; u < kSets; u++) {
+                const int n = kSets * (it + Y::stages - 1) + u, np = page_of(n + kSets);
+                const unsigned bit = 1u << (n & 31);
+                seen = copy(n, page[u]) ? seen | bit : seen & ~bit;
+                page[u] = np;
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
             asm volatile("cp.async.wait_group %0;" ::"n"(Y::stages - 1) : "memory");
             const uint8_t *st = ring + (it % Y::stages) * Y::stage + tid * 16;
-            float kf[8];
-            unpack<T>(st, kf);
-            float d[NH];
+            float x[kSets];
+            bool on[kSets], rises = false;
 #pragma unroll
-            for (int h = 0; h < NH; h++) {
-                float2 t = make_float2(0.f, 0.f);
+            for (int u = 0; u < kSets; u++) {
+                float kf[8];
+                unpack<T>(st + u * Y::set, kf);
+                float d[NH];
 #pragma unroll
-                for (int e = 0; e < 4; e++) fma2(t, q[h][e], make_float2(kf[2 * e], kf[2 * e + 1]));
-                d[h] = t.x + t.y;
+                for (int h = 0; h < NH; h++) {
+                    float2 t = make_float2(0.f, 0.f);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) fma2(t, q[h][e], make_float2(kf[2 * e], kf[2 * e + 1]));
+                    d[h] = t.x + t.y;
+                }
+                // sums over the row's lanes: eight values halve three times, the rest is one value
+                float t4[4], t2[2];
+                {
+                    const bool up = rl & (LPR / 2);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) t4[i] = (up ? d[4 + i] : d[i]) + __shfl_xor_sync(0xffffffffu, up ? d[i] : d[4 + i], LPR / 2);
+                }
+                {
+                    const bool up = rl & (LPR / 4);
+#pragma unroll
+                    for (int i = 0; i < 2; i++) t2[i] = (up ? t4[2 + i] : t4[i]) + __shfl_xor_sync(0xffffffffu, up ? t4[i] : t4[2 + i], LPR / 4);
+                }
+                {
+                    const bool up = rl & (LPR / 8);
+                    x[u] = (up ? t2[1] : t2[0]) + __shfl_xor_sync(0xffffffffu, up ? t2[0] : t2[1], LPR / 8);
+                }
+#pragma unroll
+                for (int k = LPR / 16; k; k >>= 1) x[u] += __shfl_xor_sync(0xffffffffu, x[u], k);
+                const int n = kSets * it + u, r = row0 + n * SIDE;
+                on[u] = (seen >> (n & 31)) & 1;
+                if (a.acc_out && r < hi && (rl & (LPR / 8 - 1)) == 0 && myh < ng)
+                    scores[static_cast<long long>(r) * a.gqa + myh] = on[u] ? x[u] : -INFINITY;
+                rises |= on[u] && x[u] > m + kSlack;
             }
-            // sums over the row's lanes: eight values halve three times, the rest is one value
-            float t4[4], t2[2], x;
-            {
-                const bool up = rl & (LPR / 2);
-#pragma unroll
-                for (int i = 0; i < 4; i++) t4[i] = (up ? d[4 + i] : d[i]) + __shfl_xor_sync(0xffffffffu, up ? d[i] : d[4 + i], LPR / 2);
-            }
-            {
-                const bool up = rl & (LPR / 4);
-#pragma unroll
-                for (int i = 0; i < 2; i++) t2[i] = (up ? t4[2 + i] : t4[i]) + __shfl_xor_sync(0xffffffffu, up ? t4[i] : t4[2 + i], LPR / 4);
-            }
-            {
-                const bool up = rl & (LPR / 8);
-                x = (up ? t2[1] : t2[0]) + __shfl_xor_sync(0xffffffffu, up ? t2[0] : t2[1], LPR / 8);
-            }
-#pragma unroll
-            for (int k = LPR / 16; k; k >>= 1) x += __shfl_xor_sync(0xffffffffu, x, k);
-            const bool on = (seen >> (it & 31)) & 1;
-            const int r = row0 + it * STEP;
-            if (a.acc_out && r < hi && (rl & (LPR / 8 - 1)) == 0 && myh < ng)
-                scores[static_cast<long long>(r) * a.gqa + myh] = on ? x : -INFINITY;
-            if (__any_sync(0xffffffffu, on && x > m + kSlack)) {
+            if (__any_sync(0xffffffffu, rises)) {
                 // the warp's maximum of every head; what was summed is rescaled
-                float mx = on ? x : kNone;
+                float mx = kNone;
+#pragma unroll
+                for (int u = 0; u < kSets; u++) mx = on[u] ? fmaxf(mx, x[u]) : mx;
 #pragma unroll
                 for (int k = LPR; k < 32; k <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
                 mx = fmaxf(m, mx);
@@ -212,16 +232,23 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_fma(PagedAttendArgs a) {
                     }
                 }
             }
-            const float p = on ? ex2(x - m) : 0.f;
-            l += p;
-            float vf[8];
-            unpack<T>(st + Y::chunks * 16 * kThreads, vf);
+            float p[kSets];
 #pragma unroll
-            for (int h = 0; h < NH; h++) {
-                const int src = ((h & 4) ? LPR / 2 : 0) | ((h & 2) ? LPR / 4 : 0) | ((h & 1) ? LPR / 8 : 0);
-                const float ph = __shfl_sync(0xffffffffu, p, src, LPR);
+            for (int u = 0; u < kSets; u++) {
+                p[u] = on[u] ? ex2(x[u] - m) : 0.f;
+                l += p[u];
+            }
 #pragma unroll
-                for (int e = 0; e < 4; e++) fma2(o[h][e], make_float2(ph, ph), make_float2(vf[2 * e], vf[2 * e + 1]));
+            for (int u = 0; u < kSets; u++) {
+                float vf[8];
+                unpack<T>(st + u * Y::set + Y::chunks * 16 * kThreads, vf);
+#pragma unroll
+                for (int h = 0; h < NH; h++) {
+                    const int src = ((h & 4) ? LPR / 2 : 0) | ((h & 2) ? LPR / 4 : 0) | ((h & 1) ? LPR / 8 : 0);
+                    const float ph = __shfl_sync(0xffffffffu, p[u], src, LPR);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) fma2(o[h][e], make_float2(ph, ph), make_float2(vf[2 * e], vf[2 * e + 1]));
+                }
             }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
@@ -455,7 +482,7 @@ cudaError_t finish(const PagedAttendArgs &a, cudaStream_t st) {
     const int groups = (a.gqa + NHG - 1) / NHG;
     const long long segs = static_cast<long long>(a.kv.n_seqs) * a.kv.n_kv * groups;
     // nothing is cut where no sequence can have a second tile
-    const bool cut = rows > kTile;
+    const bool cut = rows > (1ll << a.tile_shift);
     const long long want = (rows + 255) / 256, lines = static_cast<long long>(a.kv.n_seqs) * a.kv.n_kv;
     const int row_blocks = a.acc_out ? static_cast<int>(want < 4096 ? want : 4096) : 0;
     // eight warps per head where that is a wave of CTAs at most (148 SMs x 8), else one
@@ -489,7 +516,7 @@ cudaError_t launch_t(const PagedAttendArgs &a, int grid, cudaStream_t st) {
 int attend_grid(const PagedAttendArgs &a, int nh, int sms) {
     // no more CTAs than tiles there can be
     const long long tiles = static_cast<long long>(a.kv.n_seqs) * a.kv.n_kv * ((a.gqa + nh - 1) / nh) *
-                            (((static_cast<long long>(a.kv.max_pages) << a.kv.page_shift) + kTile - 1) / kTile);
+                            (((static_cast<long long>(a.kv.max_pages) << a.kv.page_shift) + (1ll << a.tile_shift) - 1) >> a.tile_shift);
     return static_cast<int>(tiles < sms ? tiles : sms);
 }
 
@@ -499,6 +526,8 @@ cudaError_t launch_attend_finish(const PagedAttendArgs &a, int nh, int pitch, cu
 }
 
 cudaError_t launch_attend_fma(PagedAttendArgs a, int sms, cudaStream_t st) {
+    a.tile_shift = a.kv.hd <= 64 ? 6 : 5;   // the rows that a CTA takes at once (head_dim above 128: twice those)
+    a.seg_cost = 3;
     const int grid = a.ctas = attend_grid(a, NH, sms);
     const cudaError_t e = a.kv.dtype == STYX_F16    ? launch_t<__half>(a, grid, st)
                           : a.kv.dtype == STYX_BF16 ? launch_t<__nv_bfloat16>(a, grid, st)

@@ -111,8 +111,8 @@ struct Part {
         ng = min(nh, a.gqa - g0);
         h0 = static_cast<long long>(b) * a.n_heads + j * a.gqa + g0;
         table = a.kv.table + static_cast<long long>(b) * a.kv.table_stride;
-        lo = max(s.first, (s.tile0 + wk.t0) * kTile);
-        hi = min(s.n, (s.tile0 + wk.t1) * kTile);
+        lo = max(s.first, (s.tile0 + wk.t0) << a.tile_shift);
+        hi = static_cast<int>(min(static_cast<long long>(s.n), static_cast<long long>(s.tile0 + wk.t1) << a.tile_shift));
         base = lo & ~(kRows - 1);
         iters = hi > lo ? (hi - base + kRows * TEAMS - 1) / (kRows * TEAMS) : 0;
     }
@@ -445,6 +445,8 @@ cudaError_t launch_t(const PagedAttendArgs &a, int team, cudaStream_t st) {
 
 cudaError_t launch_attend_mma(PagedAttendArgs a, int sms, cudaStream_t st) {
     const int team = a.gqa <= 8 ? 1 : 2;
+    a.tile_shift = 7;
+    a.seg_cost = 3;
     a.ctas = attend_grid(a, 8 * team, sms);
     return a.kv.dtype == STYX_BF16 ? launch_t<true>(a, team, st) : launch_t<false>(a, team, st);
 }

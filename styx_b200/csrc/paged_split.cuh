@@ -1,6 +1,8 @@
 // paged_split.cuh -- how the paged attention kernels cut their work: tiles of
-// 128 rows of one (sequence, kv head, group of q heads), all tiles of a call
-// in one list, an equal share of it to every CTA.
+// 2^tile_shift rows of one (sequence, kv head, group of q heads), all tiles of
+// a call in one list, an equal share of it to every CTA.  What a segment's
+// start costs a CTA (q, the first maxima, the result) counts as seg_cost
+// tiles, so that CTAs with many short segments get fewer of them.
 #pragma once
 
 #include "paged.cuh"
@@ -8,11 +10,6 @@
 namespace styx {
 namespace {
 
-constexpr int kTile = 128;                 // rows of a tile
-// what a segment's start costs a CTA (q, the first maxima, the result), in
-// tiles: the partition counts it, so that CTAs with many short segments get
-// fewer tiles
-constexpr int kSegCost = 3;
 constexpr float kNone = -3e38f;            // maximum of no scores: finite, so that differences stay numbers
 
 __device__ __forceinline__ float ex2(float x) {
@@ -28,20 +25,20 @@ struct Seq {
     __device__ __forceinline__ Seq(const PagedAttendArgs &a, int b, bool report) {
         n = paged_len(a.kv, b, report);
         first = a.window > 0 && a.window < n ? n - a.window : 0;
-        tile0 = first / kTile;
-        nt = max(1, (n + kTile - 1) / kTile - tile0);
+        tile0 = first >> a.tile_shift;
+        nt = max(1, static_cast<int>((n + (1ll << a.tile_shift) - 1) >> a.tile_shift) - tile0);
     }
 };
 
-// the CTA's share of the list, portion by portion.  A segment is kSegCost
+// the CTA's share of the list, portion by portion.  A segment is seg_cost
 // empty units, then its tiles.
 struct Walk {
-    int b, seg, u, nt;             // sequence, (kv head, group) in it, next unit of kSegCost + nt
+    int b, seg, u, nt;             // sequence, (kv head, group) in it, next unit of seg_cost + nt
     long long at, end;             // global unit numbers
     int t0, t1;                    // the portion: tiles [t0, t1) of the segment
     __device__ __forceinline__ bool next(const PagedAttendArgs &a, int segs) {
         while (at < end) {
-            if (u == kSegCost + nt) {
+            if (u == a.seg_cost + nt) {
                 u = 0;
                 if (++seg == segs) {
                     seg = 0;
@@ -52,9 +49,9 @@ struct Walk {
                     nt = Seq(a, b, false).nt;
                 }
             }
-            const int u1 = static_cast<int>(min(static_cast<long long>(kSegCost + nt), u + (end - at)));
-            t0 = max(0, u - kSegCost);
-            t1 = max(0, u1 - kSegCost);
+            const int u1 = static_cast<int>(min(static_cast<long long>(a.seg_cost + nt), u + (end - at)));
+            t0 = max(0, u - a.seg_cost);
+            t1 = max(0, u1 - a.seg_cost);
             at += u1 - u;
             u = u1;
             if (t1 > t0) return true;
@@ -84,7 +81,7 @@ __device__ __forceinline__ void share_of(const PagedAttendArgs &a, int segs, Sha
     const int tid = threadIdx.x, lane = tid & 31, n = a.kv.n_seqs;
     const int per = (n + THREADS - 1) / THREADS, lo = min(n, tid * per), hi = min(n, lo + per);
     long long mine = 0;
-    for (int b = lo; b < hi; b++) mine += static_cast<long long>(Seq(a, b, blockIdx.x == 0).nt + kSegCost) * segs;
+    for (int b = lo; b < hi; b++) mine += static_cast<long long>(Seq(a, b, blockIdx.x == 0).nt + a.seg_cost) * segs;
     sh.scan[tid] = mine;
     __syncthreads();
     if (tid < 32) {   // inclusive scan of the chunks, PER of them per lane
@@ -112,7 +109,7 @@ __device__ __forceinline__ void share_of(const PagedAttendArgs &a, int segs, Sha
         long long off = at - before;
         int b = lo;
         for (; b < hi; b++) {
-            const long long nb = static_cast<long long>(Seq(a, b, false).nt + kSegCost) * segs;
+            const long long nb = static_cast<long long>(Seq(a, b, false).nt + a.seg_cost) * segs;
             if (off < nb) break;
             off -= nb;
         }
@@ -122,8 +119,8 @@ __device__ __forceinline__ void share_of(const PagedAttendArgs &a, int segs, Sha
     __syncthreads();
     w.b = sh.b0;
     w.nt = Seq(a, w.b, false).nt;
-    w.seg = static_cast<int>(mul_div(1, sh.off, w.nt + kSegCost));
-    w.u = static_cast<int>(sh.off - static_cast<long long>(w.seg) * (w.nt + kSegCost));
+    w.seg = static_cast<int>(mul_div(1, sh.off, w.nt + a.seg_cost));
+    w.u = static_cast<int>(sh.off - static_cast<long long>(w.seg) * (w.nt + a.seg_cost));
     w.at = at;
     w.end = end;
 }
