@@ -31,6 +31,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cstddef>
 #include <cstdint>
 
 #include "cluster.cuh"
@@ -262,7 +263,7 @@ constexpr int kTopK = 120;                  // top-k by the warps' maxima (128 o
 
 struct CtaShared {
     union {
-        unsigned hist[3][kBins];            // counts, or the low and high words of the weights' sums (0, 1)
+        __align__(16) unsigned hist[3][kBins];            // counts, or the low and high words of the weights' sums (0, 1)
         u64 cand[kCap];                     // (inverted key << 32) | index: ascending = the order of the tokens
     };
     u64 red[32], ent[2][kNW + 1];
@@ -273,7 +274,9 @@ struct CtaShared {
     __align__(16) float top[kC * kNW];
     u64 sum[2][kC], before, ties;
     unsigned cnt[2][kC], n_of[kC], step, thr;
+    int n_of_warp[kNW], row;                // the order of the rows
 };
+static_assert(offsetof(CtaShared, hist) % 16 == 0 && offsetof(CtaShared, top) % 16 == 0, "read by 16 bytes");
 
 __device__ __forceinline__ void cluster_sync() {
     cl_arrive();
@@ -407,13 +410,17 @@ __device__ __forceinline__ void cta_sort(u64 *buf, int n) {
 // slice: logits of a CTA, kNW * region of them, a warp's stretch each (region
 // a multiple of 128).  bulk: the slices start on 16 bytes, and one bulk copy
 // brings a CTA's.
-__global__ void __launch_bounds__(kNT, 2) k_sample_cluster(SampleArgs a, int region, bool bulk) {
+// by_weight: clusters take the rows that need a histogram first, so that none
+// of these is begun when the others are done (rows more than fit the SMs at
+// once, settings for no more than a CTA's threads)
+__global__ void __launch_bounds__(kNT, 2) k_sample_cluster(SampleArgs a, int region, bool bulk, bool by_weight) {
     extern __shared__ __align__(128) float xs[];
     __shared__ __align__(16) CtaShared sh;
     pdl_trigger();
     cl_arrive_relaxed();                          // the others have started: waited for before the first store to them
     const uint32_t rank = cluster_ctarank();
-    const int b = blockIdx.x / kC, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n = a.n_vocab;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n = a.n_vocab;
+    int b = blockIdx.x / kC;
     const int slice = kNW * region, lo = static_cast<int>(rank) * slice, len = max(0, min(n - lo, slice));
     const int first = warp * region;              // the warp's stretch of the slice
     auto peer = [&](const void *p, uint32_t r) { return cl_map(smem_addr(p), r); };
@@ -424,6 +431,25 @@ __global__ void __launch_bounds__(kNT, 2) k_sample_cluster(SampleArgs a, int reg
         fence_mbar_init();
     }
     pdl_wait();
+    if (by_weight) {
+        bool heavy = false;
+        if (tid < a.n_rows) {
+            const int k = a.top_k ? a.top_k[tid] : 0;
+            const bool all = k <= 0 || k >= n;
+            heavy = !(a.temperature && !(a.temperature[tid] > 0.f)) && (all ? a.top_p && a.top_p[tid] < 1.f : k > kTopK);
+        }
+        const unsigned votes = __ballot_sync(0xffffffffu, heavy);
+        if (lane == 0) sh.n_of_warp[warp] = __popc(votes);
+        __syncthreads();
+        int before = __popc(votes & ((1u << lane) - 1)), all = 0;
+        for (int w = 0; w < kNW; w++) {
+            before += w < warp ? sh.n_of_warp[w] : 0;
+            all += sh.n_of_warp[w];
+        }
+        if (tid < a.n_rows && (heavy ? before : all + tid - before) == b) sh.row = tid;
+        __syncthreads();
+        b = sh.row;
+    }
     // ---------------- the slice, once; the warps' maxima
     const float *src = a.logits + b * a.row_stride + lo;
     const int whole4 = bulk ? len & ~3 : 0;
@@ -930,7 +956,8 @@ cudaError_t launch_sample(const SampleArgs &a, cudaStream_t st) {
     at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, k_sample_cluster, a, region, bulk);
+    // (two CTAs fit an SM: more than 32 clusters are more than one wave)
+    return cudaLaunchKernelEx(&cfg, k_sample_cluster, a, region, bulk, a.n_rows > 32 && a.n_rows <= kNT);
 }
 
 }  // namespace styx

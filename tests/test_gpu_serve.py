@@ -585,3 +585,20 @@ def test_refusals():
     assert L.styx_paged_attend(cx, None, kv._ref, 8, q.data_ptr(), 1.0, 0, out.data_ptr(), None, None, None, 0,
                                ws.data_ptr(), 16) == _lib.STYX_EINVAL and b"workspace" in L.styx_last_error()
     kv.ctx.check_device_error()
+
+
+@pytest.mark.parametrize("rows", [33, 130, 600])
+def test_sample_rows_do_not_depend_on_their_batch(rows):
+    """Batches of more rows than fit the device at once are taken in another order: the same tokens and logprobs, bit
+    for bit, as eight rows at a time."""
+    rng = np.random.default_rng(rows)
+    V = 1000
+    x = T(rng.normal(0, 3, (rows, V)).astype(np.float32))
+    par = [SETTINGS[i % len(SETTINGS)] for i in rng.permutation(rows)]
+    t, k, p, m = (T(np.array([q[i] for q in par], np.int32 if i == 1 else np.float32)) for i in range(4))
+    u = T(rng.uniform(0, 1, rows).astype(np.float32))
+    token, logprob = ops.sample(x, u, t, k, p, m)
+    for i in range(0, rows, 8):
+        s = slice(i, i + 8)
+        tok, lp = ops.sample(x[s], u[s], t[s], k[s], p[s], m[s])
+        assert torch.equal(tok, token[s]) and torch.equal(lp, logprob[s])
