@@ -80,7 +80,6 @@ template <class T, int LPR>
 __global__ void __launch_bounds__(kThreads, 1) k_attend_fma(PagedAttendArgs a) {
     using Y = Lay<T, LPR>;
     extern __shared__ __align__(16) uint8_t ring[];
-    __shared__ Share<kThreads> share;
     __shared__ float s_m[kWarps][NH], s_l[kWarps][NH], s_L[NH], s_M[NH];
     const PagedKv &kv = a.kv;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hd = kv.hd;
@@ -90,7 +89,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_fma(PagedAttendArgs a) {
     pdl_wait();
     long long T_, G;
     Walk wk;
-    share_of<kThreads>(a, segs, share, wk, T_, G);
+    share_of(a, segs, wk, T_, G);
     // the head whose sum the halving exchanges leave in this lane: from the lane bits LPR/2, LPR/4, LPR/8
     const int myh = ((rl & (LPR / 2)) ? 4 : 0) | ((rl & (LPR / 4)) ? 2 : 0) | ((rl & (LPR / 8)) ? 1 : 0);
     const uint32_t mine = smem_addr(ring) + tid * 16;

@@ -134,8 +134,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_mma(PagedAttendArgs a) {
     Walk wk;
     pdl_trigger();
     pdl_wait();
-    share_of<kThreads>(a, segs, *reinterpret_cast<Share<kThreads> *>(smem), wk, T, G);
-    __syncthreads();                  // what it left in the ring is read
+    share_of(a, segs, wk, T, G);
     const uint32_t ring = smem_addr(smem) + team * S * kUnit;
     float *so = reinterpret_cast<float *>(smem + kRing);
     const float l2 = a.scale * 1.4426950408889634f;   // scores in units of log2

@@ -67,60 +67,41 @@ __device__ __forceinline__ long long mul_div(long long x, long long y, long long
     return p >> 32 ? static_cast<long long>(p / d) : static_cast<long long>(static_cast<unsigned>(p) / static_cast<unsigned>(d));
 }
 
-// A CTA's share: units before each chunk of sequences, their total T, the
-// first of CTA i's units (floor(i T / G)) as (sequence, head, unit).
-template <int THREADS>
-struct Share {
-    long long scan[THREADS], off;
-    int b0;
-};
-template <int THREADS>
-__device__ __forceinline__ void share_of(const PagedAttendArgs &a, int segs, Share<THREADS> &sh, Walk &w, long long &T,
-                                         long long &G) {
-    constexpr int PER = THREADS / 32;
-    const int tid = threadIdx.x, lane = tid & 31, n = a.kv.n_seqs;
-    const int per = (n + THREADS - 1) / THREADS, lo = min(n, tid * per), hi = min(n, lo + per);
+// A CTA's share: the units of all sequences, T, and the first of CTA i's
+// (floor(i T / G)) as (sequence, head, unit).  Every warp finds it for itself,
+// a run of sequences per lane: with the CTA's barriers it was twice as long.
+__device__ __forceinline__ void share_of(const PagedAttendArgs &a, int segs, Walk &w, long long &T, long long &G) {
+    const int lane = threadIdx.x & 31, n = a.kv.n_seqs;
+    const int per = (n + 31) / 32, lo = min(n, lane * per), hi = min(n, lo + per);
+    const bool report = blockIdx.x == 0 && threadIdx.x < 32;
+    auto units = [&](int b, bool r) { return static_cast<long long>(Seq(a, b, r).nt + a.seg_cost) * segs; };
     long long mine = 0;
-    for (int b = lo; b < hi; b++) mine += static_cast<long long>(Seq(a, b, blockIdx.x == 0).nt + a.seg_cost) * segs;
-    sh.scan[tid] = mine;
-    __syncthreads();
-    if (tid < 32) {   // inclusive scan of the chunks, PER of them per lane
-        long long v[PER], run = 0;
+#pragma unroll 4
+    for (int b = lo; b < hi; b++) mine += units(b, report);
+    long long upto = mine;
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
-            run += sh.scan[lane * PER + i];
-            v[i] = run;
-        }
-        long long x = run;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long u = __shfl_up_sync(0xffffffffu, x, o);
-            if (lane >= o) x += u;
-        }
-#pragma unroll
-        for (int i = 0; i < PER; i++) sh.scan[lane * PER + i] = v[i] + x - run;
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long u = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += u;
     }
-    __syncthreads();
-    T = sh.scan[THREADS - 1];
+    T = __shfl_sync(0xffffffffu, upto, 31);
     G = min(static_cast<long long>(gridDim.x), T);
     const long long i = blockIdx.x, at = i < G ? mul_div(i, T, G) : 0, end = i < G ? mul_div(i + 1, T, G) : 0;
-    const long long before = sh.scan[tid] - mine;
-    if (mine > 0 && at >= before && at < before + mine) {
-        long long off = at - before;
-        int b = lo;
-        for (; b < hi; b++) {
-            const long long nb = static_cast<long long>(Seq(a, b, false).nt + a.seg_cost) * segs;
+    const int src = __ffs(__ballot_sync(0xffffffffu, at < upto)) - 1;   // (at < T, so there is one)
+    long long off = at - (upto - mine);
+    int b = lo;
+    if (lane == src)
+        for (; b < hi - 1; b++) {
+            const long long nb = units(b, false);
             if (off < nb) break;
             off -= nb;
         }
-        sh.b0 = b;
-        sh.off = off;
-    }
-    __syncthreads();
-    w.b = sh.b0;
+    w.b = __shfl_sync(0xffffffffu, b, src);
+    off = __shfl_sync(0xffffffffu, off, src);
     w.nt = Seq(a, w.b, false).nt;
-    w.seg = static_cast<int>(mul_div(1, sh.off, w.nt + a.seg_cost));
-    w.u = static_cast<int>(sh.off - static_cast<long long>(w.seg) * (w.nt + a.seg_cost));
+    w.seg = static_cast<int>(min(mul_div(1, off, w.nt + a.seg_cost), static_cast<long long>(segs - 1)));
+    w.u = static_cast<int>(min(off - static_cast<long long>(w.seg) * (w.nt + a.seg_cost),
+                               static_cast<long long>(w.nt + a.seg_cost)));   // (bounds: lengths that changed)
     w.at = at;
     w.end = end;
 }

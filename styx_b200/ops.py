@@ -672,20 +672,22 @@ def argmax_f32(x: torch.Tensor, out: Optional[torch.Tensor] = None, stream=None)
 _KV_TYPES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 
 
-def _checked(t: torch.Tensor, dtype: torch.dtype, shape: tuple, what: str, index: int) -> int:
-    """The address of a contiguous tensor of that type and shape on that device; ValueError for any other."""
-    if t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.get_device() == index:
-        return t.data_ptr()
+def _refuse(t: torch.Tensor, dtype: torch.dtype, shape: tuple, what: str, index: int) -> int:
     raise ValueError(f"{what}: contiguous {dtype} {tuple(shape)} on cuda:{index} expected, got {t.dtype} "
                      f"{tuple(t.shape)} strides {t.stride()} on {t.device}")
 
 
-def _f32(t: torch.Tensor, shape: tuple, what: str, index: int) -> int:
-    return _checked(t, torch.float32, shape, what, index)
+# the address of a contiguous tensor of that type and shape on that device; ValueError for any other
+def _f32(t: torch.Tensor, shape: tuple, what: str, index: int, dtype=torch.float32) -> int:
+    if t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.get_device() == index:
+        return t.data_ptr()
+    return _refuse(t, dtype, shape, what, index)
 
 
-def _i32(t: torch.Tensor, shape: tuple, what: str, index: int) -> int:
-    return _checked(t, torch.int32, shape, what, index)
+def _i32(t: torch.Tensor, shape: tuple, what: str, index: int, dtype=torch.int32) -> int:
+    if t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.get_device() == index:
+        return t.data_ptr()
+    return _refuse(t, dtype, shape, what, index)
 
 
 def _current(index: int) -> int:
@@ -776,7 +778,7 @@ class PagedKV:
             qp, qs = rows(q, n_heads, "q")
             if out is None:
                 out = _empty((n, n_heads, hd), f32, self.device, stream)
-            op = _checked(out, f32, (n, n_heads, hd), "out", dev)
+            op = _f32(out, (n, n_heads, hd), "out", dev)
         kp, ks = rows(k, n_kv, "k")
         vp, vs = rows(v, n_kv, "v")
         rc = self._lib.styx_paged_append(
@@ -812,8 +814,8 @@ class PagedKV:
         n_heads = q.shape[1] if q.dim() == 3 else 0
         shape = (b, n_heads, hd)
         qp = _f32(q, shape, "q", dev)
-        if out is None:
-            out = _empty(shape, torch.float32, self.device, stream)
+        if out is None:   # (empty_like: 1.3 us of host time, empty 2.3)
+            out = torch.empty_like(q) if stream is None else _empty(shape, torch.float32, self.device, stream)
         stride, accp, accop = 0, None, None
         if acc is not None:
             stride = acc.shape[-1]
