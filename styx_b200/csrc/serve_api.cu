@@ -244,7 +244,9 @@ int styx_paged_attend(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv
     a.cnt = reinterpret_cast<unsigned *>(ws + w.cnt);
     // the tensor cores take 16-bit rows of up to 128 elements in pages of 16
     // rows or more (a warp's 16 rows then lie together); everything else runs
-    // on the FMA units
+    // on the FMA units.  Where both could (32 / 4 heads of 128): 37 rows 6.4 us
+    // against 9.7, one sequence of 131071 f16 rows 50 against 117, 32 ragged
+    // bf16 ones 34 against 75, 64 of 64 / 4 heads 125 against 448
     if (kv->dtype != STYX_F32 && kv->head_dim <= 128 && kv->page_size >= 16)
         CK(styx::launch_attend_mma(a, sms, S(stream)));
     else
