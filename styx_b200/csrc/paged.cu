@@ -186,7 +186,7 @@ struct EvictShared {
     __align__(16) unsigned hist[kEvBins];
     unsigned scan[kEvWarps], red[3][kEvWarps];
     // what a cluster's CTAs write into each other
-    unsigned lo[8], hi[8], prot[8], sum[8], bin, before, ties[8], holes[8], movers[8];
+    unsigned lo[8], hi[8], prot[8], sum[8], bin, before, in, ties[8], holes[8], movers[8];
 };
 
 // exclusive prefix over the CTA, and the total
@@ -274,6 +274,10 @@ __global__ void __launch_bounds__(kEvThreads) k_evict_select(PagedEvictArgs a, i
     for (int i = tid; i < len; i += kEvThreads) {
         const uint32_t k = evict_key(acc[first + i], pos[first + i], np, a.n_recent, a.n_sink);
         keys[i] = k;
+        if (first + i < left) {   // (a row that leaves: overwritten by the one that moves to its place)
+            a.acc_out[line + first + i] = acc[first + i];
+            a.pos_out[line + first + i] = pos[first + i];
+        }
         if (k == kProtected) {
             prot++;
         } else {
@@ -311,7 +315,8 @@ __global__ void __launch_bounds__(kEvThreads) k_evict_select(PagedEvictArgs a, i
     unsigned ties = static_cast<unsigned>(left);
     if (prot < static_cast<unsigned>(left)) {
         unsigned need = static_cast<unsigned>(left) - prot;       // of the keys in [k_lo, k_hi], the largest
-        while (k_hi > k_lo) {
+        unsigned in = static_cast<unsigned>(n) - prot;            // that many there are
+        while (k_hi > k_lo && in > need) {
             const int shift = max(0, 21 - __clz(k_hi - k_lo));    // (range >> shift) < 2048
 #pragma unroll
             for (int i = 0; i < kEvBins / 4 / kEvThreads; i++)
@@ -361,27 +366,32 @@ __global__ void __launch_bounds__(kEvThreads) k_evict_select(PagedEvictArgs a, i
                     for (int q = 0; q < C; q++) {
                         tell(&sh.bin, s0 + i, q);
                         tell(&sh.before, before, q);
+                        tell(&sh.in, c[i], q);
                     }
                 before += c[i];
             }
             all_sync();
             need -= sh.before;
+            in = sh.in;
             const uint32_t top = k_hi - (sh.bin << shift), width = (1u << shift) - 1;
             k_lo = top - k_lo > width ? top - width : k_lo;
             k_hi = top;
             __syncthreads();   // (bin and before are read before the next round writes them)
         }
-        thr = k_lo;
-        ties = need;
+        thr = in > need ? k_lo : k_lo - 1;   // (all of the range stay; no key is 0)
+        ties = in > need ? need : 0;
     }
     // ---------------- numbering, in row order: a thread's neighbouring rows (an odd number: no bank is met twice)
     const int per = ((len + kEvThreads - 1) / kEvThreads) | 1, i0 = min(len, tid * per), i1 = min(len, i0 + per);
-    unsigned n_ties = 0, tot;
-    for (int i = i0; i < i1; i++) n_ties += keys[i] == thr;
-    unsigned tie = cta_scan(n_ties, sh.scan, tot);
-    if (tid < C) tell(&sh.ties[rank], tot, tid);
-    all_sync();
-    for (int q = 0; q < rank; q++) tie += sh.ties[q];
+    unsigned tie = 0, tot;
+    if (ties > 0) {   // (the same for all CTAs of the line)
+        unsigned n_ties = 0;
+        for (int i = i0; i < i1; i++) n_ties += keys[i] == thr;
+        tie = cta_scan(n_ties, sh.scan, tot);
+        if (tid < C) tell(&sh.ties[rank], tot, tid);
+        all_sync();
+        for (int q = 0; q < rank; q++) tie += sh.ties[q];
+    }
     unsigned n_holes = 0, n_movers = 0;
     for (int i = i0; i < i1; i++) {
         const uint32_t k = keys[i];
@@ -391,10 +401,21 @@ __global__ void __launch_bounds__(kEvThreads) k_evict_select(PagedEvictArgs a, i
         n_holes += !stay && first + i < left;
         n_movers += stay && first + i >= left;
     }
-    unsigned hole = cta_scan(n_holes, sh.scan, tot);
-    if (tid < C) tell(&sh.holes[rank], tot, tid);
-    unsigned mover = cta_scan(n_movers, sh.scan, tot);
-    if (tid < C) tell(&sh.movers[rank], tot, tid);
+    unsigned hole, mover;
+    if constexpr (STAGED) {   // (fewer than 2^16 of each in a CTA)
+        const unsigned both = cta_scan(n_movers << 16 | n_holes, sh.scan, tot);
+        hole = both & 0xFFFFu;
+        mover = both >> 16;
+        if (tid < C) {
+            tell(&sh.holes[rank], tot & 0xFFFFu, tid);
+            tell(&sh.movers[rank], tot >> 16, tid);
+        }
+    } else {
+        hole = cta_scan(n_holes, sh.scan, tot);
+        if (tid < C) tell(&sh.holes[rank], tot, tid);
+        mover = cta_scan(n_movers, sh.scan, tot);
+        if (tid < C) tell(&sh.movers[rank], tot, tid);
+    }
     all_sync();
     for (int q = 0; q < rank; q++) {
         hole += sh.holes[q];
@@ -406,13 +427,6 @@ __global__ void __launch_bounds__(kEvThreads) k_evict_select(PagedEvictArgs a, i
         if (keys[i] && first + i >= left) from[mover++] = first + i;
     }
     if (tid == 0 && rank == 0) a.moves[line_no] = static_cast<int32_t>(total(sh.movers));
-    // rows that stay where they are
-#pragma unroll 4
-    for (int i = tid; i < min(len, left - first); i += kEvThreads)
-        if (keys[i]) {
-            a.acc_out[line + first + i] = acc[first + i];
-            a.pos_out[line + first + i] = pos[first + i];
-        }
     if (C > 1) all_sync();   // no CTA leaves while another reads its counts
 }
 
