@@ -690,6 +690,19 @@ def _i32(t: torch.Tensor, shape: tuple, what: str, index: int, dtype=torch.int32
     return _refuse(t, dtype, shape, what, index)
 
 
+def _token_rows(t: torch.Tensor, n: int, heads: int, hd: int, what: str, index: int, dtype=torch.float32) -> tuple:
+    """(address, floats between tokens) of f32 [n][heads][hd] whose heads are contiguous."""
+    shape = (n, heads, hd)
+    if t.dtype is dtype and t.shape == shape and t.get_device() == index:
+        if t.is_contiguous():
+            return t.data_ptr(), heads * hd
+        sn, sh, se = t.stride()
+        if se == 1 and (sh == hd or heads == 1):
+            return t.data_ptr(), sn if n > 1 else heads * hd
+    raise ValueError(f"{what}: float32 [{n}][{heads}][{hd}] with contiguous heads on cuda:{index} expected, got "
+                     f"{t.dtype} {tuple(t.shape)} strides {t.stride()} on {t.device}")
+
+
 def _current(index: int) -> int:
     return torch.cuda.current_stream(index).cuda_stream
 
@@ -733,6 +746,7 @@ class PagedKV:
         self.ctx = ctx(self.index)
         self.n_seqs, self.n_kv_heads, self.head_dim = table.shape[0], n_kv, hd
         self.max_rows = table.shape[1] * page
+        self._scale = hd ** -0.5
         self._kv = _lib.PagedKv(k.data_ptr(), v.data_ptr(), k.stride(0) if n_pages > 1 else n_kv * page * hd,
                                 table.data_ptr(), None, _KV_TYPES[k.dtype], n_pages, page, n_kv, hd, self.n_seqs,
                                 table.shape[1], table.stride(0) if self.n_seqs > 1 else table.shape[1])
@@ -763,24 +777,14 @@ class PagedKV:
         of one projection's output (any stride between tokens)."""
         dev, hd, n_kv = self.index, self.head_dim, self.n_kv_heads
         n, n_heads = pos.shape[0], 0 if q is None else q.shape[1]
-        f32 = torch.float32
-
-        def rows(t, heads, what):
-            sn, sh, se = t.stride()
-            if t.dtype is f32 and t.shape == (n, heads, hd) and se == 1 and (sh == hd or heads == 1) and \
-                    t.get_device() == dev:
-                return t.data_ptr(), sn if n > 1 else heads * hd
-            raise ValueError(f"{what}: float32 [{n}][{heads}][{hd}] with contiguous heads on cuda:{dev} expected, got "
-                             f"{t.dtype} {tuple(t.shape)} strides {t.stride()} on {t.device}")
-
         qp, qs, op = None, 0, None
         if q is not None:
-            qp, qs = rows(q, n_heads, "q")
+            qp, qs = _token_rows(q, n, n_heads, hd, "q", dev)
             if out is None:
-                out = _empty((n, n_heads, hd), f32, self.device, stream)
+                out = _empty((n, n_heads, hd), torch.float32, self.device, stream)
             op = _f32(out, (n, n_heads, hd), "out", dev)
-        kp, ks = rows(k, n_kv, "k")
-        vp, vs = rows(v, n_kv, "v")
+        kp, ks = _token_rows(k, n, n_kv, hd, "k", dev)
+        vp, vs = _token_rows(v, n, n_kv, hd, "v", dev)
         rc = self._lib.styx_paged_append(
             self.ctx.handle, _current(dev) if stream is None else stream.cuda_stream, self._ref, n, n_heads, qp, qs,
             kp, ks, vp, vs, None if q_norm is None else _f32(q_norm, (hd,), "q_norm", dev),
@@ -810,12 +814,15 @@ class PagedKV:
         the softmax denominators; with acc f32 [n_seqs][n_kv_heads][>= rows],
         acc_out (None: acc itself) receives it plus each row's weight summed
         over the kv head's q heads."""
-        dev, b, hd = self.index, self.n_seqs, self.head_dim
+        dev, b = self.index, self.n_seqs
         n_heads = q.shape[1] if q.dim() == 3 else 0
-        shape = (b, n_heads, hd)
+        shape = (b, n_heads, self.head_dim)
         qp = _f32(q, shape, "q", dev)
         if out is None:   # (empty_like: 1.3 us of host time, empty 2.3)
             out = torch.empty_like(q) if stream is None else _empty(shape, torch.float32, self.device, stream)
+            outp = out.data_ptr()
+        else:
+            outp = _f32(out, shape, "out", dev)
         stride, accp, accop = 0, None, None
         if acc is not None:
             stride = acc.shape[-1]
@@ -827,7 +834,7 @@ class PagedKV:
         ws = self._attend_ws.get((n_heads, accp is not None)) or self._attend_workspace(n_heads, accp is not None, stream)
         rc = self._lib.styx_paged_attend(
             self.ctx.handle, _current(dev) if stream is None else stream.cuda_stream, self._ref, n_heads, qp,
-            hd ** -0.5 if scale is None else scale, window, _f32(out, shape, "out", dev),
+            self._scale if scale is None else scale, window, outp,
             None if lse is None else _f32(lse, (b, n_heads), "lse", dev), accp, accop, stride, ws[1], ws[2])
         if rc:
             check(rc)
