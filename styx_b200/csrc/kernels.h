@@ -393,16 +393,17 @@ struct PagedAttendArgs {
     long long acc_stride;
     float scale;
     int window, n_heads, gqa;
-    int ctas;                      // of the launch: portions are theirs
+    int workers;                   // of the launch: portions are theirs
+    int part_floats;               // of a portion's result
     int tile_shift, seg_cost;      // see paged_split.cuh; the kernel's
     // workspace (with acc_out): scores in units of log2, [n_seqs][n_kv][max
     // rows][gqa]; maximum and sum of every head, [n_seqs][n_heads][2]
     float *scores, *ml;
-    float *part;                   // workspace: the portions' partial results, kAttendPart floats each
-    unsigned *cnt;                 // workspace, per (sequence, kv head, group): first CTA << 16 | portions (0: not cut)
+    float *part;                   // workspace: the portions' partial results, part_floats each
+    unsigned *cnt;                 // workspace, per (sequence, kv head, group): first worker << 16 | portions (0: not cut)
 };
-// a portion of up to 16 heads of up to 128 elements, or 8 of 256: O, 16 maxima, 16 sums
-constexpr int kAttendPart = 16 * 128 + 32;
+// floats of a portion's result: O [heads][pitch], 16 maxima, 16 sums
+constexpr int attend_part(int heads, int pitch) { return heads * pitch + 32; }
 struct PagedEvictArgs {
     PagedKv kv;
     const float *acc;
@@ -430,11 +431,13 @@ struct SampleArgs {
 cudaError_t launch_paged_append(const PagedAppendArgs &a, int sms, cudaStream_t st);
 // attention on the FMA units, on the tensor cores; and what ends both:
 // portions of nh heads, pitch floats each, joined, and the weights
-// accumulated (a.ctas set)
+// accumulated (a.workers and a.part_floats set)
 cudaError_t launch_attend_fma(PagedAttendArgs a, int sms, cudaStream_t st);
-cudaError_t launch_attend_mma(PagedAttendArgs a, int sms, cudaStream_t st);
+cudaError_t launch_attend_mma(const PagedAttendArgs &a, int sms, cudaStream_t st);
 cudaError_t launch_attend_finish(const PagedAttendArgs &a, int nh, int pitch, cudaStream_t st);
 int attend_grid(const PagedAttendArgs &a, int nh, int sms);
+uint64_t attend_fma_parts(int sms);            // bytes of the portions' results
+uint64_t attend_mma_parts(int gqa, int sms);
 cudaError_t launch_paged_evict(const PagedEvictArgs &a, int sms, cudaStream_t st);
 bool evict_staged(long long rows);   // the keys of lines of so many rows fit shared memory
 cudaError_t launch_sample(const SampleArgs &a, cudaStream_t st);

@@ -96,7 +96,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_fma(PagedAttendArgs a) {
     pdl_wait();
     long long T_, G;
     Walk wk;
-    share_of(a, segs, wk, T_, G);
+    share_of(a, segs, blockIdx.x, wk, T_, G);
     // the head whose sum the halving exchanges leave in this lane: from the lane bits LPR/2, LPR/4, LPR/8
     const int myh = ((rl & (LPR / 2)) ? 4 : 0) | ((rl & (LPR / 4)) ? 2 : 0) | ((rl & (LPR / 8)) ? 1 : 0);
     const uint32_t mine = smem_addr(ring) + tid * 16;
@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_fma(PagedAttendArgs a) {
         }
         __syncthreads();
         const bool whole = wk.t0 == 0 && wk.t1 == wk.nt;
-        if (wk.t1 == wk.nt && tid == 0) a.cnt[static_cast<long long>(wk.b) * segs + wk.seg] = cut_of(wk, T_, G);
+        if (wk.t1 == wk.nt && tid == 0) a.cnt[static_cast<long long>(wk.b) * segs + wk.seg] = cut_of(wk, blockIdx.x, T_, G);
         float *part = part_at(a, blockIdx.x, wk.t0 == 0);
         for (int i = tid; i < ng * hd; i += kThreads) {
             const int h = i / hd, c = i - h * hd;
@@ -303,8 +303,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_fma(PagedAttendArgs a) {
         if (tid < ng) {
             const float M = s_M[tid], L = s_L[tid];
             if (!whole) {
-                part[kAttendPart - 32 + tid] = M;
-                part[kAttendPart - 16 + tid] = L;
+                part[a.part_floats - 32 + tid] = M;
+                part[a.part_floats - 16 + tid] = L;
             } else {
                 if (a.lse) a.lse[h0 + tid] = L > 0.f ? M * 0.6931471805599453f + logf(L) : -INFINITY;
                 if (a.acc_out) {
@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(256) k_attend_finish(PagedAttendArgs a, int jo
         const unsigned c = ld_cg(a.cnt + at);
         const int np = static_cast<int>(c & 0xFFFFu);
         if (np == 0) return;
-        if (static_cast<int>(c >> 16) + np > a.ctas) {   // (lengths that changed during the call)
+        if (static_cast<int>(c >> 16) + np > a.workers) {   // (lengths that changed during the call)
             if (threadIdx.x == 0) atomicExch(kv.err, kErrBadPos);
             return;
         }
@@ -358,8 +358,8 @@ __global__ void __launch_bounds__(256) k_attend_finish(PagedAttendArgs a, int jo
                 for (int i = 0; i < 8; i++) {
                     const int k = i0 + i * WPH, p = min(k, np - 1);
                     const float *pp = part_at(a, own0 + p, p == 0);
-                    m[i] = ld_cg(pp + kAttendPart - 32 + h);
-                    l[i] = ld_cg(pp + kAttendPart - 16 + h);
+                    m[i] = ld_cg(pp + a.part_floats - 32 + h);
+                    l[i] = ld_cg(pp + a.part_floats - 16 + h);
 #pragma unroll
                     for (int v = 0; v < NV; v++) x[i][v] = ld_cg(reinterpret_cast<const float4 *>(pp + h * 128 * NV) + v * 32 + lane);
                 }
@@ -438,7 +438,7 @@ __global__ void __launch_bounds__(256) k_attend_finish(PagedAttendArgs a, int jo
             for (int g = warp; g < gn; g += 8) {
                 const int h = gc + g, seg = j * groups + h / NHG, hh = h % NHG;
                 const unsigned c = ld_cg(a.cnt + static_cast<long long>(b) * segs + seg);
-                const int own0 = static_cast<int>(c >> 16), np = min(static_cast<int>(c & 0xFFFFu), a.ctas - own0);
+                const int own0 = static_cast<int>(c >> 16), np = min(static_cast<int>(c & 0xFFFFu), a.workers - own0);
                 float M = kNone, L = 0.f;
                 if (np == 0) {
                     const float *ml = a.ml + 2 * (static_cast<long long>(b) * a.n_heads + j * a.gqa + h);
@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(256) k_attend_finish(PagedAttendArgs a, int jo
                 } else {
                     for (int i = lane; i < np; i += 32) {
                         const float *pp = part_at(a, own0 + i, i == 0);
-                        const float m = ld_cg(pp + kAttendPart - 32 + hh), l = ld_cg(pp + kAttendPart - 16 + hh);
+                        const float m = ld_cg(pp + a.part_floats - 32 + hh), l = ld_cg(pp + a.part_floats - 16 + hh);
                         const float top = fmaxf(M, m);
                         L = L * ex2(M - top) + l * ex2(m - top);
                         M = top;
@@ -531,10 +531,13 @@ cudaError_t launch_attend_finish(const PagedAttendArgs &a, int nh, int pitch, cu
     return nh == 8 ? finish<8, 1>(a, st) : finish<16, 1>(a, st);
 }
 
+uint64_t attend_fma_parts(int sms) { return 2ull * sms * attend_part(NH, kPitch) * 4; }
+
 cudaError_t launch_attend_fma(PagedAttendArgs a, int sms, cudaStream_t st) {
     a.tile_shift = a.kv.hd <= 64 ? 6 : 5;   // the rows that a CTA takes at once (head_dim above 128: twice those)
     a.seg_cost = 3;
-    const int grid = a.ctas = attend_grid(a, NH, sms);
+    a.part_floats = attend_part(NH, kPitch);
+    const int grid = a.workers = attend_grid(a, NH, sms);
     const cudaError_t e = a.kv.dtype == STYX_F16    ? launch_t<__half>(a, grid, st)
                           : a.kv.dtype == STYX_BF16 ? launch_t<__nv_bfloat16>(a, grid, st)
                                                     : launch_t<float>(a, grid, st);

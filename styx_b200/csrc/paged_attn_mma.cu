@@ -18,21 +18,24 @@
 // A warp takes 16 rows at a time for itself; with more than eight q heads per
 // kv head, two warps share them, eight heads each.  Copies (cp.async, 4 KB of
 // K or V, contiguous in the page) go round a ring of the team's own, so that
-// nobody else waits between a portion's ends and 160 KB per SM are in flight.
-// The maximum that a row is measured against moves only when a score passes
-// it by 2^8.  The next portion's first copies, its q ahead of them and its pages
-// looked up together, are issued before the last one's result is joined from
-// the eight warps.
+// nobody else waits and 160 KB per SM are in flight.  The maximum that a row
+// is measured against moves only when a score passes it by 2^8.  Each team
+// has a share of the tile list and writes a cut segment's part from its
+// registers; with few segments the CTA's teams take one share's tiles in turn
+// and join in shared memory, so that a segment has an eighth of the parts.
+// The next portion's first copies, its q ahead of them and its pages looked
+// up together, are issued before the last one's result is written.
 //
 // Measured (B200): one sequence of 131071 f16 rows, 32 / 4 heads of 128, 268 MB
 // in 50 us (5.3 TB/s; DRAM 66 % busy, tensor pipe 19 %, issue 33 %); twice as
 // many rows 5.7 to 5.9 TB/s, what cp.async reaches here.  Bound by HBM with up
-// to eight heads per kv head.  With 16 (bf16, 64 ragged sequences, 549 MB) 125
-// us, bound by the MMAs' and exchanges' latency at eight warps: twelve warps
-// took 130, sixteen (whose registers spill) 151; one warp with all 16 heads
-// 175; a branch around each MMA step (head_dim as a variable) 145.  32 ragged
-// bf16 sequences of up to 4096 rows, 139 MB, 33.6 us: the launch, the share
-// and the first rows cost 4 us, a portion's end 2 us.
+// to eight heads per kv head.  With 16 (bf16, 64 ragged sequences, 549 MB) 113
+// us, bound by the latency of eight warps' MMAs and exchanges: as CTAs with
+// one share 125, then twelve warps 130, sixteen (whose registers spill) 151;
+// one warp with all 16 heads 175; a branch around each MMA step (head_dim as a
+// variable) 145; chains of MMAs half as long change nothing.  32 ragged bf16
+// sequences of up to 4096 rows, 139 MB, 33.5 us: launch, share and first rows
+// cost 4 us, a portion's end 2 us, the finish 3.
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -47,9 +50,11 @@ constexpr int kRows = 16;                      // rows of a tile
 constexpr int kUnit = kRows * 256;             // K or V of them, 256-byte rows (head_dim 128)
 constexpr int kUnits = 48;                     // of all rings
 constexpr int kRing = kUnits * kUnit;
-constexpr int kPad = 132;                      // floats of a head's O in the join: no two heads on one bank
-constexpr int kJoin = kWarps * 4 * kPad * 4;   // four heads of every warp
+constexpr int kPad = 132;                      // floats of a head's q in shared memory: no two heads on one bank
 constexpr int kQ = 8 * kPad * 4;               // q of eight heads
+constexpr int kJoin = kWarps * 4 * kPad * 4;   // JOINT: four heads' results of every warp
+constexpr int kRest = kWarps * kQ;             // beside the rings: q of every warp; JOINT: q, two buffers, and the join's
+static_assert(kRest >= 2 * 2 * kQ + kJoin, "JOINT fits");
 constexpr float kSlack = 8.f;                  // log2 units a score may pass the maximum by
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool on) {   // off: zeros
@@ -108,9 +113,9 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t (&t)[BF ? 3 : 
     }
 }
 
-// a portion of the CTA's share: its rows [lo, hi) of one segment, tile i of
-// team t from row base + (i teams + t) 16 on (base: lo rounded down to 16)
-template <int TEAMS>
+// a portion of the worker's share: its rows [lo, hi) of one segment, from base
+// (lo rounded down to 16) on STEP rows at a time
+template <int STEP>
 struct Part {
     int b, j, g0, ng, lo, hi, base, iters;
     long long h0;
@@ -126,17 +131,19 @@ struct Part {
         lo = max(s.first, (s.tile0 + wk.t0) << a.tile_shift);
         hi = static_cast<int>(min(static_cast<long long>(s.n), static_cast<long long>(s.tile0 + wk.t1) << a.tile_shift));
         base = lo & ~(kRows - 1);
-        iters = hi > lo ? (hi - base + kRows * TEAMS - 1) / (kRows * TEAMS) : 0;
+        iters = hi > lo ? (hi - base + STEP - 1) / STEP : 0;
     }
 };
 
+// JOINT: the CTA's teams take the tiles of one share in turn and join their
+// results at a portion's end; else each team has a share of its own.
 // TEAM: warps that share a tile, eight q heads each; KS: 16-element steps of a
 // row (what head_dim leaves of them is zeros)
-template <bool BF, int TEAM, int KS>
+template <bool BF, int TEAM, int KS, bool JOINT>
 __global__ void __launch_bounds__(kThreads, 1) k_attend_mma(PagedAttendArgs a) {
-    constexpr int TERMS = BF ? 3 : 2, NH = 8 * TEAM, TEAMS = kWarps / TEAM, S = kUnits / TEAMS;
+    constexpr int TERMS = BF ? 3 : 2, NH = 8 * TEAM, TEAMS = kWarps / TEAM, S = kUnits / TEAMS, STEP = JOINT ? kRows * TEAMS : kRows;
+    __shared__ float s_m[JOINT ? kWarps : 1][8], s_l[JOINT ? kWarps : 1][8], s_L[NH];
     extern __shared__ __align__(256) uint8_t smem[];   // (rows are swizzled by xor of address bits 4 to 7)
-    __shared__ float s_m[kWarps][8], s_l[kWarps][8], s_M[NH], s_L[NH];
     const PagedKv &kv = a.kv;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hd = kv.hd;
     const int team = warp / TEAM, in = warp % TEAM;   // in: which eight heads
@@ -146,16 +153,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_mma(PagedAttendArgs a) {
     Walk wk;
     pdl_trigger();
     pdl_wait();
-    share_of(a, segs, wk, T, G);
+    // (neighbouring shares on different SMs: few tiles spread over all of them)
+    const int worker = JOINT ? blockIdx.x : team * gridDim.x + blockIdx.x;
+    share_of(a, segs, worker, wk, T, G);
     const uint32_t ring = smem_addr(smem) + team * S * kUnit;
-    float *so = reinterpret_cast<float *>(smem + kRing);
+    uint8_t *const rest = smem + kRing;
+    float *sq = reinterpret_cast<float *>(rest + (JOINT ? 0 : warp * kQ));   // the portion's q, the CTA's or the warp's heads
+    float *so = reinterpret_cast<float *>(rest + 4 * kQ);                    // JOINT: the join's buffer
     const float l2 = a.scale * 1.4426950408889634f;   // scores in units of log2
     auto team_sync = [&] {
         if constexpr (TEAM == 1) __syncwarp();
         else asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(32 * TEAM) : "memory");
     };
 
-    Part<TEAMS> P{};
+    Part<STEP> P{};
+    const int mine = JOINT ? team * kRows : 0;   // the team's rows of a step
     // ---------------- the ring: units K(0), V(0), K(1), ... of the team's tiles
     const bool col = (lane & 15) < hd / 8;
     // the lane's copies of a unit: rows at_row + 2 TEAM i, swizzled chunk lane % 16
@@ -164,14 +176,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_mma(PagedAttendArgs a) {
     int slot = 0;                     // of the next unit to be used
     unsigned seen = 0;                // bit s: slot s holds a tile of which rows are seen
     int kpage = -1, vpage = -1;       // the page of the next K, V to be copied; -1: none
-    float *sq = reinterpret_cast<float *>(smem + kRing + kJoin);   // the portion's q; two buffers in turn
     auto page_of = [&](int it) {
-        const int r = P.base + (it * TEAMS + team) * kRows;
+        const int r = P.base + it * STEP + mine;
         return it < P.iters && r < P.hi ? ld_now(P.table + (r >> kv.page_shift)) : -1;
     };
     // copies of K or V of tile `it` in a page into slot s; rows outside [lo, hi) are zeros, a page outside the pool is reported
     auto issue = [&](bool is_v, int it, int s, int page) {
-        const int r0 = P.base + (it * TEAMS + team) * kRows;
+        const int r0 = P.base + it * STEP + mine;
         const bool some = it < P.iters && r0 < P.hi, ok = some && static_cast<unsigned>(page) < static_cast<unsigned>(kv.n_pages);
         if (some && !ok && lane == 0) atomicExch(kv.err, kErrBadPos);
         if (ok) {
@@ -188,16 +199,23 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_mma(PagedAttendArgs a) {
     };
     auto start = [&] {                // a portion's first copies: q, then S - 1 units
         P.set(a, wk, groups, NH);
-        sq = reinterpret_cast<float *>(smem + kRing + kJoin + (reinterpret_cast<uint8_t *>(sq) == smem + kRing + kJoin ? TEAM * kQ : 0));
         int pages[S / 2];
 #pragma unroll
         for (int i = 0; i < S / 2; i++) pages[i] = page_of(i);
         kpage = page_of(S / 2);
         vpage = pages[S / 2 - 1];
         const int per = hd / 4;
-        for (int i = tid; i < P.ng * per; i += kThreads) {
-            const int h = i / per, c = i - h * per;
-            copy16(smem_addr(sq + h * kPad + 4 * c), a.q + (P.h0 + h) * hd + 4 * c, true);
+        if constexpr (JOINT) {
+            sq = reinterpret_cast<float *>(rest + (reinterpret_cast<uint8_t *>(sq) == rest ? 2 * kQ : 0));
+            for (int i = tid; i < P.ng * per; i += kThreads) {
+                const int h = i / per, c = i - h * per;
+                copy16(smem_addr(sq + h * kPad + 4 * c), a.q + (P.h0 + h) * hd + 4 * c, true);
+            }
+        } else {
+            for (int i = lane; i < min(8, P.ng - 8 * in) * per; i += 32) {
+                const int h = i / per, c = i - h * per;
+                copy16(smem_addr(sq + h * kPad + 4 * c), a.q + (P.h0 + 8 * in + h) * hd + 4 * c, true);
+            }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
         int s = slot;
@@ -230,14 +248,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_mma(PagedAttendArgs a) {
     if (have) start();
     while (have) {
         asm volatile("cp.async.wait_group %0;" ::"n"(S - 1) : "memory");
-        __syncthreads();              // q is there; the last join's buffers are free again
+        // q is there; the last join's buffers are free again
+        if constexpr (JOINT) __syncthreads();
+        else __syncwarp();
         // ---------------- q as B fragments, in terms.  f16 has few exponents: a head's largest |q| is brought to
         // [2^9, 2^10), and fh says what its column of S is in units of its terms
         uint32_t qf[KS][TERMS][2];
         float fh[2];
         {
             const int h = 8 * in + lr;
-            const float *q = sq + h * kPad + 2 * lc;
+            const float *q = sq + (JOINT ? h : lr) * kPad + 2 * lc;
             float2 v[KS][2];
             float mx = 0.f;
 #pragma unroll
@@ -279,7 +299,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_mma(PagedAttendArgs a) {
         float *scores = a.scores + (static_cast<long long>(P.b) * kv.n_kv + P.j) *
                                        (static_cast<long long>(kv.max_pages) << kv.page_shift) * a.gqa + P.g0 + hh;
         for (int it = 0; it < P.iters; it++) {
-            const int r0 = P.base + (it * TEAMS + team) * kRows + lr;   // the lane's rows: r0, r0 + 8
+            const int r0 = P.base + it * STEP + mine + lr;   // the lane's rows: r0, r0 + 8
             const int kslot = advance(false, it);
             const bool live = (seen >> kslot) & 1;
             const bool in0 = r0 >= P.lo && r0 < P.hi, in1 = r0 + 8 >= P.lo && r0 + 8 < P.hi;
@@ -366,100 +386,132 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_mma(PagedAttendArgs a) {
                 }
             }
         }
-        // ---------------- the portion's end: the next one's first copies, then the warps' results joined
+        // ---------------- the portion's end: the next one's first copies, then the result
         const int ng = P.ng;
         const long long h0 = P.h0;
         const bool first = wk.t0 == 0, whole = first && wk.t1 == wk.nt;
-        if (wk.t1 == wk.nt && tid == 0) a.cnt[static_cast<long long>(wk.b) * segs + wk.seg] = cut_of(wk, T, G);
+        if (wk.t1 == wk.nt && (JOINT ? tid == 0 : in == 0 && lane == 0)) a.cnt[static_cast<long long>(wk.b) * segs + wk.seg] = cut_of(wk, worker, T, G);
         have = wk.next(a, segs);
         team_sync();
         if (have) start();
+        float *part = part_at(a, worker, first);
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-            float v = l[e];
-            v += __shfl_xor_sync(0xffffffffu, v, 4);
-            v += __shfl_xor_sync(0xffffffffu, v, 8);
-            v += __shfl_xor_sync(0xffffffffu, v, 16);
-            if (lr == 0) {
-                s_m[warp][2 * lc + e] = m[e];
-                s_l[warp][2 * lc + e] = v;
-            }
+            l[e] += __shfl_xor_sync(0xffffffffu, l[e], 4);
+            l[e] += __shfl_xor_sync(0xffffffffu, l[e], 8);
+            l[e] += __shfl_xor_sync(0xffffffffu, l[e], 16);
         }
-        float *part = part_at(a, blockIdx.x, first);
+        auto put_sums = [&](int h, float M, float L) {
+            if (!whole) {
+                part[a.part_floats - 32 + h] = M;
+                part[a.part_floats - 16 + h] = L;
+                return;
+            }
+            if (a.lse) a.lse[h0 + h] = L > 0.f ? M * 0.6931471805599453f + logf(L) : -INFINITY;
+            if (a.acc_out) {
+                a.ml[2 * (h0 + h)] = M;
+                a.ml[2 * (h0 + h) + 1] = L;
+            }
+        };
+        constexpr float kUp = BF ? 1.f : 0x1p-7f;   // (f16: p was carried times 2^7)
+        if constexpr (!JOINT) {
 #pragma unroll
-        for (int n = 0; n < 2; n++) {          // four heads of every warp at a time
-            if (lc >> 1 == n)
+            for (int e = 0; e < 2; e++) {
+                const int h = hh + e;
+                if (h >= ng) continue;
+                const float r = (whole ? (l[e] > 0.f ? 1.f / l[e] : 0.f) : 1.f) * kUp;
+                float *to = whole ? a.out + (h0 + h) * hd : part + h * 128;
 #pragma unroll
                 for (int t = 0; t < KS; t++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        so[(warp * 4 + 2 * (lc & 1) + (i & 1)) * kPad + 16 * t + lr + 8 * (i >> 1)] =
-                            BF ? o[t][i] : o[t][i] * 0x1p-7f;
-            __syncthreads();
-            if (n == 0) {
-                if (tid < NH) {
-                    float M = kNone, L = 0.f;
-                    for (int w = 0; w < TEAMS; w++) M = fmaxf(M, s_m[w * TEAM + tid / 8][tid & 7]);
-                    for (int w = 0; w < TEAMS; w++) {
-                        float &mw = s_m[w * TEAM + tid / 8][tid & 7];
-                        mw = ex2(mw - M);
-                        L += s_l[w * TEAM + tid / 8][tid & 7] * mw;
+                    for (int i = 0; i < 2; i++) {
+                        const int c = 16 * t + 8 * i + lr;
+                        if (c < hd) to[c] = o[t][2 * i + e] * r;
                     }
-                    s_M[tid] = M;
-                    s_L[tid] = L;
-                }
-                __syncthreads();
+                if (lr == 0) put_sums(h, m[e], l[e]);
             }
-            for (int i = tid; i < 4 * TEAM * hd; i += kThreads) {
-                const int g = i / hd, c = i - g * hd, e = g / 4, h4 = g & 3, h = 8 * e + 4 * n + h4;
-                if (h >= ng) continue;
-                float v = 0.f;
+        } else {
+            if (lr == 0)
 #pragma unroll
-                for (int w = 0; w < TEAMS; w++) v += so[((w * TEAM + e) * 4 + h4) * kPad + c] * s_m[w * TEAM + e][4 * n + h4];
-                if (whole) a.out[(h0 + h) * hd + c] = s_L[h] > 0.f ? v / s_L[h] : 0.f;
-                else part[h * 128 + c] = v;
-            }
-            if (n == 0) __syncthreads();
-        }
-        if (tid < ng) {
-            const float M = s_M[tid], L = s_L[tid];
-            if (!whole) {
-                part[kAttendPart - 32 + tid] = M;
-                part[kAttendPart - 16 + tid] = L;
-            } else {
-                if (a.lse) a.lse[h0 + tid] = L > 0.f ? M * 0.6931471805599453f + logf(L) : -INFINITY;
-                if (a.acc_out) {
-                    a.ml[2 * (h0 + tid)] = M;
-                    a.ml[2 * (h0 + tid) + 1] = L;
+                for (int e = 0; e < 2; e++) {
+                    s_m[warp][2 * lc + e] = m[e];
+                    s_l[warp][2 * lc + e] = l[e];
                 }
+#pragma unroll
+            for (int n = 0; n < 2; n++) {          // four heads of every warp at a time
+                if (lc >> 1 == n)
+#pragma unroll
+                    for (int t = 0; t < KS; t++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            so[(warp * 4 + 2 * (lc & 1) + (i & 1)) * kPad + 16 * t + lr + 8 * (i >> 1)] = o[t][i] * kUp;
+                __syncthreads();
+                if (n == 0) {
+                    if (tid < NH) {
+                        float M = kNone, L = 0.f;
+                        for (int w = 0; w < TEAMS; w++) M = fmaxf(M, s_m[w * TEAM + tid / 8][tid & 7]);
+                        for (int w = 0; w < TEAMS; w++) {
+                            float &mw = s_m[w * TEAM + tid / 8][tid & 7];
+                            mw = ex2(mw - M);
+                            L += s_l[w * TEAM + tid / 8][tid & 7] * mw;
+                        }
+                        s_L[tid] = L;
+                        if (tid < ng) put_sums(tid, M, L);
+                    }
+                    __syncthreads();
+                }
+                for (int i = tid; i < 4 * TEAM * hd; i += kThreads) {
+                    const int g = i / hd, c = i - g * hd, e = g / 4, h4 = g & 3, h = 8 * e + 4 * n + h4;
+                    if (h >= ng) continue;
+                    float v = 0.f;
+#pragma unroll
+                    for (int w = 0; w < TEAMS; w++) v += so[((w * TEAM + e) * 4 + h4) * kPad + c] * s_m[w * TEAM + e][4 * n + h4];
+                    if (whole) a.out[(h0 + h) * hd + c] = s_L[h] > 0.f ? v / s_L[h] : 0.f;
+                    else part[h * 128 + c] = v;
+                }
+                if (n == 0) __syncthreads();
             }
         }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-template <bool BF, int TEAM, int KS>
-cudaError_t launch(const PagedAttendArgs &a, cudaStream_t st) {
-    constexpr int smem = kRing + kJoin + TEAM * 2 * kQ;
-    const cudaError_t e = allow_smem<k_attend_mma<BF, TEAM, KS>>(smem);
+template <bool BF, int TEAM, int KS, bool JOINT>
+cudaError_t launch(PagedAttendArgs a, int sms, cudaStream_t st) {
+    constexpr int smem = kRing + kRest;
+    const cudaError_t e = allow_smem<k_attend_mma<BF, TEAM, KS, JOINT>>(smem);
     if (e != cudaSuccess) return e;
-    const cudaError_t e2 = launch_pdl(k_attend_mma<BF, TEAM, KS>, dim3(a.ctas), dim3(kThreads), smem, st, a);
+    // (a segment of up to 128 rows whole: it needs no join, the call no second kernel)
+    a.tile_shift = JOINT || static_cast<long long>(a.kv.max_pages) << a.kv.page_shift <= 128 ? 7 : 4;
+    a.seg_cost = JOINT ? 3 : 4;
+    a.part_floats = attend_part(8 * TEAM, 128);
+    const int ctas = attend_grid(a, 8 * TEAM, sms);
+    a.workers = JOINT ? ctas : ctas * (kWarps / TEAM);
+    const cudaError_t e2 = launch_pdl(k_attend_mma<BF, TEAM, KS, JOINT>, dim3(ctas), dim3(kThreads), smem, st, a);
     return e2 != cudaSuccess ? e2 : launch_attend_finish(a, 8 * TEAM, 128, st);
 }
-template <bool BF>
-cudaError_t launch_t(const PagedAttendArgs &a, int team, cudaStream_t st) {
-    if (a.kv.hd <= 64) return team == 1 ? launch<BF, 1, 4>(a, st) : launch<BF, 2, 4>(a, st);
-    return team == 1 ? launch<BF, 1, 8>(a, st) : launch<BF, 2, 8>(a, st);
+template <bool BF, int TEAM>
+cudaError_t launch_t(const PagedAttendArgs &a, int sms, cudaStream_t st) {
+    // Segments no more than SMs: a CTA's warps together on one of them (one sequence of 131071 rows 50 us, each warp
+    // for itself 68, whose 296 results per segment take long to join; 32 ragged ones 33.5 against 35).  More: each team
+    // for itself, so that a segment's start and end stop nobody else (64 sequences of up to 512 rows 15 us against 19,
+    // 128 of up to 1024 with 8 kv heads 57 against 63, 64 of up to 8192 with 64 / 4 heads 114 against 125; of up to
+    // 2048 with 32 / 4 heads 37 against 35).
+    const long long segs = static_cast<long long>(a.kv.n_seqs) * a.kv.n_kv * ((a.gqa + 8 * TEAM - 1) / (8 * TEAM));
+    if (a.kv.hd <= 64) return segs <= sms ? launch<BF, TEAM, 4, true>(a, sms, st) : launch<BF, TEAM, 4, false>(a, sms, st);
+    return segs <= sms ? launch<BF, TEAM, 8, true>(a, sms, st) : launch<BF, TEAM, 8, false>(a, sms, st);
 }
 
 }  // namespace
 
-cudaError_t launch_attend_mma(PagedAttendArgs a, int sms, cudaStream_t st) {
-    const int team = a.gqa <= 8 ? 1 : 2;
-    a.tile_shift = 7;
-    a.seg_cost = 3;
-    a.ctas = attend_grid(a, 8 * team, sms);
-    return a.kv.dtype == STYX_BF16 ? launch_t<true>(a, team, st) : launch_t<false>(a, team, st);
+uint64_t attend_mma_parts(int gqa, int sms) {
+    const int team = gqa <= 8 ? 1 : 2;
+    return 2ull * sms * (kWarps / team) * attend_part(8 * team, 128) * 4;
+}
+
+cudaError_t launch_attend_mma(const PagedAttendArgs &a, int sms, cudaStream_t st) {
+    if (a.kv.dtype == STYX_BF16) return a.gqa <= 8 ? launch_t<true, 1>(a, sms, st) : launch_t<true, 2>(a, sms, st);
+    return a.gqa <= 8 ? launch_t<false, 1>(a, sms, st) : launch_t<false, 2>(a, sms, st);
 }
 
 }  // namespace styx

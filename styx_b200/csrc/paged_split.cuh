@@ -1,8 +1,8 @@
 // paged_split.cuh -- how the paged attention kernels cut their work: tiles of
 // 2^tile_shift rows of one (sequence, kv head, group of q heads), all tiles of
-// a call in one list, an equal share of it to every CTA.  What a segment's
-// start costs a CTA (q, the first maxima, the result) counts as seg_cost
-// tiles, so that CTAs with many short segments get fewer of them.
+// a call in one list, an equal share of it to every worker (a CTA, or a team of
+// warps).  What a segment's start costs it (q, the first maxima, the result)
+// counts as seg_cost tiles, so that those with many short segments get fewer.
 #pragma once
 
 #include "paged.cuh"
@@ -30,7 +30,7 @@ struct Seq {
     }
 };
 
-// the CTA's share of the list, portion by portion.  A segment is seg_cost
+// a worker's share of the list, portion by portion.  A segment is seg_cost
 // empty units, then its tiles.
 struct Walk {
     int b, seg, u, nt;             // sequence, (kv head, group) in it, next unit of seg_cost + nt
@@ -67,10 +67,10 @@ __device__ __forceinline__ long long mul_div(long long x, long long y, long long
     return p >> 32 ? static_cast<long long>(p / d) : static_cast<long long>(static_cast<unsigned>(p) / static_cast<unsigned>(d));
 }
 
-// A CTA's share: the units of all sequences, T, and the first of CTA i's
+// A worker's share: the units of all sequences, T, and the first of worker i's
 // (floor(i T / G)) as (sequence, head, unit).  Every warp finds it for itself,
 // a run of sequences per lane: with the CTA's barriers it was twice as long.
-__device__ __forceinline__ void share_of(const PagedAttendArgs &a, int segs, Walk &w, long long &T, long long &G) {
+__device__ __forceinline__ void share_of(const PagedAttendArgs &a, int segs, int worker, Walk &w, long long &T, long long &G) {
     const int lane = threadIdx.x & 31, n = a.kv.n_seqs;
     const int per = (n + 31) / 32, lo = min(n, lane * per), hi = min(n, lo + per);
     const bool report = blockIdx.x == 0 && threadIdx.x < 32;
@@ -85,8 +85,8 @@ __device__ __forceinline__ void share_of(const PagedAttendArgs &a, int segs, Wal
         if (lane >= o) upto += u;
     }
     T = __shfl_sync(0xffffffffu, upto, 31);
-    G = min(static_cast<long long>(gridDim.x), T);
-    const long long i = blockIdx.x, at = i < G ? mul_div(i, T, G) : 0, end = i < G ? mul_div(i + 1, T, G) : 0;
+    G = min(static_cast<long long>(a.workers), T);
+    const long long i = worker, at = i < G ? mul_div(i, T, G) : 0, end = i < G ? mul_div(i + 1, T, G) : 0;
     const int src = __ffs(__ballot_sync(0xffffffffu, at < upto)) - 1;   // (at < T, so there is one)
     long long off = at - (upto - mine);
     int b = lo;
@@ -106,19 +106,19 @@ __device__ __forceinline__ void share_of(const PagedAttendArgs &a, int segs, Wal
     w.end = end;
 }
 
-// For the finish, by the CTA that has a cut segment's last tile: the CTA of
+// For the finish, by the worker that has a cut segment's last tile: that of
 // its first tile << 16 | portions; 0 for a segment that is one portion
-__device__ __forceinline__ unsigned cut_of(const Walk &w, long long T, long long G) {
+__device__ __forceinline__ unsigned cut_of(const Walk &w, int worker, long long T, long long G) {
     if (w.t0 == 0) return 0;
     const long long n = (w.at - w.nt + 1) * G - 1;
     const int own0 = static_cast<int>(T * G < (1ll << 31) ? static_cast<unsigned>(n) / static_cast<unsigned>(T) : n / T);
-    return static_cast<unsigned>(own0) << 16 | (blockIdx.x - own0 + 1);
+    return static_cast<unsigned>(own0) << 16 | (worker - own0 + 1);
 }
-// where a portion's (max, sum, O) go: CTA i's portion that begins its segment
+// where a portion's (max, sum, O) go: worker i's portion that begins its segment
 // to slot 2 i + 1, any other to slot 2 i.  O is [heads][pitch], then maxima
-// and sums from kAttendPart - 32 on.
-__device__ __forceinline__ float *part_at(const PagedAttendArgs &a, int cta, bool first) {
-    return a.part + (2ll * cta + (first ? 1 : 0)) * kAttendPart;
+// and sums from part_floats - 32 on.
+__device__ __forceinline__ float *part_at(const PagedAttendArgs &a, int worker, bool first) {
+    return a.part + (2ll * worker + (first ? 1 : 0)) * a.part_floats;
 }
 
 }  // namespace

@@ -86,11 +86,19 @@ int check_kv(const styx_paged_kv *kv, bool with_buffers, styx::PagedKv &o) {
 uint64_t max_rows(const styx_paged_kv *kv) { return static_cast<uint64_t>(kv->max_pages) * kv->page_size; }
 
 // attend's workspace: the finished portions of every (sequence, kv head,
-// group of 8 or more heads), two partial results per CTA; with weights,
+// group of 8 or more heads), two partial results per worker; with weights,
 // every head's maximum and sum, and every row's scores
 struct AttendWs {
     uint64_t cnt, part, ml, scores, total;
 };
+// the tensor cores take 16-bit rows of up to 128 elements in pages of 16 rows
+// or more (a warp's 16 rows then lie together); everything else runs on the
+// FMA units.  Where both could (32 / 4 heads of 128): 37 rows 6.4 us against
+// 9.7, one sequence of 131071 f16 rows 50 against 117, 32 ragged bf16 ones 34
+// against 75, 64 of 64 / 4 heads 113 against 448
+bool on_tensor_cores(const styx_paged_kv *kv) {
+    return kv->dtype != STYX_F32 && kv->head_dim <= 128 && kv->page_size >= 16;
+}
 AttendWs attend_ws(const styx_paged_kv *kv, int n_heads, bool with_acc, int sms) {
     AttendWs w{};
     uint64_t o = 0;
@@ -98,7 +106,7 @@ AttendWs attend_ws(const styx_paged_kv *kv, int n_heads, bool with_acc, int sms)
     w.cnt = o;
     o += a256(heads * 4);
     w.part = o;
-    o += a256(2ull * sms * styx::kAttendPart * 4);
+    o += a256(on_tensor_cores(kv) ? styx::attend_mma_parts(n_heads / kv->n_kv_heads, sms) : styx::attend_fma_parts(sms));
     w.ml = o;
     if (with_acc) o += a256(heads * 8);
     w.scores = o;
@@ -242,12 +250,7 @@ int styx_paged_attend(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv
     a.scores = reinterpret_cast<float *>(ws + w.scores);
     a.part = reinterpret_cast<float *>(ws + w.part);
     a.cnt = reinterpret_cast<unsigned *>(ws + w.cnt);
-    // the tensor cores take 16-bit rows of up to 128 elements in pages of 16
-    // rows or more (a warp's 16 rows then lie together); everything else runs
-    // on the FMA units.  Where both could (32 / 4 heads of 128): 37 rows 6.4 us
-    // against 9.7, one sequence of 131071 f16 rows 50 against 117, 32 ragged
-    // bf16 ones 34 against 75, 64 of 64 / 4 heads 125 against 448
-    if (kv->dtype != STYX_F32 && kv->head_dim <= 128 && kv->page_size >= 16)
+    if (on_tensor_cores(kv))
         CK(styx::launch_attend_mma(a, sms, S(stream)));
     else
         CK(styx::launch_attend_fma(a, sms, S(stream)));

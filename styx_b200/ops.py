@@ -727,7 +727,8 @@ class PagedKV:
     a pool of all layers); table: int32 [n_seqs][max_pages] page ids; lens:
     int32 [n_seqs] rows in use.  The tensors stay the caller's: page ids and
     lengths are changed in place (or `lens` replaced through the attribute).
-    Calls on one object share its workspaces: not on two streams at once."""
+    Calls on one object share its workspaces (10 MB for attention over 16-bit
+    rows on 148 SMs): not on two streams at once."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lens: torch.Tensor):
         if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.stride() != v.stride():
@@ -756,6 +757,13 @@ class PagedKV:
         self._attend_ws: dict[tuple, tuple] = {}     # (heads, with weights) -> (tensor, address, bytes)
         self._evict_ws: list[torch.Tensor] = []      # the last is in use; smaller ones may still be on a stream
         self._evict_bytes: dict[int, int] = {}
+
+    def share_workspaces(self, other: "PagedKV") -> None:
+        """Uses the other cache's workspaces (one of the same shapes, such as
+        another layer's), where the two are never called at the same time."""
+        if other is not self and (self.k.shape, self.k.dtype, self.table.shape) != (other.k.shape, other.k.dtype, other.table.shape):
+            raise ValueError("share_workspaces: a cache of other shapes")
+        self._attend_ws, self._evict_ws = other._attend_ws, other._evict_ws
 
     @property
     def lens(self) -> torch.Tensor:

@@ -60,6 +60,8 @@ class BatchDecoder:
         self.table = torch.zeros(n_seqs, self.max_pages, dtype=i32, device=dev)
         self.lens = torch.zeros(n_seqs, dtype=i32, device=dev)
         self.kv = [ops.PagedKV(self.pool[0, li], self.pool[1, li], self.table, self.lens) for li in range(L)]
+        for kv in self.kv[1:]:
+            kv.share_workspaces(self.kv[0])
         self.pos = torch.zeros(n_seqs, dtype=i32, device=dev)       # the next token's position
         self.tok = torch.zeros(n_seqs, dtype=i32, device=dev)
         # the host's side of the pages

@@ -602,3 +602,60 @@ def test_sample_rows_do_not_depend_on_their_batch(rows):
         s = slice(i, i + 8)
         tok, lp = ops.sample(x[s], u[s], t[s], k[s], p[s], m[s])
         assert torch.equal(tok, token[s]) and torch.equal(lp, logprob[s])
+
+
+# more segments than SMs: every warp (or pair of warps) of the tensor-core form has a share of its own
+MANY = [
+    # sequences, longest, heads, kv heads, head_dim, page, type, window
+    (50, 400, 32, 4, 128, 16, "bf16", 0),
+    (50, 400, 32, 4, 128, 64, "f16", 100),
+    (40, 700, 64, 4, 128, 32, "bf16", 0),
+    (160, 90, 12, 1, 64, 16, "f16", 0),
+    (100, 300, 10, 2, 72, 64, "bf16", 33),
+    (90, 260, 40, 2, 120, 16, "f16", 0),
+    (200, 128, 8, 1, 128, 64, "f16", 0),
+    (200, 300, 3, 1, 8, 16, "bf16", 0),
+]
+
+
+@pytest.mark.parametrize("n_seqs,longest,heads,n_kv,hd,page,dtype,window", MANY)
+def test_attend_many_sequences(n_seqs, longest, heads, n_kv, hd, page, dtype, window):
+    rng = np.random.default_rng(n_seqs + hd + heads)
+    lens = rng.integers(0, longest + 1, n_seqs)
+    lens[:6] = [0, 1, 16, 17, longest, longest - 1]
+    lens = [int(n) for n in lens]
+    test_attend(lens, heads, n_kv, hd, page, dtype, window)
+    test_attend_accumulates_the_weights(lens, heads, n_kv, hd, page, dtype, window)
+
+
+def test_attend_one_long_among_many_short():
+    """A segment cut over many warps beside segments that are whole."""
+    lens = [3] * 60 + [9000] + [0] * 20 + [40] * 80
+    test_attend(lens, 16, 2, 128, 64, "bf16", 0)
+    test_attend(lens, 16, 1, 128, 16, "f16", 0)
+
+
+def test_attend_many_with_a_page_outside_the_pool():
+    rng = np.random.default_rng(6)
+    lens = [100] * 90
+    kv, ks, vs = make_cache(rng, lens, 2, 128, 16, "f16")
+    kv.table[7, 2] = 1 << 30                    # rows 32 to 47 of sequence 7
+    q = queries(rng, 90, 16, 128)
+    ks[7], vs[7] = np.delete(ks[7], range(32, 48), 0), np.delete(vs[7], range(32, 48), 0)
+    out = attend_ref(q, ks, vs, 128 ** -0.5)[0]
+    close(kv.attend(T(q)).cpu().numpy(), out, 1e-5)
+    with pytest.raises(StyxError):
+        kv.ctx.check_device_error()
+
+
+def test_caches_of_one_shape_share_workspaces():
+    rng = np.random.default_rng(8)
+    a, ka, va = make_cache(rng, [40, 9], 2, 64, 16, "f16")
+    b, kb, vb = make_cache(rng, [21, 33], 2, 64, 16, "f16")
+    other, _, _ = make_cache(rng, [21, 33], 2, 64, 16, "bf16")
+    b.share_workspaces(a)
+    q = queries(rng, 2, 8, 64)
+    for kv, ks, vs in ((a, ka, va), (b, kb, vb), (a, ka, va)):
+        close(kv.attend(T(q)).cpu().numpy(), attend_ref(q, ks, vs, 0.125)[0], 1e-5)
+    with pytest.raises(ValueError, match="share_workspaces"):
+        other.share_workspaces(a)
