@@ -23,6 +23,11 @@
 //     tokens in one step (a flat row) are resolved by bisection of the key.
 //   the draw, where it is not the first CTA's: sums of the kept weights per
 //     warp, each over a stretch of indexes of its own, then inside one warp.
+// Measured (B200, vocabulary 151936): one row with top-k 20 and top-p 0.95 in
+// 7.5 us, the maximum alone 6.5, without filters 12, with top-p over all of it
+// 34 to 36 (the histogram 8 of them); 64 rows of mixed settings 52.5 us (39 MB:
+// 6 at HBM's rate), of which the rows with a histogram, begun first, take 38;
+// in the order given 61.
 // (The row in registers, 1024 threads of 64, spilled; a conversion of the
 // weights by F2I and sums per round of the CTA made the draw of an unfiltered
 // row 18000 of 34000 cycles.)
