@@ -13,7 +13,12 @@
 //
 // Precision.  q and p are f32 while K and V have 8 (bf16) or 11 (f16)
 // significant bits, so q and p are split into 3 or 2 terms of the cache's
-// type that add up to 24 / 22 bits; products are exact, sums f32.
+// type that add up to 24 / 22 bits; products are exact, sums f32.  The MMA
+// cuts its sums off instead of rounding them, an error to one side that grows
+// with every tile added to one accumulator (3.7e-6 of the output over 1800
+// rows), so O is added up by the FMA units: tile by tile in registers, or
+// (teams with shares of their own, whose q's place in shared memory is free
+// by then; 16 heads 122 us otherwise) kSum tiles at a time in shared memory.
 //
 // A warp takes 16 rows at a time for itself; with more than eight q heads per
 // kv head, two warps share them, eight heads each.  Copies (cp.async, 4 KB of
@@ -29,7 +34,7 @@
 // Measured (B200): one sequence of 131071 f16 rows, 32 / 4 heads of 128, 268 MB
 // in 50 us (5.3 TB/s; DRAM 66 % busy, tensor pipe 19 %, issue 33 %); twice as
 // many rows 5.7 to 5.9 TB/s, what cp.async reaches here.  Bound by HBM with up
-// to eight heads per kv head.  With 16 (bf16, 64 ragged sequences, 549 MB) 113
+// to eight heads per kv head.  With 16 (bf16, 64 ragged sequences, 549 MB) 117
 // us, bound by the latency of eight warps' MMAs and exchanges: as CTAs with
 // one share 125, then twelve warps 130, sixteen (whose registers spill) 151;
 // one warp with all 16 heads 175; a branch around each MMA step (head_dim as a
@@ -54,7 +59,8 @@ constexpr int kPad = 132;                      // floats of a head's q in shared
 constexpr int kQ = 8 * kPad * 4;               // q of eight heads
 constexpr int kJoin = kWarps * 4 * kPad * 4;   // JOINT: four heads' results of every warp
 constexpr int kRest = kWarps * kQ;             // beside the rings: q of every warp; JOINT: q, two buffers, and the join's
-static_assert(kRest >= 2 * 2 * kQ + kJoin, "JOINT fits");
+static_assert(kRest >= 2 * 2 * kQ + kJoin && kQ >= 32 * 32 * 4, "JOINT fits; O of a warp fits its q's place");
+constexpr int kSum = 16;                       // tiles that the MMAs add up by themselves (a power of two)
 constexpr float kSlack = 8.f;                  // log2 units a score may pass the maximum by
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool on) {   // off: zeros
@@ -87,6 +93,19 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
         asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
             : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// the same onto zeros
+template <bool BF>
+__device__ __forceinline__ void mma0(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (BF)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 
 // a pair of values (low half: x) as sums of terms of the cache's type, largest
@@ -295,6 +314,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_mma(PagedAttendArgs a) {
         float m[2] = {kNone, kNone}, l[2] = {0.f, 0.f}, o[KS][4];
 #pragma unroll
         for (int t = 0; t < KS; t++) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
+        float *const sum = sq + lane;          // !JOINT: the sums of whole kSum tiles, where q was
+        if constexpr (!JOINT) __syncwarp();
         const int hh = 8 * in + 2 * lc;        // the lane's heads of the group: hh, hh + 1
         float *scores = a.scores + (static_cast<long long>(P.b) * kv.n_kv + P.j) *
                                        (static_cast<long long>(kv.max_pages) << kv.page_shift) * a.gqa + P.g0 + hh;
@@ -351,6 +372,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_mma(PagedAttendArgs a) {
                         for (int t = 0; t < KS; t++) {
                             o[t][e] *= f;
                             o[t][2 + e] *= f;
+                            if (!JOINT && it >= kSum) {
+                                sum[(4 * t + e) * 32] *= f;
+                                sum[(4 * t + 2 + e) * 32] *= f;
+                            }
                         }
                     }
                 }
@@ -381,11 +406,34 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_mma(PagedAttendArgs a) {
                 for (int t = 0; t < KS; t++) {
                     uint32_t A[4];
                     ldm4t(vt ^ (t << 5), A);
+                    if constexpr (JOINT) {
+                        float d[4];
+                        mma0<BF>(d, A, pf[TERMS - 1][0], pf[TERMS - 1][1]);
 #pragma unroll
-                    for (int z = 0; z < TERMS; z++) mma<BF>(o[t], A, pf[z][0], pf[z][1]);
+                        for (int z = TERMS - 2; z >= 0; z--) mma<BF>(d, A, pf[z][0], pf[z][1]);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) o[t][i] += d[i];
+                    } else {
+#pragma unroll
+                        for (int z = TERMS - 1; z >= 0; z--) mma<BF>(o[t], A, pf[z][0], pf[z][1]);
+                    }
                 }
             }
+            if (!JOINT && (it & (kSum - 1)) == kSum - 1) {
+#pragma unroll
+                for (int t = 0; t < KS; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        sum[(4 * t + i) * 32] = it < kSum ? o[t][i] : sum[(4 * t + i) * 32] + o[t][i];
+                        o[t][i] = 0.f;
+                    }
+            }
         }
+        if (!JOINT && P.iters >= kSum)
+#pragma unroll
+            for (int t = 0; t < KS; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[t][i] += sum[(4 * t + i) * 32];
         // ---------------- the portion's end: the next one's first copies, then the result
         const int ng = P.ng;
         const long long h0 = P.h0;
@@ -495,7 +543,7 @@ cudaError_t launch_t(const PagedAttendArgs &a, int sms, cudaStream_t st) {
     // Segments no more than SMs: a CTA's warps together on one of them (one sequence of 131071 rows 50 us, each warp
     // for itself 68, whose 296 results per segment take long to join; 32 ragged ones 33.5 against 35).  More: each team
     // for itself, so that a segment's start and end stop nobody else (64 sequences of up to 512 rows 15 us against 19,
-    // 128 of up to 1024 with 8 kv heads 57 against 63, 64 of up to 8192 with 64 / 4 heads 114 against 125; of up to
+    // 128 of up to 1024 with 8 kv heads 57 against 63, 64 of up to 8192 with 64 / 4 heads 117 against 125; of up to
     // 2048 with 32 / 4 heads 37 against 35).
     const long long segs = static_cast<long long>(a.kv.n_seqs) * a.kv.n_kv * ((a.gqa + 8 * TEAM - 1) / (8 * TEAM));
     if (a.kv.hd <= 64) return segs <= sms ? launch<BF, TEAM, 4, true>(a, sms, st) : launch<BF, TEAM, 4, false>(a, sms, st);

@@ -95,7 +95,7 @@ struct AttendWs {
 // or more (a warp's 16 rows then lie together); everything else runs on the
 // FMA units.  Where both could (32 / 4 heads of 128): 37 rows 6.4 us against
 // 9.7, one sequence of 131071 f16 rows 50 against 117, 32 ragged bf16 ones 34
-// against 75, 64 of 64 / 4 heads 113 against 448
+// against 75, 64 of 64 / 4 heads 117 against 448
 bool on_tensor_cores(const styx_paged_kv *kv) {
     return kv->dtype != STYX_F32 && kv->head_dim <= 128 && kv->page_size >= 16;
 }
