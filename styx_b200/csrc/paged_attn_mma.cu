@@ -36,7 +36,7 @@
 // many rows 5.7 to 5.9 TB/s, what cp.async reaches here.  Bound by HBM with up
 // to eight heads per kv head.  With 16 (bf16, 64 ragged sequences, 549 MB) 117
 // us, bound by the latency of eight warps' MMAs and exchanges: as CTAs with
-// one share 125, then twelve warps 130, sixteen (whose registers spill) 151;
+// one share 133 (125 with sums inside the MMA, then twelve warps 130, sixteen, whose registers spill, 151);
 // one warp with all 16 heads 175; a branch around each MMA step (head_dim as a
 // variable) 145; chains of MMAs half as long change nothing.  32 ragged bf16
 // sequences of up to 4096 rows, 139 MB, 33.5 us: launch, share and first rows
@@ -543,7 +543,7 @@ cudaError_t launch_t(const PagedAttendArgs &a, int sms, cudaStream_t st) {
     // Segments no more than SMs: a CTA's warps together on one of them (one sequence of 131071 rows 50 us, each warp
     // for itself 68, whose 296 results per segment take long to join; 32 ragged ones 33.5 against 35).  More: each team
     // for itself, so that a segment's start and end stop nobody else (64 sequences of up to 512 rows 15 us against 19,
-    // 128 of up to 1024 with 8 kv heads 57 against 63, 64 of up to 8192 with 64 / 4 heads 117 against 125; of up to
+    // 128 of up to 1024 with 8 kv heads 57 against 63, 64 of up to 8192 with 64 / 4 heads 117 against 133; of up to
     // 2048 with 32 / 4 heads 37 against 35).
     const long long segs = static_cast<long long>(a.kv.n_seqs) * a.kv.n_kv * ((a.gqa + 8 * TEAM - 1) / (8 * TEAM));
     if (a.kv.hd <= 64) return segs <= sms ? launch<BF, TEAM, 4, true>(a, sms, st) : launch<BF, TEAM, 4, false>(a, sms, st);
