@@ -19,9 +19,12 @@
 //      residual add fused)
 // Exchanges are monotonic counters in the workspace, never reset (launch
 // tag = launch number + 1 from a counter every CTA increments once): a
-// phase waits until its counter reaches tag x (arrivals per launch).  Every
-// wait is bounded (~1 s): it then records an error code and goes on, so the
-// kernel always ends.
+// phase waits until its counter reaches tag x (arrivals per launch).  That
+// number has to be the same for every launch on a workspace, at whatever
+// position: a head's rows, the heads, and for the splits (which grow with
+// the rows) the grid's CTAs, of which split 0 counts for all that are not
+// splits of its head.  Every wait is bounded (~1 s): it then records an
+// error code and goes on, so the kernel always ends.
 #include <cuda_runtime.h>
 
 #include <cmath>
@@ -461,7 +464,7 @@ __global__ void __launch_bounds__(kAF, 1) k_attn_fused(const __grid_constant__ A
         __syncthreads();
         if (tid == 0) {
             __threadfence();
-            atomicAdd(p.split_cnt + kvh, 1ull);
+            atomicAdd(p.split_cnt + kvh, static_cast<unsigned long long>(split == 0 ? G - S + 1 : 1));   // (S <= G) G in all
         }
     }
     AF_STAMP(7);
@@ -469,7 +472,7 @@ __global__ void __launch_bounds__(kAF, 1) k_attn_fused(const __grid_constant__ A
     // ------------------------------------------------ phase D: merge head b's splits
     if (b < p.n_heads) {
         float *w = reinterpret_cast<float *>(w1);   // [S] split weights
-        if (tid == 0 && !wait_count(p.split_cnt + b / gqa, tag * static_cast<unsigned long long>(S), p.err))
+        if (tid == 0 && !wait_count(p.split_cnt + b / gqa, tag * static_cast<unsigned long long>(G), p.err))
             *s_ok = 0;
         __syncthreads();
         AF_STAMP(8);

@@ -252,6 +252,35 @@ def test_one_kernel_attention_at_long_context(pos):
     assert rel_to_max(outs[CLUSTER][0], outs[SEPARATE][0]) < 1e-5
 
 
+@pytest.mark.parametrize("form", [FUSED, CLUSTER], ids=["one-kernel", "cluster"])
+@pytest.mark.parametrize("H,n_heads,n_kv", [(512, 8, 2), (2048, 32, 4)])
+def test_attention_forms_at_positions_that_change_the_splits(H, n_heads, n_kv, form):
+    """One workspace over positions whose rows are cut into 1, 2, 3 and more
+    splits, rising and falling (a sequence that grows, then a new one): every
+    token is exact and no wait gives up or ends early."""
+    hd = 128
+    qts = (_lib.Q4_K, _lib.Q4_K, _lib.Q6_K, _lib.Q4_K)
+    ws, an, qn, kn = _attn_layer(3, H, n_heads, n_kv, hd, qts)
+    eps, base, n_ctx, kvd = 1e-6, 1_000_000.0, 200, n_kv * hd
+    rng = np.random.default_rng(12)
+    kc0 = rng.normal(0, 1, (n_ctx, kvd)).astype(np.float32)
+    vc0 = rng.normal(0, 1, (n_ctx, kvd)).astype(np.float32)
+    w = ops.AttnWeights(T(an), *[ops.DenseWeight(qt, T(raw)) for qt, raw in ws], q_norm=T(qn), k_norm=T(kn))
+    blk = ops.AttnBlock(H, n_heads, n_kv, hd, True, eps, base)
+    blk.ctx.set_option(_lib.OPT_ATTN_KERNELS, form)
+    try:
+        for pos in (0, 14, 15, 16, 17, 31, 32, 47, 48, 150, 199, 16, 3, 0, 40):
+            x0 = rng.normal(0, 1, H).astype(np.float32)
+            x, kc, vc = T(x0), T(kc0), T(vc0)
+            blk.forward(x, w, pos, T(np.array([pos], np.int32)), kc, vc, n_ctx)
+            blk.ctx.check_device_error()
+            assert blk.last_path() == PATH[form]
+            exp = O.attn_block(x0, an, eps, n_heads, n_kv, hd, qn, kn, base, ws, pos, kc0.copy(), vc0.copy())
+            assert rel_to_max(x.cpu().numpy(), exp) < 1e-4, pos
+    finally:
+        blk.ctx.set_option(_lib.OPT_ATTN_KERNELS, 0)
+
+
 def test_one_kernel_attention_split_launch_numbers_time_out_and_recover():
     """As tests/test_gpu_timeout.py for the attention kernel: the workspace's
     launch counter set to half a grid splits the CTAs over two launch

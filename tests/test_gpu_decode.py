@@ -11,7 +11,7 @@ import torch
 from oracle import oracle as O
 from styx_b200 import _lib, ops
 from styx_b200.decode import DecodeLayer, DecodeModel, DecodeParams
-from tests.decode_case import OracleDecoder, Q4_K, Q6_K, make_model, total_cmp_argmax_last
+from tests.decode_case import OracleDecoder, Q4_K, Q6_K, make_model, oracle_greedy, total_cmp_argmax_last
 
 pytestmark = pytest.mark.gpu
 
@@ -81,6 +81,21 @@ def test_greedy_tokens_identical_to_the_oracle(seed, cfg):
     # and generate() itself, free-running, gives the same sequence
     g.reset()
     assert g.generate(prompt, n_predict) == toks
+
+
+def test_greedy_tokens_past_the_first_split():
+    """The one-kernel attention cuts its rows into two splits from position 16
+    on, three from 32 on: the same run, and a second one from position 0,
+    give the oracle's tokens."""
+    m = make_model(2, hd=128, n_heads=8, n_kv=2)
+    prompt = [5, 17, 99, 3, 1, 4, 640]
+    expect = oracle_greedy(m, prompt, 30)
+    g = gpu_model(m, 64)
+    for _ in range(2):
+        g.reset()
+        assert g.generate(prompt, 30) == expect
+        g.moe.ctx.check_device_error()
+        assert g.attn.last_path() == 1
 
 
 @pytest.mark.parametrize("qname", ["q4_K", "q5_K", "q6_K", "q8_0"])
