@@ -695,6 +695,7 @@ __global__ void __launch_bounds__(kNT, 2) k_sample_cluster(SampleArgs a, int reg
     };
     // the largest key whose sum reaches lim, and how many of the tokens at it that takes
     auto bisect = [&](u64 lim, bool weights, uint32_t floor_key, u64 floor_ties) {
+        cluster_sync();   // every CTA has read the counts that it decided by: the first sum overwrites their slots
         uint32_t l = max(floor_key, 1u), h = key_of(m);   // measure(l) >= lim
         int slot = 0;
         while (l < h) {

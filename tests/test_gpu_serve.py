@@ -604,6 +604,30 @@ def test_sample_rows_do_not_depend_on_their_batch(rows):
         assert torch.equal(tok, token[s]) and torch.equal(lp, logprob[s])
 
 
+@pytest.mark.parametrize("vocab", [2049, 2100, 3000, 4096, 20000])
+def test_sample_many_flat_rows(vocab):
+    """More equal logits than one CTA sorts, few of them outside the first CTA's slice or all slices full: the
+    threshold by bisection of the key (its sums share slots with the counts that chose it).  Whole numbers of equal
+    weight: the token is exact."""
+    rows = 300
+    rng = np.random.default_rng(vocab)
+    x = torch.zeros(rows, vocab, device=DEV)
+    u24 = rng.integers(0, 1 << 24, rows)
+    u = T((u24 / 2.0 ** 24).astype(np.float32))
+    frac = rng.integers(1, 1 << 24, rows)                      # top-p as a fraction of 2^24
+    ks = rng.integers(121, vocab, rows)
+    one = 1 << 40
+    kept_p = [-(-max(1, (vocab * one * int(f)) >> 24) // one) for f in frac]
+    for _ in range(10):
+        for kept, kw in ((kept_p, dict(top_p=T((frac / 2.0 ** 24).astype(np.float32)))),
+                         (ks.tolist(), dict(top_k=T(ks.astype(np.int32))))):
+            token, lp = ops.sample(x, u, **kw)
+            exp = [((n * one * int(a)) >> 24) // one for n, a in zip(kept, u24)]
+            assert token.tolist() == exp
+            assert np.allclose(lp.cpu().numpy(), -np.log(np.array(kept)), atol=1e-5)
+    ops.ctx(0).check_device_error()
+
+
 # more segments than SMs: every warp (or pair of warps) of the tensor-core form has a share of its own
 MANY = [
     # sequences, longest, heads, kv heads, head_dim, page, type, window
