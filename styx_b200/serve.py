@@ -59,7 +59,10 @@ class BatchDecoder:
         self.pool = torch.empty(2, L, self.n_pages, kvh, page, hd, dtype=cache, device=dev)
         self.table = torch.zeros(n_seqs, self.max_pages, dtype=i32, device=dev)
         self.lens = torch.zeros(n_seqs, dtype=i32, device=dev)
-        self.kv = [ops.PagedKV(self.pool[0, li], self.pool[1, li], self.table, self.lens) for li in range(L)]
+        # the lengths that the caches go by: 0 for the sequences that a step leaves out, so that nothing of theirs is
+        # read, and no weight of theirs changes
+        self.live = torch.zeros(n_seqs, dtype=i32, device=dev)
+        self.kv = [ops.PagedKV(self.pool[0, li], self.pool[1, li], self.table, self.live) for li in range(L)]
         for kv in self.kv[1:]:
             kv.share_workspaces(self.kv[0])
         self.pos = torch.zeros(n_seqs, dtype=i32, device=dev)       # the next token's position
@@ -123,10 +126,14 @@ class BatchDecoder:
 
     def step(self, n: Optional[int] = None) -> torch.Tensor:
         """The tokens tok[:n] of the first n sequences at their next
-        positions; returns logits f32 [n][n_vocab]."""
+        positions; returns logits f32 [n][n_vocab].  The other sequences stay
+        as they are."""
         hp, hd = self.hp, self.hp.head_dim
         n = self.n_seqs if n is None else n
         self._grow(n)
+        self.live[:n] = self.lens[:n]
+        if n < self.n_seqs:
+            self.live[n:] = 0
         x, xn, pos = self.x[:n], self.xn[:n], self.pos[:n]
         qkv = self.qkv[:n]
         q, k, v = (t.unflatten(1, (-1, hd)) for t in qkv.split((self.n_q, self.n_k, self.n_k), dim=1))
@@ -165,6 +172,7 @@ class BatchDecoder:
 
     def evict(self) -> None:
         """Every sequence down to the budget, in every layer."""
+        self.live.copy_(self.lens)
         for li, kv in enumerate(self.kv):
             acc, row_pos = self.acc[li], self.row_pos[li]
             kv.evict(acc, row_pos, self.pos, self.budget, self.n_recent, self.n_sink, acc_out=self.acc[-1],

@@ -101,3 +101,40 @@ def test_command_line(tmp_path, capsys):
     assert serve.main(argv) == 0
     out = capsys.readouterr().out.split()
     assert len(out) == 2 and all(len(o.split(",")) == 10 for o in out)
+
+
+def test_a_step_of_some_sequences_leaves_the_others_as_they_are():
+    m = make_model(2)
+    d = decoder(m, page=8, cache=torch.float16, budget=24, n_recent=8, n_sink=2)
+    whole = decoder(m, page=8, cache=torch.float16, budget=24, n_recent=8, n_sink=2)
+    rng = np.random.default_rng(4)
+    toks = [torch.from_numpy(rng.integers(0, m.hp["n_vocab"], 4).astype(np.int32)) for _ in range(5)]
+
+    def step(dec, t, n=None):
+        dec.tok.copy_(t)
+        return dec.step(n).clone()
+
+    for t in toks[:3]:
+        step(d, t)
+        step(whole, t)
+    L = m.hp["n_layers"]
+    acc, pos, rows = [a.clone() for a in d.acc[:L]], [p.clone() for p in d.row_pos[:L]], list(d.rows)
+    used = torch.tensor([p for ps in d.pages[2:] for p in ps], device=d.device)
+    pool = d.pool[:, :, used].clone()
+    got = step(d, toks[3], 2)
+    # (other sums than a step of all four: the bound of the 16-bit rows and experts above)
+    ref = step(whole, toks[3])[:2]
+    assert (got - ref).abs().max() <= 4 * (2.0 ** -11 + 1e-3) * ref.abs().max()
+    for li in range(L):
+        assert torch.equal(d.acc[li][2:], acc[li][2:]) and not torch.equal(d.acc[li][:2], acc[li][:2])
+        assert torch.equal(d.row_pos[li][2:], pos[li][2:])
+    assert torch.equal(d.pool[:, :, used].view(torch.int16), pool.view(torch.int16))
+    assert d.rows == [rows[0] + 1, rows[1] + 1] + rows[2:] == d.lens.tolist() and d.pos.tolist() == d.rows
+    # evicting with sequences that the last step left out reaches them too
+    d.budget = 3
+    d.n_recent, d.n_sink = 1, 1
+    d.evict()
+    assert d.lens.tolist() == [3] * 4 == d.rows
+    # a step of all of them goes on from there
+    assert step(d, toks[4]).isfinite().all() and d.lens.tolist() == [4] * 4
+    d.kv[0].ctx.check_device_error()
