@@ -112,15 +112,22 @@ class BatchDecoder:
         del self.pages[b][keep:]
 
     def _grow(self, n: int) -> None:
-        """One row more for the first n sequences, a page where it starts one."""
+        """One row more for the first n sequences, a page where it starts one;
+        ValueError, and nothing changed, where one of them has no room."""
+        if not 1 <= n <= self.n_seqs:
+            raise ValueError(f"a step of {n} sequences: 1 to {self.n_seqs}")
+        starts = []                        # sequences whose new row starts a page
         for b in range(n):
             if self.rows[b] == self.n_rows:
                 raise ValueError(f"sequence {b}: KV cache full ({self.n_rows} rows)")
             if self.rows[b] == len(self.pages[b]) * self.page:
-                if not self.free:
+                if len(starts) == len(self.free):
                     raise ValueError(f"sequence {b}: no page left of {self.n_pages}")
-                self.pages[b].append(self.free.pop())
-                self.table[b, len(self.pages[b]) - 1] = self.pages[b][-1]
+                starts.append(b)
+        for b in starts:
+            self.pages[b].append(self.free.pop())
+            self.table[b, len(self.pages[b]) - 1] = self.pages[b][-1]
+        for b in range(n):
             self.rows[b] += 1
         self.lens[:n] += 1
 

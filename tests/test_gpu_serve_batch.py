@@ -138,3 +138,28 @@ def test_a_step_of_some_sequences_leaves_the_others_as_they_are():
     # a step of all of them goes on from there
     assert step(d, toks[4]).isfinite().all() and d.lens.tolist() == [4] * 4
     d.kv[0].ctx.check_device_error()
+
+
+@pytest.mark.parametrize("kind", ["pages", "rows"])
+def test_a_refused_step_changes_nothing(kind):
+    """The third of four sequences needs the page (row) that is not there: the first two have taken none either, and
+    the step goes through once there is room."""
+    m = make_model(0, n_layers=1)
+    d = decoder(m, n_ctx=8, page=4, n_pages=6 if kind == "pages" else None)
+    for i in range(4):
+        d.step()                                           # four rows each: one full page
+    if kind == "rows":
+        d.lens[2], d.rows[2] = 8, 8                        # the third is full
+        d.pages[2].append(d.free.pop())
+    before = (list(d.rows), [list(p) for p in d.pages], list(d.free), d.lens.tolist(), d.table.tolist(), d.pos.tolist())
+    for _ in range(3):
+        with pytest.raises(ValueError, match="sequence 2: no page left" if kind == "pages" else "sequence 2: KV cache full"):
+            d.step()
+        assert before == (list(d.rows), [list(p) for p in d.pages], list(d.free), d.lens.tolist(), d.table.tolist(),
+                          d.pos.tolist())
+    for n in (0, -1, 5):
+        with pytest.raises(ValueError, match="sequences"):
+            d.step(n)
+    d.step(2)
+    assert d.lens.tolist() == d.rows and d.rows[:2] == [5, 5]
+    d.kv[0].ctx.check_device_error()
