@@ -760,9 +760,11 @@ class PagedKV:
 
     def share_workspaces(self, other: "PagedKV") -> None:
         """Uses the other cache's workspaces (one of the same shapes, such as
-        another layer's), where the two are never called at the same time."""
-        if other is not self and (self.k.shape, self.k.dtype, self.table.shape) != (other.k.shape, other.k.dtype, other.table.shape):
-            raise ValueError("share_workspaces: a cache of other shapes")
+        another layer's, on one device), where the two are never called at
+        the same time."""
+        if other is not self and (self.index, self.k.shape, self.k.dtype, self.table.shape) != (
+                other.index, other.k.shape, other.k.dtype, other.table.shape):
+            raise ValueError("share_workspaces: a cache of other shapes or on another device")
         self._attend_ws, self._evict_ws = other._attend_ws, other._evict_ws
 
     @property

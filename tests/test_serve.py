@@ -92,3 +92,15 @@ def test_batch_decoder_refuses_what_it_cannot_hold():
         BatchDecoder(hp, None, [], None, None, 65, 64)
     with pytest.raises(ValueError, match="budget"):
         BatchDecoder(hp, None, [], None, None, 4, 64, budget=16, n_recent=14, n_sink=4)
+
+
+def test_caches_of_different_devices_do_not_share_workspaces():
+    a, b = (ops.PagedKV.__new__(ops.PagedKV) for _ in range(2))
+    for index, o in enumerate((a, b)):
+        o.k, o.table = torch.zeros(4, 2, 16, 64), torch.zeros(1, 4, dtype=torch.int32)
+        o.index, o._attend_ws, o._evict_ws = index, {}, []
+    with pytest.raises(ValueError, match="share_workspaces"):
+        a.share_workspaces(b)
+    b.index = 0
+    a.share_workspaces(b)
+    assert a._attend_ws is b._attend_ws and a._evict_ws is b._evict_ws
