@@ -79,6 +79,8 @@ int styx_paged_append(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv
  * [n_seqs][n_heads][head_dim], 16-byte aligned; n_heads a multiple of
  * n_kv_heads.  Rows outside the window or past the length are never used,
  * whatever they hold.
+ * A NaN in a head's q or in a row of K that is seen, or a score of +inf, makes
+ * the head's output (and its lse and weights) NaN.
  *   lse (may be NULL): f32 [n_seqs][n_heads], log sum_r e^(scale q.K[r]),
  *     -inf where there are no rows.
  *   acc_out (may be NULL): f32 [n_seqs][n_kv_heads][acc_stride], the

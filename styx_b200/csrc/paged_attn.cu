@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_fma(PagedAttendArgs a) {
             float v = 0.f;
 #pragma unroll
             for (int w = 0; w < kWarps; w++) v += so[(w * NH + h) * 8 * LPR + c] * ex2(s_m[w][h] - s_M[h]);
-            if (whole) a.out[(h0 + h) * hd + c] = s_L[h] > 0.f ? v / s_L[h] : 0.f;
+            if (whole) a.out[(h0 + h) * hd + c] = s_L[h] == 0.f ? 0.f : v / s_L[h];
             else part[h * kPitch + c] = v;
         }
         if (tid < ng) {
@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_fma(PagedAttendArgs a) {
                 part[a.part_floats - 32 + tid] = M;
                 part[a.part_floats - 16 + tid] = L;
             } else {
-                if (a.lse) a.lse[h0 + tid] = L > 0.f ? M * 0.6931471805599453f + logf(L) : -INFINITY;
+                if (a.lse) a.lse[h0 + tid] = lse_of(M, L);
                 if (a.acc_out) {
                     a.ml[2 * (h0 + tid)] = M;
                     a.ml[2 * (h0 + tid) + 1] = L;
@@ -413,13 +413,13 @@ __global__ void __launch_bounds__(256) k_attend_finish(PagedAttendArgs a, int jo
         }
         if (!on) return;
         const long long at_h = static_cast<long long>(b) * a.n_heads + j * a.gqa + g0 + h;
-        const float r = L > 0.f ? 1.f / L : 0.f;
+        const float r = inverse_sum(L);
 #pragma unroll
         for (int v = 0; v < NV; v++)
             if (4 * lane + 128 * v < kv.hd)
                 *reinterpret_cast<float4 *>(a.out + at_h * kv.hd + 4 * lane + 128 * v) =
                     make_float4(o[v].x * r, o[v].y * r, o[v].z * r, o[v].w * r);
-        if (lane == 0 && a.lse) a.lse[at_h] = L > 0.f ? M * 0.6931471805599453f + logf(L) : -INFINITY;
+        if (lane == 0 && a.lse) a.lse[at_h] = lse_of(M, L);
         return;
     }
     // ---------------- accumulated weights
@@ -462,7 +462,7 @@ __global__ void __launch_bounds__(256) k_attend_finish(PagedAttendArgs a, int jo
                 }
                 if (lane == 0) {
                     s_M[g] = M;
-                    s_L[g] = L > 0.f ? 1.f / L : 0.f;
+                    s_L[g] = inverse_sum(L);
                 }
             }
             __syncthreads();

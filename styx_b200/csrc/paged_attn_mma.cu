@@ -455,7 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_mma(PagedAttendArgs a) {
                 part[a.part_floats - 16 + h] = L;
                 return;
             }
-            if (a.lse) a.lse[h0 + h] = L > 0.f ? M * 0.6931471805599453f + logf(L) : -INFINITY;
+            if (a.lse) a.lse[h0 + h] = lse_of(M, L);
             if (a.acc_out) {
                 a.ml[2 * (h0 + h)] = M;
                 a.ml[2 * (h0 + h) + 1] = L;
@@ -467,7 +467,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_mma(PagedAttendArgs a) {
             for (int e = 0; e < 2; e++) {
                 const int h = hh + e;
                 if (h >= ng) continue;
-                const float r = (whole ? (l[e] > 0.f ? 1.f / l[e] : 0.f) : 1.f) * kUp;
+                const float r = (whole ? inverse_sum(l[e]) : 1.f) * kUp;
                 float *to = whole ? a.out + (h0 + h) * hd : part + h * 128;
 #pragma unroll
                 for (int t = 0; t < KS; t++)
@@ -514,7 +514,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend_mma(PagedAttendArgs a) {
                     float v = 0.f;
 #pragma unroll
                     for (int w = 0; w < TEAMS; w++) v += so[((w * TEAM + e) * 4 + h4) * kPad + c] * s_m[w * TEAM + e][4 * n + h4];
-                    if (whole) a.out[(h0 + h) * hd + c] = s_L[h] > 0.f ? v / s_L[h] : 0.f;
+                    if (whole) a.out[(h0 + h) * hd + c] = s_L[h] == 0.f ? 0.f : v / s_L[h];
                     else part[h * 128 + c] = v;
                 }
                 if (n == 0) __syncthreads();

@@ -18,6 +18,14 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// A softmax's sum is 0 where no row was seen, and only there: a row's weight
+// against the maximum is 1 for one of them.  NaN (of a NaN in q or K, or of a
+// score of +inf) is neither, and goes to the output.
+__device__ __forceinline__ float inverse_sum(float sum) { return sum == 0.f ? 0.f : 1.f / sum; }
+__device__ __forceinline__ float lse_of(float max, float sum) {   // max in units of log2
+    return sum == 0.f ? -INFINITY : max * 0.6931471805599453f + logf(sum);
+}
+
 // rows of a sequence that are seen, and its tiles (an empty one counts one
 // tile, so that somebody writes its zeros)
 struct Seq {

@@ -683,3 +683,50 @@ def test_caches_of_one_shape_share_workspaces():
         close(kv.attend(T(q)).cpu().numpy(), attend_ref(q, ks, vs, 0.125)[0], 1e-5)
     with pytest.raises(ValueError, match="share_workspaces"):
         other.share_workspaces(a)
+
+
+@pytest.mark.parametrize("lens,heads,n_kv,hd,page,dtype", [([40, 9], 16, 2, 128, 16, "f16"), ([40, 9], 16, 2, 128, 16, "bf16"),
+                                                            ([40, 9], 16, 2, 128, 16, "f32"), ([700, 33], 32, 2, 64, 64, "bf16"),
+                                                            ([5000, 9], 8, 1, 128, 64, "f16"), ([5000, 9], 8, 1, 128, 64, "f32"),
+                                                            ([300] * 90, 16, 2, 128, 64, "f16"), ([300] * 90, 32, 2, 72, 64, "bf16"),
+                                                            ([60, 9], 8, 2, 256, 16, "f16")])
+def test_attend_nan_and_infinite_scores_are_not_hidden(lens, heads, n_kv, hd, page, dtype):
+    """The softmax over a NaN or a score of +inf is NaN, not the zeros of a sequence without rows: in q of one head,
+    and in one row of K (all heads of its kv head).  The other heads and sequences keep their values (not their bits:
+    the heads of a group move their maxima together)."""
+    rng = np.random.default_rng(50)
+    kv, _, _ = make_cache(rng, lens, n_kv, hd, page, dtype)
+    q = T(queries(rng, len(lens), heads, hd))
+    lse = torch.zeros(len(lens), heads, device=DEV)
+    acc = torch.zeros(len(lens), n_kv, kv.max_rows, device=DEV)
+    exp, exp_lse = kv.attend(q, lse=lse, acc=acc).clone(), lse.clone()
+    exp_acc = acc.clone()
+
+    def check(hit):                       # hit: [sequences][heads], True where NaN is expected
+        got = kv.attend(q, lse=lse, acc=acc)
+        assert torch.isnan(got[hit]).all() and torch.isnan(lse[hit]).all()
+        close(got[~hit].cpu().numpy(), exp[~hit].cpu().numpy(), 2e-5)          # 1e-5 each
+        assert (lse[~hit] - exp_lse[~hit]).abs().max() <= 2e-5 * max(1, exp_lse[~hit].abs().max().item())
+        by_kv = hit.unflatten(1, (n_kv, -1)).any(2)
+        for b, n in enumerate(lens):
+            for j in range(n_kv):
+                if by_kv[b, j]:
+                    assert torch.isnan(acc[b, j, :n]).all()
+                else:
+                    assert (acc[b, j, :n] - exp_acc[b, j, :n]).abs().max() <= 2e-5 * heads / n_kv
+
+    for bad in (float("nan"), float("inf")):
+        hit = torch.zeros(len(lens), heads, dtype=torch.bool, device=DEV)
+        hit[0, 3] = True
+        keep = q[0, 3, 5].item()
+        q[0, 3, 5] = bad
+        acc.zero_()
+        check(hit)
+        q[0, 3, 5] = keep
+    page_id, row = int(kv.table[0, 0]), 1
+    kv.k[page_id, 0, row, 2] = float("nan")
+    hit = torch.zeros(len(lens), heads, dtype=torch.bool, device=DEV)
+    hit[0, :heads // n_kv] = True
+    acc.zero_()
+    check(hit)
+    kv.ctx.check_device_error()
