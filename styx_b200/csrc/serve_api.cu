@@ -1,6 +1,7 @@
 // serve_api.cu -- the C entry points of include/styx_serve.h: validation,
 // workspaces and launches; the kernels are in paged.cu, paged_attn.cu and
 // sample.cu.
+#include <algorithm>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -115,14 +116,15 @@ AttendWs attend_ws(const styx_paged_kv *kv, int n_heads, bool with_acc, int sms)
     return w;
 }
 
-// evict's workspace: the moves' sources, places and number; the keys of long lines
+// evict's workspace: the moves' sources, places and number; the keys of long lines.  A line moves no more rows than
+// the budget, nor than it has (room for those in whole slices of 4096)
 struct EvictWs {
     uint64_t places, moves, keys, total;
 };
 EvictWs evict_ws(const styx_paged_kv *kv, int budget) {
     EvictWs w{};
     const uint64_t lines = static_cast<uint64_t>(kv->n_seqs) * kv->n_kv_heads;
-    w.places = a256(lines * budget * 4);
+    w.places = a256(lines * std::min<uint64_t>(static_cast<uint64_t>(budget), (max_rows(kv) + 4095) & ~uint64_t(4095)) * 4);
     w.moves = w.places * 2;
     w.keys = w.moves + a256(lines * 4);
     w.total = w.keys + (styx::evict_staged(static_cast<long long>(max_rows(kv))) ? 0 : a256(lines * max_rows(kv) * 4));
@@ -297,7 +299,7 @@ int styx_paged_evict(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv,
     a.pos = pos;
     a.next_pos = next_pos;
     a.stride = stride;
-    a.budget = budget;
+    a.budget = static_cast<int>(std::min<uint64_t>(static_cast<uint64_t>(budget), max_rows(kv)));
     a.n_recent = n_recent;
     a.n_sink = n_sink;
     a.acc_out = acc_out;

@@ -730,3 +730,17 @@ def test_attend_nan_and_infinite_scores_are_not_hidden(lens, heads, n_kv, hd, pa
     acc.zero_()
     check(hit)
     kv.ctx.check_device_error()
+
+
+@pytest.mark.parametrize("budget", [48, 49, 2 ** 31 - 1])
+def test_evict_with_a_budget_beyond_the_rows(budget):
+    rng = np.random.default_rng(23)
+    kv, ks, vs = make_cache(rng, [48, 7, 0], 2, 64, 16, "f16")
+    acc, pos = rng.uniform(0, 1, (3, 2, 48)).astype(np.float32), rng.permutation(288).reshape(3, 2, 48).astype(np.int32)
+    a, p, n = kv.evict(T(acc), T(pos), T(np.array([300, 300, 300], np.int32)), budget, 20, 4)
+    kv.ctx.check_device_error()
+    assert n.tolist() == [48, 7, 0]
+    for b, m in enumerate([48, 7, 0]):
+        assert np.array_equal(a[b, :, :m].cpu().numpy(), acc[b, :, :m]) and np.array_equal(p[b, :, :m].cpu().numpy(), pos[b, :, :m])
+        gk, gv = read_rows(kv, b, m)
+        assert m == 0 or (np.array_equal(gk, ks[b]) and np.array_equal(gv, vs[b]))

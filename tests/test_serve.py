@@ -104,3 +104,15 @@ def test_caches_of_different_devices_do_not_share_workspaces():
     b.index = 0
     a.share_workspaces(b)
     assert a._attend_ws is b._attend_ws and a._evict_ws is b._evict_ws
+
+
+def test_evict_workspace_goes_by_the_rows_there_are():
+    """A budget beyond a sequence's rows moves nothing: from whole slices of 4096 rows on it takes no more room."""
+    L, n, most = _lib.lib(), C.c_uint64(), C.c_uint64()
+    for pages, slices in ((4, 1), (256, 1), (257, 2)):     # 64, 4096 and 4112 rows
+        of = kv(max_pages=pages, table_stride=pages)
+        assert L.styx_paged_evict_workspace_bytes(C.byref(of), 4096 * slices, C.byref(most)) == 0
+        for budget in (4096 * slices + 1, 10 ** 9, 2 ** 31 - 1):
+            assert L.styx_paged_evict_workspace_bytes(C.byref(of), budget, C.byref(n)) == 0
+            assert n.value == most.value < 2 * 6 * 4096 * slices * 4 + 1024
+        assert L.styx_paged_evict_workspace_bytes(C.byref(of), 63, C.byref(n)) == 0 and n.value < most.value
