@@ -66,8 +66,8 @@ typedef struct styx_paged_kv {
  * token whose row is negative (a slot of length 0 among them) writes no row
  * and a zero q_out; a row past max_pages * page_size or a page outside the
  * pool is skipped and reported.  n_heads may be 0 (no q); q_out, 16-byte
- * aligned, may not
- * overlap q.  Two tokens with one (sequence, row) leave either's row. */
+ * aligned, may not overlap q, k or v (nor what lies between their tokens).
+ * Two tokens with one (sequence, row) leave either's row. */
 int styx_paged_append(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv, int n_tokens, int n_heads,
                       const float *q, int64_t q_stride, const float *k, int64_t k_stride, const float *v,
                       int64_t v_stride, const float *q_norm, const float *k_norm, float eps, float freq_base,

@@ -42,6 +42,14 @@ bool rows_ok(const void *p, uint64_t rows, uint64_t stride, uint64_t n, uint64_t
     return rows == 0 || styx::range_ok(p, ((rows - 1) * stride + n) * size);
 }
 
+// the bytes of such rows, [begin, end), for checks of overlaps
+struct Span {
+    const char *begin, *end;
+    Span(const void *p, uint64_t bytes) : begin(static_cast<const char *>(p)), end(begin + (p ? bytes : 0)) {}
+    Span(const void *p, uint64_t rows, uint64_t stride, uint64_t n, uint64_t size) : Span(p, ((rows - 1) * stride + n) * size) {}
+    bool apart(const Span &o) const { return end <= o.begin || o.end <= begin; }
+};
+
 int check_kv(const styx_paged_kv *kv, bool with_buffers, styx::PagedKv &o) {
     NEED(kv, "null styx_paged_kv");
     NEED(kv->dtype == STYX_F32 || kv->dtype == STYX_F16 || kv->dtype == STYX_BF16,
@@ -165,9 +173,9 @@ int styx_paged_append(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv
              styx::range_ok(k_norm, k_norm ? kv->head_dim * 4ull : 0),
          "pos / seq / row / norms too small");
     if (n_heads) {
-        const char *q0 = reinterpret_cast<const char *>(q), *q1 = q0 + ((n_tokens - 1) * q_stride + qd) * 4;
-        const char *o0 = reinterpret_cast<const char *>(q_out), *o1 = o0 + n_tokens * qd * 4;
-        NEED(o1 <= q0 || q1 <= o0, "q_out overlaps q");
+        const Span to(q_out, n_tokens, qd, qd, 4);
+        NEED(to.apart(Span(q, n_tokens, q_stride, qd, 4)), "q_out overlaps q");
+        NEED(to.apart(Span(k, n_tokens, k_stride, kd, 4)) && to.apart(Span(v, n_tokens, v_stride, kd, 4)), "q_out overlaps k or v");
     }
     a.q = q;
     a.k = k;

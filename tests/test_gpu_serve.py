@@ -744,3 +744,22 @@ def test_evict_with_a_budget_beyond_the_rows(budget):
         assert np.array_equal(a[b, :, :m].cpu().numpy(), acc[b, :, :m]) and np.array_equal(p[b, :, :m].cpu().numpy(), pos[b, :, :m])
         gk, gv = read_rows(kv, b, m)
         assert m == 0 or (np.array_equal(gk, ks[b]) and np.array_equal(gv, vs[b]))
+
+
+def test_append_refuses_a_q_out_over_k_or_v():
+    """k and v are read by other warps than those that write q_out."""
+    rng = np.random.default_rng(42)
+    kv, _, _ = make_cache(rng, [20, 30], 2, 64, 16, "f16")
+    buf = T(rng.normal(0, 1, 2 * 8 * 64 + 2 * 2 * 64).astype(np.float32))
+    q, other = T(queries(rng, 2, 8, 64)), T(rng.normal(0, 1, (2, 2, 64)).astype(np.float32))
+    pos = torch.tensor([3, 4], dtype=torch.int32, device=DEV)
+    out = buf[:1024].view(2, 8, 64)
+    for at in (0, 64, 1024 - 4):                              # its start, inside, its last 16 bytes
+        over = buf[at:at + 256].view(2, 2, 64)
+        for k, v in ((over, other), (other, over)):
+            with pytest.raises(StyxError, match="overlaps") as e:
+                kv.append(q, k, v, pos, 1e4, out=out)
+            assert e.value.code == _lib.STYX_EINVAL
+    exp = kv.append(q, other, other, pos, 1e4)
+    assert torch.equal(kv.append(q, buf[1024:].view(2, 2, 64), other, pos, 1e4, out=out), exp)   # beside it
+    kv.ctx.check_device_error()
