@@ -87,7 +87,8 @@ int styx_paged_append(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv
  *     accumulated attention weight of every row r < lens[b]:
  *       acc_out[r] = (r == lens[b] - 1 ? 0 : acc[r]) + sum of p[r] over the
  *     kv head's q heads (acc of the newest row is not read, so a row enters
- *     with nothing to be cleared first).  acc_out may be acc.
+ *     with nothing to be cleared first).  acc_out may be acc, and out may be
+ *     q; no other overlap of these.
  * The workspace (styx_paged_attend_workspace_bytes, 256-byte aligned) holds
  * the splits' partial sums and their counters: initialise it once.  Calls
  * that share one must not run at the same time. */

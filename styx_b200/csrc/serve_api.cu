@@ -237,10 +237,12 @@ int styx_paged_attend(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv
     NEED(styx::range_ok(q, heads * kv->head_dim * 4) && styx::range_ok(out, heads * kv->head_dim * 4) &&
              styx::range_ok(lse, lse ? heads * 4 : 0),
          "q / out / lse smaller than n_seqs x n_heads");
+    NEED(out == q || Span(q, heads * kv->head_dim * 4).apart(Span(out, heads * kv->head_dim * 4)), "out overlaps q in part");
     if (acc_out) {
         const uint64_t lines = static_cast<uint64_t>(kv->n_seqs) * kv->n_kv_heads * acc_stride * 4;
         NEED(kv->n_seqs * static_cast<int64_t>(kv->n_kv_heads) <= 65535, "accumulation: n_seqs x n_kv_heads <= 65535");   // lines x row blocks: a grid's x
         NEED(styx::range_ok(acc, lines) && styx::range_ok(acc_out, lines), "acc / acc_out smaller than n_seqs x n_kv_heads lines");
+        NEED(acc == acc_out || Span(acc, lines).apart(Span(acc_out, lines)), "acc_out overlaps acc in part");
     }
     const AttendWs w = attend_ws(kv, n_heads, acc_out != nullptr, sms);
     NEED(workspace_bytes >= w.total && styx::range_ok(workspace, w.total), "workspace: %llu bytes needed",

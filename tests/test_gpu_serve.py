@@ -763,3 +763,24 @@ def test_append_refuses_a_q_out_over_k_or_v():
     exp = kv.append(q, other, other, pos, 1e4)
     assert torch.equal(kv.append(q, buf[1024:].view(2, 2, 64), other, pos, 1e4, out=out), exp)   # beside it
     kv.ctx.check_device_error()
+
+
+def test_attend_refuses_weights_and_outputs_that_overlap_in_part():
+    """acc_out may be acc and out may be q, row for row; shifted against each other a block would read what another has
+    written."""
+    rng = np.random.default_rng(43)
+    kv, _, _ = make_cache(rng, [20, 30], 2, 64, 16, "f16")
+    q = T(queries(rng, 2, 8, 64))
+    acc = torch.zeros(2 * 2 * 32 + 8, device=DEV)
+    line = lambda at: acc[at:at + 128].view(2, 2, 32)        # noqa: E731
+    buf = torch.zeros(1024 + 64, device=DEV)
+    at = lambda i: buf[i:i + 1024].view(2, 8, 64)            # noqa: E731
+    at(0).copy_(q)
+    for call in (lambda: kv.attend(q, acc=line(0), acc_out=line(4)), lambda: kv.attend(q, acc=line(4), acc_out=line(0)),
+                 lambda: kv.attend(at(0), out=at(64)), lambda: kv.attend(at(64), out=at(0))):
+        with pytest.raises(StyxError, match="overlap") as e:
+            call()
+        assert e.value.code == _lib.STYX_EINVAL
+    exp = kv.attend(q)
+    assert torch.equal(kv.attend(at(0), out=at(0)), exp)
+    kv.ctx.check_device_error()
