@@ -295,12 +295,12 @@ int styx_paged_evict(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv,
              styx::range_ok(pos_out, lines) && styx::range_ok(next_pos, kv->n_seqs * 4ull) &&
              styx::range_ok(lens_out, kv->n_seqs * 4ull),
          "weights / positions / lengths smaller than n_seqs x n_kv_heads lines");
-    auto apart = [](const void *x, const void *y, uint64_t n) {
-        const char *p = static_cast<const char *>(x), *q = static_cast<const char *>(y);
-        return p + n <= q || q + n <= p;
-    };
-    NEED(apart(acc, acc_out, lines) && apart(pos, pos_out, lines) && apart(kv->lens, lens_out, kv->n_seqs * 4ull),
-         "acc_out, pos_out and lens_out must be other arrays than the inputs");
+    const Span outs[3] = {Span(acc_out, lines), Span(pos_out, lines), Span(lens_out, kv->n_seqs * 4ull)};
+    const Span ins[4] = {Span(acc, lines), Span(pos, lines), Span(next_pos, kv->n_seqs * 4ull), Span(kv->lens, kv->n_seqs * 4ull)};
+    for (int o = 0; o < 3; o++) {
+        for (const Span &i : ins) NEED(outs[o].apart(i), "acc_out, pos_out and lens_out must be other arrays than the inputs");
+        for (int p = 0; p < o; p++) NEED(outs[o].apart(outs[p]), "acc_out, pos_out and lens_out must be other arrays than each other");
+    }
     const EvictWs w = evict_ws(kv, budget);
     NEED(workspace_bytes >= w.total && aligned(workspace, 256) && styx::range_ok(workspace, w.total),
          "workspace: %llu bytes, 256-byte aligned, needed", static_cast<unsigned long long>(w.total));

@@ -784,3 +784,20 @@ def test_attend_refuses_weights_and_outputs_that_overlap_in_part():
     exp = kv.attend(q)
     assert torch.equal(kv.attend(at(0), out=at(0)), exp)
     kv.ctx.check_device_error()
+
+
+def test_evict_refuses_outputs_over_any_input_or_each_other():
+    rng = np.random.default_rng(44)
+    kv, _, _ = make_cache(rng, [20, 30], 2, 64, 16, "f16")
+    i32 = lambda *a: torch.tensor(a, dtype=torch.int32, device=DEV)   # noqa: E731
+    acc, pos, nxt = torch.rand(2, 2, 32, device=DEV), torch.zeros(2, 2, 32, dtype=torch.int32, device=DEV), i32(40, 40)
+    f = lambda t: t.view(torch.float32)                               # noqa: E731
+    i = lambda t: t.view(torch.int32)                                 # noqa: E731
+    out = torch.zeros(2, 2, 32, device=DEV)
+    for kw in (dict(acc_out=f(pos)), dict(pos_out=i(acc)), dict(acc_out=out, pos_out=i(out)), dict(lens_out=nxt),
+               dict(lens_out=pos.view(-1)[6:8]), dict(lens_out=i(acc).view(-1)[:2]), dict(lens_out=i(out).view(-1)[2:4], acc_out=out),
+               dict(lens_out=i(out).view(-1)[2:4], pos_out=i(out))):
+        with pytest.raises(StyxError, match="other arrays") as e:
+            kv.evict(acc, pos, nxt, 8, **kw)
+        assert e.value.code == _lib.STYX_EINVAL
+    kv.ctx.check_device_error()
