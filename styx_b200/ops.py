@@ -731,16 +731,18 @@ class PagedKV:
     rows on 148 SMs): not on two streams at once."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lens: torch.Tensor):
-        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.stride() != v.stride():
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or (k.shape[0] > 1 and k.stride(0) != v.stride(0)):
             raise ValueError("k and v: two pools [n_pages][n_kv_heads][page_size][head_dim] of one type and layout")
         if k.dtype not in _KV_TYPES:
             raise ValueError(f"cache type {k.dtype}: float32, float16 or bfloat16")
         n_pages, n_kv, page, hd = k.shape
-        if k.stride()[1:] != (page * hd, hd, 1):
-            raise ValueError(f"pages must be contiguous (strides {k.stride()})")
+        for t in (k, v):     # (the stride of a dimension of one says nothing)
+            if any(n > 1 and st != want for n, st, want in zip((n_kv, page, hd), t.stride()[1:], (page * hd, hd, 1))):
+                raise ValueError(f"pages must be contiguous (strides {t.stride()})")
         if not k.is_cuda or v.device != k.device:
             raise ValueError("styx ops take CUDA tensors")
-        if table.dim() != 2 or table.dtype != torch.int32 or table.stride(1) != 1 or table.device != k.device:
+        if table.dim() != 2 or table.dtype != torch.int32 or table.device != k.device or (
+                table.shape[1] > 1 and table.stride(1) != 1):
             raise ValueError("table: int32 [n_seqs][max_pages] with contiguous rows on the pools' device")
         self.k, self.v, self.table = k, v, table
         self.device, self.index = k.device, k.device.index
@@ -891,7 +893,8 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Optional[torch.Te
     [n] (styx_sample): temperature, top_k (int32), top_p and min_p are [n]
     tensors, None for 1, all, 1 and 0.  Returns (token int32 [n], logprob f32
     [n] under the distribution drawn from); token -1 where nothing is left."""
-    if logits.dim() != 2 or logits.dtype is not torch.float32 or not logits.is_cuda or logits.stride(1) != 1:
+    if logits.dim() != 2 or logits.dtype is not torch.float32 or not logits.is_cuda or (
+            logits.stride(1) != 1 and logits.shape[1] > 1):
         raise ValueError(f"logits: float32 [n][vocab] CUDA tensor with contiguous rows expected, got {logits.dtype} "
                          f"{tuple(logits.shape)} strides {logits.stride()} on {logits.device}")
     n, vocab = logits.shape

@@ -801,3 +801,24 @@ def test_evict_refuses_outputs_over_any_input_or_each_other():
             kv.evict(acc, pos, nxt, 8, **kw)
         assert e.value.code == _lib.STYX_EINVAL
     kv.ctx.check_device_error()
+
+
+def test_sizes_of_one_have_no_stride():
+    """One kv head, one page or one row a page: the strides of such a dimension say nothing about the layout."""
+    rng = np.random.default_rng(45)
+    lens = torch.tensor([3], dtype=torch.int32, device=DEV)
+    for n_pages, n_kv, page in ((4, 1, 16), (1, 2, 16), (4, 2, 1), (1, 1, 16), (1, 1, 4), (4, 1, 1)):
+        rows = min(3, n_pages * page)
+        lens.fill_(rows)
+        pool = [T(rng.normal(0, 1, (n_pages, n_kv, page, 64)).astype(np.float32)) for _ in range(2)]
+        table = torch.arange(n_pages, dtype=torch.int32, device=DEV)[None]
+        q = T(queries(rng, 1, 4, 64))
+        exp = ops.PagedKV(*pool, table, lens).attend(q)
+        size, dense = (n_pages, n_kv, page, 64), (n_kv * page * 64, page * 64, 64, 1)
+        odd = tuple(7777 if n == 1 else s for n, s in zip(size, dense))
+        k, v = pool[0].as_strided(size, odd), pool[1].as_strided(size, dense)
+        t = table.as_strided((1, n_pages), (1, 1 if n_pages > 1 else 55))
+        assert torch.equal(ops.PagedKV(k, v, t, lens).attend(q), exp)
+    x = T(rng.normal(0, 1, (5, 1)).astype(np.float32))
+    token, lp = ops.sample(x.as_strided((5, 1), (1, 9)), torch.zeros(5, device=DEV))
+    assert token.tolist() == [0] * 5 and lp.tolist() == [0.0] * 5
