@@ -4,7 +4,13 @@ under a row budget, eviction by accumulated attention weight.
 
     python -m styx_b200.serve MODEL.gguf --prompt 1,2,3 --prompt 7,8 -n 32
            [--temperature 0.7 --top-k 40 --top-p 0.95 --min-p 0.05 --seed 1]
-           [--cache f16] [--page 64] [--ctx 4096] [--budget 1024 --recent 128 --sinks 4]
+           [--cache f16] [--experts auto] [--page 64] [--ctx 4096] [--budget 1024 --recent 128 --sinks 4]
+
+The defaults hold fewer bits than the f32 of styx_b200.generate, for speed:
+K and V as f16 (half the bytes of the cache), and, where the experts' formats
+allow, their activations as f16 (grouped tensor-core GEMMs, each expert's
+weights read once a step).  --cache f32 --experts f32 undoes both: greedy
+tokens are then those of the single-sequence step.
 
 Per token of a step: the embedding rows, then per layer RMSNorm, q / k / v,
 styx_paged_append (norms, RoPE, the new row into its page), styx_paged_attend
@@ -229,6 +235,8 @@ def main(argv=None) -> int:
     ap.add_argument("--ctx", type=int, default=4096, help="rows a sequence's cache may hold")
     ap.add_argument("--page", type=int, default=64, help="rows of a page")
     ap.add_argument("--cache", choices=sorted(CACHE_TYPES), default="f16", help="element type of the cache")
+    ap.add_argument("--experts", choices=["auto", "f32"], default="auto",
+                    help="auto: f16 operands where the formats allow, else f32; f32: token by token")
     ap.add_argument("--budget", type=int, default=0, help="rows that stay per sequence and kv head (0: all)")
     ap.add_argument("--recent", type=int, default=128, help="of them: the last so many positions")
     ap.add_argument("--sinks", type=int, default=4, help="and the first so many")
@@ -247,7 +255,8 @@ def main(argv=None) -> int:
     model, keep = G.load_decode_model(g, 1, args.device)
     g.close()
     dec = BatchDecoder.of(model, len(prompts), args.ctx, page=args.page, cache=CACHE_TYPES[args.cache],
-                          budget=args.budget, n_recent=args.recent, n_sink=args.sinks, device=args.device)
+                          budget=args.budget, n_recent=args.recent, n_sink=args.sinks,
+                          moe_batch=False if args.experts == "f32" else None, device=args.device)
     t0 = time.perf_counter()
     out = dec.generate(prompts, args.n_predict, args.temperature, args.top_k, args.top_p, args.min_p, args.seed)
     t1 = time.perf_counter()

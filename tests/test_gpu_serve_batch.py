@@ -163,3 +163,15 @@ def test_a_refused_step_changes_nothing(kind):
     d.step(2)
     assert d.lens.tolist() == d.rows and d.rows[:2] == [5, 5]
     d.kv[0].ctx.check_device_error()
+
+
+def test_command_line_in_f32_gives_the_oracles_tokens(tmp_path, capsys):
+    m = make_model(0)
+    path = str(tmp_path / "m.gguf")
+    write_gguf(m, path)
+    argv = [path, "-n", "12", "--ctx", "64", "--cache", "f32", "--experts", "f32"]
+    for p in PROMPTS:
+        argv += ["--prompt", ",".join(map(str, p))]
+    assert serve.main(argv) == 0
+    out = [[int(t) for t in o.split(",")] for o in capsys.readouterr().out.split()]
+    assert out == [oracle_greedy(m, p, 12) for p in PROMPTS]
