@@ -822,3 +822,78 @@ def test_sizes_of_one_have_no_stride():
     x = T(rng.normal(0, 1, (5, 1)).astype(np.float32))
     token, lp = ops.sample(x.as_strided((5, 1), (1, 9)), torch.zeros(5, device=DEV))
     assert token.tolist() == [0] * 5 and lp.tolist() == [0.0] * 5
+
+
+# ------------------------------------------------------------ shapes that the tests above do not reach
+@pytest.mark.parametrize("vocab,rows,kind", [(262145, 14, "plain"), (300001, 14, "ties"), (270000, 14, "mask"),
+                                             (270001, 14, "low"), (400000, 14, "nan"), (1 << 20, 7, "plain")])
+def test_sample_vocabularies_beyond_a_cluster(vocab, rows, kind):
+    """One CTA per row and radix selection, on ordinary rows: every setting, ties at the threshold, masks, NaN."""
+    test_sample(vocab, rows, kind)
+
+
+def test_sample_beyond_a_cluster_draws_what_the_cluster_draws():
+    """The same rows with and without a tail of -inf that no filter keeps: one token, one logprob (sums of whole
+    numbers do not depend on the form)."""
+    rng = np.random.default_rng(51)
+    rows, v = 28, 200000
+    x = np.round(rng.normal(0, 3, (rows, v)) * 4).astype(np.float32) / 4
+    par = [SETTINGS[i % len(SETTINGS)] for i in range(rows)]
+    t, k, p, m = (T(np.array([q[i] for q in par], np.int32 if i == 1 else np.float32)) for i in range(4))
+    u = T(rng.uniform(0, 1, rows).astype(np.float32))
+    a = ops.sample(T(x), u, t, k, p, m)
+    b = ops.sample(T(np.concatenate([x, np.full((rows, 70000), -np.inf, np.float32)], 1)), u, t, k, p, m)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("which", ["q", "k"])
+@pytest.mark.parametrize("hd,heads,n_kv", [(128, 9, 3), (12, 5, 1), (64, 4, 4)])
+def test_append_with_one_norm_alone(hd, heads, n_kv, which):
+    rng = np.random.default_rng(52)
+    kv, _, _ = make_cache(rng, [9, 30, 31], n_kv, hd, 16, "f32")
+    q, k, v = (rng.normal(0, 2, (3, h, hd)).astype(np.float32) for h in (heads, n_kv, n_kv))
+    w, pos = rng.uniform(0.5, 1.5, hd).astype(np.float32), np.array([8, 29, 100000], np.int32)
+    qn, kn = (w, None) if which == "q" else (None, w)
+    got = kv.append(T(q), T(k), T(v), T(pos), 1e4, q_norm=None if qn is None else T(qn), k_norm=None if kn is None else T(kn))
+    close(got.cpu().numpy(), rope_norm_ref(q.astype(np.float64), qn, pos, 1e4, 1e-6), 2e-6)
+    ek = rope_norm_ref(k.astype(np.float64), kn, pos, 1e4, 1e-6)
+    for b, r in enumerate((8, 29, 30)):
+        rk, rv = read_rows(kv, b, r + 1)
+        close(rk[r], ek[b], 2e-6)
+        assert np.array_equal(rv[r], v[b].astype(np.float64))
+    kv.ctx.check_device_error()
+
+
+@pytest.mark.parametrize("dtype,heads,window", [("bf16", 64, 100), ("f16", 64, 17), ("bf16", 32, 1)])
+def test_attend_windows_with_a_share_per_team(dtype, heads, window):
+    """More segments than SMs, a window that begins inside a tile; with 16 heads two warps share each."""
+    lens = [int(n) for n in np.random.default_rng(53).integers(0, 400, 50)]
+    test_attend(lens, heads, 4, 128, 16, dtype, window)
+    test_attend_accumulates_the_weights(lens, heads, 4, 128, 16, dtype, window)
+
+
+@pytest.mark.parametrize("dtype,hd,page,gap", [("f16", 128, 16, 8), ("bf16", 64, 64, 4096), ("f32", 64, 16, 4)])
+def test_pages_further_apart_than_their_size(dtype, hd, page, gap):
+    rng = np.random.default_rng(54)
+    lens = [70, 5, 0, 33]
+    kv, ks, vs = make_cache(rng, lens, 2, hd, page, dtype, gap=gap)
+    assert kv.k.stride(0) == 2 * page * hd + gap
+    q = queries(rng, 4, 8, hd)
+    close(kv.attend(T(q)).cpu().numpy(), attend_ref(q, ks, vs, hd ** -0.5)[0], 1e-5)
+    acc = rng.exponential(1, (4, 2, kv.max_rows)).astype(np.float32)
+    pos = np.broadcast_to(np.arange(kv.max_rows, dtype=np.int32), acc.shape)
+    _, _, n = kv.evict(T(acc), T(pos), T(np.array(lens, np.int32)), 20, 4, 2)
+    assert n.tolist() == [20, 5, 0, 20]
+    for b, m in enumerate(lens):
+        if m:
+            gk, gv = read_rows(kv, b, min(m, 20))
+            for j in range(2):
+                src = evict_ref(acc[b, j], pos[b, j], m, m, 20, 4, 2)
+                assert np.array_equal(gk[:, j], ks[b][src, j]) and np.array_equal(gv[:, j], vs[b][src, j])
+    kv.lens = n
+    x = T(rng.normal(0, 1, (4, 2, hd)).astype(np.float32))
+    kv.append(None, x, x, torch.zeros(4, dtype=torch.int32, device=DEV), 1e4)
+    for b, m in enumerate(n.tolist()):
+        if m:
+            assert np.array_equal(read_rows(kv, b, m)[1][m - 1], x[b].to(TYPES[dtype]).double().cpu().numpy())
+    kv.ctx.check_device_error()
