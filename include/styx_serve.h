@@ -136,7 +136,8 @@ int styx_paged_evict(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv,
  * NaN logits count as -inf.  A row with nothing to draw from (all -inf)
  * gives token -1 and logprob -inf.  temperature, top_k, top_p, min_p: device
  * arrays of n_rows, each NULL for 1, all, 1 and 0; logprob may be NULL.
- * n_vocab <= 2^22. */
+ * n_vocab <= 2^22.  token and logprob may not overlap the inputs or each
+ * other; either may be u. */
 int styx_sample(styx_ctx *ctx, styx_stream stream, const float *logits, int64_t row_stride, int n_rows, int n_vocab,
                 const float *u, const float *temperature, const int32_t *top_k, const float *top_p,
                 const float *min_p, int32_t *token, float *logprob);

@@ -336,6 +336,16 @@ int styx_sample(styx_ctx *ctx, styx_stream stream, const float *logits, int64_t 
     NEED(rows_ok(logits, n_rows, row_stride, n_vocab, 4) && opt(u) && opt(temperature) && opt(top_k) && opt(top_p) &&
              opt(min_p) && opt(token) && opt(logprob),
          "logits or a per-row array smaller than n_rows");
+    // rows are ordered by all rows' settings: one that a finished row overwrites could order them differently for another
+    // (each row's u is read by that row alone, before its outputs are written)
+    const Span ins[5] = {Span(logits, n_rows, row_stride, n_vocab, 4), Span(temperature, n4), Span(top_k, n4), Span(top_p, n4),
+                         Span(min_p, n4)};
+    const Span outs[2] = {Span(token, n4), Span(logprob, n4)}, us(u, n4);
+    for (const Span &o : outs) {
+        for (const Span &i : ins) NEED(o.apart(i), "token or logprob overlaps an input");
+        NEED(o.begin == us.begin || o.apart(us), "token or logprob overlaps u in part");
+    }
+    NEED(outs[0].apart(outs[1]), "token overlaps logprob");
     a.logits = logits;
     a.row_stride = row_stride;
     a.n_rows = n_rows;

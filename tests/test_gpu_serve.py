@@ -897,3 +897,28 @@ def test_pages_further_apart_than_their_size(dtype, hd, page, gap):
         if m:
             assert np.array_equal(read_rows(kv, b, m)[1][m - 1], x[b].to(TYPES[dtype]).double().cpu().numpy())
     kv.ctx.check_device_error()
+
+
+def test_sample_refuses_outputs_over_its_inputs():
+    """All rows' settings are read to order the rows; u may be overwritten in place."""
+    n, v = 40, 500
+    rng = np.random.default_rng(55)
+    x, u = T(rng.normal(0, 2, (n, v)).astype(np.float32)), T(rng.uniform(0, 1, n).astype(np.float32))
+    one = lambda value: torch.full((n,), value, device=DEV)                     # noqa: E731
+    t, p, m, k = one(0.9), one(0.8), one(0.01), torch.full((n,), 30, dtype=torch.int32, device=DEV)
+    both = torch.zeros(2 * n, device=DEV)
+    i = lambda a: a.view(torch.int32)                                           # noqa: E731
+    for kw in (dict(token=k), dict(logprob=t), dict(logprob=p), dict(logprob=m), dict(token=i(t)), dict(logprob=k.view(torch.float32)),
+               dict(logprob=x.view(-1)[v * n - n:]), dict(token=i(x).view(-1)[:n]),
+               dict(token=i(both)[:n], logprob=both[n - 1:2 * n - 1])):
+        with pytest.raises(StyxError, match="overlaps") as e:
+            ops.sample(x, u, t, k, p, m, **kw)
+        assert e.value.code == _lib.STYX_EINVAL
+    shifted = both[:n]
+    shifted.copy_(u)
+    with pytest.raises(StyxError, match="overlaps"):
+        ops.sample(x, shifted, t, k, p, m, logprob=both[1:n + 1])
+    exp = ops.sample(x, u, t, k, p, m)
+    got = ops.sample(x, shifted, t, k, p, m, logprob=shifted)
+    assert torch.equal(got[0], exp[0]) and torch.equal(got[1], exp[1])
+    ops.ctx(0).check_device_error()
