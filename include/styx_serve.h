@@ -38,7 +38,9 @@ extern "C" {
  *   page * page_stride + (j * page_size + r % page_size) * head_dim
  * (a page holds one head's rows together).  Page ids are < n_pages; entries
  * past a sequence's rows are not read.  A sequence with lens[b] = 0 is an
- * empty slot.  Layers may share a pool and its tables with other k / v. */
+ * empty slot.  Layers may share a pool and its tables with other k / v.  table
+ * and lens may change between calls (of one stream, or ordered by an event), not
+ * while one runs. */
 typedef struct styx_paged_kv {
     void *k, *v;               /* pools, 16-byte aligned */
     int64_t page_stride;       /* elements from page to page, rows 16-byte aligned */

@@ -92,6 +92,11 @@ int check_kv(const styx_paged_kv *kv, bool with_buffers, styx::PagedKv &o) {
     o.table_stride = kv->table_stride;
     return STYX_OK;
 }
+// warps find their work from lens and the table, each for itself: one that changed in between would part them at a barrier
+bool clear_of_lengths(const styx_paged_kv *kv, const Span &o) {
+    return o.apart(Span(kv->lens, kv->n_seqs * 4ull)) &&
+           o.apart(Span(kv->table, kv->n_seqs, kv->table_stride, kv->max_pages, 4));
+}
 uint64_t max_rows(const styx_paged_kv *kv) { return static_cast<uint64_t>(kv->max_pages) * kv->page_size; }
 
 // attend's workspace: the finished portions of every (sequence, kv head,
@@ -247,6 +252,10 @@ int styx_paged_attend(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv
     const AttendWs w = attend_ws(kv, n_heads, acc_out != nullptr, sms);
     NEED(workspace_bytes >= w.total && styx::range_ok(workspace, w.total), "workspace: %llu bytes needed",
          static_cast<unsigned long long>(w.total));
+    NEED(clear_of_lengths(kv, Span(out, heads * kv->head_dim * 4)) && clear_of_lengths(kv, Span(lse, heads * 4)) &&
+             clear_of_lengths(kv, Span(acc_out, static_cast<uint64_t>(kv->n_seqs) * kv->n_kv_heads * acc_stride * 4)) &&
+             clear_of_lengths(kv, Span(workspace, w.total)),
+         "an output or the workspace overlaps lens or the table");
     char *ws = static_cast<char *>(workspace);
     a.q = q;
     a.out = out;
@@ -304,6 +313,9 @@ int styx_paged_evict(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv,
     const EvictWs w = evict_ws(kv, budget);
     NEED(workspace_bytes >= w.total && aligned(workspace, 256) && styx::range_ok(workspace, w.total),
          "workspace: %llu bytes, 256-byte aligned, needed", static_cast<unsigned long long>(w.total));
+    NEED(clear_of_lengths(kv, outs[0]) && clear_of_lengths(kv, outs[1]) && clear_of_lengths(kv, outs[2]) &&
+             clear_of_lengths(kv, Span(workspace, w.total)),
+         "an output or the workspace overlaps lens or the table");
     char *ws = static_cast<char *>(workspace);
     a.acc = acc;
     a.pos = pos;

@@ -922,3 +922,29 @@ def test_sample_refuses_outputs_over_its_inputs():
     got = ops.sample(x, shifted, t, k, p, m, logprob=shifted)
     assert torch.equal(got[0], exp[0]) and torch.equal(got[1], exp[1])
     ops.ctx(0).check_device_error()
+
+
+def test_outputs_over_lengths_or_table_are_refused():
+    rng = np.random.default_rng(56)
+    kv, _, _ = make_cache(rng, [20, 30], 2, 64, 16, "f16")
+    room = torch.zeros(8192, dtype=torch.int32, device=DEV)
+    lens, table = room[512:514], room[1024:1024 + kv.table.numel()].view(kv.table.shape)
+    lens.copy_(kv.lens)
+    table.copy_(kv.table)
+    over = ops.PagedKV(kv.k, kv.v, table, lens)
+    f = lambda at, *shape: room[at:at + int(np.prod(shape))].view(shape).view(torch.float32)   # noqa: E731
+    i = lambda at, *shape: room[at:at + int(np.prod(shape))].view(shape)                       # noqa: E731
+    q = T(queries(rng, 2, 8, 64))
+    acc, pos, nxt = torch.rand(2, 2, 32, device=DEV), torch.zeros(2, 2, 32, dtype=torch.int32, device=DEV), T(np.array([40, 40], np.int32))
+    for call in (lambda: over.attend(q, out=f(0, 2, 8, 64)), lambda: over.attend(q, out=f(1024, 2, 8, 64)),
+                 lambda: over.attend(q, lse=f(500, 2, 8)), lambda: over.attend(q, acc=acc, acc_out=f(400, 2, 2, 32)),
+                 lambda: over.attend(q, acc=acc, acc_out=f(1020, 2, 2, 32)),
+                 lambda: over.evict(acc, pos, nxt, 8, acc_out=f(1020, 2, 2, 32)), lambda: over.evict(acc, pos, nxt, 8, pos_out=i(1020, 2, 2, 32)),
+                 lambda: over.evict(acc, pos, nxt, 8, lens_out=i(1024, 2))):
+        with pytest.raises(StyxError, match="lens or the table") as e:
+            call()
+        assert e.value.code == _lib.STYX_EINVAL
+    with pytest.raises(StyxError, match="other arrays"):
+        over.evict(acc, pos, nxt, 8, acc_out=f(400, 2, 2, 32))
+    assert torch.equal(over.attend(q, out=f(4096, 2, 8, 64)), kv.attend(q))
+    kv.ctx.check_device_error()
