@@ -130,11 +130,13 @@ int styx_paged_evict(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv,
  *   top_k: the k first tokens by (larger x, lower index); 0 or less: all;
  *   top_p: of those, in that order, the fewest whose W reach
  *          rint(p * 2^24) / 2^24 of their sum (one at least);
- *   min_p: of those, w[i] >= min_p;
+ *   min_p: of those, w[i] >= min_p (above 1, or NaN: as 1, the maximum and its
+ *          equals stay);
  *   token: the first kept i with sum of kept W up to and with i >
  *          floor(floor(u 2^24) S / 2^24), S the sum of all kept;
  *   logprob = (x - m) / temperature - log(S / 2^40).
- * temperature <= 0 takes the maximum (lowest index among equals; logprob 0).
+ * temperature <= 0 (or NaN) takes the maximum (lowest index among equals;
+ * logprob 0).
  * NaN logits count as -inf.  A row with nothing to draw from (all -inf)
  * gives token -1 and logprob -inf.  temperature, top_k, top_p, min_p: device
  * arrays of n_rows, each NULL for 1, all, 1 and 0; logprob may be NULL.

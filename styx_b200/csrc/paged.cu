@@ -225,10 +225,11 @@ __device__ __forceinline__ unsigned cta_scan(unsigned v, unsigned *sh, unsigned 
 // line of 2176 rows, scans tile by tile as many; counting 16 steps at once in
 // registers made the whole call 28 us instead of 22, since weights spread over
 // many exponents and then take eight rounds.)
-// Bound by the chain of exchanges, not by bytes: with the moves, 18.4 us from
+// Bound by the chain of exchanges, not by bytes: with the moves, 18.3 us from
 // 32768 rows to 4096 (one sequence, 4 kv heads; 2.5 us at HBM's rate: keys 4,
-// threshold 7, numbering 1.5, places 2), 19.4 us for 32 sequences from 2176 to
-// 2048 (3.1; keys 2.5, threshold 4, numbering 1, moves 5, two launches).
+// threshold 7, numbering 1.5, places 2), 19.2 us for 32 sequences from 2176 to
+// 2048 (3.1; keys 2.5, threshold 4, numbering 1, moves 5, two launches), in a
+// graph over one state; 21 and 20 as called over several.
 template <bool STAGED>
 __global__ void __launch_bounds__(kEvThreads) k_evict_select(PagedEvictArgs a, int C) {
     extern __shared__ uint32_t staged[];

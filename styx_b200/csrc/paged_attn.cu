@@ -3,19 +3,22 @@
 //
 // k_attend_fma.  CTA (an equal share of the tile list, paged_split.cuh): eight
 // warps take rows in turn, LPR lanes per row with eight elements each, so that
-// q (8 heads x 8 elements) and O stay in registers and K and V are read once.
+// q (8 heads x 8 elements) and O stay in registers and K and V are read once
+// per eight q heads (with more of them per kv head, once per group of eight).
 // A lane copies exactly the bytes that it will use itself (cp.async into a
 // ring of its own), so no barrier is needed between copy and use and 128 KB
 // or more per SM are in flight.  The 8 heads' dot products are summed over
 // the row's lanes by halving exchanges, which leave each lane one head's
 // score; maxima move only when a score passes them by 2^8.  A lane has two
 // rows at once, whose exchanges overlap.
-// Measured (B200): 8 sequences, the last 2048 f32 rows of 32 / 4 heads of 128
-// (64 MB) in 21.5 us, with the finish: 2 us until a CTA knows its share, 4 for
-// pages, q and the first copies, 11 of rows (issue and exchanges, not memory:
-// 16-bit rows cost as much), 2 for the result, 2 for the finish.  One row at a
-// time and tiles of 128 rows: 27 us (some CTAs had four times the work of
-// others); pages one by one and q by 4 bytes: 31 us.
+// Measured (B200): 8 sequences (one empty, two shorter), the last 2048 f32 rows
+// of 32 / 4 heads of 128 (52.7 MB) in 22.4 us in a graph over one state, which
+// then lies in L2, 25 as called over several.  Of the first, with the finish:
+// 2 us until a CTA knows its share, 4 for pages, q and the first copies, 11 of
+// rows (issue and exchanges, not memory: 16-bit rows cost as much), 2 for the
+// result, 2 for the finish.  One row at a time and tiles of 128 rows: 27 us
+// (some CTAs had four times the work of others); pages one by one and q by 4
+// bytes: 31 us.
 #include <cuda_runtime.h>
 
 #include <cstdint>

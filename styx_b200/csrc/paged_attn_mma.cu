@@ -32,7 +32,7 @@
 // up together, are issued before the last one's result is written.
 //
 // Measured (B200): one sequence of 131071 f16 rows, 32 / 4 heads of 128, 268 MB
-// in 50 us (5.3 TB/s; DRAM 66 % busy, tensor pipe 19 %, issue 33 %); twice as
+// in 50 us (5.3 TB/s; DRAM 66 % busy, tensor pipe 19 %, issue 34 %); twice as
 // many rows 5.7 to 5.9 TB/s, what cp.async reaches here.  Bound by HBM with up
 // to eight heads per kv head.  With 16 (bf16, 64 ragged sequences, 549 MB) 117
 // us, bound by the latency of eight warps' MMAs and exchanges: as CTAs with

@@ -20,7 +20,10 @@
 //     there are at most 2048 they go to the first CTA as above; else only that
 //     step's tokens go there and the threshold comes back.  Top-p after such
 //     a top-k is a second histogram, of the tokens kept.  Only more than 2048
-//     tokens in one step (a flat row) are resolved by bisection of the key.
+//     tokens in one step (a flat row, or very many tokens at a high temperature)
+//     are resolved by bisection of the key, up to 32 passes over the slices with
+//     a cluster barrier each: a flat row of 151936 with top-p 0.5 251 us, 64 of
+//     them 791; 200000 tokens of spread 1 at temperature 3, top-p 0.5, 371 us.
 //   the draw, where it is not the first CTA's: sums of the kept weights per
 //     warp, each over a stretch of indexes of its own, then inside one warp.
 // Measured (B200, vocabulary 151936): one row with top-k 20 and top-p 0.95 in
@@ -32,7 +35,9 @@
 // weights by F2I and sums per round of the CTA made the draw of an unfiltered
 // row 18000 of 34000 cycles.)
 //
-// k_sample (larger vocabularies): one CTA per row, radix selection from L2.
+// k_sample (larger vocabularies): one CTA per row, radix selection from L2, the
+// row read up to twelve times.  300000 tokens: 1.0 ms unfiltered, 4.7 to 4.9
+// greedy, with top-k or top-p; 64 rows 1.7 and 8.0 to 8.4 ms.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -962,7 +967,8 @@ cudaError_t launch_sample(const SampleArgs &a, cudaStream_t st) {
     at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 2;
-    // (two CTAs fit an SM: more than 32 clusters are more than one wave)
+    // (up to 163840 logits two CTAs fit an SM, and more than 32 clusters are more than one wave; beyond that one fits,
+    // and 19 to 32 rows, more than a wave too, are taken in the order given)
     return cudaLaunchKernelEx(&cfg, k_sample_cluster, a, region, bulk, a.n_rows > 32 && a.n_rows <= kNT);
 }
 

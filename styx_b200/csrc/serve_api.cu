@@ -106,8 +106,9 @@ struct AttendWs {
     uint64_t cnt, part, ml, scores, total;
 };
 // the tensor cores take 16-bit rows of up to 128 elements in pages of 16 rows
-// or more (a warp's 16 rows then lie together); everything else runs on the
-// FMA units.  Where both could (32 / 4 heads of 128): 37 rows 6.4 us against
+// or more (a warp's 16 rows then lie together; its ring, and q and O in its
+// registers, are laid out for rows of up to 256 bytes); everything else runs on
+// the FMA units.  Where both could (32 / 4 heads of 128): 37 rows 6.4 us against
 // 9.7, one sequence of 131071 f16 rows 50 against 117, 32 ragged bf16 ones 34
 // against 75, 64 of 64 / 4 heads 117 against 448
 bool on_tensor_cores(const styx_paged_kv *kv) {
