@@ -92,7 +92,9 @@ int styx_paged_append(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv
  *     with nothing to be cleared first).  acc_out may be acc, and out may be
  *     q; no other overlap of these.
  * The workspace (styx_paged_attend_workspace_bytes, 256-byte aligned) holds
- * the splits' partial sums and their counters: initialise it once.  Calls
+ * the splits' partial sums and their counters, and with acc a score of 4 bytes
+ * for every q head of every row that the table has room for (n_seqs x n_heads x
+ * max_pages x page_size): initialise it once.  Calls
  * that share one must not run at the same time. */
 int styx_paged_attend_workspace_bytes(styx_ctx *ctx, const styx_paged_kv *kv, int n_heads, int with_acc,
                                       uint64_t *out);
