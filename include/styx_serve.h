@@ -103,6 +103,113 @@ int styx_paged_attend(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv
                       float scale, int window, float *out, float *lse, const float *acc, float *acc_out,
                       int64_t acc_stride, void *workspace, uint64_t workspace_bytes);
 
+/* ------------------------------------------------- prompts in chunks
+ * Many new tokens of many sequences in one pass: styx_paged_plan says which
+ * rows and pages they get, styx_paged_append(_rope) writes them,
+ * styx_paged_attend_chunk reads them. */
+
+/* Pages and lengths of n_seqs sequences of one pool, all device memory:
+ * sequence b has lens[b] rows in the first held[b] entries of its line of the
+ * table; free[0 .. *n_free - 1] is the stack of pages that nobody has (room
+ * for n_pages). */
+typedef struct styx_page_table {
+    int32_t *table;            /* [n_seqs][table_stride] */
+    int32_t *free;             /* [n_pages] */
+    const int32_t *n_free;     /* [1] */
+    const int32_t *lens;       /* [n_seqs] */
+    const int32_t *held;       /* [n_seqs] */
+    int32_t n_seqs, max_pages, table_stride;
+    int32_t page_size;         /* rows, a power of two, <= 4096 */
+    int32_t n_pages;
+} styx_page_table;
+
+/* The next tokens of every sequence, sequence after sequence, as far as
+ * n_tokens and the pages go.  In the order of the sequences
+ *   t[b] = min(want[b] (negative: 0), rows the table has left for b,
+ *              what the t of those before leave of n_tokens);
+ *   pages past the first ceil((lens + t) / page_size) go onto the stack; what
+ *   is missing to as many is taken from its top (after all those returned),
+ *   as far as the stack goes;
+ *   granted[b] = min(t[b], rows of the pages that b has now).
+ * So want 0 with lens 0 (a finished request), or a length lowered by
+ * styx_paged_evict, gives pages back.  Written are
+ *   start[n_seqs + 1]: the granted tokens of b are start[b] .. start[b+1] - 1;
+ *   seq, row, pos [n_tokens]: of every token, as styx_paged_append takes them,
+ *     pos counting on from next_pos[b] (next_pos NULL: the row); past
+ *     start[n_seqs] they are 0, -1 and 0 (padding that writes no row);
+ *   lens_out = lens + granted, held_out, *n_free_out, next_pos_out =
+ *     next_pos + granted (NULL with next_pos): each may be its input, no other
+ *     overlap; the table's and the stack's entries that change.
+ * Inputs that stay may be used again: with the same ones, table and stack
+ * included, the call gives the same results.  A sequence whose length or pages
+ * contradict each other or the table is left as it is, granted nothing, and
+ * reported by styx_check_device_error. */
+int styx_paged_plan(styx_ctx *ctx, styx_stream stream, const styx_page_table *pt, const int32_t *want, int n_tokens,
+                    const int32_t *next_pos, int32_t *start, int32_t *seq, int32_t *row, int32_t *pos,
+                    int32_t *lens_out, int32_t *held_out, int32_t *n_free_out, int32_t *next_pos_out);
+
+/* Rotary frequencies, in radians per position, of the n_dims / 2 pairs:
+ *   f[i] = base^(-2i/n_dims), / factors[i] where there are factors (host
+ *          array), then by `scaling`:
+ *   STYX_ROPE_LINEAR  f / factor
+ *   STYX_ROPE_YARN    f (1 - r) + r f / factor with r = clamp((i - lo) /
+ *          max(hi - lo, 0.001), 0, 1), lo = max(0, floor d(beta_fast)), hi =
+ *          min(n_dims - 1, ceil d(beta_slow)), d(turns) = n_dims ln(orig_ctx /
+ *          (2 pi turns)) / (2 ln base); *magnitude = 1 + 0.1 ln(factor)
+ * (else *magnitude = 1).  Host only: freq is a host array of n_dims / 2. */
+#define STYX_ROPE_NONE 0
+#define STYX_ROPE_LINEAR 1
+#define STYX_ROPE_YARN 2
+typedef struct styx_rope_params {
+    int32_t n_dims;            /* even */
+    int32_t scaling;
+    double base, factor, orig_ctx, beta_fast, beta_slow;   /* factor and what follows: as `scaling` needs them */
+} styx_rope_params;
+int styx_rope_freqs(const styx_rope_params *params, const float *factors, double *freq, float *magnitude);
+
+/* How a head is turned: of its first n_dims elements the pairs (i, i +
+ * n_dims / 2) (interleaved 0) or (2i, 2i + 1) (1) by pos * freq[i], then times
+ * magnitude; the others stay as they are. */
+typedef struct styx_rope {
+    const double *freq;        /* device [n_dims / 2], radians per position */
+    int32_t n_dims;            /* even, <= head_dim */
+    int32_t interleaved;
+    float magnitude;
+} styx_rope;
+
+/* styx_paged_append with any rotary form, and q_out (16-byte aligned) in
+ * q_type: STYX_F32 or the cache's type (rounded once, from f32). */
+int styx_paged_append_rope(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv, int n_tokens, int n_heads,
+                           const float *q, int64_t q_stride, const float *k, int64_t k_stride, const float *v,
+                           int64_t v_stride, const float *q_norm, const float *k_norm, float eps,
+                           const styx_rope *rope, const int32_t *pos, const int32_t *seq, const int32_t *row,
+                           int q_type, void *q_out);
+
+/* Causal attention of new tokens: token t of start[b] <= t < start[b + 1]
+ * (device [n_seqs + 1], as styx_paged_plan gives it) is row
+ * r(t) = lens[b] - (start[b + 1] - t) of sequence b, and
+ *   out[t][h] = sum_r p[r] V[r], p = softmax of scale * q[t][h] . K[r] over the
+ *   rows r(t) - window < r <= r(t) (window 0: r <= r(t)).
+ * q [n_tokens][n_heads][head_dim], tokens q_stride elements apart, and out
+ * (contiguous) are of q_type: STYX_F32 (computed to f32's precision whatever
+ * the cache's type) or the cache's 16-bit type (p rounded to it once, sums in
+ * f32, out rounded once); both 16-byte aligned, q_stride a multiple of 16
+ * bytes.  lse (may be NULL): f32 [n_tokens][n_heads], log of the softmax's sum.
+ * Rows of out and lse outside all sequences' tokens stay as they are.  Rows
+ * that a token does not see are not used, whatever they hold.  A NaN in q or in
+ * a row of K that is seen makes the head's output NaN; one in V, or an
+ * infinity, that element of it (an infinity: infinite or NaN).
+ * A sequence whose tokens are no ascending range of [0, n_tokens), or more than
+ * its rows, is skipped, a page outside the pool likewise (its rows are not
+ * seen); both are reported by styx_check_device_error.
+ * The workspace (256-byte aligned) needs no initialisation.  Calls that share
+ * one must not run at the same time.  out may not overlap q, nor out or lse
+ * what the call reads. */
+int styx_paged_chunk_workspace_bytes(styx_ctx *ctx, const styx_paged_kv *kv, int n_heads, int q_type, uint64_t *out);
+int styx_paged_attend_chunk(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv, int n_tokens, int n_heads,
+                            int q_type, const void *q, int64_t q_stride, const int32_t *start, float scale, int window,
+                            void *out, float *lse, void *workspace, uint64_t workspace_bytes);
+
 /* Brings every sequence down to at most `budget` rows, per kv head.  Of the
  * n = lens[b] rows those stay that come first by
  *   protected rows: pos[r] >= next_pos[b] - n_recent or pos[r] < n_sink,

@@ -20,6 +20,7 @@ STYX_OK, STYX_EINVAL, STYX_ECUDA, STYX_ENOMEM, STYX_ETIMEOUT, STYX_EUNSUPPORTED 
 STYX_EIO, STYX_EEOF, STYX_EDATA = -6, -7, -8
 F32, Q8_0, Q4_K, Q5_K, Q6_K = 0, 8, 12, 13, 14
 F16, BF16 = 1, 30
+ROPE_NONE, ROPE_LINEAR, ROPE_YARN = 0, 1, 2
 QTYPES = {"q8_0": Q8_0, "q4_K": Q4_K, "q5_K": Q5_K, "q6_K": Q6_K}
 BLOCK = {Q8_0: (32, 34), Q4_K: (256, 144), Q5_K: (256, 176), Q6_K: (256, 210)}
 SKIP = 0xFFFFFFFF
@@ -75,6 +76,21 @@ class AttnDims(C.Structure):
 class AttnLayer(C.Structure):
     _fields_ = [("attn_norm", C.c_void_p), ("wq", DenseTensor), ("wk", DenseTensor), ("wv", DenseTensor),
                 ("wo", DenseTensor), ("q_norm", C.c_void_p), ("k_norm", C.c_void_p)]
+
+
+class PageTable(C.Structure):
+    _fields_ = [("table", C.c_void_p), ("free", C.c_void_p), ("n_free", C.c_void_p), ("lens", C.c_void_p),
+                ("held", C.c_void_p), ("n_seqs", C.c_int32), ("max_pages", C.c_int32), ("table_stride", C.c_int32),
+                ("page_size", C.c_int32), ("n_pages", C.c_int32)]
+
+
+class RopeParams(C.Structure):
+    _fields_ = [("n_dims", C.c_int32), ("scaling", C.c_int32), ("base", C.c_double), ("factor", C.c_double),
+                ("orig_ctx", C.c_double), ("beta_fast", C.c_double), ("beta_slow", C.c_double)]
+
+
+class RopeForm(C.Structure):
+    _fields_ = [("freq", C.c_void_p), ("n_dims", C.c_int32), ("interleaved", C.c_int32), ("magnitude", C.c_float)]
 
 
 class PagedKv(C.Structure):
@@ -203,6 +219,13 @@ _SIGS = {
     "styx_paged_evict": (_i, [_vp, _vp, C.POINTER(PagedKv), _vp, _vp, _vp, C.c_int64, _i, _i, _i, _vp, _vp, _vp, _vp,
                               _u64]),
     "styx_sample": (_i, [_vp, _vp, _vp, C.c_int64, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "styx_paged_plan": (_i, [_vp, _vp, C.POINTER(PageTable), _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "styx_rope_freqs": (_i, [C.POINTER(RopeParams), _vp, _vp, C.POINTER(_f)]),
+    "styx_paged_append_rope": (_i, [_vp, _vp, C.POINTER(PagedKv), _i, _i, _vp, C.c_int64, _vp, C.c_int64, _vp, C.c_int64,
+                                    _vp, _vp, _f, C.POINTER(RopeForm), _vp, _vp, _vp, _i, _vp]),
+    "styx_paged_chunk_workspace_bytes": (_i, [_vp, C.POINTER(PagedKv), _i, _i, C.POINTER(_u64)]),
+    "styx_paged_attend_chunk": (_i, [_vp, _vp, C.POINTER(PagedKv), _i, _i, _i, _vp, C.c_int64, _vp, _f, _i, _vp, _vp, _vp,
+                                     _u64]),
 }
 
 _lib = None

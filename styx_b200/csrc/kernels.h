@@ -404,6 +404,38 @@ struct PagedAttendArgs {
 };
 // floats of a portion's result: O [heads][pitch], 16 maxima, 16 sums
 constexpr int attend_part(int heads, int pitch) { return heads * pitch + 32; }
+// the next tokens of every sequence, their rows and pages (paged_plan.cu)
+struct PagedPlanArgs {
+    int32_t *table, *free;                     // pages of the sequences; stack of the others
+    const int32_t *want, *lens, *held, *n_free, *next_pos;   // next_pos may be null
+    int32_t *start, *seq, *row, *pos, *lens_out, *held_out, *n_free_out, *next_pos_out;
+    long long table_stride;
+    int n_seqs, max_pages, page_shift, n_pages, n_tokens;
+    int own_maps;                              // the planning kernel writes seq, row and pos itself
+    int *err;
+};
+// what append_rope takes beside PagedAppendArgs (whose log2_base, step and q_out are not used)
+struct PagedRope {
+    const double *freq;                        // device [n_dims / 2], radians per position
+    int n_dims, interleaved;
+    float magnitude;
+};
+struct PagedChunkArgs {
+    PagedKv kv;
+    const void *q;                             // [n_tokens][n_heads][hd]
+    void *out;
+    float *lse;                                // may be null
+    const int32_t *start;                      // device [n_seqs + 1]
+    long long q_stride;                        // elements between tokens
+    float scale;
+    int window, n_tokens, n_heads, gqa;
+    int q16;                                   // q and out are of the cache's 16-bit type
+    // the launch's cut of the work, see paged_chunk.cuh
+    int hg, groups, heads;                     // heads of a tile; groups of a kv head; kv heads x groups
+    int tok_shift, key_shift, seg_cost, workers, part_floats;
+    float *part;                               // workspace
+    void *joins;                               // workspace, one ChunkJoin per worker
+};
 struct PagedEvictArgs {
     PagedKv kv;
     const float *acc;
@@ -438,6 +470,11 @@ cudaError_t launch_attend_finish(const PagedAttendArgs &a, int nh, int pitch, cu
 int attend_grid(const PagedAttendArgs &a, int nh, int sms);
 uint64_t attend_fma_parts(int sms);            // bytes of the portions' results
 uint64_t attend_mma_parts(int gqa, int sms);
+cudaError_t launch_paged_plan(PagedPlanArgs a, cudaStream_t st);
+cudaError_t launch_paged_append_rope(const PagedAppendArgs &a, const PagedRope &r, void *q_out, bool q16, int sms, cudaStream_t st);
+// attention of chunks on mma.sync: 16-bit caches, f32 caches; bytes of their portions' results
+cudaError_t launch_chunk_mma(PagedChunkArgs a, int sms, cudaStream_t st);
+uint64_t chunk_mma_parts(const PagedKv &kv, int sms);
 cudaError_t launch_paged_evict(const PagedEvictArgs &a, int sms, cudaStream_t st);
 bool evict_staged(long long rows);   // the keys of lines of so many rows fit shared memory
 cudaError_t launch_sample(const SampleArgs &a, cudaStream_t st);

@@ -1,0 +1,784 @@
+// paged_chunk.cu -- causal attention of every sequence's new tokens over its
+// paged rows (styx_paged_attend_chunk) on mma.sync: caches of every type,
+// head_dim up to 256, pages of any size.
+//
+// A CTA takes M rows of queries (tokens x the q heads of a kv head), 16 per
+// warp, over tiles of keys that cp.async brings two stages deep; scores,
+// softmax and the weights of a tile stay in the warp's registers:
+//   S = Q K^T,   m' = max(m, rowmax S),   P = 2^(S - m'),
+//   O = O 2^(m - m') + P V,   l likewise
+// and a portion that does not cover its segment writes (O, m, l) for
+// k_chunk_join, which adds the portions up in order.
+//
+// k_chunk_mma, 16-bit caches: q of the cache's type is one term; f32 q (and
+// then p too) is split into 2 (f16) or 3 (bf16) terms of the cache's type, 22 /
+// 24 bits, whose products are exact.  The MMA cuts its sums off instead of
+// rounding them, so a tile's P V is added to O by the FMA that rescales O.
+// k_chunk_tf32, f32 caches: both factors as two tf32 terms, the product of the
+// two small ones (2^-22 of the whole) left out.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <type_traits>
+
+#include "paged_chunk.cuh"
+
+namespace styx {
+namespace {
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool on) {   // off: zeros
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldm4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldm4t(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+template <bool BF>
+__device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (BF)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma8(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {   // tf32
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// f32 as two tf32 terms: the upper 11 significant bits, and the rest rounded to as many
+__device__ __forceinline__ void split_tf32(float x, uint32_t &hi, uint32_t &lo) {
+    hi = __float_as_uint(x) & 0xFFFFE000u;
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(x - __uint_as_float(hi)));
+}
+// a pair of values (low half: x) as sums of N terms of the type, largest first;
+// one term: rounded.  bf16, three: the f32's 24 significant bits cut into 8 + 8
+// + 8, exactly; f16, two: rounded to 11, the rest rounded to 11.
+template <bool BF, int N>
+__device__ __forceinline__ void split2(float x, float y, uint32_t (&t)[N]) {
+    if constexpr (N == 1) {
+        t[0] = BF ? [&] { const __nv_bfloat162 h = __floats2bfloat162_rn(x, y); return *reinterpret_cast<const uint32_t *>(&h); }()
+                  : [&] { const __half2 h = __floats2half2_rn(x, y); return *reinterpret_cast<const uint32_t *>(&h); }();
+    } else if constexpr (BF) {
+        uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            t[i] = __byte_perm(a, b, 0x7632);
+            const uint32_t c = __float_as_uint(__uint_as_float(a) - __uint_as_float(a & 0xFFFF0000u));
+            const uint32_t d = __float_as_uint(__uint_as_float(b) - __uint_as_float(b & 0xFFFF0000u));
+            a = c;
+            b = d;
+        }
+    } else {
+        const __half2 h = __floats2half2_rn(x, y);
+        const float2 f = __half22float2(h);
+        const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+        t[0] = *reinterpret_cast<const uint32_t *>(&h);
+        t[1] = *reinterpret_cast<const uint32_t *>(&l);
+    }
+}
+
+// a portion: its segment's tokens and heads, its keys [lo, hi)
+struct Portion {
+    int b, j, g0, ng, tok0, ntok, base;     // base: row of the segment's first token
+    int kb0, tiles, lo, hi;                 // first tile's first key, tiles
+    int free_lo, free_hi;                   // every token sees all keys in [free_lo, free_hi)
+    bool begins, ends;
+    const int32_t *table;
+    __device__ __forceinline__ void set(const PagedChunkArgs &a, const ChunkWalk &w) {
+        const Chunk c(a, w.b, false);
+        b = w.b;
+        j = w.head / a.groups;
+        g0 = (w.head - j * a.groups) * a.hg;
+        ng = min(a.hg, a.gqa - g0);
+        const int first = w.seg << a.tok_shift;
+        tok0 = c.tok0 + first;
+        ntok = max(1, min(1 << a.tok_shift, c.n - first));
+        base = c.base + first;
+        const int ft = c.first_tile(a, w.seg);
+        kb0 = (ft + w.t0) << a.key_shift;
+        tiles = w.t1 - w.t0;
+        lo = max(kb0, c.first_row(a, w.seg));
+        hi = static_cast<int>(min(static_cast<long long>(c.end_row(a, w.seg)), static_cast<long long>(ft + w.t1) << a.key_shift));
+        free_hi = base + 1;
+        free_lo = a.window > 0 ? max(0, base + ntok - a.window) : 0;
+        begins = w.t0 == 0;
+        ends = w.t1 == w.nt;
+        table = a.kv.table + static_cast<long long>(b) * a.kv.table_stride;
+    }
+    // query row i of the tile: its token and head, token -1 where there is none
+    __device__ __forceinline__ void row(const PagedChunkArgs &a, int i, int &tok, int &head) const {
+        tok = i / a.hg;
+        head = i - tok * a.hg;
+        if (tok >= ntok || head >= ng) tok = -1;
+    }
+};
+__device__ __forceinline__ long long out_row(const PagedChunkArgs &a, const Portion &P, int tok, int head) {
+    return static_cast<long long>(P.tok0 + tok) * a.n_heads + P.j * a.gqa + P.g0 + head;
+}
+// the portion's result of one query row goes to its output, or to the workspace
+template <int ROWS>
+__device__ __forceinline__ float *part_rows(const PagedChunkArgs &a, const Portion &P, int worker) {
+    return chunk_part(a, worker, P.begins);
+}
+// what k_chunk_join needs to know of the worker's first portion; later ones begin their segments
+__device__ __forceinline__ void note_join(const PagedChunkArgs &a, const Portion *P, const ChunkWalk &w, int worker, long long T,
+                                          long long G) {
+    ChunkJoin j{-1, 0, 0, 0};
+    if (P && !P->begins && P->ends) j = {chunk_owner(a, w, T, G), w.b, w.head, w.seg};
+    static_cast<ChunkJoin *>(a.joins)[worker] = j;
+}
+// the value, where V's element is not a finite number: what a sum that has it with a positive weight becomes
+__device__ __forceinline__ float not_finite(float v) { return fabsf(v) <= 3.4028234e38f ? 0.f : v; }
+
+// ------------------------------------------------------------ 16-bit caches
+template <int HD>
+struct Mma {
+    static constexpr int warps = HD > 128 ? 4 : 8, threads = 32 * warps, M = 16 * warps;
+    static constexpr int KT = HD > 128 ? 32 : 64;      // keys of a tile
+    static constexpr int pitch = HD * 2 + 16;          // bytes of a row in shared memory: an odd number of 16-byte groups
+    static constexpr int tile = KT * pitch;
+    static constexpr int smem(int terms) { return terms * M * pitch + 4 * tile; }
+};
+
+template <bool BF, int TERMS, int HD>
+__global__ void __launch_bounds__(Mma<HD>::threads, 1) k_chunk_mma(PagedChunkArgs a) {
+    using C = Mma<HD>;
+    using T = std::conditional_t<BF, __nv_bfloat16, __half>;
+    using TQ = std::conditional_t<TERMS == 1, T, float>;
+    constexpr int KT = C::KT, M = C::M, PITCH = C::pitch, NS = KT / 8, KS = HD / 16, CH = HD / 8, ROWS = C::threads / CH;
+    constexpr bool ROUND = C::threads % CH != 0;       // (HD 96: 12 chunks of a row)
+    constexpr float PSCALE = BF ? 1.f : 16384.f;       // f16 has few exponents: p in [0, 1] as p * 2^14
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ float s_scale[M];                       // f16 terms of f32 q: what a row's scores are in units of
+    __shared__ int s_poison, s_badpage;
+    const PagedKv &kv = a.kv;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hd = kv.hd;
+    const int lr = lane >> 2, lc = lane & 3;
+    const uint32_t sQ = smem_addr(smem), sK = sQ + TERMS * M * PITCH, sV = sK + 2 * C::tile;
+    uint8_t *const kmem = smem + TERMS * M * PITCH;
+    const float l2 = a.scale * 1.4426950408889634f;    // scores in units of log2
+    pdl_trigger();
+    pdl_wait();
+    long long T_, G = 0;
+    ChunkWalk wk;
+    const int worker = blockIdx.x;
+    chunk_share(a, worker, wk, T_, G);
+    if (tid == 0) s_poison = s_badpage = 0;
+    Portion P{};
+    bool first = true;
+
+    auto load_tile = [&](int it, int stage) {
+        const int kb = P.kb0 + it * KT;
+        if (it < P.tiles) {
+            for (int i = tid; i < KT * CH; i += C::threads) {
+                const int row = i / CH, c = i - row * CH, r = kb + row;
+                bool on = r >= P.lo && r < P.hi && c * 8 < hd;
+                long long off = 0;
+                if (r >= P.lo && r < P.hi) {
+                    off = paged_off(kv, P.b, P.j, r);
+                    if (off < 0) {
+                        if (c == 0) atomicExch(kv.err, kErrBadPos);
+                        s_badpage = 1;
+                        on = false;
+                        off = 0;
+                    }
+                }
+                const uint32_t at = stage * C::tile + row * PITCH + c * 16;
+                const long long e = on ? (off + c * 8) * 2 : 0;
+                copy16(sK + at, static_cast<const uint8_t *>(kv.k) + e, on);
+                copy16(sV + at, static_cast<const uint8_t *>(kv.v) + e, on);
+            }
+        }
+        copies_end();
+    };
+    // V elements that are no finite numbers, in a tile that some token sees in part: 0 x them would be NaN.  They become
+    // zeros, and are added to the rows that see them at the portion's end.  (Every thread looks at its own copies.)
+    auto clean_tile = [&](int stage) {
+        for (int i = tid; i < KT * CH; i += C::threads) {
+            const int row = i / CH, c = i - row * CH;
+            uint4 *p = reinterpret_cast<uint4 *>(kmem + (2 + stage) * C::tile + row * PITCH + c * 16);
+            uint4 v = *p;
+            uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            bool bad = false;
+            constexpr uint32_t E = BF ? 0x7F80u : 0x7C00u;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                if ((w[k] & E) == E) w[k] &= 0xFFFF0000u, bad = true;
+                if ((w[k] >> 16 & E) == E) w[k] &= 0xFFFFu, bad = true;
+            }
+            if (bad) {
+                *p = make_uint4(w[0], w[1], w[2], w[3]);
+                s_poison = 1;
+            }
+        }
+    };
+
+    while (wk.next(a)) {
+        P.set(a, wk);
+        __syncthreads();                               // the last portion's tiles and q have been read
+        load_tile(0, 0);
+        // ---------------- q as A operands, in terms: a warp per row
+        for (int i = warp; i < M; i += C::warps) {
+            int tok, head;
+            P.row(a, i, tok, head);
+            const TQ *q = static_cast<const TQ *>(a.q) + static_cast<long long>(P.tok0 + max(tok, 0)) * a.q_stride +
+                          static_cast<long long>(P.j * a.gqa + P.g0 + head) * hd;
+            uint8_t *dst = smem + i * PITCH;
+            if constexpr (TERMS == 1) {
+                for (int c = lane; c < HD / 2; c += 32) {
+                    uint32_t v = 0;
+                    if (tok >= 0 && 2 * c < hd) v = ld_now(reinterpret_cast<const uint32_t *>(q) + c);
+                    *reinterpret_cast<uint32_t *>(dst + 4 * c) = v;
+                }
+            } else {
+                float2 v[HD / 64 + (HD % 64 != 0)];
+                float mx = 0.f;
+#pragma unroll
+                for (int k = 0; k < HD / 64 + (HD % 64 != 0); k++) {
+                    const int c = lane + 32 * k;
+                    v[k] = make_float2(0.f, 0.f);
+                    if (tok >= 0 && 2 * c < hd) {
+                        const float2 x = ld_now(reinterpret_cast<const float2 *>(q) + c);
+                        v[k] = make_float2(x.x * l2, x.y * l2);
+                    }
+                    mx = fmaxf(mx, fmaxf(fabsf(v[k].x), fabsf(v[k].y)));
+                }
+                float up = 1.f, down = 1.f;
+                if constexpr (!BF) {                   // the row's largest |q| is brought to [2^9, 2^10)
+#pragma unroll
+                    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                    const int e = max(-110, min(110, static_cast<int>(__float_as_uint(mx) >> 23) - 127 - 9));
+                    up = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+                    down = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+                }
+                if (lane == 0) s_scale[i] = down;
+#pragma unroll
+                for (int k = 0; k < HD / 64 + (HD % 64 != 0); k++) {
+                    const int c = lane + 32 * k;
+                    uint32_t t[TERMS];
+                    split2<BF, TERMS>(v[k].x * up, v[k].y * up, t);
+                    if (2 * c < HD)
+#pragma unroll
+                        for (int z = 0; z < TERMS; z++) *reinterpret_cast<uint32_t *>(dst + z * M * PITCH + 4 * c) = t[z];
+                }
+            }
+        }
+        load_tile(1, 1);
+        // the thread's rows lr, lr + 8 of the warp: the keys they see
+        int tok[2], head[2], see_lo[2], see_hi[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            P.row(a, 16 * warp + lr + 8 * i, tok[i], head[i]);
+            see_hi[i] = tok[i] < 0 ? 0 : min(P.hi, P.base + tok[i] + 1);
+            see_lo[i] = max(P.lo, a.window > 0 ? P.base + tok[i] + 1 - a.window : 0);
+        }
+        float m[2] = {kNone, kNone}, l[2] = {0.f, 0.f}, o[HD / 8][4];
+#pragma unroll
+        for (int t = 0; t < HD / 8; t++) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
+        float unit[2] = {l2, l2};
+        for (int it = 0; it < P.tiles; it++) {
+            const int stage = it & 1, kb = P.kb0 + it * KT;
+            const bool partial = kb + KT > P.free_hi || kb < P.free_lo;   // (the keys outside [lo, hi) are zeros)
+            copies_wait<1>();
+            if (partial) clean_tile(stage);
+            __syncthreads();
+            if constexpr (TERMS > 1)
+                if (it == 0) {
+                    unit[0] = BF ? 1.f : s_scale[16 * warp + lr];
+                    unit[1] = BF ? 1.f : s_scale[16 * warp + lr + 8];
+                }
+            // ---------------- S: rows lr (+ 8), keys 8 n + 2 lc (+ 1)
+            float s[NS][TERMS][4];
+#pragma unroll
+            for (int n = 0; n < NS; n++)
+#pragma unroll
+                for (int z = 0; z < TERMS; z++) s[n][z][0] = s[n][z][1] = s[n][z][2] = s[n][z][3] = 0.f;
+            const uint32_t qa = sQ + (16 * warp + (lane & 15)) * PITCH + (lane >> 4) * 16;
+            const uint32_t ka = sK + stage * C::tile + ((lane & 7) + (lane >> 4) * 8) * PITCH + (lane >> 3 & 1) * 16;
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                uint32_t A[TERMS][4];
+#pragma unroll
+                for (int z = 0; z < TERMS; z++) ldm4(qa + z * M * PITCH + 32 * k, A[z]);
+#pragma unroll
+                for (int n = 0; n < NS; n += 2) {
+                    uint32_t B[4];                     // keys 8 n ..: elements 0-7, 8-15 of the step; keys 8 n + 8 ..
+                    ldm4(ka + n * 8 * PITCH + 32 * k, B);
+#pragma unroll
+                    for (int z = 0; z < TERMS; z++) {
+                        mma16<BF>(s[n][z], A[z], B[0], B[1]);
+                        mma16<BF>(s[n + 1][z], A[z], B[2], B[3]);
+                    }
+                }
+            }
+            float x[NS][4], top[2] = {m[0], m[1]};
+            const bool bad = *reinterpret_cast<volatile int *>(&s_badpage) != 0;
+#pragma unroll
+            for (int n = 0; n < NS; n++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    float y = s[n][0][i];
+                    if constexpr (TERMS == 2) y += s[n][TERMS - 1][i];
+                    if constexpr (TERMS == 3) y += s[n][1 % TERMS][i] + s[n][TERMS - 1][i];
+                    if (TERMS == 1 || !BF) y *= unit[i >> 1];
+                    const int key = kb + 8 * n + 2 * lc + (i & 1);
+                    if (partial && (key >= see_hi[i >> 1] || key < see_lo[i >> 1])) y = -INFINITY;
+                    if (bad && key < P.hi && paged_off(kv, P.b, P.j, key) < 0) y = -INFINITY;
+                    x[n][i] = y;
+                    top[i >> 1] = fmaxf(top[i >> 1], y);
+                }
+            float f[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+                top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
+                f[i] = ex2(m[i] - top[i]);
+                m[i] = top[i];
+                l[i] *= f[i];
+            }
+            // ---------------- P as A operands: keys 16 k .. + 15
+            uint32_t pf[KT / 16][TERMS][4];
+#pragma unroll
+            for (int n = 0; n < NS; n++) {
+                float p[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    p[i] = ex2(x[n][i] - m[i >> 1]);
+                    l[i >> 1] += p[i];
+                    p[i] *= PSCALE;
+                }
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    uint32_t t[TERMS];
+                    split2<BF, TERMS>(p[2 * i], p[2 * i + 1], t);
+#pragma unroll
+                    for (int z = 0; z < TERMS; z++) pf[n / 2][z][(n & 1) * 2 + i] = t[z];
+                }
+            }
+            // ---------------- O: rows lr (+ 8), elements 8 t + 2 lc (+ 1)
+            const uint32_t va = sV + stage * C::tile + (lane & 15) * PITCH + (lane >> 4) * 16;
+#pragma unroll
+            for (int t = 0; t < HD / 8; t += 2) {
+                float d[2][4] = {};
+#pragma unroll
+                for (int k = 0; k < KT / 16; k++) {
+                    uint32_t B[4];
+                    ldm4t(va + 16 * k * PITCH + 16 * t, B);
+#pragma unroll
+                    for (int z = TERMS - 1; z >= 0; z--) {
+                        mma16<BF>(d[0], pf[k][z], B[0], B[1]);
+                        mma16<BF>(d[1], pf[k][z], B[2], B[3]);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    o[t][i] = fmaf(o[t][i], f[i >> 1], d[0][i]);
+                    o[t + 1][i] = fmaf(o[t + 1][i], f[i >> 1], d[1][i]);
+                }
+            }
+            __syncthreads();
+            load_tile(it + 2, stage);
+        }
+        // ---------------- the portion's end
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+        }
+#pragma unroll
+        for (int t = 0; t < HD / 8; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[t][i] *= 1.f / PSCALE;
+        if (*reinterpret_cast<volatile int *>(&s_poison)) {
+            for (int it = 0; it < P.tiles; it++) {
+                const int kb = P.kb0 + it * KT;
+                if (kb + KT <= P.free_hi && kb >= P.free_lo) continue;
+                for (int key = max(kb, P.lo); key < min(kb + KT, P.hi); key++) {
+                    const long long off = paged_off(kv, P.b, P.j, key);
+                    if (off < 0) continue;
+                    const T *v = static_cast<const T *>(kv.v) + off;
+#pragma unroll
+                    for (int i = 0; i < 2; i++)
+                        if (key >= see_lo[i] && key < see_hi[i])
+#pragma unroll
+                            for (int t = 0; t < HD / 8; t++)
+#pragma unroll
+                                for (int e = 0; e < 2; e++)
+                                    if (8 * t + 2 * lc + e < hd) o[t][2 * i + e] += not_finite(to_f(v[8 * t + 2 * lc + e]));
+                }
+            }
+        }
+        const bool whole = P.begins && P.ends;
+        if (first && tid == 0) note_join(a, &P, wk, worker, T_, G);
+        first = false;
+        float *part = chunk_part(a, worker, P.begins);
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            if (tok[i] < 0) continue;
+            const int r = 16 * warp + lr + 8 * i;
+            if (whole) {
+                const long long row = out_row(a, P, tok[i], head[i]);
+                const float inv = inverse_sum(l[i]);
+                TQ *dst = static_cast<TQ *>(a.out) + row * hd + 2 * lc;
+#pragma unroll
+                for (int t = 0; t < HD / 8; t++)
+                    if (8 * t < hd) st_pair(dst + 8 * t, o[t][2 * i] * inv, o[t][2 * i + 1] * inv);
+                if (a.lse && lc == 0) a.lse[row] = lse_of(m[i], l[i]);
+            } else {
+#pragma unroll
+                for (int t = 0; t < HD / 8; t++) st_pair(part + r * HD + 8 * t + 2 * lc, o[t][2 * i], o[t][2 * i + 1]);
+                if (lc == 0) {
+                    part[M * HD + r] = m[i];
+                    part[M * HD + M + r] = l[i];
+                }
+            }
+        }
+    }
+    copies_wait<0>();
+    if (first && tid == 0) note_join(a, nullptr, wk, worker, T_, G);
+}
+
+// ------------------------------------------------------------ f32 caches
+template <int HD>
+struct Tf {
+    static constexpr int warps = HD > 128 ? 4 : 8, threads = 32 * warps, M = 16 * warps, KT = 32;
+    // floats of a row: pairs of eight rows (Q, K) on 64 different banks; rows 2 lc of eight columns (V) on 32
+    static constexpr int kpitch = HD + 8, vpitch = HD + 4;
+    static constexpr int smem = (M * kpitch + 2 * KT * (kpitch + vpitch)) * 4;
+};
+
+template <int HD>
+__global__ void __launch_bounds__(Tf<HD>::threads, 1) k_chunk_tf32(PagedChunkArgs a) {
+    using C = Tf<HD>;
+    constexpr int KT = C::KT, M = C::M, NS = KT / 8, CH = HD / 4;
+    extern __shared__ __align__(16) float fmem[];
+    __shared__ int s_poison, s_badpage;
+    const PagedKv &kv = a.kv;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hd = kv.hd;
+    const int lr = lane >> 2, lc = lane & 3;
+    float *const sQ = fmem, *const sK = sQ + M * C::kpitch, *const sV = sK + 2 * KT * C::kpitch;
+    const float l2 = a.scale * 1.4426950408889634f;
+    pdl_trigger();
+    pdl_wait();
+    long long T_, G = 0;
+    ChunkWalk wk;
+    const int worker = blockIdx.x;
+    chunk_share(a, worker, wk, T_, G);
+    if (tid == 0) s_poison = s_badpage = 0;
+    Portion P{};
+    bool first = true;
+
+    auto load_tile = [&](int it, int stage) {
+        const int kb = P.kb0 + it * KT;
+        if (it < P.tiles) {
+            for (int i = tid; i < KT * CH; i += C::threads) {
+                const int row = i / CH, c = i - row * CH, r = kb + row;
+                bool on = r >= P.lo && r < P.hi && c * 4 < hd;
+                long long off = 0;
+                if (r >= P.lo && r < P.hi) {
+                    off = paged_off(kv, P.b, P.j, r);
+                    if (off < 0) {
+                        if (c == 0) atomicExch(kv.err, kErrBadPos);
+                        s_badpage = 1;
+                        on = false;
+                        off = 0;
+                    }
+                }
+                const long long e = on ? off + c * 4 : 0;
+                copy16(smem_addr(sK + (stage * KT + row) * C::kpitch + c * 4), static_cast<const float *>(kv.k) + e, on);
+                copy16(smem_addr(sV + (stage * KT + row) * C::vpitch + c * 4), static_cast<const float *>(kv.v) + e, on);
+            }
+        }
+        copies_end();
+    };
+    auto clean_tile = [&](int stage) {                 // as in k_chunk_mma
+        for (int i = tid; i < KT * CH; i += C::threads) {
+            const int row = i / CH, c = i - row * CH;
+            float *p = sV + (stage * KT + row) * C::vpitch + c * 4;
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (not_finite(p[e]) != 0.f) {
+                    p[e] = 0.f;
+                    s_poison = 1;
+                }
+        }
+    };
+
+    while (wk.next(a)) {
+        P.set(a, wk);
+        __syncthreads();
+        load_tile(0, 0);
+        for (int i = warp; i < M; i += C::warps) {
+            int tok, head;
+            P.row(a, i, tok, head);
+            const float *q = static_cast<const float *>(a.q) + static_cast<long long>(P.tok0 + max(tok, 0)) * a.q_stride +
+                             static_cast<long long>(P.j * a.gqa + P.g0 + head) * hd;
+            for (int c = lane; c < HD; c += 32) sQ[i * C::kpitch + c] = tok >= 0 && c < hd ? ld_now(q + c) * l2 : 0.f;
+        }
+        load_tile(1, 1);
+        int tok[2], head[2], see_lo[2], see_hi[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            P.row(a, 16 * warp + lr + 8 * i, tok[i], head[i]);
+            see_hi[i] = tok[i] < 0 ? 0 : min(P.hi, P.base + tok[i] + 1);
+            see_lo[i] = max(P.lo, a.window > 0 ? P.base + tok[i] + 1 - a.window : 0);
+        }
+        float m[2] = {kNone, kNone}, l[2] = {0.f, 0.f}, o[HD / 8][4];
+#pragma unroll
+        for (int t = 0; t < HD / 8; t++) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
+        for (int it = 0; it < P.tiles; it++) {
+            const int stage = it & 1, kb = P.kb0 + it * KT;
+            const bool partial = kb + KT > P.free_hi || kb < P.free_lo;
+            copies_wait<1>();
+            if (partial) clean_tile(stage);
+            __syncthreads();
+            // ---------------- S.  The order of a sum's elements is free: of eight, the MMA's k and k + 4 are 2 k, 2 k + 1
+            float s[NS][4] = {}, c_[NS][4] = {};       // the product of the upper terms; those with a lower one
+            const float *qa = sQ + (16 * warp + lr) * C::kpitch + 2 * lc, *ka = sK + (stage * KT + lr) * C::kpitch + 2 * lc;
+#pragma unroll 4
+            for (int k = 0; k < HD / 8; k++) {
+                uint32_t ah[4], al[4];
+                const float2 q0 = *reinterpret_cast<const float2 *>(qa + 8 * k);
+                const float2 q1 = *reinterpret_cast<const float2 *>(qa + 8 * C::kpitch + 8 * k);
+                split_tf32(q0.x, ah[0], al[0]);
+                split_tf32(q1.x, ah[1], al[1]);
+                split_tf32(q0.y, ah[2], al[2]);
+                split_tf32(q1.y, ah[3], al[3]);
+#pragma unroll
+                for (int n = 0; n < NS; n++) {
+                    const float2 b = *reinterpret_cast<const float2 *>(ka + 8 * n * C::kpitch + 8 * k);
+                    uint32_t bh[2], bl[2];
+                    split_tf32(b.x, bh[0], bl[0]);
+                    split_tf32(b.y, bh[1], bl[1]);
+                    mma8(s[n], ah, bh[0], bh[1]);
+                    mma8(c_[n], al, bh[0], bh[1]);
+                    mma8(c_[n], ah, bl[0], bl[1]);
+                }
+            }
+            float top[2] = {m[0], m[1]};
+            const bool bad = *reinterpret_cast<volatile int *>(&s_badpage) != 0;
+#pragma unroll
+            for (int n = 0; n < NS; n++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    float y = s[n][i] + c_[n][i];
+                    const int key = kb + 8 * n + 2 * lc + (i & 1);
+                    if (partial && (key >= see_hi[i >> 1] || key < see_lo[i >> 1])) y = -INFINITY;
+                    if (bad && key < P.hi && paged_off(kv, P.b, P.j, key) < 0) y = -INFINITY;
+                    s[n][i] = y;
+                    top[i >> 1] = fmaxf(top[i >> 1], y);
+                }
+            float f[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+                top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
+                f[i] = ex2(m[i] - top[i]);
+                m[i] = top[i];
+                l[i] *= f[i];
+            }
+            uint32_t ph[NS][4], pl[NS][4];             // keys 8 n + 2 k, + 1 as the MMA's k, k + 4
+#pragma unroll
+            for (int n = 0; n < NS; n++) {
+                float p[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    p[i] = ex2(s[n][i] - m[i >> 1]);
+                    l[i >> 1] += p[i];
+                }
+                split_tf32(p[0], ph[n][0], pl[n][0]);
+                split_tf32(p[2], ph[n][1], pl[n][1]);
+                split_tf32(p[1], ph[n][2], pl[n][2]);
+                split_tf32(p[3], ph[n][3], pl[n][3]);
+            }
+            const float *va = sV + (stage * KT + 2 * lc) * C::vpitch + lr;
+#pragma unroll
+            for (int t = 0; t < HD / 8; t++) {
+                float d[4] = {}, e[4] = {};
+#pragma unroll
+                for (int n = 0; n < NS; n++) {
+                    uint32_t bh[2], bl[2];
+                    split_tf32(va[8 * n * C::vpitch + 8 * t], bh[0], bl[0]);
+                    split_tf32(va[(8 * n + 1) * C::vpitch + 8 * t], bh[1], bl[1]);
+                    mma8(e, pl[n], bh[0], bh[1]);
+                    mma8(e, ph[n], bl[0], bl[1]);
+                    mma8(d, ph[n], bh[0], bh[1]);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[t][i] = fmaf(o[t][i], f[i >> 1], d[i] + e[i]);
+            }
+            __syncthreads();
+            load_tile(it + 2, stage);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+        }
+        if (*reinterpret_cast<volatile int *>(&s_poison)) {
+            for (int it = 0; it < P.tiles; it++) {
+                const int kb = P.kb0 + it * KT;
+                if (kb + KT <= P.free_hi && kb >= P.free_lo) continue;
+                for (int key = max(kb, P.lo); key < min(kb + KT, P.hi); key++) {
+                    const long long off = paged_off(kv, P.b, P.j, key);
+                    if (off < 0) continue;
+                    const float *v = static_cast<const float *>(kv.v) + off;
+#pragma unroll
+                    for (int i = 0; i < 2; i++)
+                        if (key >= see_lo[i] && key < see_hi[i])
+#pragma unroll
+                            for (int t = 0; t < HD / 8; t++)
+#pragma unroll
+                                for (int e = 0; e < 2; e++)
+                                    if (8 * t + 2 * lc + e < hd) o[t][2 * i + e] += not_finite(v[8 * t + 2 * lc + e]);
+                }
+            }
+        }
+        const bool whole = P.begins && P.ends;
+        if (first && tid == 0) note_join(a, &P, wk, worker, T_, G);
+        first = false;
+        float *part = chunk_part(a, worker, P.begins);
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            if (tok[i] < 0) continue;
+            const int r = 16 * warp + lr + 8 * i;
+            const long long row = out_row(a, P, tok[i], head[i]);
+            const float inv = whole ? inverse_sum(l[i]) : 1.f;
+            float *dst = whole ? static_cast<float *>(a.out) + row * hd + 2 * lc : part + r * HD + 2 * lc;
+#pragma unroll
+            for (int t = 0; t < HD / 8; t++)
+                if (!whole || 8 * t + 2 * lc < hd) st_pair(dst + 8 * t, o[t][2 * i] * inv, o[t][2 * i + 1] * inv);
+            if (lc == 0 && whole && a.lse) a.lse[row] = lse_of(m[i], l[i]);
+            if (lc == 0 && !whole) {
+                part[M * HD + r] = m[i];
+                part[M * HD + M + r] = l[i];
+            }
+        }
+    }
+    copies_wait<0>();
+    if (first && tid == 0) note_join(a, nullptr, wk, worker, T_, G);
+}
+
+// ------------------------------------------------------------ joining
+// A cut segment's portions added up in order, a warp per query row.  M rows of
+// pitch floats a portion.
+constexpr int kJoinThreads = 256;
+template <class TQ>
+__global__ void __launch_bounds__(kJoinThreads) k_chunk_join(PagedChunkArgs a, int M, int pitch) {
+    pdl_trigger();
+    pdl_wait();
+    const int worker = blockIdx.x, lane = threadIdx.x & 31;
+    const ChunkJoin j = static_cast<const ChunkJoin *>(a.joins)[worker];
+    if (j.first < 0) return;
+    const int r = blockIdx.y * (kJoinThreads / 32) + (threadIdx.x >> 5), hd = a.kv.hd;
+    const int tok = r / a.hg, hr = r - tok * a.hg, kvh = j.head / a.groups, g0 = (j.head - kvh * a.groups) * a.hg;
+    const Chunk c(a, j.b, false);
+    const int first = j.seg << a.tok_shift;
+    if (r >= M || tok >= min(1 << a.tok_shift, c.n - first) || hr >= min(a.hg, a.gqa - g0)) return;
+    const long long row = static_cast<long long>(c.tok0 + first + tok) * a.n_heads + kvh * a.gqa + g0 + hr;
+    float top = kNone;
+    for (int w = j.first; w <= worker; w++) top = fmaxf(top, chunk_part(a, w, w == j.first)[M * pitch + r]);
+    float l = 0.f, o[8] = {};
+    for (int w = j.first; w <= worker; w++) {
+        const float *p = chunk_part(a, w, w == j.first);
+        const float f = ex2(p[M * pitch + r] - top);
+        l += p[M * pitch + M + r] * f;
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (lane + 32 * k < hd) o[k] += p[r * pitch + lane + 32 * k] * f;
+    }
+    const float inv = inverse_sum(l);
+    TQ *out = static_cast<TQ *>(a.out) + row * hd;
+#pragma unroll
+    for (int k = 0; k < 8; k++)
+        if (lane + 32 * k < hd) out[lane + 32 * k] = from_f<TQ>(o[k] * inv);
+    if (a.lse && lane == 0) a.lse[row] = lse_of(top, l);
+}
+
+int log2_floor(int v) { return 31 - __builtin_clz(static_cast<unsigned>(v)); }
+// rows of a query tile and keys of a tile of the kernels above
+int rows_of(const PagedKv &kv) { return kv.hd > 128 ? 64 : 128; }
+int key_shift_of(const PagedKv &kv) { return kv.dtype == STYX_F32 || kv.hd > 128 ? 5 : 6; }
+int pitch_of(const PagedKv &kv) { return kv.hd <= 64 ? 64 : kv.dtype != STYX_F32 && kv.hd <= 96 ? 96 : kv.hd <= 128 ? 128 : 256; }
+
+template <auto kern>
+cudaError_t go(const PagedChunkArgs &a, int threads, int smem, cudaStream_t st) {
+    cudaError_t e = allow_smem<kern>(smem);
+    return e != cudaSuccess ? e : launch_pdl(kern, dim3(a.workers), dim3(threads), smem, st, a);
+}
+template <bool BF, int TERMS, int HD>
+cudaError_t go_mma(const PagedChunkArgs &a, cudaStream_t st) {
+    static_assert(Mma<HD>::smem(TERMS) <= 226 * 1024, "shared memory");
+    return go<k_chunk_mma<BF, TERMS, HD>>(a, Mma<HD>::threads, Mma<HD>::smem(TERMS), st);
+}
+template <bool BF, int TERMS>
+cudaError_t go_hd(const PagedChunkArgs &a, cudaStream_t st) {
+    switch (pitch_of(a.kv)) {
+        case 64: return go_mma<BF, TERMS, 64>(a, st);
+        case 96: return go_mma<BF, TERMS, 96>(a, st);
+        case 128: return go_mma<BF, TERMS, 128>(a, st);
+        default: return go_mma<BF, TERMS, 256>(a, st);
+    }
+}
+template <int HD>
+cudaError_t go_tf32(const PagedChunkArgs &a, cudaStream_t st) {
+    static_assert(Tf<HD>::smem <= 226 * 1024, "shared memory");
+    return go<k_chunk_tf32<HD>>(a, Tf<HD>::threads, Tf<HD>::smem, st);
+}
+
+}  // namespace
+
+uint64_t chunk_mma_parts(const PagedKv &kv, int sms) {
+    return 2ull * sms * rows_of(kv) * (pitch_of(kv) + 2) * 4;
+}
+
+// the portions joined; a's cut of the work and workspace are set
+cudaError_t launch_chunk_join(const PagedChunkArgs &a, int M, int pitch, cudaStream_t st) {
+    const dim3 grid(a.workers, (M + kJoinThreads / 32 - 1) / (kJoinThreads / 32));
+    if (!a.q16) return launch_pdl(k_chunk_join<float>, grid, dim3(kJoinThreads), 0, st, a, M, pitch);
+    if (a.kv.dtype == STYX_F16) return launch_pdl(k_chunk_join<__half>, grid, dim3(kJoinThreads), 0, st, a, M, pitch);
+    return launch_pdl(k_chunk_join<__nv_bfloat16>, grid, dim3(kJoinThreads), 0, st, a, M, pitch);
+}
+
+cudaError_t launch_chunk_mma(PagedChunkArgs a, int sms, cudaStream_t st) {
+    const int M = rows_of(a.kv);
+    a.hg = std::min(a.gqa, M);
+    a.groups = (a.gqa + a.hg - 1) / a.hg;
+    a.heads = a.kv.n_kv * a.groups;
+    a.tok_shift = log2_floor(M / a.hg);
+    a.key_shift = key_shift_of(a.kv);
+    // a table of one tile's rows: no segment can be cut
+    const bool cut = (static_cast<long long>(a.kv.max_pages) << a.kv.page_shift) > (1 << a.key_shift);
+    a.seg_cost = cut ? 2 : 0;
+    a.workers = sms;
+    const int pitch = pitch_of(a.kv);
+    a.part_floats = M * (pitch + 2);
+    cudaError_t e;
+    if (a.kv.dtype == STYX_F32)
+        e = pitch == 64 ? go_tf32<64>(a, st) : pitch == 128 ? go_tf32<128>(a, st) : go_tf32<256>(a, st);
+    else if (a.kv.dtype == STYX_F16)
+        e = a.q16 ? go_hd<false, 1>(a, st) : go_hd<false, 2>(a, st);
+    else
+        e = a.q16 ? go_hd<true, 1>(a, st) : go_hd<true, 3>(a, st);
+    return e != cudaSuccess || !cut ? e : launch_chunk_join(a, M, pitch, st);
+}
+
+}  // namespace styx

@@ -1,0 +1,198 @@
+// paged_chunk.cuh -- how the attention of chunks (styx_paged_attend_chunk) cuts
+// its work.  A segment is 2^tok_shift new tokens of one sequence with the q
+// heads of one kv head (or a group of hg of them): rows of a query tile.  It
+// walks tiles of 2^key_shift cached rows, from the first one that its first
+// token sees to its last token's own.  All segments' tiles of a call are one
+// list (sequence, kv head and group, segment, tile), cut evenly over the
+// workers, so ragged lengths and few tokens over a long cache fill the SMs
+// alike; segments that are cut are joined in order.  A segment's start and end
+// count as seg_cost tiles.  How many tiles a sequence has, and in which segment
+// its u-th lies, are closed sums over its causal staircase, so every warp finds
+// its share by itself, whatever the lengths.
+#pragma once
+
+#include "paged_split.cuh"
+
+namespace styx {
+namespace {
+
+// sum over i < m of floor((c + (i << ts)) / 2^ks), c >= 0
+__device__ __forceinline__ long long sum_floor(long long c, long long m, int ts, int ks) {
+    if (m <= 0) return 0;
+    if (ts >= ks) return m * (c >> ks) + ((m * (m - 1) / 2) << (ts - ks));
+    const int k = ks - ts;
+    const long long y = c >> ts;
+    auto upto = [&](long long x) {   // sum over 0 <= v < x of floor(v / 2^k)
+        const long long q = x >> k;
+        return ((q * (q - 1) / 2) << k) + q * (x - (q << k));
+    };
+    return upto(y + m) - upto(y);
+}
+
+// a sequence's new tokens: start of the tokens, their number, the row of the first one
+struct Chunk {
+    int tok0, n, base;
+    __device__ __forceinline__ Chunk(const PagedChunkArgs &a, int b, bool report) {
+        const int len = paged_len(a.kv, b, report), lo = ld_now(a.start + b), hi = ld_now(a.start + b + 1);
+        const bool ok = lo >= 0 && hi >= lo && hi <= a.n_tokens && hi - lo <= len;
+        if (!ok && report) atomicExch(a.kv.err, kErrBadPos);
+        tok0 = lo;
+        n = ok ? hi - lo : 0;
+        base = len - n;
+    }
+    __device__ __forceinline__ int segs(const PagedChunkArgs &a) const {
+        return static_cast<int>((static_cast<long long>(n) + (1 << a.tok_shift) - 1) >> a.tok_shift);
+    }
+    // tiles of segment i: [first, first + count)
+    __device__ __forceinline__ int first_row(const PagedChunkArgs &a, int i) const {   // that its first token sees
+        const long long r = static_cast<long long>(base) + (static_cast<long long>(i) << a.tok_shift) + 1 - a.window;
+        return a.window > 0 && r > 0 ? static_cast<int>(r) : 0;
+    }
+    __device__ __forceinline__ int end_row(const PagedChunkArgs &a, int i) const {     // past its last token's
+        return static_cast<int>(base + min(static_cast<long long>(n), static_cast<long long>(i + 1) << a.tok_shift));
+    }
+    __device__ __forceinline__ int first_tile(const PagedChunkArgs &a, int i) const { return first_row(a, i) >> a.key_shift; }
+    __device__ __forceinline__ int tiles(const PagedChunkArgs &a, int i) const {
+        return ((end_row(a, i) - 1) >> a.key_shift) + 1 - first_tile(a, i);
+    }
+    // units (tiles and seg_cost) of the first m segments, m < segs or m = segs
+    __device__ __forceinline__ long long upto(const PagedChunkArgs &a, int m) const {
+        if (m <= 0) return 0;
+        const int ts = a.tok_shift, ks = a.key_shift;
+        long long u = static_cast<long long>(m) * (1 + a.seg_cost);
+        const int whole = min(m, n >> ts);     // segments with all their tokens
+        u += sum_floor(static_cast<long long>(base) + (1ll << ts) - 1, whole, ts, ks);
+        if (whole < m) u += (base + n - 1) >> ks;
+        if (a.window > 0) {
+            const long long c = static_cast<long long>(base) + 1 - a.window;
+            const long long i0 = c >= 0 ? 0 : (-c + (1ll << ts) - 1) >> ts;
+            u -= sum_floor(c + (i0 << ts), m - i0, ts, ks);
+        }
+        return u;
+    }
+};
+
+// a worker's share of the list, portion by portion
+struct ChunkWalk {
+    int b, head, seg;              // sequence, (kv head, group), segment of its tokens
+    int u, nt;                     // next unit of the segment's seg_cost + nt
+    long long at, end;             // global unit numbers
+    int t0, t1;                    // the portion: tiles [t0, t1) of the segment, from its first
+    __device__ __forceinline__ bool next(const PagedChunkArgs &a) {
+        while (at < end) {
+            if (u == a.seg_cost + nt) {
+                u = 0;
+                Chunk c(a, b, false);
+                if (++seg >= c.segs(a)) {
+                    seg = 0;
+                    if (++head == a.heads) {
+                        head = 0;
+                        do {
+                            if (++b >= a.kv.n_seqs) {   // (lengths that changed during the call)
+                                end = at;
+                                return false;
+                            }
+                            c = Chunk(a, b, false);
+                        } while (c.n == 0);
+                    }
+                }
+                nt = c.tiles(a, seg);
+            }
+            const int u1 = static_cast<int>(min(static_cast<long long>(a.seg_cost + nt), u + (end - at)));
+            t0 = max(0, u - a.seg_cost);
+            t1 = max(0, u1 - a.seg_cost);
+            at += u1 - u;
+            u = u1;
+            if (t1 > t0) return true;
+        }
+        return false;
+    }
+};
+
+// Worker i's share of T units in G parts: [floor(i T / G), floor((i + 1) T / G)).  All lanes of a warp together.
+__device__ __forceinline__ void chunk_share(const PagedChunkArgs &a, int worker, ChunkWalk &w, long long &T, long long &G) {
+    const int lane = threadIdx.x & 31, n = a.kv.n_seqs;
+    const int per = (n + 31) / 32, lo = min(n, lane * per), hi = min(n, lo + per);
+    const bool report = blockIdx.x == 0 && threadIdx.x < 32;
+    auto units = [&](int b, bool r) {
+        const Chunk c(a, b, r);
+        return c.upto(a, c.segs(a)) * a.heads;
+    };
+    long long mine = 0;
+    for (int b = lo; b < hi; b++) mine += units(b, report);
+    long long upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long u = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += u;
+    }
+    T = __shfl_sync(0xffffffffu, upto, 31);
+    w.b = w.head = w.seg = w.u = w.nt = w.t0 = w.t1 = 0;
+    w.at = w.end = 0;
+    if (T == 0) return;
+    G = min(static_cast<long long>(a.workers), T);
+    if (worker >= G) return;
+    const long long at = T / G * worker + T % G * worker / G;
+    w.end = T / G * (worker + 1) + T % G * (worker + 1) / G;
+    w.at = at;
+    const int src = __ffs(__ballot_sync(0xffffffffu, at < upto)) - 1;   // (at < T, so there is one)
+    long long off = at - (upto - mine);
+    int b = lo;
+    if (lane == src)
+        for (; b < hi - 1; b++) {
+            const long long nb = units(b, false);
+            if (off < nb) break;
+            off -= nb;
+        }
+    w.b = __shfl_sync(0xffffffffu, b, src);
+    off = __shfl_sync(0xffffffffu, off, src);
+    const Chunk c(a, w.b, false);
+    const int ns = c.segs(a);
+    const long long head_units = max(1ll, c.upto(a, ns));
+    w.head = static_cast<int>(min(off / head_units, static_cast<long long>(a.heads - 1)));
+    off -= w.head * head_units;
+    int s0 = 0, s1 = max(0, ns - 1);             // the last segment with upto(s) <= off
+    while (s0 < s1) {
+        const int mid = (s0 + s1 + 1) >> 1;
+        if (c.upto(a, mid) <= off) s0 = mid;
+        else s1 = mid - 1;
+    }
+    w.seg = s0;
+    w.nt = c.tiles(a, s0);
+    w.u = static_cast<int>(min(off - c.upto(a, s0), static_cast<long long>(a.seg_cost + w.nt)));
+}
+
+// the first worker with a tile of the segment in which the walk's portion (its worker's, up to w.at) has the last one
+__device__ __forceinline__ int chunk_owner(const PagedChunkArgs &a, const ChunkWalk &w, long long T, long long G) {
+    const long long first = w.at - w.nt;         // the segment's first tile, as a unit of the list
+    long long i = (first + 1) * G;               // (both below 2^31 x 2^16 or so)
+    i = (i - 1) / T;
+    // floor(i T / G) <= first < floor((i + 1) T / G), for the shares as they are computed above
+    auto share = [&](long long k) { return T / G * k + T % G * k / G; };
+    while (i > 0 && share(i) > first) i--;
+    while (share(i + 1) <= first) i++;
+    return static_cast<int>(i);
+}
+
+// what joins a cut segment: filled in by the worker that has its last tile, for every call
+struct ChunkJoin {
+    int first, b, head, seg;       // first worker (-1: nothing to join); the segment
+};
+// where a portion's (O, max, sum) go: worker i's portion that begins its segment to slot 2 i + 1, any other to 2 i.
+// O is [rows][pitch], then a maximum (in units of log2) and a sum for every row.
+__device__ __forceinline__ float *chunk_part(const PagedChunkArgs &a, int worker, bool begins) {
+    return a.part + (2ll * worker + (begins ? 1 : 0)) * a.part_floats;
+}
+
+template <class T>
+__device__ __forceinline__ void st_pair(T *p, float x, float y) {
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float2 *>(p) = make_float2(x, y);
+    } else {
+        const T u[2] = {from_f<T>(x), from_f<T>(y)};
+        *reinterpret_cast<uint32_t *>(p) = *reinterpret_cast<const uint32_t *>(u);
+    }
+}
+
+}  // namespace
+}  // namespace styx

@@ -1,0 +1,217 @@
+// paged_plan.cu -- which rows and pages the next tokens of every sequence get
+// (styx_paged_plan), from lengths on the device.
+//
+//   w[b]     = min(max(want, 0), rows that the table has left)
+//   t[b]     = min(w, tokens that the sequences before leave)       (prefix sum of w)
+//   target   = ceil((lens + t) / page): more pages than that go back to the
+//              stack (prefix sum), fewer are filled up from its top
+//              (prefix sum of what is missing, cut off at the stack's end)
+//   granted  = min(t, rows of the pages that there are then)        (prefix sum: start)
+//
+// One CTA, 1024 sequences at a time: four prefix sums of whole numbers, so the
+// result does not depend on any order.  Pages and tokens are handed out by
+// all threads, each finding its sequence by bisection in the sums.  What every
+// token gets (12 bytes) is written by the same CTA for few tokens, by a second
+// kernel of as many CTAs as it takes for many.
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "paged.cuh"
+
+namespace styx {
+namespace {
+
+constexpr int kThreads = 1024, kWarps = kThreads / 32;
+constexpr int kOwnTokens = 4096;   // tokens whose places the planning CTA writes itself
+constexpr int kMapThreads = 256, kMapTokens = 1024;
+
+__device__ __forceinline__ long long scan(long long v, long long *sh, long long &total) {   // inclusive, over the CTA
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += u;
+    }
+    __syncthreads();
+    if (lane == 31) sh[w] = v;
+    __syncthreads();
+    long long x = sh[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long u = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += u;
+    }
+    total = __shfl_sync(0xffffffffu, x, 31);
+    const long long before = __shfl_sync(0xffffffffu, x, w ? w - 1 : 0);
+    return v + (w ? before : 0);
+}
+
+// the first of n ascending sums that is above i (there is one)
+template <class T>
+__device__ __forceinline__ int first_above(const T *sums, int n, long long i) {
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (sums[mid] > i) hi = mid;
+        else lo = mid + 1;
+    }
+    return lo;
+}
+
+struct Row {                 // one sequence of the tile
+    int lens, held, t, target;
+    bool ok;
+};
+
+__global__ void __launch_bounds__(kThreads, 1) k_paged_plan(PagedPlanArgs a) {
+    __shared__ long long sh[kWarps];
+    __shared__ int s_sum[kThreads], s_from[kThreads], s_pos[kThreads];   // of the tile: inclusive sums, and what they start from
+    pdl_trigger();
+    pdl_wait();
+    const int tid = threadIdx.x;
+    const long long most = static_cast<long long>(a.max_pages) << a.page_shift;
+    long long n_free = ld_now(a.n_free);
+    if (n_free < 0 || n_free > a.n_pages) {
+        if (tid == 0) atomicExch(a.err, kErrBadPos);
+        n_free = n_free < 0 ? 0 : a.n_pages;
+    }
+    // a sequence of the tile, and the tokens it may have
+    long long tokens = 0;      // that the tiles before want
+    auto load = [&](int b) {
+        Row r{0, 0, 0, 0, false};
+        long long w = 0;
+        if (b < a.n_seqs) {
+            r.lens = ld_now(a.lens + b);
+            r.held = ld_now(a.held + b);
+            r.ok = r.lens >= 0 && r.held >= 0 && r.held <= a.max_pages &&
+                   r.lens <= static_cast<long long>(r.held) << a.page_shift;
+            if (!r.ok) atomicExch(a.err, kErrBadPos);
+            else w = min(static_cast<long long>(max(0, ld_now(a.want + b))), most - r.lens);
+        }
+        long long total;
+        const long long before = tokens + scan(w, sh, total) - w;
+        tokens += total;
+        r.t = static_cast<int>(min(w, max(0ll, a.n_tokens - before)));
+        r.target = r.ok ? static_cast<int>((static_cast<long long>(r.lens) + r.t + (1 << a.page_shift) - 1) >> a.page_shift) : r.held;
+        return r;
+    };
+    const bool one = a.n_seqs <= kThreads;
+    Row r{};
+    // ---------------- pages that are not needed any more
+    long long top = n_free;
+    for (int b0 = 0; b0 < a.n_seqs; b0 += kThreads) {
+        r = load(b0 + tid);
+        const int back = max(0, r.held - r.target);
+        long long total;
+        const long long upto = scan(back, sh, total);
+        if (total) {
+            // (of one tile at most 1024 x max_pages: below 2^31 only where pages are few, so by their number cut off)
+            const int n = static_cast<int>(min(total, a.n_pages - top));
+            if (n < total && tid == 0) atomicExch(a.err, kErrBadPos);   // more pages than there are
+            s_sum[tid] = static_cast<int>(min(upto, static_cast<long long>(n)));
+            s_from[tid] = r.target;
+            __syncthreads();
+            for (int i = tid; i < n; i += kThreads) {
+                const int q = first_above(s_sum, kThreads, i), nth = i - (q ? s_sum[q - 1] : 0);
+                a.free[top + i] = ld_now(a.table + static_cast<long long>(b0 + q) * a.table_stride + s_from[q] + nth);
+            }
+            top += n;
+            __syncthreads();
+        }
+    }
+    // ---------------- pages that are, and the tokens
+    long long needed = 0, given = 0;   // by the tiles before: pages wanted, tokens granted
+    tokens = 0;
+    for (int b0 = 0; b0 < a.n_seqs; b0 += kThreads) {
+        const int b = b0 + tid;
+        if (!one) r = load(b);
+        const long long need = max(0, r.target - r.held);
+        long long total;
+        const long long before = needed + scan(need, sh, total) - need;
+        needed += total;
+        const int got = static_cast<int>(min(need, max(0ll, top - before)));
+        // the tile's pages are numbers first, first + 1, ... from the stack's top
+        const long long first = min(needed - total, top);
+        const int n = static_cast<int>(min(needed, top) - first);
+        if (n > 0) {
+            s_sum[tid] = static_cast<int>(min(before + need, top) - first);
+            s_from[tid] = r.held;
+            __syncthreads();
+            for (int i = tid; i < n; i += kThreads) {
+                const int q = first_above(s_sum, kThreads, i), nth = i - (q ? s_sum[q - 1] : 0);
+                a.table[static_cast<long long>(b0 + q) * a.table_stride + s_from[q] + nth] = ld_now(a.free + top - 1 - first - i);
+            }
+        }
+        const int held = min(r.held, r.target) + got;
+        const int granted = r.ok ? static_cast<int>(max(0ll, min(static_cast<long long>(r.t), (static_cast<long long>(held) << a.page_shift) - r.lens))) : 0;
+        const long long upto = given + scan(granted, sh, total);   // (its barriers end the loop above)
+        if (b < a.n_seqs) {
+            const int pos = a.next_pos ? ld_now(a.next_pos + b) : r.lens;
+            a.lens_out[b] = r.lens + granted;
+            a.held_out[b] = held;
+            a.start[b] = static_cast<int>(upto - granted);
+            if (a.next_pos) a.next_pos_out[b] = pos + granted;
+            s_pos[tid] = pos;
+        }
+        if (a.own_maps) {
+            s_sum[tid] = static_cast<int>(upto - given);
+            s_from[tid] = r.lens;
+            __syncthreads();
+            for (int i = tid; i < total; i += kThreads) {
+                const int q = first_above(s_sum, kThreads, i), nth = i - (q ? s_sum[q - 1] : 0);
+                a.seq[given + i] = b0 + q;
+                a.row[given + i] = s_from[q] + nth;
+                a.pos[given + i] = s_pos[q] + nth;
+            }
+        }
+        given += total;
+        __syncthreads();
+    }
+    if (tid == 0) {
+        a.start[a.n_seqs] = static_cast<int>(given);
+        *a.n_free_out = static_cast<int>(top - min(needed, top));
+    }
+    if (a.own_maps)
+        for (long long i = given + tid; i < a.n_tokens; i += kThreads) {
+            a.seq[i] = 0;
+            a.row[i] = -1;
+            a.pos[i] = 0;
+        }
+}
+
+// Sequence, row and position of every token from start and the lengths after
+// it: a CTA's tokens lie between two sequences that it finds once.
+__global__ void __launch_bounds__(kMapThreads) k_paged_maps(PagedPlanArgs a) {
+    __shared__ int s_at[2];
+    pdl_trigger();
+    pdl_wait();
+    const int tid = threadIdx.x, lo = blockIdx.x * kMapTokens, hi = min(a.n_tokens, lo + kMapTokens);
+    const int total = ld_now(a.start + a.n_seqs);
+    if (tid < 2) s_at[tid] = total > 0 ? first_above(a.start + 1, a.n_seqs, min(tid ? hi - 1 : lo, total - 1)) : 0;
+    __syncthreads();
+    const int first = s_at[0], n = s_at[1] - first + 1;
+    for (int i = lo + tid; i < hi; i += kMapThreads) {
+        int b = 0, row = -1, pos = 0;
+        if (i < total) {
+            b = first + first_above(a.start + 1 + first, n, i);
+            const int from = ld_now(a.start + b), granted = ld_now(a.start + b + 1) - from, nth = i - from;
+            row = ld_now(a.lens_out + b) - granted + nth;
+            pos = a.next_pos ? ld_now(a.next_pos_out + b) - granted + nth : row;
+        }
+        a.seq[i] = b;
+        a.row[i] = row;
+        a.pos[i] = pos;
+    }
+}
+
+}  // namespace
+
+cudaError_t launch_paged_plan(PagedPlanArgs a, cudaStream_t st) {
+    a.own_maps = a.n_tokens <= kOwnTokens;
+    cudaError_t e = launch_pdl(k_paged_plan, dim3(1), dim3(kThreads), 0, st, a);
+    if (e != cudaSuccess || a.own_maps) return e;
+    return launch_pdl(k_paged_maps, dim3((a.n_tokens + kMapTokens - 1) / kMapTokens), dim3(kMapThreads), 0, st, a);
+}
+
+}  // namespace styx

@@ -1,6 +1,6 @@
 // serve_api.cu -- the C entry points of include/styx_serve.h: validation,
-// workspaces and launches; the kernels are in paged.cu, paged_attn.cu and
-// sample.cu.
+// workspaces and launches; the kernels are in paged.cu, paged_attn.cu,
+// sample.cu, paged_plan.cu, paged_rope.cu and paged_chunk.cu.
 #include <algorithm>
 #include <cmath>
 #include <cstdarg>
@@ -151,16 +151,11 @@ EvictWs evict_ws(const styx_paged_kv *kv, int budget) {
         if (rc_) return rc_;                                                                       \
     } while (0)
 
-}  // namespace
-
-extern "C" {
-
-int styx_paged_append(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv, int n_tokens, int n_heads,
-                      const float *q, int64_t q_stride, const float *k, int64_t k_stride, const float *v,
-                      int64_t v_stride, const float *q_norm, const float *k_norm, float eps, float freq_base,
-                      const int32_t *pos, const int32_t *seq, const int32_t *row, float *q_out) {
-    styx::PagedAppendArgs a{};
-    int sms = 0;
+// what styx_paged_append and its rotary form have in common; q_size: bytes of an element of q_out
+int append_args(styx_ctx *ctx, const styx_paged_kv *kv, int n_tokens, int n_heads, const float *q, int64_t q_stride, const float *k,
+                int64_t k_stride, const float *v, int64_t v_stride, const float *q_norm, const float *k_norm, float eps,
+                const int32_t *pos, const int32_t *seq, const int32_t *row, const void *q_out, uint64_t q_size,
+                styx::PagedAppendArgs &a, int &sms) {
     CHECK(styx::ctx_enter(ctx, &sms, &a.kv.err));
     CHECK(check_kv(kv, true, a.kv));
     NEED(n_tokens > 0 && n_heads >= 0 && static_cast<int64_t>(n_tokens) * (n_heads + kv->n_kv_heads) < (int64_t(1) << 31),
@@ -170,8 +165,7 @@ int styx_paged_append(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv
     const int64_t qd = static_cast<int64_t>(n_heads) * kv->head_dim, kd = static_cast<int64_t>(kv->n_kv_heads) * kv->head_dim;
     NEED(k && v && pos && (n_heads == 0 || (q && q_out)), "null pointer");
     NEED((n_heads == 0 || q_stride >= qd) && k_stride >= kd && v_stride >= kd, "a token stride smaller than its heads");
-    NEED(freq_base > 0.f, "freq_base must be positive");
-    NEED((n_heads == 0 || (rows_ok(q, n_tokens, q_stride, qd, 4) && rows_ok(q_out, n_tokens, qd, qd, 4))) &&
+    NEED((n_heads == 0 || (rows_ok(q, n_tokens, q_stride, qd, 4) && rows_ok(q_out, n_tokens, qd, qd, q_size))) &&
              rows_ok(k, n_tokens, k_stride, kd, 4) && rows_ok(v, n_tokens, v_stride, kd, 4),
          "q / k / v / q_out smaller than n_tokens");
     NEED(styx::range_ok(pos, n_tokens * 4ull) && styx::range_ok(seq, seq ? n_tokens * 4ull : 0) &&
@@ -179,7 +173,7 @@ int styx_paged_append(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv
              styx::range_ok(k_norm, k_norm ? kv->head_dim * 4ull : 0),
          "pos / seq / row / norms too small");
     if (n_heads) {
-        const Span to(q_out, n_tokens, qd, qd, 4);
+        const Span to(q_out, n_tokens, qd, qd, q_size);
         NEED(to.apart(Span(q, n_tokens, q_stride, qd, 4)), "q_out overlaps q");
         NEED(to.apart(Span(k, n_tokens, k_stride, kd, 4)) && to.apart(Span(v, n_tokens, v_stride, kd, 4)), "q_out overlaps k or v");
     }
@@ -192,15 +186,213 @@ int styx_paged_append(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv
     a.q_norm = q_norm;
     a.k_norm = k_norm;
     a.eps = eps;
-    a.log2_base = -2.0 / static_cast<double>(kv->head_dim) * std::log2(static_cast<double>(freq_base));
-    a.step = std::exp2(a.log2_base);
     a.pos = pos;
     a.seq = seq;
     a.row = row;
-    a.q_out = q_out;
     a.n_tokens = n_tokens;
     a.n_heads = n_heads;
+    return STYX_OK;
+}
+
+// attend_chunk's workspace: two partial results per worker, and what has to be joined
+struct ChunkWs {
+    uint64_t joins, total;
+};
+ChunkWs chunk_ws(const styx::PagedKv &kv, int sms) {
+    ChunkWs w{};
+    w.joins = a256(styx::chunk_mma_parts(kv, sms));
+    w.total = w.joins + a256(sms * 16ull);
+    return w;
+}
+
+}  // namespace
+
+extern "C" {
+
+int styx_paged_append(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv, int n_tokens, int n_heads,
+                      const float *q, int64_t q_stride, const float *k, int64_t k_stride, const float *v,
+                      int64_t v_stride, const float *q_norm, const float *k_norm, float eps, float freq_base,
+                      const int32_t *pos, const int32_t *seq, const int32_t *row, float *q_out) {
+    styx::PagedAppendArgs a{};
+    int sms = 0;
+    CHECK(append_args(ctx, kv, n_tokens, n_heads, q, q_stride, k, k_stride, v, v_stride, q_norm, k_norm, eps, pos, seq, row,
+                      q_out, 4, a, sms));
+    NEED(freq_base > 0.f, "freq_base must be positive");
+    a.log2_base = -2.0 / static_cast<double>(kv->head_dim) * std::log2(static_cast<double>(freq_base));
+    a.step = std::exp2(a.log2_base);
+    a.q_out = q_out;
     CK(styx::launch_paged_append(a, sms, S(stream)));
+    return STYX_OK;
+}
+
+int styx_paged_append_rope(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv, int n_tokens, int n_heads,
+                           const float *q, int64_t q_stride, const float *k, int64_t k_stride, const float *v,
+                           int64_t v_stride, const float *q_norm, const float *k_norm, float eps,
+                           const styx_rope *rope, const int32_t *pos, const int32_t *seq, const int32_t *row,
+                           int q_type, void *q_out) {
+    styx::PagedAppendArgs a{};
+    int sms = 0;
+    NEED(kv, "null styx_paged_kv");
+    NEED(q_type == STYX_F32 || q_type == kv->dtype, "q_type %d: f32 (0) or the cache's type", q_type);
+    CHECK(append_args(ctx, kv, n_tokens, n_heads, q, q_stride, k, k_stride, v, v_stride, q_norm, k_norm, eps, pos, seq, row,
+                      q_out, q_type == STYX_F32 ? 4 : 2, a, sms));
+    NEED(rope && rope->freq, "null rope");
+    NEED(rope->n_dims > 0 && rope->n_dims % 2 == 0 && rope->n_dims <= kv->head_dim, "n_dims %d: even, <= head_dim %d", rope->n_dims,
+         kv->head_dim);
+    NEED(aligned(rope->freq, 8) && styx::range_ok(rope->freq, rope->n_dims * 4ull), "freq smaller than n_dims / 2");
+    if (n_heads) {
+        const int64_t qd = static_cast<int64_t>(n_heads) * kv->head_dim;
+        NEED(Span(q_out, n_tokens, qd, qd, q_type == STYX_F32 ? 4 : 2).apart(Span(rope->freq, rope->n_dims * 4ull)), "q_out overlaps freq");
+    }
+    const styx::PagedRope r{rope->freq, rope->n_dims, rope->interleaved != 0, rope->magnitude};
+    CK(styx::launch_paged_append_rope(a, r, q_out, q_type != STYX_F32, sms, S(stream)));
+    return STYX_OK;
+}
+
+int styx_rope_freqs(const styx_rope_params *p, const float *factors, double *freq, float *magnitude) {
+    NEED(p && freq && magnitude, "null pointer");
+    NEED(p->n_dims > 0 && p->n_dims % 2 == 0 && p->n_dims <= 4096, "n_dims %d: even, <= 4096", p->n_dims);
+    NEED(p->base > 1.0 && std::isfinite(p->base), "base %g: above 1", p->base);
+    NEED(p->scaling == STYX_ROPE_NONE || p->scaling == STYX_ROPE_LINEAR || p->scaling == STYX_ROPE_YARN, "scaling %d", p->scaling);
+    const bool yarn = p->scaling == STYX_ROPE_YARN;
+    NEED(p->scaling == STYX_ROPE_NONE || (p->factor >= 1.0 && std::isfinite(p->factor)), "factor %g: at least 1", p->factor);
+    NEED(!yarn || (p->orig_ctx > 0 && std::isfinite(p->orig_ctx) && p->beta_fast > 0 && p->beta_slow > 0 &&
+                   std::isfinite(p->beta_fast) && std::isfinite(p->beta_slow)),
+         "yarn: orig_ctx %g, beta_fast %g, beta_slow %g must be positive", p->orig_ctx, p->beta_fast, p->beta_slow);
+    const int n = p->n_dims;
+    for (int i = 0; factors && i < n / 2; i++) NEED(factors[i] > 0.f && std::isfinite(factors[i]), "factors[%d] must be positive", i);
+    auto dim = [&](double turns) {
+        return n * std::log(p->orig_ctx / (2 * 3.14159265358979323846 * turns)) / (2 * std::log(p->base));
+    };
+    const double lo = yarn ? std::max(0.0, std::floor(dim(p->beta_fast))) : 0.0;
+    const double hi = yarn ? std::min(n - 1.0, std::ceil(dim(p->beta_slow))) : 0.0;
+    for (int i = 0; i < n / 2; i++) {
+        double f = std::pow(p->base, -2.0 * i / n);
+        if (factors) f /= static_cast<double>(factors[i]);
+        const double r = yarn ? std::min(1.0, std::max(0.0, (i - lo) / std::max(hi - lo, 0.001))) : 0.0;
+        freq[i] = p->scaling == STYX_ROPE_LINEAR ? f / p->factor : yarn ? f * (1.0 - r) + f / p->factor * r : f;
+    }
+    *magnitude = yarn ? static_cast<float>(1.0 + 0.1 * std::log(p->factor)) : 1.f;
+    return STYX_OK;
+}
+
+int styx_paged_plan(styx_ctx *ctx, styx_stream stream, const styx_page_table *pt, const int32_t *want, int n_tokens,
+                    const int32_t *next_pos, int32_t *start, int32_t *seq, int32_t *row, int32_t *pos,
+                    int32_t *lens_out, int32_t *held_out, int32_t *n_free_out, int32_t *next_pos_out) {
+    styx::PagedPlanArgs a{};
+    CHECK(styx::ctx_enter(ctx, nullptr, &a.err));
+    NEED(pt, "null styx_page_table");
+    NEED(pt->page_size > 0 && pt->page_size <= 4096 && (pt->page_size & (pt->page_size - 1)) == 0,
+         "page_size %d: a power of two, <= 4096, needed", pt->page_size);
+    NEED(pt->n_seqs > 0 && pt->n_seqs <= 65535, "n_seqs %d: 1 to 65535", pt->n_seqs);
+    NEED(pt->n_pages > 0 && pt->max_pages > 0 && pt->table_stride >= pt->max_pages, "n_pages %d, max_pages %d, table_stride %d",
+         pt->n_pages, pt->max_pages, pt->table_stride);
+    NEED(static_cast<int64_t>(pt->max_pages) * pt->page_size < (int64_t(1) << 31) - 4096,
+         "max_pages %d x page_size %d: fewer than 2^31 rows needed", pt->max_pages, pt->page_size);
+    NEED(n_tokens > 0 && n_tokens <= (1 << 30), "n_tokens %d", n_tokens);
+    NEED(pt->table && pt->free && pt->n_free && pt->lens && pt->held && want && start && seq && row && pos && lens_out &&
+             held_out && n_free_out,
+         "null pointer");
+    NEED((next_pos != nullptr) == (next_pos_out != nullptr), "next_pos and next_pos_out: both or neither");
+    const uint64_t n4 = pt->n_seqs * 4ull, t4 = n_tokens * 4ull;
+    // outputs first; of the inputs the last four may each be the output of the same number
+    const Span outs[10] = {{lens_out, n4}, {held_out, n4}, {n_free_out, 4}, {next_pos_out, n4}, {start, n4 + 4}, {seq, t4},
+                           {row, t4}, {pos, t4}, {pt->free, pt->n_pages * 4ull},
+                           Span(pt->table, pt->n_seqs, pt->table_stride, pt->max_pages, 4)};
+    const Span ins[5] = {{pt->lens, n4}, {pt->held, n4}, {pt->n_free, 4}, {next_pos, n4}, {want, n4}};
+    for (const Span &o : outs) NEED(styx::range_ok(o.begin, static_cast<uint64_t>(o.end - o.begin)), "an output smaller than needed");
+    for (const Span &i : ins) NEED(styx::range_ok(i.begin, static_cast<uint64_t>(i.end - i.begin)), "an input smaller than n_seqs");
+    for (int o = 0; o < 10; o++) {
+        for (int i = 0; i < 5; i++)
+            NEED(outs[o].apart(ins[i]) || (o == i && o < 4 && outs[o].begin == ins[i].begin), "an output overlaps an input that is not its own");
+        for (int p = 0; p < o; p++) NEED(outs[o].apart(outs[p]), "outputs overlap");
+    }
+    a.table = pt->table;
+    a.free = pt->free;
+    a.want = want;
+    a.lens = pt->lens;
+    a.held = pt->held;
+    a.n_free = pt->n_free;
+    a.next_pos = next_pos;
+    a.start = start;
+    a.seq = seq;
+    a.row = row;
+    a.pos = pos;
+    a.lens_out = lens_out;
+    a.held_out = held_out;
+    a.n_free_out = n_free_out;
+    a.next_pos_out = next_pos_out;
+    a.table_stride = pt->table_stride;
+    a.n_seqs = pt->n_seqs;
+    a.max_pages = pt->max_pages;
+    a.page_shift = __builtin_ctz(static_cast<unsigned>(pt->page_size));
+    a.n_pages = pt->n_pages;
+    a.n_tokens = n_tokens;
+    CK(styx::launch_paged_plan(a, S(stream)));
+    return STYX_OK;
+}
+
+int styx_paged_chunk_workspace_bytes(styx_ctx *ctx, const styx_paged_kv *kv, int n_heads, int q_type, uint64_t *out) {
+    styx::PagedKv o{};
+    int sms = 0;
+    CHECK(styx::ctx_enter(ctx, &sms, nullptr));
+    CHECK(check_kv(kv, false, o));
+    NEED(out && n_heads > 0 && n_heads % kv->n_kv_heads == 0, "n_heads %d must be a multiple of n_kv_heads %d", n_heads,
+         kv->n_kv_heads);
+    NEED(q_type == STYX_F32 || q_type == kv->dtype, "q_type %d: f32 (0) or the cache's type", q_type);
+    *out = chunk_ws(o, sms).total;
+    return STYX_OK;
+}
+
+int styx_paged_attend_chunk(styx_ctx *ctx, styx_stream stream, const styx_paged_kv *kv, int n_tokens, int n_heads,
+                            int q_type, const void *q, int64_t q_stride, const int32_t *start, float scale, int window,
+                            void *out, float *lse, void *workspace, uint64_t workspace_bytes) {
+    styx::PagedChunkArgs a{};
+    int sms = 0;
+    CHECK(styx::ctx_enter(ctx, &sms, &a.kv.err));
+    CHECK(check_kv(kv, true, a.kv));
+    NEED(n_heads > 0 && n_heads <= 65535 && n_heads % kv->n_kv_heads == 0, "n_heads %d must be a multiple of n_kv_heads %d",
+         n_heads, kv->n_kv_heads);
+    NEED(n_tokens > 0 && static_cast<int64_t>(n_tokens) * n_heads < (int64_t(1) << 31), "n_tokens %d, n_heads %d", n_tokens, n_heads);
+    NEED(q_type == STYX_F32 || q_type == kv->dtype, "q_type %d: f32 (0) or the cache's type", q_type);
+    const uint64_t size = q_type == STYX_F32 ? 4 : 2;
+    const int64_t qd = static_cast<int64_t>(n_heads) * kv->head_dim;
+    NEED(q && out && start && workspace, "null pointer");
+    NEED(aligned(q, 16) && aligned(out, 16) && aligned(workspace, 256),
+         "q and out must be 16-byte aligned, the workspace 256-byte");
+    NEED(q_stride >= qd && q_stride * size % 16 == 0, "q_stride %lld: at least n_heads x head_dim, 16-byte multiples",
+         static_cast<long long>(q_stride));
+    NEED(window >= 0, "window %d", window);
+    NEED(std::isfinite(scale), "scale must be finite");
+    const Span outs[3] = {Span(out, n_tokens, qd, qd, size), Span(lse, lse ? static_cast<uint64_t>(n_tokens) * n_heads * 4 : 0),
+                          Span(workspace, workspace_bytes)};
+    const Span ins[2] = {Span(q, n_tokens, q_stride, qd, size), Span(start, kv->n_seqs * 4ull + 4)};
+    NEED(rows_ok(q, n_tokens, q_stride, qd, size) && rows_ok(out, n_tokens, qd, qd, size) &&
+             styx::range_ok(lse, lse ? static_cast<uint64_t>(n_tokens) * n_heads * 4 : 0) && styx::range_ok(start, kv->n_seqs * 4ull + 4),
+         "q / out / lse / start smaller than n_tokens, n_seqs + 1");
+    const ChunkWs w = chunk_ws(a.kv, sms);
+    NEED(workspace_bytes >= w.total && styx::range_ok(workspace, w.total), "workspace: %llu bytes needed",
+         static_cast<unsigned long long>(w.total));
+    for (int o = 0; o < 3; o++) {
+        NEED(outs[o].apart(ins[0]) && outs[o].apart(ins[1]) && clear_of_lengths(kv, outs[o]),
+             "an output or the workspace overlaps q, start, lens or the table");
+        for (int p = 0; p < o; p++) NEED(outs[o].apart(outs[p]), "outputs or the workspace overlap each other");
+    }
+    char *ws = static_cast<char *>(workspace);
+    a.q = q;
+    a.out = out;
+    a.lse = lse;
+    a.start = start;
+    a.q_stride = q_stride;
+    a.scale = scale;
+    a.window = window;
+    a.n_tokens = n_tokens;
+    a.n_heads = n_heads;
+    a.gqa = n_heads / kv->n_kv_heads;
+    a.q16 = q_type != STYX_F32;
+    a.part = reinterpret_cast<float *>(ws);
+    a.joins = ws + w.joins;
+    CK(styx::launch_chunk_mma(a, sms, S(stream)));
     return STYX_OK;
 }
 

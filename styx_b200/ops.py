@@ -691,7 +691,7 @@ def _i32(t: torch.Tensor, shape: tuple, what: str, index: int, dtype=torch.int32
 
 
 def _token_rows(t: torch.Tensor, n: int, heads: int, hd: int, what: str, index: int, dtype=torch.float32) -> tuple:
-    """(address, floats between tokens) of f32 [n][heads][hd] whose heads are contiguous."""
+    """(address, elements between tokens) of [n][heads][hd] whose heads are contiguous."""
     shape = (n, heads, hd)
     if t.dtype is dtype and t.shape == shape and t.get_device() == index:
         if t.is_contiguous():
@@ -699,7 +699,7 @@ def _token_rows(t: torch.Tensor, n: int, heads: int, hd: int, what: str, index: 
         sn, sh, se = t.stride()
         if se == 1 and (sh == hd or heads == 1):
             return t.data_ptr(), sn if n > 1 else heads * hd
-    raise ValueError(f"{what}: float32 [{n}][{heads}][{hd}] with contiguous heads on cuda:{index} expected, got "
+    raise ValueError(f"{what}: {dtype} [{n}][{heads}][{hd}] with contiguous heads on cuda:{index} expected, got "
                      f"{t.dtype} {tuple(t.shape)} strides {t.stride()} on {t.device}")
 
 
@@ -779,33 +779,80 @@ class PagedKV:
         self._lens = t
 
     def append(self, q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor,
-               freq_base: float, q_norm: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None,
-               eps: float = 1e-6, seq: Optional[torch.Tensor] = None, row: Optional[torch.Tensor] = None,
-               out: Optional[torch.Tensor] = None, stream=None) -> Optional[torch.Tensor]:
+               freq_base: Optional[float] = None, q_norm: Optional[torch.Tensor] = None,
+               k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6, seq: Optional[torch.Tensor] = None,
+               row: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None, stream=None,
+               rope: Optional["Rope"] = None) -> Optional[torch.Tensor]:
         """Per-head RMSNorm and RoPE of q [n][n_heads][head_dim] and k
         [n][n_kv_heads][head_dim] at pos int32 [n], the K and V rows into the
         pages; returns the rotated q.  Token t is of sequence seq[t] (None: t)
         and goes to its row row[t] (None: lens - 1).  q, k and v may be slices
-        of one projection's output (any stride between tokens)."""
+        of one projection's output (any stride between tokens).  The rotation
+        is NEOX over the whole head with base freq_base, or what `rope` says;
+        with it q may be written in the cache's type (that of `out`)."""
         dev, hd, n_kv = self.index, self.head_dim, self.n_kv_heads
+        if (freq_base is None) == (rope is None):
+            raise ValueError("append: freq_base or rope")
         n, n_heads = pos.shape[0], 0 if q is None else q.shape[1]
-        qp, qs, op = None, 0, None
+        qp, qs, op, q_type = None, 0, None, _lib.F32
         if q is not None:
             qp, qs = _token_rows(q, n, n_heads, hd, "q", dev)
             if out is None:
                 out = _empty((n, n_heads, hd), torch.float32, self.device, stream)
-            op = _f32(out, (n, n_heads, hd), "out", dev)
+            if rope is not None and out.dtype is self.k.dtype:
+                q_type = self._kv.dtype
+                op = _i32(out, (n, n_heads, hd), "out", dev, out.dtype)
+            else:
+                op = _f32(out, (n, n_heads, hd), "out", dev)
         kp, ks = _token_rows(k, n, n_kv, hd, "k", dev)
         vp, vs = _token_rows(v, n, n_kv, hd, "v", dev)
-        rc = self._lib.styx_paged_append(
-            self.ctx.handle, _current(dev) if stream is None else stream.cuda_stream, self._ref, n, n_heads, qp, qs,
-            kp, ks, vp, vs, None if q_norm is None else _f32(q_norm, (hd,), "q_norm", dev),
-            None if k_norm is None else _f32(k_norm, (hd,), "k_norm", dev), eps, freq_base,
-            _i32(pos, (n,), "pos", dev), None if seq is None else _i32(seq, (n,), "seq", dev),
-            None if row is None else _i32(row, (n,), "row", dev), op)
+        head = (self.ctx.handle, _current(dev) if stream is None else stream.cuda_stream, self._ref, n, n_heads, qp, qs,
+                kp, ks, vp, vs, None if q_norm is None else _f32(q_norm, (hd,), "q_norm", dev),
+                None if k_norm is None else _f32(k_norm, (hd,), "k_norm", dev), eps)
+        tail = (_i32(pos, (n,), "pos", dev), None if seq is None else _i32(seq, (n,), "seq", dev),
+                None if row is None else _i32(row, (n,), "row", dev))
+        if rope is None:
+            rc = self._lib.styx_paged_append(*head, freq_base, *tail, op)
+        else:
+            if rope.index != dev:
+                raise ValueError(f"rope on cuda:{rope.index}, cache on cuda:{dev}")
+            rc = self._lib.styx_paged_append_rope(*head, rope._ref, *tail, q_type, op)
         if rc:
             check(rc)
         return out if q is not None else None
+
+    def attend_chunk(self, q: torch.Tensor, start: torch.Tensor, scale: Optional[float] = None, window: int = 0,
+                     out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
+                     stream=None) -> torch.Tensor:
+        """Causal attention of new tokens, q [n][n_heads][head_dim] (any stride
+        between tokens), over their sequences' rows: tokens start[b] ..
+        start[b + 1] - 1 (int32 [n_seqs + 1]) are the last rows of sequence b,
+        and each sees the rows up to its own (the last `window` of them, 0:
+        all); scale None: head_dim ** -0.5.  q and out are f32, or both of a
+        16-bit cache's type.  lse f32 [n][n_heads] receives the log of the
+        softmax denominators.  Rows of out and lse that are no sequence's stay
+        as they are."""
+        dev, hd = self.index, self.head_dim
+        if q.dim() != 3 or q.dtype is not torch.float32 and q.dtype is not self.k.dtype:
+            raise ValueError(f"q: [n][n_heads][{hd}], float32 or {self.k.dtype}, expected, got {q.dtype} {tuple(q.shape)}")
+        n, n_heads = q.shape[0], q.shape[1]
+        qp, qs = _token_rows(q, n, n_heads, hd, "q", dev, q.dtype)
+        q_type = _KV_TYPES[q.dtype]
+        out = _empty((n, n_heads, hd), q.dtype, self.device, stream) if out is None else out
+        ws = self._attend_ws.get((n_heads, q_type, "chunk"))
+        if ws is None:
+            nb = C.c_uint64()
+            check(self._lib.styx_paged_chunk_workspace_bytes(self.ctx.handle, self._ref, n_heads, q_type, C.byref(nb)))
+            t = _empty((nb.value,), torch.uint8, self.device, stream)
+            ws = self._attend_ws[(n_heads, q_type, "chunk")] = (t, t.data_ptr(), nb.value)
+        rc = self._lib.styx_paged_attend_chunk(
+            self.ctx.handle, _current(dev) if stream is None else stream.cuda_stream, self._ref, n, n_heads, q_type, qp, qs,
+            _i32(start, (self.n_seqs + 1,), "start", dev), self._scale if scale is None else scale, window,
+            _f32(out, (n, n_heads, hd), "out", dev, q.dtype), None if lse is None else _f32(lse, (n, n_heads), "lse", dev),
+            ws[1], ws[2])
+        if rc:
+            check(rc)
+        return out
 
     def _attend_workspace(self, n_heads: int, with_acc: bool, stream=None) -> tuple:
         nb = C.c_uint64()
@@ -883,6 +930,94 @@ class PagedKV:
         if rc:
             check(rc)
         return acc_out, pos_out, lens_out
+
+
+class Rope:
+    """How heads are turned (styx_rope): of the first n_dims elements the pairs
+    (i, i + n_dims / 2), or (2i, 2i + 1) with `interleaved`, by frequencies
+    base ** (-2i / n_dims), divided by `factors` [n_dims / 2] where given and
+    scaled for longer contexts: scaling "linear" (all by `factor`) or "yarn"
+    (slow pairs by `factor`, fast ones not, in between by the turns that they
+    make over orig_ctx; q and k grow by 1 + 0.1 ln(factor), or `magnitude`)."""
+
+    _SCALINGS = {None: _lib.ROPE_NONE, "linear": _lib.ROPE_LINEAR, "yarn": _lib.ROPE_YARN}
+
+    def __init__(self, n_dims: int, base: float, interleaved: bool = False, scaling: Optional[str] = None,
+                 factor: float = 1.0, orig_ctx: int = 0, beta_fast: float = 32.0, beta_slow: float = 1.0,
+                 factors: Optional[torch.Tensor] = None, magnitude: Optional[float] = None,
+                 device: Optional[int] = None):
+        freq, grow = self.frequencies(n_dims, base, scaling, factor, orig_ctx, beta_fast, beta_slow, factors)
+        self.index = torch.cuda.current_device() if device is None else device
+        self.freq = freq.to(f"cuda:{self.index}")
+        self.n_dims, self.interleaved = n_dims, interleaved
+        self.magnitude = grow if magnitude is None else magnitude
+        self._form = _lib.RopeForm(self.freq.data_ptr(), n_dims, int(interleaved), self.magnitude)
+        self._ref = C.byref(self._form)
+
+    @classmethod
+    def frequencies(cls, n_dims: int, base: float, scaling: Optional[str] = None, factor: float = 1.0, orig_ctx: int = 0,
+                    beta_fast: float = 32.0, beta_slow: float = 1.0, factors: Optional[torch.Tensor] = None):
+        """(radians per position float64 [n_dims / 2] on the host, magnitude) (styx_rope_freqs)."""
+        if scaling not in cls._SCALINGS:
+            raise ValueError(f"scaling {scaling!r}: one of {list(cls._SCALINGS)}")
+        if factors is not None:
+            if factors.shape != (n_dims // 2,):
+                raise ValueError(f"factors: [{n_dims // 2}] expected, got {tuple(factors.shape)}")
+            factors = factors.detach().to("cpu", torch.float32).contiguous()
+        freq, grow = torch.empty(max(0, n_dims // 2), dtype=torch.float64), C.c_float()
+        params = _lib.RopeParams(n_dims, cls._SCALINGS[scaling], base, factor, orig_ctx, beta_fast, beta_slow)
+        check(lib().styx_rope_freqs(C.byref(params), None if factors is None else factors.data_ptr(), freq.data_ptr(),
+                                    C.byref(grow)))
+        return freq, grow.value
+
+
+class PagedPlan:
+    """Rows and pages of the next tokens of every sequence (styx_paged_plan).
+
+    table int32 [n_seqs][max_pages] and free int32 [n_pages], the stack of
+    pages that nobody has, are the caller's and changed in place; n_tokens is
+    how many tokens a run hands out at most.  The results are attributes,
+    written anew by every run: start [n_seqs + 1]; seq, row and pos [n_tokens]
+    as PagedKV.append takes them (past start[n_seqs] padding that writes no
+    row); lens, held, n_free and next_pos after the granted tokens, which the
+    next run may take as its inputs."""
+
+    def __init__(self, table: torch.Tensor, page_size: int, free: torch.Tensor, n_tokens: int, stream=None):
+        if table.dim() != 2 or table.dtype != torch.int32 or not table.is_cuda or (table.shape[1] > 1 and table.stride(1) != 1):
+            raise ValueError("table: int32 [n_seqs][max_pages] CUDA tensor with contiguous rows")
+        if n_tokens < 1:
+            raise ValueError(f"n_tokens {n_tokens}")
+        n, dev = table.shape[0], table.device
+        self.table, self.free, self.n_tokens, self.n_seqs, self.index = table, free, n_tokens, n, dev.index
+        self.ctx = ctx(self.index)
+        i32 = torch.int32
+        self.start = _empty((n + 1,), i32, dev, stream)
+        self.seq, self.row, self.pos = (_empty((n_tokens,), i32, dev, stream) for _ in range(3))
+        self.lens, self.held, self.next_pos = (_empty((n,), i32, dev, stream) for _ in range(3))
+        self.n_free = _empty((1,), i32, dev, stream)
+        self._pt = _lib.PageTable(table.data_ptr(), _i32(free, (free.numel(),), "free", self.index), None, None, None, n,
+                                  table.shape[1], table.stride(0) if n > 1 else table.shape[1], page_size, free.numel())
+        self._ref = C.byref(self._pt)
+        self._out = tuple(t.data_ptr() for t in (self.start, self.seq, self.row, self.pos, self.lens, self.held, self.n_free))
+        self._lib = lib()
+
+    def run(self, want: torch.Tensor, lens: torch.Tensor, held: torch.Tensor, n_free: torch.Tensor,
+            next_pos: Optional[torch.Tensor] = None, stream=None) -> "PagedPlan":
+        """As many of the want[b] next tokens of every sequence as n_tokens and
+        the pages allow, in the order of the sequences; pages past what a
+        sequence needs go back.  lens and held: its rows and pages now,
+        n_free [1]: pages on the stack, next_pos: the next token's position
+        (None: its row).  All int32.  Returns self."""
+        dev, pt, one = self.index, self._pt, (self.n_seqs,)
+        pt.lens, pt.held = _i32(lens, one, "lens", dev), _i32(held, one, "held", dev)
+        pt.n_free = _i32(n_free, (1,), "n_free", dev)
+        rc = self._lib.styx_paged_plan(
+            self.ctx.handle, _current(dev) if stream is None else stream.cuda_stream, self._ref,
+            _i32(want, one, "want", dev), self.n_tokens, None if next_pos is None else _i32(next_pos, one, "next_pos", dev),
+            *self._out, None if next_pos is None else self.next_pos.data_ptr())
+        if rc:
+            check(rc)
+        return self
 
 
 def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Optional[torch.Tensor] = None,
