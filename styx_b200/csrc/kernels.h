@@ -432,6 +432,7 @@ struct PagedChunkArgs {
     int q16;                                   // q and out are of the cache's 16-bit type
     // the launch's cut of the work, see paged_chunk.cuh
     int hg, groups, heads;                     // heads of a tile; groups of a kv head; kv heads x groups
+    int tile_tok;                              // tokens of a query tile
     int tok_shift, key_shift, seg_cost, workers, part_floats;
     float *part;                               // workspace
     void *joins;                               // workspace, one ChunkJoin per worker
@@ -472,9 +473,14 @@ uint64_t attend_fma_parts(int sms);            // bytes of the portions' results
 uint64_t attend_mma_parts(int gqa, int sms);
 cudaError_t launch_paged_plan(PagedPlanArgs a, cudaStream_t st);
 cudaError_t launch_paged_append_rope(const PagedAppendArgs &a, const PagedRope &r, void *q_out, bool q16, int sms, cudaStream_t st);
-// attention of chunks on mma.sync: 16-bit caches, f32 caches; bytes of their portions' results
+// attention of chunks on mma.sync (any shape), on tcgen05; bytes of their portions' results; what ends both: portions of
+// M rows, query tiles of `tile` rows, joined
 cudaError_t launch_chunk_mma(PagedChunkArgs a, int sms, cudaStream_t st);
 uint64_t chunk_mma_parts(const PagedKv &kv, int sms);
+bool chunk_on_tc(const PagedChunkArgs &a);
+cudaError_t launch_chunk_tc(PagedChunkArgs a, int sms, cudaStream_t st);
+uint64_t chunk_tc_parts(int sms);
+cudaError_t launch_chunk_join(const PagedChunkArgs &a, int M, int tile, int pitch, cudaStream_t st);
 cudaError_t launch_paged_evict(const PagedEvictArgs &a, int sms, cudaStream_t st);
 bool evict_staged(long long rows);   // the keys of lines of so many rows fit shared memory
 cudaError_t launch_sample(const SampleArgs &a, cudaStream_t st);

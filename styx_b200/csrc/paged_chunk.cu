@@ -679,20 +679,21 @@ __global__ void __launch_bounds__(Tf<HD>::threads, 1) k_chunk_tf32(PagedChunkArg
 
 // ------------------------------------------------------------ joining
 // A cut segment's portions added up in order, a warp per query row.  M rows of
-// pitch floats a portion.
+// pitch floats a portion, tiles of `tile` rows with a.tile_tok tokens each.
 constexpr int kJoinThreads = 256;
 template <class TQ>
-__global__ void __launch_bounds__(kJoinThreads) k_chunk_join(PagedChunkArgs a, int M, int pitch) {
+__global__ void __launch_bounds__(kJoinThreads) k_chunk_join(PagedChunkArgs a, int M, int tile, int pitch) {
     pdl_trigger();
     pdl_wait();
     const int worker = blockIdx.x, lane = threadIdx.x & 31;
     const ChunkJoin j = static_cast<const ChunkJoin *>(a.joins)[worker];
     if (j.first < 0) return;
     const int r = blockIdx.y * (kJoinThreads / 32) + (threadIdx.x >> 5), hd = a.kv.hd;
-    const int tok = r / a.hg, hr = r - tok * a.hg, kvh = j.head / a.groups, g0 = (j.head - kvh * a.groups) * a.hg;
+    const int nth = r / tile, rt = (r - nth * tile) / a.hg, hr = (r - nth * tile) - rt * a.hg, tok = nth * a.tile_tok + rt;
+    const int kvh = j.head / a.groups, g0 = (j.head - kvh * a.groups) * a.hg;
     const Chunk c(a, j.b, false);
     const int first = j.seg << a.tok_shift;
-    if (r >= M || tok >= min(1 << a.tok_shift, c.n - first) || hr >= min(a.hg, a.gqa - g0)) return;
+    if (r >= M || rt >= a.tile_tok || tok >= min(1 << a.tok_shift, c.n - first) || hr >= min(a.hg, a.gqa - g0)) return;
     const long long row = static_cast<long long>(c.tok0 + first + tok) * a.n_heads + kvh * a.gqa + g0 + hr;
     float top = kNone;
     for (int w = j.first; w <= worker; w++) top = fmaxf(top, chunk_part(a, w, w == j.first)[M * pitch + r]);
@@ -751,11 +752,11 @@ uint64_t chunk_mma_parts(const PagedKv &kv, int sms) {
 }
 
 // the portions joined; a's cut of the work and workspace are set
-cudaError_t launch_chunk_join(const PagedChunkArgs &a, int M, int pitch, cudaStream_t st) {
+cudaError_t launch_chunk_join(const PagedChunkArgs &a, int M, int tile, int pitch, cudaStream_t st) {
     const dim3 grid(a.workers, (M + kJoinThreads / 32 - 1) / (kJoinThreads / 32));
-    if (!a.q16) return launch_pdl(k_chunk_join<float>, grid, dim3(kJoinThreads), 0, st, a, M, pitch);
-    if (a.kv.dtype == STYX_F16) return launch_pdl(k_chunk_join<__half>, grid, dim3(kJoinThreads), 0, st, a, M, pitch);
-    return launch_pdl(k_chunk_join<__nv_bfloat16>, grid, dim3(kJoinThreads), 0, st, a, M, pitch);
+    if (!a.q16) return launch_pdl(k_chunk_join<float>, grid, dim3(kJoinThreads), 0, st, a, M, tile, pitch);
+    if (a.kv.dtype == STYX_F16) return launch_pdl(k_chunk_join<__half>, grid, dim3(kJoinThreads), 0, st, a, M, tile, pitch);
+    return launch_pdl(k_chunk_join<__nv_bfloat16>, grid, dim3(kJoinThreads), 0, st, a, M, tile, pitch);
 }
 
 cudaError_t launch_chunk_mma(PagedChunkArgs a, int sms, cudaStream_t st) {
@@ -764,6 +765,7 @@ cudaError_t launch_chunk_mma(PagedChunkArgs a, int sms, cudaStream_t st) {
     a.groups = (a.gqa + a.hg - 1) / a.hg;
     a.heads = a.kv.n_kv * a.groups;
     a.tok_shift = log2_floor(M / a.hg);
+    a.tile_tok = 1 << a.tok_shift;
     a.key_shift = key_shift_of(a.kv);
     // a table of one tile's rows: no segment can be cut
     const bool cut = (static_cast<long long>(a.kv.max_pages) << a.kv.page_shift) > (1 << a.key_shift);
@@ -778,7 +780,7 @@ cudaError_t launch_chunk_mma(PagedChunkArgs a, int sms, cudaStream_t st) {
         e = a.q16 ? go_hd<false, 1>(a, st) : go_hd<false, 2>(a, st);
     else
         e = a.q16 ? go_hd<true, 1>(a, st) : go_hd<true, 3>(a, st);
-    return e != cudaSuccess || !cut ? e : launch_chunk_join(a, M, pitch, st);
+    return e != cudaSuccess || !cut ? e : launch_chunk_join(a, M, M, pitch, st);
 }
 
 }  // namespace styx

@@ -1,0 +1,642 @@
+// paged_chunk_tc.cu -- attention of chunks (styx_paged_attend_chunk) on the
+// 5th-generation tensor cores: q and cache of one 16-bit type, head_dim 64 to
+// 128, pages of 16 rows or more.
+//
+// A CTA takes two query tiles of 128 rows (tokens x the q heads of a kv head,
+// so that a kv head's rows are read once for all of them) over tiles of 128
+// keys:
+//   S = Q K^T          tcgen05.mma, both operands from shared memory
+//   P = 2^(S l2 - m)   a thread per query row: no exchange between threads
+//   O += P V           tcgen05.mma, P from TMEM, where it lies over S
+// The two tiles take turns: while one's S and O are being multiplied the
+// other's rows are exponentiated.  The maximum that a row is measured against
+// moves only when a score passes it by 2^8, so O is rescaled rarely and then by
+// the row's own thread.
+//
+// Roles, linked by mbarriers with bounded waits: eight softmax warps (a
+// warpgroup per query tile), a warp that copies (TMA: boxes of min(page, 128)
+// rows x 64 elements of a page, 128-byte swizzled; q with one box per tile and
+// 64 elements), a thread that issues the products, and two warps that go over
+// V where a tile is not seen in whole by all rows: rows outside the sequence
+// (TMA brings whole pages) and numbers that are not finite become zeros, since 0
+// times them would not be 0; the latter are added, at the portion's end, to the
+// rows that see them.  K and V share one ring of slots in the order of use.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <cstring>
+#include <type_traits>
+
+#include "paged_chunk.cuh"
+
+namespace styx {
+namespace {
+
+constexpr int kThreads = 384;
+constexpr int kWarpLoad = 8, kWarpMma = 9, kWarpClean = 10;
+constexpr int kTile = 128;                          // query rows of a tile, keys of a tile
+constexpr int kHalf = kTile * 128;                  // 128 rows of 64 16-bit elements
+constexpr int kSlot = 2 * kHalf;                    // a K or V tile
+constexpr int kSlots = 5;
+constexpr int kSmem = 2 * kSlot + kSlots * kSlot + 1024;
+constexpr uint32_t kTmemCols = 512, kColS = 0, kColO = 256;   // S (and P over it) and O of the two query tiles
+constexpr float kSlack = 8.f;                       // log2 units a score may pass the maximum by
+
+struct Bars {
+    uint64_t full[kSlots], empty[kSlots];
+    uint64_t clean[4];                              // V tile i: clean[i % 4]
+    uint64_t qfull, qempty;
+    uint64_t sfull[2], pfull[2], odone[2];
+    uint64_t drain;
+};
+
+// ------------------------------------------------------------ tensor-core helpers
+// Shared-memory operand descriptors (version 1, 128-byte swizzle).  The high
+// word is the same for all: 1024 bytes between groups of 8 rows (K-major: Q,
+// K) or of 8 along the sum (V, whose elements lie along N).  The low word is
+// address / 16, and for V the bytes / 16 between blocks of 64 elements.
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lbo) { return (addr >> 4) | ((lbo >> 4) << 16); }
+// f32 accumulator, A and B of one type, M 128; b_mn: B's elements lie along N
+__device__ __forceinline__ uint32_t idesc(bool bf, int n, bool b_mn) {
+    return (1u << 4) | (bf ? (1u << 7) | (1u << 10) : 0u) | (b_mn ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) |
+           (static_cast<uint32_t>(kTile >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t id, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}\n" ::"r"(d),
+        "r"(a_lo), "r"(b_lo), "r"(id), "r"(acc), "n"(kDescHi)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t id, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "mov.b64 db, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}\n" ::"r"(d),
+        "r"(a), "r"(b_lo), "r"(id), "r"(acc), "n"(kDescHi)
+        : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t *bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// 32 consecutive columns of this thread's lane
+__device__ __forceinline__ void ld32(uint32_t addr, float *v) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
+        "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr));
+#pragma unroll
+    for (int j = 0; j < 32; j++) v[j] = __uint_as_float(r[j]);
+}
+__device__ __forceinline__ void st32(uint32_t addr, const uint32_t *r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
+        "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
+        "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
+        "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// the loads above are done; no use of their values moves up across this
+template <int N>
+__device__ __forceinline__ void ld_wait(float (&v)[N]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int c = 0; c < N; c++) asm volatile("" : "+f"(v[c]));
+}
+__device__ __forceinline__ void tma3(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+        "[%5];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar))
+        : "memory");
+}
+template <bool BF>
+__device__ __forceinline__ uint32_t pack(float x, float y) {   // low half: x
+    if constexpr (BF) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    } else {
+        const __half2 h = __floats2half2_rn(x, y);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+}
+__device__ __forceinline__ float not_finite(float v) { return fabsf(v) <= 3.4028234e38f ? 0.f : v; }
+
+// a portion: its segment's tokens and heads, its keys [lo, hi)
+struct Part {
+    int b, j, g0, ng, tok0, ntok, base, kb0, tiles, lo, hi, free_lo, free_hi;
+    bool two, begins, ends;
+    __device__ __forceinline__ void set(const PagedChunkArgs &a, const ChunkWalk &w) {
+        const Chunk c(a, w.b, false);
+        b = w.b;
+        j = w.head / a.groups;
+        g0 = (w.head - j * a.groups) * a.hg;
+        ng = min(a.hg, a.gqa - g0);
+        const int first = w.seg << a.tok_shift;
+        tok0 = c.tok0 + first;
+        ntok = max(1, min(1 << a.tok_shift, c.n - first));
+        two = ntok > a.tile_tok;
+        base = c.base + first;
+        const int ft = c.first_tile(a, w.seg);
+        kb0 = (ft + w.t0) << a.key_shift;
+        tiles = w.t1 - w.t0;
+        lo = max(kb0, c.first_row(a, w.seg));
+        hi = static_cast<int>(min(static_cast<long long>(c.end_row(a, w.seg)), static_cast<long long>(ft + w.t1) << a.key_shift));
+        free_hi = base + 1;                         // every token sees all keys in [free_lo, free_hi)
+        free_lo = a.window > 0 ? max(0, base + ntok - a.window) : 0;
+        begins = w.t0 == 0;
+        ends = w.t1 == w.nt;
+    }
+    __device__ __forceinline__ bool partial(int kb) const { return kb + kTile > free_hi || kb < free_lo; }
+};
+
+template <bool BF>
+__global__ void __launch_bounds__(kThreads, 1)
+    k_chunk_tc(PagedChunkArgs a, const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+               const __grid_constant__ CUtensorMap mv) {
+    using T = std::conditional_t<BF, __nv_bfloat16, __half>;
+    constexpr float kBias = BF ? 0.f : 7.f;         // f16 has few exponents: p is carried as p * 2^7
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ Bars bars;
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_abort, s_badpage, s_poison, s_dirty[4];
+    uint8_t *const sm = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
+    const uint32_t sQ = smem_addr(sm), ring = sQ + 2 * kSlot;
+    const PagedKv &kv = a.kv;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, hd = kv.hd;
+    const int halves = hd > 64 ? 2 : 1;
+
+    if (tid == 0) {
+        for (int i = 0; i < kSlots; i++) {
+            mbar_init(&bars.full[i], 1);
+            mbar_init(&bars.empty[i], 1);
+        }
+        for (int i = 0; i < 4; i++) mbar_init(&bars.clean[i], 2);
+        mbar_init(&bars.qfull, 1);
+        mbar_init(&bars.qempty, 1);
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&bars.sfull[i], 1);
+            mbar_init(&bars.pfull[i], 4);
+            mbar_init(&bars.odone[i], 1);
+        }
+        mbar_init(&bars.drain, 1);
+        fence_mbar_init();
+        s_abort = s_badpage = s_poison = 0;
+    }
+    if (tid == 32 * kWarpLoad) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&mq));
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&mk));
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&mv));
+    }
+    pdl_wait();
+    if (warp == kWarpMma) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)),
+                     "r"(kTmemCols));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        fence_before();
+    }
+    __syncthreads();
+    fence_after();
+    pdl_trigger();
+    const uint32_t tmem = s_tmem;
+    long long T_ = 0, G = 0;
+    ChunkWalk wk;
+    const int worker = blockIdx.x;
+    chunk_share(a, worker, wk, T_, G);
+    Part P;
+
+    auto wait = [&](uint64_t *bar, uint32_t parity) {
+        if (mbar_try_wait(bar, parity)) return true;
+        const long long t0 = clock64();
+        while (true) {
+            if (mbar_try_wait_suspend(bar, parity)) return true;
+            if (*reinterpret_cast<volatile int *>(&s_abort)) return false;
+            if (clock64() - t0 > kSpinCycles) {
+                atomicExch(kv.err, kErrWaitFull);
+                *reinterpret_cast<volatile int *>(&s_abort) = 1;
+                return false;
+            }
+        }
+    };
+    auto warp_wait = [&](uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
+
+    if (warp == kWarpLoad) {
+        // ---------------- copies.  A lane has one box of a tile: rows, and 64 of the elements
+        const int rb_shift = min(kv.page_shift, 7), rb = 1 << rb_shift, boxes = kTile >> rb_shift;
+        const int pi = lane / halves, half = lane - pi * halves;
+        const bool mine = pi < boxes;
+        const uint32_t dst = half * kHalf + (pi << rb_shift) * 128;
+        const uint32_t q_bytes = 128u * a.hg * a.tile_tok;
+        int portion = 0, use = 0, slot = 0, nv = 0;       // use: how often the ring has gone round
+        bool live = true;
+        while (live && wk.next(a)) {
+            P.set(a, wk);
+            const int32_t *table = kv.table + static_cast<long long>(P.b) * kv.table_stride;
+            auto page_of = [&](int it) {
+                const int r0 = P.kb0 + it * kTile + (pi << rb_shift);
+                return mine && it < P.tiles && r0 < P.hi && r0 + rb > P.lo ? ld_now(table + (r0 >> kv.page_shift)) : -1;
+            };
+            int page = page_of(0);
+            if (portion > 0) live = warp_wait(&bars.qempty, static_cast<uint32_t>((portion - 1) & 1));
+            if (!live) break;
+            if (lane == 0) {
+                const int nq = P.two ? 2 : 1;
+                mbar_arrive_expect_tx(&bars.qfull, nq * halves * q_bytes);
+                for (int t = 0; t < nq; t++)
+                    for (int h = 0; h < halves; h++)
+                        tma3(sQ + t * kSlot + h * kHalf, &mq, h * 64, P.j * a.gqa + P.g0, P.tok0 + t * a.tile_tok, &bars.qfull);
+            }
+            __syncwarp();
+            portion++;
+            for (int it = 0; it < P.tiles && live; it++) {
+                const int r0 = P.kb0 + it * kTile + (pi << rb_shift), here = page;
+                const bool some = mine && r0 < P.hi && r0 + rb > P.lo;
+                const bool on = some && static_cast<unsigned>(here) < static_cast<unsigned>(kv.n_pages);
+                page = page_of(it + 1);
+                const unsigned n = __popc(__ballot_sync(0xffffffffu, on));
+                const bool bad = __any_sync(0xffffffffu, some && !on);
+                const int y = (P.j << kv.page_shift) + (r0 & ((1 << kv.page_shift) - 1));
+                for (int v = 0; v < 2; v++) {
+                    if (use > 0 && !warp_wait(&bars.empty[slot], static_cast<uint32_t>((use - 1) & 1))) {
+                        live = false;
+                        break;
+                    }
+                    if (lane == 0) {
+                        if (bad) {
+                            atomicExch(kv.err, kErrBadPos);
+                            *reinterpret_cast<volatile int *>(&s_badpage) = 1;
+                        }
+                        if (v) *reinterpret_cast<volatile int *>(&s_dirty[nv & 3]) = bad || P.partial(P.kb0 + it * kTile);
+                        mbar_arrive_expect_tx(&bars.full[slot], n * static_cast<uint32_t>(rb) * 128u);
+                    }
+                    __syncwarp();
+                    if (on) tma3(ring + slot * kSlot + dst, v ? &mv : &mk, half * 64, y, here, &bars.full[slot]);
+                    if (++slot == kSlots) slot = 0, use++;
+                }
+                nv++;
+            }
+        }
+        // Every copy is waited for by the products that read it.  Where a wait gave up, nothing of this warp's may still
+        // be landing when the CTA ends: copies take microseconds, a millisecond is given to them.
+        if (*reinterpret_cast<volatile int *>(&s_abort))
+            for (const long long c0 = clock64(); clock64() - c0 < 2000000;) {
+            }
+    } else if (warp == kWarpMma) {
+        // ---------------- products, all issued by one thread, executed in the order of issue
+        if (lane == 0) {
+            const int ks = (hd + 15) / 16;
+            const uint32_t id_s = idesc(BF, kTile, false), id_o = idesc(BF, ks * 16, true);
+            const uint32_t dQ = desc_lo(sQ, 16);
+            int portion = 0, nv = 0;
+            int kslot = 0, kuse = 0, vslot = 1, vuse = 0;   // ring: K(0) V(0) K(1) V(1) ..., over all portions
+            uint32_t pph[2] = {0, 0};
+            bool live = true;
+            auto step = [](int &slot, int &use) {
+                slot += 2;
+                if (slot >= kSlots) slot -= kSlots, use++;
+            };
+            auto scores = [&](int t) {
+                const uint32_t q = dQ + t * (kSlot / 16), k = desc_lo(ring + kslot * kSlot, 16), d = tmem + kColS + t * kTile;
+                for (int i = 0; i < ks; i++) {
+                    const uint32_t o = (i >> 2) * (kHalf / 16) + (i & 3) * 2;
+                    mma_ss(d, q + o, k + o, id_s, i > 0);
+                }
+                commit(&bars.sfull[t]);
+            };
+            auto values = [&](int t, bool first) {
+                const uint32_t v = desc_lo(ring + vslot * kSlot, kHalf), p = tmem + kColS + t * kTile, d = tmem + kColO + t * kTile;
+#pragma unroll
+                for (int i = 0; i < kTile / 16; i++) mma_ts(d, p + i * 8, v + i * (2048 / 16), id_o, !first || i > 0);
+                commit(&bars.odone[t]);
+            };
+            while (live && wk.next(a)) {
+                P.set(a, wk);
+                const int nq = P.two ? 2 : 1;
+                live = wait(&bars.qfull, static_cast<uint32_t>(portion & 1)) && wait(&bars.full[kslot], static_cast<uint32_t>(kuse & 1));
+                if (!live) break;
+                fence_after();
+                for (int t = 0; t < nq; t++) scores(t);
+                commit(&bars.empty[kslot]);
+                if (P.tiles == 1) commit(&bars.qempty);
+                step(kslot, kuse);
+                for (int it = 0; it < P.tiles && live; it++) {
+                    const bool more = it + 1 < P.tiles;
+                    for (int t = 0; t < nq && live; t++) {
+                        live = wait(&bars.pfull[t], pph[t]) && (t > 0 || wait(&bars.clean[nv & 3], static_cast<uint32_t>((nv >> 2) & 1)));
+                        pph[t] ^= 1;
+                        if (!live) break;
+                        fence_after();
+                        values(t, it == 0);
+                        if (t == nq - 1) commit(&bars.empty[vslot]);
+                        if (more) {
+                            if (t == 0) {
+                                live = wait(&bars.full[kslot], static_cast<uint32_t>(kuse & 1));
+                                if (!live) break;
+                                fence_after();
+                            }
+                            scores(t);
+                            if (t == nq - 1) {
+                                commit(&bars.empty[kslot]);
+                                if (it + 2 == P.tiles) commit(&bars.qempty);
+                            }
+                        }
+                    }
+                    if (more) step(kslot, kuse);
+                    step(vslot, vuse);
+                    nv++;
+                }
+                portion++;
+            }
+            // every product issued here has completed before TMEM is freed
+            commit(&bars.drain);
+            mbar_wait(&bars.drain, 0u, kv.err, kErrWaitFull);
+        }
+        __syncwarp();
+    } else if (warp >= kWarpClean) {
+        // ---------------- V tiles that are not seen in whole
+        const int ct = tid - 32 * kWarpClean;
+        int slot = 1, use = 0, nv = 0;
+        bool live = true;
+        while (live && wk.next(a)) {
+            P.set(a, wk);
+            for (int it = 0; it < P.tiles; it++, nv++) {
+                live = warp_wait(&bars.full[slot], static_cast<uint32_t>(use & 1));
+                if (!live) break;
+                if (*reinterpret_cast<volatile int *>(&s_dirty[nv & 3])) {
+                    const int32_t *table = kv.table + static_cast<long long>(P.b) * kv.table_stride;
+                    uint8_t *v = sm + 2 * kSlot + slot * kSlot;
+                    for (int row = ct; row < kTile; row += 64) {
+                        const int key = P.kb0 + it * kTile + row;
+                        const bool in = key >= P.lo && key < P.hi &&
+                                        static_cast<unsigned>(ld_now(table + (key >> kv.page_shift))) < static_cast<unsigned>(kv.n_pages);
+                        for (int c = 0; c < 8 * halves; c++) {
+                            // (the swizzle permutes the 16-byte groups of a row: all of them are looked at)
+                            uint4 *p = reinterpret_cast<uint4 *>(v + (c >> 3) * kHalf + row * 128 + (c & 7) * 16);
+                            if (!in) {
+                                *p = make_uint4(0, 0, 0, 0);
+                                continue;
+                            }
+                            const uint4 x = *p;
+                            uint32_t w[4] = {x.x, x.y, x.z, x.w};
+                            bool bad = false;
+                            constexpr uint32_t E = BF ? 0x7F80u : 0x7C00u;
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                if ((w[k] & E) == E) w[k] &= 0xFFFF0000u, bad = true;
+                                if ((w[k] >> 16 & E) == E) w[k] &= 0xFFFFu, bad = true;
+                            }
+                            if (bad) {
+                                *p = make_uint4(w[0], w[1], w[2], w[3]);
+                                *reinterpret_cast<volatile int *>(&s_poison) = 1;
+                            }
+                        }
+                    }
+                    fence_async();
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars.clean[nv & 3]);
+                slot += 2;
+                if (slot >= kSlots) slot -= kSlots, use++;
+            }
+        }
+    } else {
+        // ---------------- softmax: thread = query row
+        const int t = warp >> 2, r = tid & 127;
+        const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
+        const uint32_t colS = tmem + kColS + t * kTile + lanes, colO = tmem + kColO + t * kTile + lanes;
+        const float l2 = a.scale * 1.4426950408889634f;   // scores in units of log2
+        const int rt = r / a.hg, rh = r - rt * a.hg;
+        uint32_t sph = 0, oph = 0;
+        bool first = true, live = true;
+        while (live && wk.next(a)) {
+            P.set(a, wk);
+            if (first && tid == 0) {
+                ChunkJoin j{-1, 0, 0, 0};
+                if (!P.begins && P.ends) j = {chunk_owner(a, wk, T_, G), wk.b, wk.head, wk.seg};
+                static_cast<ChunkJoin *>(a.joins)[worker] = j;
+            }
+            first = false;
+            if (t == 1 && !P.two) continue;
+            const int tok = t * a.tile_tok + rt;
+            const bool real = rt < a.tile_tok && tok < P.ntok && rh < P.ng;
+            const int see_hi = real ? min(P.hi, P.base + tok + 1) : 0;
+            const int see_lo = real ? max(P.lo, a.window > 0 ? P.base + tok + 1 - a.window : 0) : 0;
+            const int tile_free_hi = P.base + t * a.tile_tok + 1;
+            const int tile_free_lo = a.window > 0 ? P.base + min(P.ntok, (t + 1) * a.tile_tok) - a.window : 0;
+            float m = kNone, l = 0.f;
+            for (int it = 0; it < P.tiles; it++) {
+                const int kb = P.kb0 + it * kTile;
+                live = warp_wait(&bars.sfull[t], sph);
+                sph ^= 1;
+                if (!live) break;
+                fence_after();
+                float s[kTile];
+#pragma unroll
+                for (int c = 0; c < kTile; c += 32) ld32(colS + c, s + c);
+                ld_wait(s);
+                if (kb + kTile > tile_free_hi || kb < tile_free_lo || kb < P.lo) {
+                    const int c0 = see_lo - kb, c1 = see_hi - kb;
+#pragma unroll
+                    for (int c = 0; c < kTile; c++)
+                        if (c < c0 || c >= c1) s[c] = -INFINITY;
+                }
+                if (*reinterpret_cast<volatile int *>(&s_badpage)) {
+#pragma unroll 1
+                    for (int g = 0; g < kTile / 16; g++) {
+                        const int key = kb + 16 * g;
+                        if (key < P.hi && paged_off(kv, P.b, P.j, key) < 0) {
+#pragma unroll
+                            for (int c = 0; c < kTile; c++)
+                                if (c >> 4 == g) s[c] = -INFINITY;
+                        }
+                    }
+                }
+                float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                for (int c = 4; c < kTile; c++) mx[c & 3] = fmaxf(mx[c & 3], s[c]);
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * l2 - kBias;
+                const bool up = top > m + kSlack;
+                if (__any_sync(0xffffffffu, up)) {
+                    // the row's maximum moves up; what was summed against the old one is rescaled
+                    const float to = up ? top : m, f = ex2(m - to);
+                    l *= f;
+                    m = to;
+                    if (it > 0) {
+                        live = warp_wait(&bars.odone[t], oph ^ 1);   // (of the tile before: that phase is the last one)
+                        if (!live) break;
+                        fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < ((hd + 15) & ~15); c += 32) {
+                            float o[32];
+                            ld32(colO + c, o);
+                            ld_wait(o);
+#pragma unroll
+                            for (int k = 0; k < 32; k++) o[k] *= f;
+                            st32(colO + c, reinterpret_cast<const uint32_t *>(o));
+                        }
+                        st_wait();
+                    }
+                }
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    uint32_t p[32];
+#pragma unroll
+                    for (int c = 0; c < 32; c++) {
+                        const float x = ex2(fmaf(s[64 * h + 2 * c], l2, -m)), y = ex2(fmaf(s[64 * h + 2 * c + 1], l2, -m));
+                        sum[(2 * c) & 3] += x;
+                        sum[(2 * c + 1) & 3] += y;
+                        p[c] = pack<BF>(x, y);
+                    }
+                    st32(colS + 32 * h, p);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                st_wait();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars.pfull[t]);
+                oph ^= 1;
+            }
+            if (!live) break;
+            // ---------------- the portion's end
+            live = warp_wait(&bars.odone[t], oph ^ 1);
+            if (!live) break;
+            fence_after();
+            const bool whole = P.begins && P.ends, poison = *reinterpret_cast<volatile int *>(&s_poison) != 0;
+            const long long row = static_cast<long long>(P.tok0 + tok) * a.n_heads + P.j * a.gqa + P.g0 + rh;
+            const float inv = whole ? inverse_sum(l) : 1.f;
+            float *part = chunk_part(a, worker, P.begins);
+#pragma unroll 1
+            for (int c = 0; c < ((hd + 15) & ~15); c += 32) {
+                float o[32];
+                ld32(colO + c, o);
+                ld_wait(o);
+                if (real && poison)
+                    for (int it = 0; it < P.tiles; it++) {
+                        const int kb = P.kb0 + it * kTile;
+                        if (!P.partial(kb)) continue;
+                        for (int key = max(kb, see_lo); key < min(kb + kTile, see_hi); key++) {
+                            const long long off = paged_off(kv, P.b, P.j, key);
+                            if (off < 0) continue;
+                            const T *v = static_cast<const T *>(kv.v) + off + c;
+#pragma unroll
+                            for (int k = 0; k < 32; k++)
+                                if (c + k < hd) o[k] += not_finite(to_f(v[k]));
+                        }
+                    }
+                if (real && whole) {
+                    T *out = static_cast<T *>(a.out) + row * hd + c;
+#pragma unroll
+                    for (int k = 0; k < 32; k += 8)
+                        if (c + k < hd)
+                            *reinterpret_cast<uint4 *>(out + k) =
+                                make_uint4(pack<BF>(o[k] * inv, o[k + 1] * inv), pack<BF>(o[k + 2] * inv, o[k + 3] * inv),
+                                           pack<BF>(o[k + 4] * inv, o[k + 5] * inv), pack<BF>(o[k + 6] * inv, o[k + 7] * inv));
+                } else if (real) {
+                    float *out = part + (t * kTile + r) * kTile + c;
+#pragma unroll
+                    for (int k = 0; k < 32; k += 4)
+                        *reinterpret_cast<float4 *>(out + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                }
+                __syncwarp();
+            }
+            if (real && whole && a.lse) a.lse[row] = lse_of(m, l);
+            if (real && !whole) {
+                part[2 * kTile * kTile + t * kTile + r] = m;
+                part[2 * kTile * kTile + 2 * kTile + t * kTile + r] = l;
+            }
+            fence_before();
+        }
+        if (first && tid == 0) static_cast<ChunkJoin *>(a.joins)[worker] = ChunkJoin{-1, 0, 0, 0};
+    }
+    __syncthreads();
+    fence_after();
+    if (warp == kWarpMma)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+}
+
+// cuTensorMapEncodeTiled through the runtime's driver entry point (no link against libcuda)
+using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                              const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encode_fn() {
+    static EncodeFn fn = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q{};
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess) {
+            cudaGetLastError();
+            p = nullptr;
+        }
+        return reinterpret_cast<EncodeFn>(p);
+    }();
+    return fn;
+}
+// 16-bit elements [z][y][x], rows (x) of hd; boxes of 64 x ny x nz
+bool encode(CUtensorMap &m, bool bf, const void *base, uint64_t nx, uint64_t ny, uint64_t nz, uint64_t sy, uint64_t sz,
+            uint32_t by, uint32_t bz) {
+    const cuuint64_t dims[3] = {nx, ny, nz}, strides[2] = {sy * 2, sz * 2};
+    const cuuint32_t box[3] = {64, by, bz}, es[3] = {1, 1, 1};
+    return encode_fn()(&m, bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void *>(base),
+                       dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <bool BF>
+cudaError_t go(const PagedChunkArgs &a, const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv, cudaStream_t st) {
+    cudaError_t e = allow_smem<k_chunk_tc<BF>>(kSmem);
+    return e != cudaSuccess ? e : launch_pdl(k_chunk_tc<BF>, dim3(a.workers), dim3(kThreads), kSmem, st, a, mq, mk, mv);
+}
+
+}  // namespace
+
+// A page's rows and a tile's queries have to be boxes (rows of 128 bytes and more, 16 rows and more).  Scores are
+// compared before they are scaled, so the scale is positive.
+bool chunk_on_tc(const PagedChunkArgs &a) {
+    return a.q16 && a.kv.hd >= 64 && a.kv.hd <= 128 && a.kv.page_shift >= 4 && a.scale > 0.f && encode_fn();
+}
+uint64_t chunk_tc_parts(int sms) { return 2ull * sms * 2 * kTile * (kTile + 2) * 4; }
+
+cudaError_t launch_chunk_tc(PagedChunkArgs a, int sms, cudaStream_t st) {
+    a.hg = std::min(a.gqa, kTile);
+    a.groups = (a.gqa + a.hg - 1) / a.hg;
+    a.heads = a.kv.n_kv * a.groups;
+    const int shift = 31 - __builtin_clz(static_cast<unsigned>(kTile / a.hg));
+    a.tile_tok = 1 << shift;
+    a.tok_shift = shift + 1;
+    a.key_shift = 7;
+    // a table of one tile's rows: no segment can be cut
+    const bool cut = (static_cast<long long>(a.kv.max_pages) << a.kv.page_shift) > kTile;
+    a.seg_cost = cut ? 2 : 0;
+    a.workers = sms;
+    a.part_floats = 2 * kTile * (kTile + 2);
+    const PagedKv &kv = a.kv;
+    const bool bf = kv.dtype == STYX_BF16;
+    const uint64_t rows = static_cast<uint64_t>(kv.n_kv) << kv.page_shift;
+    const uint32_t box = 1u << std::min(kv.page_shift, 7);
+    CUtensorMap mq, mk, mv;
+    if (!encode(mq, bf, a.q, kv.hd, a.n_heads, a.n_tokens, kv.hd, a.q_stride, a.hg, a.tile_tok) ||
+        !encode(mk, bf, kv.k, kv.hd, rows, kv.n_pages, kv.hd, kv.page_stride, box, 1) ||
+        !encode(mv, bf, kv.v, kv.hd, rows, kv.n_pages, kv.hd, kv.page_stride, box, 1))
+        return cudaErrorInvalidValue;
+    cudaError_t e = bf ? go<true>(a, mq, mk, mv, st) : go<false>(a, mq, mk, mv, st);
+    return e != cudaSuccess || !cut ? e : launch_chunk_join(a, 2 * kTile, kTile, kTile, st);
+}
+
+}  // namespace styx

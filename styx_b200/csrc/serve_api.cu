@@ -1,6 +1,7 @@
 // serve_api.cu -- the C entry points of include/styx_serve.h: validation,
 // workspaces and launches; the kernels are in paged.cu, paged_attn.cu,
-// sample.cu, paged_plan.cu, paged_rope.cu and paged_chunk.cu.
+// sample.cu, paged_plan.cu, paged_rope.cu, paged_chunk.cu
+// and paged_chunk_tc.cu.
 #include <algorithm>
 #include <cmath>
 #include <cstdarg>
@@ -200,7 +201,7 @@ struct ChunkWs {
 };
 ChunkWs chunk_ws(const styx::PagedKv &kv, int sms) {
     ChunkWs w{};
-    w.joins = a256(styx::chunk_mma_parts(kv, sms));
+    w.joins = a256(std::max(styx::chunk_mma_parts(kv, sms), kv.dtype == STYX_F32 ? 0 : styx::chunk_tc_parts(sms)));
     w.total = w.joins + a256(sms * 16ull);
     return w;
 }
@@ -392,7 +393,8 @@ int styx_paged_attend_chunk(styx_ctx *ctx, styx_stream stream, const styx_paged_
     a.q16 = q_type != STYX_F32;
     a.part = reinterpret_cast<float *>(ws);
     a.joins = ws + w.joins;
-    CK(styx::launch_chunk_mma(a, sms, S(stream)));
+    if (styx::chunk_on_tc(a)) CK(styx::launch_chunk_tc(a, sms, S(stream)));
+    else CK(styx::launch_chunk_mma(a, sms, S(stream)));
     return STYX_OK;
 }
 
