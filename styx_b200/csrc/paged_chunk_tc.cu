@@ -9,9 +9,10 @@
 //   P = 2^(S l2 - m)   a thread per query row: no exchange between threads
 //   O += P V           tcgen05.mma, P from TMEM, where it lies over S
 // The two tiles take turns: while one's S and O are being multiplied the
-// other's rows are exponentiated.  The maximum that a row is measured against
-// moves only when a score passes it by 2^8, so O is rescaled rarely and then by
-// the row's own thread.
+// other's rows are exponentiated.  What a row's scores are measured against is
+// not the running maximum but that of its first tile, until weights become too
+// large for it: no tile but the first is searched for its maximum, and O is
+// rescaled rarely, by the row's own thread.
 //
 // Roles, linked by mbarriers with bounded waits: eight softmax warps (a
 // warpgroup per query tile), a warp that copies (TMA: boxes of min(page, 128)
@@ -20,7 +21,9 @@
 // V where a tile is not seen in whole by all rows: rows outside the sequence
 // (TMA brings whole pages) and numbers that are not finite become zeros, since 0
 // times them would not be 0; the latter are added, at the portion's end, to the
-// rows that see them.  K and V share one ring of slots in the order of use.
+// rows that see them.  K and V have a ring of slots each, whose barriers one role
+// alone waits on, phase after phase (a role that looked at every other phase of a
+// barrier could take one for another).
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -39,16 +42,19 @@ constexpr int kWarpLoad = 8, kWarpMma = 9, kWarpClean = 10;
 constexpr int kTile = 128;                          // query rows of a tile, keys of a tile
 constexpr int kHalf = kTile * 128;                  // 128 rows of 64 16-bit elements
 constexpr int kSlot = 2 * kHalf;                    // a K or V tile
-constexpr int kSlots = 5;
-constexpr int kSmem = 2 * kSlot + kSlots * kSlot + 1024;
+constexpr int kRingK = 2, kRingV = 3;
+constexpr int kSmem = (2 + kRingK + kRingV) * kSlot + 1024;
 constexpr uint32_t kTmemCols = 512, kColS = 0, kColO = 256;   // S (and P over it) and O of the two query tiles
-constexpr float kSlack = 8.f;                       // log2 units a score may pass the maximum by
+// A row's weights are 2^(score - m), m the largest score of the portion's first tile (f16: + 7 in the exponent, since it
+// has few), and m moves only when 64 weights add up to more than this; f16's largest number is 2^16.
+constexpr float kMost = 32768.f;
+constexpr float kSlack = 8.f;                       // (log2 units; where a tile is searched all the same)
 
 struct Bars {
-    uint64_t full[kSlots], empty[kSlots];
+    uint64_t kfull[kRingK], kempty[kRingK], vfull[kRingV], vempty[kRingV];
     uint64_t clean[4];                              // V tile i: clean[i % 4]
     uint64_t qfull, qempty;
-    uint64_t sfull[2], pfull[2], odone[2];
+    uint64_t sfull[2], pfull[2][2], odone[2][2];       // pfull, odone: by halves of the keys
     uint64_t drain;
 };
 
@@ -79,6 +85,11 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, ui
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}\n" ::"r"(d),
         "r"(a), "r"(b_lo), "r"(id), "r"(acc), "n"(kDescHi)
         : "memory");
+}
+__device__ __forceinline__ bool elect() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
 }
 __device__ __forceinline__ void commit(uint64_t *bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
@@ -136,6 +147,95 @@ __device__ __forceinline__ uint32_t pack(float x, float y) {   // low half: x
         return *reinterpret_cast<const uint32_t *>(&h);
     }
 }
+// ------------------------------------------------------------ softmax helpers
+// two f32 at once (the FMA units take pairs of registers)
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pair(float x, float y) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void unpair(f32x2 v, float &x, float &y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// the largest of three, NaN where one is
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// 64 scores to the weights 2^(s l2 - m), packed, and their sum.  The special
+// function units give an exponential per warp and 8 clocks; what goes before and
+// after it fits in between, if it is issued there: left to the compiler, the
+// stages follow one another (2000 clocks instead of 1300 for a tile of 128).
+// (Part of the exponentials as polynomials on the FMA units made it slower.)
+template <bool BF>
+__device__ __forceinline__ float weights(const float *s, float l2, float m, uint32_t (&p)[32]) {
+    constexpr int kAhead = 2, kBehind = 3;             // pairs between the stages
+    f32x2 sum[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
+    const f32x2 l22 = pair(l2, l2), nm = pair(-m, -m);
+    f32x2 x2[32];
+    float x[32], y[32];
+#pragma unroll
+    for (int c = -kAhead; c < 32 + kBehind; c++) {
+        if (c + kAhead < 32) {
+            const int i = c + kAhead;
+            asm volatile("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(x2[i]) : "l"(pair(s[2 * i], s[2 * i + 1])), "l"(l22), "l"(nm));
+        }
+        if (c >= 0 && c < 32) {
+            float u, v;
+            unpair(x2[c], u, v);
+            asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(x[c]) : "f"(u));
+            asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y[c]) : "f"(v));
+        }
+        if (c >= kBehind) {
+            const int i = c - kBehind;
+            asm volatile("add.rn.f32x2 %0, %0, %1;" : "+l"(sum[i & 1]) : "l"(pair(x[i], y[i])));
+            if constexpr (BF) asm volatile("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(p[i]) : "f"(y[i]), "f"(x[i]));
+            else asm volatile("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(p[i]) : "f"(y[i]), "f"(x[i]));
+        }
+    }
+    float u, v;
+    unpair(add2(sum[0], sum[1]), u, v);
+    return u + v;
+}
+// the largest of N scores, in units of log2; NaN where one is NaN or +inf
+template <int N>
+__device__ __forceinline__ float largest(const float *s, float l2) {
+    float mx[2] = {s[0], s[1]};
+#pragma unroll
+    for (int c = 2; c < N - 2; c += 4) {
+        mx[0] = max3(mx[0], s[c], s[c + 1]);
+        mx[1] = max3(mx[1], s[c + 2], s[c + 3]);
+    }
+    const float top = max3(max3(mx[0], s[N - 2], s[N - 1]), mx[1], mx[1]) * l2;
+    return top == INFINITY ? __int_as_float(0x7FFFFFFF) : top;
+}
+// of four neighbouring lanes: lane i's x[k] becomes what was lane k's x[i]
+__device__ __forceinline__ void turn4(uint4 (&x)[4], int lane) {
+    auto swap = [&](uint4 &lo, uint4 &hi, int bit) {   // hi of the lane without the bit for lo of the one with it
+        const bool up = lane & bit;
+        uint4 v = up ? lo : hi;
+        v.x = __shfl_xor_sync(0xffffffffu, v.x, bit);
+        v.y = __shfl_xor_sync(0xffffffffu, v.y, bit);
+        v.z = __shfl_xor_sync(0xffffffffu, v.z, bit);
+        v.w = __shfl_xor_sync(0xffffffffu, v.w, bit);
+        if (up) lo = v;
+        else hi = v;
+    };
+    swap(x[0], x[1], 1);
+    swap(x[2], x[3], 1);
+    swap(x[0], x[2], 2);
+    swap(x[1], x[3], 2);
+}
 __device__ __forceinline__ float not_finite(float v) { return fabsf(v) <= 3.4028234e38f ? 0.f : v; }
 
 // a portion: its segment's tokens and heads, its keys [lo, hi)
@@ -177,23 +277,29 @@ __global__ void __launch_bounds__(kThreads, 1)
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort, s_badpage, s_poison, s_dirty[4];
     uint8_t *const sm = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
-    const uint32_t sQ = smem_addr(sm), ring = sQ + 2 * kSlot;
+    const uint32_t sQ = smem_addr(sm), sK = sQ + 2 * kSlot, sV = sK + kRingK * kSlot;
     const PagedKv &kv = a.kv;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, hd = kv.hd;
     const int halves = hd > 64 ? 2 : 1;
 
     if (tid == 0) {
-        for (int i = 0; i < kSlots; i++) {
-            mbar_init(&bars.full[i], 1);
-            mbar_init(&bars.empty[i], 1);
+        for (int i = 0; i < kRingK; i++) {
+            mbar_init(&bars.kfull[i], 1);
+            mbar_init(&bars.kempty[i], 1);
+        }
+        for (int i = 0; i < kRingV; i++) {
+            mbar_init(&bars.vfull[i], 1);
+            mbar_init(&bars.vempty[i], 1);
         }
         for (int i = 0; i < 4; i++) mbar_init(&bars.clean[i], 2);
         mbar_init(&bars.qfull, 1);
         mbar_init(&bars.qempty, 1);
         for (int i = 0; i < 2; i++) {
             mbar_init(&bars.sfull[i], 1);
-            mbar_init(&bars.pfull[i], 4);
-            mbar_init(&bars.odone[i], 1);
+            mbar_init(&bars.pfull[i][0], 4);
+            mbar_init(&bars.pfull[i][1], 4);
+            mbar_init(&bars.odone[i][0], 1);
+            mbar_init(&bars.odone[i][1], 1);
         }
         mbar_init(&bars.drain, 1);
         fence_mbar_init();
@@ -236,187 +342,208 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     auto warp_wait = [&](uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
 
-    if (warp == kWarpLoad) {
-        // ---------------- copies.  A lane has one box of a tile: rows, and 64 of the elements
-        const int rb_shift = min(kv.page_shift, 7), rb = 1 << rb_shift, boxes = kTile >> rb_shift;
-        const int pi = lane / halves, half = lane - pi * halves;
-        const bool mine = pi < boxes;
-        const uint32_t dst = half * kHalf + (pi << rb_shift) * 128;
-        const uint32_t q_bytes = 128u * a.hg * a.tile_tok;
-        int portion = 0, use = 0, slot = 0, nv = 0;       // use: how often the ring has gone round
-        bool live = true;
-        while (live && wk.next(a)) {
-            P.set(a, wk);
-            const int32_t *table = kv.table + static_cast<long long>(P.b) * kv.table_stride;
-            auto page_of = [&](int it) {
-                const int r0 = P.kb0 + it * kTile + (pi << rb_shift);
-                return mine && it < P.tiles && r0 < P.hi && r0 + rb > P.lo ? ld_now(table + (r0 >> kv.page_shift)) : -1;
-            };
-            int page = page_of(0);
-            if (portion > 0) live = warp_wait(&bars.qempty, static_cast<uint32_t>((portion - 1) & 1));
-            if (!live) break;
-            if (lane == 0) {
-                const int nq = P.two ? 2 : 1;
-                mbar_arrive_expect_tx(&bars.qfull, nq * halves * q_bytes);
-                for (int t = 0; t < nq; t++)
-                    for (int h = 0; h < halves; h++)
-                        tma3(sQ + t * kSlot + h * kHalf, &mq, h * 64, P.j * a.gqa + P.g0, P.tok0 + t * a.tile_tok, &bars.qfull);
-            }
-            __syncwarp();
-            portion++;
-            for (int it = 0; it < P.tiles && live; it++) {
-                const int r0 = P.kb0 + it * kTile + (pi << rb_shift), here = page;
-                const bool some = mine && r0 < P.hi && r0 + rb > P.lo;
-                const bool on = some && static_cast<unsigned>(here) < static_cast<unsigned>(kv.n_pages);
-                page = page_of(it + 1);
-                const unsigned n = __popc(__ballot_sync(0xffffffffu, on));
-                const bool bad = __any_sync(0xffffffffu, some && !on);
-                const int y = (P.j << kv.page_shift) + (r0 & ((1 << kv.page_shift) - 1));
-                for (int v = 0; v < 2; v++) {
-                    if (use > 0 && !warp_wait(&bars.empty[slot], static_cast<uint32_t>((use - 1) & 1))) {
-                        live = false;
-                        break;
-                    }
-                    if (lane == 0) {
-                        if (bad) {
-                            atomicExch(kv.err, kErrBadPos);
-                            *reinterpret_cast<volatile int *>(&s_badpage) = 1;
-                        }
-                        if (v) *reinterpret_cast<volatile int *>(&s_dirty[nv & 3]) = bad || P.partial(P.kb0 + it * kTile);
-                        mbar_arrive_expect_tx(&bars.full[slot], n * static_cast<uint32_t>(rb) * 128u);
-                    }
-                    __syncwarp();
-                    if (on) tma3(ring + slot * kSlot + dst, v ? &mv : &mk, half * 64, y, here, &bars.full[slot]);
-                    if (++slot == kSlots) slot = 0, use++;
+    // the softmax warps take the registers that the others do not need (256 x 208 + 128 x 88 = 384 x 168)
+    if (warp >= kWarpLoad) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if (warp == kWarpLoad) {
+            // ---------------- copies.  A lane has one box of a tile: rows, and 64 of the elements
+            const int rb_shift = min(kv.page_shift, 7), rb = 1 << rb_shift, boxes = kTile >> rb_shift;
+            const int pi = lane / halves, half = lane - pi * halves;
+            const bool mine = pi < boxes;
+            const uint32_t dst = half * kHalf + (pi << rb_shift) * 128;
+            const uint32_t q_bytes = 128u * a.hg * a.tile_tok;
+            int portion = 0, n_tile = 0;
+            bool live = true;
+            while (live && wk.next(a)) {
+                P.set(a, wk);
+                const int32_t *table = kv.table + static_cast<long long>(P.b) * kv.table_stride;
+                auto page_of = [&](int it) {
+                    const int r0 = P.kb0 + it * kTile + (pi << rb_shift);
+                    return mine && it < P.tiles && r0 < P.hi && r0 + rb > P.lo ? ld_now(table + (r0 >> kv.page_shift)) : -1;
+                };
+                int page = page_of(0);
+                if (portion > 0) live = warp_wait(&bars.qempty, static_cast<uint32_t>((portion - 1) & 1));
+                if (!live) break;
+                if (lane == 0) {
+                    const int nq = P.two ? 2 : 1;
+                    mbar_arrive_expect_tx(&bars.qfull, nq * halves * q_bytes);
+                    for (int t = 0; t < nq; t++)
+                        for (int h = 0; h < halves; h++)
+                            tma3(sQ + t * kSlot + h * kHalf, &mq, h * 64, P.j * a.gqa + P.g0, P.tok0 + t * a.tile_tok, &bars.qfull);
                 }
-                nv++;
+                __syncwarp();
+                portion++;
+                for (int it = 0; it < P.tiles && live; it++) {
+                    const int r0 = P.kb0 + it * kTile + (pi << rb_shift), here = page;
+                    const bool some = mine && r0 < P.hi && r0 + rb > P.lo;
+                    const bool on = some && static_cast<unsigned>(here) < static_cast<unsigned>(kv.n_pages);
+                    page = page_of(it + 1);
+                    const unsigned n = __popc(__ballot_sync(0xffffffffu, on));
+                    const bool bad = __any_sync(0xffffffffu, some && !on);
+                    const int y = (P.j << kv.page_shift) + (r0 & ((1 << kv.page_shift) - 1));
+                    const bool dirty = bad || P.partial(P.kb0 + it * kTile);
+                    for (int v = 0; v < 2; v++) {
+                        const int ring = v ? kRingV : kRingK, slot = n_tile % ring, use = n_tile / ring;
+                        uint64_t *full = (v ? bars.vfull : bars.kfull) + slot, *empty = (v ? bars.vempty : bars.kempty) + slot;
+                        if (use > 0 && !warp_wait(empty, static_cast<uint32_t>((use - 1) & 1))) {
+                            live = false;
+                            break;
+                        }
+                        if (lane == 0) {
+                            if (bad) {
+                                atomicExch(kv.err, kErrBadPos);
+                                *reinterpret_cast<volatile int *>(&s_badpage) = 1;
+                            }
+                            if (v) *reinterpret_cast<volatile int *>(&s_dirty[n_tile & 3]) = dirty;
+                            mbar_arrive_expect_tx(full, n * static_cast<uint32_t>(rb) * 128u);
+                        }
+                        __syncwarp();
+                        if (on) tma3((v ? sV : sK) + slot * kSlot + dst, v ? &mv : &mk, half * 64, y, here, full);
+                    }
+                    n_tile++;
+                }
             }
-        }
-        // Every copy is waited for by the products that read it.  Where a wait gave up, nothing of this warp's may still
-        // be landing when the CTA ends: copies take microseconds, a millisecond is given to them.
-        if (*reinterpret_cast<volatile int *>(&s_abort))
-            for (const long long c0 = clock64(); clock64() - c0 < 2000000;) {
-            }
-    } else if (warp == kWarpMma) {
-        // ---------------- products, all issued by one thread, executed in the order of issue
-        if (lane == 0) {
+            // Every copy is waited for by the products that read it.  Where a wait gave up, nothing of this warp's may still
+            // be landing when the CTA ends: copies take microseconds, a millisecond is given to them.
+            if (*reinterpret_cast<volatile int *>(&s_abort))
+                for (const long long c0 = clock64(); clock64() - c0 < 2000000;) {
+                }
+        } else if (warp == kWarpMma) {
+            // ---------------- products, all issued by one thread, executed in the order of issue.  The warp walks together,
+            // so that what a product is given stays in uniform registers (115 clocks a product otherwise, twice its time).
+            const bool leader = elect();
             const int ks = (hd + 15) / 16;
             const uint32_t id_s = idesc(BF, kTile, false), id_o = idesc(BF, ks * 16, true);
-            const uint32_t dQ = desc_lo(sQ, 16);
-            int portion = 0, nv = 0;
-            int kslot = 0, kuse = 0, vslot = 1, vuse = 0;   // ring: K(0) V(0) K(1) V(1) ..., over all portions
+            const uint32_t dQ = desc_lo(sQ, 16), dK = desc_lo(sK, 16), dV = desc_lo(sV, kHalf);
+            int portion = 0;
+            uint32_t kslot = 0, kph = 0, vslot = 0, cslot = 0, cph = 0;   // the rings' next slots and phases
             uint32_t pph[2] = {0, 0};
             bool live = true;
-            auto step = [](int &slot, int &use) {
-                slot += 2;
-                if (slot >= kSlots) slot -= kSlots, use++;
-            };
             auto scores = [&](int t) {
-                const uint32_t q = dQ + t * (kSlot / 16), k = desc_lo(ring + kslot * kSlot, 16), d = tmem + kColS + t * kTile;
-                for (int i = 0; i < ks; i++) {
-                    const uint32_t o = (i >> 2) * (kHalf / 16) + (i & 3) * 2;
-                    mma_ss(d, q + o, k + o, id_s, i > 0);
-                }
-                commit(&bars.sfull[t]);
-            };
-            auto values = [&](int t, bool first) {
-                const uint32_t v = desc_lo(ring + vslot * kSlot, kHalf), p = tmem + kColS + t * kTile, d = tmem + kColO + t * kTile;
+                if (leader) {
+                    const uint32_t q = dQ + t * (kSlot / 16), k = dK + kslot * (kSlot / 16), d = tmem + kColS + t * kTile;
 #pragma unroll
-                for (int i = 0; i < kTile / 16; i++) mma_ts(d, p + i * 8, v + i * (2048 / 16), id_o, !first || i > 0);
-                commit(&bars.odone[t]);
+                    for (int i = 0; i < 8; i++)
+                        if (i < ks) mma_ss(d, q + (i >> 2) * (kHalf / 16) + (i & 3) * 2, k + (i >> 2) * (kHalf / 16) + (i & 3) * 2, id_s, i > 0);
+                    commit(&bars.sfull[t]);
+                }
+            };
+            // the first or second half of the keys
+            auto values = [&](int t, int h, uint32_t acc) {
+                if (leader) {
+                    const uint32_t v = dV + vslot * (kSlot / 16), p = tmem + kColS + t * kTile, d = tmem + kColO + t * kTile;
+#pragma unroll
+                    for (int i = 0; i < kTile / 32; i++) {
+                        const int k = h * (kTile / 32) + i;
+                        mma_ts(d, p + k * 8, v + k * (2048 / 16), id_o, acc | (i > 0));
+                    }
+                    commit(&bars.odone[t][h]);
+                }
+            };
+            auto done_k = [&](bool last) {                      // this portion's last scores: q is free too
+                if (leader) {
+                    commit(&bars.kempty[kslot]);
+                    if (last) commit(&bars.qempty);
+                }
+                if (++kslot == kRingK) kslot = 0, kph ^= 1;
             };
             while (live && wk.next(a)) {
                 P.set(a, wk);
-                const int nq = P.two ? 2 : 1;
-                live = wait(&bars.qfull, static_cast<uint32_t>(portion & 1)) && wait(&bars.full[kslot], static_cast<uint32_t>(kuse & 1));
+                const int tiles = __shfl_sync(0xffffffffu, P.tiles, 0);
+                const bool two = __shfl_sync(0xffffffffu, P.two, 0);
+                live = warp_wait(&bars.qfull, static_cast<uint32_t>(portion & 1)) && warp_wait(&bars.kfull[kslot], kph);
                 if (!live) break;
                 fence_after();
-                for (int t = 0; t < nq; t++) scores(t);
-                commit(&bars.empty[kslot]);
-                if (P.tiles == 1) commit(&bars.qempty);
-                step(kslot, kuse);
-                for (int it = 0; it < P.tiles && live; it++) {
-                    const bool more = it + 1 < P.tiles;
-                    for (int t = 0; t < nq && live; t++) {
-                        live = wait(&bars.pfull[t], pph[t]) && (t > 0 || wait(&bars.clean[nv & 3], static_cast<uint32_t>((nv >> 2) & 1)));
-                        pph[t] ^= 1;
+                scores(0);
+                if (two) scores(1);
+                done_k(tiles == 1);
+                for (int it = 0; it < tiles; it++) {
+                    const bool more = it + 1 < tiles;
+#pragma unroll
+                    for (int t = 0; t < 2; t++) {
+                        if (t == 1 && !two) break;
+                        const bool last = t == 1 || !two;
+                        live = warp_wait(&bars.pfull[t][0], pph[t]) && (t > 0 || warp_wait(&bars.clean[cslot], cph));
                         if (!live) break;
                         fence_after();
-                        values(t, it == 0);
-                        if (t == nq - 1) commit(&bars.empty[vslot]);
+                        values(t, 0, it > 0);
+                        live = warp_wait(&bars.pfull[t][1], pph[t]);
+                        if (!live) break;
+                        pph[t] ^= 1;
+                        fence_after();
+                        values(t, 1, 1);
+                        if (leader && last) commit(&bars.vempty[vslot]);
                         if (more) {
                             if (t == 0) {
-                                live = wait(&bars.full[kslot], static_cast<uint32_t>(kuse & 1));
+                                live = warp_wait(&bars.kfull[kslot], kph);
                                 if (!live) break;
                                 fence_after();
                             }
                             scores(t);
-                            if (t == nq - 1) {
-                                commit(&bars.empty[kslot]);
-                                if (it + 2 == P.tiles) commit(&bars.qempty);
-                            }
+                            if (last) done_k(it + 2 == tiles);
                         }
                     }
-                    if (more) step(kslot, kuse);
-                    step(vslot, vuse);
-                    nv++;
+                    if (!live) break;
+                    if (++vslot == kRingV) vslot = 0;
+                    if (++cslot == 4) cslot = 0, cph ^= 1;
                 }
                 portion++;
             }
             // every product issued here has completed before TMEM is freed
-            commit(&bars.drain);
-            mbar_wait(&bars.drain, 0u, kv.err, kErrWaitFull);
-        }
-        __syncwarp();
-    } else if (warp >= kWarpClean) {
-        // ---------------- V tiles that are not seen in whole
-        const int ct = tid - 32 * kWarpClean;
-        int slot = 1, use = 0, nv = 0;
-        bool live = true;
-        while (live && wk.next(a)) {
-            P.set(a, wk);
-            for (int it = 0; it < P.tiles; it++, nv++) {
-                live = warp_wait(&bars.full[slot], static_cast<uint32_t>(use & 1));
-                if (!live) break;
-                if (*reinterpret_cast<volatile int *>(&s_dirty[nv & 3])) {
-                    const int32_t *table = kv.table + static_cast<long long>(P.b) * kv.table_stride;
-                    uint8_t *v = sm + 2 * kSlot + slot * kSlot;
-                    for (int row = ct; row < kTile; row += 64) {
-                        const int key = P.kb0 + it * kTile + row;
-                        const bool in = key >= P.lo && key < P.hi &&
-                                        static_cast<unsigned>(ld_now(table + (key >> kv.page_shift))) < static_cast<unsigned>(kv.n_pages);
-                        for (int c = 0; c < 8 * halves; c++) {
-                            // (the swizzle permutes the 16-byte groups of a row: all of them are looked at)
-                            uint4 *p = reinterpret_cast<uint4 *>(v + (c >> 3) * kHalf + row * 128 + (c & 7) * 16);
-                            if (!in) {
-                                *p = make_uint4(0, 0, 0, 0);
-                                continue;
-                            }
-                            const uint4 x = *p;
-                            uint32_t w[4] = {x.x, x.y, x.z, x.w};
-                            bool bad = false;
-                            constexpr uint32_t E = BF ? 0x7F80u : 0x7C00u;
-#pragma unroll
-                            for (int k = 0; k < 4; k++) {
-                                if ((w[k] & E) == E) w[k] &= 0xFFFF0000u, bad = true;
-                                if ((w[k] >> 16 & E) == E) w[k] &= 0xFFFFu, bad = true;
-                            }
-                            if (bad) {
-                                *p = make_uint4(w[0], w[1], w[2], w[3]);
-                                *reinterpret_cast<volatile int *>(&s_poison) = 1;
+            if (leader) {
+                commit(&bars.drain);
+                mbar_wait(&bars.drain, 0u, kv.err, kErrWaitFull);
+            }
+            __syncwarp();
+        } else {
+            // ---------------- V tiles that are not seen in whole
+            const int ct = tid - 32 * kWarpClean;
+            int nv = 0;
+            bool live = true;
+            while (live && wk.next(a)) {
+                P.set(a, wk);
+                for (int it = 0; it < P.tiles; it++, nv++) {
+                    live = warp_wait(&bars.vfull[nv % kRingV], static_cast<uint32_t>(nv / kRingV & 1));
+                    if (!live) break;
+                    if (*reinterpret_cast<volatile int *>(&s_dirty[nv & 3])) {
+                        const int32_t *table = kv.table + static_cast<long long>(P.b) * kv.table_stride;
+                        uint8_t *v = sm + (2 + kRingK + nv % kRingV) * kSlot;
+                        for (int row = ct; row < kTile; row += 64) {
+                            const int key = P.kb0 + it * kTile + row;
+                            const bool in = key >= P.lo && key < P.hi &&
+                                            static_cast<unsigned>(ld_now(table + (key >> kv.page_shift))) < static_cast<unsigned>(kv.n_pages);
+                            for (int c = 0; c < 8 * halves; c++) {
+                                // (the swizzle permutes the 16-byte groups of a row: all of them are looked at)
+                                uint4 *p = reinterpret_cast<uint4 *>(v + (c >> 3) * kHalf + row * 128 + (c & 7) * 16);
+                                if (!in) {
+                                    *p = make_uint4(0, 0, 0, 0);
+                                    continue;
+                                }
+                                const uint4 x = *p;
+                                uint32_t w[4] = {x.x, x.y, x.z, x.w};
+                                bool bad = false;
+                                constexpr uint32_t E = BF ? 0x7F80u : 0x7C00u;
+    #pragma unroll
+                                for (int k = 0; k < 4; k++) {
+                                    if ((w[k] & E) == E) w[k] &= 0xFFFF0000u, bad = true;
+                                    if ((w[k] >> 16 & E) == E) w[k] &= 0xFFFFu, bad = true;
+                                }
+                                if (bad) {
+                                    *p = make_uint4(w[0], w[1], w[2], w[3]);
+                                    *reinterpret_cast<volatile int *>(&s_poison) = 1;
+                                }
                             }
                         }
+                        fence_async();
                     }
-                    fence_async();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bars.clean[nv & 3]);
                 }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bars.clean[nv & 3]);
-                slot += 2;
-                if (slot >= kSlots) slot -= kSlots, use++;
             }
         }
     } else {
         // ---------------- softmax: thread = query row
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int t = warp >> 2, r = tid & 127;
         const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
         const uint32_t colS = tmem + kColS + t * kTile + lanes, colO = tmem + kColO + t * kTile + lanes;
@@ -450,36 +577,32 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int c = 0; c < kTile; c += 32) ld32(colS + c, s + c);
                 ld_wait(s);
-                if (kb + kTile > tile_free_hi || kb < tile_free_lo || kb < P.lo) {
+                const bool masked = kb + kTile > tile_free_hi || kb < tile_free_lo || kb < P.lo ||
+                                    *reinterpret_cast<volatile int *>(&s_badpage);
+                if (masked) {
                     const int c0 = see_lo - kb, c1 = see_hi - kb;
 #pragma unroll
                     for (int c = 0; c < kTile; c++)
                         if (c < c0 || c >= c1) s[c] = -INFINITY;
-                }
-                if (*reinterpret_cast<volatile int *>(&s_badpage)) {
+                    if (*reinterpret_cast<volatile int *>(&s_badpage)) {
 #pragma unroll 1
-                    for (int g = 0; g < kTile / 16; g++) {
-                        const int key = kb + 16 * g;
-                        if (key < P.hi && paged_off(kv, P.b, P.j, key) < 0) {
+                        for (int g = 0; g < kTile / 16; g++) {
+                            const int key = kb + 16 * g;
+                            if (key < P.hi && paged_off(kv, P.b, P.j, key) < 0) {
 #pragma unroll
-                            for (int c = 0; c < kTile; c++)
-                                if (c >> 4 == g) s[c] = -INFINITY;
+                                for (int c = 0; c < kTile; c++)
+                                    if (c >> 4 == g) s[c] = -INFINITY;
+                            }
                         }
                     }
                 }
-                float mx[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-                for (int c = 4; c < kTile; c++) mx[c & 3] = fmaxf(mx[c & 3], s[c]);
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * l2 - kBias;
-                const bool up = top > m + kSlack;
-                if (__any_sync(0xffffffffu, up)) {
-                    // the row's maximum moves up; what was summed against the old one is rescaled
-                    const float to = up ? top : m, f = ex2(m - to);
+                // what was summed against the old m is rescaled, once the products before half h are done
+                auto raise = [&](float to, int h) {
+                    const float f = ex2(m - to);
                     l *= f;
                     m = to;
-                    if (it > 0) {
-                        live = warp_wait(&bars.odone[t], oph ^ 1);   // (of the tile before: that phase is the last one)
-                        if (!live) break;
+                    if (it > 0 || h > 0) {
+                        if (!(h ? warp_wait(&bars.odone[t][0], oph) : warp_wait(&bars.odone[t][1], oph ^ 1))) return false;
                         fence_after();
 #pragma unroll 1
                         for (int c = 0; c < ((hd + 15) & ~15); c += 32) {
@@ -492,36 +615,52 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                         st_wait();
                     }
+                    return true;
+                };
+                if (it == 0 || masked) {               // (a masked tile: so that no row stays without a maximum)
+                    const float top = largest<kTile>(s, l2) - kBias;
+                    const bool up = real && !(top <= m + (m > kNone ? kSlack : 0.f));
+                    if (__any_sync(0xffffffffu, up)) live = raise(up ? top : m, 0);
+                    if (!live) break;
                 }
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
                     uint32_t p[32];
-#pragma unroll
-                    for (int c = 0; c < 32; c++) {
-                        const float x = ex2(fmaf(s[64 * h + 2 * c], l2, -m)), y = ex2(fmaf(s[64 * h + 2 * c + 1], l2, -m));
-                        sum[(2 * c) & 3] += x;
-                        sum[(2 * c + 1) & 3] += y;
-                        p[c] = pack<BF>(x, y);
+                    float sum = weights<BF>(s + 64 * h, l2, m, p);
+                    const bool over = real && !(sum <= kMost);   // (NaN: of a NaN, or of a score of +inf)
+                    if (__any_sync(0xffffffffu, over)) {
+                        const float top = largest<64>(s + 64 * h, l2) - kBias;
+                        live = raise(over && !(top <= m) ? top : m, h);
+                        if (!live) break;
+                        sum = weights<BF>(s + 64 * h, l2, m, p);
                     }
+                    l += sum;
                     st32(colS + 32 * h, p);
+                    st_wait();
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bars.pfull[t][h]);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                st_wait();
-                fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bars.pfull[t]);
+                if (!live) break;
                 oph ^= 1;
             }
             if (!live) break;
             // ---------------- the portion's end
-            live = warp_wait(&bars.odone[t], oph ^ 1);
+            live = warp_wait(&bars.odone[t][1], oph ^ 1);
             if (!live) break;
             fence_after();
             const bool whole = P.begins && P.ends, poison = *reinterpret_cast<volatile int *>(&s_poison) != 0;
             const long long row = static_cast<long long>(P.tok0 + tok) * a.n_heads + P.j * a.gqa + P.g0 + rh;
             const float inv = whole ? inverse_sum(l) : 1.f;
             float *part = chunk_part(a, worker, P.begins);
+            // the four rows of the lane's group of four: where they are, and which there are
+            long long rows4[4];
+            unsigned there = 0;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                rows4[k] = __shfl_sync(0xffffffffu, row, (lane & ~3) + k);
+                there |= static_cast<unsigned>(__shfl_sync(0xffffffffu, static_cast<int>(real), (lane & ~3) + k)) << k;
+            }
 #pragma unroll 1
             for (int c = 0; c < ((hd + 15) & ~15); c += 32) {
                 float o[32];
@@ -540,19 +679,33 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 if (c + k < hd) o[k] += not_finite(to_f(v[k]));
                         }
                     }
-                if (real && whole) {
-                    T *out = static_cast<T *>(a.out) + row * hd + c;
+                // Four lanes have four rows' 64 bytes (whole: 16-bit; else 2 x 64 of f32): they exchange them, so that each
+                // store is of four lanes' 64 bytes of one row.  (A row per lane: 4000 clocks a portion.)
+                if (whole) {
+                    uint4 x[4];
 #pragma unroll
-                    for (int k = 0; k < 32; k += 8)
-                        if (c + k < hd)
-                            *reinterpret_cast<uint4 *>(out + k) =
-                                make_uint4(pack<BF>(o[k] * inv, o[k + 1] * inv), pack<BF>(o[k + 2] * inv, o[k + 3] * inv),
-                                           pack<BF>(o[k + 4] * inv, o[k + 5] * inv), pack<BF>(o[k + 6] * inv, o[k + 7] * inv));
-                } else if (real) {
-                    float *out = part + (t * kTile + r) * kTile + c;
+                    for (int k = 0; k < 4; k++)
+                        x[k] = make_uint4(pack<BF>(o[8 * k] * inv, o[8 * k + 1] * inv), pack<BF>(o[8 * k + 2] * inv, o[8 * k + 3] * inv),
+                                          pack<BF>(o[8 * k + 4] * inv, o[8 * k + 5] * inv), pack<BF>(o[8 * k + 6] * inv, o[8 * k + 7] * inv));
+                    turn4(x, lane);
+                    const int e = c + 8 * (lane & 3);
 #pragma unroll
-                    for (int k = 0; k < 32; k += 4)
-                        *reinterpret_cast<float4 *>(out + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                    for (int k = 0; k < 4; k++)
+                        if ((there >> k & 1) && e < hd) *reinterpret_cast<uint4 *>(static_cast<T *>(a.out) + rows4[k] * hd + e) = x[k];
+                } else {
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        uint4 x[4];
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            x[k] = make_uint4(__float_as_uint(o[16 * h + 4 * k]), __float_as_uint(o[16 * h + 4 * k + 1]),
+                                              __float_as_uint(o[16 * h + 4 * k + 2]), __float_as_uint(o[16 * h + 4 * k + 3]));
+                        turn4(x, lane);
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            if (there >> k & 1)
+                                *reinterpret_cast<uint4 *>(part + (t * kTile + (r & ~3) + k) * kTile + c + 16 * h + 4 * (lane & 3)) = x[k];
+                    }
                 }
                 __syncwarp();
             }
@@ -623,7 +776,7 @@ cudaError_t launch_chunk_tc(PagedChunkArgs a, int sms, cudaStream_t st) {
     a.key_shift = 7;
     // a table of one tile's rows: no segment can be cut
     const bool cut = (static_cast<long long>(a.kv.max_pages) << a.kv.page_shift) > kTile;
-    a.seg_cost = cut ? 2 : 0;
+    a.seg_cost = cut ? 3 : 0;
     a.workers = sms;
     a.part_floats = 2 * kTile * (kTile + 2);
     const PagedKv &kv = a.kv;
