@@ -1,29 +1,35 @@
 // paged_chunk_tc.cu -- attention of chunks (styx_paged_attend_chunk) on the
-// 5th-generation tensor cores: q and cache of one 16-bit type, head_dim 64 to
-// 128, pages of 16 rows or more.
+// 5th-generation tensor cores: 16-bit caches, q of the cache's type or (f16
+// caches) f32, head_dim 64 to 128, pages of 16 rows or more.
 //
 // A CTA takes two query tiles of 128 rows (tokens x the q heads of a kv head,
 // so that a kv head's rows are read once for all of them) over tiles of 128
 // keys:
 //   S = Q K^T          tcgen05.mma, both operands from shared memory
-//   P = 2^(S l2 - m)   a thread per query row: no exchange between threads
+//   P = 2^(S - m)      two threads per query row, half of the keys each
 //   O += P V           tcgen05.mma, P from TMEM, where it lies over S
 // The two tiles take turns: while one's S and O are being multiplied the
 // other's rows are exponentiated.  What a row's scores are measured against is
 // not the running maximum but that of its first tile, until weights become too
 // large for it: no tile but the first is searched for its maximum, and O is
-// rescaled rarely, by the row's own thread.
+// rescaled rarely, by the row's own threads.
 //
-// Roles, linked by mbarriers with bounded waits: eight softmax warps (a
-// warpgroup per query tile), a warp that copies (TMA: boxes of min(page, 128)
-// rows x 64 elements of a page, 128-byte swizzled; q with one box per tile and
-// 64 elements), a thread that issues the products, and two warps that go over
-// V where a tile is not seen in whole by all rows: rows outside the sequence
-// (TMA brings whole pages) and numbers that are not finite become zeros, since 0
-// times them would not be 0; the latter are added, at the portion's end, to the
-// rows that see them.  K and V have a ring of slots each, whose barriers one role
-// alone waits on, phase after phase (a role that looked at every other phase of a
-// barrier could take one for another).
+// f32 q (TERMS 2): q and p are split into two f16 terms, 22 bits; products are
+// exact, twice as many.  The MMA cuts its sums off instead of rounding them, an
+// error to one side that grows with every step (some 2^-26 of O each), so O is
+// added to a sum of its own in the workspace every kFlush tiles.
+//
+// Roles, linked by mbarriers with bounded waits: sixteen softmax warps (eight
+// per query tile), a warp that copies (TMA: boxes of min(page, 128) rows x 64
+// elements of a page, 128-byte swizzled; 16-bit q with one box per tile and 64
+// elements; f32 q is brought and split by the softmax warps), a warp that issues
+// the products, and two warps that go over V where a tile is not seen in whole
+// by all rows: rows outside the sequence (TMA brings whole pages) and numbers
+// that are not finite become zeros, since 0 times them would not be 0; the
+// latter are added, at the portion's end, to the rows that see them.  K and V
+// have a ring of slots each, whose barriers one role alone waits on, phase
+// after phase (a role that looked at every other phase of a barrier could take
+// one for another).
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -37,26 +43,42 @@
 namespace styx {
 namespace {
 
-constexpr int kThreads = 384;
-constexpr int kWarpLoad = 8, kWarpMma = 9, kWarpClean = 10;
+constexpr int kSoftmax = 16;                        // warps; the others behind them
+constexpr int kThreads = 32 * (kSoftmax + 4);
+constexpr int kWarpLoad = kSoftmax, kWarpMma = kSoftmax + 1, kWarpClean = kSoftmax + 2;
 constexpr int kTile = 128;                          // query rows of a tile, keys of a tile
 constexpr int kHalf = kTile * 128;                  // 128 rows of 64 16-bit elements
-constexpr int kSlot = 2 * kHalf;                    // a K or V tile
-constexpr int kRingK = 2, kRingV = 3;
-constexpr int kSmem = (2 + kRingK + kRingV) * kSlot + 1024;
+constexpr int kSlot = 2 * kHalf;                    // a K or V tile, a term of a query tile
+// slots of the rings; with the query tiles seven in all
+template <int TERMS>
+struct Ring {
+    static constexpr int k = TERMS == 1 ? 2 : 1, v = TERMS == 1 ? 3 : 2;
+};
 constexpr uint32_t kTmemCols = 512, kColS = 0, kColO = 256;   // S (and P over it) and O of the two query tiles
 // A row's weights are 2^(score - m), m the largest score of the portion's first tile (f16: + 7 in the exponent, since it
 // has few), and m moves only when 64 weights add up to more than this; f16's largest number is 2^16.
 constexpr float kMost = 32768.f;
 constexpr float kSlack = 8.f;                       // (log2 units; where a tile is searched all the same)
+constexpr int kFlush = 4;                           // tiles whose P V the MMA adds up by itself (TERMS 2)
 
 struct Bars {
-    uint64_t kfull[kRingK], kempty[kRingK], vfull[kRingV], vempty[kRingV];
+    uint64_t kfull[2], kempty[2], vfull[3], vempty[3];
     uint64_t clean[4];                              // V tile i: clean[i % 4]
     uint64_t qfull, qempty;
-    uint64_t sfull[2], pfull[2][2], odone[2][2];       // pfull, odone: by halves of the keys
+    uint64_t sfull[2], pfull[2], odone[2];
     uint64_t drain;
 };
+
+// behind the seven slots
+struct Rest {
+    Bars bars;
+    uint32_t tmem;
+    int abort, badpage, poison, dirty[4];
+    float x[2][2][kTile];                           // of a tile's rows: what the two halves tell each other
+    uint8_t unit[2][2][kTile];                      // f32 q, by portions: the exponent of what a row's scores are in units of
+};
+constexpr int kSmem = 7 * kSlot + sizeof(Rest);
+static_assert(kSmem <= 227 * 1024, "shared memory");
 
 // ------------------------------------------------------------ tensor-core helpers
 // Shared-memory operand descriptors (version 1, 128-byte swizzle).  The high
@@ -111,6 +133,16 @@ __device__ __forceinline__ void ld32(uint32_t addr, float *v) {
         : "r"(addr));
 #pragma unroll
     for (int j = 0; j < 32; j++) v[j] = __uint_as_float(r[j]);
+}
+__device__ __forceinline__ void ld16(uint32_t addr, float *v) {
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr));
+#pragma unroll
+    for (int j = 0; j < 16; j++) v[j] = __uint_as_float(r[j]);
 }
 __device__ __forceinline__ void st32(uint32_t addr, const uint32_t *r) {
     asm volatile(
@@ -172,52 +204,48 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-// 64 scores to the weights 2^(s l2 - m), packed, and their sum.  The special
-// function units give an exponential per warp and 8 clocks; what goes before and
-// after it fits in between, if it is issued there: left to the compiler, the
-// stages follow one another (2000 clocks instead of 1300 for a tile of 128).
+// 64 scores to the weights 2^(s unit - m), packed (in terms), and their sum.
 // (Part of the exponentials as polynomials on the FMA units made it slower.)
-template <bool BF>
-__device__ __forceinline__ float weights(const float *s, float l2, float m, uint32_t (&p)[32]) {
-    constexpr int kAhead = 2, kBehind = 3;             // pairs between the stages
+template <bool BF, int TERMS>
+__device__ __forceinline__ float weights(const float (&s)[64], float unit, float m, uint32_t (&p)[TERMS][32]) {
     f32x2 sum[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
-    const f32x2 l22 = pair(l2, l2), nm = pair(-m, -m);
-    f32x2 x2[32];
-    float x[32], y[32];
+    const f32x2 u2 = pair(unit, unit), nm = pair(-m, -m);
 #pragma unroll
-    for (int c = -kAhead; c < 32 + kBehind; c++) {
-        if (c + kAhead < 32) {
-            const int i = c + kAhead;
-            asm volatile("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(x2[i]) : "l"(pair(s[2 * i], s[2 * i + 1])), "l"(l22), "l"(nm));
-        }
-        if (c >= 0 && c < 32) {
-            float u, v;
-            unpair(x2[c], u, v);
-            asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(x[c]) : "f"(u));
-            asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y[c]) : "f"(v));
-        }
-        if (c >= kBehind) {
-            const int i = c - kBehind;
-            asm volatile("add.rn.f32x2 %0, %0, %1;" : "+l"(sum[i & 1]) : "l"(pair(x[i], y[i])));
-            if constexpr (BF) asm volatile("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(p[i]) : "f"(y[i]), "f"(x[i]));
-            else asm volatile("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(p[i]) : "f"(y[i]), "f"(x[i]));
+    for (int c = 0; c < 32; c++) {
+        float x, y;
+        unpair(fma2(pair(s[2 * c], s[2 * c + 1]), u2, nm), x, y);
+        x = ex2(x);
+        y = ex2(y);
+        sum[c & 1] = add2(sum[c & 1], pair(x, y));
+        p[0][c] = pack<BF>(x, y);
+        if constexpr (TERMS == 2) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&p[0][c]));
+            p[TERMS - 1][c] = pack<BF>(x - f.x, y - f.y);
         }
     }
-    float u, v;
-    unpair(add2(sum[0], sum[1]), u, v);
-    return u + v;
+    float x, y;
+    unpair(add2(sum[0], sum[1]), x, y);
+    return x + y;
 }
 // the largest of N scores, in units of log2; NaN where one is NaN or +inf
 template <int N>
-__device__ __forceinline__ float largest(const float *s, float l2) {
+__device__ __forceinline__ float largest(const float (&s)[N], float unit) {
     float mx[2] = {s[0], s[1]};
 #pragma unroll
     for (int c = 2; c < N - 2; c += 4) {
         mx[0] = max3(mx[0], s[c], s[c + 1]);
         mx[1] = max3(mx[1], s[c + 2], s[c + 3]);
     }
-    const float top = max3(max3(mx[0], s[N - 2], s[N - 1]), mx[1], mx[1]) * l2;
+    const float top = max3(max3(mx[0], s[N - 2], s[N - 1]), mx[1], mx[1]) * unit;
     return top == INFINITY ? __int_as_float(0x7FFFFFFF) : top;
+}
+__device__ __forceinline__ void as_quads(const float *o, uint4 (&x)[4]) {
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+        x[k] = make_uint4(__float_as_uint(o[4 * k]), __float_as_uint(o[4 * k + 1]), __float_as_uint(o[4 * k + 2]), __float_as_uint(o[4 * k + 3]));
+}
+__device__ __forceinline__ float4 as_float4(uint4 v) {
+    return make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
 }
 // of four neighbouring lanes: lane i's x[k] becomes what was lane k's x[i]
 __device__ __forceinline__ void turn4(uint4 (&x)[4], int lane) {
@@ -235,6 +263,18 @@ __device__ __forceinline__ void turn4(uint4 (&x)[4], int lane) {
     swap(x[2], x[3], 1);
     swap(x[0], x[2], 2);
     swap(x[1], x[3], 2);
+}
+// barriers of the two warps that share 32 query rows
+__device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ bool pair_any(int id, bool v) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\t"
+        "barrier.cta.red.or.pred q, %2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"(static_cast<uint32_t>(v)), "r"(id)
+        : "memory");
+    return r != 0;
 }
 __device__ __forceinline__ float not_finite(float v) { return fabsf(v) <= 3.4028234e38f ? 0.f : v; }
 
@@ -266,53 +306,54 @@ struct Part {
     __device__ __forceinline__ bool partial(int kb) const { return kb + kTile > free_hi || kb < free_lo; }
 };
 
-template <bool BF>
+template <bool BF, int TERMS>
 __global__ void __launch_bounds__(kThreads, 1)
     k_chunk_tc(PagedChunkArgs a, const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                const __grid_constant__ CUtensorMap mv) {
     using T = std::conditional_t<BF, __nv_bfloat16, __half>;
+    constexpr int RK = Ring<TERMS>::k, RV = Ring<TERMS>::v;
     constexpr float kBias = BF ? 0.f : 7.f;         // f16 has few exponents: p is carried as p * 2^7
-    extern __shared__ uint8_t smem_raw[];
-    __shared__ Bars bars;
-    __shared__ uint32_t s_tmem;
-    __shared__ int s_abort, s_badpage, s_poison, s_dirty[4];
-    uint8_t *const sm = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
-    const uint32_t sQ = smem_addr(sm), sK = sQ + 2 * kSlot, sV = sK + kRingK * kSlot;
+    extern __shared__ __align__(1024) uint8_t sm[];   // (the swizzle goes by address bits 4 to 9)
+    Rest &R = *reinterpret_cast<Rest *>(sm + 7 * kSlot);
+    Bars &bars = R.bars;
+    const uint32_t sQ = smem_addr(sm), sK = sQ + 2 * TERMS * kSlot, sV = sK + RK * kSlot;
     const PagedKv &kv = a.kv;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, hd = kv.hd;
     const int halves = hd > 64 ? 2 : 1;
 
+    if (sQ & 1023) {                                // (it is aligned; else the products would read other elements)
+        if (tid == 0) atomicExch(kv.err, kErrWaitFull);
+        return;
+    }
     if (tid == 0) {
-        for (int i = 0; i < kRingK; i++) {
+        for (int i = 0; i < 2; i++) {
             mbar_init(&bars.kfull[i], 1);
             mbar_init(&bars.kempty[i], 1);
         }
-        for (int i = 0; i < kRingV; i++) {
+        for (int i = 0; i < 3; i++) {
             mbar_init(&bars.vfull[i], 1);
             mbar_init(&bars.vempty[i], 1);
         }
         for (int i = 0; i < 4; i++) mbar_init(&bars.clean[i], 2);
-        mbar_init(&bars.qfull, 1);
+        mbar_init(&bars.qfull, TERMS == 1 ? 1 : kSoftmax);
         mbar_init(&bars.qempty, 1);
         for (int i = 0; i < 2; i++) {
             mbar_init(&bars.sfull[i], 1);
-            mbar_init(&bars.pfull[i][0], 4);
-            mbar_init(&bars.pfull[i][1], 4);
-            mbar_init(&bars.odone[i][0], 1);
-            mbar_init(&bars.odone[i][1], 1);
+            mbar_init(&bars.pfull[i], kSoftmax / 2);
+            mbar_init(&bars.odone[i], 1);
         }
         mbar_init(&bars.drain, 1);
         fence_mbar_init();
-        s_abort = s_badpage = s_poison = 0;
+        R.abort = R.badpage = R.poison = 0;
     }
     if (tid == 32 * kWarpLoad) {
-        asm volatile("prefetch.tensormap [%0];" ::"l"(&mq));
+        if (TERMS == 1) asm volatile("prefetch.tensormap [%0];" ::"l"(&mq));
         asm volatile("prefetch.tensormap [%0];" ::"l"(&mk));
         asm volatile("prefetch.tensormap [%0];" ::"l"(&mv));
     }
     pdl_wait();
     if (warp == kWarpMma) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)),
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&R.tmem)),
                      "r"(kTmemCols));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
         fence_before();
@@ -320,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     fence_after();
     pdl_trigger();
-    const uint32_t tmem = s_tmem;
+    const uint32_t tmem = R.tmem;
     long long T_ = 0, G = 0;
     ChunkWalk wk;
     const int worker = blockIdx.x;
@@ -332,19 +373,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         const long long t0 = clock64();
         while (true) {
             if (mbar_try_wait_suspend(bar, parity)) return true;
-            if (*reinterpret_cast<volatile int *>(&s_abort)) return false;
+            if (*reinterpret_cast<volatile int *>(&R.abort)) return false;
             if (clock64() - t0 > kSpinCycles) {
                 atomicExch(kv.err, kErrWaitFull);
-                *reinterpret_cast<volatile int *>(&s_abort) = 1;
+                *reinterpret_cast<volatile int *>(&R.abort) = 1;
                 return false;
             }
         }
     };
     auto warp_wait = [&](uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
 
-    // the softmax warps take the registers that the others do not need (256 x 208 + 128 x 88 = 384 x 168)
+    // the softmax warps take the registers that the others do not need (512 x 104 + 128 x 64 = 640 x 96)
     if (warp >= kWarpLoad) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         if (warp == kWarpLoad) {
             // ---------------- copies.  A lane has one box of a tile: rows, and 64 of the elements
             const int rb_shift = min(kv.page_shift, 7), rb = 1 << rb_shift, boxes = kTile >> rb_shift;
@@ -362,17 +403,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                     return mine && it < P.tiles && r0 < P.hi && r0 + rb > P.lo ? ld_now(table + (r0 >> kv.page_shift)) : -1;
                 };
                 int page = page_of(0);
-                if (portion > 0) live = warp_wait(&bars.qempty, static_cast<uint32_t>((portion - 1) & 1));
-                if (!live) break;
-                if (lane == 0) {
-                    const int nq = P.two ? 2 : 1;
-                    mbar_arrive_expect_tx(&bars.qfull, nq * halves * q_bytes);
-                    for (int t = 0; t < nq; t++)
-                        for (int h = 0; h < halves; h++)
-                            tma3(sQ + t * kSlot + h * kHalf, &mq, h * 64, P.j * a.gqa + P.g0, P.tok0 + t * a.tile_tok, &bars.qfull);
+                if constexpr (TERMS == 1) {
+                    if (portion > 0) live = warp_wait(&bars.qempty, static_cast<uint32_t>((portion - 1) & 1));
+                    if (!live) break;
+                    if (lane == 0) {
+                        const int nq = P.two ? 2 : 1;
+                        mbar_arrive_expect_tx(&bars.qfull, nq * halves * q_bytes);
+                        for (int t = 0; t < nq; t++)
+                            for (int h = 0; h < halves; h++)
+                                tma3(sQ + t * kSlot + h * kHalf, &mq, h * 64, P.j * a.gqa + P.g0, P.tok0 + t * a.tile_tok, &bars.qfull);
+                    }
+                    __syncwarp();
+                    portion++;
                 }
-                __syncwarp();
-                portion++;
                 for (int it = 0; it < P.tiles && live; it++) {
                     const int r0 = P.kb0 + it * kTile + (pi << rb_shift), here = page;
                     const bool some = mine && r0 < P.hi && r0 + rb > P.lo;
@@ -383,7 +426,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const int y = (P.j << kv.page_shift) + (r0 & ((1 << kv.page_shift) - 1));
                     const bool dirty = bad || P.partial(P.kb0 + it * kTile);
                     for (int v = 0; v < 2; v++) {
-                        const int ring = v ? kRingV : kRingK, slot = n_tile % ring, use = n_tile / ring;
+                        const int ring = v ? RV : RK, slot = n_tile % ring, use = n_tile / ring;
                         uint64_t *full = (v ? bars.vfull : bars.kfull) + slot, *empty = (v ? bars.vempty : bars.kempty) + slot;
                         if (use > 0 && !warp_wait(empty, static_cast<uint32_t>((use - 1) & 1))) {
                             live = false;
@@ -392,9 +435,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (lane == 0) {
                             if (bad) {
                                 atomicExch(kv.err, kErrBadPos);
-                                *reinterpret_cast<volatile int *>(&s_badpage) = 1;
+                                *reinterpret_cast<volatile int *>(&R.badpage) = 1;
                             }
-                            if (v) *reinterpret_cast<volatile int *>(&s_dirty[n_tile & 3]) = dirty;
+                            if (v) *reinterpret_cast<volatile int *>(&R.dirty[n_tile & 3]) = dirty;
                             mbar_arrive_expect_tx(full, n * static_cast<uint32_t>(rb) * 128u);
                         }
                         __syncwarp();
@@ -405,7 +448,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             // Every copy is waited for by the products that read it.  Where a wait gave up, nothing of this warp's may still
             // be landing when the CTA ends: copies take microseconds, a millisecond is given to them.
-            if (*reinterpret_cast<volatile int *>(&s_abort))
+            if (*reinterpret_cast<volatile int *>(&R.abort))
                 for (const long long c0 = clock64(); clock64() - c0 < 2000000;) {
                 }
         } else if (warp == kWarpMma) {
@@ -421,23 +464,28 @@ __global__ void __launch_bounds__(kThreads, 1)
             bool live = true;
             auto scores = [&](int t) {
                 if (leader) {
-                    const uint32_t q = dQ + t * (kSlot / 16), k = dK + kslot * (kSlot / 16), d = tmem + kColS + t * kTile;
+                    const uint32_t k = dK + kslot * (kSlot / 16), d = tmem + kColS + t * kTile;
 #pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        if (i < ks) mma_ss(d, q + (i >> 2) * (kHalf / 16) + (i & 3) * 2, k + (i >> 2) * (kHalf / 16) + (i & 3) * 2, id_s, i > 0);
+                    for (int z = TERMS - 1; z >= 0; z--) {           // (the small term first: its sums lose less)
+                        const uint32_t q = dQ + (2 * z + t) * (kSlot / 16);
+#pragma unroll
+                        for (int i = 0; i < 8; i++)
+                            if (i < ks)
+                                mma_ss(d, q + (i >> 2) * (kHalf / 16) + (i & 3) * 2, k + (i >> 2) * (kHalf / 16) + (i & 3) * 2, id_s,
+                                       z < TERMS - 1 || i > 0);
+                    }
                     commit(&bars.sfull[t]);
                 }
             };
-            // the first or second half of the keys
-            auto values = [&](int t, int h, uint32_t acc) {
+            auto values = [&](int t, uint32_t acc) {
                 if (leader) {
                     const uint32_t v = dV + vslot * (kSlot / 16), p = tmem + kColS + t * kTile, d = tmem + kColO + t * kTile;
 #pragma unroll
-                    for (int i = 0; i < kTile / 32; i++) {
-                        const int k = h * (kTile / 32) + i;
-                        mma_ts(d, p + k * 8, v + k * (2048 / 16), id_o, acc | (i > 0));
-                    }
-                    commit(&bars.odone[t][h]);
+                    for (int i = 0; i < kTile / 16; i++)
+#pragma unroll
+                        for (int z = 0; z < TERMS; z++)
+                            mma_ts(d, p + (i >> 2) * 64 + z * 32 + (i & 3) * 8, v + i * (2048 / 16), id_o, acc | (i + z > 0));
+                    commit(&bars.odone[t]);
                 }
             };
             auto done_k = [&](bool last) {                      // this portion's last scores: q is free too
@@ -445,7 +493,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     commit(&bars.kempty[kslot]);
                     if (last) commit(&bars.qempty);
                 }
-                if (++kslot == kRingK) kslot = 0, kph ^= 1;
+                if (++kslot == RK) kslot = 0, kph ^= 1;
             };
             while (live && wk.next(a)) {
                 P.set(a, wk);
@@ -463,15 +511,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int t = 0; t < 2; t++) {
                         if (t == 1 && !two) break;
                         const bool last = t == 1 || !two;
-                        live = warp_wait(&bars.pfull[t][0], pph[t]) && (t > 0 || warp_wait(&bars.clean[cslot], cph));
-                        if (!live) break;
-                        fence_after();
-                        values(t, 0, it > 0);
-                        live = warp_wait(&bars.pfull[t][1], pph[t]);
+                        live = warp_wait(&bars.pfull[t], pph[t]) && (t > 0 || warp_wait(&bars.clean[cslot], cph));
                         if (!live) break;
                         pph[t] ^= 1;
                         fence_after();
-                        values(t, 1, 1);
+                        values(t, TERMS == 1 ? it > 0 : it % kFlush > 0);
                         if (leader && last) commit(&bars.vempty[vslot]);
                         if (more) {
                             if (t == 0) {
@@ -484,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     }
                     if (!live) break;
-                    if (++vslot == kRingV) vslot = 0;
+                    if (++vslot == RV) vslot = 0;
                     if (++cslot == 4) cslot = 0, cph ^= 1;
                 }
                 portion++;
@@ -503,11 +547,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             while (live && wk.next(a)) {
                 P.set(a, wk);
                 for (int it = 0; it < P.tiles; it++, nv++) {
-                    live = warp_wait(&bars.vfull[nv % kRingV], static_cast<uint32_t>(nv / kRingV & 1));
+                    live = warp_wait(&bars.vfull[nv % RV], static_cast<uint32_t>(nv / RV & 1));
                     if (!live) break;
-                    if (*reinterpret_cast<volatile int *>(&s_dirty[nv & 3])) {
+                    if (*reinterpret_cast<volatile int *>(&R.dirty[nv & 3])) {
                         const int32_t *table = kv.table + static_cast<long long>(P.b) * kv.table_stride;
-                        uint8_t *v = sm + (2 + kRingK + nv % kRingV) * kSlot;
+                        uint8_t *v = sm + (2 * TERMS + RK + nv % RV) * kSlot;
                         for (int row = ct; row < kTile; row += 64) {
                             const int key = P.kb0 + it * kTile + row;
                             const bool in = key >= P.lo && key < P.hi &&
@@ -530,7 +574,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 }
                                 if (bad) {
                                     *p = make_uint4(w[0], w[1], w[2], w[3]);
-                                    *reinterpret_cast<volatile int *>(&s_poison) = 1;
+                                    *reinterpret_cast<volatile int *>(&R.poison) = 1;
                                 }
                             }
                         }
@@ -542,70 +586,122 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
     } else {
-        // ---------------- softmax: thread = query row
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-        const int t = warp >> 2, r = tid & 127;
+        // ---------------- softmax: thread = half of the keys of a query row.  A wait that gave up is not looked at here:
+        // every warp goes on to the end, so that pairs stay together at their barriers (later waits return at once, the
+        // results are void and the error word says so).
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+        const int t = warp >> 3, h = warp >> 2 & 1, r = tid & 127, bar = 1 + t * 4 + (warp & 3);
         const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
-        const uint32_t colS = tmem + kColS + t * kTile + lanes, colO = tmem + kColO + t * kTile + lanes;
+        const uint32_t colS = tmem + kColS + t * kTile + 64 * h + lanes, colO = tmem + kColO + t * kTile + 64 * h + lanes;
+        const int hd16 = (hd + 15) & ~15, my_cols = min(64, hd16 - 64 * h);   // of O: its half (none: <= 0)
         const float l2 = a.scale * 1.4426950408889634f;   // scores in units of log2
         const int rt = r / a.hg, rh = r - rt * a.hg;
         uint32_t sph = 0, oph = 0;
-        bool first = true, live = true;
-        while (live && wk.next(a)) {
+        int portion = 0;
+        // f32 q of a portion into its terms, 16 rows by each warp of a tile; f16 has few exponents: a row's largest |q| is
+        // brought to [2^9, 2^10)
+        auto stage = [&]() {
+            if (portion > 0) warp_wait(&bars.qempty, static_cast<uint32_t>((portion - 1) & 1));
+            if (t == 0 || P.two)
+                for (int i = 0; i < 16; i++) {
+                    const int row = (warp & 7) * 16 + i, tk = row / a.hg, hh = row - tk * a.hg, tok = t * a.tile_tok + tk;
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (tk < a.tile_tok && tok < P.ntok && hh < P.ng && 4 * lane < hd)
+                        v = ld_now(reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + (P.tok0 + tok) * a.q_stride +
+                                                                    static_cast<long long>(P.j * a.gqa + P.g0 + hh) * hd) + lane);
+                    v.x *= l2, v.y *= l2, v.z *= l2, v.w *= l2;
+                    const unsigned mx = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)))));
+                    const int e = max(-110, min(110, static_cast<int>(mx >> 23) - 127 - 9));
+                    const float up = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+                    if (lane == 0) R.unit[portion & 1][t][row] = static_cast<uint8_t>(127 + e);
+                    v.x *= up, v.y *= up, v.z *= up, v.w *= up;
+                    uint2 hi, lo;
+                    hi.x = pack<false>(v.x, v.y);
+                    hi.y = pack<false>(v.z, v.w);
+                    const float2 f0 = __half22float2(*reinterpret_cast<const __half2 *>(&hi.x));
+                    const float2 f1 = __half22float2(*reinterpret_cast<const __half2 *>(&hi.y));
+                    lo.x = pack<false>(v.x - f0.x, v.y - f0.y);
+                    lo.y = pack<false>(v.z - f1.x, v.w - f1.y);
+                    const uint32_t at = t * kSlot + (lane >> 4) * kHalf + row * 128 + (((lane >> 1 & 7) ^ (row & 7)) << 4) + (lane & 1) * 8;
+                    *reinterpret_cast<uint2 *>(sm + at) = hi;
+                    *reinterpret_cast<uint2 *>(sm + 2 * kSlot + at) = lo;
+                }
+            fence_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.qfull);
+        };
+        bool have = wk.next(a);
+        if (tid == 0) {                               // (later portions begin their segments)
+            ChunkJoin j{-1, 0, 0, 0};
+            if (have && wk.t0 > 0 && wk.t1 == wk.nt) j = {chunk_owner(a, wk, T_, G), wk.b, wk.head, wk.seg};
+            static_cast<ChunkJoin *>(a.joins)[worker] = j;
+        }
+        if (have) {
             P.set(a, wk);
-            if (first && tid == 0) {
-                ChunkJoin j{-1, 0, 0, 0};
-                if (!P.begins && P.ends) j = {chunk_owner(a, wk, T_, G), wk.b, wk.head, wk.seg};
-                static_cast<ChunkJoin *>(a.joins)[worker] = j;
-            }
-            first = false;
-            if (t == 1 && !P.two) continue;
+            if constexpr (TERMS == 2) stage();
+        }
+        while (have) {
+            const bool run = t == 0 || P.two;         // (else there is no second tile)
             const int tok = t * a.tile_tok + rt;
             const bool real = rt < a.tile_tok && tok < P.ntok && rh < P.ng;
             const int see_hi = real ? min(P.hi, P.base + tok + 1) : 0;
             const int see_lo = real ? max(P.lo, a.window > 0 ? P.base + tok + 1 - a.window : 0) : 0;
             const int tile_free_hi = P.base + t * a.tile_tok + 1;
             const int tile_free_lo = a.window > 0 ? P.base + min(P.ntok, (t + 1) * a.tile_tok) - a.window : 0;
-            float m = kNone, l = 0.f;
-            for (int it = 0; it < P.tiles; it++) {
-                const int kb = P.kb0 + it * kTile;
-                live = warp_wait(&bars.sfull[t], sph);
+            const bool whole = P.begins && P.ends;
+            const long long row = static_cast<long long>(P.tok0 + tok) * a.n_heads + P.j * a.gqa + P.g0 + rh;
+            float *const part = chunk_part(a, worker, P.begins) + (t * kTile + (r & ~3)) * kTile + 4 * (lane & 3);
+            float m = kNone, l = 0.f, unit = l2, m_acc = 0.f;
+            bool acc = false;                         // TERMS 2: `part` holds a sum, measured against m_acc
+            const int tiles = run ? P.tiles : 0;
+            for (int it = 0; it < tiles; it++) {
+                const int kb = P.kb0 + it * kTile + 64 * h;
+                warp_wait(&bars.sfull[t], sph);
                 sph ^= 1;
-                if (!live) break;
                 fence_after();
-                float s[kTile];
+                if (TERMS == 2 && it == 0) unit = __uint_as_float(static_cast<uint32_t>(R.unit[portion & 1][t][r]) << 23);
+                const bool badpage = *reinterpret_cast<volatile int *>(&R.badpage) != 0;
+                const int kb_all = kb - 64 * h;
+                const bool masked = kb_all + kTile > tile_free_hi || kb_all < tile_free_lo || kb_all < P.lo || badpage;
+                float s[64];
+                auto read = [&]() {
+                    ld32(colS, s);
+                    ld32(colS + 32, s + 32);
+                    ld_wait(s);
+                    if (masked) {
+                        const int c0 = see_lo - kb, c1 = see_hi - kb;
 #pragma unroll
-                for (int c = 0; c < kTile; c += 32) ld32(colS + c, s + c);
-                ld_wait(s);
-                const bool masked = kb + kTile > tile_free_hi || kb < tile_free_lo || kb < P.lo ||
-                                    *reinterpret_cast<volatile int *>(&s_badpage);
-                if (masked) {
-                    const int c0 = see_lo - kb, c1 = see_hi - kb;
-#pragma unroll
-                    for (int c = 0; c < kTile; c++)
-                        if (c < c0 || c >= c1) s[c] = -INFINITY;
-                    if (*reinterpret_cast<volatile int *>(&s_badpage)) {
+                        for (int c = 0; c < 64; c++)
+                            if (c < c0 || c >= c1) s[c] = -INFINITY;
+                        if (badpage) {
 #pragma unroll 1
-                        for (int g = 0; g < kTile / 16; g++) {
-                            const int key = kb + 16 * g;
-                            if (key < P.hi && paged_off(kv, P.b, P.j, key) < 0) {
+                            for (int g = 0; g < 4; g++) {
+                                const int key = kb + 16 * g;
+                                if (key < P.hi && paged_off(kv, P.b, P.j, key) < 0) {
 #pragma unroll
-                                for (int c = 0; c < kTile; c++)
-                                    if (c >> 4 == g) s[c] = -INFINITY;
+                                    for (int c = 0; c < 64; c++)
+                                        if (c >> 4 == g) s[c] = -INFINITY;
+                                }
                             }
                         }
                     }
-                }
-                // what was summed against the old m is rescaled, once the products before half h are done
-                auto raise = [&](float to, int h) {
+                };
+                // the row's largest score of the tile, from both halves
+                auto top_of = [&]() {
+                    R.x[t][h][r] = largest<64>(s, unit);
+                    pair_sync(bar);
+                    return max3(R.x[t][0][r], R.x[t][1][r], R.x[t][1][r]) - kBias;
+                };
+                // what was summed against the old m is rescaled, once its products are done
+                auto raise = [&](float to) {
                     const float f = ex2(m - to);
                     l *= f;
                     m = to;
-                    if (it > 0 || h > 0) {
-                        if (!(h ? warp_wait(&bars.odone[t][0], oph) : warp_wait(&bars.odone[t][1], oph ^ 1))) return false;
+                    if (it > 0) {
+                        warp_wait(&bars.odone[t], oph ^ 1);   // (of the tile before: that phase is the last one)
                         fence_after();
 #pragma unroll 1
-                        for (int c = 0; c < ((hd + 15) & ~15); c += 32) {
+                        for (int c = 0; c < my_cols; c += 32) {
                             float o[32];
                             ld32(colO + c, o);
                             ld_wait(o);
@@ -615,108 +711,165 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                         st_wait();
                     }
-                    return true;
                 };
+                read();
                 if (it == 0 || masked) {               // (a masked tile: so that no row stays without a maximum)
-                    const float top = largest<kTile>(s, l2) - kBias;
+                    const float top = top_of();
                     const bool up = real && !(top <= m + (m > kNone ? kSlack : 0.f));
-                    if (__any_sync(0xffffffffu, up)) live = raise(up ? top : m, 0);
-                    if (!live) break;
+                    if (__any_sync(0xffffffffu, up)) raise(up ? top : m);
+                }
+                uint32_t p[TERMS][32];
+                float sum = weights<BF, TERMS>(s, unit, m, p);
+                if (pair_any(bar, real && !(sum <= kMost))) {   // (NaN: of a NaN, or of a score of +inf)
+                    read();
+                    const float top = top_of();
+                    raise(real && !(top <= m) ? top : m);
+                    sum = weights<BF, TERMS>(s, unit, m, p);
+                }
+                l += sum;
+                if constexpr (TERMS == 2) {
+                    if (it > 0 && it % kFlush == 0) {  // O so far to the sum in the workspace; the next products start from 0
+                        warp_wait(&bars.odone[t], oph ^ 1);
+                        fence_after();
+                        const float f = acc ? ex2(m_acc - m) : 0.f;
+#pragma unroll 1
+                        for (int c = 0; c < my_cols; c += 16) {
+                            float o[16];
+                            ld16(colO + c, o);
+                            ld_wait(o);
+                            uint4 x[4];
+                            as_quads(o, x);
+                            turn4(x, lane);
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                const float fk = __shfl_sync(0xffffffffu, f, (lane & ~3) + k);
+                                float4 *z = reinterpret_cast<float4 *>(part + k * kTile + 64 * h + c);
+                                float4 y = as_float4(x[k]);
+                                if (acc) {
+                                    const float4 w = *z;
+                                    y = make_float4(fmaf(w.x, fk, y.x), fmaf(w.y, fk, y.y), fmaf(w.z, fk, y.z), fmaf(w.w, fk, y.w));
+                                }
+                                *z = y;
+                            }
+                        }
+                        acc = true;
+                        m_acc = m;
+                    }
                 }
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    uint32_t p[32];
-                    float sum = weights<BF>(s + 64 * h, l2, m, p);
-                    const bool over = real && !(sum <= kMost);   // (NaN: of a NaN, or of a score of +inf)
-                    if (__any_sync(0xffffffffu, over)) {
-                        const float top = largest<64>(s + 64 * h, l2) - kBias;
-                        live = raise(over && !(top <= m) ? top : m, h);
-                        if (!live) break;
-                        sum = weights<BF>(s + 64 * h, l2, m, p);
-                    }
-                    l += sum;
-                    st32(colS + 32 * h, p);
-                    st_wait();
-                    fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&bars.pfull[t][h]);
-                }
-                if (!live) break;
+                for (int z = 0; z < TERMS; z++) st32(colS + 32 * z, p[z]);
+                st_wait();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars.pfull[t]);
                 oph ^= 1;
             }
-            if (!live) break;
             // ---------------- the portion's end
-            live = warp_wait(&bars.odone[t][1], oph ^ 1);
-            if (!live) break;
-            fence_after();
-            const bool whole = P.begins && P.ends, poison = *reinterpret_cast<volatile int *>(&s_poison) != 0;
-            const long long row = static_cast<long long>(P.tok0 + tok) * a.n_heads + P.j * a.gqa + P.g0 + rh;
-            const float inv = whole ? inverse_sum(l) : 1.f;
-            float *part = chunk_part(a, worker, P.begins);
-            // the four rows of the lane's group of four: where they are, and which there are
-            long long rows4[4];
-            unsigned there = 0;
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                rows4[k] = __shfl_sync(0xffffffffu, row, (lane & ~3) + k);
-                there |= static_cast<unsigned>(__shfl_sync(0xffffffffu, static_cast<int>(real), (lane & ~3) + k)) << k;
+            const ChunkWalk cur = wk;
+            portion++;
+            have = wk.next(a);
+            if constexpr (TERMS == 2) {                // the next portion's q, while the last products run
+                if (have) {
+                    P.set(a, wk);
+                    stage();
+                }
             }
+            if (run) {
+                pair_sync(bar);                        // (the last maxima have been read)
+                R.x[t][h][r] = l;
+                pair_sync(bar);
+                l = R.x[t][0][r] + R.x[t][1][r];
+                pair_sync(bar);
+                warp_wait(&bars.odone[t], oph ^ 1);
+                fence_after();
+                const float inv = whole ? inverse_sum(l) : 1.f, f = acc ? ex2(m_acc - m) : 0.f;
+                // The results of four rows lie with four lanes, which exchange them: each store is of four lanes' 64 bytes
+                // of one row.  (A row per lane: 4000 clocks a portion.)  The rows of the lane's group, and which there are:
+                long long rows4[4];
+                float inv4[4], f4[4];
+                unsigned there = 0;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    rows4[k] = __shfl_sync(0xffffffffu, row, (lane & ~3) + k);
+                    inv4[k] = __shfl_sync(0xffffffffu, inv, (lane & ~3) + k);
+                    f4[k] = __shfl_sync(0xffffffffu, f, (lane & ~3) + k);
+                    there |= static_cast<unsigned>(__shfl_sync(0xffffffffu, static_cast<int>(real), (lane & ~3) + k)) << k;
+                }
+                const bool poison = *reinterpret_cast<volatile int *>(&R.poison) != 0;
 #pragma unroll 1
-            for (int c = 0; c < ((hd + 15) & ~15); c += 32) {
-                float o[32];
-                ld32(colO + c, o);
-                ld_wait(o);
-                if (real && poison)
-                    for (int it = 0; it < P.tiles; it++) {
-                        const int kb = P.kb0 + it * kTile;
-                        if (!P.partial(kb)) continue;
-                        for (int key = max(kb, see_lo); key < min(kb + kTile, see_hi); key++) {
-                            const long long off = paged_off(kv, P.b, P.j, key);
-                            if (off < 0) continue;
-                            const T *v = static_cast<const T *>(kv.v) + off + c;
+                for (int c = 0; c < my_cols; c += 32) {
+                    const int e0 = 64 * h + c;         // elements e0 ..
+                    float o[32];
+                    ld32(colO + c, o);
+                    ld_wait(o);
+                    if (poison) {
+                        Part Q;
+                        Q.set(a, cur);
+                        for (int it = 0; real && it < Q.tiles; it++) {
+                            const int kb = Q.kb0 + it * kTile;
+                            if (!Q.partial(kb)) continue;
+                            for (int key = max(kb, see_lo); key < min(kb + kTile, see_hi); key++) {
+                                const long long off = paged_off(kv, Q.b, Q.j, key);
+                                if (off < 0) continue;
+                                const T *v = static_cast<const T *>(kv.v) + off + e0;
 #pragma unroll
-                            for (int k = 0; k < 32; k++)
-                                if (c + k < hd) o[k] += not_finite(to_f(v[k]));
+                                for (int k = 0; k < 32; k++)
+                                    if (e0 + k < hd) o[k] += not_finite(to_f(v[k]));
+                            }
                         }
+                        __syncwarp();
                     }
-                // Four lanes have four rows' 64 bytes (whole: 16-bit; else 2 x 64 of f32): they exchange them, so that each
-                // store is of four lanes' 64 bytes of one row.  (A row per lane: 4000 clocks a portion.)
-                if (whole) {
-                    uint4 x[4];
-#pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        x[k] = make_uint4(pack<BF>(o[8 * k] * inv, o[8 * k + 1] * inv), pack<BF>(o[8 * k + 2] * inv, o[8 * k + 3] * inv),
-                                          pack<BF>(o[8 * k + 4] * inv, o[8 * k + 5] * inv), pack<BF>(o[8 * k + 6] * inv, o[8 * k + 7] * inv));
-                    turn4(x, lane);
-                    const int e = c + 8 * (lane & 3);
-#pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        if ((there >> k & 1) && e < hd) *reinterpret_cast<uint4 *>(static_cast<T *>(a.out) + rows4[k] * hd + e) = x[k];
-                } else {
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
+                    if (TERMS == 1 && whole) {
                         uint4 x[4];
 #pragma unroll
                         for (int k = 0; k < 4; k++)
-                            x[k] = make_uint4(__float_as_uint(o[16 * h + 4 * k]), __float_as_uint(o[16 * h + 4 * k + 1]),
-                                              __float_as_uint(o[16 * h + 4 * k + 2]), __float_as_uint(o[16 * h + 4 * k + 3]));
+                            x[k] = make_uint4(pack<BF>(o[8 * k] * inv, o[8 * k + 1] * inv), pack<BF>(o[8 * k + 2] * inv, o[8 * k + 3] * inv),
+                                              pack<BF>(o[8 * k + 4] * inv, o[8 * k + 5] * inv), pack<BF>(o[8 * k + 6] * inv, o[8 * k + 7] * inv));
                         turn4(x, lane);
+                        const int e = e0 + 8 * (lane & 3);
 #pragma unroll
                         for (int k = 0; k < 4; k++)
-                            if (there >> k & 1)
-                                *reinterpret_cast<uint4 *>(part + (t * kTile + (r & ~3) + k) * kTile + c + 16 * h + 4 * (lane & 3)) = x[k];
+                            if ((there >> k & 1) && e < hd) *reinterpret_cast<uint4 *>(static_cast<T *>(a.out) + rows4[k] * hd + e) = x[k];
+                    } else {
+#pragma unroll
+                        for (int g = 0; g < 2; g++) {
+                            uint4 x[4];
+                            as_quads(o + 16 * g, x);
+                            turn4(x, lane);
+                            const int e = e0 + 16 * g + 4 * (lane & 3);
+#pragma unroll
+                            for (int k = 0; k < 4; k++)
+                                if (there >> k & 1) {
+                                    float4 y = as_float4(x[k]), *z = reinterpret_cast<float4 *>(part + k * kTile + e0 + 16 * g);
+                                    if (TERMS == 2 && acc) {
+                                        const float4 w = *z;
+                                        y = make_float4(fmaf(w.x, f4[k], y.x), fmaf(w.y, f4[k], y.y), fmaf(w.z, f4[k], y.z), fmaf(w.w, f4[k], y.w));
+                                    }
+                                    if (!whole) {
+                                        *z = y;
+                                    } else if (e < hd) {
+                                        const float i = inv4[k];
+                                        *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + rows4[k] * hd + e) =
+                                            make_float4(y.x * i, y.y * i, y.z * i, y.w * i);
+                                    }
+                                }
+                        }
                     }
                 }
-                __syncwarp();
+                if (h == 0 && real) {
+                    if (whole && a.lse) a.lse[row] = lse_of(m, l);
+                    if (!whole) {
+                        float *ml = chunk_part(a, worker, cur.t0 == 0) + 2 * kTile * kTile + t * kTile + r;
+                        ml[0] = m;
+                        ml[2 * kTile] = l;
+                    }
+                }
+                fence_before();
             }
-            if (real && whole && a.lse) a.lse[row] = lse_of(m, l);
-            if (real && !whole) {
-                part[2 * kTile * kTile + t * kTile + r] = m;
-                part[2 * kTile * kTile + 2 * kTile + t * kTile + r] = l;
+            if constexpr (TERMS == 1) {
+                if (have) P.set(a, wk);
             }
-            fence_before();
         }
-        if (first && tid == 0) static_cast<ChunkJoin *>(a.joins)[worker] = ChunkJoin{-1, 0, 0, 0};
     }
     __syncthreads();
     fence_after();
@@ -751,10 +904,10 @@ bool encode(CUtensorMap &m, bool bf, const void *base, uint64_t nx, uint64_t ny,
                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <bool BF>
+template <bool BF, int TERMS>
 cudaError_t go(const PagedChunkArgs &a, const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv, cudaStream_t st) {
-    cudaError_t e = allow_smem<k_chunk_tc<BF>>(kSmem);
-    return e != cudaSuccess ? e : launch_pdl(k_chunk_tc<BF>, dim3(a.workers), dim3(kThreads), kSmem, st, a, mq, mk, mv);
+    cudaError_t e = allow_smem<k_chunk_tc<BF, TERMS>>(kSmem);
+    return e != cudaSuccess ? e : launch_pdl(k_chunk_tc<BF, TERMS>, dim3(a.workers), dim3(kThreads), kSmem, st, a, mq, mk, mv);
 }
 
 }  // namespace
@@ -762,7 +915,7 @@ cudaError_t go(const PagedChunkArgs &a, const CUtensorMap &mq, const CUtensorMap
 // A page's rows and a tile's queries have to be boxes (rows of 128 bytes and more, 16 rows and more).  Scores are
 // compared before they are scaled, so the scale is positive.
 bool chunk_on_tc(const PagedChunkArgs &a) {
-    return a.q16 && a.kv.hd >= 64 && a.kv.hd <= 128 && a.kv.page_shift >= 4 && a.scale > 0.f && encode_fn();
+    return (a.q16 || a.kv.dtype == STYX_F16) && a.kv.hd >= 64 && a.kv.hd <= 128 && a.kv.page_shift >= 4 && a.scale > 0.f && encode_fn();
 }
 uint64_t chunk_tc_parts(int sms) { return 2ull * sms * 2 * kTile * (kTile + 2) * 4; }
 
@@ -784,11 +937,12 @@ cudaError_t launch_chunk_tc(PagedChunkArgs a, int sms, cudaStream_t st) {
     const uint64_t rows = static_cast<uint64_t>(kv.n_kv) << kv.page_shift;
     const uint32_t box = 1u << std::min(kv.page_shift, 7);
     CUtensorMap mq, mk, mv;
-    if (!encode(mq, bf, a.q, kv.hd, a.n_heads, a.n_tokens, kv.hd, a.q_stride, a.hg, a.tile_tok) ||
+    if (!a.q16) memset(&mq, 0, sizeof(mq));
+    if ((a.q16 && !encode(mq, bf, a.q, kv.hd, a.n_heads, a.n_tokens, kv.hd, a.q_stride, a.hg, a.tile_tok)) ||
         !encode(mk, bf, kv.k, kv.hd, rows, kv.n_pages, kv.hd, kv.page_stride, box, 1) ||
         !encode(mv, bf, kv.v, kv.hd, rows, kv.n_pages, kv.hd, kv.page_stride, box, 1))
         return cudaErrorInvalidValue;
-    cudaError_t e = bf ? go<true>(a, mq, mk, mv, st) : go<false>(a, mq, mk, mv, st);
+    cudaError_t e = bf ? go<true, 1>(a, mq, mk, mv, st) : a.q16 ? go<false, 1>(a, mq, mk, mv, st) : go<false, 2>(a, mq, mk, mv, st);
     return e != cudaSuccess || !cut ? e : launch_chunk_join(a, 2 * kTile, kTile, kTile, st);
 }
 

@@ -173,6 +173,47 @@ def test_sharp_and_flat_heads(dtype, q_type):
     assert np.all(np.abs(got - ref[0]) <= 6e-5 * np.abs(ref[0]).max() + h * (ref[2] + np.abs(ref[0]) * (1 + h)))
 
 
+@pytest.mark.parametrize("dtype,q_type", [("f16", "f16"), ("bf16", "bf16"), ("f16", "f32"), ("bf16", "f32"), ("f32", "f32")])
+@pytest.mark.parametrize("rise", [0.0, 30.0, 200.0, -200.0])
+def test_long_portions_and_rising_scores(dtype, q_type, rise):
+    """Enough tiles that every worker has many of one segment in a row, and
+    scores that rise (or fall) by `rise` from the first row to the last: what a
+    row is measured against has to move, in tiles of every kind."""
+    rng = np.random.default_rng(12)
+    lens, news, heads, n_kv, hd, page = [2050, 1100, 2304, 700], [300, 290, 310, 700], 16, 8, 128, 64
+    kv, ks, vs = make_cache(rng, lens, n_kv, hd, page, dtype)
+    start = starts(news)
+    q = torch.from_numpy(rng.normal(0, 1, (start[-1], heads, hd)).astype(np.float32))
+    q[..., 0] = 8.0
+    q = q.to(TYPES[q_type]).to(DEV)
+    for b, n in enumerate(lens):      # score += 8 K[r][0] / sqrt(128)
+        step = torch.arange(n, dtype=torch.float64) * (rise * 128 ** 0.5 / 8 / max(lens))
+        k0 = step.to(torch.float32).to(TYPES[dtype])
+        r = torch.arange(n)
+        kv.k[kv.table[b].long().cpu()[r // page].to(DEV), :, (r % page).to(DEV), 0] = k0.to(DEV)[:, None]
+        ks[b][:, :, 0] = k0.double().numpy()[:, None]
+    lse = torch.zeros(start[-1], heads, device=DEV)
+    got = kv.attend_chunk(q, I(start), lse=lse).double()
+    kv.ctx.check_device_error()
+    h = 0.0 if q_type == "f32" else torch.finfo(TYPES[q_type]).eps / 2
+    f32 = 1e-5 + 2.0 ** -24 * 4 * abs(rise)          # scores of that size in f32: 2^-24 x 4 of them move a weight
+    for b, n in enumerate(lens):
+        k, v = T(ks[b]), T(vs[b])
+        at = slice(start[b], start[b + 1])
+        x = torch.einsum("tjgd,rjd->jgtr", q[at].double().unflatten(1, (n_kv, 2)), k) * hd ** -0.5
+        hidden = torch.arange(n, device=DEV)[None] > torch.arange(n - news[b], n, device=DEV)[:, None]
+        x.masked_fill_(hidden, -torch.inf)
+        p = torch.softmax(x, -1)
+        out = torch.einsum("jgtr,rjd->tjgd", p, v).flatten(1, 2)
+        mag = torch.einsum("jgtr,rjd->tjgd", p, v.abs()).flatten(1, 2)
+        tol = f32 * out.abs().max() + h * (mag + out.abs() * (1 + h))
+        assert ((got[at] - out).abs() <= tol).all(), f"{((got[at] - out).abs() / tol).max().item():.2f} of the tolerance"
+        ref = torch.logsumexp(x, -1).permute(2, 0, 1).flatten(1, 2)
+        assert ((lse[at].double() - ref).abs() <= 1e-5 * ref.abs().clamp(min=1)).all()
+    again = kv.attend_chunk(q, I(start))
+    assert torch.equal(again.double(), got)
+
+
 def test_strided_queries_scales_and_many_segments():
     """q as a slice of a projection's output; another scale; more segments than SMs."""
     rng = np.random.default_rng(5)
