@@ -6,21 +6,22 @@
 // so that a kv head's rows are read once for all of them) over tiles of 128
 // keys:
 //   S = Q K^T          tcgen05.mma, both operands from shared memory
-//   P = 2^(S - m)      two threads per query row, half of the keys each
+//   P = 2^(S - m)      a thread per query row: no exchange between threads
 //   O += P V           tcgen05.mma, P from TMEM, where it lies over S
 // The two tiles take turns: while one's S and O are being multiplied the
 // other's rows are exponentiated.  What a row's scores are measured against is
 // not the running maximum but that of its first tile, until weights become too
 // large for it: no tile but the first is searched for its maximum, and O is
-// rescaled rarely, by the row's own threads.
+// rescaled rarely, by the row's own thread.
 //
 // f32 q (TERMS 2): q and p are split into two f16 terms, 22 bits; products are
 // exact, twice as many.  The MMA cuts its sums off instead of rounding them, an
 // error to one side that grows with every step (some 2^-26 of O each), so O is
 // added to a sum of its own in the workspace every kFlush tiles.
 //
-// Roles, linked by mbarriers with bounded waits: sixteen softmax warps (eight
-// per query tile), a warp that copies (TMA: boxes of min(page, 128) rows x 64
+// Roles, linked by mbarriers with bounded waits: eight softmax warps (four per
+// query tile; with eight per tile, half of the keys each, 594 us instead of
+// @@ for a prompt of 8192), a warp that copies (TMA: boxes of min(page, 128) rows x 64
 // elements of a page, 128-byte swizzled; 16-bit q with one box per tile and 64
 // elements; f32 q is brought and split by the softmax warps), a warp that issues
 // the products, and two warps that go over V where a tile is not seen in whole
@@ -43,7 +44,7 @@
 namespace styx {
 namespace {
 
-constexpr int kSoftmax = 16;                        // warps; the others behind them
+constexpr int kSoftmax = 8;                         // warps; the others behind them
 constexpr int kThreads = 32 * (kSoftmax + 4);
 constexpr int kWarpLoad = kSoftmax, kWarpMma = kSoftmax + 1, kWarpClean = kSoftmax + 2;
 constexpr int kTile = 128;                          // query rows of a tile, keys of a tile
@@ -74,7 +75,6 @@ struct Rest {
     Bars bars;
     uint32_t tmem;
     int abort, badpage, poison, dirty[4];
-    float x[2][2][kTile];                           // of a tile's rows: what the two halves tell each other
     uint8_t unit[2][2][kTile];                      // f32 q, by portions: the exponent of what a row's scores are in units of
 };
 constexpr int kSmem = 7 * kSlot + sizeof(Rest);
@@ -204,23 +204,23 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-// 64 scores to the weights 2^(s unit - m), packed (in terms), and their sum.
+// 32 scores to the weights 2^(s unit - m), packed (in terms), and their sum.
 // (Part of the exponentials as polynomials on the FMA units made it slower.)
 template <bool BF, int TERMS>
-__device__ __forceinline__ float weights(const float (&s)[64], float unit, float m, uint32_t (&p)[TERMS][32]) {
+__device__ __forceinline__ float weights(const float (&s)[32], float unit, float m, uint32_t (&p)[TERMS][32], int at) {
     f32x2 sum[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
     const f32x2 u2 = pair(unit, unit), nm = pair(-m, -m);
 #pragma unroll
-    for (int c = 0; c < 32; c++) {
+    for (int c = 0; c < 16; c++) {
         float x, y;
         unpair(fma2(pair(s[2 * c], s[2 * c + 1]), u2, nm), x, y);
         x = ex2(x);
         y = ex2(y);
         sum[c & 1] = add2(sum[c & 1], pair(x, y));
-        p[0][c] = pack<BF>(x, y);
+        p[0][at + c] = pack<BF>(x, y);
         if constexpr (TERMS == 2) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&p[0][c]));
-            p[TERMS - 1][c] = pack<BF>(x - f.x, y - f.y);
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&p[0][at + c]));
+            p[TERMS - 1][at + c] = pack<BF>(x - f.x, y - f.y);
         }
     }
     float x, y;
@@ -264,17 +264,16 @@ __device__ __forceinline__ void turn4(uint4 (&x)[4], int lane) {
     swap(x[0], x[2], 2);
     swap(x[1], x[3], 2);
 }
-// barriers of the two warps that share 32 query rows
-__device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
-__device__ __forceinline__ bool pair_any(int id, bool v) {
-    uint32_t r;
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\t"
-        "barrier.cta.red.or.pred q, %2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-        : "=r"(r)
-        : "r"(static_cast<uint32_t>(v)), "r"(id)
-        : "memory");
-    return r != 0;
+// two packed 16-bit numbers times a power of two
+template <bool BF>
+__device__ __forceinline__ uint32_t scaled(uint32_t v, float f) {
+    if constexpr (BF) {
+        const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&v));
+        return pack<true>(x.x * f, x.y * f);
+    } else {
+        const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&v));
+        return pack<false>(x.x * f, x.y * f);
+    }
 }
 __device__ __forceinline__ float not_finite(float v) { return fabsf(v) <= 3.4028234e38f ? 0.f : v; }
 
@@ -339,7 +338,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(&bars.qempty, 1);
         for (int i = 0; i < 2; i++) {
             mbar_init(&bars.sfull[i], 1);
-            mbar_init(&bars.pfull[i], kSoftmax / 2);
+            mbar_init(&bars.pfull[i], kSoftmax / 2);      // (a tile's warps)
             mbar_init(&bars.odone[i], 1);
         }
         mbar_init(&bars.drain, 1);
@@ -383,9 +382,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     auto warp_wait = [&](uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
 
-    // the softmax warps take the registers that the others do not need (512 x 104 + 128 x 64 = 640 x 96)
+    // the softmax warps take the registers that the others do not need (256 x 208 + 128 x 88 = 384 x 168)
     if (warp >= kWarpLoad) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         if (warp == kWarpLoad) {
             // ---------------- copies.  A lane has one box of a tile: rows, and 64 of the elements
             const int rb_shift = min(kv.page_shift, 7), rb = 1 << rb_shift, boxes = kTile >> rb_shift;
@@ -586,25 +585,24 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
     } else {
-        // ---------------- softmax: thread = half of the keys of a query row.  A wait that gave up is not looked at here:
-        // every warp goes on to the end, so that pairs stay together at their barriers (later waits return at once, the
-        // results are void and the error word says so).
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
-        const int t = warp >> 3, h = warp >> 2 & 1, r = tid & 127, bar = 1 + t * 4 + (warp & 3);
+        // ---------------- softmax: thread = query row.  A wait that gave up is not looked at here: every warp goes on to
+        // the end (later waits return at once, the results are void and the error word says so).
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        const int t = warp >> 2, r = tid & 127;
         const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
-        const uint32_t colS = tmem + kColS + t * kTile + 64 * h + lanes, colO = tmem + kColO + t * kTile + 64 * h + lanes;
-        const int hd16 = (hd + 15) & ~15, my_cols = min(64, hd16 - 64 * h);   // of O: its half (none: <= 0)
+        const uint32_t colS = tmem + kColS + t * kTile + lanes, colO = tmem + kColO + t * kTile + lanes;
+        const int hd16 = (hd + 15) & ~15;
         const float l2 = a.scale * 1.4426950408889634f;   // scores in units of log2
         const int rt = r / a.hg, rh = r - rt * a.hg;
         uint32_t sph = 0, oph = 0;
         int portion = 0;
-        // f32 q of a portion into its terms, 16 rows by each warp of a tile; f16 has few exponents: a row's largest |q| is
+        // f32 q of a portion into its terms, 32 rows by each warp of a tile; f16 has few exponents: a row's largest |q| is
         // brought to [2^9, 2^10)
         auto stage = [&]() {
             if (portion > 0) warp_wait(&bars.qempty, static_cast<uint32_t>((portion - 1) & 1));
             if (t == 0 || P.two)
-                for (int i = 0; i < 16; i++) {
-                    const int row = (warp & 7) * 16 + i, tk = row / a.hg, hh = row - tk * a.hg, tok = t * a.tile_tok + tk;
+                for (int i = 0; i < 32; i++) {
+                    const int row = (warp & 3) * 32 + i, tk = row / a.hg, hh = row - tk * a.hg, tok = t * a.tile_tok + tk;
                     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
                     if (tk < a.tile_tok && tok < P.ntok && hh < P.ng && 4 * lane < hd)
                         v = ld_now(reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + (P.tok0 + tok) * a.q_stride +
@@ -655,44 +653,33 @@ __global__ void __launch_bounds__(kThreads, 1)
             bool acc = false;                         // TERMS 2: `part` holds a sum, measured against m_acc
             const int tiles = run ? P.tiles : 0;
             for (int it = 0; it < tiles; it++) {
-                const int kb = P.kb0 + it * kTile + 64 * h;
+                const int kb = P.kb0 + it * kTile;
                 warp_wait(&bars.sfull[t], sph);
                 sph ^= 1;
                 fence_after();
                 if (TERMS == 2 && it == 0) unit = __uint_as_float(static_cast<uint32_t>(R.unit[portion & 1][t][r]) << 23);
                 const bool badpage = *reinterpret_cast<volatile int *>(&R.badpage) != 0;
-                const int kb_all = kb - 64 * h;
-                const bool masked = kb_all + kTile > tile_free_hi || kb_all < tile_free_lo || kb_all < P.lo || badpage;
-                float s[64];
-                auto read = [&]() {
-                    ld32(colS, s);
-                    ld32(colS + 32, s + 32);
+                const bool masked = kb + kTile > tile_free_hi || kb < tile_free_lo || kb < P.lo || badpage;
+                // scores 32 i .. of the row: loads begun, and there
+                auto get = [&](int i, float (&s)[32]) { ld32(colS + 32 * i, s); };
+                auto have_it = [&](int i, float (&s)[32]) {
                     ld_wait(s);
                     if (masked) {
-                        const int c0 = see_lo - kb, c1 = see_hi - kb;
+                        const int c0 = see_lo - kb - 32 * i, c1 = see_hi - kb - 32 * i;
 #pragma unroll
-                        for (int c = 0; c < 64; c++)
+                        for (int c = 0; c < 32; c++)
                             if (c < c0 || c >= c1) s[c] = -INFINITY;
-                        if (badpage) {
-#pragma unroll 1
-                            for (int g = 0; g < 4; g++) {
-                                const int key = kb + 16 * g;
-                                if (key < P.hi && paged_off(kv, P.b, P.j, key) < 0) {
+                        if (badpage)
 #pragma unroll
-                                    for (int c = 0; c < 64; c++)
-                                        if (c >> 4 == g) s[c] = -INFINITY;
-                                }
+                            for (int g = 0; g < 2; g++) {
+                                const int key = kb + 32 * i + 16 * g;
+                                if (key < P.hi && paged_off(kv, P.b, P.j, key) < 0)
+#pragma unroll
+                                    for (int c = 0; c < 16; c++) s[16 * g + c] = -INFINITY;
                             }
-                        }
                     }
                 };
-                // the row's largest score of the tile, from both halves
-                auto top_of = [&]() {
-                    R.x[t][h][r] = largest<64>(s, unit);
-                    pair_sync(bar);
-                    return max3(R.x[t][0][r], R.x[t][1][r], R.x[t][1][r]) - kBias;
-                };
-                // what was summed against the old m is rescaled, once its products are done
+                // O so far (once its products are done) is rescaled to another m
                 auto raise = [&](float to) {
                     const float f = ex2(m - to);
                     l *= f;
@@ -701,7 +688,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         warp_wait(&bars.odone[t], oph ^ 1);   // (of the tile before: that phase is the last one)
                         fence_after();
 #pragma unroll 1
-                        for (int c = 0; c < my_cols; c += 32) {
+                        for (int c = 0; c < hd16; c += 32) {
                             float o[32];
                             ld32(colO + c, o);
                             ld_wait(o);
@@ -711,29 +698,72 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                         st_wait();
                     }
+                    return f;
                 };
-                read();
+                float s0[32], s1[32];
                 if (it == 0 || masked) {               // (a masked tile: so that no row stays without a maximum)
-                    const float top = top_of();
+                    float top = -INFINITY;
+#pragma unroll 1
+                    for (int i = 0; i < 4; i++) {
+                        get(i, s0);
+                        have_it(i, s0);
+                        const float v = largest<32>(s0, unit);
+                        top = max3(top, v, v);
+                    }
+                    top -= kBias;
                     const bool up = real && !(top <= m + (m > kNone ? kSlack : 0.f));
                     if (__any_sync(0xffffffffu, up)) raise(up ? top : m);
                 }
+                // 32 scores at a time, the next ones' load under way; P half by half over the scores that it is made of
                 uint32_t p[TERMS][32];
-                float sum = weights<BF, TERMS>(s, unit, m, p);
-                if (pair_any(bar, real && !(sum <= kMost))) {   // (NaN: of a NaN, or of a score of +inf)
-                    read();
-                    const float top = top_of();
-                    raise(real && !(top <= m) ? top : m);
-                    sum = weights<BF, TERMS>(s, unit, m, p);
+                get(0, s0);
+                have_it(0, s0);
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    get(2 * h + 1, s1);
+                    float sum = weights<BF, TERMS>(s0, unit, m, p, 0);
+                    have_it(2 * h + 1, s1);
+                    if (h == 0) get(2, s0);
+                    sum += weights<BF, TERMS>(s1, unit, m, p, 16);
+                    if (h == 0) have_it(2, s0);
+                    if (__any_sync(0xffffffffu, real && !(sum <= kMost))) {   // (NaN: of a NaN, or of a score of +inf)
+                        // m rises by a whole number, so that what is there is rescaled exactly, the first half of P too
+                        float top = -INFINITY;
+#pragma unroll 1
+                        for (int i = 0; i < 2; i++) {
+                            get(2 * h + i, s1);
+                            have_it(2 * h + i, s1);
+                            const float v = largest<32>(s1, unit);
+                            top = max3(top, v, v);
+                        }
+                        top -= kBias;
+                        const float f = raise(!real || top <= m ? m : m > kNone ? m + ceilf(top - m) : top);
+                        if (h == 1)
+#pragma unroll
+                            for (int z = 0; z < TERMS; z++) {
+                                float o[32];
+                                ld32(colS + 32 * z, o);
+                                ld_wait(o);
+#pragma unroll
+                                for (int k = 0; k < 32; k++) o[k] = __uint_as_float(scaled<BF>(__float_as_uint(o[k]), f));
+                                st32(colS + 32 * z, reinterpret_cast<const uint32_t *>(o));
+                            }
+                        sum = weights<BF, TERMS>(s1, unit, m, p, 16);
+                        get(2 * h, s1);
+                        have_it(2 * h, s1);
+                        sum += weights<BF, TERMS>(s1, unit, m, p, 0);
+                    }
+                    l += sum;
+#pragma unroll
+                    for (int z = 0; z < TERMS; z++) st32(colS + 64 * h + 32 * z, p[z]);
                 }
-                l += sum;
                 if constexpr (TERMS == 2) {
                     if (it > 0 && it % kFlush == 0) {  // O so far to the sum in the workspace; the next products start from 0
                         warp_wait(&bars.odone[t], oph ^ 1);
                         fence_after();
                         const float f = acc ? ex2(m_acc - m) : 0.f;
 #pragma unroll 1
-                        for (int c = 0; c < my_cols; c += 16) {
+                        for (int c = 0; c < hd16; c += 16) {
                             float o[16];
                             ld16(colO + c, o);
                             ld_wait(o);
@@ -743,7 +773,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                             for (int k = 0; k < 4; k++) {
                                 const float fk = __shfl_sync(0xffffffffu, f, (lane & ~3) + k);
-                                float4 *z = reinterpret_cast<float4 *>(part + k * kTile + 64 * h + c);
+                                float4 *z = reinterpret_cast<float4 *>(part + k * kTile + c);
                                 float4 y = as_float4(x[k]);
                                 if (acc) {
                                     const float4 w = *z;
@@ -756,8 +786,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                         m_acc = m;
                     }
                 }
-#pragma unroll
-                for (int z = 0; z < TERMS; z++) st32(colS + 32 * z, p[z]);
                 st_wait();
                 fence_before();
                 __syncwarp();
@@ -775,11 +803,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
             if (run) {
-                pair_sync(bar);                        // (the last maxima have been read)
-                R.x[t][h][r] = l;
-                pair_sync(bar);
-                l = R.x[t][0][r] + R.x[t][1][r];
-                pair_sync(bar);
                 warp_wait(&bars.odone[t], oph ^ 1);
                 fence_after();
                 const float inv = whole ? inverse_sum(l) : 1.f, f = acc ? ex2(m_acc - m) : 0.f;
@@ -797,10 +820,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 const bool poison = *reinterpret_cast<volatile int *>(&R.poison) != 0;
 #pragma unroll 1
-                for (int c = 0; c < my_cols; c += 32) {
-                    const int e0 = 64 * h + c;         // elements e0 ..
+                for (int e0 = 0; e0 < hd16; e0 += 32) {
                     float o[32];
-                    ld32(colO + c, o);
+                    ld32(colO + e0, o);
                     ld_wait(o);
                     if (poison) {
                         Part Q;
@@ -856,7 +878,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     }
                 }
-                if (h == 0 && real) {
+                if (real) {
                     if (whole && a.lse) a.lse[row] = lse_of(m, l);
                     if (!whole) {
                         float *ml = chunk_part(a, worker, cur.t0 == 0) + 2 * kTile * kTile + t * kTile + r;
