@@ -60,13 +60,13 @@ constexpr uint32_t kTmemCols = 512, kColS = 0, kColO = 256;   // S (and P over i
 // has few), and m moves only when 64 weights add up to more than this; f16's largest number is 2^16.
 constexpr float kMost = 32768.f;
 constexpr float kSlack = 8.f;                       // (log2 units; where a tile is searched all the same)
-constexpr int kFlush = 4;                           // tiles whose P V the MMA adds up by itself (TERMS 2)
+constexpr int kFlush = 8;                           // tiles whose P V the MMA adds up by itself (TERMS 2)
 
 struct Bars {
     uint64_t kfull[2], kempty[2], vfull[3], vempty[3];
     uint64_t clean[4];                              // V tile i: clean[i % 4]
     uint64_t qfull, qempty;
-    uint64_t sfull[2], pfull[2], odone[2];
+    uint64_t sfull[2], pfull[2][2], odone[2][2];       // pfull, odone: by halves of the keys (TERMS 2: of the second alone)
     uint64_t drain;
 };
 
@@ -247,6 +247,9 @@ __device__ __forceinline__ void as_quads(const float *o, uint4 (&x)[4]) {
 __device__ __forceinline__ float4 as_float4(uint4 v) {
     return make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
 }
+__device__ __forceinline__ void add_at(float *p, float4 v) {
+    asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+}
 // of four neighbouring lanes: lane i's x[k] becomes what was lane k's x[i]
 __device__ __forceinline__ void turn4(uint4 (&x)[4], int lane) {
     auto swap = [&](uint4 &lo, uint4 &hi, int bit) {   // hi of the lane without the bit for lo of the one with it
@@ -263,17 +266,6 @@ __device__ __forceinline__ void turn4(uint4 (&x)[4], int lane) {
     swap(x[2], x[3], 1);
     swap(x[0], x[2], 2);
     swap(x[1], x[3], 2);
-}
-// two packed 16-bit numbers times a power of two
-template <bool BF>
-__device__ __forceinline__ uint32_t scaled(uint32_t v, float f) {
-    if constexpr (BF) {
-        const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&v));
-        return pack<true>(x.x * f, x.y * f);
-    } else {
-        const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&v));
-        return pack<false>(x.x * f, x.y * f);
-    }
 }
 __device__ __forceinline__ float not_finite(float v) { return fabsf(v) <= 3.4028234e38f ? 0.f : v; }
 
@@ -338,8 +330,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(&bars.qempty, 1);
         for (int i = 0; i < 2; i++) {
             mbar_init(&bars.sfull[i], 1);
-            mbar_init(&bars.pfull[i], kSoftmax / 2);      // (a tile's warps)
-            mbar_init(&bars.odone[i], 1);
+            mbar_init(&bars.pfull[i][0], kSoftmax / 2);   // (a tile's warps)
+            mbar_init(&bars.pfull[i][1], kSoftmax / 2);
+            mbar_init(&bars.odone[i][0], 1);
+            mbar_init(&bars.odone[i][1], 1);
         }
         mbar_init(&bars.drain, 1);
         fence_mbar_init();
@@ -476,15 +470,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                     commit(&bars.sfull[t]);
                 }
             };
-            auto values = [&](int t, uint32_t acc) {
+            // the first or second half of the keys
+            auto values = [&](int t, int h, uint32_t acc) {
                 if (leader) {
-                    const uint32_t v = dV + vslot * (kSlot / 16), p = tmem + kColS + t * kTile, d = tmem + kColO + t * kTile;
+                    const uint32_t v = dV + vslot * (kSlot / 16) + h * (4 * 2048 / 16), p = tmem + kColS + t * kTile + h * 64, d = tmem + kColO + t * kTile;
 #pragma unroll
-                    for (int i = 0; i < kTile / 16; i++)
+                    for (int i = 0; i < kTile / 32; i++)
 #pragma unroll
-                        for (int z = 0; z < TERMS; z++)
-                            mma_ts(d, p + (i >> 2) * 64 + z * 32 + (i & 3) * 8, v + i * (2048 / 16), id_o, acc | (i + z > 0));
-                    commit(&bars.odone[t]);
+                        for (int z = 0; z < TERMS; z++) mma_ts(d, p + z * 32 + i * 8, v + i * (2048 / 16), id_o, acc | (i + z > 0));
+                    commit(&bars.odone[t][h]);
                 }
             };
             auto done_k = [&](bool last) {                      // this portion's last scores: q is free too
@@ -510,11 +504,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int t = 0; t < 2; t++) {
                         if (t == 1 && !two) break;
                         const bool last = t == 1 || !two;
-                        live = warp_wait(&bars.pfull[t], pph[t]) && (t > 0 || warp_wait(&bars.clean[cslot], cph));
+                        const uint32_t acc = TERMS == 1 ? it > 0 : it % kFlush > 0;
+                        if constexpr (TERMS == 1) {            // (TERMS 2 has products enough: 367 us instead of 320 for 2048 over 4096)
+                            live = warp_wait(&bars.pfull[t][0], pph[t]) && (t > 0 || warp_wait(&bars.clean[cslot], cph));
+                            if (!live) break;
+                            fence_after();
+                            values(t, 0, acc);
+                        }
+                        live = warp_wait(&bars.pfull[t][1], pph[t]) && (TERMS == 1 || t > 0 || warp_wait(&bars.clean[cslot], cph));
                         if (!live) break;
-                        pph[t] ^= 1;
                         fence_after();
-                        values(t, TERMS == 1 ? it > 0 : it % kFlush > 0);
+                        if constexpr (TERMS == 2) values(t, 0, acc);
+                        values(t, 1, 1);
+                        pph[t] ^= 1;
                         if (leader && last) commit(&bars.vempty[vslot]);
                         if (more) {
                             if (t == 0) {
@@ -657,6 +659,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 warp_wait(&bars.sfull[t], sph);
                 sph ^= 1;
                 fence_after();
+                float s0[32], s1[32];
+                ld32(colS, s0);                        // (the first scores are on their way while it is seen what they are)
                 if (TERMS == 2 && it == 0) unit = __uint_as_float(static_cast<uint32_t>(R.unit[portion & 1][t][r]) << 23);
                 const bool badpage = *reinterpret_cast<volatile int *>(&R.badpage) != 0;
                 const bool masked = kb + kTile > tile_free_hi || kb < tile_free_lo || kb < P.lo || badpage;
@@ -679,13 +683,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                             }
                     }
                 };
-                // O so far (once its products are done) is rescaled to another m
-                auto raise = [&](float to) {
+                // O so far, the products before this tile's half h, is rescaled to another m.  (There is one product at most
+                // under way, so the phases that nobody waits for are no matter.)
+                auto raise = [&](float to, int h) {
                     const float f = ex2(m - to);
                     l *= f;
                     m = to;
-                    if (it > 0) {
-                        warp_wait(&bars.odone[t], oph ^ 1);   // (of the tile before: that phase is the last one)
+                    if (it > 0 || h > 0) {
+                        warp_wait(&bars.odone[t][h ^ 1], h ? oph : oph ^ 1);
                         fence_after();
 #pragma unroll 1
                         for (int c = 0; c < hd16; c += 32) {
@@ -698,25 +703,22 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                         st_wait();
                     }
-                    return f;
                 };
-                float s0[32], s1[32];
                 if (it == 0 || masked) {               // (a masked tile: so that no row stays without a maximum)
                     float top = -INFINITY;
 #pragma unroll 1
                     for (int i = 0; i < 4; i++) {
-                        get(i, s0);
-                        have_it(i, s0);
-                        const float v = largest<32>(s0, unit);
+                        get(i, s1);
+                        have_it(i, s1);
+                        const float v = largest<32>(s1, unit);
                         top = max3(top, v, v);
                     }
                     top -= kBias;
                     const bool up = real && !(top <= m + (m > kNone ? kSlack : 0.f));
-                    if (__any_sync(0xffffffffu, up)) raise(up ? top : m);
+                    if (__any_sync(0xffffffffu, up)) raise(up ? top : m, 0);
                 }
                 // 32 scores at a time, the next ones' load under way; P half by half over the scores that it is made of
                 uint32_t p[TERMS][32];
-                get(0, s0);
                 have_it(0, s0);
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
@@ -727,7 +729,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                     sum += weights<BF, TERMS>(s1, unit, m, p, 16);
                     if (h == 0) have_it(2, s0);
                     if (__any_sync(0xffffffffu, real && !(sum <= kMost))) {   // (NaN: of a NaN, or of a score of +inf)
-                        // m rises by a whole number, so that what is there is rescaled exactly, the first half of P too
                         float top = -INFINITY;
 #pragma unroll 1
                         for (int i = 0; i < 2; i++) {
@@ -737,17 +738,27 @@ __global__ void __launch_bounds__(kThreads, 1)
                             top = max3(top, v, v);
                         }
                         top -= kBias;
-                        const float f = raise(!real || top <= m ? m : m > kNone ? m + ceilf(top - m) : top);
-                        if (h == 1)
+                        if constexpr (TERMS == 1) {
+                            raise(!real || top <= m ? m : top, h);
+                        } else {
+                            // the first half of P is there, and not multiplied yet: m rises by a whole number, so that it is
+                            // rescaled exactly
+                            const float to = !real || top <= m ? m : m > kNone ? m + ceilf(top - m) : top, f = ex2(m - to);
+                            raise(to, 0);
+                            if (h == 1)
 #pragma unroll
-                            for (int z = 0; z < TERMS; z++) {
-                                float o[32];
-                                ld32(colS + 32 * z, o);
-                                ld_wait(o);
+                                for (int z = 0; z < TERMS; z++) {
+                                    float o[32];
+                                    ld32(colS + 32 * z, o);
+                                    ld_wait(o);
 #pragma unroll
-                                for (int k = 0; k < 32; k++) o[k] = __uint_as_float(scaled<BF>(__float_as_uint(o[k]), f));
-                                st32(colS + 32 * z, reinterpret_cast<const uint32_t *>(o));
-                            }
+                                    for (int k = 0; k < 32; k++) {
+                                        const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&o[k]));
+                                        o[k] = __uint_as_float(pack<false>(x.x * f, x.y * f));
+                                    }
+                                    st32(colS + 32 * z, reinterpret_cast<const uint32_t *>(o));
+                                }
+                        }
                         sum = weights<BF, TERMS>(s1, unit, m, p, 16);
                         get(2 * h, s1);
                         have_it(2 * h, s1);
@@ -756,40 +767,48 @@ __global__ void __launch_bounds__(kThreads, 1)
                     l += sum;
 #pragma unroll
                     for (int z = 0; z < TERMS; z++) st32(colS + 64 * h + 32 * z, p[z]);
-                }
-                if constexpr (TERMS == 2) {
-                    if (it > 0 && it % kFlush == 0) {  // O so far to the sum in the workspace; the next products start from 0
-                        warp_wait(&bars.odone[t], oph ^ 1);
-                        fence_after();
-                        const float f = acc ? ex2(m_acc - m) : 0.f;
+                    if constexpr (TERMS == 2) {
+                        if (h == 1 && it > 0 && it % kFlush == 0) {  // O so far to the sum in the workspace; the next products start from 0
+                            warp_wait(&bars.odone[t][1], oph ^ 1);
+                            fence_after();
+                            // (while m stands still the sum is added to at L2: nothing comes back that had to be waited for)
+                            const float f = acc ? ex2(m_acc - m) : 0.f;
+                            const bool add = __all_sync(0xffffffffu, f == 1.f || !real);
 #pragma unroll 1
-                        for (int c = 0; c < hd16; c += 16) {
-                            float o[16];
-                            ld16(colO + c, o);
-                            ld_wait(o);
-                            uint4 x[4];
-                            as_quads(o, x);
-                            turn4(x, lane);
+                            for (int c = 0; c < hd16; c += 16) {
+                                float o[16];
+                                ld16(colO + c, o);
+                                ld_wait(o);
+                                uint4 x[4];
+                                as_quads(o, x);
+                                turn4(x, lane);
 #pragma unroll
-                            for (int k = 0; k < 4; k++) {
-                                const float fk = __shfl_sync(0xffffffffu, f, (lane & ~3) + k);
-                                float4 *z = reinterpret_cast<float4 *>(part + k * kTile + c);
-                                float4 y = as_float4(x[k]);
-                                if (acc) {
-                                    const float4 w = *z;
-                                    y = make_float4(fmaf(w.x, fk, y.x), fmaf(w.y, fk, y.y), fmaf(w.z, fk, y.z), fmaf(w.w, fk, y.w));
+                                for (int k = 0; k < 4; k++) {
+                                    float *z = part + k * kTile + c;
+                                    float4 y = as_float4(x[k]);
+                                    if (add) {
+                                        add_at(z, y);
+                                        continue;
+                                    }
+                                    const float fk = __shfl_sync(0xffffffffu, f, (lane & ~3) + k);
+                                    if (acc) {
+                                        const float4 w = ld_cg(reinterpret_cast<const float4 *>(z));
+                                        y = make_float4(fmaf(w.x, fk, y.x), fmaf(w.y, fk, y.y), fmaf(w.z, fk, y.z), fmaf(w.w, fk, y.w));
+                                    }
+                                    *reinterpret_cast<float4 *>(z) = y;
                                 }
-                                *z = y;
                             }
+                            acc = true;
+                            m_acc = m;
                         }
-                        acc = true;
-                        m_acc = m;
+                    }
+                    if (TERMS == 1 || h == 1) {
+                        st_wait();
+                        fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&bars.pfull[t][h]);
                     }
                 }
-                st_wait();
-                fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bars.pfull[t]);
                 oph ^= 1;
             }
             // ---------------- the portion's end
@@ -803,7 +822,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
             if (run) {
-                warp_wait(&bars.odone[t], oph ^ 1);
+                warp_wait(&bars.odone[t][1], oph ^ 1);
                 fence_after();
                 const float inv = whole ? inverse_sum(l) : 1.f, f = acc ? ex2(m_acc - m) : 0.f;
                 // The results of four rows lie with four lanes, which exchange them: each store is of four lanes' 64 bytes
@@ -864,7 +883,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 if (there >> k & 1) {
                                     float4 y = as_float4(x[k]), *z = reinterpret_cast<float4 *>(part + k * kTile + e0 + 16 * g);
                                     if (TERMS == 2 && acc) {
-                                        const float4 w = *z;
+                                        const float4 w = ld_cg(z);
                                         y = make_float4(fmaf(w.x, f4[k], y.x), fmaf(w.y, f4[k], y.y), fmaf(w.z, f4[k], y.z), fmaf(w.w, f4[k], y.w));
                                     }
                                     if (!whole) {
