@@ -695,22 +695,46 @@ __global__ void __launch_bounds__(kJoinThreads) k_chunk_join(PagedChunkArgs a, i
     const int first = j.seg << a.tok_shift;
     if (r >= M || rt >= a.tile_tok || tok >= min(1 << a.tok_shift, c.n - first) || hr >= min(a.hg, a.gqa - g0)) return;
     const long long row = static_cast<long long>(c.tok0 + first + tok) * a.n_heads + kvh * a.gqa + g0 + hr;
+    // a lane per portion for maxima and sums; then the portions' rows in order, eight loads under way
+    const int n = worker - j.first + 1;
+    auto row_of = [&](int p) { return chunk_part(a, j.first + p, p == 0); };
     float top = kNone;
-    for (int w = j.first; w <= worker; w++) top = fmaxf(top, chunk_part(a, w, w == j.first)[M * pitch + r]);
-    float l = 0.f, o[8] = {};
-    for (int w = j.first; w <= worker; w++) {
-        const float *p = chunk_part(a, w, w == j.first);
-        const float f = ex2(p[M * pitch + r] - top);
-        l += p[M * pitch + M + r] * f;
+    for (int p = lane; p < n; p += 32) top = fmaxf(top, row_of(p)[M * pitch + r]);
 #pragma unroll
-        for (int k = 0; k < 8; k++)
-            if (lane + 32 * k < hd) o[k] += p[r * pitch + lane + 32 * k] * f;
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float l = 0.f;
+    float4 o[2] = {};
+    for (int p0 = 0; p0 < n; p0 += 32) {
+        float f = 0.f;
+        if (p0 + lane < n) {
+            const float *p = row_of(p0 + lane) + M * pitch + r;
+            f = ex2(p[0] - top);
+            l += p[M] * f;
+        }
+        const int here = min(32, n - p0);
+#pragma unroll
+        for (int v = 0; v < 2; v++)
+            if (128 * v < pitch) {
+                const bool in = 128 * v + 4 * lane < hd;
+#pragma unroll 8
+                for (int k = 0; k < here; k++) {
+                    const float fk = __shfl_sync(0xffffffffu, f, k);
+                    const float4 x = in ? *reinterpret_cast<const float4 *>(row_of(p0 + k) + r * pitch + 128 * v + 4 * lane)
+                                        : make_float4(0.f, 0.f, 0.f, 0.f);
+                    o[v] = make_float4(fmaf(x.x, fk, o[v].x), fmaf(x.y, fk, o[v].y), fmaf(x.z, fk, o[v].z), fmaf(x.w, fk, o[v].w));
+                }
+            }
     }
+#pragma unroll
+    for (int i = 16; i; i >>= 1) l += __shfl_xor_sync(0xffffffffu, l, i);
     const float inv = inverse_sum(l);
     TQ *out = static_cast<TQ *>(a.out) + row * hd;
 #pragma unroll
-    for (int k = 0; k < 8; k++)
-        if (lane + 32 * k < hd) out[lane + 32 * k] = from_f<TQ>(o[k] * inv);
+    for (int v = 0; v < 2; v++)
+        if (128 * v + 4 * lane < hd) {
+            st_pair(out + 128 * v + 4 * lane, o[v].x * inv, o[v].y * inv);
+            st_pair(out + 128 * v + 4 * lane + 2, o[v].z * inv, o[v].w * inv);
+        }
     if (a.lse && lane == 0) a.lse[row] = lse_of(top, l);
 }
 

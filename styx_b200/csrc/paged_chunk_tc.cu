@@ -20,10 +20,9 @@
 // added to a sum of its own in the workspace every kFlush tiles.
 //
 // Roles, linked by mbarriers with bounded waits: eight softmax warps (four per
-// query tile; with eight per tile, half of the keys each, 594 us instead of
-// @@ for a prompt of 8192), a warp that copies (TMA: boxes of min(page, 128) rows x 64
-// elements of a page, 128-byte swizzled; 16-bit q with one box per tile and 64
-// elements; f32 q is brought and split by the softmax warps), a warp that issues
+// query tile; eight, with half of the keys each, were slower), a warp that copies
+// (TMA: boxes of min(page, 128) rows x 64 elements of a page, 128-byte swizzled;
+// 16-bit q with one box per tile and 64 elements; f32 q is brought and split by the softmax warps), a warp that issues
 // the products, and two warps that go over V where a tile is not seen in whole
 // by all rows: rows outside the sequence (TMA brings whole pages) and numbers
 // that are not finite become zeros, since 0 times them would not be 0; the
@@ -60,7 +59,7 @@ constexpr uint32_t kTmemCols = 512, kColS = 0, kColO = 256;   // S (and P over i
 // has few), and m moves only when 64 weights add up to more than this; f16's largest number is 2^16.
 constexpr float kMost = 32768.f;
 constexpr float kSlack = 8.f;                       // (log2 units; where a tile is searched all the same)
-constexpr int kFlush = 8;                           // tiles whose P V the MMA adds up by itself (TERMS 2)
+constexpr int kFlush = 4;                           // tiles whose P V the MMA adds up by itself (TERMS 2)
 
 struct Bars {
     uint64_t kfull[2], kempty[2], vfull[3], vempty[3];
@@ -602,30 +601,40 @@ __global__ void __launch_bounds__(kThreads, 1)
         // brought to [2^9, 2^10)
         auto stage = [&]() {
             if (portion > 0) warp_wait(&bars.qempty, static_cast<uint32_t>((portion - 1) & 1));
-            if (t == 0 || P.two)
-                for (int i = 0; i < 32; i++) {
-                    const int row = (warp & 3) * 32 + i, tk = row / a.hg, hh = row - tk * a.hg, tok = t * a.tile_tok + tk;
-                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            // (of one tile by the warps of both)
+            const int tq = P.two ? t : 0, row0 = P.two ? (warp & 3) * 32 : warp * 16, rows = P.two ? 32 : 16;
+#pragma unroll 1
+            for (int i0 = 0; i0 < rows; i0 += 8) {     // loads first
+                float4 v[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int row = row0 + i0 + i, tk = row / a.hg, hh = row - tk * a.hg, tok = tq * a.tile_tok + tk;
+                    v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
                     if (tk < a.tile_tok && tok < P.ntok && hh < P.ng && 4 * lane < hd)
-                        v = ld_now(reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + (P.tok0 + tok) * a.q_stride +
-                                                                    static_cast<long long>(P.j * a.gqa + P.g0 + hh) * hd) + lane);
-                    v.x *= l2, v.y *= l2, v.z *= l2, v.w *= l2;
-                    const unsigned mx = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)))));
+                        v[i] = ld_now(reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + (P.tok0 + tok) * a.q_stride +
+                                                                       static_cast<long long>(P.j * a.gqa + P.g0 + hh) * hd) + lane);
+                }
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int row = row0 + i0 + i;
+                    float4 x = make_float4(v[i].x * l2, v[i].y * l2, v[i].z * l2, v[i].w * l2);
+                    const unsigned mx = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)))));
                     const int e = max(-110, min(110, static_cast<int>(mx >> 23) - 127 - 9));
                     const float up = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-                    if (lane == 0) R.unit[portion & 1][t][row] = static_cast<uint8_t>(127 + e);
-                    v.x *= up, v.y *= up, v.z *= up, v.w *= up;
+                    if (lane == 0) R.unit[portion & 1][tq][row] = static_cast<uint8_t>(127 + e);
+                    x.x *= up, x.y *= up, x.z *= up, x.w *= up;
                     uint2 hi, lo;
-                    hi.x = pack<false>(v.x, v.y);
-                    hi.y = pack<false>(v.z, v.w);
+                    hi.x = pack<false>(x.x, x.y);
+                    hi.y = pack<false>(x.z, x.w);
                     const float2 f0 = __half22float2(*reinterpret_cast<const __half2 *>(&hi.x));
                     const float2 f1 = __half22float2(*reinterpret_cast<const __half2 *>(&hi.y));
-                    lo.x = pack<false>(v.x - f0.x, v.y - f0.y);
-                    lo.y = pack<false>(v.z - f1.x, v.w - f1.y);
-                    const uint32_t at = t * kSlot + (lane >> 4) * kHalf + row * 128 + (((lane >> 1 & 7) ^ (row & 7)) << 4) + (lane & 1) * 8;
+                    lo.x = pack<false>(x.x - f0.x, x.y - f0.y);
+                    lo.y = pack<false>(x.z - f1.x, x.w - f1.y);
+                    const uint32_t at = tq * kSlot + (lane >> 4) * kHalf + row * 128 + (((lane >> 1 & 7) ^ (row & 7)) << 4) + (lane & 1) * 8;
                     *reinterpret_cast<uint2 *>(sm + at) = hi;
                     *reinterpret_cast<uint2 *>(sm + 2 * kSlot + at) = lo;
                 }
+            }
             fence_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars.qfull);
