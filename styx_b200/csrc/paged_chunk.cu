@@ -236,48 +236,54 @@ __global__ void __launch_bounds__(Mma<HD>::threads, 1) k_chunk_mma(PagedChunkArg
         __syncthreads();                               // the last portion's tiles and q have been read
         load_tile(0, 0);
         // ---------------- q as A operands, in terms: a warp per row
-        for (int i = warp; i < M; i += C::warps) {
-            int tok, head;
-            P.row(a, i, tok, head);
-            const TQ *q = static_cast<const TQ *>(a.q) + static_cast<long long>(P.tok0 + max(tok, 0)) * a.q_stride +
-                          static_cast<long long>(P.j * a.gqa + P.g0 + head) * hd;
-            uint8_t *dst = smem + i * PITCH;
-            if constexpr (TERMS == 1) {
-                for (int c = lane; c < HD / 2; c += 32) {
-                    uint32_t v = 0;
-                    if (tok >= 0 && 2 * c < hd) v = ld_now(reinterpret_cast<const uint32_t *>(q) + c);
-                    *reinterpret_cast<uint32_t *>(dst + 4 * c) = v;
-                }
-            } else {
-                float2 v[HD / 64 + (HD % 64 != 0)];
-                float mx = 0.f;
+        constexpr int NV = HD / 64 + (HD % 64 != 0), NB = HD > 128 ? 2 : 4;   // pairs of elements of a lane; rows at once: loads first
+        for (int i0 = warp * 16; i0 < warp * 16 + 16; i0 += NB) {
+            using V = std::conditional_t<TERMS == 1, uint32_t, float2>;
+            V x[NB][NV];
 #pragma unroll
-                for (int k = 0; k < HD / 64 + (HD % 64 != 0); k++) {
-                    const int c = lane + 32 * k;
-                    v[k] = make_float2(0.f, 0.f);
-                    if (tok >= 0 && 2 * c < hd) {
-                        const float2 x = ld_now(reinterpret_cast<const float2 *>(q) + c);
-                        v[k] = make_float2(x.x * l2, x.y * l2);
+            for (int i = 0; i < NB; i++) {
+                int tok, head;
+                P.row(a, i0 + i, tok, head);
+                const V *q = reinterpret_cast<const V *>(static_cast<const TQ *>(a.q) + static_cast<long long>(P.tok0 + max(tok, 0)) * a.q_stride +
+                                                         static_cast<long long>(P.j * a.gqa + P.g0 + head) * hd);
+#pragma unroll
+                for (int k = 0; k < NV; k++) {
+                    x[i][k] = V{};
+                    if (tok >= 0 && 2 * (lane + 32 * k) < hd) x[i][k] = ld_now(q + lane + 32 * k);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < NB; i++) {
+                uint8_t *dst = smem + (i0 + i) * PITCH;
+                if constexpr (TERMS == 1) {
+#pragma unroll
+                    for (int k = 0; k < NV; k++)
+                        if (2 * (lane + 32 * k) < HD) *reinterpret_cast<uint32_t *>(dst + 4 * (lane + 32 * k)) = x[i][k];
+                } else {
+                    float mx = 0.f;
+#pragma unroll
+                    for (int k = 0; k < NV; k++) {
+                        x[i][k] = make_float2(x[i][k].x * l2, x[i][k].y * l2);
+                        mx = fmaxf(mx, fmaxf(fabsf(x[i][k].x), fabsf(x[i][k].y)));
                     }
-                    mx = fmaxf(mx, fmaxf(fabsf(v[k].x), fabsf(v[k].y)));
-                }
-                float up = 1.f, down = 1.f;
-                if constexpr (!BF) {                   // the row's largest |q| is brought to [2^9, 2^10)
+                    float up = 1.f, down = 1.f;
+                    if constexpr (!BF) {               // the row's largest |q| is brought to [2^9, 2^10)
 #pragma unroll
-                    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                    const int e = max(-110, min(110, static_cast<int>(__float_as_uint(mx) >> 23) - 127 - 9));
-                    up = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-                    down = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-                }
-                if (lane == 0) s_scale[i] = down;
+                        for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                        const int e = max(-110, min(110, static_cast<int>(__float_as_uint(mx) >> 23) - 127 - 9));
+                        up = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+                        down = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+                    }
+                    if (lane == 0) s_scale[i0 + i] = down;
 #pragma unroll
-                for (int k = 0; k < HD / 64 + (HD % 64 != 0); k++) {
-                    const int c = lane + 32 * k;
-                    uint32_t t[TERMS];
-                    split2<BF, TERMS>(v[k].x * up, v[k].y * up, t);
-                    if (2 * c < HD)
+                    for (int k = 0; k < NV; k++) {
+                        const int c = lane + 32 * k;
+                        uint32_t t[TERMS];
+                        split2<BF, TERMS>(x[i][k].x * up, x[i][k].y * up, t);
+                        if (2 * c < HD)
 #pragma unroll
-                        for (int z = 0; z < TERMS; z++) *reinterpret_cast<uint32_t *>(dst + z * M * PITCH + 4 * c) = t[z];
+                            for (int z = 0; z < TERMS; z++) *reinterpret_cast<uint32_t *>(dst + z * M * PITCH + 4 * c) = t[z];
+                    }
                 }
             }
         }
@@ -376,23 +382,22 @@ __global__ void __launch_bounds__(Mma<HD>::threads, 1) k_chunk_mma(PagedChunkArg
             // ---------------- O: rows lr (+ 8), elements 8 t + 2 lc (+ 1)
             const uint32_t va = sV + stage * C::tile + (lane & 15) * PITCH + (lane >> 4) * 16;
 #pragma unroll
-            for (int t = 0; t < HD / 8; t += 2) {
-                float d[2][4] = {};
+            for (int t = 0; t < HD / 8; t += 4) {      // (four chains of products side by side)
+                float d[4][4] = {};
 #pragma unroll
                 for (int k = 0; k < KT / 16; k++) {
-                    uint32_t B[4];
-                    ldm4t(va + 16 * k * PITCH + 16 * t, B);
+                    uint32_t B[2][4];
+                    ldm4t(va + 16 * k * PITCH + 16 * t, B[0]);
+                    ldm4t(va + 16 * k * PITCH + 16 * t + 32, B[1]);
 #pragma unroll
-                    for (int z = TERMS - 1; z >= 0; z--) {
-                        mma16<BF>(d[0], pf[k][z], B[0], B[1]);
-                        mma16<BF>(d[1], pf[k][z], B[2], B[3]);
-                    }
+                    for (int z = TERMS - 1; z >= 0; z--)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) mma16<BF>(d[i], pf[k][z], B[i >> 1][2 * (i & 1)], B[i >> 1][2 * (i & 1) + 1]);
                 }
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    o[t][i] = fmaf(o[t][i], f[i >> 1], d[0][i]);
-                    o[t + 1][i] = fmaf(o[t + 1][i], f[i >> 1], d[1][i]);
-                }
+                for (int j = 0; j < 4; j++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) o[t + j][i] = fmaf(o[t + j][i], f[i >> 1], d[j][i]);
             }
             __syncthreads();
             load_tile(it + 2, stage);
@@ -459,7 +464,7 @@ __global__ void __launch_bounds__(Mma<HD>::threads, 1) k_chunk_mma(PagedChunkArg
 // ------------------------------------------------------------ f32 caches
 template <int HD>
 struct Tf {
-    static constexpr int warps = HD > 128 ? 4 : 8, threads = 32 * warps, M = 16 * warps, KT = 32;
+    static constexpr int warps = HD > 128 ? 4 : 8, threads = 32 * warps, M = 16 * warps, KT = HD > 128 ? 32 : 64;
     // floats of a row: pairs of eight rows (Q, K) on 64 different banks; rows 2 lc of eight columns (V) on 32
     static constexpr int kpitch = HD + 8, vpitch = HD + 4;
     static constexpr int smem = (M * kpitch + 2 * KT * (kpitch + vpitch)) * 4;
@@ -526,12 +531,21 @@ __global__ void __launch_bounds__(Tf<HD>::threads, 1) k_chunk_tf32(PagedChunkArg
         P.set(a, wk);
         __syncthreads();
         load_tile(0, 0);
-        for (int i = warp; i < M; i += C::warps) {
-            int tok, head;
-            P.row(a, i, tok, head);
-            const float *q = static_cast<const float *>(a.q) + static_cast<long long>(P.tok0 + max(tok, 0)) * a.q_stride +
-                             static_cast<long long>(P.j * a.gqa + P.g0 + head) * hd;
-            for (int c = lane; c < HD; c += 32) sQ[i * C::kpitch + c] = tok >= 0 && c < hd ? ld_now(q + c) * l2 : 0.f;
+        for (int i0 = warp * 16; i0 < warp * 16 + 16; i0 += 4) {   // four rows' loads first
+            float x[4][HD / 32];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                int tok, head;
+                P.row(a, i0 + i, tok, head);
+                const float *q = static_cast<const float *>(a.q) + static_cast<long long>(P.tok0 + max(tok, 0)) * a.q_stride +
+                                 static_cast<long long>(P.j * a.gqa + P.g0 + head) * hd;
+#pragma unroll
+                for (int k = 0; k < HD / 32; k++) x[i][k] = tok >= 0 && lane + 32 * k < hd ? ld_now(q + lane + 32 * k) * l2 : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int k = 0; k < HD / 32; k++) sQ[(i0 + i) * C::kpitch + lane + 32 * k] = x[i][k];
         }
         load_tile(1, 1);
         int tok[2], head[2], see_lo[2], see_hi[2];
@@ -563,14 +577,20 @@ __global__ void __launch_bounds__(Tf<HD>::threads, 1) k_chunk_tf32(PagedChunkArg
                 split_tf32(q0.y, ah[2], al[2]);
                 split_tf32(q1.y, ah[3], al[3]);
 #pragma unroll
-                for (int n = 0; n < NS; n++) {
-                    const float2 b = *reinterpret_cast<const float2 *>(ka + 8 * n * C::kpitch + 8 * k);
-                    uint32_t bh[2], bl[2];
-                    split_tf32(b.x, bh[0], bl[0]);
-                    split_tf32(b.y, bh[1], bl[1]);
-                    mma8(s[n], ah, bh[0], bh[1]);
-                    mma8(c_[n], al, bh[0], bh[1]);
-                    mma8(c_[n], ah, bl[0], bl[1]);
+                for (int n0 = 0; n0 < NS; n0 += 4) {   // (products that follow one another are of different sums)
+                    uint32_t bh[4][2], bl[4][2];
+#pragma unroll
+                    for (int n = 0; n < 4; n++) {
+                        const float2 b = *reinterpret_cast<const float2 *>(ka + 8 * (n0 + n) * C::kpitch + 8 * k);
+                        split_tf32(b.x, bh[n][0], bl[n][0]);
+                        split_tf32(b.y, bh[n][1], bl[n][1]);
+                    }
+#pragma unroll
+                    for (int n = 0; n < 4; n++) mma8(c_[n0 + n], al, bh[n][0], bh[n][1]);
+#pragma unroll
+                    for (int n = 0; n < 4; n++) mma8(s[n0 + n], ah, bh[n][0], bh[n][1]);
+#pragma unroll
+                    for (int n = 0; n < 4; n++) mma8(c_[n0 + n], ah, bl[n][0], bl[n][1]);
                 }
             }
             float top[2] = {m[0], m[1]};
@@ -611,19 +631,27 @@ __global__ void __launch_bounds__(Tf<HD>::threads, 1) k_chunk_tf32(PagedChunkArg
             }
             const float *va = sV + (stage * KT + 2 * lc) * C::vpitch + lr;
 #pragma unroll
-            for (int t = 0; t < HD / 8; t++) {
-                float d[4] = {}, e[4] = {};
+            for (int t = 0; t < HD / 8; t += 4) {
+                float d[4][4] = {}, e[4][4] = {};
 #pragma unroll
                 for (int n = 0; n < NS; n++) {
-                    uint32_t bh[2], bl[2];
-                    split_tf32(va[8 * n * C::vpitch + 8 * t], bh[0], bl[0]);
-                    split_tf32(va[(8 * n + 1) * C::vpitch + 8 * t], bh[1], bl[1]);
-                    mma8(e, pl[n], bh[0], bh[1]);
-                    mma8(e, ph[n], bl[0], bl[1]);
-                    mma8(d, ph[n], bh[0], bh[1]);
+                    uint32_t bh[4][2], bl[4][2];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        split_tf32(va[8 * n * C::vpitch + 8 * (t + j)], bh[j][0], bl[j][0]);
+                        split_tf32(va[(8 * n + 1) * C::vpitch + 8 * (t + j)], bh[j][1], bl[j][1]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; j++) mma8(e[j], pl[n], bh[j][0], bh[j][1]);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) mma8(d[j], ph[n], bh[j][0], bh[j][1]);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) mma8(e[j], ph[n], bl[j][0], bl[j][1]);
                 }
 #pragma unroll
-                for (int i = 0; i < 4; i++) o[t][i] = fmaf(o[t][i], f[i >> 1], d[i] + e[i]);
+                for (int j = 0; j < 4; j++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) o[t + j][i] = fmaf(o[t + j][i], f[i >> 1], d[j][i] + e[j][i]);
             }
             __syncthreads();
             load_tile(it + 2, stage);
@@ -741,7 +769,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_chunk_join(PagedChunkArgs a, i
 int log2_floor(int v) { return 31 - __builtin_clz(static_cast<unsigned>(v)); }
 // rows of a query tile and keys of a tile of the kernels above
 int rows_of(const PagedKv &kv) { return kv.hd > 128 ? 64 : 128; }
-int key_shift_of(const PagedKv &kv) { return kv.dtype == STYX_F32 || kv.hd > 128 ? 5 : 6; }
+int key_shift_of(const PagedKv &kv) { return kv.hd > 128 ? 5 : 6; }
 int pitch_of(const PagedKv &kv) { return kv.hd <= 64 ? 64 : kv.dtype != STYX_F32 && kv.hd <= 96 ? 96 : kv.hd <= 128 ? 128 : 256; }
 
 template <auto kern>
