@@ -130,6 +130,11 @@ struct Portion {
         if (tok >= ntok || head >= ng) tok = -1;
     }
 };
+__device__ __noinline__ Portion portion_of(const PagedChunkArgs &a, ChunkWalk w) {
+    Portion p;
+    p.set(a, w);
+    return p;
+}
 __device__ __forceinline__ long long out_row(const PagedChunkArgs &a, const Portion &P, int tok, int head) {
     return static_cast<long long>(P.tok0 + tok) * a.n_heads + P.j * a.gqa + P.g0 + head;
 }
@@ -139,15 +144,12 @@ __device__ __forceinline__ float *part_rows(const PagedChunkArgs &a, const Porti
     return chunk_part(a, worker, P.begins);
 }
 // what k_chunk_join needs to know of the worker's first portion; later ones begin their segments
-__device__ __forceinline__ void note_join(const PagedChunkArgs &a, const Portion *P, const ChunkWalk &w, int worker, long long T,
-                                          long long G) {
+__device__ __forceinline__ void note_join(const PagedChunkArgs &a, const Portion *P, const ChunkWalk &w, int worker,
+                                          const ChunkShare &s) {
     ChunkJoin j{-1, 0, 0, 0};
-    if (P && !P->begins && P->ends) j = {chunk_owner(a, w, T, G), w.b, w.head, w.seg};
+    if (P && !P->begins && P->ends) j = {chunk_owner(w, s.T, s.G), w.b, w.head, w.seg};
     static_cast<ChunkJoin *>(a.joins)[worker] = j;
 }
-// the value, where V's element is not a finite number: what a sum that has it with a positive weight becomes
-__device__ __forceinline__ float not_finite(float v) { return fabsf(v) <= 3.4028234e38f ? 0.f : v; }
-
 // ------------------------------------------------------------ 16-bit caches
 template <int HD>
 struct Mma {
@@ -159,7 +161,7 @@ struct Mma {
 };
 
 template <bool BF, int TERMS, int HD>
-__global__ void __launch_bounds__(Mma<HD>::threads, 1) k_chunk_mma(PagedChunkArgs a) {
+__global__ void __launch_bounds__(Mma<HD>::threads, 1) k_chunk_mma(const __grid_constant__ PagedChunkArgs a) {
     using C = Mma<HD>;
     using T = std::conditional_t<BF, __nv_bfloat16, __half>;
     using TQ = std::conditional_t<TERMS == 1, T, float>;
@@ -177,10 +179,9 @@ __global__ void __launch_bounds__(Mma<HD>::threads, 1) k_chunk_mma(PagedChunkArg
     const float l2 = a.scale * 1.4426950408889634f;    // scores in units of log2
     pdl_trigger();
     pdl_wait();
-    long long T_, G = 0;
-    ChunkWalk wk;
     const int worker = blockIdx.x;
-    chunk_share(a, worker, wk, T_, G);
+    const ChunkShare share = chunk_share(a, worker);
+    ChunkWalk wk = share.w;
     if (tid == 0) s_poison = s_badpage = 0;
     Portion P{};
     bool first = true;
@@ -188,6 +189,7 @@ __global__ void __launch_bounds__(Mma<HD>::threads, 1) k_chunk_mma(PagedChunkArg
     auto load_tile = [&](int it, int stage) {
         const int kb = P.kb0 + it * KT;
         if (it < P.tiles) {
+#pragma unroll 4
             for (int i = tid; i < KT * CH; i += C::threads) {
                 const int row = i / CH, c = i - row * CH, r = kb + row;
                 bool on = r >= P.lo && r < P.hi && c * 8 < hd;
@@ -212,6 +214,7 @@ __global__ void __launch_bounds__(Mma<HD>::threads, 1) k_chunk_mma(PagedChunkArg
     // V elements that are no finite numbers, in a tile that some token sees in part: 0 x them would be NaN.  They become
     // zeros, and are added to the rows that see them at the portion's end.  (Every thread looks at its own copies.)
     auto clean_tile = [&](int stage) {
+#pragma unroll 1
         for (int i = tid; i < KT * CH; i += C::threads) {
             const int row = i / CH, c = i - row * CH;
             uint4 *p = reinterpret_cast<uint4 *>(kmem + (2 + stage) * C::tile + row * PITCH + c * 16);
@@ -231,8 +234,10 @@ __global__ void __launch_bounds__(Mma<HD>::threads, 1) k_chunk_mma(PagedChunkArg
         }
     };
 
-    while (wk.next(a)) {
-        P.set(a, wk);
+    for (bool more;;) {
+        wk = chunk_next(a, wk, more);
+        if (!more) break;
+        P = portion_of(a, wk);
         __syncthreads();                               // the last portion's tiles and q have been read
         load_tile(0, 0);
         // ---------------- q as A operands, in terms: a warp per row
@@ -336,7 +341,10 @@ __global__ void __launch_bounds__(Mma<HD>::threads, 1) k_chunk_mma(PagedChunkArg
                 }
             }
             float x[NS][4], top[2] = {m[0], m[1]};
-            const bool bad = *reinterpret_cast<volatile int *>(&s_badpage) != 0;
+            uint32_t bad[KT / 32] = {};
+            if (*reinterpret_cast<volatile int *>(&s_badpage))
+#pragma unroll
+                for (int i = 0; i < KT / 32; i++) bad[i] = keys_without_page(a, P.b, kb + 32 * i, P.hi);
 #pragma unroll
             for (int n = 0; n < NS; n++)
 #pragma unroll
@@ -347,7 +355,7 @@ __global__ void __launch_bounds__(Mma<HD>::threads, 1) k_chunk_mma(PagedChunkArg
                     if (TERMS == 1 || !BF) y *= unit[i >> 1];
                     const int key = kb + 8 * n + 2 * lc + (i & 1);
                     if (partial && (key >= see_hi[i >> 1] || key < see_lo[i >> 1])) y = -INFINITY;
-                    if (bad && key < P.hi && paged_off(kv, P.b, P.j, key) < 0) y = -INFINITY;
+                    if (bad[n / 4] >> (8 * (n % 4) + 2 * lc + (i & 1)) & 1) y = -INFINITY;
                     x[n][i] = y;
                     top[i >> 1] = fmaxf(top[i >> 1], y);
                 }
@@ -412,27 +420,8 @@ __global__ void __launch_bounds__(Mma<HD>::threads, 1) k_chunk_mma(PagedChunkArg
         for (int t = 0; t < HD / 8; t++)
 #pragma unroll
             for (int i = 0; i < 4; i++) o[t][i] *= 1.f / PSCALE;
-        if (*reinterpret_cast<volatile int *>(&s_poison)) {
-            for (int it = 0; it < P.tiles; it++) {
-                const int kb = P.kb0 + it * KT;
-                if (kb + KT <= P.free_hi && kb >= P.free_lo) continue;
-                for (int key = max(kb, P.lo); key < min(kb + KT, P.hi); key++) {
-                    const long long off = paged_off(kv, P.b, P.j, key);
-                    if (off < 0) continue;
-                    const T *v = static_cast<const T *>(kv.v) + off;
-#pragma unroll
-                    for (int i = 0; i < 2; i++)
-                        if (key >= see_lo[i] && key < see_hi[i])
-#pragma unroll
-                            for (int t = 0; t < HD / 8; t++)
-#pragma unroll
-                                for (int e = 0; e < 2; e++)
-                                    if (8 * t + 2 * lc + e < hd) o[t][2 * i + e] += not_finite(to_f(v[8 * t + 2 * lc + e]));
-                }
-            }
-        }
         const bool whole = P.begins && P.ends;
-        if (first && tid == 0) note_join(a, &P, wk, worker, T_, G);
+        if (first && tid == 0) note_join(a, &P, wk, worker, share);
         first = false;
         float *part = chunk_part(a, worker, P.begins);
 #pragma unroll
@@ -456,9 +445,18 @@ __global__ void __launch_bounds__(Mma<HD>::threads, 1) k_chunk_mma(PagedChunkArg
                 }
             }
         }
+        if (*reinterpret_cast<volatile int *>(&s_poison)) {
+            __syncthreads();                           // (the results are there)
+            const int mine = tid % M;
+            int tk, hh;
+            P.row(a, mine, tk, hh);
+            if (tid < M && tk >= 0)
+                add_poison<TQ>(a, P.b, P.j, max(P.lo, a.window > 0 ? P.base + tk + 1 - a.window : 0), min(P.hi, P.base + tk + 1),
+                              whole ? static_cast<TQ *>(a.out) + out_row(a, P, tk, hh) * hd : nullptr, part + mine * HD);
+        }
     }
     copies_wait<0>();
-    if (first && tid == 0) note_join(a, nullptr, wk, worker, T_, G);
+    if (first && tid == 0) note_join(a, nullptr, wk, worker, share);
 }
 
 // ------------------------------------------------------------ f32 caches
@@ -471,7 +469,7 @@ struct Tf {
 };
 
 template <int HD>
-__global__ void __launch_bounds__(Tf<HD>::threads, 1) k_chunk_tf32(PagedChunkArgs a) {
+__global__ void __launch_bounds__(Tf<HD>::threads, 1) k_chunk_tf32(const __grid_constant__ PagedChunkArgs a) {
     using C = Tf<HD>;
     constexpr int KT = C::KT, M = C::M, NS = KT / 8, CH = HD / 4;
     extern __shared__ __align__(16) float fmem[];
@@ -483,10 +481,9 @@ __global__ void __launch_bounds__(Tf<HD>::threads, 1) k_chunk_tf32(PagedChunkArg
     const float l2 = a.scale * 1.4426950408889634f;
     pdl_trigger();
     pdl_wait();
-    long long T_, G = 0;
-    ChunkWalk wk;
     const int worker = blockIdx.x;
-    chunk_share(a, worker, wk, T_, G);
+    const ChunkShare share = chunk_share(a, worker);
+    ChunkWalk wk = share.w;
     if (tid == 0) s_poison = s_badpage = 0;
     Portion P{};
     bool first = true;
@@ -494,6 +491,7 @@ __global__ void __launch_bounds__(Tf<HD>::threads, 1) k_chunk_tf32(PagedChunkArg
     auto load_tile = [&](int it, int stage) {
         const int kb = P.kb0 + it * KT;
         if (it < P.tiles) {
+#pragma unroll 4
             for (int i = tid; i < KT * CH; i += C::threads) {
                 const int row = i / CH, c = i - row * CH, r = kb + row;
                 bool on = r >= P.lo && r < P.hi && c * 4 < hd;
@@ -515,6 +513,7 @@ __global__ void __launch_bounds__(Tf<HD>::threads, 1) k_chunk_tf32(PagedChunkArg
         copies_end();
     };
     auto clean_tile = [&](int stage) {                 // as in k_chunk_mma
+#pragma unroll 1
         for (int i = tid; i < KT * CH; i += C::threads) {
             const int row = i / CH, c = i - row * CH;
             float *p = sV + (stage * KT + row) * C::vpitch + c * 4;
@@ -527,8 +526,10 @@ __global__ void __launch_bounds__(Tf<HD>::threads, 1) k_chunk_tf32(PagedChunkArg
         }
     };
 
-    while (wk.next(a)) {
-        P.set(a, wk);
+    for (bool more;;) {
+        wk = chunk_next(a, wk, more);
+        if (!more) break;
+        P = portion_of(a, wk);
         __syncthreads();
         load_tile(0, 0);
         for (int i0 = warp * 16; i0 < warp * 16 + 16; i0 += 4) {   // four rows' loads first
@@ -594,7 +595,10 @@ __global__ void __launch_bounds__(Tf<HD>::threads, 1) k_chunk_tf32(PagedChunkArg
                 }
             }
             float top[2] = {m[0], m[1]};
-            const bool bad = *reinterpret_cast<volatile int *>(&s_badpage) != 0;
+            uint32_t bad[KT / 32] = {};
+            if (*reinterpret_cast<volatile int *>(&s_badpage))
+#pragma unroll
+                for (int i = 0; i < KT / 32; i++) bad[i] = keys_without_page(a, P.b, kb + 32 * i, P.hi);
 #pragma unroll
             for (int n = 0; n < NS; n++)
 #pragma unroll
@@ -602,7 +606,7 @@ __global__ void __launch_bounds__(Tf<HD>::threads, 1) k_chunk_tf32(PagedChunkArg
                     float y = s[n][i] + c_[n][i];
                     const int key = kb + 8 * n + 2 * lc + (i & 1);
                     if (partial && (key >= see_hi[i >> 1] || key < see_lo[i >> 1])) y = -INFINITY;
-                    if (bad && key < P.hi && paged_off(kv, P.b, P.j, key) < 0) y = -INFINITY;
+                    if (bad[n / 4] >> (8 * (n % 4) + 2 * lc + (i & 1)) & 1) y = -INFINITY;
                     s[n][i] = y;
                     top[i >> 1] = fmaxf(top[i >> 1], y);
                 }
@@ -661,27 +665,8 @@ __global__ void __launch_bounds__(Tf<HD>::threads, 1) k_chunk_tf32(PagedChunkArg
             l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
             l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
         }
-        if (*reinterpret_cast<volatile int *>(&s_poison)) {
-            for (int it = 0; it < P.tiles; it++) {
-                const int kb = P.kb0 + it * KT;
-                if (kb + KT <= P.free_hi && kb >= P.free_lo) continue;
-                for (int key = max(kb, P.lo); key < min(kb + KT, P.hi); key++) {
-                    const long long off = paged_off(kv, P.b, P.j, key);
-                    if (off < 0) continue;
-                    const float *v = static_cast<const float *>(kv.v) + off;
-#pragma unroll
-                    for (int i = 0; i < 2; i++)
-                        if (key >= see_lo[i] && key < see_hi[i])
-#pragma unroll
-                            for (int t = 0; t < HD / 8; t++)
-#pragma unroll
-                                for (int e = 0; e < 2; e++)
-                                    if (8 * t + 2 * lc + e < hd) o[t][2 * i + e] += not_finite(v[8 * t + 2 * lc + e]);
-                }
-            }
-        }
         const bool whole = P.begins && P.ends;
-        if (first && tid == 0) note_join(a, &P, wk, worker, T_, G);
+        if (first && tid == 0) note_join(a, &P, wk, worker, share);
         first = false;
         float *part = chunk_part(a, worker, P.begins);
 #pragma unroll
@@ -700,9 +685,18 @@ __global__ void __launch_bounds__(Tf<HD>::threads, 1) k_chunk_tf32(PagedChunkArg
                 part[M * HD + M + r] = l[i];
             }
         }
+        if (*reinterpret_cast<volatile int *>(&s_poison)) {
+            __syncthreads();                           // (the results are there)
+            const int mine = tid % M;
+            int tk, hh;
+            P.row(a, mine, tk, hh);
+            if (tid < M && tk >= 0)
+                add_poison<float>(a, P.b, P.j, max(P.lo, a.window > 0 ? P.base + tk + 1 - a.window : 0), min(P.hi, P.base + tk + 1),
+                              whole ? static_cast<float *>(a.out) + out_row(a, P, tk, hh) * hd : nullptr, part + mine * HD);
+        }
     }
     copies_wait<0>();
-    if (first && tid == 0) note_join(a, nullptr, wk, worker, T_, G);
+    if (first && tid == 0) note_join(a, nullptr, wk, worker, share);
 }
 
 // ------------------------------------------------------------ joining

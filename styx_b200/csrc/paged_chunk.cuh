@@ -109,8 +109,21 @@ struct ChunkWalk {
     }
 };
 
-// Worker i's share of T units in G parts: [floor(i T / G), floor((i + 1) T / G)).  All lanes of a warp together.
-__device__ __forceinline__ void chunk_share(const PagedChunkArgs &a, int worker, ChunkWalk &w, long long &T, long long &G) {
+// the walk's next step, out of line (not for kernels whose roles have registers of their own: the compiler gives up)
+__device__ __noinline__ ChunkWalk chunk_next(const PagedChunkArgs &a, ChunkWalk w, bool &more) {
+    more = w.next(a);
+    return w;
+}
+
+// Worker i's share of T units in G parts: [floor(i T / G), floor((i + 1) T / G)).  All lanes of a warp together.  (Out of
+// line, as what is done once a portion or less is: code that does not fit the instruction caches costs more than a call.)
+struct ChunkShare {
+    ChunkWalk w;
+    long long T, G;
+};
+__device__ __noinline__ ChunkShare chunk_share(const PagedChunkArgs &a, int worker) {
+    ChunkShare s{};
+    ChunkWalk &w = s.w;
     const int lane = threadIdx.x & 31, n = a.kv.n_seqs;
     const int per = (n + 31) / 32, lo = min(n, lane * per), hi = min(n, lo + per);
     const bool report = blockIdx.x == 0 && threadIdx.x < 32;
@@ -119,6 +132,7 @@ __device__ __forceinline__ void chunk_share(const PagedChunkArgs &a, int worker,
         return c.upto(a, c.segs(a)) * a.heads;
     };
     long long mine = 0;
+#pragma unroll 1
     for (int b = lo; b < hi; b++) mine += units(b, report);
     long long upto = mine;
 #pragma unroll
@@ -126,19 +140,21 @@ __device__ __forceinline__ void chunk_share(const PagedChunkArgs &a, int worker,
         const long long u = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += u;
     }
-    T = __shfl_sync(0xffffffffu, upto, 31);
-    w.b = w.head = w.seg = w.u = w.nt = w.t0 = w.t1 = 0;
-    w.at = w.end = 0;
-    if (T == 0) return;
-    G = min(static_cast<long long>(a.workers), T);
-    if (worker >= G) return;
-    const long long at = T / G * worker + T % G * worker / G;
-    w.end = T / G * (worker + 1) + T % G * (worker + 1) / G;
+    const long long T = s.T = __shfl_sync(0xffffffffu, upto, 31);
+    if (T == 0) return s;
+    const long long G = s.G = min(static_cast<long long>(a.workers), T);
+    if (worker >= G) return s;
+    // (32-bit divisions where the numbers allow it: a 64-bit one is some 300 clocks)
+    const bool small = T < (1ll << 31);
+    const long long each = small ? static_cast<unsigned>(T) / static_cast<unsigned>(G) : T / G, rest = T - each * G;
+    const long long at = each * worker + static_cast<unsigned>(rest * worker) / static_cast<unsigned>(G);
+    w.end = each * (worker + 1) + static_cast<unsigned>(rest * (worker + 1)) / static_cast<unsigned>(G);
     w.at = at;
     const int src = __ffs(__ballot_sync(0xffffffffu, at < upto)) - 1;   // (at < T, so there is one)
     long long off = at - (upto - mine);
     int b = lo;
     if (lane == src)
+#pragma unroll 1
         for (; b < hi - 1; b++) {
             const long long nb = units(b, false);
             if (off < nb) break;
@@ -149,9 +165,11 @@ __device__ __forceinline__ void chunk_share(const PagedChunkArgs &a, int worker,
     const Chunk c(a, w.b, false);
     const int ns = c.segs(a);
     const long long head_units = max(1ll, c.upto(a, ns));
-    w.head = static_cast<int>(min(off / head_units, static_cast<long long>(a.heads - 1)));
+    w.head = static_cast<int>(min(small ? static_cast<long long>(static_cast<unsigned>(off) / static_cast<unsigned>(head_units)) : off / head_units,
+                                  static_cast<long long>(a.heads - 1)));
     off -= w.head * head_units;
     int s0 = 0, s1 = max(0, ns - 1);             // the last segment with upto(s) <= off
+#pragma unroll 1
     while (s0 < s1) {
         const int mid = (s0 + s1 + 1) >> 1;
         if (c.upto(a, mid) <= off) s0 = mid;
@@ -160,15 +178,16 @@ __device__ __forceinline__ void chunk_share(const PagedChunkArgs &a, int worker,
     w.seg = s0;
     w.nt = c.tiles(a, s0);
     w.u = static_cast<int>(min(off - c.upto(a, s0), static_cast<long long>(a.seg_cost + w.nt)));
+    return s;
 }
 
 // the first worker with a tile of the segment in which the walk's portion (its worker's, up to w.at) has the last one
-__device__ __forceinline__ int chunk_owner(const PagedChunkArgs &a, const ChunkWalk &w, long long T, long long G) {
+__device__ __noinline__ int chunk_owner(ChunkWalk w, long long T, long long G) {
     const long long first = w.at - w.nt;         // the segment's first tile, as a unit of the list
-    long long i = (first + 1) * G;               // (both below 2^31 x 2^16 or so)
-    i = (i - 1) / T;
+    const long long each = T / G, rest = T - each * G;
     // floor(i T / G) <= first < floor((i + 1) T / G), for the shares as they are computed above
-    auto share = [&](long long k) { return T / G * k + T % G * k / G; };
+    auto share = [&](long long k) { return each * k + static_cast<unsigned>(rest * k) / static_cast<unsigned>(G); };
+    long long i = ((first + 1) * G - 1) / T;     // (T below 2^47 or so, G below 2^16)
     while (i > 0 && share(i) > first) i--;
     while (share(i + 1) <= first) i++;
     return static_cast<int>(i);
@@ -182,6 +201,35 @@ struct ChunkJoin {
 // O is [rows][pitch], then a maximum (in units of log2) and a sum for every row.
 __device__ __forceinline__ float *chunk_part(const PagedChunkArgs &a, int worker, bool begins) {
     return a.part + (2ll * worker + (begins ? 1 : 0)) * a.part_floats;
+}
+
+// 0, or the value where it is not a finite number
+__device__ __forceinline__ float not_finite(float v) { return fabsf(v) <= 3.4028234e38f ? 0.f : v; }
+// of the 32 keys from key on, those in pages outside the pool
+__device__ __noinline__ uint32_t keys_without_page(const PagedChunkArgs &a, int b, int key, int hi) {
+    uint32_t bad = 0;
+    for (int i = 0; i < 32 && key + i < hi; i++)
+        if (paged_off(a.kv, b, 0, key + i) < 0) bad |= 1u << i;
+    return bad;
+}
+// Numbers of V that are not finite are left out of the products of tiles that are not seen in whole, and then added to the
+// query rows that see them, here: a row that sees the keys [lo, hi) of kv head j, TO's at `out`, or f32 at `part`.  (Adding
+// once more what other tiles have brought changes nothing.)
+template <class TO>
+__device__ __noinline__ void add_poison(const PagedChunkArgs &a, int b, int j, int lo, int hi, TO *out, float *part) {
+    const int hd = a.kv.hd;
+    for (int key = lo; key < hi; key++) {
+        const long long off = paged_off(a.kv, b, j, key);
+        if (off < 0) continue;
+        for (int e = 0; e < hd; e++) {
+            const float v = not_finite(a.kv.dtype == STYX_F32    ? static_cast<const float *>(a.kv.v)[off + e]
+                                       : a.kv.dtype == STYX_BF16 ? to_f(static_cast<const __nv_bfloat16 *>(a.kv.v)[off + e])
+                                                                 : to_f(static_cast<const __half *>(a.kv.v)[off + e]));
+            if (v == 0.f) continue;
+            if (out) out[e] = from_f<TO>(to_f(out[e]) + v);
+            else part[e] += v;
+        }
+    }
 }
 
 template <class T>

@@ -266,7 +266,6 @@ __device__ __forceinline__ void turn4(uint4 (&x)[4], int lane) {
     swap(x[0], x[2], 2);
     swap(x[1], x[3], 2);
 }
-__device__ __forceinline__ float not_finite(float v) { return fabsf(v) <= 3.4028234e38f ? 0.f : v; }
 
 // a portion: its segment's tokens and heads, its keys [lo, hi)
 struct Part {
@@ -298,7 +297,7 @@ struct Part {
 
 template <bool BF, int TERMS>
 __global__ void __launch_bounds__(kThreads, 1)
-    k_chunk_tc(PagedChunkArgs a, const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+    k_chunk_tc(const __grid_constant__ PagedChunkArgs a, const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                const __grid_constant__ CUtensorMap mv) {
     using T = std::conditional_t<BF, __nv_bfloat16, __half>;
     constexpr int RK = Ring<TERMS>::k, RV = Ring<TERMS>::v;
@@ -354,10 +353,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     fence_after();
     pdl_trigger();
     const uint32_t tmem = R.tmem;
-    long long T_ = 0, G = 0;
-    ChunkWalk wk;
     const int worker = blockIdx.x;
-    chunk_share(a, worker, wk, T_, G);
+    const ChunkShare share = chunk_share(a, worker);
+    ChunkWalk wk = share.w;
     Part P;
 
     auto wait = [&](uint64_t *bar, uint32_t parity) {
@@ -642,7 +640,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool have = wk.next(a);
         if (tid == 0) {                               // (later portions begin their segments)
             ChunkJoin j{-1, 0, 0, 0};
-            if (have && wk.t0 > 0 && wk.t1 == wk.nt) j = {chunk_owner(a, wk, T_, G), wk.b, wk.head, wk.seg};
+            if (have && wk.t0 > 0 && wk.t1 == wk.nt) j = {chunk_owner(wk, share.T, share.G), wk.b, wk.head, wk.seg};
             static_cast<ChunkJoin *>(a.joins)[worker] = j;
         }
         if (have) {
@@ -678,18 +676,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 auto have_it = [&](int i, float (&s)[32]) {
                     ld_wait(s);
                     if (masked) {
-                        const int c0 = see_lo - kb - 32 * i, c1 = see_hi - kb - 32 * i;
+                        const int c0 = max(0, min(32, see_lo - kb - 32 * i)), c1 = max(c0, min(32, see_hi - kb - 32 * i));
+                        uint32_t seen = static_cast<uint32_t>((1ull << c1) - (1ull << c0));
+                        if (badpage) {                 // (pages have 16 rows at least)
+                            if ((seen & 0xFFFFu) && paged_off(kv, P.b, P.j, kb + 32 * i) < 0) seen &= 0xFFFF0000u;
+                            if ((seen >> 16) && paged_off(kv, P.b, P.j, kb + 32 * i + 16) < 0) seen &= 0xFFFFu;
+                        }
 #pragma unroll
-                        for (int c = 0; c < 32; c++)
-                            if (c < c0 || c >= c1) s[c] = -INFINITY;
-                        if (badpage)
-#pragma unroll
-                            for (int g = 0; g < 2; g++) {
-                                const int key = kb + 32 * i + 16 * g;
-                                if (key < P.hi && paged_off(kv, P.b, P.j, key) < 0)
-#pragma unroll
-                                    for (int c = 0; c < 16; c++) s[16 * g + c] = -INFINITY;
-                            }
+                        for (int c = 0; c < 32; c++) s[c] = seen >> c & 1 ? s[c] : -INFINITY;
                     }
                 };
                 // O so far, the products before this tile's half h, is rescaled to another m.  (There is one product at most
@@ -846,29 +840,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                     f4[k] = __shfl_sync(0xffffffffu, f, (lane & ~3) + k);
                     there |= static_cast<unsigned>(__shfl_sync(0xffffffffu, static_cast<int>(real), (lane & ~3) + k)) << k;
                 }
-                const bool poison = *reinterpret_cast<volatile int *>(&R.poison) != 0;
 #pragma unroll 1
                 for (int e0 = 0; e0 < hd16; e0 += 32) {
                     float o[32];
                     ld32(colO + e0, o);
                     ld_wait(o);
-                    if (poison) {
-                        Part Q;
-                        Q.set(a, cur);
-                        for (int it = 0; real && it < Q.tiles; it++) {
-                            const int kb = Q.kb0 + it * kTile;
-                            if (!Q.partial(kb)) continue;
-                            for (int key = max(kb, see_lo); key < min(kb + kTile, see_hi); key++) {
-                                const long long off = paged_off(kv, Q.b, Q.j, key);
-                                if (off < 0) continue;
-                                const T *v = static_cast<const T *>(kv.v) + off + e0;
-#pragma unroll
-                                for (int k = 0; k < 32; k++)
-                                    if (e0 + k < hd) o[k] += not_finite(to_f(v[k]));
-                            }
-                        }
-                        __syncwarp();
-                    }
                     if (TERMS == 1 && whole) {
                         uint4 x[4];
 #pragma unroll
@@ -905,6 +881,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 }
                         }
                     }
+                }
+                if (*reinterpret_cast<volatile int *>(&R.poison)) {
+                    __syncwarp();                      // (its rows were written by four lanes each)
+                    using TO = std::conditional_t<TERMS == 1, T, float>;
+                    if (real)
+                        add_poison<TO>(a, cur.b, cur.head / a.groups, see_lo, see_hi, whole ? static_cast<TO *>(a.out) + row * hd : nullptr,
+                                       chunk_part(a, worker, cur.t0 == 0) + (t * kTile + r) * kTile);
                 }
                 if (real) {
                     if (whole && a.lse) a.lse[row] = lse_of(m, l);
