@@ -411,7 +411,7 @@ struct PagedPlanArgs {
     int32_t *start, *seq, *row, *pos, *lens_out, *held_out, *n_free_out, *next_pos_out;
     long long table_stride;
     int n_seqs, max_pages, page_shift, n_pages, n_tokens;
-    int own_maps;                              // the planning kernel writes seq, row and pos itself
+    int own_maps, vec;                         // the planning kernel writes seq, row and pos itself; they are 16-byte aligned
     int *err;
 };
 // what append_rope takes beside PagedAppendArgs (whose log2_base, step and q_out are not used)
@@ -477,7 +477,7 @@ cudaError_t launch_paged_append_rope(const PagedAppendArgs &a, const PagedRope &
 // M rows, query tiles of `tile` rows, joined
 cudaError_t launch_chunk_mma(PagedChunkArgs a, int sms, cudaStream_t st);
 uint64_t chunk_mma_parts(const PagedKv &kv, int sms);
-bool chunk_on_tc(const PagedChunkArgs &a);
+bool chunk_on_tc(const PagedChunkArgs &a);      // (kv, q16, scale, n_tokens and gqa are set)
 cudaError_t launch_chunk_tc(PagedChunkArgs a, int sms, cudaStream_t st);
 uint64_t chunk_tc_parts(int sms);
 cudaError_t launch_chunk_join(const PagedChunkArgs &a, int M, int tile, int pitch, cudaStream_t st);

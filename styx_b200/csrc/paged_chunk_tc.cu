@@ -946,9 +946,13 @@ cudaError_t go(const PagedChunkArgs &a, const CUtensorMap &mq, const CUtensorMap
 }  // namespace
 
 // A page's rows and a tile's queries have to be boxes (rows of 128 bytes and more, 16 rows and more).  Scores are
-// compared before they are scaled, so the scale is positive.
+// compared before they are scaled, so the scale is positive.  A few queries over a short cache take as long as the kernel
+// takes to begin, and k_chunk_mma begins sooner (5 tokens of 32 / 4 heads over 37 rows, f32 over f16: 12.7 us, here 15.8;
+// over 300 rows of f16 15.7 and 16.7); beyond, this one is faster (16 sequences of 20 tokens over 500 rows 28 us, there 44).
 bool chunk_on_tc(const PagedChunkArgs &a) {
-    return (a.q16 || a.kv.dtype == STYX_F16) && a.kv.hd >= 64 && a.kv.hd <= 128 && a.kv.page_shift >= 4 && a.scale > 0.f && encode_fn();
+    const bool few = static_cast<long long>(a.n_tokens) * a.gqa <= kTile && (static_cast<long long>(a.kv.max_pages) << a.kv.page_shift) <= 512;
+    return (a.q16 || a.kv.dtype == STYX_F16) && a.kv.hd >= 64 && a.kv.hd <= 128 && a.kv.page_shift >= 4 && a.scale > 0.f && !few &&
+           encode_fn();
 }
 uint64_t chunk_tc_parts(int sms) { return 2ull * sms * 2 * kTile * (kTile + 2) * 4; }
 

@@ -22,11 +22,12 @@
 namespace styx {
 namespace {
 
-constexpr int kThreads = 1024, kWarps = kThreads / 32;
-constexpr int kOwnTokens = 4096;   // tokens whose places the planning CTA writes itself
+constexpr int kOwnTokens = 8192;   // tokens whose places the planning CTA writes itself
 constexpr int kMapThreads = 256, kMapTokens = 1024;
 
-__device__ __forceinline__ long long scan(long long v, long long *sh, long long &total) {   // inclusive, over the CTA
+template <int N>
+__device__ __forceinline__ long long scan(long long v, long long *sh, long long &total) {   // inclusive, over the CTA's N threads
+    constexpr int kWarps = N / 32;
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -36,13 +37,13 @@ __device__ __forceinline__ long long scan(long long v, long long *sh, long long 
     __syncthreads();
     if (lane == 31) sh[w] = v;
     __syncthreads();
-    long long x = sh[lane];
+    long long x = lane < kWarps ? sh[lane] : 0;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
+    for (int o = 1; o < kWarps; o <<= 1) {
         const long long u = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += u;
     }
-    total = __shfl_sync(0xffffffffu, x, 31);
+    total = __shfl_sync(0xffffffffu, x, kWarps - 1);
     const long long before = __shfl_sync(0xffffffffu, x, w ? w - 1 : 0);
     return v + (w ? before : 0);
 }
@@ -64,8 +65,11 @@ struct Row {                 // one sequence of the tile
     bool ok;
 };
 
-__global__ void __launch_bounds__(kThreads, 1) k_paged_plan(PagedPlanArgs a) {
-    __shared__ long long sh[kWarps];
+// N threads: 1024, or 256 where sequences and tokens are few (its barriers cost less)
+template <int N>
+__global__ void __launch_bounds__(N, 1) k_paged_plan(PagedPlanArgs a) {
+    constexpr int kThreads = N;
+    __shared__ long long sh[N / 32];
     __shared__ int s_sum[kThreads], s_from[kThreads], s_pos[kThreads];   // of the tile: inclusive sums, and what they start from
     pdl_trigger();
     pdl_wait();
@@ -90,7 +94,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_plan(PagedPlanArgs a) {
             else w = min(static_cast<long long>(max(0, ld_now(a.want + b))), most - r.lens);
         }
         long long total;
-        const long long before = tokens + scan(w, sh, total) - w;
+        const long long before = tokens + scan<N>(w, sh, total) - w;
         tokens += total;
         r.t = static_cast<int>(min(w, max(0ll, a.n_tokens - before)));
         r.target = r.ok ? static_cast<int>((static_cast<long long>(r.lens) + r.t + (1 << a.page_shift) - 1) >> a.page_shift) : r.held;
@@ -104,7 +108,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_plan(PagedPlanArgs a) {
         r = load(b0 + tid);
         const int back = max(0, r.held - r.target);
         long long total;
-        const long long upto = scan(back, sh, total);
+        const long long upto = scan<N>(back, sh, total);
         if (total) {
             // (of one tile at most 1024 x max_pages: below 2^31 only where pages are few, so by their number cut off)
             const int n = static_cast<int>(min(total, a.n_pages - top));
@@ -128,7 +132,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_plan(PagedPlanArgs a) {
         if (!one) r = load(b);
         const long long need = max(0, r.target - r.held);
         long long total;
-        const long long before = needed + scan(need, sh, total) - need;
+        const long long before = needed + scan<N>(need, sh, total) - need;
         needed += total;
         const int got = static_cast<int>(min(need, max(0ll, top - before)));
         // the tile's pages are numbers first, first + 1, ... from the stack's top
@@ -145,7 +149,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_plan(PagedPlanArgs a) {
         }
         const int held = min(r.held, r.target) + got;
         const int granted = r.ok ? static_cast<int>(max(0ll, min(static_cast<long long>(r.t), (static_cast<long long>(held) << a.page_shift) - r.lens))) : 0;
-        const long long upto = given + scan(granted, sh, total);   // (its barriers end the loop above)
+        const long long upto = given + scan<N>(granted, sh, total);   // (its barriers end the loop above)
         if (b < a.n_seqs) {
             const int pos = a.next_pos ? ld_now(a.next_pos + b) : r.lens;
             a.lens_out[b] = r.lens + granted;
@@ -158,11 +162,34 @@ __global__ void __launch_bounds__(kThreads, 1) k_paged_plan(PagedPlanArgs a) {
             s_sum[tid] = static_cast<int>(upto - given);
             s_from[tid] = r.lens;
             __syncthreads();
-            for (int i = tid; i < total; i += kThreads) {
-                const int q = first_above(s_sum, kThreads, i), nth = i - (q ? s_sum[q - 1] : 0);
-                a.seq[given + i] = b0 + q;
-                a.row[given + i] = s_from[q] + nth;
-                a.pos[given + i] = s_pos[q] + nth;
+            // four neighbouring tokens a thread, one search; whole groups as 16 bytes each
+            const long long end = given + total;
+            for (long long x = (given & ~3ll) + 4 * tid; x < end; x += 4 * kThreads) {
+                int q = first_above(s_sum, kThreads, max(x, given) - given);
+                int4 seq, row, pos;
+                int *const v[3] = {&seq.x, &row.x, &pos.x};
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int i = static_cast<int>(x + e - given);
+                    if (i < 0 || x + e >= end) continue;
+                    while (i >= s_sum[q]) q++;
+                    const int nth = i - (q ? s_sum[q - 1] : 0);
+                    v[0][e] = b0 + q;
+                    v[1][e] = s_from[q] + nth;
+                    v[2][e] = s_pos[q] + nth;
+                }
+                if (a.vec && x >= given && x + 4 <= end) {
+                    *reinterpret_cast<int4 *>(a.seq + x) = seq;
+                    *reinterpret_cast<int4 *>(a.row + x) = row;
+                    *reinterpret_cast<int4 *>(a.pos + x) = pos;
+                } else {
+                    for (int e = 0; e < 4; e++)
+                        if (x + e >= given && x + e < end) {
+                            a.seq[x + e] = v[0][e];
+                            a.row[x + e] = v[1][e];
+                            a.pos[x + e] = v[2][e];
+                        }
+                }
             }
         }
         given += total;
@@ -209,7 +236,10 @@ __global__ void __launch_bounds__(kMapThreads) k_paged_maps(PagedPlanArgs a) {
 
 cudaError_t launch_paged_plan(PagedPlanArgs a, cudaStream_t st) {
     a.own_maps = a.n_tokens <= kOwnTokens;
-    cudaError_t e = launch_pdl(k_paged_plan, dim3(1), dim3(kThreads), 0, st, a);
+    a.vec = ((reinterpret_cast<uintptr_t>(a.seq) | reinterpret_cast<uintptr_t>(a.row) | reinterpret_cast<uintptr_t>(a.pos)) & 15) == 0;
+    const bool few = a.n_seqs <= 256 && a.n_tokens <= 1024;
+    cudaError_t e = few ? launch_pdl(k_paged_plan<256>, dim3(1), dim3(256), 0, st, a)
+                        : launch_pdl(k_paged_plan<1024>, dim3(1), dim3(1024), 0, st, a);
     if (e != cudaSuccess || a.own_maps) return e;
     return launch_pdl(k_paged_maps, dim3((a.n_tokens + kMapTokens - 1) / kMapTokens), dim3(kMapThreads), 0, st, a);
 }

@@ -94,13 +94,7 @@ __global__ void __launch_bounds__(kThreads, 8) k_paged_append_rope(PagedAppendAr
     };
     pdl_wait();
     // (the frequencies and the norms may be an earlier kernel's)
-    double turn[4];
-    bool turned[4];
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-        turned[e] = p0 + e < n / 2;
-        turn[e] = turned[e] ? ld_now(rope.freq + p0 + e) * 0.15915494309189535 : 0.0;   // 1 / 2 pi
-    }
+    const int nt = max(0, min(4, n / 2 - p0));         // how many of the lane's pairs are turned
     float wq[2][4], wk[2][4];
 #pragma unroll
     for (int e = 0; e < 4; e++) wq[0][e] = wq[1][e] = wk[0][e] = wk[1][e] = 1.f;
@@ -143,7 +137,8 @@ __global__ void __launch_bounds__(kThreads, 8) k_paged_append_rope(PagedAppendAr
         float c[4], s[4];
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const double f = pos * turn[e];
+            // (read for every token: in registers all along they cost the occupancy that hides the loads)
+            const double f = e < nt ? pos * (ld_now(rope.freq + p0 + e) * 0.15915494309189535) : 0.0;   // 1 / 2 pi
             sincospif(static_cast<float>(2.0 * (f - rint(f))), &s[e], &c[e]);
             c[e] *= rope.magnitude;
             s[e] *= rope.magnitude;
@@ -170,7 +165,7 @@ __global__ void __launch_bounds__(kThreads, 8) k_paged_append_rope(PagedAppendAr
                 float p[4], q[4];
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const bool as_is = is_v || !turned[e];   // (0 x a NaN of the other element would be one too)
+                    const bool as_is = is_v || e >= nt;   // (0 x a NaN of the other element would be one too)
                     p[e] = as_is ? x[j][e] : x[j][e] * c[e] - y[j][e] * s[e];
                     q[e] = as_is ? y[j][e] : x[j][e] * s[e] + y[j][e] * c[e];
                     if (r < 0) p[e] = q[e] = 0.f;          // padding, or an empty slot
