@@ -96,3 +96,13 @@ def test_plan_definition():
     assert start.tolist() == [0, 2, 2, 7] and row.tolist() == [3, 4, 1, 2, 3, 4, 5, -1]
     assert t.table[0, 2] == ids[1, 0] and t.table[2, 1:3].tolist() == stack[::-1] and t.n_free == 0
     assert t.lens == [5, 0, 6] and t.held == [3, 0, 3] and pos.tolist()[:3] == [3, 4, 15] and seq.tolist() == [0, 0, 2, 2, 2, 2, 2, 0]
+
+
+def test_batch_decoder_refuses_chunks_it_cannot_have():
+    from styx_b200.decode import DecodeParams
+    from styx_b200.serve import BatchDecoder
+    hp = DecodeParams(1, 512, 8, 2, 64, 256, 16, 4, 1024)
+    with pytest.raises(ValueError, match="chunks"):
+        BatchDecoder(hp, None, [], None, None, 4, 64, chunk=-1)
+    with pytest.raises(ValueError, match="budget"):
+        BatchDecoder(hp, None, [], None, None, 4, 64, chunk=8, budget=32, n_recent=8, n_sink=4)
