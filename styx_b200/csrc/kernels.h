@@ -434,6 +434,7 @@ struct PagedChunkArgs {
     int hg, groups, heads;                     // heads of a tile; groups of a kv head; kv heads x groups
     int tile_tok;                              // tokens of a query tile
     int tok_shift, key_shift, seg_cost, workers, part_floats;
+    int whole;                                 // segments are not cut: each counts one unit
     float *part;                               // workspace
     void *joins;                               // workspace, one ChunkJoin per worker
 };
@@ -480,6 +481,7 @@ uint64_t chunk_mma_parts(const PagedKv &kv, int sms);
 bool chunk_on_tc(const PagedChunkArgs &a);      // (kv, q16, scale, n_tokens and gqa are set)
 cudaError_t launch_chunk_tc(PagedChunkArgs a, int sms, cudaStream_t st);
 uint64_t chunk_tc_parts(int sms);
+bool chunk_whole(const PagedChunkArgs &a, int sms, double tile_ns);
 cudaError_t launch_chunk_join(const PagedChunkArgs &a, int M, int tile, int pitch, cudaStream_t st);
 cudaError_t launch_paged_evict(const PagedEvictArgs &a, int sms, cudaStream_t st);
 bool evict_staged(long long rows);   // the keys of lines of so many rows fit shared memory

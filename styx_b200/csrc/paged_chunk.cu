@@ -19,6 +19,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
 #include <type_traits>
 
@@ -114,9 +115,10 @@ struct Portion {
         base = c.base + first;
         const int ft = c.first_tile(a, w.seg);
         kb0 = (ft + w.t0) << a.key_shift;
-        tiles = w.t1 - w.t0;
+        const int t1 = a.whole ? c.tiles(a, w.seg) : w.t1;
+        tiles = t1 - w.t0;
         lo = max(kb0, c.first_row(a, w.seg));
-        hi = static_cast<int>(min(static_cast<long long>(c.end_row(a, w.seg)), static_cast<long long>(ft + w.t1) << a.key_shift));
+        hi = static_cast<int>(min(static_cast<long long>(c.end_row(a, w.seg)), static_cast<long long>(ft + t1) << a.key_shift));
         free_hi = base + 1;
         free_lo = a.window > 0 ? max(0, base + ntok - a.window) : 0;
         begins = w.t0 == 0;
@@ -793,6 +795,16 @@ cudaError_t go_tf32(const PagedChunkArgs &a, cudaStream_t st) {
 
 }  // namespace
 
+// Whether segments are better not cut.  Whole, a worker has at worst its number of segments of as many tiles as the table has
+// room for; cut, its share of all tiles (segments half as long as that, say), one at least, and what further portions and the
+// launch that joins them cost: 12 us.  A tile takes tile_ns.  (Tensor cores, 8 sequences of 40 tokens over 500 / 1000 rows: 29
+// and 34 us cut, 20 and 27 whole; a prompt of 8192 525 cut, 880 whole.  5 tokens over 300 rows on mma.sync: 16 cut, 23 whole.)
+bool chunk_whole(const PagedChunkArgs &a, int sms, double tile_ns) {
+    const double tiles = static_cast<double>(((static_cast<long long>(a.kv.max_pages) << a.kv.page_shift) + (1 << a.key_shift) - 1) >> a.key_shift);
+    const double segs = static_cast<double>(a.heads) *
+                        static_cast<double>(std::min<long long>(a.n_tokens, a.kv.n_seqs + (static_cast<long long>(a.n_tokens) >> a.tok_shift)));
+    return tiles * std::ceil(segs / sms) * tile_ns <= std::max(1.0, 0.5 * tiles * segs / sms) * tile_ns + 12000.0;
+}
 uint64_t chunk_mma_parts(const PagedKv &kv, int sms) {
     return 2ull * sms * rows_of(kv) * (pitch_of(kv) + 2) * 4;
 }
@@ -813,8 +825,8 @@ cudaError_t launch_chunk_mma(PagedChunkArgs a, int sms, cudaStream_t st) {
     a.tok_shift = log2_floor(M / a.hg);
     a.tile_tok = 1 << a.tok_shift;
     a.key_shift = key_shift_of(a.kv);
-    // a table of one tile's rows: no segment can be cut
-    const bool cut = (static_cast<long long>(a.kv.max_pages) << a.kv.page_shift) > (1 << a.key_shift);
+    const bool cut = !chunk_whole(a, sms, a.kv.dtype == STYX_F32 ? 12000 : 3200);
+    a.whole = !cut;
     a.seg_cost = cut ? 2 : 0;
     a.workers = sms;
     const int pitch = pitch_of(a.kv);

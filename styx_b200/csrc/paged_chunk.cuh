@@ -6,7 +6,8 @@
 // list (sequence, kv head and group, segment, tile), cut evenly over the
 // workers, so ragged lengths and few tokens over a long cache fill the SMs
 // alike; segments that are cut are joined in order.  A segment's start and end
-// count as seg_cost tiles.  How many tiles a sequence has, and in which segment
+// count as seg_cost tiles.  (Over short caches segments are not cut, and count
+// one unit each: the launch that joins them takes longer than a few tiles.)  How many tiles a sequence has, and in which segment
 // its u-th lies, are closed sums over its causal staircase, so every warp finds
 // its share by itself, whatever the lengths.
 #pragma once
@@ -55,9 +56,11 @@ struct Chunk {
     __device__ __forceinline__ int tiles(const PagedChunkArgs &a, int i) const {
         return ((end_row(a, i) - 1) >> a.key_shift) + 1 - first_tile(a, i);
     }
+    __device__ __forceinline__ int units(const PagedChunkArgs &a, int i) const { return a.whole ? 1 : tiles(a, i); }   // of the walk
     // units (tiles and seg_cost) of the first m segments, m < segs or m = segs
     __device__ __forceinline__ long long upto(const PagedChunkArgs &a, int m) const {
         if (m <= 0) return 0;
+        if (a.whole) return m;
         const int ts = a.tok_shift, ks = a.key_shift;
         long long u = static_cast<long long>(m) * (1 + a.seg_cost);
         const int whole = min(m, n >> ts);     // segments with all their tokens
@@ -77,7 +80,7 @@ struct ChunkWalk {
     int b, head, seg;              // sequence, (kv head, group), segment of its tokens
     int u, nt;                     // next unit of the segment's seg_cost + nt
     long long at, end;             // global unit numbers
-    int t0, t1;                    // the portion: tiles [t0, t1) of the segment, from its first
+    int t0, t1;                    // the portion: tiles [t0, t1) of the segment, from its first (a.whole: 0, 1, for all of them)
     __device__ __forceinline__ bool next(const PagedChunkArgs &a) {
         while (at < end) {
             if (u == a.seg_cost + nt) {
@@ -96,7 +99,7 @@ struct ChunkWalk {
                         } while (c.n == 0);
                     }
                 }
-                nt = c.tiles(a, seg);
+                nt = c.units(a, seg);
             }
             const int u1 = static_cast<int>(min(static_cast<long long>(a.seg_cost + nt), u + (end - at)));
             t0 = max(0, u - a.seg_cost);
@@ -176,7 +179,7 @@ __device__ __noinline__ ChunkShare chunk_share(const PagedChunkArgs &a, int work
         else s1 = mid - 1;
     }
     w.seg = s0;
-    w.nt = c.tiles(a, s0);
+    w.nt = c.units(a, s0);
     w.u = static_cast<int>(min(off - c.upto(a, s0), static_cast<long long>(a.seg_cost + w.nt)));
     return s;
 }

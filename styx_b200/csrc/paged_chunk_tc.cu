@@ -284,9 +284,10 @@ struct Part {
         base = c.base + first;
         const int ft = c.first_tile(a, w.seg);
         kb0 = (ft + w.t0) << a.key_shift;
-        tiles = w.t1 - w.t0;
+        const int t1 = a.whole ? c.tiles(a, w.seg) : w.t1;
+        tiles = t1 - w.t0;
         lo = max(kb0, c.first_row(a, w.seg));
-        hi = static_cast<int>(min(static_cast<long long>(c.end_row(a, w.seg)), static_cast<long long>(ft + w.t1) << a.key_shift));
+        hi = static_cast<int>(min(static_cast<long long>(c.end_row(a, w.seg)), static_cast<long long>(ft + t1) << a.key_shift));
         free_hi = base + 1;                         // every token sees all keys in [free_lo, free_hi)
         free_lo = a.window > 0 ? max(0, base + ntok - a.window) : 0;
         begins = w.t0 == 0;
@@ -964,8 +965,8 @@ cudaError_t launch_chunk_tc(PagedChunkArgs a, int sms, cudaStream_t st) {
     a.tile_tok = 1 << shift;
     a.tok_shift = shift + 1;
     a.key_shift = 7;
-    // a table of one tile's rows: no segment can be cut
-    const bool cut = (static_cast<long long>(a.kv.max_pages) << a.kv.page_shift) > kTile;
+    const bool cut = !chunk_whole(a, sms, a.q16 ? 1800 : 2600);
+    a.whole = !cut;
     a.seg_cost = cut ? 3 : 0;
     a.workers = sms;
     a.part_floats = 2 * kTile * (kTile + 2);

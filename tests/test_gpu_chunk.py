@@ -86,6 +86,8 @@ CASES = [
     ([4100], [3], 8, 1, 128, 128, "f16", "f32", 0),
     ([4100, 1, 2050], [2, 1, 9], 4, 1, 128, 64, "f32", "f32", 0),
     ([2500, 900], [20, 700], 2, 1, 128, 64, "f16", "f16", 1000),
+    ([600, 600, 512], [40, 9, 40], 8, 2, 128, 64, "f16", "f32", 0),
+    ([600, 600, 512], [40, 9, 40], 8, 2, 128, 64, "bf16", "bf16", 400),
 ]
 
 
