@@ -22,14 +22,24 @@
 // Roles, linked by mbarriers with bounded waits: eight softmax warps (four per
 // query tile; eight, with half of the keys each, were slower), a warp that copies
 // (TMA: boxes of min(page, 128) rows x 64 elements of a page, 128-byte swizzled;
-// 16-bit q with one box per tile and 64 elements; f32 q is brought and split by the softmax warps), a warp that issues
-// the products, and two warps that go over V where a tile is not seen in whole
-// by all rows: rows outside the sequence (TMA brings whole pages) and numbers
+// 16-bit q with one box per tile and 64 elements; f32 q is brought and split by
+// the softmax warps), a warp that issues the products, and two warps that go over
+// V where a tile is not seen in whole by all rows: rows outside the sequence (TMA brings whole pages) and numbers
 // that are not finite become zeros, since 0 times them would not be 0; the
 // latter are added, at the portion's end, to the rows that see them.  K and V
 // have a ring of slots each, whose barriers one role alone waits on, phase
 // after phase (a role that looked at every other phase of a barrier could take
 // one for another).
+//
+// Measured, 32 / 4 heads of 128: a prompt of 8192 tokens f16 524 us, 1050
+// TFLOP/s of what its triangle needs, at a short burst's clocks (636 for many in
+// a row, under the power limit); 512 tokens over 131071 rows bf16 1208; 2048
+// tokens f32 over 4096 rows f16 276 and 340.  Of the 524 the products alone take
+// 397: the rest is the way S -> P -> O of a tile, for TMEM has room for one S per
+// query tile.  (Two of 64 keys each hide the softmax, but their products alone
+// take 537.)  Five drafted tokens of each of 31 sequences are one query tile,
+// which has none to take turns with: 52 us over up to 4096 rows, some 3200 clocks
+// a tile.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -949,7 +959,7 @@ cudaError_t go(const PagedChunkArgs &a, const CUtensorMap &mq, const CUtensorMap
 // A page's rows and a tile's queries have to be boxes (rows of 128 bytes and more, 16 rows and more).  Scores are
 // compared before they are scaled, so the scale is positive.  A few queries over a short cache take as long as the kernel
 // takes to begin, and k_chunk_mma begins sooner (5 tokens of 32 / 4 heads over 37 rows, f32 over f16: 12.7 us, here 15.8;
-// over 300 rows of f16 15.7 and 16.7); beyond, this one is faster (16 sequences of 20 tokens over 500 rows 28 us, there 44).
+// over 300 rows of f16 15.7 and 16.7); beyond, this one is faster (16 sequences of 20 tokens over 500 rows 20 us, there 44).
 bool chunk_on_tc(const PagedChunkArgs &a) {
     const bool few = static_cast<long long>(a.n_tokens) * a.gqa <= kTile && (static_cast<long long>(a.kv.max_pages) << a.kv.page_shift) <= 512;
     return (a.q16 || a.kv.dtype == STYX_F16) && a.kv.hd >= 64 && a.kv.hd <= 128 && a.kv.page_shift >= 4 && a.scale > 0.f && !few &&
@@ -979,7 +989,7 @@ cudaError_t launch_chunk_tc(PagedChunkArgs a, int sms, cudaStream_t st) {
     if ((a.q16 && !encode(mq, bf, a.q, kv.hd, a.n_heads, a.n_tokens, kv.hd, a.q_stride, a.hg, a.tile_tok)) ||
         !encode(mk, bf, kv.k, kv.hd, rows, kv.n_pages, kv.hd, kv.page_stride, box, 1) ||
         !encode(mv, bf, kv.v, kv.hd, rows, kv.n_pages, kv.hd, kv.page_stride, box, 1))
-        return cudaErrorInvalidValue;
+        return launch_chunk_mma(a, sms, st);           // (a layout that the maps cannot say)
     cudaError_t e = bf ? go<true, 1>(a, mq, mk, mv, st) : a.q16 ? go<false, 1>(a, mq, mk, mv, st) : go<false, 2>(a, mq, mk, mv, st);
     return e != cudaSuccess || !cut ? e : launch_chunk_join(a, 2 * kTile, kTile, kTile, st);
 }

@@ -87,6 +87,8 @@ CASES = [
     ([4100, 1, 2050], [2, 1, 9], 4, 1, 128, 64, "f32", "f32", 0),
     ([2500, 900], [20, 700], 2, 1, 128, 64, "f16", "f16", 1000),
     ([600, 600, 512], [40, 9, 40], 8, 2, 128, 64, "f16", "f32", 0),
+    ([150, 40], [12, 5], 200, 1, 64, 64, "f16", "f16", 0),
+    ([150, 40], [9, 5], 274, 2, 72, 16, "bf16", "bf16", 60),
     ([600, 600, 512], [40, 9, 40], 8, 2, 128, 64, "bf16", "bf16", 400),
 ]
 
@@ -342,6 +344,34 @@ def test_chunk_on_another_stream_and_in_a_graph():
         g.replay()
         assert torch.equal(out, first)
         kv.ctx.check_device_error()
+
+
+def test_many_calls_of_ragged_batches():
+    """Calls back to back, lengths and ranges of one after the other: each
+    gives the bits that it gives alone, and no wait gives up."""
+    rng = np.random.default_rng(13)
+    for dtype, q_type, hd in (("bf16", "bf16", 128), ("f16", "f32", 128), ("f16", "f16", 64)):
+        kv, _, _ = make_cache(rng, [1500] * 24, 4, hd, 64, dtype)
+        n = 700
+        q = queries(rng, n, 32, hd, TYPES[q_type])
+        sets = []
+        for _ in range(6):
+            lens = np.where(rng.random(24) < 0.2, 0, rng.integers(1, 1501, 24))
+            news = np.minimum(lens, np.where(rng.random(24) < 0.5, rng.integers(1, 8, 24), rng.integers(1, 50, 24)))
+            news[np.cumsum(news) > n] = 0
+            sets.append((I(lens.tolist()), I(starts(news.tolist()))))
+        alone = []
+        for lens, start in sets:
+            kv.lens = lens
+            alone.append(kv.attend_chunk(q, start, out=torch.zeros_like(q)))
+            torch.cuda.synchronize()
+        outs = [torch.zeros_like(q) for _ in sets]
+        for i in range(600):
+            kv.lens = sets[i % 6][0]
+            kv.attend_chunk(q, sets[i % 6][1], out=outs[i % 6])
+        kv.ctx.check_device_error()
+        for a, b in zip(alone, outs):
+            assert torch.equal(a, b)
 
 
 # ------------------------------------------------------------------ append with rotary forms
