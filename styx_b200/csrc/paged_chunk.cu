@@ -16,6 +16,21 @@
 // rounding them, so a tile's P V is added to O by the FMA that rescales O.
 // k_chunk_tf32, f32 caches: both factors as two tf32 terms, the product of the
 // two small ones (2^-22 of the whole) left out.
+//
+// Bound by mma.sync's rate: for f32 caches three products per pair of factors
+// (3 sequences of some 500 tokens over up to 4099 rows, 32 / 4 heads of 128, a
+// window of 1024: 685 us, of which the products alone are 255 at half of the
+// 16-bit rate that mma.sync reaches here).  On small calls by the latency of
+// start, pages' numbers and first tile: 5 tokens, f32 over 37 rows of f16,
+// 12.6 us, f16 10.5; over 300 rows of f16 15.8.
+//
+// Bound by the products that mma.sync has, three per pair of factors for f32
+// caches (2 sequences of 512 tokens, 32 / 4 heads of 128, over 4608 rows, a
+// window of 1024: 685 us, 12 times its reads of 8 MB a kv head and sequence and
+// its products together at the tensor cores' tf32 rate; portions of 64 rows keep
+// S, P and O of 16 rows a warp in registers without spills), and by the latency
+// of the start, of the pages' numbers and of the first tile on small calls (5
+// tokens over 300 rows of f16 15.8 us, over 37 rows 10.5).
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -140,16 +155,11 @@ __device__ __noinline__ Portion portion_of(const PagedChunkArgs &a, ChunkWalk w)
 __device__ __forceinline__ long long out_row(const PagedChunkArgs &a, const Portion &P, int tok, int head) {
     return static_cast<long long>(P.tok0 + tok) * a.n_heads + P.j * a.gqa + P.g0 + head;
 }
-// the portion's result of one query row goes to its output, or to the workspace
-template <int ROWS>
-__device__ __forceinline__ float *part_rows(const PagedChunkArgs &a, const Portion &P, int worker) {
-    return chunk_part(a, worker, P.begins);
-}
 // what k_chunk_join needs to know of the worker's first portion; later ones begin their segments
 __device__ __forceinline__ void note_join(const PagedChunkArgs &a, const Portion *P, const ChunkWalk &w, int worker,
                                           const ChunkShare &s) {
     ChunkJoin j{-1, 0, 0, 0};
-    if (P && !P->begins && P->ends) j = {chunk_owner(w, s.T, s.G), w.b, w.head, w.seg};
+    if (P && !P->begins && P->ends) j = {chunk_owner(w, s.T, s.G), P->tok0, P->ntok, w.head};
     static_cast<ChunkJoin *>(a.joins)[worker] = j;
 }
 // ------------------------------------------------------------ 16-bit caches
@@ -704,62 +714,73 @@ __global__ void __launch_bounds__(Tf<HD>::threads, 1) k_chunk_tf32(const __grid_
 // ------------------------------------------------------------ joining
 // A cut segment's portions added up in order, a warp per query row.  M rows of
 // pitch floats a portion, tiles of `tile` rows with a.tile_tok tokens each.
-constexpr int kJoinThreads = 256;
-template <class TQ>
+// Bound by latency, behind a kernel that fills the SMs: of memory (what the
+// segment is comes in one load, then LOADS portions a trip), and of the code
+// itself, which no SM has fetched yet: it is kept short (LOADS 8 instead of 2: 4 us
+// more for 31 sequences of 5 tokens, which mostly have two; all loads of 32
+// portions under way by shuffles likewise).
+constexpr int kJoinThreads = 256, kJoinCtas = 8;
+template <class TQ, int LOADS>
 __global__ void __launch_bounds__(kJoinThreads) k_chunk_join(PagedChunkArgs a, int M, int tile, int pitch) {
     pdl_trigger();
     pdl_wait();
-    const int worker = blockIdx.x, lane = threadIdx.x & 31;
-    const ChunkJoin j = static_cast<const ChunkJoin *>(a.joins)[worker];
+    const int worker = blockIdx.x, lane = threadIdx.x & 31, hd = a.kv.hd;
+    const int4 jj = reinterpret_cast<const int4 *>(a.joins)[worker];
+    const ChunkJoin j{jj.x, jj.y, jj.z, jj.w};
     if (j.first < 0) return;
-    const int r = blockIdx.y * (kJoinThreads / 32) + (threadIdx.x >> 5), hd = a.kv.hd;
-    const int nth = r / tile, rt = (r - nth * tile) / a.hg, hr = (r - nth * tile) - rt * a.hg, tok = nth * a.tile_tok + rt;
-    const int kvh = j.head / a.groups, g0 = (j.head - kvh * a.groups) * a.hg;
-    const Chunk c(a, j.b, false);
-    const int first = j.seg << a.tok_shift;
-    if (r >= M || rt >= a.tile_tok || tok >= min(1 << a.tok_shift, c.n - first) || hr >= min(a.hg, a.gqa - g0)) return;
-    const long long row = static_cast<long long>(c.tok0 + first + tok) * a.n_heads + kvh * a.gqa + g0 + hr;
-    // a lane per portion for maxima and sums; then the portions' rows in order, eight loads under way
     const int n = worker - j.first + 1;
-    auto row_of = [&](int p) { return chunk_part(a, j.first + p, p == 0); };
-    float top = kNone;
-    for (int p = lane; p < n; p += 32) top = fmaxf(top, row_of(p)[M * pitch + r]);
+    const int kvh = j.head / a.groups, g0 = (j.head - kvh * a.groups) * a.hg, ng = min(a.hg, a.gqa - g0);
+    const float *const part = chunk_part(a, j.first, false);
+    const long long step = 2ll * a.part_floats;
+#pragma unroll 1
+    for (int r = blockIdx.y * (kJoinThreads / 32) + (threadIdx.x >> 5); r < M; r += kJoinCtas * (kJoinThreads / 32)) {
+        const int nth = r / tile, rt = (r - nth * tile) / a.hg, hr = r - nth * tile - rt * a.hg, tok = nth * a.tile_tok + rt;
+        if (rt >= a.tile_tok || tok >= j.ntok || hr >= ng) continue;
+        const long long row = static_cast<long long>(j.tok0 + tok) * a.n_heads + kvh * a.gqa + g0 + hr;
+#pragma unroll 1
+        for (int c = 4 * lane; c < pitch; c += 128) {
+            float top = kNone, l = 0.f;
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+            for (int p0 = 0; p0 < n; p0 += LOADS) {
+                float m[LOADS], lp[LOADS];
+                float4 x[LOADS];
 #pragma unroll
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float l = 0.f;
-    float4 o[2] = {};
-    for (int p0 = 0; p0 < n; p0 += 32) {
-        float f = 0.f;
-        if (p0 + lane < n) {
-            const float *p = row_of(p0 + lane) + M * pitch + r;
-            f = ex2(p[0] - top);
-            l += p[M] * f;
-        }
-        const int here = min(32, n - p0);
+                for (int k = 0; k < LOADS; k++) {
+                    const int p = p0 + k;
+                    const float *q = part + p * step + (p == 0 ? a.part_floats : 0);   // (the first one begins the segment)
+                    m[k] = kNone;
+                    lp[k] = 0.f;
+                    x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (p < n) {
+                        x[k] = *reinterpret_cast<const float4 *>(q + r * pitch + c);
+                        m[k] = q[M * pitch + r];
+                        lp[k] = q[M * pitch + M + r];
+                    }
+                }
+                float t = top;
 #pragma unroll
-        for (int v = 0; v < 2; v++)
-            if (128 * v < pitch) {
-                const bool in = 128 * v + 4 * lane < hd;
-#pragma unroll 8
-                for (int k = 0; k < here; k++) {
-                    const float fk = __shfl_sync(0xffffffffu, f, k);
-                    const float4 x = in ? *reinterpret_cast<const float4 *>(row_of(p0 + k) + r * pitch + 128 * v + 4 * lane)
-                                        : make_float4(0.f, 0.f, 0.f, 0.f);
-                    o[v] = make_float4(fmaf(x.x, fk, o[v].x), fmaf(x.y, fk, o[v].y), fmaf(x.z, fk, o[v].z), fmaf(x.w, fk, o[v].w));
+                for (int k = 0; k < LOADS; k++) t = fmaxf(t, m[k]);
+                const float f = ex2(top - t);
+                top = t;
+                l *= f;
+                o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+#pragma unroll
+                for (int k = 0; k < LOADS; k++) {
+                    const float w = ex2(m[k] - top);
+                    l = fmaf(lp[k], w, l);
+                    o = make_float4(fmaf(x[k].x, w, o.x), fmaf(x[k].y, w, o.y), fmaf(x[k].z, w, o.z), fmaf(x[k].w, w, o.w));
                 }
             }
-    }
-#pragma unroll
-    for (int i = 16; i; i >>= 1) l += __shfl_xor_sync(0xffffffffu, l, i);
-    const float inv = inverse_sum(l);
-    TQ *out = static_cast<TQ *>(a.out) + row * hd;
-#pragma unroll
-    for (int v = 0; v < 2; v++)
-        if (128 * v + 4 * lane < hd) {
-            st_pair(out + 128 * v + 4 * lane, o[v].x * inv, o[v].y * inv);
-            st_pair(out + 128 * v + 4 * lane + 2, o[v].z * inv, o[v].w * inv);
+            if (c < hd) {
+                const float inv = inverse_sum(l);
+                TQ *out = static_cast<TQ *>(a.out) + row * hd + c;
+                st_pair(out, o.x * inv, o.y * inv);
+                st_pair(out + 2, o.z * inv, o.w * inv);
+            }
+            if (a.lse && c == 0) a.lse[row] = lse_of(top, l);
         }
-    if (a.lse && lane == 0) a.lse[row] = lse_of(top, l);
+    }
 }
 
 int log2_floor(int v) { return 31 - __builtin_clz(static_cast<unsigned>(v)); }
@@ -787,6 +808,17 @@ cudaError_t go_hd(const PagedChunkArgs &a, cudaStream_t st) {
         default: return go_mma<BF, TERMS, 256>(a, st);
     }
 }
+// segments of a call, at most
+long long most_segs(const PagedChunkArgs &a) {
+    return a.heads * std::min<long long>(a.n_tokens, a.kv.n_seqs + (static_cast<long long>(a.n_tokens) >> a.tok_shift));
+}
+// two portions a trip where segments are as many as half of the workers or more (5 tokens of 31 sequences over 2048 rows 48 us;
+// eight a trip 53), else eight (16 tokens of one over 65536, 37 portions each: 56; two 60)
+template <class TQ>
+cudaError_t go_join(const PagedChunkArgs &a, int M, int tile, int pitch, cudaStream_t st) {
+    auto *kern = 2 * most_segs(a) >= a.workers ? k_chunk_join<TQ, 2> : k_chunk_join<TQ, 8>;
+    return launch_pdl(kern, dim3(a.workers, kJoinCtas), dim3(kJoinThreads), 0, st, a, M, tile, pitch);
+}
 template <int HD>
 cudaError_t go_tf32(const PagedChunkArgs &a, cudaStream_t st) {
     static_assert(Tf<HD>::smem <= 226 * 1024, "shared memory");
@@ -801,8 +833,7 @@ cudaError_t go_tf32(const PagedChunkArgs &a, cudaStream_t st) {
 // and 34 us cut, 20 and 27 whole; a prompt of 8192 525 cut, 880 whole.  5 tokens over 300 rows on mma.sync: 16 cut, 23 whole.)
 bool chunk_whole(const PagedChunkArgs &a, int sms, double tile_ns) {
     const double tiles = static_cast<double>(((static_cast<long long>(a.kv.max_pages) << a.kv.page_shift) + (1 << a.key_shift) - 1) >> a.key_shift);
-    const double segs = static_cast<double>(a.heads) *
-                        static_cast<double>(std::min<long long>(a.n_tokens, a.kv.n_seqs + (static_cast<long long>(a.n_tokens) >> a.tok_shift)));
+    const double segs = static_cast<double>(most_segs(a));
     return tiles * std::ceil(segs / sms) * tile_ns <= std::max(1.0, 0.5 * tiles * segs / sms) * tile_ns + 12000.0;
 }
 uint64_t chunk_mma_parts(const PagedKv &kv, int sms) {
@@ -811,10 +842,8 @@ uint64_t chunk_mma_parts(const PagedKv &kv, int sms) {
 
 // the portions joined; a's cut of the work and workspace are set
 cudaError_t launch_chunk_join(const PagedChunkArgs &a, int M, int tile, int pitch, cudaStream_t st) {
-    const dim3 grid(a.workers, (M + kJoinThreads / 32 - 1) / (kJoinThreads / 32));
-    if (!a.q16) return launch_pdl(k_chunk_join<float>, grid, dim3(kJoinThreads), 0, st, a, M, tile, pitch);
-    if (a.kv.dtype == STYX_F16) return launch_pdl(k_chunk_join<__half>, grid, dim3(kJoinThreads), 0, st, a, M, tile, pitch);
-    return launch_pdl(k_chunk_join<__nv_bfloat16>, grid, dim3(kJoinThreads), 0, st, a, M, tile, pitch);
+    if (!a.q16) return go_join<float>(a, M, tile, pitch, st);
+    return a.kv.dtype == STYX_F16 ? go_join<__half>(a, M, tile, pitch, st) : go_join<__nv_bfloat16>(a, M, tile, pitch, st);
 }
 
 cudaError_t launch_chunk_mma(PagedChunkArgs a, int sms, cudaStream_t st) {

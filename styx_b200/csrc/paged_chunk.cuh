@@ -7,9 +7,10 @@
 // workers, so ragged lengths and few tokens over a long cache fill the SMs
 // alike; segments that are cut are joined in order.  A segment's start and end
 // count as seg_cost tiles.  (Over short caches segments are not cut, and count
-// one unit each: the launch that joins them takes longer than a few tiles.)  How many tiles a sequence has, and in which segment
-// its u-th lies, are closed sums over its causal staircase, so every warp finds
-// its share by itself, whatever the lengths.
+// one unit each: the launch that joins them takes longer than a few tiles.)  How
+// many tiles a sequence has, and in which segment its u-th lies, are closed sums
+// over its causal staircase, so every warp finds its share by itself, whatever the
+// lengths.
 #pragma once
 
 #include "paged_split.cuh"
@@ -198,7 +199,8 @@ __device__ __noinline__ int chunk_owner(ChunkWalk w, long long T, long long G) {
 
 // what joins a cut segment: filled in by the worker that has its last tile, for every call
 struct ChunkJoin {
-    int first, b, head, seg;       // first worker (-1: nothing to join); the segment
+    int first;                     // worker (-1: nothing to join)
+    int tok0, ntok, head;          // the segment's tokens; kv head and group
 };
 // where a portion's (O, max, sum) go: worker i's portion that begins its segment to slot 2 i + 1, any other to 2 i.
 // O is [rows][pitch], then a maximum (in units of log2) and a sum for every row.

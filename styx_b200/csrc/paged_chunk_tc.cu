@@ -649,15 +649,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (lane == 0) mbar_arrive(&bars.qfull);
         };
         bool have = wk.next(a);
+        if (have) P.set(a, wk);
         if (tid == 0) {                               // (later portions begin their segments)
             ChunkJoin j{-1, 0, 0, 0};
-            if (have && wk.t0 > 0 && wk.t1 == wk.nt) j = {chunk_owner(wk, share.T, share.G), wk.b, wk.head, wk.seg};
+            if (have && !P.begins && P.ends) j = {chunk_owner(wk, share.T, share.G), P.tok0, P.ntok, wk.head};
             static_cast<ChunkJoin *>(a.joins)[worker] = j;
         }
-        if (have) {
-            P.set(a, wk);
-            if constexpr (TERMS == 2) stage();
-        }
+        if constexpr (TERMS == 2)
+            if (have) stage();
         while (have) {
             const bool run = t == 0 || P.two;         // (else there is no second tile)
             const int tok = t * a.tile_tok + rt;
