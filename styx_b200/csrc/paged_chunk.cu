@@ -17,20 +17,14 @@
 // k_chunk_tf32, f32 caches: both factors as two tf32 terms, the product of the
 // two small ones (2^-22 of the whole) left out.
 //
-// Bound by mma.sync's rate: for f32 caches three products per pair of factors
-// (3 sequences of some 500 tokens over up to 4099 rows, 32 / 4 heads of 128, a
-// window of 1024: 685 us, of which the products alone are 255 at half of the
-// 16-bit rate that mma.sync reaches here).  On small calls by the latency of
-// start, pages' numbers and first tile: 5 tokens, f32 over 37 rows of f16,
-// 12.6 us, f16 10.5; over 300 rows of f16 15.8.
-//
-// Bound by the products that mma.sync has, three per pair of factors for f32
-// caches (2 sequences of 512 tokens, 32 / 4 heads of 128, over 4608 rows, a
-// window of 1024: 685 us, 12 times its reads of 8 MB a kv head and sequence and
-// its products together at the tensor cores' tf32 rate; portions of 64 rows keep
-// S, P and O of 16 rows a warp in registers without spills), and by the latency
-// of the start, of the pages' numbers and of the first tile on small calls (5
-// tokens over 300 rows of f16 15.8 us, over 37 rows 10.5).
+// Bound by mma.sync: for f32 caches three products per pair of factors (3
+// sequences of some 500 tokens over up to 4099 rows, 32 / 4 heads of 128, a
+// window of 1024: 685 us, of which the products alone are 272 at the 270 TFLOP/s
+// that mma.sync reaches with tf32; two warps per scheduler leave latencies open,
+// and with four O, S and P have no room in registers, nor gains the exchange of P
+// through shared memory: 1166 us instead of 1072 for 500 over 2048).  On small
+// calls by the latency of start, pages' numbers and first tile: 5 tokens, f32 over
+// 37 rows of f16, 12.6 us, f16 10.5; over 300 rows of f16 14.6.
 #include <cuda_runtime.h>
 
 #include <algorithm>

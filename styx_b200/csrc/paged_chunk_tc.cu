@@ -31,15 +31,15 @@
 // after phase (a role that looked at every other phase of a barrier could take
 // one for another).
 //
-// Measured, 32 / 4 heads of 128: a prompt of 8192 tokens f16 524 us, 1050
+// Measured, 32 / 4 heads of 128: a prompt of 8192 tokens f16 515 us, 1068
 // TFLOP/s of what its triangle needs, at a short burst's clocks (636 for many in
 // a row, under the power limit); 512 tokens over 131071 rows bf16 1208; 2048
-// tokens f32 over 4096 rows f16 276 and 340.  Of the 524 the products alone take
+// tokens f32 over 4096 rows f16 272 and 340.  Of the 515 the products alone take
 // 397: the rest is the way S -> P -> O of a tile, for TMEM has room for one S per
 // query tile.  (Two of 64 keys each hide the softmax, but their products alone
-// take 537.)  Five drafted tokens of each of 31 sequences are one query tile,
-// which has none to take turns with: 52 us over up to 4096 rows, some 3200 clocks
-// a tile.
+// take 537.)  Five drafted tokens of each of 31 sequences over 2048 rows take 48:
+// 23 for the rows at HBM's rate (from 2048 rows on 5.4 to 5.8 TB/s), the rest
+// start, portions' ends and joining.
 #include <cuda.h>
 #include <cuda_runtime.h>
 

@@ -727,8 +727,8 @@ class PagedKV:
     a pool of all layers); table: int32 [n_seqs][max_pages] page ids; lens:
     int32 [n_seqs] rows in use.  The tensors stay the caller's: page ids and
     lengths are changed in place (or `lens` replaced through the attribute).
-    Calls on one object share its workspaces (10 MB for attention over 16-bit
-    rows on 148 SMs): not on two streams at once."""
+    Calls on one object share its workspaces (on 148 SMs and over 16-bit rows 10
+    MB for `attend`, 39 MB for `attend_chunk`): not on two streams at once."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lens: torch.Tensor):
         if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or (k.shape[0] > 1 and k.stride(0) != v.stride(0)):

@@ -90,6 +90,8 @@ CASES = [
     ([150, 40], [12, 5], 200, 1, 64, 64, "f16", "f16", 0),
     ([150, 40], [9, 5], 274, 2, 72, 16, "bf16", "bf16", 60),
     ([600, 600, 512], [40, 9, 40], 8, 2, 128, 64, "bf16", "bf16", 400),
+    ([1300], [4], 2, 1, 256, 16, "bf16", "bf16", 0),         # (forty portions and more of one segment)
+    ([1300], [3], 3, 1, 192, 32, "f32", "f32", 0),
 ]
 
 
